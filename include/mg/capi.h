@@ -399,6 +399,78 @@ int mg_gae(void* stream, const float* reward, const uint8_t* done, const float* 
            float* advantage, float* ret);
 
 /* ---------------------------------------------------------------------------
+ * Training operators for blocks of any width, beside the fused update (which
+ * holds its LayerNorm, of width 128, and Adam inside its kernels): LayerNorm
+ * forward and backward. No reference counterpart. Device pointers throughout. Every call enqueues on
+ * `stream` (a hipStream_t; NULL: the current device's default stream) and
+ * returns without waiting; none allocates, so all may be captured into a HIP
+ * graph. Workspaces are the caller's: calls that may run at the same time need
+ * one each, as do graphs that may replay at the same time; the contents need no
+ * clearing. Distinct arrays of one call must not overlap except where a comment
+ * says so. Every sum has a fixed order, so a rerun gives the same bits.
+ * ------------------------------------------------------------------------- */
+enum { MG_TYPE_FP32 = 0, MG_TYPE_BF16 = 1, MG_TYPE_FP16 = 2 };
+
+/* y = (s - mean) rstd gamma + beta per row, with s = x, or x + residual rounded
+ * to the arrays' type; rstd = 1 / sqrt(var + eps), var the mean of (s - mean)^2.
+ * Row r of an array begins r * its ld elements after the array (ld 0: cols).
+ * x, residual, sum and y are of `type` (MG_TYPE_*), the rest fp32; statistics
+ * and products are fp32, y is rounded once. y may be x, residual or sum, and sum
+ * may be x or residual, where both have one ld. rows may be 0; cols is at least
+ * 1 and at most 2^24, eps finite and not negative. */
+typedef struct mg_layernorm_args {
+    const void* x;
+    const void* residual; /* nullable */
+    void* sum;            /* s: required with residual, else NULL */
+    const float* gamma;   /* [cols], NULL: 1 */
+    const float* beta;    /* [cols], NULL: 0 */
+    void* y;
+    float* mean; /* [rows], nullable: what the backward pass needs */
+    float* rstd; /* [rows], nullable */
+    uint64_t x_ld;
+    uint64_t residual_ld;
+    uint64_t sum_ld;
+    uint64_t y_ld;
+    uint32_t rows;
+    uint32_t cols;
+    uint32_t type;
+    float eps;
+} mg_layernorm_args;
+int mg_layernorm(void* stream, const mg_layernorm_args* args);
+
+/* Backward of mg_layernorm for the gradient dy of y. With xn = (x - mean) rstd
+ * and d = dy gamma: dx = rstd (d - mean(d) - xn mean(d xn)) + dsum, dgamma =
+ * sum over rows of dy xn, dbeta = sum over rows of dy. x is what was normalised
+ * (the forward's sum where it had a residual); dx is then the gradient of both
+ * x and residual. Without rows dgamma and dbeta are 0. dx may be x, dy or dsum
+ * where both have one ld. workspace: at least mg_layernorm_backward_workspace
+ * bytes, 16-byte aligned; may be NULL where that is 0, or where dgamma and dbeta
+ * are NULL. */
+typedef struct mg_layernorm_backward_args {
+    const void* x;
+    const void* dy;
+    const void* dsum; /* nullable: the gradient that reaches s past the norm */
+    const float* gamma; /* [cols], NULL: 1 */
+    const float* mean;  /* [rows], the forward's */
+    const float* rstd;
+    void* dx;
+    float* dgamma; /* [cols], nullable */
+    float* dbeta;  /* [cols], nullable */
+    uint64_t x_ld;
+    uint64_t dy_ld;
+    uint64_t dsum_ld;
+    uint64_t dx_ld;
+    uint32_t rows;
+    uint32_t cols;
+    uint32_t type;
+    uint32_t reserved; /* 0 */
+    void* workspace;
+    uint64_t workspace_bytes;
+} mg_layernorm_backward_args;
+int mg_layernorm_backward_workspace(uint32_t rows, uint32_t cols, uint64_t* bytes);
+int mg_layernorm_backward(void* stream, const mg_layernorm_backward_args* args);
+
+/* ---------------------------------------------------------------------------
  * Kernel timing for measurement: when enabled, the library records HIP events
  * around each launch on the stream it uses and accumulates durations.
  * ------------------------------------------------------------------------- */

@@ -8,6 +8,7 @@ if the library has not been built, importing ``lib()`` raises.
 """
 from ._capi import (  # noqa: F401
     LIB_PATH,
+    TYPES,
     COLLECT_FN,
     CapiError,
     CollectArgs,
@@ -24,6 +25,9 @@ from ._capi import (  # noqa: F401
     env_desc,
     env_names,
     h2d,
+    layernorm,
+    layernorm_backward,
+    layernorm_backward_workspace,
     lib,
     timing_enable,
     timing_get,

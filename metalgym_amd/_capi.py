@@ -22,7 +22,8 @@ class CapiError(RuntimeError):
 
 
 P = C.c_void_p
-u32, f32 = C.c_uint32, C.c_float
+u32, u64, f32 = C.c_uint32, C.c_uint64, C.c_float
+TYPES = {"fp32": 0, "bf16": 1, "fp16": 2}  # MG_TYPE_*
 
 
 class EnvDesc(C.Structure):
@@ -80,6 +81,20 @@ class LossStats(C.Structure):
 class PPOSlots(C.Structure):
     _fields_ = [(n, P) for n in ("obs", "actions", "logp", "value", "reward", "done", "advantage", "ret")] + [
         ("n", u32), ("horizon", u32)]
+
+
+class LayernormArgs(C.Structure):
+    """mg_layernorm_args"""
+    _fields_ = [(n, P) for n in ("x", "residual", "sum", "gamma", "beta", "y", "mean", "rstd")] + [
+        (n, u64) for n in ("x_ld", "residual_ld", "sum_ld", "y_ld")] + [(n, u32) for n in ("rows", "cols", "type")] + [
+        ("eps", f32)]
+
+
+class LayernormBackwardArgs(C.Structure):
+    """mg_layernorm_backward_args"""
+    _fields_ = [(n, P) for n in ("x", "dy", "dsum", "gamma", "mean", "rstd", "dx", "dgamma", "dbeta")] + [
+        (n, u64) for n in ("x_ld", "dy_ld", "dsum_ld", "dx_ld")] + [
+        (n, u32) for n in ("rows", "cols", "type", "reserved")] + [("workspace", P), ("workspace_bytes", u64)]
 
 
 class KernelTimes(C.Structure):
@@ -156,6 +171,9 @@ def lib():
         "mg_ppo_last_order": (I, [P, P, u32, P]),
         "mg_ppo_sample": (I, [P, P, u32, P, P, P, P]),
         "mg_gae": (I, [P, P, P, P, P, u32, u32, u32, u32, f32, f32, P, P]),
+        "mg_layernorm": (I, [P, P]),
+        "mg_layernorm_backward_workspace": (I, [u32, u32, P]),
+        "mg_layernorm_backward": (I, [P, P]),
         "mg_timing_enable": (I, [I]),
         "mg_timing_get": (I, [P]),
         "mg_timing_reset": (I, []),
@@ -196,6 +214,31 @@ def timing_get() -> dict:
     t = KernelTimes()
     check(lib().mg_timing_get(C.byref(t)))
     return t.as_dict()
+
+
+def layernorm(x: int, y: int, rows: int, cols: int, dtype: str = "fp32", *, gamma: int = None, beta: int = None,
+              eps: float = 1e-5, residual: int = None, sum: int = None, mean: int = None, rstd: int = None,
+              x_ld: int = 0, residual_ld: int = 0, sum_ld: int = 0, y_ld: int = 0, stream: int = None) -> None:
+    """mg_layernorm on device addresses; asynchronous on the HIP stream `stream`."""
+    a = LayernormArgs(x, residual, sum, gamma, beta, y, mean, rstd, x_ld, residual_ld, sum_ld, y_ld, rows, cols,
+                      TYPES[dtype], eps)
+    check(lib().mg_layernorm(stream, C.byref(a)))
+
+
+def layernorm_backward_workspace(rows: int, cols: int) -> int:
+    n = u64()
+    check(lib().mg_layernorm_backward_workspace(rows, cols, C.byref(n)))
+    return n.value
+
+
+def layernorm_backward(x: int, dy: int, mean: int, rstd: int, dx: int, rows: int, cols: int, dtype: str = "fp32", *,
+                       gamma: int = None, dsum: int = None, dgamma: int = None, dbeta: int = None, x_ld: int = 0,
+                       dy_ld: int = 0, dsum_ld: int = 0, dx_ld: int = 0, workspace: int = None,
+                       workspace_bytes: int = 0, stream: int = None) -> None:
+    """mg_layernorm_backward on device addresses; asynchronous."""
+    a = LayernormBackwardArgs(x, dy, dsum, gamma, mean, rstd, dx, dgamma, dbeta, x_ld, dy_ld, dsum_ld, dx_ld, rows,
+                              cols, TYPES[dtype], 0, workspace, workspace_bytes)
+    check(lib().mg_layernorm_backward(stream, C.byref(a)))
 
 
 class DeviceBuffer:
