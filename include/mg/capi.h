@@ -401,7 +401,8 @@ int mg_gae(void* stream, const float* reward, const uint8_t* done, const float* 
 /* ---------------------------------------------------------------------------
  * Training operators for blocks of any width, beside the fused update (which
  * holds its LayerNorm, of width 128, and Adam inside its kernels): LayerNorm
- * forward and backward. No reference counterpart. Device pointers throughout. Every call enqueues on
+ * forward and backward, and matrices orthogonalised for the Muon update. No
+ * reference counterpart. Device pointers throughout. Every call enqueues on
  * `stream` (a hipStream_t; NULL: the current device's default stream) and
  * returns without waiting; none allocates, so all may be captured into a HIP
  * graph. Workspaces are the caller's: calls that may run at the same time need
@@ -469,6 +470,68 @@ typedef struct mg_layernorm_backward_args {
 } mg_layernorm_backward_args;
 int mg_layernorm_backward_workspace(uint32_t rows, uint32_t cols, uint64_t* bytes);
 int mg_layernorm_backward(void* stream, const mg_layernorm_backward_args* args);
+
+/* The Newton-Schulz iteration of a matrix G: X = G / (|G| + eps) with the
+ * Frobenius norm, then `steps` times X = a X + b (X X') X + c (X X')^2 X, which
+ * moves every singular value to p(s) = a s + b s^3 + c s^5 and keeps the singular
+ * vectors. On the short side, whichever it is, so a matrix and its transpose give
+ * transposed results. NULL stands for 5 steps of (3.4445, -4.7750, 2.0315), eps
+ * 1e-7: singular values from 0.7 to 1.2, except those under about 1e-3 of the norm.
+ * steps is in [1, 32], eps positive and finite; the polynomial must keep [0, 1]
+ * inside [-2, 2] over the steps and a + b s^2 + c s^4 inside [-64, 64] there. The
+ * products go through the matrix units as pairs of binary16 halves (22 bits,
+ * three products, fp32 sums), for every type: a small singular value's error grows
+ * by a with each step, so one 16-bit product would lose the small directions of
+ * a matrix with a few strong ones. */
+typedef struct mg_newton_schulz {
+    uint32_t steps;
+    float a;
+    float b;
+    float c;
+    float eps;
+} mg_newton_schulz;
+
+/* `count` row-major matrices of rows x cols elements: element (i, j) of matrix k
+ * at data[k stride + i ld + j]. ld 0: cols; stride 0: rows ld. rows and cols are
+ * at least 1 and at most 65536, the smaller at most 8192; count may be 0, at most
+ * 65535. type is MG_TYPE_*. Matrices of one batch must not overlap. */
+typedef struct mg_matrices {
+    void* data;
+    uint64_t ld;
+    uint64_t stride;
+    uint32_t type;
+    uint32_t count;
+    uint32_t rows;
+    uint32_t cols;
+} mg_matrices;
+
+/* out = the iteration's result for each matrix of in, rounded once to out's type
+ * (any, as in's). out may be in. A matrix that holds NaN or infinity gives NaN
+ * throughout, one of zeros gives zeros; the others of the batch do not feel it.
+ * workspace: at least mg_orthogonalize_workspace bytes, 256-byte aligned. */
+int mg_orthogonalize_workspace(const mg_newton_schulz* ns, uint32_t count, uint32_t rows, uint32_t cols,
+                               uint64_t* bytes);
+int mg_orthogonalize(void* stream, const mg_newton_schulz* ns, const mg_matrices* in, const mg_matrices* out,
+                     void* workspace, uint64_t workspace_bytes);
+
+/* One step of the Muon optimiser on each matrix: M = M + (1 - momentum)(G - M);
+ * U = nesterov ? G + momentum (M - G) : M; W = (1 - lr weight_decay) W - lr scale O,
+ * O the Newton-Schulz result of U. scale 0 stands for sqrt(max(1, cols / rows)):
+ * rows are a layer's inputs and cols its outputs, as in the policy's matrices.
+ * lr, weight_decay and scale are finite and not negative, momentum in [0, 1). */
+typedef struct mg_muon_config {
+    float lr;
+    float momentum;
+    float weight_decay;
+    float scale;
+    uint32_t nesterov;
+    mg_newton_schulz ns; /* steps 0: the default iteration */
+} mg_muon_config;
+/* params (any type) and momentum (fp32) are updated in place; grad (any type) is
+ * read. All three have the same count, rows and cols, each its own ld and stride.
+ * Sums are fp32, params are rounded once. The workspace is mg_orthogonalize's. */
+int mg_muon_step(void* stream, const mg_muon_config* config, const mg_matrices* params, const mg_matrices* momentum,
+                 const mg_matrices* grad, void* workspace, uint64_t workspace_bytes);
 
 /* ---------------------------------------------------------------------------
  * Kernel timing for measurement: when enabled, the library records HIP events

@@ -15,6 +15,9 @@ from ._capi import (  # noqa: F401
     Gym,
     KernelTimes,
     LossStats,
+    Matrices,
+    MuonConfig,
+    NewtonSchulz,
     PPOConfig,
     PPOHParams,
     PPOModel,
@@ -29,6 +32,10 @@ from ._capi import (  # noqa: F401
     layernorm_backward,
     layernorm_backward_workspace,
     lib,
+    matrices,
+    muon_step,
+    orthogonalize,
+    orthogonalize_workspace,
     timing_enable,
     timing_get,
     timing_reset,

@@ -97,6 +97,22 @@ class LayernormBackwardArgs(C.Structure):
         (n, u32) for n in ("rows", "cols", "type", "reserved")] + [("workspace", P), ("workspace_bytes", u64)]
 
 
+class NewtonSchulz(C.Structure):
+    """mg_newton_schulz; steps 0 stands for the default iteration."""
+    _fields_ = [("steps", u32)] + [(n, f32) for n in ("a", "b", "c", "eps")]
+
+
+class Matrices(C.Structure):
+    """mg_matrices"""
+    _fields_ = [("data", P), ("ld", u64), ("stride", u64)] + [(n, u32) for n in ("type", "count", "rows", "cols")]
+
+
+class MuonConfig(C.Structure):
+    """mg_muon_config"""
+    _fields_ = [(n, f32) for n in ("lr", "momentum", "weight_decay", "scale")] + [("nesterov", u32),
+                                                                                  ("ns", NewtonSchulz)]
+
+
 class KernelTimes(C.Structure):
     _fields_ = [("total_ms", C.c_double * len(K_NAMES)), ("launches", C.c_uint64 * len(K_NAMES))]
 
@@ -174,6 +190,9 @@ def lib():
         "mg_layernorm": (I, [P, P]),
         "mg_layernorm_backward_workspace": (I, [u32, u32, P]),
         "mg_layernorm_backward": (I, [P, P]),
+        "mg_orthogonalize_workspace": (I, [P, u32, u32, u32, P]),
+        "mg_orthogonalize": (I, [P, P, P, P, P, u64]),
+        "mg_muon_step": (I, [P, P, P, P, P, P, u64]),
         "mg_timing_enable": (I, [I]),
         "mg_timing_get": (I, [P]),
         "mg_timing_reset": (I, []),
@@ -239,6 +258,34 @@ def layernorm_backward(x: int, dy: int, mean: int, rstd: int, dx: int, rows: int
     a = LayernormBackwardArgs(x, dy, dsum, gamma, mean, rstd, dx, dgamma, dbeta, x_ld, dy_ld, dsum_ld, dx_ld, rows,
                               cols, TYPES[dtype], 0, workspace, workspace_bytes)
     check(lib().mg_layernorm_backward(stream, C.byref(a)))
+
+
+def matrices(data: int, count: int, rows: int, cols: int, dtype: str = "fp32", ld: int = 0,
+             stride: int = 0) -> Matrices:
+    """mg_matrices: `count` row-major matrices at a device address."""
+    return Matrices(data, ld, stride, TYPES[dtype], count, rows, cols)
+
+
+def orthogonalize_workspace(count: int, rows: int, cols: int, ns: NewtonSchulz = None) -> int:
+    n = u64()
+    check(lib().mg_orthogonalize_workspace(C.byref(ns) if ns else None, count, rows, cols, C.byref(n)))
+    return n.value
+
+
+def orthogonalize(inp: Matrices, out: Matrices, *, ns: NewtonSchulz = None, workspace: int = None,
+                  workspace_bytes: int = 0, stream: int = None) -> None:
+    """mg_orthogonalize; asynchronous."""
+    check(lib().mg_orthogonalize(stream, C.byref(ns) if ns else None, C.byref(inp), C.byref(out), workspace,
+                                 workspace_bytes))
+
+
+def muon_step(params: Matrices, momentum_buffer: Matrices, grad: Matrices, *, lr: float = 0.02, momentum: float = 0.95,
+              weight_decay: float = 0.0, scale: float = 0.0, nesterov: bool = True, ns: NewtonSchulz = None,
+              workspace: int = None, workspace_bytes: int = 0, stream: int = None) -> None:
+    """mg_muon_step; asynchronous."""
+    cfg = MuonConfig(lr, momentum, weight_decay, scale, int(nesterov), ns or NewtonSchulz())
+    check(lib().mg_muon_step(stream, C.byref(cfg), C.byref(params), C.byref(momentum_buffer), C.byref(grad), workspace,
+                             workspace_bytes))
 
 
 class DeviceBuffer:

@@ -1,0 +1,618 @@
+// Matrices orthogonalised by Newton-Schulz steps (mg_orthogonalize) and the Muon
+// update built on them (mg_muon_step).
+//
+// X is m x n, m the short side. A step is X <- P X with P = a I + b A + c A^2 and
+// A = X X'. All of A, P and their products are symmetric and commute, so steps can
+// also be taken on m x m matrices alone: A <- P A P, Q <- P Q, and X <- Q X once
+// for several steps (a segment). On long matrices that saves the two products with
+// X of each step but the segment's first and last. An error of A grows by a^2 with
+// each step of a segment, the most where the small singular values are still small,
+// so segments are short: 1, 2 and 2 of the default's 5 steps are as close to 64 bits
+// as steps on X (128 x 512 with few strong directions: relative error 2.0e-6
+// against 1.8e-6, and plain fp32 1.9e-6; 2 and 3 steps 6.5e-6, one segment 5e-5).
+//
+// Products run on the matrix units as pairs of binary16 halves: x 2^e = hi + lo
+// with 22 bits, hi hi + hi lo + lo hi summed in fp32. The iteration's bounds are
+// known before it starts (singular values at most 2, polynomials at most 64, or the
+// call is refused), so every operand has a fixed exponent and nothing is measured
+// on the way. One binary16 product would lose the small singular values of a
+// matrix with few strong ones: 3e-2 of the result. The matrix units cut their sums
+// off instead of rounding them, which makes A's diagonal a little short each time;
+// chains of 64 contraction elements, added up in fp32, keep that under the rest
+// (4.0e-6 of the result in one chain, 2.1e-6 so).
+//
+// Every operand is kept with its contraction index contiguous and both sides
+// padded to the tile with zeros, so the product kernel has no bounds checks.
+#include <math.h>
+
+#include <vector>
+
+#include "kernels.h"
+#include "mg/device/common.h"
+#include "operator_types.h"
+
+namespace mg {
+namespace dev {
+
+typedef _Float16 f16;
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kPT = 128;  // edge of a product tile; both sides are padded to it
+constexpr int kPK = 32;   // contraction elements of a stage
+constexpr int kNormParts = 128;  // most partial sums of a matrix's squares
+
+// A batch of matrices of any type as a kernel reads or writes it.
+struct Batch {
+    void* data;
+    size_t ld, stride;
+    uint32_t type;
+};
+__device__ __forceinline__ float batch_load(const Batch& b, size_t at) {
+    if (b.type == MG_TYPE_FP32) return static_cast<const float*>(b.data)[at];
+    if (b.type == MG_TYPE_BF16) return (float)static_cast<const __bf16*>(b.data)[at];
+    return (float)static_cast<const f16*>(b.data)[at];
+}
+__device__ __forceinline__ void batch_store(const Batch& b, size_t at, float x) {
+    if (b.type == MG_TYPE_FP32)
+        static_cast<float*>(b.data)[at] = x;
+    else if (b.type == MG_TYPE_BF16)
+        static_cast<__bf16*>(b.data)[at] = (__bf16)x;
+    else
+        static_cast<f16*>(b.data)[at] = (f16)x;
+}
+
+// What is orthogonalised: `in`, or with a momentum batch the Muon update's U from
+// the gradient `in`, times the gradient's clip scale.
+struct SourceArgs {
+    Batch in, momentum;  // momentum.data NULL: in alone
+    uint32_t rows, cols;
+    float beta;
+    uint32_t nesterov;
+};
+// U(i, j) of matrix k; UPDATE also moves the momentum to this gradient.
+template <bool UPDATE>
+__device__ __forceinline__ float source_value(const SourceArgs& a, uint32_t k, uint32_t i, uint32_t j) {
+    const float g = batch_load(a.in, k * a.in.stride + i * a.in.ld + j);
+    if (!a.momentum.data) return g;
+    float* const mp = static_cast<float*>(a.momentum.data) + k * a.momentum.stride + i * a.momentum.ld + j;
+    float m = *mp;
+    if constexpr (UPDATE) {
+        m = m + (1.0f - a.beta) * (g - m);
+        *mp = m;
+    }
+    return a.nesterov ? g + a.beta * (m - g) : m;
+}
+
+// Partial sums of U^2 in 64 bits (fp32 squares leave its range), [count][gridDim.x]
+// of them, and the momentum's update.
+__global__ void __launch_bounds__(256) source_norm_kernel(const SourceArgs a, double* partial) {
+    __shared__ double red[4];
+    const uint32_t k = blockIdx.y, tiles_c = (a.cols + 63) / 64, tiles = tiles_c * ((a.rows + 63) / 64);
+    double s = 0.0;
+    for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+        const uint32_t j = (t % tiles_c) * 64 + (threadIdx.x & 63), i0 = (t / tiles_c) * 64 + (threadIdx.x >> 6);
+        if (j < a.cols)
+            for (uint32_t i = i0; i < i0 + 64 && i < a.rows; i += 4) {
+                const double u = source_value<true>(a, k, i, j);
+                s += u * u;
+            }
+    }
+    for (int step = 1; step < 64; step *= 2) s += __shfl_xor(s, step);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) partial[(size_t)k * gridDim.x + blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+// 1 / (|U| + eps) in every thread, NaN where the norm is not finite. red holds 1.
+__device__ __forceinline__ float source_scale(const double* partial, uint32_t parts, float eps, float* red) {
+    if (threadIdx.x < 64) {
+        double s = 0.0;
+        for (uint32_t p = threadIdx.x; p < parts; p += 64) s += partial[p];
+        for (int step = 1; step < 64; step *= 2) s += __shfl_xor(s, step);
+        if (threadIdx.x == 0) {
+            const double norm = sqrt(s);
+            *red = norm < (double)__builtin_huge_valf() ? (float)(1.0 / (norm + (double)eps)) : __builtin_nanf("");
+        }
+    }
+    __syncthreads();
+    return *red;
+}
+
+// A pair of planes: the low halves lie `plane` elements after the high ones.
+struct Planes {
+    f16* hi;
+    size_t plane;   // elements of one plane
+    size_t stride;  // elements between matrices of the batch
+    uint32_t ld;
+};
+__device__ __forceinline__ void split(float x, f16& hi, f16& lo) {
+    hi = (f16)x;
+    lo = (f16)(x - (float)hi);
+}
+
+// U / (|U| + eps) times 2^e as pairs, X [mp][np] and its transpose XT [np][mp],
+// zeros in the padding; one 64 x 64 tile of X a workgroup.
+__global__ void __launch_bounds__(256) source_split_kernel(const SourceArgs a, const double* partial, uint32_t parts,
+                                                           float eps, float unit, Planes X, Planes XT) {
+    __shared__ float lds[64][65];
+    __shared__ float red;
+    const uint32_t k = blockIdx.z, t = threadIdx.x;
+    const float scale = source_scale(partial + (size_t)k * parts, parts, eps, &red);
+    const bool tall = a.rows > a.cols;
+    // the tile in the source's orientation, so that reads run along its rows
+    const uint32_t x0 = blockIdx.y * 64, y0 = blockIdx.x * 64;  // X's row and column
+    const uint32_t i0 = tall ? y0 : x0, j0 = tall ? x0 : y0;
+    for (uint32_t e = t >> 6; e < 64; e += 4) {
+        const uint32_t i = i0 + e, j = j0 + (t & 63);
+        const float u = i < a.rows && j < a.cols ? source_value<false>(a, k, i, j) * scale * unit : 0.0f;
+        if (tall)
+            lds[t & 63][e] = u;
+        else
+            lds[e][t & 63] = u;
+    }
+    __syncthreads();
+    f16* const x = X.hi + k * X.stride;
+    f16* const xt = XT.hi + k * XT.stride;
+    const uint32_t c = (t & 15) * 4;
+    for (uint32_t r = t >> 4; r < 64; r += 16) {
+        f16x4 h, l, ht, lt;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            f16 p, q;
+            split(lds[r][c + e], p, q);
+            h[e] = p, l[e] = q;
+            split(lds[c + e][r], p, q);
+            ht[e] = p, lt[e] = q;
+        }
+        const size_t at = (size_t)(x0 + r) * X.ld + y0 + c, at_t = (size_t)(y0 + r) * XT.ld + x0 + c;
+        *reinterpret_cast<f16x4*>(x + at) = h;
+        *reinterpret_cast<f16x4*>(x + X.plane + at) = l;
+        *reinterpret_cast<f16x4*>(xt + at_t) = ht;
+        *reinterpret_cast<f16x4*>(xt + XT.plane + at_t) = lt;
+    }
+}
+
+// What becomes of a product's element v = (a b')(i, j).
+enum {
+    kSymmetric = 0,  // out(i, j) = out(j, i) = v
+    kPolynomial,     // the same with c v + b A(i, j) + a [i = j], v = (A A)(i, j)
+    kUpdate,         // X' = v, both X [i][j] and XT [j][i]
+    kFinal,          // the result: out = v, or w = keep w - rate v
+};
+struct ProductArgs {
+    Planes a, b;       // [rows][K], [cols][K]
+    uint32_t k;        // K, a multiple of two stages
+    uint32_t tiles_j;  // tile columns (symmetric results: tile rows and columns)
+    float unit;        // takes the operands' exponents out of the sums and puts the result's in
+    Planes out, out_t;
+    // kPolynomial
+    Planes gram;
+    float ca, cb, cc;  // with the result's exponent; cc also takes the operands' out
+    uint32_t m;        // rows that hold a matrix: no a I in the padding
+    // kFinal
+    Batch dst;
+    uint32_t rows, cols;
+    uint32_t step;  // an optimiser step
+    float keep, rate;
+};
+
+// One 128 x 128 tile of a product a b' of pairs. Four waves, 64 x 64 each as 2 x 2
+// tiles of v_mfma_f32_32x32x16_f16. Stages of 32 contraction elements go from
+// memory straight to LDS (16 bytes a lane, two buffers, so a stage's loads run
+// under the one before). In a 64-byte LDS row the 16-byte chunk c of row r sits at
+// c ^ (r / 2 % 4), which spreads a fragment's reads over all banks; the loads take
+// the chunk from where it belongs, since the LDS side of such a load is linear.
+template <int KIND>
+__global__ void __launch_bounds__(256) product_kernel(const ProductArgs p) {
+    constexpr int kRowB = kPK * 2, kPlaneB = kPT * kRowB, kStageB = 4 * kPlaneB;  // bytes
+    __shared__ __align__(1024) char lds[2 * kStageB];
+    uint32_t ti, tj;
+    if constexpr (KIND <= kPolynomial) {
+        // tiles on and under the diagonal, row by row
+        ti = (uint32_t)((sqrtf(8.0f * (float)blockIdx.x + 1.0f) - 1.0f) * 0.5f);
+        while (ti * (ti + 1) / 2 > blockIdx.x) --ti;
+        while ((ti + 1) * (ti + 2) / 2 <= blockIdx.x) ++ti;
+        tj = blockIdx.x - ti * (ti + 1) / 2;
+    } else {
+        ti = blockIdx.x / p.tiles_j, tj = blockIdx.x % p.tiles_j;
+    }
+    const uint32_t mat = blockIdx.y;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // this lane's part of a stage's loads: wave w brings plane w (a hi, a lo, b hi, b
+    // lo), 16 rows an instruction
+    const Planes& src = wave < 2 ? p.a : p.b;
+    const f16* from = src.hi + mat * src.stride + (wave & 1) * src.plane +
+                      (size_t)((wave < 2 ? ti : tj) * kPT + (lane >> 2)) * src.ld +
+                      ((lane & 3) ^ ((lane >> 3) & 3)) * 8;
+    const size_t step16 = (size_t)16 * src.ld;
+    auto load = [&](int buf) {
+        char* to = lds + buf * kStageB + wave * kPlaneB;
+#pragma unroll
+        for (int r = 0; r < kPT / 16; ++r)
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void*)(from + r * step16),
+                (__attribute__((address_space(3))) void*)(to + r * 16 * kRowB), 16, 0, 0);
+        from += kPK;
+    };
+    const int wi = (wave >> 1) * 64, wj = (wave & 1) * 64, row = lane & 31;
+    f32x16 acc[2][2] = {}, sum[2][2];
+    const uint32_t stages = p.k / kPK;
+    load(0);
+    for (uint32_t s = 0; s < stages; s += 2) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            // this stage has arrived, and every wave is done with the buffer that the next goes to
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (s + half + 1 < stages) load(half ^ 1);
+            const char* base = lds + half * kStageB;
+#pragma unroll
+            for (int kk = 0; kk < kPK / 16; ++kk) {
+                const int chunk = (kk * 2 + (lane >> 5)) ^ ((row >> 1) & 3);
+                f16x8 fa[2][2], fb[2][2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int at = (32 * q + row) * kRowB + chunk * 16;
+                        fa[q][h] = *reinterpret_cast<const f16x8*>(base + h * kPlaneB + wi * kRowB + at);
+                        fb[q][h] = *reinterpret_cast<const f16x8*>(base + (2 + h) * kPlaneB + wj * kRowB + at);
+                    }
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const f32x16 zero = {};
+                        f32x16 t = half == 0 && kk == 0 ? zero : sum[i][j];
+                        t = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][1], fb[j][0], t, 0, 0, 0);
+                        t = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][0], fb[j][1], t, 0, 0, 0);
+                        sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][0], fb[j][0], t, 0, 0, 0);
+                    }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) acc[i][j] += sum[i][j];
+    }
+#pragma unroll
+    for (int qi = 0; qi < 2; ++qi)
+#pragma unroll
+        for (int qj = 0; qj < 2; ++qj) {
+            const uint32_t i0 = ti * kPT + wi + 32 * qi + 4 * (lane >> 5), j = tj * kPT + wj + 32 * qj + row;
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const uint32_t i = i0 + 2 * r;  // four rows from here: registers r .. r + 3
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = acc[qi][qj][r + e];
+                if constexpr (KIND == kFinal) {
+                    const bool tall = p.rows > p.cols;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t y = tall ? j : i + e, x = tall ? i + e : j;
+                        if (y >= p.rows || x >= p.cols) continue;
+                        const size_t at = mat * p.dst.stride + y * p.dst.ld + x;
+                        const float o = v[e] * p.unit;
+                        batch_store(p.dst, at, p.step ? p.keep * batch_load(p.dst, at) - p.rate * o : o);
+                    }
+                } else {
+                    const f16* gram = p.gram.hi + mat * p.gram.stride;
+                    f16* out = p.out.hi + mat * p.out.stride;
+                    f16* out_t = p.out_t.hi + mat * p.out_t.stride;
+                    f16x4 th, tl;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float x = v[e] * p.unit;
+                        if constexpr (KIND == kPolynomial) {
+                            const size_t at = (size_t)(i + e) * p.gram.ld + j;
+                            x = p.cc * v[e] + p.cb * ((float)gram[at] + (float)gram[p.gram.plane + at]) +
+                                (i + e == j && j < p.m ? p.ca : 0.0f);
+                        }
+                        f16 h, l;
+                        split(x, h, l);
+                        th[e] = h, tl[e] = l;
+                        const size_t at = (size_t)(i + e) * p.out.ld + j;
+                        out[at] = h;
+                        out[p.out.plane + at] = l;
+                    }
+                    const size_t at = (size_t)j * p.out_t.ld + i;
+                    if (KIND == kUpdate || ti != tj) {
+                        *reinterpret_cast<f16x4*>(out_t + at) = th;
+                        *reinterpret_cast<f16x4*>(out_t + p.out_t.plane + at) = tl;
+                    }
+                }
+            }
+        }
+}
+
+}  // namespace dev
+
+namespace {
+
+constexpr mg_newton_schulz kDefaultNs = {5, 3.4445f, -4.7750f, 2.0315f, 1e-7f};
+constexpr uint32_t kMostSide = 65536, kMostShort = 8192, kMostSteps = 32;
+constexpr double kMostSingular = 2.0, kMostPolynomial = 64.0;
+// Exponents of the operands' pairs: X and A at most 2 and 4 in size, P at most
+// 64, so that 2^13 and 2^9 keep them under 2^15, half of binary16's range.
+constexpr float kUnitX = 8192.0f, kUnitA = 8192.0f, kUnitP = 512.0f;
+
+size_t align256(size_t x) { return (x + 255) / 256 * 256; }
+uint32_t pad(uint32_t x) { return (x + dev::kPT - 1) / dev::kPT * dev::kPT; }
+
+// Steps of the next segment of the `left` that remain. On X where the sides are
+// alike (no products saved), where the matrices are too small for a rounding error
+// of A to average out, and for polynomials that grow small singular values faster
+// than the default's.
+uint32_t segment_steps(const mg_newton_schulz& ns, uint32_t m, uint32_t n, uint32_t left) {
+    if (n < m + m / 4 || m < 32 || fabsf(ns.a) > 4.0f) return 1;
+    return left & 1 ? 1 : 2;
+}
+
+// Takes [0, *reach] to the largest |p(s)| on it, and gives the largest
+// |a + b s^2 + c s^4| there: both have their extremes at 0, at the end, or where
+// the derivative in s^2 is 0.
+double step_bounds(const mg_newton_schulz& ns, double* reach) {
+    const double a = ns.a, b = ns.b, c = ns.c, end = *reach * *reach;
+    double most = 0.0, poly = 0.0;
+    auto look = [&](double t) {  // t = s^2
+        if (!(t >= 0.0 && t <= end)) return;
+        const double q = fabs(a + t * (b + t * c));
+        poly = q > poly ? q : poly;
+        most = sqrt(t) * q > most ? sqrt(t) * q : most;
+    };
+    look(0.0);
+    look(end);
+    if (c != 0.0) {
+        look(-b / (2 * c));
+        const double d = 9 * b * b - 20 * a * c;
+        if (d >= 0.0) {
+            look((-3 * b + sqrt(d)) / (10 * c));
+            look((-3 * b - sqrt(d)) / (10 * c));
+        }
+    } else if (b != 0.0) {
+        look(-a / (3 * b));
+    }
+    *reach = most;
+    return poly;
+}
+
+int check_ns(const char* what, const mg_newton_schulz* in, mg_newton_schulz* ns) {
+    *ns = in ? *in : kDefaultNs;
+    MG_CHECK(ns->steps >= 1 && ns->steps <= kMostSteps, MG_ERR_INVALID, "%s: steps %u must be in [1, %u]", what, ns->steps,
+             kMostSteps);
+    MG_CHECK(ns->eps > 0.0f && ns->eps < __builtin_huge_valf(), MG_ERR_INVALID, "%s: eps must be positive and finite",
+             what);
+    double reach = 1.0;
+    for (uint32_t k = 0; k < ns->steps; ++k) {
+        const double poly = step_bounds(*ns, &reach);
+        MG_CHECK(isfinite(ns->a) && isfinite(ns->b) && isfinite(ns->c) && reach <= kMostSingular &&
+                     poly <= kMostPolynomial,
+                 MG_ERR_INVALID,
+                 "%s: the polynomial (%g, %g, %g) leaves [-2, 2] in step %u, or a + b s^2 + c s^4 [-64, 64]", what,
+                 (double)ns->a, (double)ns->b, (double)ns->c, k + 1);
+    }
+    return MG_OK;
+}
+
+int check_shape(const char* what, uint32_t count, uint32_t rows, uint32_t cols) {
+    MG_CHECK(rows >= 1 && cols >= 1 && rows <= kMostSide && cols <= kMostSide, MG_ERR_INVALID,
+             "%s: %u x %u: the sides must be in [1, %u]", what, rows, cols, kMostSide);
+    MG_CHECK((rows < cols ? rows : cols) <= kMostShort, MG_ERR_INVALID,
+             "%s: %u x %u: the smaller side must be at most %u", what, rows, cols, kMostShort);
+    MG_CHECK(count <= 65535, MG_ERR_INVALID, "%s: count %u must be at most 65535", what, count);
+    return MG_OK;
+}
+
+int check_batch(const char* what, const char* name, const mg_matrices* in, dev::Batch* out) {
+    MG_CHECK(in, MG_ERR_INVALID, "%s: %s is NULL", what, name);
+    int rc = check_shape(what, in->count, in->rows, in->cols);
+    if (rc) return rc;
+    MG_CHECK(type_known(in->type), MG_ERR_INVALID, "%s: %s has unknown type %u", what, name, in->type);
+    MG_CHECK(in->data || !in->count, MG_ERR_INVALID, "%s: %s has no data", what, name);
+    MG_CHECK(aligned(in->data, type_bytes(in->type)), MG_ERR_INVALID, "%s: %s is not aligned to its type", what, name);
+    const uint64_t ld = in->ld ? in->ld : in->cols;
+    MG_CHECK(ld >= in->cols && ld <= (1ull << 32), MG_ERR_INVALID, "%s: %s: ld %llu must be at least cols", what, name,
+             (unsigned long long)ld);
+    const uint64_t stride = in->stride ? in->stride : in->rows * ld;
+    MG_CHECK(in->count <= 1 || (stride >= (in->rows - 1) * ld + in->cols && stride <= (1ull << 44)), MG_ERR_INVALID,
+             "%s: %s: stride %llu: the matrices overlap", what, name, (unsigned long long)stride);
+    *out = dev::Batch{in->data, (size_t)ld, (size_t)stride, in->type};
+    return MG_OK;
+}
+
+int check_same(const char* what, const mg_matrices* a, const mg_matrices* b) {
+    MG_CHECK(a->count == b->count && a->rows == b->rows && a->cols == b->cols, MG_ERR_INVALID,
+             "%s: the batches differ in shape: %u of %u x %u and %u of %u x %u", what, a->count, a->rows, a->cols,
+             b->count, b->rows, b->cols);
+    return MG_OK;
+}
+
+// The workspace of a batch.
+struct Workspace {
+    size_t norms, x, xt[2], gram, product, poly, q[2], total;  // byte offsets
+    uint32_t m, n, mp, np;
+    Workspace(uint32_t count, uint32_t rows, uint32_t cols) {
+        m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+        mp = pad(m), np = pad(n);
+        const size_t wide = (size_t)count * mp * np * 4, square = (size_t)count * mp * mp * 4;
+        total = 0;
+        auto take = [&](size_t bytes) {
+            const size_t at = total;
+            total += align256(bytes);
+            return at;
+        };
+        norms = take((size_t)count * dev::kNormParts * 8);
+        x = take(wide), xt[0] = take(wide), xt[1] = take(wide);
+        gram = take(square), product = take(square), poly = take(square), q[0] = take(square), q[1] = take(square);
+    }
+};
+
+struct FinalArgs {
+    dev::Batch dst;
+    uint32_t step;
+    float keep, rate;
+};
+
+int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, const dev::SourceArgs& src,
+                  const FinalArgs& fin, void* workspace) {
+    const Workspace w(count, src.rows, src.cols);
+    char* const base = static_cast<char*>(workspace);
+    auto planes = [&](size_t at, uint32_t rows, uint32_t ld) {
+        const size_t plane = (size_t)rows * ld;
+        return dev::Planes{reinterpret_cast<dev::f16*>(base + at), plane, 2 * plane, ld};
+    };
+    double* const norms = reinterpret_cast<double*>(base + w.norms);
+    const dev::Planes X = planes(w.x, w.mp, w.np);
+    const dev::Planes XT[2] = {planes(w.xt[0], w.np, w.mp), planes(w.xt[1], w.np, w.mp)};
+    const dev::Planes gram = planes(w.gram, w.mp, w.mp), prod = planes(w.product, w.mp, w.mp),
+                      poly = planes(w.poly, w.mp, w.mp);
+    const dev::Planes Q[2] = {planes(w.q[0], w.mp, w.mp), planes(w.q[1], w.mp, w.mp)};
+    const uint32_t tiles = ((src.rows + 63) / 64) * ((src.cols + 63) / 64);
+    const uint32_t parts = tiles < (uint32_t)dev::kNormParts ? tiles : dev::kNormParts;
+    hipLaunchKernelGGL(dev::source_norm_kernel, dim3(parts, count), dim3(256), 0, st, src, norms);
+    MG_HIP(hipGetLastError(), "newton-schulz norm launch");
+    hipLaunchKernelGGL(dev::source_split_kernel, dim3(w.np / 64, w.mp / 64, count), dim3(256), 0, st, src, norms, parts,
+                       ns.eps, kUnitX, X, XT[0]);
+    MG_HIP(hipGetLastError(), "newton-schulz split launch");
+
+    const uint32_t mt = w.mp / dev::kPT, nt = w.np / dev::kPT;
+    const dim3 half(mt * (mt + 1) / 2, count), full(mt * nt, count), block(256);
+    dev::ProductArgs p{};
+    p.m = w.m;
+    // out = a b' of symmetric results
+    auto symmetric = [&](const dev::Planes& a, const dev::Planes& b, uint32_t k, float unit_a, float unit_b,
+                         const dev::Planes& out, float unit_out) -> int {
+        p.a = a, p.b = b, p.k = k, p.tiles_j = mt, p.out = out, p.out_t = out;
+        p.unit = unit_out / (unit_a * unit_b);
+        hipLaunchKernelGGL((dev::product_kernel<dev::kSymmetric>), half, block, 0, st, p);
+        MG_HIP(hipGetLastError(), "newton-schulz product launch");
+        return MG_OK;
+    };
+    auto polynomial = [&](const dev::Planes& out) -> int {
+        p.a = p.b = p.gram = gram, p.k = w.mp, p.tiles_j = mt, p.out = out, p.out_t = out;
+        p.ca = ns.a * kUnitP, p.cb = ns.b * (kUnitP / kUnitA), p.cc = ns.c * (kUnitP / (kUnitA * kUnitA));
+        hipLaunchKernelGGL((dev::product_kernel<dev::kPolynomial>), half, block, 0, st, p);
+        MG_HIP(hipGetLastError(), "newton-schulz polynomial launch");
+        return MG_OK;
+    };
+    int rc, cur = 0;
+    double reach = 1.0;
+    for (uint32_t left = ns.steps; left;) {
+        const uint32_t steps = segment_steps(ns, w.m, w.n, left);
+        if ((rc = symmetric(X, X, w.np, kUnitX, kUnitX, gram, kUnitA))) return rc;
+        int q = 0;
+        float unit_q = kUnitP;
+        double most_q = step_bounds(ns, &reach);
+        if ((rc = polynomial(Q[0]))) return rc;
+        for (uint32_t k = 1; k < steps; ++k) {
+            const dev::Planes& last = k == 1 ? Q[0] : poly;
+            if ((rc = symmetric(last, gram, w.mp, kUnitP, kUnitA, prod, kUnitA)) ||
+                (rc = symmetric(last, prod, w.mp, kUnitP, kUnitA, gram, kUnitA)) || (rc = polynomial(poly)))
+                return rc;
+            most_q *= step_bounds(ns, &reach);
+            // the largest power of two that keeps the product under 2^15
+            const float unit = ldexpf(1.0f, 15 - ilogb(most_q > 1.0 ? most_q : 1.0) - 1);
+            if ((rc = symmetric(poly, Q[q], w.mp, kUnitP, unit_q, Q[q ^ 1], unit))) return rc;
+            unit_q = unit, q ^= 1;
+        }
+        left -= steps;
+        p.a = Q[q], p.b = XT[cur], p.k = w.mp, p.tiles_j = nt;
+        if (left) {
+            p.out = X, p.out_t = XT[cur ^ 1], p.unit = 1.0f / unit_q;
+            hipLaunchKernelGGL((dev::product_kernel<dev::kUpdate>), full, block, 0, st, p);
+            MG_HIP(hipGetLastError(), "newton-schulz update launch");
+            cur ^= 1;
+        } else {
+            p.dst = fin.dst, p.step = fin.step, p.keep = fin.keep, p.rate = fin.rate, p.rows = src.rows, p.cols = src.cols;
+            p.unit = 1.0f / (unit_q * kUnitX);
+            hipLaunchKernelGGL((dev::product_kernel<dev::kFinal>), full, block, 0, st, p);
+            MG_HIP(hipGetLastError(), "newton-schulz result launch");
+        }
+    }
+    return MG_OK;
+}
+
+int check_workspace(const char* what, uint32_t count, uint32_t rows, uint32_t cols, const void* workspace,
+                    uint64_t bytes) {
+    const uint64_t need = Workspace(count, rows, cols).total;
+    MG_CHECK(workspace && bytes >= need, MG_ERR_INVALID, "%s: the workspace needs %llu bytes", what,
+             (unsigned long long)need);
+    MG_CHECK(aligned(workspace, 256), MG_ERR_INVALID, "%s: the workspace is not 256-byte aligned", what);
+    return MG_OK;
+}
+
+}  // namespace
+}  // namespace mg
+
+using namespace mg;
+
+extern "C" {
+
+int mg_orthogonalize_workspace(const mg_newton_schulz* in, uint32_t count, uint32_t rows, uint32_t cols,
+                               uint64_t* bytes) {
+    const char* what = "orthogonalize workspace";
+    MG_CHECK(bytes, MG_ERR_INVALID, "orthogonalize workspace: null argument");
+    mg_newton_schulz ns;
+    int rc;
+    if ((rc = check_ns(what, in, &ns)) || (rc = check_shape(what, count, rows, cols))) return rc;
+    *bytes = count ? Workspace(count, rows, cols).total : 0;
+    return MG_OK;
+}
+
+int mg_orthogonalize(void* stream, const mg_newton_schulz* in_ns, const mg_matrices* in, const mg_matrices* out,
+                     void* workspace, uint64_t workspace_bytes) {
+    const char* what = "orthogonalize";
+    mg_newton_schulz ns;
+    dev::SourceArgs src{};
+    FinalArgs fin{};
+    int rc;
+    if ((rc = check_ns(what, in_ns, &ns)) || (rc = check_batch(what, "in", in, &src.in)) ||
+        (rc = check_batch(what, "out", out, &fin.dst)) || (rc = check_same(what, in, out)))
+        return rc;
+    if (!in->count) return MG_OK;
+    if ((rc = check_workspace(what, in->count, in->rows, in->cols, workspace, workspace_bytes))) return rc;
+    src.rows = in->rows, src.cols = in->cols;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    StreamDevice on;
+    if ((rc = on.enter(st, "orthogonalize: stream device"))) return rc;
+    return newton_schulz(st, ns, in->count, src, fin, workspace);
+}
+
+int mg_muon_step(void* stream, const mg_muon_config* c, const mg_matrices* params, const mg_matrices* momentum,
+                 const mg_matrices* grad, void* workspace, uint64_t workspace_bytes) {
+    const char* what = "muon step";
+    MG_CHECK(c, MG_ERR_INVALID, "muon step: null argument");
+    auto fine = [](float x) { return x >= 0.0f && x < __builtin_huge_valf(); };
+    MG_CHECK(fine(c->lr) && fine(c->weight_decay) && fine(c->scale), MG_ERR_INVALID,
+             "muon step: lr, weight_decay and scale must be finite and not negative");
+    MG_CHECK(c->momentum >= 0.0f && c->momentum < 1.0f, MG_ERR_INVALID, "muon step: momentum must be in [0, 1)");
+    mg_newton_schulz ns;
+    dev::SourceArgs src{};
+    FinalArgs fin{};
+    int rc;
+    if ((rc = check_ns(what, c->ns.steps ? &c->ns : nullptr, &ns)) ||
+        (rc = check_batch(what, "params", params, &fin.dst)) ||
+        (rc = check_batch(what, "momentum", momentum, &src.momentum)) ||
+        (rc = check_batch(what, "grad", grad, &src.in)) || (rc = check_same(what, params, momentum)) ||
+        (rc = check_same(what, params, grad)))
+        return rc;
+    MG_CHECK(momentum->type == MG_TYPE_FP32, MG_ERR_INVALID, "muon step: momentum must be fp32");
+    if (!params->count) return MG_OK;
+    if ((rc = check_workspace(what, params->count, params->rows, params->cols, workspace, workspace_bytes))) return rc;
+    src.rows = params->rows, src.cols = params->cols;
+    src.beta = c->momentum, src.nesterov = c->nesterov != 0;
+    const float scale = c->scale > 0.0f ? c->scale
+                        : params->cols > params->rows ? sqrtf((float)params->cols / (float)params->rows)
+                                                      : 1.0f;
+    fin.step = 1;
+    fin.keep = 1.0f - c->lr * c->weight_decay;
+    fin.rate = c->lr * scale;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    StreamDevice on;
+    if ((rc = on.enter(st, "muon step: stream device"))) return rc;
+    return newton_schulz(st, ns, params->count, src, fin, workspace);
+}
+
+}  // extern "C"
