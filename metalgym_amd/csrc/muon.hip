@@ -23,66 +23,14 @@
 //
 // Every operand is kept with its contraction index contiguous and both sides
 // padded to the tile with zeros, so the product kernel has no bounds checks.
-#include <math.h>
-
-#include <vector>
-
-#include "kernels.h"
-#include "mg/device/common.h"
-#include "operator_types.h"
+#include "muon_short.h"
 
 namespace mg {
 namespace dev {
 
-typedef _Float16 f16;
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
 constexpr int kPT = 128;  // edge of a product tile; both sides are padded to it
 constexpr int kPK = 32;   // contraction elements of a stage
 constexpr int kNormParts = 128;  // most partial sums of a matrix's squares
-
-// A batch of matrices of any type as a kernel reads or writes it.
-struct Batch {
-    void* data;
-    size_t ld, stride;
-    uint32_t type;
-};
-__device__ __forceinline__ float batch_load(const Batch& b, size_t at) {
-    if (b.type == MG_TYPE_FP32) return static_cast<const float*>(b.data)[at];
-    if (b.type == MG_TYPE_BF16) return (float)static_cast<const __bf16*>(b.data)[at];
-    return (float)static_cast<const f16*>(b.data)[at];
-}
-__device__ __forceinline__ void batch_store(const Batch& b, size_t at, float x) {
-    if (b.type == MG_TYPE_FP32)
-        static_cast<float*>(b.data)[at] = x;
-    else if (b.type == MG_TYPE_BF16)
-        static_cast<__bf16*>(b.data)[at] = (__bf16)x;
-    else
-        static_cast<f16*>(b.data)[at] = (f16)x;
-}
-
-// What is orthogonalised: `in`, or with a momentum batch the Muon update's U from
-// the gradient `in`, times the gradient's clip scale.
-struct SourceArgs {
-    Batch in, momentum;  // momentum.data NULL: in alone
-    uint32_t rows, cols;
-    float beta;
-    uint32_t nesterov;
-};
-// U(i, j) of matrix k; UPDATE also moves the momentum to this gradient.
-template <bool UPDATE>
-__device__ __forceinline__ float source_value(const SourceArgs& a, uint32_t k, uint32_t i, uint32_t j) {
-    const float g = batch_load(a.in, k * a.in.stride + i * a.in.ld + j);
-    if (!a.momentum.data) return g;
-    float* const mp = static_cast<float*>(a.momentum.data) + k * a.momentum.stride + i * a.momentum.ld + j;
-    float m = *mp;
-    if constexpr (UPDATE) {
-        m = m + (1.0f - a.beta) * (g - m);
-        *mp = m;
-    }
-    return a.nesterov ? g + a.beta * (m - g) : m;
-}
 
 // Partial sums of U^2 in 64 bits (fp32 squares leave its range), [count][gridDim.x]
 // of them, and the momentum's update.
@@ -126,10 +74,6 @@ struct Planes {
     size_t stride;  // elements between matrices of the batch
     uint32_t ld;
 };
-__device__ __forceinline__ void split(float x, f16& hi, f16& lo) {
-    hi = (f16)x;
-    lo = (f16)(x - (float)hi);
-}
 
 // U / (|U| + eps) times 2^e as pairs, X [mp][np] and its transpose XT [np][mp],
 // zeros in the padding; one 64 x 64 tile of X a workgroup.
@@ -334,20 +278,23 @@ namespace {
 constexpr mg_newton_schulz kDefaultNs = {5, 3.4445f, -4.7750f, 2.0315f, 1e-7f};
 constexpr uint32_t kMostSide = 65536, kMostShort = 8192, kMostSteps = 32;
 constexpr double kMostSingular = 2.0, kMostPolynomial = 64.0;
-// Exponents of the operands' pairs: X and A at most 2 and 4 in size, P at most
-// 64, so that 2^13 and 2^9 keep them under 2^15, half of binary16's range.
-constexpr float kUnitX = 8192.0f, kUnitA = 8192.0f, kUnitP = 512.0f;
+using dev::kUnitA;
+using dev::kUnitP;
+using dev::kUnitX;
 
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 uint32_t pad(uint32_t x) { return (x + dev::kPT - 1) / dev::kPT * dev::kPT; }
 
-// Steps of the next segment of the `left` that remain. On X where the sides are
-// alike (no products saved), where the matrices are too small for a rounding error
-// of A to average out, and for polynomials that grow small singular values faster
-// than the default's.
+// Steps of the next segment of the `left` that remain. On X for small matrices,
+// where a rounding error of A does not average out, and for polynomials that grow
+// small singular values, and their errors, faster than the default's.
+uint32_t segment_steps(const mg_newton_schulz& ns, uint32_t m, uint32_t left) {
+    return (left & 1) || m < 32 || fabsf(ns.a) > 4.0f ? 1 : 2;
+}
+// The same for tiled products: on X where the sides are alike, as a segment then
+// saves no products.
 uint32_t segment_steps(const mg_newton_schulz& ns, uint32_t m, uint32_t n, uint32_t left) {
-    if (n < m + m / 4 || m < 32 || fabsf(ns.a) > 4.0f) return 1;
-    return left & 1 ? 1 : 2;
+    return n < m + m / 4 ? 1 : segment_steps(ns, m, left);
 }
 
 // Takes [0, *reach] to the largest |p(s)| on it, and gives the largest
@@ -377,6 +324,9 @@ double step_bounds(const mg_newton_schulz& ns, double* reach) {
     *reach = most;
     return poly;
 }
+
+// A power of two that keeps values of up to `most` under 2^15.
+float unit_of(double most) { return ldexpf(1.0f, 14 - ilogb(most > 1.0 ? most : 1.0)); }
 
 int check_ns(const char* what, const mg_newton_schulz* in, mg_newton_schulz* ns) {
     *ns = in ? *in : kDefaultNs;
@@ -449,14 +399,77 @@ struct Workspace {
     }
 };
 
+// The workspace of a batch whose short side is at most 128 (muon_short.h).
+struct ShortWorkspace {
+    size_t xt, partial, q, state, total;
+    uint32_t mp, slabs, parts;
+    ShortWorkspace(uint32_t count, uint32_t rows, uint32_t cols) {
+        const uint32_t m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+        mp = m <= 32 ? 32 : m <= 64 ? 64 : 128;
+        slabs = (n + dev::kSlab - 1) / dev::kSlab;
+        parts = slabs < (uint32_t)dev::kShortParts ? slabs : dev::kShortParts;
+        const uint32_t tiles = mp / 32 * (mp / 32 + 1) / 2;
+        xt = 0;
+        partial = xt + align256((size_t)count * slabs * dev::kSlab * mp * 4);
+        q = partial + align256((size_t)count * parts * tiles * 4096);
+        state = q + align256((size_t)count * mp * mp * 4);
+        total = state + align256((size_t)count * sizeof(dev::ShortState));
+    }
+};
+constexpr uint32_t kShortSide = 128;
+bool is_short(uint32_t rows, uint32_t cols) { return rows <= kShortSide || cols <= kShortSide; }
+size_t workspace_bytes_of(uint32_t count, uint32_t rows, uint32_t cols) {
+    return is_short(rows, cols) ? ShortWorkspace(count, rows, cols).total : Workspace(count, rows, cols).total;
+}
+
 struct FinalArgs {
     dev::Batch dst;
     uint32_t step;
     float keep, rate;
 };
 
+template <int MP>
+int newton_schulz_short(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, dev::ShortArgs a) {
+    const uint32_t m = a.src.rows < a.src.cols ? a.src.rows : a.src.cols;
+    const dim3 slabs(a.parts, count), block(256);
+    hipLaunchKernelGGL((dev::short_first_kernel<MP>), slabs, block, 0, st, a);
+    MG_HIP(hipGetLastError(), "newton-schulz first launch");
+    double reach = 1.0;
+    a.start = 1;
+    for (uint32_t left = ns.steps; left; a.start = 0) {
+        a.steps = segment_steps(ns, m, left);
+        double most = step_bounds(ns, &reach);
+        if (a.steps == 2) most *= step_bounds(ns, &reach);
+        a.unit_q = a.steps == 1 ? kUnitP : unit_of(most);
+        left -= a.steps;
+        hipLaunchKernelGGL((dev::short_square_kernel<MP>), dim3(count), block, 0, st, a);
+        MG_HIP(hipGetLastError(), "newton-schulz square launch");
+        if (left)
+            hipLaunchKernelGGL((dev::short_update_kernel<MP, false>), slabs, block, 0, st, a);
+        else
+            hipLaunchKernelGGL((dev::short_update_kernel<MP, true>), slabs, block, 0, st, a);
+        MG_HIP(hipGetLastError(), "newton-schulz update launch");
+    }
+    return MG_OK;
+}
+
 int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, const dev::SourceArgs& src,
                   const FinalArgs& fin, void* workspace) {
+    if (is_short(src.rows, src.cols)) {
+        const ShortWorkspace w(count, src.rows, src.cols);
+        char* const base = static_cast<char*>(workspace);
+        dev::ShortArgs a{};
+        a.src = src, a.slabs = w.slabs, a.parts = w.parts;
+        a.xt = reinterpret_cast<dev::f16*>(base + w.xt);
+        a.partial = reinterpret_cast<float*>(base + w.partial);
+        a.q = reinterpret_cast<dev::f16*>(base + w.q);
+        a.state = reinterpret_cast<dev::ShortState*>(base + w.state);
+        a.eps = ns.eps, a.a = ns.a, a.b = ns.b, a.c = ns.c;
+        a.dst = fin.dst, a.step = fin.step, a.keep = fin.keep, a.rate = fin.rate;
+        return w.mp == 32   ? newton_schulz_short<32>(st, ns, count, a)
+               : w.mp == 64 ? newton_schulz_short<64>(st, ns, count, a)
+                            : newton_schulz_short<128>(st, ns, count, a);
+    }
     const Workspace w(count, src.rows, src.cols);
     char* const base = static_cast<char*>(workspace);
     auto planes = [&](size_t at, uint32_t rows, uint32_t ld) {
@@ -512,8 +525,7 @@ int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, co
                 (rc = symmetric(last, prod, w.mp, kUnitP, kUnitA, gram, kUnitA)) || (rc = polynomial(poly)))
                 return rc;
             most_q *= step_bounds(ns, &reach);
-            // the largest power of two that keeps the product under 2^15
-            const float unit = ldexpf(1.0f, 15 - ilogb(most_q > 1.0 ? most_q : 1.0) - 1);
+            const float unit = unit_of(most_q);
             if ((rc = symmetric(poly, Q[q], w.mp, kUnitP, unit_q, Q[q ^ 1], unit))) return rc;
             unit_q = unit, q ^= 1;
         }
@@ -536,7 +548,7 @@ int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, co
 
 int check_workspace(const char* what, uint32_t count, uint32_t rows, uint32_t cols, const void* workspace,
                     uint64_t bytes) {
-    const uint64_t need = Workspace(count, rows, cols).total;
+    const uint64_t need = workspace_bytes_of(count, rows, cols);
     MG_CHECK(workspace && bytes >= need, MG_ERR_INVALID, "%s: the workspace needs %llu bytes", what,
              (unsigned long long)need);
     MG_CHECK(aligned(workspace, 256), MG_ERR_INVALID, "%s: the workspace is not 256-byte aligned", what);
@@ -557,7 +569,7 @@ int mg_orthogonalize_workspace(const mg_newton_schulz* in, uint32_t count, uint3
     mg_newton_schulz ns;
     int rc;
     if ((rc = check_ns(what, in, &ns)) || (rc = check_shape(what, count, rows, cols))) return rc;
-    *bytes = count ? Workspace(count, rows, cols).total : 0;
+    *bytes = count ? workspace_bytes_of(count, rows, cols) : 0;
     return MG_OK;
 }
 

@@ -1,0 +1,84 @@
+// What both Newton-Schulz paths (muon.hip, muon_short.h) share: batches of matrices
+// of any type, the matrix that is orthogonalised, and the operands' pairs.
+#pragma once
+#include <math.h>
+
+#include <type_traits>
+
+#include "kernels.h"
+#include "mg/device/common.h"
+#include "operator_types.h"
+
+namespace mg {
+namespace dev {
+
+typedef _Float16 f16;
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// Exponents of the operands' pairs: X and A at most 2 and 4 in size, P at most
+// 64, so that 2^13 and 2^9 keep them under 2^15, half of binary16's range.
+constexpr float kUnitX = 8192.0f, kUnitA = 8192.0f, kUnitP = 512.0f;
+
+// x = hi + lo to 22 bits. x is made one value first: where it is a product or a
+// multiply-add, the compiler otherwise rounds that to binary16 in one step for hi
+// (v_fma_mixlo_f16) and to fp32 for lo, and where the two roundings fall on
+// different sides of a tie, hi and lo are off by a step of hi.
+__device__ __forceinline__ void split(float x, f16& hi, f16& lo) {
+    asm("" : "+v"(x));
+    hi = (f16)x;
+    lo = (f16)(x - (float)hi);
+}
+__device__ __forceinline__ void split4(const float (&x)[4], float f, f16x4& hi, f16x4& lo) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        f16 h, l;
+        split(x[e] * f, h, l);
+        hi[e] = h, lo[e] = l;
+    }
+}
+
+// A batch of matrices of any type as a kernel reads or writes it.
+struct Batch {
+    void* data;
+    size_t ld, stride;
+    uint32_t type;
+};
+__device__ __forceinline__ float batch_load(const Batch& b, size_t at) {
+    if (b.type == MG_TYPE_FP32) return static_cast<const float*>(b.data)[at];
+    if (b.type == MG_TYPE_BF16) return (float)static_cast<const __bf16*>(b.data)[at];
+    return (float)static_cast<const f16*>(b.data)[at];
+}
+__device__ __forceinline__ void batch_store(const Batch& b, size_t at, float x) {
+    if (b.type == MG_TYPE_FP32)
+        static_cast<float*>(b.data)[at] = x;
+    else if (b.type == MG_TYPE_BF16)
+        static_cast<__bf16*>(b.data)[at] = (__bf16)x;
+    else
+        static_cast<f16*>(b.data)[at] = (f16)x;
+}
+
+// What is orthogonalised: `in`, or with a momentum batch the Muon update's U from
+// the gradient `in`.
+struct SourceArgs {
+    Batch in, momentum;  // momentum.data NULL: in alone
+    uint32_t rows, cols;
+    float beta;
+    uint32_t nesterov;
+};
+// U(i, j) of matrix k; UPDATE also moves the momentum to this gradient.
+template <bool UPDATE>
+__device__ __forceinline__ float source_value(const SourceArgs& a, uint32_t k, uint32_t i, uint32_t j) {
+    const float g = batch_load(a.in, k * a.in.stride + i * a.in.ld + j);
+    if (!a.momentum.data) return g;
+    float* const mp = static_cast<float*>(a.momentum.data) + k * a.momentum.stride + i * a.momentum.ld + j;
+    float m = *mp;
+    if constexpr (UPDATE) {
+        m = m + (1.0f - a.beta) * (g - m);
+        *mp = m;
+    }
+    return a.nesterov ? g + a.beta * (m - g) : m;
+}
+
+}  // namespace dev
+}  // namespace mg
