@@ -431,7 +431,8 @@ struct FinalArgs {
 template <int MP>
 int newton_schulz_short(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, dev::ShortArgs a) {
     const uint32_t m = a.src.rows < a.src.cols ? a.src.rows : a.src.cols;
-    const dim3 slabs(a.parts, count), block(256);
+    using Shape = dev::ShortShape<MP>;
+    const dim3 slabs(a.parts, count), block(Shape::THREADS);
     hipLaunchKernelGGL((dev::short_first_kernel<MP>), slabs, block, 0, st, a);
     MG_HIP(hipGetLastError(), "newton-schulz first launch");
     double reach = 1.0;
@@ -442,7 +443,7 @@ int newton_schulz_short(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
         if (a.steps == 2) most *= step_bounds(ns, &reach);
         a.unit_q = a.steps == 1 ? kUnitP : unit_of(most);
         left -= a.steps;
-        hipLaunchKernelGGL((dev::short_square_kernel<MP>), dim3(count), block, 0, st, a);
+        hipLaunchKernelGGL((dev::short_square_kernel<MP>), dim3(count), dim3(64 * Shape::TILES), 0, st, a);
         MG_HIP(hipGetLastError(), "newton-schulz square launch");
         if (left)
             hipLaunchKernelGGL((dev::short_update_kernel<MP, false>), slabs, block, 0, st, a);

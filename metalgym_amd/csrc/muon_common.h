@@ -30,12 +30,15 @@ __device__ __forceinline__ void split(float x, f16& hi, f16& lo) {
     lo = (f16)(x - (float)hi);
 }
 __device__ __forceinline__ void split4(const float (&x)[4], float f, f16x4& hi, f16x4& lo) {
+    f32x4 v;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        f16 h, l;
-        split(x[e] * f, h, l);
-        hi[e] = h, lo[e] = l;
+        float y = x[e] * f;
+        asm("" : "+v"(y));
+        v[e] = y;
     }
+    hi = __builtin_convertvector(v, f16x4);
+    lo = __builtin_convertvector(v - __builtin_convertvector(hi, f32x4), f16x4);
 }
 
 // A batch of matrices of any type as a kernel reads or writes it.
@@ -66,6 +69,12 @@ struct SourceArgs {
     float beta;
     uint32_t nesterov;
 };
+__device__ __forceinline__ float moved_momentum(const SourceArgs& a, float m, float g) {
+    return m + (1.0f - a.beta) * (g - m);
+}
+__device__ __forceinline__ float update_of(const SourceArgs& a, float m, float g) {
+    return a.nesterov ? g + a.beta * (m - g) : m;
+}
 // U(i, j) of matrix k; UPDATE also moves the momentum to this gradient.
 template <bool UPDATE>
 __device__ __forceinline__ float source_value(const SourceArgs& a, uint32_t k, uint32_t i, uint32_t j) {
@@ -73,11 +82,8 @@ __device__ __forceinline__ float source_value(const SourceArgs& a, uint32_t k, u
     if (!a.momentum.data) return g;
     float* const mp = static_cast<float*>(a.momentum.data) + k * a.momentum.stride + i * a.momentum.ld + j;
     float m = *mp;
-    if constexpr (UPDATE) {
-        m = m + (1.0f - a.beta) * (g - m);
-        *mp = m;
-    }
-    return a.nesterov ? g + a.beta * (m - g) : m;
+    if constexpr (UPDATE) *mp = m = moved_momentum(a, m, g);
+    return update_of(a, m, g);
 }
 
 }  // namespace dev

@@ -11,9 +11,10 @@
 //          segment's steps to Q in LDS.
 //  update: X <- Q X slab by slab, and the slabs' part of the new X X', or at the
 //          end the result.
-// With m = 128 and n = 512 a segment of two steps is five m x m products (2 us
-// each on one CU, of which 1.3 us matrix instructions) between launches of a few
-// microseconds.
+// Each kernel runs its code once or a few times, so what it costs is latencies: loads
+// are issued in batches, one wave holds one 32 x 32 tile, and code is kept in loops
+// (unrolled four waves' worth of tiles each, the same kernels spent 13 to 25 us
+// fetching 20 to 50 KB of instructions).
 #pragma once
 #include "muon_common.h"
 
@@ -24,24 +25,26 @@ constexpr int kSlab = 128;      // columns of a slab
 constexpr int kShortParts = 16;  // most workgroups that share a matrix's slabs
 constexpr int kMostExp = 120;    // exponent of a slab of zeros, or of next to nothing
 
-// A matrix of MP x C pairs in LDS: two planes of rows of 2 C bytes, cut into
-// 16-byte chunks; chunk c of row r sits at c ^ turn(r), so that 32 rows' reads of
-// one chunk, and a fragment's, fall on all banks.
-template <int R, int C>
-struct PairTile {
-    static constexpr int kRow = 2 * C, kPlane = R * kRow, kBytes = 2 * kPlane;
-    static __device__ __forceinline__ int turn(int r) { return (r / (128 / C)) & (C / 8 - 1); }
-    // eight elements from column 8 chunk
-    static __device__ __forceinline__ f16x8 chunk(const char* t, int plane, int r, int c) {
-        return *reinterpret_cast<const f16x8*>(t + plane * kPlane + r * kRow + ((c ^ turn(r)) << 4));
+// Pairs in the order of the matrix instructions' operands, in LDS and in memory: a
+// matrix of K columns (the contraction) is cut into 32 rows x 16 columns, each two
+// planes of 64 lanes x 8 elements: lane 32 h + r holds row r and columns 8 h ... A
+// fragment is then 1 KB in a row, and a wave's stores of results (four columns of
+// eight rows at a time) run along 128 bytes.
+template <int K>
+struct Frags {
+    static constexpr int kBlock = K / 16 * 2 * 512;  // elements of 32 rows
+    // columns c ... of row r: c a multiple of 4
+    static __device__ __forceinline__ int at(int plane, int r, int c) {
+        return (r >> 5) * kBlock + ((c >> 4) * 2 + plane) * 512 + ((c & 8) << 5) + ((r & 31) << 3) + (c & 4);
     }
-    // four elements from column c, a multiple of 4
-    static __device__ __forceinline__ char* quad(char* t, int plane, int r, int c) {
-        return t + plane * kPlane + r * kRow + (((c >> 3) ^ turn(r)) << 4) + ((c & 4) << 1);
+    // the fragment of rows 32 b ... and columns 16 k ... for this lane
+    static __device__ __forceinline__ f16x8 frag(const f16* m, int plane, int b, int k) {
+        return *reinterpret_cast<const f16x8*>(m + b * kBlock + (k * 2 + plane) * 512 + (threadIdx.x & 63) * 8);
     }
-    static __device__ __forceinline__ void put(char* t, int r, int c, f16x4 hi, f16x4 lo) {
-        *reinterpret_cast<f16x4*>(quad(t, 0, r, c)) = hi;
-        *reinterpret_cast<f16x4*>(quad(t, 1, r, c)) = lo;
+    static __device__ __forceinline__ void put(f16* m, int r, int c, f16x4 hi, f16x4 lo) {
+        f16* const to = m + at(0, r, c);
+        *reinterpret_cast<f16x4*>(to) = hi;
+        *reinterpret_cast<f16x4*>(to + 512) = lo;
     }
 };
 
@@ -79,9 +82,9 @@ struct ShortState {
 struct ShortArgs {
     SourceArgs src;
     uint32_t slabs, parts;
-    f16* xt;        // [count][2][slabs 128][MP] X transposed, planes hi and lo
+    f16* xt;        // [count][slabs] X transposed: 128 columns of X by MP, Frags<MP>
     float* partial;  // [count][parts][tiles][16][64] X X' on and under the diagonal, in register order
-    f16* q;         // [count][2][MP][MP]
+    f16* q;         // [count] MP x MP, Frags<MP>
     ShortState* state;  // [count]
     float eps;
     // square
@@ -102,105 +105,142 @@ __device__ __forceinline__ void short_tile(int t, int& bi, int& bj) {
 }
 template <int MP>
 struct ShortShape {
-    static constexpr int NB = MP / 32, TILES = NB * (NB + 1) / 2, PER = (TILES + 3) / 4;  // tiles a wave, four waves
-    using Sq = PairTile<MP, MP>;
-    using Rows = PairTile<MP, kSlab>;  // a slab of X
+    static constexpr int NB = MP / 32, TILES = NB * (NB + 1) / 2;  // of 32 x 32, on and under the diagonal
+    static constexpr int W = 4 * NB < 8 ? 4 * NB : 8;  // waves over a slab's four column blocks
+    static constexpr int NT = 64 * W;
+    static constexpr int THREADS = 64 * (W > TILES ? W : TILES);  // first and update: a wave a tile of X X'
+    static constexpr int SQ = 2 * MP * MP, SLAB = 2 * MP * kSlab;  // elements of a pair of planes
 };
 
-// Adds the slab's part of X X' (rows in LDS as pairs) to each wave's tiles, in
-// chains of 32 contraction elements.
-template <int MP>
-__device__ __forceinline__ void short_gram(const char* rows, f32x16 (&gram)[ShortShape<MP>::PER]) {
-    using S = ShortShape<MP>;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
+// 32 x 32 of x y' over K contraction elements, rows 32 bi of x and 32 bj of y, in
+// chains of 32.
+template <int K>
+__device__ __forceinline__ f32x16 short_product(const f16* x, const f16* y, int bi, int bj) {
+    f32x16 v = {};
+#pragma unroll 2
+    for (int kk = 0; kk < K / 16; kk += 2) {
+        f32x16 s = {};
 #pragma unroll
-    for (int u = 0; u < S::PER; ++u) {
-        const int t = wave + 4 * u;
-        if (t >= S::TILES) break;
-        int bi, bj;
-        short_tile(t, bi, bj);
+        for (int e = 0; e < 2; ++e) {
+            f16x8 a[2], b[2];
 #pragma unroll
-        for (int kk = 0; kk < kSlab / 16; kk += 2) {
-            f32x16 s = {};
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                f16x8 a[2], b[2];
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    a[p] = S::Rows::chunk(rows, p, 32 * bi + r, 2 * (kk + e) + h);
-                    b[p] = S::Rows::chunk(rows, p, 32 * bj + r, 2 * (kk + e) + h);
-                }
-                s = pair_mfma(a, b, s);
+            for (int p = 0; p < 2; ++p) {
+                a[p] = Frags<K>::frag(x, p, bi, kk + e);
+                b[p] = Frags<K>::frag(y, p, bj, kk + e);
             }
-            gram[u] += s;
+            s = pair_mfma(a, b, s);
         }
+        v += s;
     }
+    return v;
 }
+
+// The slab's part of X X' (rows in LDS as pairs), a wave a tile, into this
+// workgroup's partial sums; added to those of its slabs before unless `first`.
 template <int MP>
-__device__ __forceinline__ void short_gram_store(const ShortArgs& a, uint32_t mat,
-                                                 const f32x16 (&gram)[ShortShape<MP>::PER]) {
+__device__ __forceinline__ void short_gram(const ShortArgs& a, uint32_t mat, const f16* rows, bool first) {
     using S = ShortShape<MP>;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    float* out = a.partial + ((size_t)mat * a.parts + blockIdx.x) * S::TILES * 1024;
+    const int lane = threadIdx.x & 63, t = threadIdx.x >> 6;
+    if (t >= S::TILES) return;
+    int bi, bj;
+    short_tile(t, bi, bj);
+    f32x16 v = short_product<kSlab>(rows, rows, bi, bj);
+    float* out = a.partial + (((size_t)mat * a.parts + blockIdx.x) * S::TILES + t) * 1024 + lane;
+    if (!first) {
+        f32x16 old;
 #pragma unroll
-    for (int u = 0; u < S::PER; ++u) {
-        const int t = wave + 4 * u;
-        if (t >= S::TILES) break;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) out[(size_t)t * 1024 + r * 64 + lane] = gram[u][r];
+        for (int r = 0; r < 16; ++r) old[r] = out[r * 64];
+        v += old;
     }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) out[r * 64] = v[r];
 }
 
 __device__ __forceinline__ float magnitude(float x) {
     return fabsf(x) < __builtin_huge_valf() ? fabsf(x) : __builtin_huge_valf();
 }
 
+// Slab s of U into the stage [MP][kSlab + 1] as X(i, j), zeros in the padding;
+// returns the thread's largest magnitude, infinite where one is not finite. UPDATE
+// also moves the momentum. A thread's loads are issued together, from clamped
+// places: one at a time, each would cost a memory latency.
+template <int MP, bool UPDATE, class T>
+__device__ __forceinline__ float short_fill(const SourceArgs& a, uint32_t mat, uint32_t s, float* stage) {
+    constexpr int NT = ShortShape<MP>::NT, LD = kSlab + 1;
+    constexpr int PER = MP * kSlab / NT, N = PER < 16 ? PER : 16;  // elements a thread, and in flight
+    const bool tall = a.rows > a.cols;
+    const int t = threadIdx.x;
+    if (t >= NT) return 0.0f;
+    // element e of the thread is X(i0 + e di, j0 + e dj): threads run along the source's rows
+    const int i0 = tall ? t % MP : t / kSlab, j0 = tall ? t / MP : t % kSlab;
+    const int di = tall ? 0 : NT / kSlab, dj = tall ? NT / MP : 0;
+    const uint32_t m = tall ? a.cols : a.rows, n = tall ? a.rows : a.cols;
+    const T* const in = static_cast<const T*>(a.in.data) + mat * a.in.stride;
+    float* const mom = static_cast<float*>(a.momentum.data) + mat * a.momentum.stride;
+    float most = 0.0f;
+#pragma unroll 1
+    for (int base = 0; base < PER; base += N) {
+        float g[N], b[N];
+        bool on[N];
+        size_t at[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const uint32_t i = i0 + (base + e) * di, j = s * kSlab + j0 + (base + e) * dj;
+            on[e] = i < m && j < n;
+            const uint32_t ic = i < m ? i : m - 1, jc = j < n ? j : n - 1;
+            const uint32_t y = tall ? jc : ic, x = tall ? ic : jc;
+            g[e] = (float)in[y * a.in.ld + x];
+            at[e] = y * a.momentum.ld + x;
+        }
+        if (a.momentum.data) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) b[e] = mom[at[e]];
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                if constexpr (UPDATE) {
+                    b[e] = moved_momentum(a, b[e], g[e]);
+                    if (on[e]) mom[at[e]] = b[e];
+                }
+                g[e] = update_of(a, b[e], g[e]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float u = on[e] ? g[e] : 0.0f;
+            stage[(i0 + (base + e) * di) * LD + j0 + (base + e) * dj] = u;
+            most = fmaxf(most, magnitude(u));
+        }
+    }
+    return most;
+}
+
 // Grid (parts, count). A slab goes through LDS as fp32 (rows i of X, padded), from
 // there as pairs to the Gram product's rows and, transposed, to xt.
 template <int MP>
-__global__ void __launch_bounds__(256) short_first_kernel(const ShortArgs a) {
+__global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_first_kernel(const ShortArgs a) {
     using S = ShortShape<MP>;
-    constexpr int LD = kSlab + 1;
-    __shared__ __align__(16) char rows[S::Rows::kBytes];
+    constexpr int LD = kSlab + 1, W = S::THREADS / 64;
+    __shared__ __align__(16) f16 rows[S::SLAB];
     __shared__ float stage[MP * LD];
-    __shared__ float wmax[4];
+    __shared__ float wmax[W];
     const uint32_t mat = blockIdx.y;
     const int t = threadIdx.x;
-    const uint32_t n_rows = a.src.rows, n_cols = a.src.cols;
-    const bool tall = n_rows > n_cols;
-    // slab s into the stage, as X(i, j); returns the thread's largest magnitude,
-    // infinite where one is not finite
+    // slab s into the stage; returns the thread's largest magnitude
     auto fill = [&](uint32_t s, auto update) {
-        float most = 0.0f;
-        const uint32_t j0 = s * kSlab;
-        if (tall) {  // source rows are X's columns
-            constexpr int RP = 256 / MP;
-            const int i = t % MP;
-#pragma unroll 8
-            for (int j = t / MP; j < kSlab; j += RP) {
-                const bool in = j0 + j < n_rows && (uint32_t)i < n_cols;
-                const float u = in ? source_value<decltype(update)::value>(a.src, mat, j0 + j, i) : 0.0f;
-                stage[i * LD + j] = u;
-                most = fmaxf(most, magnitude(u));
-            }
-        } else {
-            const int j = t & (kSlab - 1);
-#pragma unroll 8
-            for (int i = t / kSlab; i < MP; i += 256 / kSlab) {
-                const bool in = j0 + j < n_cols && (uint32_t)i < n_rows;
-                const float u = in ? source_value<decltype(update)::value>(a.src, mat, i, j0 + j) : 0.0f;
-                stage[i * LD + j] = u;
-                most = fmaxf(most, magnitude(u));
-            }
+        constexpr bool U = decltype(update)::value;
+        switch (a.src.in.type) {
+            case MG_TYPE_FP32: return short_fill<MP, U, float>(a.src, mat, s, stage);
+            case MG_TYPE_BF16: return short_fill<MP, U, __bf16>(a.src, mat, s, stage);
+            default: return short_fill<MP, U, f16>(a.src, mat, s, stage);
         }
-        return most;
     };
     float most = 0.0f;
     for (uint32_t s = blockIdx.x; s < a.slabs; s += a.parts) most = fmaxf(most, fill(s, std::true_type{}));
     most = group_max<64>(most);
     if ((t & 63) == 0) wmax[t >> 6] = most;
     __syncthreads();
-    most = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+    most = wmax[0];
+    for (int w = 1; w < W; ++w) most = fmaxf(most, wmax[w]);
     // 2^12 <= most 2^exp < 2^13; without a finite size the products carry the NaN
     int e = 0;
     if (most < __builtin_huge_valf()) {
@@ -209,7 +249,6 @@ __global__ void __launch_bounds__(256) short_first_kernel(const ShortArgs a) {
     }
     const float unit = ldexpf(1.0f, e);
     if (t == 0) a.state[mat].exp[blockIdx.x] = e;
-    f32x16 gram[S::PER] = {};
     const bool one = a.slabs <= a.parts;  // the stage still holds the only slab
     for (uint32_t s = blockIdx.x; s < a.slabs; s += a.parts) {
         if (!one) {
@@ -217,254 +256,208 @@ __global__ void __launch_bounds__(256) short_first_kernel(const ShortArgs a) {
             fill(s, std::false_type{});
         }
         __syncthreads();
-        for (int q = t; q < MP * (kSlab / 4); q += 256) {
+#pragma unroll 2
+        for (int q = t; q < MP * (kSlab / 4); q += S::THREADS) {
             const int i = q / (kSlab / 4), j = 4 * (q % (kSlab / 4));
+            const float x[4] = {stage[i * LD + j], stage[i * LD + j + 1], stage[i * LD + j + 2], stage[i * LD + j + 3]};
             f16x4 hi, lo;
-            for (int k = 0; k < 4; ++k) {
-                f16 h, l;
-                split(stage[i * LD + j + k] * unit, h, l);
-                hi[k] = h, lo[k] = l;
-            }
-            S::Rows::put(rows, i, j, hi, lo);
+            split4(x, unit, hi, lo);
+            Frags<kSlab>::put(rows, i, j, hi, lo);
         }
-        f16* xt = a.xt + (size_t)mat * 2 * a.slabs * kSlab * MP + (size_t)s * kSlab * MP;
-        const size_t plane = (size_t)a.slabs * kSlab * MP;
-        for (int q = t; q < kSlab * (MP / 8); q += 256) {
-            const int j = q / (MP / 8), i = 8 * (q % (MP / 8));
+        f16* xt = a.xt + ((size_t)mat * a.slabs + s) * S::SLAB;
+#pragma unroll 1
+        for (int q = t; q < kSlab * (MP / 8); q += S::THREADS) {
+            // a wave writes the fragment of 32 columns j and 16 rows i
+            const int j = 32 * (q / (4 * MP)) + (q & 31), i = 8 * (q / 32 % (MP / 8));
             f16x8 hi, lo;
-            for (int k = 0; k < 8; ++k) {
-                f16 h, l;
-                split(stage[(i + k) * LD + j] * unit, h, l);
-                hi[k] = h, lo[k] = l;
+#pragma unroll
+            for (int k = 0; k < 8; k += 4) {
+                const float x[4] = {stage[(i + k) * LD + j], stage[(i + k + 1) * LD + j], stage[(i + k + 2) * LD + j],
+                                    stage[(i + k + 3) * LD + j]};
+                f16x4 h4, l4;
+                split4(x, unit, h4, l4);
+#pragma unroll
+                for (int e4 = 0; e4 < 4; ++e4) hi[k + e4] = h4[e4], lo[k + e4] = l4[e4];
             }
-            *reinterpret_cast<f16x8*>(xt + (size_t)j * MP + i) = hi;
-            *reinterpret_cast<f16x8*>(xt + plane + (size_t)j * MP + i) = lo;
+            f16* const to = xt + Frags<MP>::at(0, j, i);
+            *reinterpret_cast<f16x8*>(to) = hi;
+            *reinterpret_cast<f16x8*>(to + 512) = lo;
         }
         __syncthreads();
-        short_gram<MP>(rows, gram);
+        short_gram<MP>(a, mat, rows, s == blockIdx.x);
     }
-    short_gram_store<MP>(a, mat, gram);
 }
 
-// out = x y of two symmetric matrices in LDS, the wave's tiles in registers: wave
-// w holds the tiles (bi, bj) with bi in {w / 2 NB / 2 ..}, 2 x 2 of them at MP = 128
-// and one at 64; at 32 the first wave holds the only one.
+// One workgroup a matrix, a wave a tile on or under the diagonal: A from the partial
+// products, then the segment's steps. Two matrices in LDS are enough for two steps:
+// A and P, then B = P A over A, A' = P B over B, P' over A', and Q = P' P. All are
+// symmetric: what a tile holds goes to both places.
 template <int MP>
-struct ShortProduct {
-    using Sq = PairTile<MP, MP>;
-    static constexpr int W = MP == 128 ? 2 : 1;  // tile rows and columns of a wave
-    f32x16 v[W][W];
-    int bi, bj;
-    bool on;
-    __device__ __forceinline__ ShortProduct() {
-        const int wave = threadIdx.x >> 6;
-        bi = MP == 32 ? 0 : (wave >> 1) * W, bj = MP == 32 ? 0 : (wave & 1) * W;
-        on = MP > 32 || wave == 0;
-    }
-    __device__ __forceinline__ void run(const char* x, const char* y) {
-        if (!on) return;
-        const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
-#pragma unroll
-        for (int i = 0; i < W; ++i)
-#pragma unroll
-            for (int j = 0; j < W; ++j) v[i][j] = f32x16{};
-#pragma unroll
-        for (int kk = 0; kk < MP / 16; kk += 2) {
-            f32x16 s[W][W] = {};
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                f16x8 fa[W][2], fb[W][2];
-#pragma unroll
-                for (int i = 0; i < W; ++i)
-#pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        fa[i][p] = Sq::chunk(x, p, 32 * (bi + i) + r, 2 * (kk + e) + h);
-                        fb[i][p] = Sq::chunk(y, p, 32 * (bj + i) + r, 2 * (kk + e) + h);
-                    }
-#pragma unroll
-                for (int i = 0; i < W; ++i)
-#pragma unroll
-                    for (int j = 0; j < W; ++j) s[i][j] = pair_mfma(fa[i], fb[j], s[i][j]);
-            }
-#pragma unroll
-            for (int i = 0; i < W; ++i)
-#pragma unroll
-                for (int j = 0; j < W; ++j) v[i][j] += s[i][j];
-        }
-    }
-    // f(value x 4, row i of the first, column j): four rows i .. i + 3 of one column
-    template <class F>
-    __device__ __forceinline__ void each(F&& f) const {
-        if (!on) return;
-        const int lane = threadIdx.x & 63;
-#pragma unroll
-        for (int x = 0; x < W; ++x)
-#pragma unroll
-            for (int y = 0; y < W; ++y)
-#pragma unroll
-                for (int r = 0; r < 16; r += 4) {
-                    const float q[4] = {v[x][y][r], v[x][y][r + 1], v[x][y][r + 2], v[x][y][r + 3]};
-                    f(q, 32 * (bi + x) + 2 * r + 4 * (lane >> 5), 32 * (bj + y) + (lane & 31));
-                }
-    }
-    // The result times f as pairs into `out` after every wave has read what it overwrites.
-    __device__ __forceinline__ void put(char* out, float f) const {
-        __syncthreads();
-        each([&](const float (&q)[4], int i, int j) {
-            f16x4 hi, lo;
-            split4(q, f, hi, lo);
-            Sq::put(out, j, i, hi, lo);
-        });
-        __syncthreads();
-    }
-};
-
-// One workgroup a matrix: A from the partial products, then the segment's steps. Two
-// matrices in LDS are enough for two steps: A and P, then B = P A over A, A' = P B
-// over B, P' over A', and Q = P' P.
-template <int MP>
-__global__ void __launch_bounds__(256) short_square_kernel(const ShortArgs a) {
+__global__ void __launch_bounds__(64 * ShortShape<MP>::TILES) short_square_kernel(const ShortArgs a) {
     using S = ShortShape<MP>;
-    using Sq = typename S::Sq;
-    __shared__ __align__(16) char gram[Sq::kBytes], poly[Sq::kBytes];
-    __shared__ float wtrace[4];
+    using F = Frags<MP>;
+    __shared__ __align__(16) f16 lds[2][S::SQ];
+    __shared__ float wtrace[S::TILES];
     const uint32_t mat = blockIdx.x;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     ShortState& state = a.state[mat];
-    int least = kMostExp;
+    int least = kMostExp, bi, bj;
+    short_tile(wave, bi, bj);
+    const int i0 = 32 * bi + 4 * (lane >> 5), j0 = 32 * bj + (lane & 31);
     if (a.start)
         for (uint32_t p = 0; p < a.parts; ++p) least = state.exp[p] < least ? state.exp[p] : least;
-    f32x16 sum[S::PER] = {};
-    const float* in = a.partial + (size_t)mat * a.parts * S::TILES * 1024 + lane;
-    for (uint32_t p = 0; p < a.parts; ++p, in += S::TILES * 1024) {
-        const float f = a.start ? ldexpf(1.0f, 2 * (least - state.exp[p])) : 1.0f;
+    f32x16 v = {};
+    const float* in = a.partial + ((size_t)mat * a.parts * S::TILES + wave) * 1024 + lane;
+#pragma unroll 1
+    for (uint32_t p0 = 0; p0 < a.parts; p0 += 4) {  // four parts in flight
+        float x[4][16];
 #pragma unroll
-        for (int u = 0; u < S::PER; ++u) {
-            const int t = wave + 4 * u;
-            if (t >= S::TILES) break;
+        for (uint32_t p = 0; p < 4; ++p) {
+            const float* from = in + (size_t)(p0 + p < a.parts ? p0 + p : p0) * S::TILES * 1024;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sum[u][r] += f * in[(size_t)t * 1024 + r * 64];
+            for (int r = 0; r < 16; ++r) x[p][r] = from[r * 64];
+        }
+#pragma unroll
+        for (uint32_t p = 0; p < 4; ++p) {
+            const float f = p0 + p >= a.parts ? 0.0f
+                            : a.start         ? ldexpf(1.0f, 2 * (least - state.exp[p0 + p]))
+                                              : 1.0f;
+            if (f != 0.0f)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) v[r] += f * x[p][r];
         }
     }
-    float to_unit = kUnitA / (kUnitX * kUnitX);
+    float to_out = kUnitA / (kUnitX * kUnitX);
     if (a.start) {
         float trace = 0.0f;
 #pragma unroll
-        for (int u = 0; u < S::PER; ++u) {
-            int bi, bj;
-            short_tile(wave + 4 * u, bi, bj);
-            if (wave + 4 * u >= S::TILES || bi != bj) continue;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) trace += c32_row(r, lane) == (lane & 31) ? sum[u][r] : 0.0f;
-        }
+        for (int r = 0; r < 16; ++r) trace += bi == bj && c32_row(r, lane) == (lane & 31) ? v[r] : 0.0f;
         trace = group_sum<64>(trace);
         if (lane == 0) wtrace[wave] = trace;
         __syncthreads();
-        trace = wtrace[0] + wtrace[1] + wtrace[2] + wtrace[3];
+        trace = 0.0f;
+        for (int w = 0; w < S::TILES; ++w) trace += wtrace[w];
         const float scale = 1.0f / (sqrtf(trace) + a.eps * ldexpf(1.0f, least));
         if (threadIdx.x == 0) state.least = least, state.scale = scale;
-        to_unit = scale * scale * kUnitA;
+        to_out = scale * scale * kUnitA;
     }
-#pragma unroll
-    for (int u = 0; u < S::PER; ++u) {
-        const int t = wave + 4 * u;
-        if (t >= S::TILES) break;
-        int bi, bj;
-        short_tile(t, bi, bj);
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const float q[4] = {sum[u][r], sum[u][r + 1], sum[u][r + 2], sum[u][r + 3]};
-            const int i = 32 * bi + 2 * r + 4 * (lane >> 5), j = 32 * bj + (lane & 31);
-            f16x4 hi, lo;
-            split4(q, to_unit, hi, lo);
-            Sq::put(gram, j, i, hi, lo);
-            if (bi != bj) Sq::put(gram, i + (lane & 3), j & ~3, quad_transpose(hi), quad_transpose(lo));
-        }
-    }
-    __syncthreads();
-    ShortProduct<MP> prod;
-    // a I + b A + c (A A) in registers, times kUnitP
-    auto polynomial = [&](const char* A) {
-        prod.run(A, A);
-        const float cc = a.c * (kUnitP / (kUnitA * kUnitA)), cb = a.b * (kUnitP / kUnitA), ca = a.a * kUnitP;
-        if (!prod.on) return;
-#pragma unroll
-        for (int x = 0; x < prod.W; ++x)
-#pragma unroll
-            for (int y = 0; y < prod.W; ++y)
+    f16* const q = a.q + (size_t)mat * S::SQ;
+    // op -1 stores A; then the products of a segment, each of two of the matrices in
+    // LDS, over one of them or to Q
+    const int last = a.steps == 2 ? 4 : 0;
+#pragma unroll 1
+    for (int op = -1; op <= last; ++op) {
+        f16* const out = op == last ? q : lds[op == 0];
+        if (op >= 0) {
+            const f16* x = lds[op == 1 || op == 2];
+            const f16* y = lds[op == 4];
+            v = short_product<MP>(x, y, bi, bj);
+            to_out = op == 1 || op == 2 ? 1.0f / kUnitP : 1.0f;
+            if (op == last) to_out = a.unit_q / (op == 4 ? kUnitP * kUnitP : kUnitP);
+            if (op == 0 || op == 3) {  // a I + b A + c (A A), at kUnitP
+                const float cc = a.c * (kUnitP / (kUnitA * kUnitA)), cb = a.b * (kUnitP / kUnitA);
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
-                    const int i = 32 * (prod.bi + x) + 2 * r + 4 * (lane >> 5), j = 32 * (prod.bj + y) + (lane & 31);
-                    const f16x4 hi = *reinterpret_cast<const f16x4*>(Sq::quad(const_cast<char*>(A), 0, j, i));
-                    const f16x4 lo = *reinterpret_cast<const f16x4*>(Sq::quad(const_cast<char*>(A), 1, j, i));
+                    const int i = i0 + 2 * r;
+                    const f16* from = lds[0] + F::at(0, j0, i);
+                    const f16x4 hi = *reinterpret_cast<const f16x4*>(from);
+                    const f16x4 lo = *reinterpret_cast<const f16x4*>(from + 512);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        prod.v[x][y][r + e] = cc * prod.v[x][y][r + e] + cb * ((float)hi[e] + (float)lo[e]) +
-                                              (i + e == j ? ca : 0.0f);
+                        v[r + e] = cc * v[r + e] + cb * ((float)hi[e] + (float)lo[e]) +
+                                   (i + e == j0 ? a.a * kUnitP : 0.0f);
                 }
-    };
-    float to_q = a.unit_q / kUnitP;
-    polynomial(gram);
-    if (a.steps == 2) {
-        prod.put(poly, 1.0f);
-        prod.run(poly, gram);
-        prod.put(gram, 1.0f / kUnitP);
-        prod.run(poly, gram);
-        prod.put(gram, 1.0f / kUnitP);
-        polynomial(gram);
-        prod.put(gram, 1.0f);
-        prod.run(gram, poly);
-        to_q = a.unit_q / (kUnitP * kUnitP);
+            }
+            __syncthreads();  // every wave has read what this goes over
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const float w[4] = {v[r], v[r + 1], v[r + 2], v[r + 3]};
+            const int i = i0 + 2 * r;
+            f16x4 hi, lo;
+            split4(w, to_out, hi, lo);
+            F::put(out, j0, i, hi, lo);
+            if (bi != bj) F::put(out, i + (lane & 3), j0 & ~3, quad_transpose(hi), quad_transpose(lo));
+        }
+        __syncthreads();
     }
-    f16* q = a.q + (size_t)mat * 2 * MP * MP;
-    prod.each([&](const float (&w)[4], int i, int j) {
-        f16x4 hi, lo;
-        split4(w, to_q, hi, lo);
-        *reinterpret_cast<f16x4*>(q + j * MP + i) = hi;
-        *reinterpret_cast<f16x4*>(q + MP * MP + j * MP + i) = lo;
-    });
 }
 
-// Grid (parts, count). X' X = Q X as X' rows: a wave holds 32 columns of X, its
-// fragments straight from xt, Q in LDS. FINAL writes the result; otherwise the new
-// pairs replace the old in xt (each workgroup's own slabs) and go to LDS in rows
-// for the Gram product.
+// The slab's part of the result, from the stage ([j][i] of tall matrices, else
+// [i][j]) to dst: the result itself or the optimiser's step.
+template <int MP, class T>
+__device__ __forceinline__ void short_write(const ShortArgs& a, uint32_t mat, uint32_t s, const float* stage) {
+    constexpr int NT = ShortShape<MP>::NT, LD = kSlab + 1, LDT = MP + 1;
+    constexpr int PER = MP * kSlab / NT, N = PER < 8 ? PER : 8;
+    const bool tall = a.src.rows > a.src.cols;
+    const int t = threadIdx.x;
+    if (t >= NT) return;
+    const uint32_t y0 = tall ? s * kSlab + t / MP : t / kSlab, x = tall ? t % MP : s * kSlab + t % kSlab;
+    const uint32_t dy = tall ? NT / MP : NT / kSlab;
+    const float* from = tall ? stage + t / MP * LDT + t % MP : stage + t / kSlab * LD + t % kSlab;
+    const uint32_t step = tall ? dy * LDT : dy * LD;
+    T* const out = static_cast<T*>(a.dst.data) + mat * a.dst.stride;
+    if (x >= a.src.cols) return;
+#pragma unroll 1
+    for (int base = 0; base < PER; base += N) {
+        float w[N];
+        if (a.step) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const uint32_t y = y0 + (base + e) * dy, yc = y < a.src.rows ? y : a.src.rows - 1;
+                w[e] = (float)out[yc * a.dst.ld + x];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const uint32_t y = y0 + (base + e) * dy;
+            const float o = from[(base + e) * step];
+            if (y < a.src.rows) out[y * a.dst.ld + x] = (T)(a.step ? a.keep * w[e] - a.rate * o : o);
+        }
+    }
+}
+
+// Grid (parts, count). X' X = Q X as X' rows, 32 columns of X a wave (or two waves
+// that share the rows of Q), its fragments straight from xt, Q in LDS. FINAL writes
+// the result; otherwise the new pairs replace the old in xt (each workgroup's own
+// slabs) and go to LDS in rows for the Gram product.
 template <int MP, bool FINAL>
-__global__ void __launch_bounds__(256) short_update_kernel(const ShortArgs a) {
+__global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_update_kernel(const ShortArgs a) {
     using S = ShortShape<MP>;
-    using Sq = typename S::Sq;
     constexpr int LD = kSlab + 1, LDT = MP + 1;
-    constexpr int kStage = FINAL ? (MP * LD > kSlab * LDT ? MP * LD : kSlab * LDT) * 4 : S::Rows::kBytes;
-    __shared__ __align__(16) char q[Sq::kBytes];
+    constexpr int kStage = FINAL ? (MP * LD > kSlab * LDT ? MP * LD : kSlab * LDT) * 4 : S::SLAB * 2;
+    __shared__ __align__(16) f16 q[S::SQ];
     __shared__ __align__(16) char stage[kStage];
     const uint32_t mat = blockIdx.y;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 31, h = lane >> 5;
-    const f16* qin = a.q + (size_t)mat * 2 * MP * MP;
-    for (int c = t; c < 2 * MP * (MP / 8); c += 256) {
-        const int p = c / (MP * (MP / 8)), row = c / (MP / 8) % MP, ch = c % (MP / 8);
-        *reinterpret_cast<f16x8*>(q + p * Sq::kPlane + row * Sq::kRow + ((ch ^ Sq::turn(row)) << 4)) =
-            *reinterpret_cast<const f16x8*>(qin + (size_t)c * 8);
+    const int jb = wave & 3;  // the wave's 32 columns of the slab
+    const f16* qin = a.q + (size_t)mat * S::SQ;
+    if (t < S::NT) {
+        constexpr int PER = S::SQ / 8 / S::NT;  // all in flight at once
+        f16x8 part[PER];
+#pragma unroll
+        for (int k = 0; k < PER; ++k) part[k] = *reinterpret_cast<const f16x8*>(qin + (t + S::NT * k) * 8);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) *reinterpret_cast<f16x8*>(q + (t + S::NT * k) * 8) = part[k];
     }
     // takes the exponents out of X Q, and puts X's own in
     const ShortState& state = a.state[mat];
     float f = 1.0f / (a.unit_q * kUnitX);
     if (a.start) f = state.scale * ldexpf(1.0f, state.least - state.exp[blockIdx.x]) / a.unit_q;
     if (!FINAL) f *= kUnitX;
-    const size_t plane = (size_t)a.slabs * kSlab * MP;
-    const uint32_t n_rows = a.src.rows, n_cols = a.src.cols;
-    const bool tall = n_rows > n_cols;
-    f32x16 gram[FINAL ? 1 : S::PER] = {};
+    const bool tall = a.src.rows > a.src.cols;
     for (uint32_t s = blockIdx.x; s < a.slabs; s += a.parts) {
-        f16* const xt = a.xt + (size_t)mat * 2 * plane + ((size_t)s * kSlab + 32 * wave) * MP;
+        f16* const xt = a.xt + ((size_t)mat * a.slabs + s) * S::SLAB;
         f16x8 x[MP / 16][2];
+        if (wave < S::W)
 #pragma unroll
-        for (int kk = 0; kk < MP / 16; ++kk)
+            for (int kk = 0; kk < MP / 16; ++kk)
 #pragma unroll
-            for (int p = 0; p < 2; ++p)
-                x[kk][p] = *reinterpret_cast<const f16x8*>(xt + p * plane + (size_t)r * MP + 16 * kk + 8 * h);
-        __syncthreads();  // Q is in place, and the slab before has left the stage
-#pragma unroll
-        for (int b = 0; b < S::NB; ++b) {
+                for (int p = 0; p < 2; ++p)
+                    x[kk][p] = Frags<MP>::frag(xt, p, jb, kk);
+        __syncthreads();  // Q is in place, the slab before has left the stage, and both waves of a column block hold X
+#pragma unroll 1
+        for (int b = wave / 4; wave < S::W && b < S::NB; b += S::W / 4) {
             f32x16 acc = {};
 #pragma unroll
             for (int kk = 0; kk < MP / 16; kk += 2) {
@@ -473,58 +466,41 @@ __global__ void __launch_bounds__(256) short_update_kernel(const ShortArgs a) {
                 for (int e = 0; e < 2; ++e) {
                     f16x8 y[2];
 #pragma unroll
-                    for (int p = 0; p < 2; ++p) y[p] = Sq::chunk(q, p, 32 * b + r, 2 * (kk + e) + h);
+                    for (int p = 0; p < 2; ++p) y[p] = Frags<MP>::frag(q, p, b, kk + e);
                     c = pair_mfma(x[kk + e], y, c);
                 }
                 acc += c;
             }
             // X'(i, j .. j + 3) with i = 32 b + r
+            const int i = 32 * b + r;
 #pragma unroll
             for (int g = 0; g < 16; g += 4) {
                 const float w[4] = {acc[g], acc[g + 1], acc[g + 2], acc[g + 3]};
-                const int i = 32 * b + r, j = 2 * g + 4 * h;
+                const int j = 32 * jb + 2 * g + 4 * h;
                 if constexpr (FINAL) {
                     float* o = reinterpret_cast<float*>(stage);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (tall)
-                            o[(32 * wave + j + e) * LDT + i] = w[e] * f;
-                        else
-                            o[i * LD + 32 * wave + j + e] = w[e] * f;
-                    }
+                    for (int e = 0; e < 4; ++e) o[tall ? (j + e) * LDT + i : i * LD + j + e] = w[e] * f;
                 } else {
                     f16x4 hi, lo;
                     split4(w, f, hi, lo);
-                    S::Rows::put(stage, i, 32 * wave + j, hi, lo);
-                    f16* at = xt + (size_t)(j + (lane & 3)) * MP + (i & ~3);
-                    *reinterpret_cast<f16x4*>(at) = quad_transpose(hi);
-                    *reinterpret_cast<f16x4*>(at + plane) = quad_transpose(lo);
+                    Frags<kSlab>::put(reinterpret_cast<f16*>(stage), i, j, hi, lo);
+                    Frags<MP>::put(xt, j + (lane & 3), i & ~3, quad_transpose(hi), quad_transpose(lo));
                 }
             }
         }
         __syncthreads();
         if constexpr (FINAL) {
             const float* o = reinterpret_cast<const float*>(stage);
-            const uint32_t j0 = s * kSlab;
-            auto write = [&](uint32_t y, uint32_t c, float value) {
-                const size_t at = mat * a.dst.stride + y * a.dst.ld + c;
-                batch_store(a.dst, at, a.step ? a.keep * batch_load(a.dst, at) - a.rate * value : value);
-            };
-            if (tall) {
-#pragma unroll 4
-                for (int j = t / MP; j < kSlab; j += 256 / MP)
-                    if (j0 + j < n_rows && (uint32_t)(t % MP) < n_cols) write(j0 + j, t % MP, o[j * LDT + t % MP]);
-            } else {
-                const int j = t & (kSlab - 1);
-#pragma unroll 4
-                for (int i = t / kSlab; i < MP; i += 256 / kSlab)
-                    if ((uint32_t)i < n_rows && j0 + j < n_cols) write(i, j0 + j, o[i * LD + j]);
+            switch (a.dst.type) {
+                case MG_TYPE_FP32: short_write<MP, float>(a, mat, s, o); break;
+                case MG_TYPE_BF16: short_write<MP, __bf16>(a, mat, s, o); break;
+                default: short_write<MP, f16>(a, mat, s, o);
             }
         } else {
-            short_gram<MP>(stage, gram);
+            short_gram<MP>(a, mat, reinterpret_cast<const f16*>(stage), s == blockIdx.x);
         }
     }
-    if constexpr (!FINAL) short_gram_store<MP>(a, mat, gram);
 }
 
 }  // namespace dev
