@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(256) product_kernel(const ProductArgs p) {
                     for (int e = 0; e < 4; ++e) {
                         const uint32_t y = tall ? j : i + e, x = tall ? i + e : j;
                         if (y >= p.rows || x >= p.cols) continue;
-                        const size_t at = mat * p.dst.stride + y * p.dst.ld + x;
+                        const size_t at = p.dst.at(mat, y, x);
                         const float o = v[e] * p.unit;
                         batch_store(p.dst, at, p.step ? p.keep * batch_load(p.dst, at) - p.rate * o : o);
                     }
@@ -363,12 +363,12 @@ int check_batch(const char* what, const char* name, const mg_matrices* in, dev::
     MG_CHECK(in->data || !in->count, MG_ERR_INVALID, "%s: %s has no data", what, name);
     MG_CHECK(aligned(in->data, type_bytes(in->type)), MG_ERR_INVALID, "%s: %s is not aligned to its type", what, name);
     const uint64_t ld = in->ld ? in->ld : in->cols;
-    MG_CHECK(ld >= in->cols && ld <= (1ull << 32), MG_ERR_INVALID, "%s: %s: ld %llu must be at least cols", what, name,
+    MG_CHECK(ld >= in->cols && ld < (1ull << 31), MG_ERR_INVALID, "%s: %s: ld %llu must be in [cols, 2^31)", what, name,
              (unsigned long long)ld);
     const uint64_t stride = in->stride ? in->stride : in->rows * ld;
     MG_CHECK(in->count <= 1 || (stride >= (in->rows - 1) * ld + in->cols && stride <= (1ull << 44)), MG_ERR_INVALID,
              "%s: %s: stride %llu: the matrices overlap", what, name, (unsigned long long)stride);
-    *out = dev::Batch{in->data, (size_t)ld, (size_t)stride, in->type};
+    *out = dev::Batch{in->data, (size_t)stride, (uint32_t)ld, in->type};
     return MG_OK;
 }
 
@@ -443,12 +443,12 @@ int newton_schulz_short(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
         if (a.steps == 2) most *= step_bounds(ns, &reach);
         a.unit_q = a.steps == 1 ? kUnitP : unit_of(most);
         left -= a.steps;
-        hipLaunchKernelGGL((dev::short_square_kernel<MP>), dim3(count), dim3(64 * Shape::TILES), 0, st, a);
+        hipLaunchKernelGGL((dev::short_square_kernel<MP>), dim3(count), dim3(64 * Shape::NB * Shape::NB), 0, st, a);
         MG_HIP(hipGetLastError(), "newton-schulz square launch");
         if (left)
             hipLaunchKernelGGL((dev::short_update_kernel<MP, false>), slabs, block, 0, st, a);
         else
-            hipLaunchKernelGGL((dev::short_update_kernel<MP, true>), slabs, block, 0, st, a);
+            hipLaunchKernelGGL((dev::short_update_kernel<MP, true>), slabs, dim3(Shape::NT), 0, st, a);
         MG_HIP(hipGetLastError(), "newton-schulz update launch");
     }
     return MG_OK;

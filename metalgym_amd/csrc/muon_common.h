@@ -44,8 +44,12 @@ __device__ __forceinline__ void split4(const float (&x)[4], float f, f16x4& hi, 
 // A batch of matrices of any type as a kernel reads or writes it.
 struct Batch {
     void* data;
-    size_t ld, stride;
+    size_t stride;
+    uint32_t ld;
     uint32_t type;
+    __device__ __forceinline__ size_t at(uint32_t k, uint32_t i, uint32_t j) const {
+        return k * stride + (uint64_t)i * ld + j;
+    }
 };
 __device__ __forceinline__ float batch_load(const Batch& b, size_t at) {
     if (b.type == MG_TYPE_FP32) return static_cast<const float*>(b.data)[at];
@@ -78,9 +82,9 @@ __device__ __forceinline__ float update_of(const SourceArgs& a, float m, float g
 // U(i, j) of matrix k; UPDATE also moves the momentum to this gradient.
 template <bool UPDATE>
 __device__ __forceinline__ float source_value(const SourceArgs& a, uint32_t k, uint32_t i, uint32_t j) {
-    const float g = batch_load(a.in, k * a.in.stride + i * a.in.ld + j);
+    const float g = batch_load(a.in, a.in.at(k, i, j));
     if (!a.momentum.data) return g;
-    float* const mp = static_cast<float*>(a.momentum.data) + k * a.momentum.stride + i * a.momentum.ld + j;
+    float* const mp = static_cast<float*>(a.momentum.data) + a.momentum.at(k, i, j);
     float m = *mp;
     if constexpr (UPDATE) *mp = m = moved_momentum(a, m, g);
     return update_of(a, m, g);

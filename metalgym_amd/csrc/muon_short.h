@@ -66,9 +66,12 @@ __device__ __forceinline__ f16x4 quad_transpose(f16x4 v) {
     return __builtin_bit_cast(f16x4, out);
 }
 
+// c + a b of pairs, a's low halves first; SWAP: b's, which gives the bits of the
+// product with a and b in each other's place.
+template <bool SWAP = false>
 __device__ __forceinline__ f32x16 pair_mfma(const f16x8 (&a)[2], const f16x8 (&b)[2], f32x16 c) {
-    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], b[0], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[!SWAP], b[SWAP], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[SWAP], b[!SWAP], c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[0], c, 0, 0, 0);
 }
 
@@ -107,7 +110,7 @@ template <int MP>
 struct ShortShape {
     static constexpr int NB = MP / 32, TILES = NB * (NB + 1) / 2;  // of 32 x 32, on and under the diagonal
     static constexpr int W = 4 * NB < 8 ? 4 * NB : 8;  // waves over a slab's four column blocks
-    static constexpr int NT = 64 * W;
+    static constexpr int NT = 64 * W, PER = MP * kSlab / NT;  // elements of a slab a thread
     static constexpr int THREADS = 64 * (W > TILES ? W : TILES);  // first and update: a wave a tile of X X'
     static constexpr int SQ = 2 * MP * MP, SLAB = 2 * MP * kSlab;  // elements of a pair of planes
 };
@@ -160,82 +163,87 @@ __device__ __forceinline__ float magnitude(float x) {
     return fabsf(x) < __builtin_huge_valf() ? fabsf(x) : __builtin_huge_valf();
 }
 
-// Slab s of U into the stage [MP][kSlab + 1] as X(i, j), zeros in the padding;
-// returns the thread's largest magnitude, infinite where one is not finite. UPDATE
-// also moves the momentum. A thread's loads are issued together, from clamped
-// places: one at a time, each would cost a memory latency.
-template <int MP, bool UPDATE, class T>
-__device__ __forceinline__ float short_fill(const SourceArgs& a, uint32_t mat, uint32_t s, float* stage) {
-    constexpr int NT = ShortShape<MP>::NT, LD = kSlab + 1;
-    constexpr int PER = MP * kSlab / NT, N = PER < 16 ? PER : 16;  // elements a thread, and in flight
-    const bool tall = a.rows > a.cols;
-    const int t = threadIdx.x;
-    if (t >= NT) return 0.0f;
-    // element e of the thread is X(i0 + e di, j0 + e dj): threads run along the source's rows
-    const int i0 = tall ? t % MP : t / kSlab, j0 = tall ? t / MP : t % kSlab;
-    const int di = tall ? 0 : NT / kSlab, dj = tall ? NT / MP : 0;
-    const uint32_t m = tall ? a.cols : a.rows, n = tall ? a.rows : a.cols;
-    const T* const in = static_cast<const T*>(a.in.data) + mat * a.in.stride;
-    float* const mom = static_cast<float*>(a.momentum.data) + mat * a.momentum.stride;
-    float most = 0.0f;
-#pragma unroll 1
-    for (int base = 0; base < PER; base += N) {
-        float g[N], b[N];
-        bool on[N];
-        size_t at[N];
+// A thread's part of a slab of the source: PER consecutive elements across the
+// source's rows at one place along them, so that threads run along the rows. Of
+// tall matrices those are X(i, j .. ), of others X(i .. , j).
+template <int MP>
+struct ShortPart {
+    using S = ShortShape<MP>;
+    int i, j;
+    float u[S::PER];
+    __device__ __forceinline__ explicit ShortPart(bool tall) {
+        const int t = threadIdx.x;
+        i = tall ? t % MP : t / kSlab * S::PER, j = tall ? t / MP * S::PER : t % kSlab;
+    }
+    // U with zeros in the padding; UPDATE also moves the momentum. The loads are
+    // issued together, from clamped places: one at a time, each would cost a latency.
+    template <bool UPDATE, class T>
+    __device__ __forceinline__ void load(const SourceArgs& a, uint32_t mat, uint32_t s) {
+        const bool tall = a.rows > a.cols;
+        const uint32_t y0 = tall ? s * kSlab + j : i, x = tall ? i : s * kSlab + j;
+        const uint32_t xc = x < a.cols ? x : a.cols - 1;
+        const uint32_t yc = y0 < a.rows ? y0 : a.rows - 1;
+        const T* in = static_cast<const T*>(a.in.data) + a.in.at(mat, yc, xc);
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const uint32_t i = i0 + (base + e) * di, j = s * kSlab + j0 + (base + e) * dj;
-            on[e] = i < m && j < n;
-            const uint32_t ic = i < m ? i : m - 1, jc = j < n ? j : n - 1;
-            const uint32_t y = tall ? jc : ic, x = tall ? ic : jc;
-            g[e] = (float)in[y * a.in.ld + x];
-            at[e] = y * a.momentum.ld + x;
+        for (int e = 0; e < S::PER; ++e) {
+            u[e] = (float)*in;
+            in += y0 + e + 1 < a.rows ? a.in.ld : 0u;
         }
         if (a.momentum.data) {
+            float* const mom = static_cast<float*>(a.momentum.data) + a.momentum.at(mat, yc, xc);
+            const float* from = mom;
+            float b[S::PER];
 #pragma unroll
-            for (int e = 0; e < N; ++e) b[e] = mom[at[e]];
+            for (int e = 0; e < S::PER; ++e) {
+                b[e] = *from;
+                from += y0 + e + 1 < a.rows ? a.momentum.ld : 0u;
+            }
+            float* to = mom;
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
+            for (int e = 0; e < S::PER; ++e) {
                 if constexpr (UPDATE) {
-                    b[e] = moved_momentum(a, b[e], g[e]);
-                    if (on[e]) mom[at[e]] = b[e];
+                    b[e] = moved_momentum(a, b[e], u[e]);
+                    if (x < a.cols && y0 + e < a.rows) *to = b[e];
+                    to += a.momentum.ld;
                 }
-                g[e] = update_of(a, b[e], g[e]);
+                u[e] = update_of(a, b[e], u[e]);
             }
         }
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const float u = on[e] ? g[e] : 0.0f;
-            stage[(i0 + (base + e) * di) * LD + j0 + (base + e) * dj] = u;
-            most = fmaxf(most, magnitude(u));
+        for (int e = 0; e < S::PER; ++e) u[e] = x < a.cols && y0 + e < a.rows ? u[e] : 0.0f;
+    }
+    template <bool UPDATE>
+    __device__ __forceinline__ void load(const SourceArgs& a, uint32_t mat, uint32_t s) {
+        if (threadIdx.x >= S::NT) return;  // whole waves
+        switch (a.in.type) {
+            case MG_TYPE_FP32: return load<UPDATE, float>(a, mat, s);
+            case MG_TYPE_BF16: return load<UPDATE, __bf16>(a, mat, s);
+            default: return load<UPDATE, f16>(a, mat, s);
         }
     }
-    return most;
-}
+};
 
-// Grid (parts, count). A slab goes through LDS as fp32 (rows i of X, padded), from
-// there as pairs to the Gram product's rows and, transposed, to xt.
+// Grid (parts, count). The slabs as pairs, to xt and in rows to LDS for the Gram
+// product: one of the two takes a thread's four elements as they are, the other
+// those of four threads.
 template <int MP>
 __global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_first_kernel(const ShortArgs a) {
     using S = ShortShape<MP>;
-    constexpr int LD = kSlab + 1, W = S::THREADS / 64;
+    constexpr int W = S::THREADS / 64;
     __shared__ __align__(16) f16 rows[S::SLAB];
-    __shared__ float stage[MP * LD];
     __shared__ float wmax[W];
     const uint32_t mat = blockIdx.y;
     const int t = threadIdx.x;
-    // slab s into the stage; returns the thread's largest magnitude
-    auto fill = [&](uint32_t s, auto update) {
-        constexpr bool U = decltype(update)::value;
-        switch (a.src.in.type) {
-            case MG_TYPE_FP32: return short_fill<MP, U, float>(a.src, mat, s, stage);
-            case MG_TYPE_BF16: return short_fill<MP, U, __bf16>(a.src, mat, s, stage);
-            default: return short_fill<MP, U, f16>(a.src, mat, s, stage);
-        }
-    };
+    const bool tall = a.src.rows > a.src.cols;
+    ShortPart<MP> part(tall);
     float most = 0.0f;
-    for (uint32_t s = blockIdx.x; s < a.slabs; s += a.parts) most = fmaxf(most, fill(s, std::true_type{}));
+#pragma unroll 1
+    for (uint32_t s = blockIdx.x; s < a.slabs; s += a.parts) {
+        part.template load<true>(a.src, mat, s);
+        if (t < S::NT)
+#pragma unroll
+            for (int e = 0; e < S::PER; ++e) most = fmaxf(most, magnitude(part.u[e]));
+    }
     most = group_max<64>(most);
     if ((t & 63) == 0) wmax[t >> 6] = most;
     __syncthreads();
@@ -249,67 +257,59 @@ __global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_first_kernel(co
     }
     const float unit = ldexpf(1.0f, e);
     if (t == 0) a.state[mat].exp[blockIdx.x] = e;
-    const bool one = a.slabs <= a.parts;  // the stage still holds the only slab
-    for (uint32_t s = blockIdx.x; s < a.slabs; s += a.parts) {
-        if (!one) {
-            __syncthreads();
-            fill(s, std::false_type{});
-        }
-        __syncthreads();
-#pragma unroll 2
-        for (int q = t; q < MP * (kSlab / 4); q += S::THREADS) {
-            const int i = q / (kSlab / 4), j = 4 * (q % (kSlab / 4));
-            const float x[4] = {stage[i * LD + j], stage[i * LD + j + 1], stage[i * LD + j + 2], stage[i * LD + j + 3]};
-            f16x4 hi, lo;
-            split4(x, unit, hi, lo);
-            Frags<kSlab>::put(rows, i, j, hi, lo);
-        }
-        f16* xt = a.xt + ((size_t)mat * a.slabs + s) * S::SLAB;
 #pragma unroll 1
-        for (int q = t; q < kSlab * (MP / 8); q += S::THREADS) {
-            // a wave writes the fragment of 32 columns j and 16 rows i
-            const int j = 32 * (q / (4 * MP)) + (q & 31), i = 8 * (q / 32 % (MP / 8));
-            f16x8 hi, lo;
-#pragma unroll
-            for (int k = 0; k < 8; k += 4) {
-                const float x[4] = {stage[(i + k) * LD + j], stage[(i + k + 1) * LD + j], stage[(i + k + 2) * LD + j],
-                                    stage[(i + k + 3) * LD + j]};
-                f16x4 h4, l4;
-                split4(x, unit, h4, l4);
-#pragma unroll
-                for (int e4 = 0; e4 < 4; ++e4) hi[k + e4] = h4[e4], lo[k + e4] = l4[e4];
-            }
-            f16* const to = xt + Frags<MP>::at(0, j, i);
-            *reinterpret_cast<f16x8*>(to) = hi;
-            *reinterpret_cast<f16x8*>(to + 512) = lo;
+    for (uint32_t s = blockIdx.x; s < a.slabs; s += a.parts) {
+        if (a.slabs > a.parts) {  // else the only slab is still held
+            part.template load<false>(a.src, mat, s);
+            __syncthreads();
         }
+        f16* const xt = a.xt + ((size_t)mat * a.slabs + s) * S::SLAB;
+        if (t < S::NT)
+#pragma unroll
+            for (int k = 0; k < S::PER; k += 4) {
+                const float x[4] = {part.u[k], part.u[k + 1], part.u[k + 2], part.u[k + 3]};
+                f16x4 hi, lo;
+                split4(x, unit, hi, lo);
+                const f16x4 hi_t = quad_transpose(hi), lo_t = quad_transpose(lo);
+                if (tall) {
+                    Frags<kSlab>::put(rows, part.i, part.j + k, hi, lo);
+                    Frags<MP>::put(xt, part.j + k + (t & 3), part.i & ~3, hi_t, lo_t);
+                } else {
+                    Frags<MP>::put(xt, part.j, part.i + k, hi, lo);
+                    Frags<kSlab>::put(rows, part.i + k + (t & 3), part.j & ~3, hi_t, lo_t);
+                }
+            }
         __syncthreads();
         short_gram<MP>(a, mat, rows, s == blockIdx.x);
     }
 }
 
-// One workgroup a matrix, a wave a tile on or under the diagonal: A from the partial
-// products, then the segment's steps. Two matrices in LDS are enough for two steps:
-// A and P, then B = P A over A, A' = P B over B, P' over A', and Q = P' P. All are
-// symmetric: what a tile holds goes to both places.
+// One workgroup a matrix, a wave a tile: A from the partial products (the waves on
+// and under the diagonal), then the segment's steps. Two matrices in LDS are enough
+// for two steps: A and P, then B = P A over A, A' = B P over B, P' over A', and Q =
+// P P'. A wave's four consecutive results lie in one column, and are kept as four of
+// a row, so what is kept is the product's transpose: in this order A' = P A P keeps
+// its symmetry under rounding (with P P A an error of A grows up to threefold).
 template <int MP>
-__global__ void __launch_bounds__(64 * ShortShape<MP>::TILES) short_square_kernel(const ShortArgs a) {
+__global__ void __launch_bounds__(64 * ShortShape<MP>::NB * ShortShape<MP>::NB) short_square_kernel(const ShortArgs a) {
     using S = ShortShape<MP>;
     using F = Frags<MP>;
     __shared__ __align__(16) f16 lds[2][S::SQ];
-    __shared__ float wtrace[S::TILES];
+    __shared__ float wtrace[S::NB * S::NB];
     const uint32_t mat = blockIdx.x;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     ShortState& state = a.state[mat];
-    int least = kMostExp, bi, bj;
-    short_tile(wave, bi, bj);
+    int least = kMostExp;
+    // the lower tiles spread over the SIMDs (wave % 4)
+    const int bi = wave / S::NB, bj = (wave - bi) & (S::NB - 1);
+    const bool lower = bi >= bj;
     const int i0 = 32 * bi + 4 * (lane >> 5), j0 = 32 * bj + (lane & 31);
     if (a.start)
         for (uint32_t p = 0; p < a.parts; ++p) least = state.exp[p] < least ? state.exp[p] : least;
     f32x16 v = {};
-    const float* in = a.partial + ((size_t)mat * a.parts * S::TILES + wave) * 1024 + lane;
+    const float* in = a.partial + ((size_t)mat * a.parts * S::TILES + bi * (bi + 1) / 2 + bj) * 1024 + lane;
 #pragma unroll 1
-    for (uint32_t p0 = 0; p0 < a.parts; p0 += 4) {  // four parts in flight
+    for (uint32_t p0 = 0; p0 < (lower ? a.parts : 0); p0 += 4) {  // four parts in flight
         float x[4][16];
 #pragma unroll
         for (uint32_t p = 0; p < 4; ++p) {
@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(64 * ShortShape<MP>::TILES) short_square_kerne
         if (lane == 0) wtrace[wave] = trace;
         __syncthreads();
         trace = 0.0f;
-        for (int w = 0; w < S::TILES; ++w) trace += wtrace[w];
+        for (int w = 0; w < S::NB * S::NB; ++w) trace += wtrace[w];
         const float scale = 1.0f / (sqrtf(trace) + a.eps * ldexpf(1.0f, least));
         if (threadIdx.x == 0) state.least = least, state.scale = scale;
         to_out = scale * scale * kUnitA;
@@ -349,8 +349,8 @@ __global__ void __launch_bounds__(64 * ShortShape<MP>::TILES) short_square_kerne
     for (int op = -1; op <= last; ++op) {
         f16* const out = op == last ? q : lds[op == 0];
         if (op >= 0) {
-            const f16* x = lds[op == 1 || op == 2];
-            const f16* y = lds[op == 4];
+            const f16* x = lds[op == 2];
+            const f16* y = lds[op == 1 || op == 4];
             v = short_product<MP>(x, y, bi, bj);
             to_out = op == 1 || op == 2 ? 1.0f / kUnitP : 1.0f;
             if (op == last) to_out = a.unit_q / (op == 4 ? kUnitP * kUnitP : kUnitP);
@@ -376,67 +376,73 @@ __global__ void __launch_bounds__(64 * ShortShape<MP>::TILES) short_square_kerne
             const int i = i0 + 2 * r;
             f16x4 hi, lo;
             split4(w, to_out, hi, lo);
-            F::put(out, j0, i, hi, lo);
-            if (bi != bj) F::put(out, i + (lane & 3), j0 & ~3, quad_transpose(hi), quad_transpose(lo));
+            if (op >= 0 || lower) F::put(out, j0, i, hi, lo);
+            if (op < 0 && bi > bj) F::put(out, i + (lane & 3), j0 & ~3, quad_transpose(hi), quad_transpose(lo));
         }
         __syncthreads();
     }
 }
 
-// The slab's part of the result, from the stage ([j][i] of tall matrices, else
-// [i][j]) to dst: the result itself or the optimiser's step.
-template <int MP, class T>
-__device__ __forceinline__ void short_write(const ShortArgs& a, uint32_t mat, uint32_t s, const float* stage) {
-    constexpr int NT = ShortShape<MP>::NT, LD = kSlab + 1, LDT = MP + 1;
-    constexpr int PER = MP * kSlab / NT, N = PER < 8 ? PER : 8;
-    const bool tall = a.src.rows > a.src.cols;
-    const int t = threadIdx.x;
-    if (t >= NT) return;
-    const uint32_t y0 = tall ? s * kSlab + t / MP : t / kSlab, x = tall ? t % MP : s * kSlab + t % kSlab;
-    const uint32_t dy = tall ? NT / MP : NT / kSlab;
-    const float* from = tall ? stage + t / MP * LDT + t % MP : stage + t / kSlab * LD + t % kSlab;
-    const uint32_t step = tall ? dy * LDT : dy * LD;
-    T* const out = static_cast<T*>(a.dst.data) + mat * a.dst.stride;
+// A tile of the result, or of the optimiser's step: register e of a lane lies 8 (e /
+// 4) + e % 4 rows under y0, at column x of dst.
+template <class T>
+__device__ __forceinline__ void short_read(const ShortArgs& a, uint32_t mat, uint32_t y0, uint32_t x, float (&w)[16]) {
+    const T* const from = static_cast<const T*>(a.dst.data) + a.dst.at(mat, 0, x < a.src.cols ? x : 0);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const uint32_t y = y0 + 2 * (e & ~3) + (e & 3);
+        w[e] = (float)from[(uint64_t)(y < a.src.rows ? y : a.src.rows - 1) * a.dst.ld];
+    }
+}
+template <class T>
+__device__ __forceinline__ void short_write(const ShortArgs& a, uint32_t mat, uint32_t y0, uint32_t x, const float (&w)[16]) {
     if (x >= a.src.cols) return;
-#pragma unroll 1
-    for (int base = 0; base < PER; base += N) {
-        float w[N];
-        if (a.step) {
+    T* const to = static_cast<T*>(a.dst.data) + a.dst.at(mat, 0, x);
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const uint32_t y = y0 + (base + e) * dy, yc = y < a.src.rows ? y : a.src.rows - 1;
-                w[e] = (float)out[yc * a.dst.ld + x];
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const uint32_t y = y0 + (base + e) * dy;
-            const float o = from[(base + e) * step];
-            if (y < a.src.rows) out[y * a.dst.ld + x] = (T)(a.step ? a.keep * w[e] - a.rate * o : o);
-        }
+    for (int e = 0; e < 16; ++e) {
+        const uint32_t y = y0 + 2 * (e & ~3) + (e & 3);
+        if (y < a.src.rows) to[(uint64_t)y * a.dst.ld] = (T)w[e];
+    }
+}
+// f(value of the type) with a value of the type's T
+template <class F>
+__device__ __forceinline__ void with_type(uint32_t type, F&& f) {
+    switch (type) {
+        case MG_TYPE_FP32: return f(float{});
+        case MG_TYPE_BF16: return f(__bf16{});
+        default: return f(f16{});
     }
 }
 
-// Grid (parts, count). X' X = Q X as X' rows, 32 columns of X a wave (or two waves
-// that share the rows of Q), its fragments straight from xt, Q in LDS. FINAL writes
-// the result; otherwise the new pairs replace the old in xt (each workgroup's own
-// slabs) and go to LDS in rows for the Gram product.
+// Grid (parts, count): X <- Q X. A wave holds 32 columns of X, its fragments straight
+// from xt (two waves share them and split the rows of Q); Q is in LDS. FINAL writes
+// the result, in the orientation that runs along dst's rows. Otherwise the new pairs
+// replace the old in xt (each workgroup's own slabs) and go to LDS in rows for the
+// Gram product.
 template <int MP, bool FINAL>
-__global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_update_kernel(const ShortArgs a) {
+__global__ void __launch_bounds__(FINAL ? ShortShape<MP>::NT : ShortShape<MP>::THREADS) short_update_kernel(const ShortArgs a) {
     using S = ShortShape<MP>;
-    constexpr int LD = kSlab + 1, LDT = MP + 1;
-    constexpr int kStage = FINAL ? (MP * LD > kSlab * LDT ? MP * LD : kSlab * LDT) * 4 : S::SLAB * 2;
     __shared__ __align__(16) f16 q[S::SQ];
-    __shared__ __align__(16) char stage[kStage];
+    __shared__ __align__(16) f16 rows[FINAL ? 8 : S::SLAB];
     const uint32_t mat = blockIdx.y;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 31, h = lane >> 5;
     const int jb = wave & 3;  // the wave's 32 columns of the slab
-    const f16* qin = a.q + (size_t)mat * S::SQ;
+    f16x8 x[MP / 16][2];
+    auto load_x = [&](uint32_t s) {
+        const f16* xt = a.xt + ((size_t)mat * a.slabs + s) * S::SLAB;
+        if (wave < S::W)
+#pragma unroll
+            for (int kk = 0; kk < MP / 16; ++kk)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) x[kk][p] = Frags<MP>::frag(xt, p, jb, kk);
+    };
     if (t < S::NT) {
         constexpr int PER = S::SQ / 8 / S::NT;  // all in flight at once
+        const f16* qin = a.q + (size_t)mat * S::SQ;
         f16x8 part[PER];
 #pragma unroll
         for (int k = 0; k < PER; ++k) part[k] = *reinterpret_cast<const f16x8*>(qin + (t + S::NT * k) * 8);
+        load_x(blockIdx.x);
 #pragma unroll
         for (int k = 0; k < PER; ++k) *reinterpret_cast<f16x8*>(q + (t + S::NT * k) * 8) = part[k];
     }
@@ -446,18 +452,12 @@ __global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_update_kernel(c
     if (a.start) f = state.scale * ldexpf(1.0f, state.least - state.exp[blockIdx.x]) / a.unit_q;
     if (!FINAL) f *= kUnitX;
     const bool tall = a.src.rows > a.src.cols;
+#pragma unroll 1
     for (uint32_t s = blockIdx.x; s < a.slabs; s += a.parts) {
         f16* const xt = a.xt + ((size_t)mat * a.slabs + s) * S::SLAB;
-        f16x8 x[MP / 16][2];
-        if (wave < S::W)
-#pragma unroll
-            for (int kk = 0; kk < MP / 16; ++kk)
-#pragma unroll
-                for (int p = 0; p < 2; ++p)
-                    x[kk][p] = Frags<MP>::frag(xt, p, jb, kk);
-        __syncthreads();  // Q is in place, the slab before has left the stage, and both waves of a column block hold X
-#pragma unroll 1
-        for (int b = wave / 4; wave < S::W && b < S::NB; b += S::W / 4) {
+        __syncthreads();  // Q is in place, the slab before has left the rows, and both waves of a column block hold X
+        // x y' of 32 x 32 in chains of 32, or its transpose
+        auto product = [&](int b, bool transpose) {
             f32x16 acc = {};
 #pragma unroll
             for (int kk = 0; kk < MP / 16; kk += 2) {
@@ -467,38 +467,46 @@ __global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_update_kernel(c
                     f16x8 y[2];
 #pragma unroll
                     for (int p = 0; p < 2; ++p) y[p] = Frags<MP>::frag(q, p, b, kk + e);
-                    c = pair_mfma(x[kk + e], y, c);
+                    c = transpose ? pair_mfma<true>(y, x[kk + e], c) : pair_mfma(x[kk + e], y, c);
                 }
                 acc += c;
             }
-            // X'(i, j .. j + 3) with i = 32 b + r
-            const int i = 32 * b + r;
+            return acc;
+        };
+#pragma unroll 1
+        for (int b = wave / 4; wave < S::W && b < S::NB; b += S::W / 4) {
+            if constexpr (FINAL) {
+                // tall: a lane holds row i of X, its registers columns j, which are dst's rows
+                const uint32_t along = s * kSlab + 32 * jb, across = 32 * b;
+                const uint32_t y0 = (tall ? along : across) + 4 * h, c = (tall ? across : along) + r;
+                float w[16];
+                if (a.step) with_type(a.dst.type, [&](auto t) { short_read<decltype(t)>(a, mat, y0, c, w); });
+                f32x16 acc;
+                if (tall)
+                    acc = product(b, false);
+                else
+                    acc = product(b, true);
 #pragma unroll
-            for (int g = 0; g < 16; g += 4) {
-                const float w[4] = {acc[g], acc[g + 1], acc[g + 2], acc[g + 3]};
-                const int j = 32 * jb + 2 * g + 4 * h;
-                if constexpr (FINAL) {
-                    float* o = reinterpret_cast<float*>(stage);
+                for (int e = 0; e < 16; ++e) w[e] = a.step ? a.keep * w[e] - a.rate * (acc[e] * f) : acc[e] * f;
+                with_type(a.dst.type, [&](auto t) { short_write<decltype(t)>(a, mat, y0, c, w); });
+            } else {
+                const f32x16 acc = product(b, false);
+                const int i = 32 * b + r;  // X'(i, j .. j + 3)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[tall ? (j + e) * LDT + i : i * LD + j + e] = w[e] * f;
-                } else {
+                for (int g = 0; g < 16; g += 4) {
+                    const float w[4] = {acc[g], acc[g + 1], acc[g + 2], acc[g + 3]};
+                    const int j = 32 * jb + 2 * g + 4 * h;
                     f16x4 hi, lo;
                     split4(w, f, hi, lo);
-                    Frags<kSlab>::put(reinterpret_cast<f16*>(stage), i, j, hi, lo);
+                    Frags<kSlab>::put(rows, i, j, hi, lo);
                     Frags<MP>::put(xt, j + (lane & 3), i & ~3, quad_transpose(hi), quad_transpose(lo));
                 }
             }
         }
-        __syncthreads();
-        if constexpr (FINAL) {
-            const float* o = reinterpret_cast<const float*>(stage);
-            switch (a.dst.type) {
-                case MG_TYPE_FP32: short_write<MP, float>(a, mat, s, o); break;
-                case MG_TYPE_BF16: short_write<MP, __bf16>(a, mat, s, o); break;
-                default: short_write<MP, f16>(a, mat, s, o);
-            }
-        } else {
-            short_gram<MP>(a, mat, reinterpret_cast<const f16*>(stage), s == blockIdx.x);
+        if (s + a.parts < a.slabs) load_x(s + a.parts);
+        if constexpr (!FINAL) {
+            __syncthreads();
+            short_gram<MP>(a, mat, rows, s == blockIdx.x);
         }
     }
 }
