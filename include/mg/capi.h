@@ -518,7 +518,8 @@ int mg_orthogonalize(void* stream, const mg_newton_schulz* ns, const mg_matrices
  * U = nesterov ? G + momentum (M - G) : M; W = (1 - lr weight_decay) W - lr scale O,
  * O the Newton-Schulz result of U. scale 0 stands for sqrt(max(1, cols / rows)):
  * rows are a layer's inputs and cols its outputs, as in the policy's matrices.
- * lr, weight_decay and scale are finite and not negative, momentum in [0, 1). */
+ * lr, weight_decay and scale are finite and not negative, lr weight_decay at most
+ * 1, momentum in [0, 1). */
 typedef struct mg_muon_config {
     float lr;
     float momentum;
@@ -532,6 +533,14 @@ typedef struct mg_muon_config {
  * Sums are fp32, params are rounded once. The workspace is mg_orthogonalize's. */
 int mg_muon_step(void* stream, const mg_muon_config* config, const mg_matrices* params, const mg_matrices* momentum,
                  const mg_matrices* grad, void* workspace, uint64_t workspace_bytes);
+/* The optimiser of a model's block matrices (up and down of every block): Muon
+ * with this configuration, or Adam again (config NULL, and the start). Every train
+ * call follows it, mg_ppo_train_block_noalloc included (the workspace is allocated
+ * here). The gradient is clipped by the global norm first, as for Adam; the vector
+ * parameters and the head stay on Adam at the model's lr. The momentum lies in the
+ * block matrices' part of mg_ppo_adam_state's m. A change of optimiser sets that
+ * part of m and v to 0. Blocking. */
+int mg_ppo_set_muon(mg_ppo* model, const mg_muon_config* config);
 
 /* ---------------------------------------------------------------------------
  * Kernel timing for measurement: when enabled, the library records HIP events

@@ -92,6 +92,17 @@ struct PPOModel {
         mg::check(mg_ppo_train(handle, epochs), "train");
         headFresh_ = paramsFresh_ = false;
     }
+    // The block matrices' optimiser (no reference counterpart): Muon at its own
+    // learning rate, or Adam again. Everything else stays on Adam.
+    void useMuon(float learningRate = 0.02f, float momentum = 0.95f, float weightDecay = 0.0f, bool nesterov = true) {
+        mg_muon_config cfg{};
+        cfg.lr = learningRate;
+        cfg.momentum = momentum;
+        cfg.weight_decay = weightDecay;
+        cfg.nesterov = nesterov ? 1 : 0;
+        mg::check(mg_ppo_set_muon(handle, &cfg), "useMuon");
+    }
+    void useAdam() { mg::check(mg_ppo_set_muon(handle, nullptr), "useAdam"); }
     // model/ppo.h:906-916: the minibatches of slot t, in row order.
     void trainSlot(uint32_t t) {
         pushHParams();

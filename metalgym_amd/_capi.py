@@ -181,6 +181,7 @@ def lib():
         "mg_ppo_policy": (I, [P, P]),
         "mg_ppo_set_params": (I, [P, P, u32]),
         "mg_ppo_params_updated": (I, [P]),
+        "mg_ppo_set_muon": (I, [P, P]),
         "mg_ppo_adam_state": (I, [P, P, P, P]),
         "mg_ppo_train_capture": (I, [P, u32, P, P, P, P]),
         "mg_ppo_set_log_std": (I, [P, f32]),
@@ -544,6 +545,16 @@ class PPOModel:
         m, v, st = C.c_void_p(), C.c_void_p(), u32()
         check(lib().mg_ppo_adam_state(self.h, C.byref(m), C.byref(v), C.byref(st)))
         return d2h(m.value, np.float32, (self.pv.count,)), d2h(v.value, np.float32, (self.pv.count,)), st.value
+
+    def set_muon(self, lr: float = 0.02, momentum: float = 0.95, weight_decay: float = 0.0, scale: float = 0.0,
+                 nesterov: bool = True, ns: NewtonSchulz = None) -> None:
+        """mg_ppo_set_muon: the block matrices take Muon steps."""
+        cfg = MuonConfig(lr, momentum, weight_decay, scale, int(nesterov), ns or NewtonSchulz())
+        check(lib().mg_ppo_set_muon(self.h, C.byref(cfg)))
+
+    def set_adam(self) -> None:
+        """mg_ppo_set_muon(NULL): the block matrices take Adam steps again."""
+        check(lib().mg_ppo_set_muon(self.h, None))
 
     def train_capture(self, which: int) -> np.ndarray:
         """Capture `which` (0 LN outputs, 1 relu'd hidden, 2 dh, 3 dV) of the last

@@ -44,6 +44,8 @@ struct TrainStep {
     uint32_t rows;       // B
     uint32_t mb_index;   // index into the per-minibatch stats output
     float beta1_pow, beta2_pow;
+    const mg_muon_config* muon;  // the block matrices' optimiser, NULL: Adam as for the rest
+    void* muon_ws;               // muon_blocks_bytes
 };
 
 // All fragment-tiled copies of the block matrices (frag_fwd32, frag_fwd16,
@@ -65,5 +67,14 @@ int launch_train_step(hipStream_t st, const mg_policy_view& pv, const mg_ppo_hpa
                       const TrainWs& ws, const TrainStep& step, const float* obs_slots, const void* action_slots,
                       const float* adv_slots, const float* ret_slots, const float* logp_slots,
                       const float* adv_stats, float* m, float* v, float* head_out, float* mb_stats);
+
+// The Muon update of a policy's block matrices (muon.hip): their gradients in the
+// arena `grad`, clipped as Adam clips, the momentum in the arena `momentum`.
+int check_muon_config(const char* what, const mg_muon_config* config);
+size_t muon_blocks_bytes(const mg_policy_view& pv);
+// What one update moves a weight by at most.
+float muon_blocks_reach(const mg_policy_view& pv, const mg_muon_config& config);
+int launch_muon_blocks(hipStream_t st, const mg_policy_view& pv, const mg_muon_config& config, const float* grad,
+                       const float* normpart, float max_grad_norm, float* momentum, void* workspace);
 
 }  // namespace mg

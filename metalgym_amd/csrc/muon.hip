@@ -425,7 +425,7 @@ size_t workspace_bytes_of(uint32_t count, uint32_t rows, uint32_t cols) {
 struct FinalArgs {
     dev::Batch dst;
     uint32_t step;
-    float keep, rate;
+    float keep, rate, odd_rate;
 };
 
 template <int MP>
@@ -466,7 +466,7 @@ int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, co
         a.q = reinterpret_cast<dev::f16*>(base + w.q);
         a.state = reinterpret_cast<dev::ShortState*>(base + w.state);
         a.eps = ns.eps, a.a = ns.a, a.b = ns.b, a.c = ns.c;
-        a.dst = fin.dst, a.step = fin.step, a.keep = fin.keep, a.rate = fin.rate;
+        a.dst = fin.dst, a.step = fin.step, a.keep = fin.keep, a.rate = fin.rate, a.odd_rate = fin.odd_rate;
         return w.mp == 32   ? newton_schulz_short<32>(st, ns, count, a)
                : w.mp == 64 ? newton_schulz_short<64>(st, ns, count, a)
                             : newton_schulz_short<128>(st, ns, count, a);
@@ -547,6 +547,20 @@ int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, co
     return MG_OK;
 }
 
+// The configuration's own checks; *ns receives the iteration.
+int check_muon(const char* what, const mg_muon_config* c, mg_newton_schulz* ns) {
+    MG_CHECK(c, MG_ERR_INVALID, "%s: null argument", what);
+    auto fine = [](float x) { return x >= 0.0f && x < __builtin_huge_valf(); };
+    MG_CHECK(fine(c->lr) && fine(c->weight_decay) && fine(c->scale), MG_ERR_INVALID,
+             "%s: lr, weight_decay and scale must be finite and not negative", what);
+    MG_CHECK(c->lr * c->weight_decay <= 1.0f, MG_ERR_INVALID, "%s: lr * weight_decay must be at most 1", what);
+    MG_CHECK(c->momentum >= 0.0f && c->momentum < 1.0f, MG_ERR_INVALID, "%s: momentum must be in [0, 1)", what);
+    return check_ns(what, c->ns.steps ? &c->ns : nullptr, ns);
+}
+float muon_rate(const mg_muon_config& c, uint32_t rows, uint32_t cols) {
+    return c.lr * (c.scale > 0.0f ? c.scale : cols > rows ? sqrtf((float)cols / (float)rows) : 1.0f);
+}
+
 int check_workspace(const char* what, uint32_t count, uint32_t rows, uint32_t cols, const void* workspace,
                     uint64_t bytes) {
     const uint64_t need = workspace_bytes_of(count, rows, cols);
@@ -557,6 +571,37 @@ int check_workspace(const char* what, uint32_t count, uint32_t rows, uint32_t co
 }
 
 }  // namespace
+
+int check_muon_config(const char* what, const mg_muon_config* config) {
+    mg_newton_schulz ns;
+    return check_muon(what, config, &ns);
+}
+
+size_t muon_blocks_bytes(const mg_policy_view& pv) {
+    return ShortWorkspace(2 * pv.layers, MG_EMBED, pv.hidden).total;
+}
+
+float muon_blocks_reach(const mg_policy_view& pv, const mg_muon_config& c) {
+    // an element of the result is at most its largest singular value; decay only shrinks
+    return (float)kMostSingular * fmaxf(muon_rate(c, MG_EMBED, pv.hidden), muon_rate(c, pv.hidden, MG_EMBED));
+}
+
+int launch_muon_blocks(hipStream_t st, const mg_policy_view& pv, const mg_muon_config& c, const float* grad,
+                       const float* normpart, float max_grad_norm, float* momentum, void* workspace) {
+    mg_newton_schulz ns;
+    if (int rc = check_muon("muon blocks", &c, &ns)) return rc;
+    const uint32_t E = MG_EMBED, H = pv.hidden;
+    auto batch = [&](const float* arena) {
+        return dev::Batch{const_cast<float*>(arena) + pv.float_group, (size_t)E * H, H, MG_TYPE_FP32};
+    };
+    dev::SourceArgs src{};
+    src.in = batch(grad), src.momentum = batch(momentum), src.rows = E, src.cols = H;
+    src.beta = c.momentum, src.nesterov = c.nesterov != 0;
+    src.blocks = 1, src.normpart = normpart, src.max_norm = max_grad_norm;
+    const FinalArgs fin{batch(pv.params), 1, 1.0f - c.lr * c.weight_decay, muon_rate(c, E, H), muon_rate(c, H, E)};
+    return newton_schulz(st, ns, 2 * pv.layers, src, fin, workspace);
+}
+
 }  // namespace mg
 
 using namespace mg;
@@ -596,16 +641,11 @@ int mg_orthogonalize(void* stream, const mg_newton_schulz* in_ns, const mg_matri
 int mg_muon_step(void* stream, const mg_muon_config* c, const mg_matrices* params, const mg_matrices* momentum,
                  const mg_matrices* grad, void* workspace, uint64_t workspace_bytes) {
     const char* what = "muon step";
-    MG_CHECK(c, MG_ERR_INVALID, "muon step: null argument");
-    auto fine = [](float x) { return x >= 0.0f && x < __builtin_huge_valf(); };
-    MG_CHECK(fine(c->lr) && fine(c->weight_decay) && fine(c->scale), MG_ERR_INVALID,
-             "muon step: lr, weight_decay and scale must be finite and not negative");
-    MG_CHECK(c->momentum >= 0.0f && c->momentum < 1.0f, MG_ERR_INVALID, "muon step: momentum must be in [0, 1)");
     mg_newton_schulz ns;
     dev::SourceArgs src{};
     FinalArgs fin{};
     int rc;
-    if ((rc = check_ns(what, c->ns.steps ? &c->ns : nullptr, &ns)) ||
+    if ((rc = check_muon(what, c, &ns)) ||
         (rc = check_batch(what, "params", params, &fin.dst)) ||
         (rc = check_batch(what, "momentum", momentum, &src.momentum)) ||
         (rc = check_batch(what, "grad", grad, &src.in)) || (rc = check_same(what, params, momentum)) ||
@@ -616,12 +656,9 @@ int mg_muon_step(void* stream, const mg_muon_config* c, const mg_matrices* param
     if ((rc = check_workspace(what, params->count, params->rows, params->cols, workspace, workspace_bytes))) return rc;
     src.rows = params->rows, src.cols = params->cols;
     src.beta = c->momentum, src.nesterov = c->nesterov != 0;
-    const float scale = c->scale > 0.0f ? c->scale
-                        : params->cols > params->rows ? sqrtf((float)params->cols / (float)params->rows)
-                                                      : 1.0f;
     fin.step = 1;
     fin.keep = 1.0f - c->lr * c->weight_decay;
-    fin.rate = c->lr * scale;
+    fin.rate = muon_rate(*c, params->rows, params->cols);
     hipStream_t st = static_cast<hipStream_t>(stream);
     StreamDevice on;
     if ((rc = on.enter(st, "muon step: stream device"))) return rc;

@@ -72,7 +72,22 @@ struct SourceArgs {
     uint32_t rows, cols;
     float beta;
     uint32_t nesterov;
+    // a policy's block matrices (short path): contiguous, the odd ones cols x rows, the
+    // gradient clipped to max_norm by the partial squared norms (NULL: not clipped)
+    uint32_t blocks;
+    const float* normpart;
+    float max_norm;
 };
+// model/optimizer.metal:49 from the partial norms, added as Adam adds them; every
+// wave must be whole.
+__device__ __forceinline__ float source_clip(const SourceArgs& a) {
+    if (!a.normpart || !(a.max_norm > 0.0f)) return 1.0f;
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kReduceBlocks / 64; ++k) sum += a.normpart[(threadIdx.x & 63) + 64 * k];
+    const float norm = sqrtf(group_sum<64>(sum));
+    return norm > a.max_norm ? a.max_norm / (norm + 1e-6f) : 1.0f;
+}
 __device__ __forceinline__ float moved_momentum(const SourceArgs& a, float m, float g) {
     return m + (1.0f - a.beta) * (g - m);
 }

@@ -98,7 +98,17 @@ struct ShortArgs {
     // update
     Batch dst;
     uint32_t step;
-    float keep, rate;
+    float keep, rate, odd_rate;  // odd_rate: of the odd matrices of a policy's blocks
+    // The arguments as they are for matrix k.
+    __device__ __forceinline__ ShortArgs of(uint32_t k) const {
+        ShortArgs a = *this;
+        if (src.blocks && (k & 1)) {
+            a.src.rows = src.cols, a.src.cols = src.rows;
+            a.src.in.ld = a.src.momentum.ld = a.dst.ld = a.src.cols;
+            a.rate = odd_rate;
+        }
+        return a;
+    }
 };
 
 // Tile t of the lower triangle in rows: (0,0) (1,0) (1,1) (2,0) ...
@@ -178,7 +188,7 @@ struct ShortPart {
     // U with zeros in the padding; UPDATE also moves the momentum. The loads are
     // issued together, from clamped places: one at a time, each would cost a latency.
     template <bool UPDATE, class T>
-    __device__ __forceinline__ void load(const SourceArgs& a, uint32_t mat, uint32_t s) {
+    __device__ __forceinline__ void load(const SourceArgs& a, uint32_t mat, uint32_t s, float clip) {
         const bool tall = a.rows > a.cols;
         const uint32_t y0 = tall ? s * kSlab + j : i, x = tall ? i : s * kSlab + j;
         const uint32_t xc = x < a.cols ? x : a.cols - 1;
@@ -186,7 +196,7 @@ struct ShortPart {
         const T* in = static_cast<const T*>(a.in.data) + a.in.at(mat, yc, xc);
 #pragma unroll
         for (int e = 0; e < S::PER; ++e) {
-            u[e] = (float)*in;
+            u[e] = (float)*in * clip;
             in += y0 + e + 1 < a.rows ? a.in.ld : 0u;
         }
         if (a.momentum.data) {
@@ -213,12 +223,12 @@ struct ShortPart {
         for (int e = 0; e < S::PER; ++e) u[e] = x < a.cols && y0 + e < a.rows ? u[e] : 0.0f;
     }
     template <bool UPDATE>
-    __device__ __forceinline__ void load(const SourceArgs& a, uint32_t mat, uint32_t s) {
+    __device__ __forceinline__ void load(const SourceArgs& a, uint32_t mat, uint32_t s, float clip) {
         if (threadIdx.x >= S::NT) return;  // whole waves
         switch (a.in.type) {
-            case MG_TYPE_FP32: return load<UPDATE, float>(a, mat, s);
-            case MG_TYPE_BF16: return load<UPDATE, __bf16>(a, mat, s);
-            default: return load<UPDATE, f16>(a, mat, s);
+            case MG_TYPE_FP32: return load<UPDATE, float>(a, mat, s, clip);
+            case MG_TYPE_BF16: return load<UPDATE, __bf16>(a, mat, s, clip);
+            default: return load<UPDATE, f16>(a, mat, s, clip);
         }
     }
 };
@@ -227,19 +237,21 @@ struct ShortPart {
 // product: one of the two takes a thread's four elements as they are, the other
 // those of four threads.
 template <int MP>
-__global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_first_kernel(const ShortArgs a) {
+__global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_first_kernel(const ShortArgs args) {
     using S = ShortShape<MP>;
     constexpr int W = S::THREADS / 64;
     __shared__ __align__(16) f16 rows[S::SLAB];
     __shared__ float wmax[W];
     const uint32_t mat = blockIdx.y;
+    const ShortArgs a = args.of(mat);
     const int t = threadIdx.x;
     const bool tall = a.src.rows > a.src.cols;
+    const float clip = source_clip(a.src);
     ShortPart<MP> part(tall);
     float most = 0.0f;
 #pragma unroll 1
     for (uint32_t s = blockIdx.x; s < a.slabs; s += a.parts) {
-        part.template load<true>(a.src, mat, s);
+        part.template load<true>(a.src, mat, s, clip);
         if (t < S::NT)
 #pragma unroll
             for (int e = 0; e < S::PER; ++e) most = fmaxf(most, magnitude(part.u[e]));
@@ -260,7 +272,7 @@ __global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_first_kernel(co
 #pragma unroll 1
     for (uint32_t s = blockIdx.x; s < a.slabs; s += a.parts) {
         if (a.slabs > a.parts) {  // else the only slab is still held
-            part.template load<false>(a.src, mat, s);
+            part.template load<false>(a.src, mat, s, clip);
             __syncthreads();
         }
         f16* const xt = a.xt + ((size_t)mat * a.slabs + s) * S::SLAB;
@@ -420,11 +432,12 @@ __device__ __forceinline__ void with_type(uint32_t type, F&& f) {
 // replace the old in xt (each workgroup's own slabs) and go to LDS in rows for the
 // Gram product.
 template <int MP, bool FINAL>
-__global__ void __launch_bounds__(FINAL ? ShortShape<MP>::NT : ShortShape<MP>::THREADS) short_update_kernel(const ShortArgs a) {
+__global__ void __launch_bounds__(FINAL ? ShortShape<MP>::NT : ShortShape<MP>::THREADS) short_update_kernel(const ShortArgs args) {
     using S = ShortShape<MP>;
     __shared__ __align__(16) f16 q[S::SQ];
     __shared__ __align__(16) f16 rows[FINAL ? 8 : S::SLAB];
     const uint32_t mat = blockIdx.y;
+    const ShortArgs a = args.of(mat);
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 31, h = lane >> 5;
     const int jb = wave & 3;  // the wave's 32 columns of the slab
     f16x8 x[MP / 16][2];

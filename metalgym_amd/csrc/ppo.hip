@@ -44,6 +44,9 @@ struct mg_ppo {
     float* mb_stats = nullptr;
     uint32_t mb_cap = 0;
     std::vector<float> mb_host;
+    bool muon_on = false;  // the block matrices' optimiser: Muon, else Adam
+    mg_muon_config muon{};
+    void* muon_ws = nullptr;
 };
 
 namespace mg {
@@ -185,6 +188,8 @@ int enqueue_minibatch(mg_ppo* p, uint32_t block, uint32_t mb_index, const TrainW
     ts.mb_index = mb_index;
     ts.beta1_pow = powf(0.9f, stepF);
     ts.beta2_pow = powf(0.999f, stepF);
+    ts.muon = p->muon_on ? &p->muon : nullptr;
+    ts.muon_ws = p->muon_ws;
     return launch_train_step(p->gym->stream, p->pv, p->hp, p->cfg.lr, ws, ts, p->obs_slots, p->action_slots,
                              p->adv, p->ret, p->logp, p->adv_stats, p->m, p->v, p->head, stats);
 }
@@ -405,6 +410,7 @@ int mg_ppo_destroy(mg_ppo* p) {
     (void)hipFree(p->head);
     (void)hipFree(p->ws_base);
     (void)hipFree(p->mb_stats);
+    (void)hipFree(p->muon_ws);
     delete p;
     return MG_OK;
 }
@@ -424,6 +430,26 @@ int mg_ppo_set_hparams(mg_ppo* p, const mg_ppo_hparams* hp) {
 int mg_ppo_get_hparams(mg_ppo* p, mg_ppo_hparams* hp) {
     MG_CHECK(p && hp, MG_ERR_INVALID, "mg_ppo_get_hparams: null argument");
     *hp = p->hp;
+    return MG_OK;
+}
+
+int mg_ppo_set_muon(mg_ppo* p, const mg_muon_config* config) {
+    MG_CHECK(p, MG_ERR_INVALID, "set_muon: null model");
+    if (config) {
+        if (int rc = check_muon_config("set_muon", config)) return rc;
+        if (!p->muon_ws)
+            if (int rc = device_alloc(&p->muon_ws, muon_blocks_bytes(p->pv), "PPOModel Muon workspace")) return rc;
+        p->muon = *config;
+    }
+    const bool on = config != nullptr;
+    if (on != p->muon_on) {
+        // one optimiser's moments mean nothing to the other
+        const size_t bytes = (size_t)(p->pv.off_head - p->pv.float_group) * sizeof(float);
+        MG_HIP(hipMemsetAsync(p->m + p->pv.float_group, 0, bytes, p->gym->stream), "set_muon clear");
+        MG_HIP(hipMemsetAsync(p->v + p->pv.float_group, 0, bytes, p->gym->stream), "set_muon clear");
+        MG_HIP(hipStreamSynchronize(p->gym->stream), "set_muon synchronize");
+        p->muon_on = on;
+    }
     return MG_OK;
 }
 

@@ -21,11 +21,15 @@
 //     launch.)
 //  4. adam: every workgroup adds the partial norms in the same fixed order
 //     (so no cross-workgroup synchronisation is needed), applies the clip
-//     scale and Adam (model/optimizer.metal:23-60).
+//     scale and Adam (model/optimizer.metal:23-60). With mg_ppo_set_muon the
+//     block matrices take the Muon update first (muon.hip, seven launches), and
+//     this launch only writes their copies.
 //
 // Every reduction has a fixed order, so a rerun gives the same bits (the
 // reference uses float atomics for several of these).
 #include <string.h>
+
+#include <type_traits>
 
 #include "kernels.h"
 #include "mg/device/policy_bf16.h"
@@ -1482,8 +1486,10 @@ __device__ __forceinline__ float adam_clip_scale(const AdamArgs& a) {
 // write it to the fragment-tiled copies as well; the rest update the vector
 // group and the head elementwise. Workgroup 0 also records the pre-clip norm.
 // FP32: each tile's largest magnitude goes to PairScale.tilemax; PAIRS: the
-// tiles go to the pair planes instead of the copies (policy_pair.h).
-template <bool FP32, bool PAIRS>
+// tiles go to the pair planes instead of the copies (policy_pair.h). MUON: the
+// block matrices have been updated already (launch_muon_blocks), so that their
+// tiles only go to the copies.
+template <bool FP32, bool PAIRS, bool MUON = false>
 __global__ void __launch_bounds__(256) adam_kernel(const AdamArgs a) {
     __shared__ float lds[kTT * kTileLd];
     __shared__ float wmax[FP32 ? 4 : 1];
@@ -1498,7 +1504,10 @@ __global__ void __launch_bounds__(256) adam_kernel(const AdamArgs a) {
         for (int e = 0; e < PER; ++e) {
             const int r = (256 / kTT) * e + t / kTT;
             idx[e] = m.base + (m.r0 + r) * m.cols + m.c0 + c;
-            in[e] = adam_load(a, idx[e]);
+            if constexpr (MUON)
+                in[e].p = a.param[idx[e]];
+            else
+                in[e] = adam_load(a, idx[e]);
         }
         const uint32_t per = a.hidden * kEmbed / (kTT * kTT), mat = blockIdx.x / per;
         const int exp = PAIRS ? a.pairs->next[mat] : 0;
@@ -1507,7 +1516,7 @@ __global__ void __launch_bounds__(256) adam_kernel(const AdamArgs a) {
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
             const int r = (256 / kTT) * e + t / kTT;
-            const float p = adam_elem(a, idx[e], in[e], scale);
+            const float p = MUON ? in[e].p : adam_elem(a, idx[e], in[e], scale);
             lds[r * kTileLd + c] = p;
             if (FP32) most = fmaxf(most, finite_magnitude(p));
         }
@@ -1710,7 +1719,8 @@ int launch_train_step(hipStream_t st, const mg_policy_view& pv, const mg_ppo_hpa
         ra.logp_slots = logp_slots;
         ra.adv_stats = adv_stats;
         ra.head_out = head_out;
-        ra.lr = lr;
+        // the exponents of the next planes allow for what the update may add: kAdamReach lr
+        ra.lr = step.muon ? fmaxf(lr, muon_blocks_reach(pv, *step.muon) / dev::kAdamReach) : lr;
         if (bf)
             hipLaunchKernelGGL(dev::train_rows_kernel<true>, dim3(B / dev::kTR), dim3(dev::kTNT), 0, st, ra);
         else if (rows_on_pairs(pv))
@@ -1802,8 +1812,11 @@ int launch_train_step(hipStream_t st, const mg_policy_view& pv, const mg_ppo_hpa
             MG_HIP(hipGetLastError(), "grad reduce launch");
         }
     }
-    {  // 4. Adam
+    {  // 4. Adam, after the block matrices' own update where they have one
         TimedLaunch tl(MG_K_ADAM, st);
+        if (step.muon)
+            if (int rc = launch_muon_blocks(st, pv, *step.muon, ws.grad, ws.normpart, hp.max_grad_norm, m, step.muon_ws))
+                return rc;
         dev::AdamArgs aa;
         aa.param = pv.params;
         // only the copies the next minibatch's row pass reads; the others are
@@ -1834,12 +1847,19 @@ int launch_train_step(hipStream_t st, const mg_policy_view& pv, const mg_ppo_hpa
         aa.max_grad_norm = hp.max_grad_norm;
         const uint32_t lin = pv.float_group + (pv.count - pv.off_head);
         const dim3 grid(aa.mat_tiles + (lin + 255) / 256);
-        if (bf)
-            hipLaunchKernelGGL((dev::adam_kernel<false, false>), grid, dim3(256), 0, st, aa);
-        else if (pairs)
-            hipLaunchKernelGGL((dev::adam_kernel<true, true>), grid, dim3(256), 0, st, aa);
+        auto launch = [&](auto muon) {
+            constexpr bool M = decltype(muon)::value;
+            if (bf)
+                hipLaunchKernelGGL((dev::adam_kernel<false, false, M>), grid, dim3(256), 0, st, aa);
+            else if (pairs)
+                hipLaunchKernelGGL((dev::adam_kernel<true, true, M>), grid, dim3(256), 0, st, aa);
+            else
+                hipLaunchKernelGGL((dev::adam_kernel<true, false, M>), grid, dim3(256), 0, st, aa);
+        };
+        if (step.muon)
+            launch(std::true_type{});
         else
-            hipLaunchKernelGGL((dev::adam_kernel<true, false>), grid, dim3(256), 0, st, aa);
+            launch(std::false_type{});
         MG_HIP(hipGetLastError(), "adam launch");
     }
     return MG_OK;

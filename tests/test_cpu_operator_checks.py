@@ -158,3 +158,12 @@ def test_matrix_null_arguments(mg):
     assert L.mg_orthogonalize_workspace(None, 1, 8, 8, None) == -1
     mg.orthogonalize(batch(mg, count=0, data=None), batch(mg, count=0, data=None))
     mg.muon_step(*(batch(mg, count=0, data=None) for _ in range(3)))
+
+
+def test_muon_decay_is_bounded(mg):
+    full = dict(workspace=1 << 20, workspace_bytes=1 << 40)
+    refused(lambda: mg.muon_step(batch(mg), batch(mg), batch(mg), lr=2.0, weight_decay=0.6, **full), "at most 1")
+
+
+def test_set_muon_needs_a_model(mg):
+    assert mg.lib().mg_ppo_set_muon(None, None) == -1
