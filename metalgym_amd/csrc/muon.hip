@@ -21,258 +21,11 @@
 // chains of 64 contraction elements, added up in fp32, keep that under the rest
 // (4.0e-6 of the result in one chain, 2.1e-6 so).
 //
-// Every operand is kept with its contraction index contiguous and both sides
-// padded to the tile with zeros, so the product kernel has no bounds checks.
+// muon_short.h takes matrices with a side of at most 128, muon_tiled.h the others.
 #include "muon_short.h"
+#include "muon_tiled.h"
 
 namespace mg {
-namespace dev {
-
-constexpr int kPT = 128;  // edge of a product tile; both sides are padded to it
-constexpr int kPK = 32;   // contraction elements of a stage
-constexpr int kNormParts = 128;  // most partial sums of a matrix's squares
-
-// Partial sums of U^2 in 64 bits (fp32 squares leave its range), [count][gridDim.x]
-// of them, and the momentum's update.
-__global__ void __launch_bounds__(256) source_norm_kernel(const SourceArgs a, double* partial) {
-    __shared__ double red[4];
-    const uint32_t k = blockIdx.y, tiles_c = (a.cols + 63) / 64, tiles = tiles_c * ((a.rows + 63) / 64);
-    double s = 0.0;
-    for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-        const uint32_t j = (t % tiles_c) * 64 + (threadIdx.x & 63), i0 = (t / tiles_c) * 64 + (threadIdx.x >> 6);
-        if (j < a.cols)
-            for (uint32_t i = i0; i < i0 + 64 && i < a.rows; i += 4) {
-                const double u = source_value<true>(a, k, i, j);
-                s += u * u;
-            }
-    }
-    for (int step = 1; step < 64; step *= 2) s += __shfl_xor(s, step);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) partial[(size_t)k * gridDim.x + blockIdx.x] = red[0] + red[1] + red[2] + red[3];
-}
-
-// 1 / (|U| + eps) in every thread, NaN where the norm is not finite. red holds 1.
-__device__ __forceinline__ float source_scale(const double* partial, uint32_t parts, float eps, float* red) {
-    if (threadIdx.x < 64) {
-        double s = 0.0;
-        for (uint32_t p = threadIdx.x; p < parts; p += 64) s += partial[p];
-        for (int step = 1; step < 64; step *= 2) s += __shfl_xor(s, step);
-        if (threadIdx.x == 0) {
-            const double norm = sqrt(s);
-            *red = norm < (double)__builtin_huge_valf() ? (float)(1.0 / (norm + (double)eps)) : __builtin_nanf("");
-        }
-    }
-    __syncthreads();
-    return *red;
-}
-
-// A pair of planes: the low halves lie `plane` elements after the high ones.
-struct Planes {
-    f16* hi;
-    size_t plane;   // elements of one plane
-    size_t stride;  // elements between matrices of the batch
-    uint32_t ld;
-};
-
-// U / (|U| + eps) times 2^e as pairs, X [mp][np] and its transpose XT [np][mp],
-// zeros in the padding; one 64 x 64 tile of X a workgroup.
-__global__ void __launch_bounds__(256) source_split_kernel(const SourceArgs a, const double* partial, uint32_t parts,
-                                                           float eps, float unit, Planes X, Planes XT) {
-    __shared__ float lds[64][65];
-    __shared__ float red;
-    const uint32_t k = blockIdx.z, t = threadIdx.x;
-    const float scale = source_scale(partial + (size_t)k * parts, parts, eps, &red);
-    const bool tall = a.rows > a.cols;
-    // the tile in the source's orientation, so that reads run along its rows
-    const uint32_t x0 = blockIdx.y * 64, y0 = blockIdx.x * 64;  // X's row and column
-    const uint32_t i0 = tall ? y0 : x0, j0 = tall ? x0 : y0;
-    for (uint32_t e = t >> 6; e < 64; e += 4) {
-        const uint32_t i = i0 + e, j = j0 + (t & 63);
-        const float u = i < a.rows && j < a.cols ? source_value<false>(a, k, i, j) * scale * unit : 0.0f;
-        if (tall)
-            lds[t & 63][e] = u;
-        else
-            lds[e][t & 63] = u;
-    }
-    __syncthreads();
-    f16* const x = X.hi + k * X.stride;
-    f16* const xt = XT.hi + k * XT.stride;
-    const uint32_t c = (t & 15) * 4;
-    for (uint32_t r = t >> 4; r < 64; r += 16) {
-        f16x4 h, l, ht, lt;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            f16 p, q;
-            split(lds[r][c + e], p, q);
-            h[e] = p, l[e] = q;
-            split(lds[c + e][r], p, q);
-            ht[e] = p, lt[e] = q;
-        }
-        const size_t at = (size_t)(x0 + r) * X.ld + y0 + c, at_t = (size_t)(y0 + r) * XT.ld + x0 + c;
-        *reinterpret_cast<f16x4*>(x + at) = h;
-        *reinterpret_cast<f16x4*>(x + X.plane + at) = l;
-        *reinterpret_cast<f16x4*>(xt + at_t) = ht;
-        *reinterpret_cast<f16x4*>(xt + XT.plane + at_t) = lt;
-    }
-}
-
-// What becomes of a product's element v = (a b')(i, j).
-enum {
-    kSymmetric = 0,  // out(i, j) = out(j, i) = v
-    kPolynomial,     // the same with c v + b A(i, j) + a [i = j], v = (A A)(i, j)
-    kUpdate,         // X' = v, both X [i][j] and XT [j][i]
-    kFinal,          // the result: out = v, or w = keep w - rate v
-};
-struct ProductArgs {
-    Planes a, b;       // [rows][K], [cols][K]
-    uint32_t k;        // K, a multiple of two stages
-    uint32_t tiles_j;  // tile columns (symmetric results: tile rows and columns)
-    float unit;        // takes the operands' exponents out of the sums and puts the result's in
-    Planes out, out_t;
-    // kPolynomial
-    Planes gram;
-    float ca, cb, cc;  // with the result's exponent; cc also takes the operands' out
-    uint32_t m;        // rows that hold a matrix: no a I in the padding
-    // kFinal
-    Batch dst;
-    uint32_t rows, cols;
-    uint32_t step;  // an optimiser step
-    float keep, rate;
-};
-
-// One 128 x 128 tile of a product a b' of pairs. Four waves, 64 x 64 each as 2 x 2
-// tiles of v_mfma_f32_32x32x16_f16. Stages of 32 contraction elements go from
-// memory straight to LDS (16 bytes a lane, two buffers, so a stage's loads run
-// under the one before). In a 64-byte LDS row the 16-byte chunk c of row r sits at
-// c ^ (r / 2 % 4), which spreads a fragment's reads over all banks; the loads take
-// the chunk from where it belongs, since the LDS side of such a load is linear.
-template <int KIND>
-__global__ void __launch_bounds__(256) product_kernel(const ProductArgs p) {
-    constexpr int kRowB = kPK * 2, kPlaneB = kPT * kRowB, kStageB = 4 * kPlaneB;  // bytes
-    __shared__ __align__(1024) char lds[2 * kStageB];
-    uint32_t ti, tj;
-    if constexpr (KIND <= kPolynomial) {
-        // tiles on and under the diagonal, row by row
-        ti = (uint32_t)((sqrtf(8.0f * (float)blockIdx.x + 1.0f) - 1.0f) * 0.5f);
-        while (ti * (ti + 1) / 2 > blockIdx.x) --ti;
-        while ((ti + 1) * (ti + 2) / 2 <= blockIdx.x) ++ti;
-        tj = blockIdx.x - ti * (ti + 1) / 2;
-    } else {
-        ti = blockIdx.x / p.tiles_j, tj = blockIdx.x % p.tiles_j;
-    }
-    const uint32_t mat = blockIdx.y;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    // this lane's part of a stage's loads: wave w brings plane w (a hi, a lo, b hi, b
-    // lo), 16 rows an instruction
-    const Planes& src = wave < 2 ? p.a : p.b;
-    const f16* from = src.hi + mat * src.stride + (wave & 1) * src.plane +
-                      (size_t)((wave < 2 ? ti : tj) * kPT + (lane >> 2)) * src.ld +
-                      ((lane & 3) ^ ((lane >> 3) & 3)) * 8;
-    const size_t step16 = (size_t)16 * src.ld;
-    auto load = [&](int buf) {
-        char* to = lds + buf * kStageB + wave * kPlaneB;
-#pragma unroll
-        for (int r = 0; r < kPT / 16; ++r)
-            __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void*)(from + r * step16),
-                (__attribute__((address_space(3))) void*)(to + r * 16 * kRowB), 16, 0, 0);
-        from += kPK;
-    };
-    const int wi = (wave >> 1) * 64, wj = (wave & 1) * 64, row = lane & 31;
-    f32x16 acc[2][2] = {}, sum[2][2];
-    const uint32_t stages = p.k / kPK;
-    load(0);
-    for (uint32_t s = 0; s < stages; s += 2) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            // this stage has arrived, and every wave is done with the buffer that the next goes to
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (s + half + 1 < stages) load(half ^ 1);
-            const char* base = lds + half * kStageB;
-#pragma unroll
-            for (int kk = 0; kk < kPK / 16; ++kk) {
-                const int chunk = (kk * 2 + (lane >> 5)) ^ ((row >> 1) & 3);
-                f16x8 fa[2][2], fb[2][2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const int at = (32 * q + row) * kRowB + chunk * 16;
-                        fa[q][h] = *reinterpret_cast<const f16x8*>(base + h * kPlaneB + wi * kRowB + at);
-                        fb[q][h] = *reinterpret_cast<const f16x8*>(base + (2 + h) * kPlaneB + wj * kRowB + at);
-                    }
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const f32x16 zero = {};
-                        f32x16 t = half == 0 && kk == 0 ? zero : sum[i][j];
-                        t = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][1], fb[j][0], t, 0, 0, 0);
-                        t = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][0], fb[j][1], t, 0, 0, 0);
-                        sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][0], fb[j][0], t, 0, 0, 0);
-                    }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) acc[i][j] += sum[i][j];
-    }
-#pragma unroll
-    for (int qi = 0; qi < 2; ++qi)
-#pragma unroll
-        for (int qj = 0; qj < 2; ++qj) {
-            const uint32_t i0 = ti * kPT + wi + 32 * qi + 4 * (lane >> 5), j = tj * kPT + wj + 32 * qj + row;
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const uint32_t i = i0 + 2 * r;  // four rows from here: registers r .. r + 3
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[qi][qj][r + e];
-                if constexpr (KIND == kFinal) {
-                    const bool tall = p.rows > p.cols;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t y = tall ? j : i + e, x = tall ? i + e : j;
-                        if (y >= p.rows || x >= p.cols) continue;
-                        const size_t at = p.dst.at(mat, y, x);
-                        const float o = v[e] * p.unit;
-                        batch_store(p.dst, at, p.step ? p.keep * batch_load(p.dst, at) - p.rate * o : o);
-                    }
-                } else {
-                    const f16* gram = p.gram.hi + mat * p.gram.stride;
-                    f16* out = p.out.hi + mat * p.out.stride;
-                    f16* out_t = p.out_t.hi + mat * p.out_t.stride;
-                    f16x4 th, tl;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float x = v[e] * p.unit;
-                        if constexpr (KIND == kPolynomial) {
-                            const size_t at = (size_t)(i + e) * p.gram.ld + j;
-                            x = p.cc * v[e] + p.cb * ((float)gram[at] + (float)gram[p.gram.plane + at]) +
-                                (i + e == j && j < p.m ? p.ca : 0.0f);
-                        }
-                        f16 h, l;
-                        split(x, h, l);
-                        th[e] = h, tl[e] = l;
-                        const size_t at = (size_t)(i + e) * p.out.ld + j;
-                        out[at] = h;
-                        out[p.out.plane + at] = l;
-                    }
-                    const size_t at = (size_t)j * p.out_t.ld + i;
-                    if (KIND == kUpdate || ti != tj) {
-                        *reinterpret_cast<f16x4*>(out_t + at) = th;
-                        *reinterpret_cast<f16x4*>(out_t + p.out_t.plane + at) = tl;
-                    }
-                }
-            }
-        }
-}
-
-}  // namespace dev
-
 namespace {
 
 constexpr mg_newton_schulz kDefaultNs = {5, 3.4445f, -4.7750f, 2.0315f, 1e-7f};
@@ -473,9 +226,8 @@ int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, co
     }
     const Workspace w(count, src.rows, src.cols);
     char* const base = static_cast<char*>(workspace);
-    auto planes = [&](size_t at, uint32_t rows, uint32_t ld) {
-        const size_t plane = (size_t)rows * ld;
-        return dev::Planes{reinterpret_cast<dev::f16*>(base + at), plane, 2 * plane, ld};
+    auto planes = [&](size_t at, uint32_t rows, uint32_t k) {
+        return dev::Planes{reinterpret_cast<dev::f16*>(base + at), (size_t)rows * k * 2, k / 16};
     };
     double* const norms = reinterpret_cast<double*>(base + w.norms);
     const dev::Planes X = planes(w.x, w.mp, w.np);
@@ -485,27 +237,28 @@ int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, co
     const dev::Planes Q[2] = {planes(w.q[0], w.mp, w.mp), planes(w.q[1], w.mp, w.mp)};
     const uint32_t tiles = ((src.rows + 63) / 64) * ((src.cols + 63) / 64);
     const uint32_t parts = tiles < (uint32_t)dev::kNormParts ? tiles : dev::kNormParts;
+    const uint32_t mt = w.mp / dev::kPT, nt = w.np / dev::kPT;
     hipLaunchKernelGGL(dev::source_norm_kernel, dim3(parts, count), dim3(256), 0, st, src, norms);
     MG_HIP(hipGetLastError(), "newton-schulz norm launch");
-    hipLaunchKernelGGL(dev::source_split_kernel, dim3(w.np / 64, w.mp / 64, count), dim3(256), 0, st, src, norms, parts,
+    const bool tall = src.rows > src.cols;
+    hipLaunchKernelGGL(dev::source_split_kernel, dim3((tall ? w.mp : w.np) / 64, (tall ? w.np : w.mp) / 64, count), dim3(256), 0, st, src, norms, parts,
                        ns.eps, kUnitX, X, XT[0]);
     MG_HIP(hipGetLastError(), "newton-schulz split launch");
 
-    const uint32_t mt = w.mp / dev::kPT, nt = w.np / dev::kPT;
     const dim3 half(mt * (mt + 1) / 2, count), full(mt * nt, count), block(256);
     dev::ProductArgs p{};
     p.m = w.m;
     // out = a b' of symmetric results
     auto symmetric = [&](const dev::Planes& a, const dev::Planes& b, uint32_t k, float unit_a, float unit_b,
                          const dev::Planes& out, float unit_out) -> int {
-        p.a = a, p.b = b, p.k = k, p.tiles_j = mt, p.out = out, p.out_t = out;
+        p.a = a, p.b = b, p.stages = k / dev::kPK, p.tiles_j = mt, p.out = out;
         p.unit = unit_out / (unit_a * unit_b);
         hipLaunchKernelGGL((dev::product_kernel<dev::kSymmetric>), half, block, 0, st, p);
         MG_HIP(hipGetLastError(), "newton-schulz product launch");
         return MG_OK;
     };
     auto polynomial = [&](const dev::Planes& out) -> int {
-        p.a = p.b = p.gram = gram, p.k = w.mp, p.tiles_j = mt, p.out = out, p.out_t = out;
+        p.a = p.b = p.gram = gram, p.stages = w.mp / dev::kPK, p.tiles_j = mt, p.out = out;
         p.ca = ns.a * kUnitP, p.cb = ns.b * (kUnitP / kUnitA), p.cc = ns.c * (kUnitP / (kUnitA * kUnitA));
         hipLaunchKernelGGL((dev::product_kernel<dev::kPolynomial>), half, block, 0, st, p);
         MG_HIP(hipGetLastError(), "newton-schulz polynomial launch");
@@ -531,7 +284,7 @@ int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, co
             unit_q = unit, q ^= 1;
         }
         left -= steps;
-        p.a = Q[q], p.b = XT[cur], p.k = w.mp, p.tiles_j = nt;
+        p.a = Q[q], p.b = XT[cur], p.stages = w.mp / dev::kPK, p.tiles_j = nt;
         if (left) {
             p.out = X, p.out_t = XT[cur ^ 1], p.unit = 1.0f / unit_q;
             hipLaunchKernelGGL((dev::product_kernel<dev::kUpdate>), full, block, 0, st, p);
@@ -540,7 +293,12 @@ int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, co
         } else {
             p.dst = fin.dst, p.step = fin.step, p.keep = fin.keep, p.rate = fin.rate, p.rows = src.rows, p.cols = src.cols;
             p.unit = 1.0f / (unit_q * kUnitX);
-            hipLaunchKernelGGL((dev::product_kernel<dev::kFinal>), full, block, 0, st, p);
+            if (tall) {
+                p.a = XT[cur], p.b = Q[q], p.tiles_j = mt;
+                hipLaunchKernelGGL((dev::product_kernel<dev::kFinalTall>), full, block, 0, st, p);
+            } else {
+                hipLaunchKernelGGL((dev::product_kernel<dev::kFinal>), full, block, 0, st, p);
+            }
             MG_HIP(hipGetLastError(), "newton-schulz result launch");
         }
     }

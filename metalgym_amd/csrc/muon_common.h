@@ -51,18 +51,41 @@ struct Batch {
         return k * stride + (uint64_t)i * ld + j;
     }
 };
-__device__ __forceinline__ float batch_load(const Batch& b, size_t at) {
-    if (b.type == MG_TYPE_FP32) return static_cast<const float*>(b.data)[at];
-    if (b.type == MG_TYPE_BF16) return (float)static_cast<const __bf16*>(b.data)[at];
-    return (float)static_cast<const f16*>(b.data)[at];
+// f(a value of the type's T)
+template <class F>
+__device__ __forceinline__ void with_type(uint32_t type, F&& f) {
+    switch (type) {
+        case MG_TYPE_FP32: return f(float{});
+        case MG_TYPE_BF16: return f(__bf16{});
+        default: return f(f16{});
+    }
 }
-__device__ __forceinline__ void batch_store(const Batch& b, size_t at, float x) {
-    if (b.type == MG_TYPE_FP32)
-        static_cast<float*>(b.data)[at] = x;
-    else if (b.type == MG_TYPE_BF16)
-        static_cast<__bf16*>(b.data)[at] = (__bf16)x;
-    else
-        static_cast<f16*>(b.data)[at] = (f16)x;
+// A lane's 16 elements of a 32 x 32 tile as the matrix instructions leave them:
+// element e lies 8 (e / 4) + e % 4 rows under y0, in column x, if the matrix (rows x
+// cols) reaches there.
+__device__ __forceinline__ void tile_read(const Batch& b, uint32_t rows, uint32_t cols, uint32_t k, uint32_t y0,
+                                          uint32_t x, float (&w)[16]) {
+    with_type(b.type, [&](auto t) {
+        const auto* from = static_cast<const decltype(t)*>(b.data) + b.at(k, 0, x < cols ? x : 0);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const uint32_t y = y0 + 2 * (e & ~3) + (e & 3);
+            w[e] = (float)from[(uint64_t)(y < rows ? y : rows - 1) * b.ld];
+        }
+    });
+}
+__device__ __forceinline__ void tile_write(const Batch& b, uint32_t rows, uint32_t cols, uint32_t k, uint32_t y0,
+                                           uint32_t x, const float (&w)[16]) {
+    if (x >= cols) return;
+    with_type(b.type, [&](auto t) {
+        using T = decltype(t);
+        T* const to = static_cast<T*>(b.data) + b.at(k, 0, x);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const uint32_t y = y0 + 2 * (e & ~3) + (e & 3);
+            if (y < rows) to[(uint64_t)y * b.ld] = (T)w[e];
+        }
+    });
 }
 
 // What is orthogonalised: `in`, or with a momentum batch the Muon update's U from
@@ -94,16 +117,5 @@ __device__ __forceinline__ float moved_momentum(const SourceArgs& a, float m, fl
 __device__ __forceinline__ float update_of(const SourceArgs& a, float m, float g) {
     return a.nesterov ? g + a.beta * (m - g) : m;
 }
-// U(i, j) of matrix k; UPDATE also moves the momentum to this gradient.
-template <bool UPDATE>
-__device__ __forceinline__ float source_value(const SourceArgs& a, uint32_t k, uint32_t i, uint32_t j) {
-    const float g = batch_load(a.in, a.in.at(k, i, j));
-    if (!a.momentum.data) return g;
-    float* const mp = static_cast<float*>(a.momentum.data) + a.momentum.at(k, i, j);
-    float m = *mp;
-    if constexpr (UPDATE) *mp = m = moved_momentum(a, m, g);
-    return update_of(a, m, g);
-}
-
 }  // namespace dev
 }  // namespace mg

@@ -49,20 +49,21 @@ struct Frags {
 };
 
 // Lane q of each four lanes holds four values of column 4 a + q; gives it value q
-// of the four columns 4 a .. 4 a + 3.
+// of the four columns 4 a .. 4 a + 3. Byte permutes with a lane's own selectors:
+// selects become branches here.
 __device__ __forceinline__ f16x4 quad_transpose(f16x4 v) {
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-    const int q = threadIdx.x & 3;
-    u32x2 w = __builtin_bit_cast(u32x2, v);  // values (0, 1), (2, 3)
+    const uint32_t q = threadIdx.x & 3;
+    const uint32_t halves = q & 1 ? 0x03020706u : 0x05040100u;  // (partner's high, own high) or (own low, partner's low)
+    const uint32_t first = q & 2 ? 0x07060504u : 0x03020100u;   // the permute's first operand, or its second
+    const u32x2 w = __builtin_bit_cast(u32x2, v);  // values (0, 1), (2, 3)
     // lanes q and q ^ 1 trade halves: even lanes get value 0 of both columns, then 2
     const uint32_t n0 = __builtin_amdgcn_mov_dpp(w[0], 0xB1, 0xF, 0xF, true);
     const uint32_t n1 = __builtin_amdgcn_mov_dpp(w[1], 0xB1, 0xF, 0xF, true);
-    const uint32_t p0 = q & 1 ? (n0 >> 16) | (w[0] & 0xFFFF0000u) : (w[0] & 0xFFFFu) | (n0 << 16);
-    const uint32_t p1 = q & 1 ? (n1 >> 16) | (w[1] & 0xFFFF0000u) : (w[1] & 0xFFFFu) | (n1 << 16);
+    const uint32_t p0 = __builtin_amdgcn_perm(n0, w[0], halves), p1 = __builtin_amdgcn_perm(n1, w[1], halves);
     // lanes q and q ^ 2 trade words: the lower two lanes keep values 0 and 1
-    const uint32_t give = q & 2 ? p0 : p1;
-    const uint32_t got = __builtin_amdgcn_mov_dpp(give, 0x4E, 0xF, 0xF, true);
-    const u32x2 out = q & 2 ? u32x2{got, p1} : u32x2{p0, got};
+    const uint32_t got = __builtin_amdgcn_mov_dpp(__builtin_amdgcn_perm(p0, p1, first), 0x4E, 0xF, 0xF, true);
+    const u32x2 out = {__builtin_amdgcn_perm(got, p0, first), __builtin_amdgcn_perm(p1, got, first)};
     return __builtin_bit_cast(f16x4, out);
 }
 
@@ -395,37 +396,6 @@ __global__ void __launch_bounds__(64 * ShortShape<MP>::NB * ShortShape<MP>::NB) 
     }
 }
 
-// A tile of the result, or of the optimiser's step: register e of a lane lies 8 (e /
-// 4) + e % 4 rows under y0, at column x of dst.
-template <class T>
-__device__ __forceinline__ void short_read(const ShortArgs& a, uint32_t mat, uint32_t y0, uint32_t x, float (&w)[16]) {
-    const T* const from = static_cast<const T*>(a.dst.data) + a.dst.at(mat, 0, x < a.src.cols ? x : 0);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const uint32_t y = y0 + 2 * (e & ~3) + (e & 3);
-        w[e] = (float)from[(uint64_t)(y < a.src.rows ? y : a.src.rows - 1) * a.dst.ld];
-    }
-}
-template <class T>
-__device__ __forceinline__ void short_write(const ShortArgs& a, uint32_t mat, uint32_t y0, uint32_t x, const float (&w)[16]) {
-    if (x >= a.src.cols) return;
-    T* const to = static_cast<T*>(a.dst.data) + a.dst.at(mat, 0, x);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const uint32_t y = y0 + 2 * (e & ~3) + (e & 3);
-        if (y < a.src.rows) to[(uint64_t)y * a.dst.ld] = (T)w[e];
-    }
-}
-// f(value of the type) with a value of the type's T
-template <class F>
-__device__ __forceinline__ void with_type(uint32_t type, F&& f) {
-    switch (type) {
-        case MG_TYPE_FP32: return f(float{});
-        case MG_TYPE_BF16: return f(__bf16{});
-        default: return f(f16{});
-    }
-}
-
 // Grid (parts, count): X <- Q X. A wave holds 32 columns of X, its fragments straight
 // from xt (two waves share them and split the rows of Q); Q is in LDS. FINAL writes
 // the result, in the orientation that runs along dst's rows. Otherwise the new pairs
@@ -493,7 +463,7 @@ __global__ void __launch_bounds__(FINAL ? ShortShape<MP>::NT : ShortShape<MP>::T
                 const uint32_t along = s * kSlab + 32 * jb, across = 32 * b;
                 const uint32_t y0 = (tall ? along : across) + 4 * h, c = (tall ? across : along) + r;
                 float w[16];
-                if (a.step) with_type(a.dst.type, [&](auto t) { short_read<decltype(t)>(a, mat, y0, c, w); });
+                if (a.step) tile_read(a.dst, a.src.rows, a.src.cols, mat, y0, c, w);
                 f32x16 acc;
                 if (tall)
                     acc = product(b, false);
@@ -501,7 +471,7 @@ __global__ void __launch_bounds__(FINAL ? ShortShape<MP>::NT : ShortShape<MP>::T
                     acc = product(b, true);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) w[e] = a.step ? a.keep * w[e] - a.rate * (acc[e] * f) : acc[e] * f;
-                with_type(a.dst.type, [&](auto t) { short_write<decltype(t)>(a, mat, y0, c, w); });
+                tile_write(a.dst, a.src.rows, a.src.cols, mat, y0, c, w);
             } else {
                 const f32x16 acc = product(b, false);
                 const int i = 32 * b + r;  // X'(i, j .. j + 3)

@@ -1,0 +1,300 @@
+// Newton-Schulz steps of matrices whose sides are both over 128: one launch a
+// product of 128 x 128 tiles, half the tiles of symmetric results.
+//
+// Operands are pairs in the order of the matrix instructions' operands (Frags of
+// muon_short.h): a tile's stage is contiguous runs of 4 KB that go to LDS as they
+// lie, and LDS reads have no bank conflicts. Both sides are padded to the tile with
+// zeros, so the product kernel has no bounds checks.
+#pragma once
+#include "muon_short.h"
+
+namespace mg {
+namespace dev {
+
+constexpr int kPT = 128;  // edge of a product tile; both sides are padded to it
+constexpr int kPK = 32;   // contraction elements of a stage
+constexpr int kRing = 4;  // stages in LDS
+constexpr int kNormParts = 1024;  // most partial sums of a matrix's squares
+
+// A thread's 16 elements of a 64 x 64 tile of the source at (i0, j0): column t % 64,
+// rows 16 (t / 64) .. of it; zeros outside. UPDATE also moves the momentum.
+template <bool UPDATE, class T>
+__device__ __forceinline__ void tile_load(const SourceArgs& a, uint32_t k, uint32_t i0, uint32_t j0, float (&u)[16]) {
+    const uint32_t j = j0 + (threadIdx.x & 63), i = i0 + (threadIdx.x >> 6) * 16;
+    const uint32_t jc = j < a.cols ? j : a.cols - 1, ic = i < a.rows ? i : a.rows - 1;
+    const T* in = static_cast<const T*>(a.in.data) + a.in.at(k, ic, jc);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        u[e] = (float)*in;
+        in += i + e + 1 < a.rows ? a.in.ld : 0u;
+    }
+    if (a.momentum.data) {
+        float* to = static_cast<float*>(a.momentum.data) + a.momentum.at(k, ic, jc);
+        const float* from = to;
+        float b[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            b[e] = *from;
+            from += i + e + 1 < a.rows ? a.momentum.ld : 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            if constexpr (UPDATE) {
+                b[e] = moved_momentum(a, b[e], u[e]);
+                if (j < a.cols && i + e < a.rows) *to = b[e];
+                to += a.momentum.ld;
+            }
+            u[e] = update_of(a, b[e], u[e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) u[e] = j < a.cols && i + e < a.rows ? u[e] : 0.0f;
+}
+template <bool UPDATE>
+__device__ __forceinline__ void tile_load(const SourceArgs& a, uint32_t k, uint32_t i0, uint32_t j0, float (&u)[16]) {
+    with_type(a.in.type, [&](auto t) { tile_load<UPDATE, decltype(t)>(a, k, i0, j0, u); });
+}
+
+// Partial sums of U^2 in 64 bits (fp32 squares leave its range), [count][gridDim.x]
+// of them, and the momentum's update.
+__global__ void __launch_bounds__(256) source_norm_kernel(const SourceArgs a, double* partial) {
+    __shared__ double red[4];
+    const uint32_t k = blockIdx.y, tiles_c = (a.cols + 63) / 64, tiles = tiles_c * ((a.rows + 63) / 64);
+    double s = 0.0;
+    for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+        float u[16];
+        tile_load<true>(a, k, t / tiles_c * 64, t % tiles_c * 64, u);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s += (double)u[e] * (double)u[e];
+    }
+    for (int step = 1; step < 64; step *= 2) s += __shfl_xor(s, step);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) partial[(size_t)k * gridDim.x + blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+// 1 / (|U| + eps) in every thread, NaN where the norm is not finite. red holds 1.
+__device__ __forceinline__ float source_scale(const double* partial, uint32_t parts, float eps, float* red) {
+    if (threadIdx.x < 64) {
+        double s = 0.0;
+#pragma unroll 4
+        for (uint32_t p = threadIdx.x; p < parts; p += 64) s += partial[p];
+        for (int step = 1; step < 64; step *= 2) s += __shfl_xor(s, step);
+        if (threadIdx.x == 0) {
+            const double norm = sqrt(s);
+            *red = norm < (double)__builtin_huge_valf() ? (float)(1.0 / (norm + (double)eps)) : __builtin_nanf("");
+        }
+    }
+    __syncthreads();
+    return *red;
+}
+
+// A matrix of pairs: kb blocks of 16 contraction elements for each 32 rows.
+struct Planes {
+    f16* base;
+    size_t stride;  // elements between matrices of the batch
+    uint32_t kb;
+    // columns c ... of row r of matrix k: c a multiple of 4; the low halves 512 further
+    __device__ __forceinline__ f16* at(uint32_t k, uint32_t r, uint32_t c) const {
+        return base + k * stride + ((size_t)(r >> 5) * kb + (c >> 4)) * 1024 + ((c & 8) << 5) + ((r & 31) << 3) + (c & 4);
+    }
+    __device__ __forceinline__ void put(uint32_t k, uint32_t r, uint32_t c, f16x4 hi, f16x4 lo) const {
+        f16* const to = at(k, r, c);
+        *reinterpret_cast<f16x4*>(to) = hi;
+        *reinterpret_cast<f16x4*>(to + 512) = lo;
+    }
+};
+
+// U / (|U| + eps) times `unit` as pairs, X [mp][np] and its transpose XT [np][mp],
+// zeros in the padding; one 64 x 64 tile of the source a workgroup. A thread's
+// elements are a run along one of the two; the other takes four threads'.
+__global__ void __launch_bounds__(256) source_split_kernel(const SourceArgs a, const double* partial, uint32_t parts,
+                                                           float eps, float unit, Planes X, Planes XT) {
+    __shared__ float red;
+    const uint32_t k = blockIdx.z, i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
+    float u[16];
+    tile_load<false>(a, k, i0, j0, u);
+    const float scale = source_scale(partial + (size_t)k * parts, parts, eps, &red) * unit;
+    const bool tall = a.rows > a.cols;
+    const Planes& by_column = tall ? X : XT;  // rows of it are the source's columns
+    const Planes& by_row = tall ? XT : X;
+    const uint32_t j = j0 + (threadIdx.x & 63), i = i0 + (threadIdx.x >> 6) * 16;
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+        const float x[4] = {u[e], u[e + 1], u[e + 2], u[e + 3]};
+        f16x4 hi, lo;
+        split4(x, scale, hi, lo);
+        by_column.put(k, j, i + e, hi, lo);
+        by_row.put(k, i + e + (threadIdx.x & 3), j & ~3u, quad_transpose(hi), quad_transpose(lo));
+    }
+}
+
+// What becomes of a product's element v = (a b')(i, j).
+enum {
+    kSymmetric = 0,  // out(i, j) = out(j, i) = v
+    kPolynomial,     // the same with c v + b A(i, j) + a [i = j], v = (A A)(i, j)
+    kUpdate,         // X' = v, both X [i][j] and XT [j][i]
+    kFinal,          // the result of a wide matrix: dst(i, j) = v, or keep dst(i, j) - rate v
+    kFinalTall,      // and of a tall one, whose product has a and b in each other's place
+};
+struct ProductArgs {
+    Planes a, b;       // [rows][K], [cols][K]
+    uint32_t stages;   // K / kPK, a multiple of 4
+    uint32_t tiles_j;  // tile columns (symmetric results: tile rows and columns)
+    float unit;        // takes the operands' exponents out of the sums and puts the result's in
+    Planes out, out_t;  // X [i][j] and XT [j][i], or a symmetric out
+    // kPolynomial
+    Planes gram;
+    float ca, cb, cc;  // with the result's exponent; cc also takes the operands' out
+    uint32_t m;        // rows that hold a matrix: no a I in the padding
+    // kFinal
+    Batch dst;
+    uint32_t rows, cols;
+    uint32_t step;  // an optimiser step
+    float keep, rate;
+};
+
+// Workgroups go to the 8 XCDs in turn, each of which has its own L2: gives every XCD
+// one run of tiles.
+__device__ __forceinline__ uint32_t xcd_run(uint32_t b, uint32_t count) {
+    const uint32_t x = b & 7, each = count >> 3, more = count & 7;
+    return x * each + (x < more ? x : more) + (b >> 3);
+}
+
+// One 128 x 128 tile of a product a b' of pairs. Four waves, 64 x 64 each as 2 x 2
+// tiles of v_mfma_f32_32x32x16_f16. Stages of 32 contraction elements (32 KB) go from
+// memory straight to a ring of four in LDS. In the middle of a stage, with its second
+// half already in registers, the waves meet once: the next stage has then arrived
+// (vmcnt counts in order, 8 loads a wave and stage), this stage's place is free for
+// the fourth one on, and the next stage's first fragments are read under the second
+// half's products.
+template <int KIND>
+__global__ void __launch_bounds__(256) product_kernel(const ProductArgs p) {
+    constexpr bool kResult = KIND >= kFinal, kSwap = KIND == kFinalTall;
+    constexpr int kStage = 4 * kPT * kPK;  // elements: a and b, two planes each
+    __shared__ __align__(1024) f16 lds[kRing * kStage];
+    const uint32_t mat = blockIdx.y, tile = xcd_run(blockIdx.x, gridDim.x);
+    uint32_t ti, tj;
+    if constexpr (KIND <= kPolynomial) {
+        // tiles on and under the diagonal, row by row
+        ti = (uint32_t)((sqrtf(8.0f * (float)tile + 1.0f) - 1.0f) * 0.5f);
+        while (ti * (ti + 1) / 2 > tile) --ti;
+        while ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
+        tj = tile - ti * (ti + 1) / 2;
+    } else {
+        const uint32_t tiles_i = gridDim.x / p.tiles_j;
+        ti = tile % tiles_i, tj = tile / tiles_i;
+    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // wave w brings 32 rows of a and of b: 4 KB a stage each
+    const f16* from_a = p.a.base + mat * p.a.stride + (size_t)(ti * 4 + wave) * p.a.kb * 1024 + lane * 8;
+    const f16* from_b = p.b.base + mat * p.b.stride + (size_t)(tj * 4 + wave) * p.b.kb * 1024 + lane * 8;
+    auto load = [&](uint32_t stage) {
+        f16* to = lds + (stage & (kRing - 1)) * kStage + wave * 2048;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from_a + c * 512),
+                                             (__attribute__((address_space(3))) void*)(to + c * 512), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from_b + c * 512),
+                                             (__attribute__((address_space(3))) void*)(to + 8192 + c * 512), 16, 0, 0);
+        }
+        from_a += 2048, from_b += 2048;
+    };
+    const int wi = wave >> 1, wj = wave & 1;
+    f16x8 fa[2][2][2], fb[2][2][2];  // [half of a stage][32 rows][plane]
+    auto read = [&](uint32_t stage, int kk) {
+        const f16* at = lds + (stage & (kRing - 1)) * kStage + kk * 1024 + lane * 8;
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                fa[kk][q][h] = *reinterpret_cast<const f16x8*>(at + (2 * wi + q) * 2048 + h * 512);
+                fb[kk][q][h] = *reinterpret_cast<const f16x8*>(at + 8192 + (2 * wj + q) * 2048 + h * 512);
+            }
+    };
+    f32x16 acc[2][2] = {}, sum[2][2];
+    auto multiply = [&](int kk, bool fresh) {
+#pragma unroll
+        for (int term = 0; term < 3; ++term)  // lo hi, hi lo, hi hi; kSwap: the bits of the other product
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                        fa[kk][i][term == (kSwap ? 1 : 0)], fb[kk][j][term == (kSwap ? 0 : 1)], fresh && term == 0 ? f32x16{} : sum[i][j], 0, 0, 0);
+    };
+    auto meet = [&](bool tail) {
+        if (tail)
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    const uint32_t stages = p.stages;
+    load(0), load(1), load(2);
+    meet(false);
+    load(3);
+    read(0, 0);
+    for (uint32_t s = 0; s < stages; s += 2) {
+#pragma unroll
+        for (int odd = 0; odd < 2; ++odd) {  // a chain of two stages
+            const uint32_t now = s + odd;
+            read(now, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(0, odd == 0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (now + 1 < stages) {
+                meet(now + 3 >= stages);
+                if (now + 4 < stages) load(now + 4);
+                read(now + 1, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(1, false);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) acc[i][j] += sum[i][j];
+    }
+#pragma unroll
+    for (int qi = 0; qi < 2; ++qi)
+#pragma unroll
+        for (int qj = 0; qj < 2; ++qj) {
+            const uint32_t i0 = ti * kPT + wi * 64 + 32 * qi + 4 * (lane >> 5), j = tj * kPT + wj * 64 + 32 * qj + (lane & 31);
+            if constexpr (kResult) {
+                float w[16];
+                if (p.step) tile_read(p.dst, p.rows, p.cols, mat, i0, j, w);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float o = acc[qi][qj][e] * p.unit;
+                    w[e] = p.step ? p.keep * w[e] - p.rate * o : o;
+                }
+                tile_write(p.dst, p.rows, p.cols, mat, i0, j, w);
+                continue;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const uint32_t i = i0 + 2 * r;  // four rows from here: registers r .. r + 3
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = acc[qi][qj][r + e];
+                if constexpr (KIND == kPolynomial) {
+                    const f16* g = p.gram.at(mat, j, i);
+                    const f16x4 gh = *reinterpret_cast<const f16x4*>(g), gl = *reinterpret_cast<const f16x4*>(g + 512);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        v[e] = p.cc * v[e] + p.cb * ((float)gh[e] + (float)gl[e]) + (i + e == j && j < p.m ? p.ca : 0.0f);
+                }
+                f16x4 hi, lo;
+                split4(v, KIND == kPolynomial ? 1.0f : p.unit, hi, lo);
+                (KIND == kUpdate ? p.out_t : p.out).put(mat, j, i, hi, lo);
+                if (KIND == kUpdate || ti != tj)
+                    p.out.put(mat, i + (lane & 3), j & ~3u, quad_transpose(hi), quad_transpose(lo));
+            }
+        }
+}
+
+}  // namespace dev
+}  // namespace mg
