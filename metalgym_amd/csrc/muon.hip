@@ -139,7 +139,9 @@ struct Workspace {
     Workspace(uint32_t count, uint32_t rows, uint32_t cols) {
         m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
         mp = pad(m), np = pad(n);
-        const size_t wide = (size_t)count * mp * np * 4, square = (size_t)count * mp * mp * 4;
+        // X by rows of np, its transpose by rows of mp
+        const size_t wide = dev::planes_block(np) * (mp / 32) * 2 * count, tall = dev::planes_block(mp) * (np / 32) * 2 * count;
+        const size_t square = dev::planes_block(mp) * (mp / 32) * 2 * count;
         total = 0;
         auto take = [&](size_t bytes) {
             const size_t at = total;
@@ -147,7 +149,7 @@ struct Workspace {
             return at;
         };
         norms = take((size_t)count * dev::kNormParts * 8);
-        x = take(wide), xt[0] = take(wide), xt[1] = take(wide);
+        x = take(wide), xt[0] = take(tall), xt[1] = take(tall);
         gram = take(square), product = take(square), poly = take(square), q[0] = take(square), q[1] = take(square);
     }
 };
@@ -227,7 +229,7 @@ int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, co
     const Workspace w(count, src.rows, src.cols);
     char* const base = static_cast<char*>(workspace);
     auto planes = [&](size_t at, uint32_t rows, uint32_t k) {
-        return dev::Planes{reinterpret_cast<dev::f16*>(base + at), (size_t)rows * k * 2, k / 16};
+        return dev::Planes{reinterpret_cast<dev::f16*>(base + at), dev::planes_block(k) * (rows / 32), dev::planes_block(k)};
     };
     double* const norms = reinterpret_cast<double*>(base + w.norms);
     const dev::Planes X = planes(w.x, w.mp, w.np);
@@ -245,7 +247,7 @@ int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, co
                        ns.eps, kUnitX, X, XT[0]);
     MG_HIP(hipGetLastError(), "newton-schulz split launch");
 
-    const dim3 half(mt * (mt + 1) / 2, count), full(mt * nt, count), block(256);
+    const dim3 half(mt * (mt + 1) / 2, count), full(mt * nt, count), block(512);
     dev::ProductArgs p{};
     p.m = w.m;
     // out = a b' of symmetric results

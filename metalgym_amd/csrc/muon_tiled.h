@@ -89,14 +89,20 @@ __device__ __forceinline__ float source_scale(const double* partial, uint32_t pa
     return *red;
 }
 
-// A matrix of pairs: kb blocks of 16 contraction elements for each 32 rows.
+// A matrix of pairs: every 32 rows' blocks of 16 contraction elements, and 4 KB
+// more. Tiles read the same stage of all their rows at once; without the extra 4 KB
+// those lie a power of two apart, in the same few memory channels (2048 x 2048 x 2048
+// in 60 us instead of SKEWED).
+constexpr uint32_t kSkew = 2048;  // elements
+__host__ __device__ __forceinline__ size_t planes_block(uint32_t k) { return (size_t)k * 64 + kSkew; }
 struct Planes {
     f16* base;
     size_t stride;  // elements between matrices of the batch
-    uint32_t kb;
+    size_t block;   // and between 32 rows
+
     // columns c ... of row r of matrix k: c a multiple of 4; the low halves 512 further
     __device__ __forceinline__ f16* at(uint32_t k, uint32_t r, uint32_t c) const {
-        return base + k * stride + ((size_t)(r >> 5) * kb + (c >> 4)) * 1024 + ((c & 8) << 5) + ((r & 31) << 3) + (c & 4);
+        return base + k * stride + (r >> 5) * block + (c >> 4) * 1024 + ((c & 8) << 5) + ((r & 31) << 3) + (c & 4);
     }
     __device__ __forceinline__ void put(uint32_t k, uint32_t r, uint32_t c, f16x4 hi, f16x4 lo) const {
         f16* const to = at(k, r, c);
@@ -161,15 +167,16 @@ __device__ __forceinline__ uint32_t xcd_run(uint32_t b, uint32_t count) {
     return x * each + (x < more ? x : more) + (b >> 3);
 }
 
-// One 128 x 128 tile of a product a b' of pairs. Four waves, 64 x 64 each as 2 x 2
-// tiles of v_mfma_f32_32x32x16_f16. Stages of 32 contraction elements (32 KB) go from
-// memory straight to a ring of four in LDS. In the middle of a stage, with its second
-// half already in registers, the waves meet once: the next stage has then arrived
-// (vmcnt counts in order, 8 loads a wave and stage), this stage's place is free for
-// the fourth one on, and the next stage's first fragments are read under the second
-// half's products.
+// One 128 x 128 tile of a product a b' of pairs. Eight waves, 64 x 64 each as 2 x 2
+// tiles of v_mfma_f32_32x32x16_f16: four of them take the first half of each stage's
+// 32 contraction elements, four the second, and the two halves' sums meet at the end.
+// So each SIMD has two waves, and one's waits are under the other's products. Stages
+// (32 KB) go from memory straight to a ring of four in LDS. The waves meet once a
+// stage: the next one has then arrived (vmcnt counts in order, 4 loads a wave and
+// stage), this one is in registers and its place free for the fourth one on, and the
+// next one's fragments are read under this one's products.
 template <int KIND>
-__global__ void __launch_bounds__(256) product_kernel(const ProductArgs p) {
+__global__ void __launch_bounds__(512) product_kernel(const ProductArgs p) {
     constexpr bool kResult = KIND >= kFinal, kSwap = KIND == kFinalTall;
     constexpr int kStage = 4 * kPT * kPK;  // elements: a and b, two planes each
     __shared__ __align__(1024) f16 lds[kRing * kStage];
@@ -186,71 +193,69 @@ __global__ void __launch_bounds__(256) product_kernel(const ProductArgs p) {
         ti = tile % tiles_i, tj = tile / tiles_i;
     }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    // wave w brings 32 rows of a and of b: 4 KB a stage each
-    const f16* from_a = p.a.base + mat * p.a.stride + (size_t)(ti * 4 + wave) * p.a.kb * 1024 + lane * 8;
-    const f16* from_b = p.b.base + mat * p.b.stride + (size_t)(tj * 4 + wave) * p.b.kb * 1024 + lane * 8;
-    auto load = [&](uint32_t stage) {
-        f16* to = lds + (stage & (kRing - 1)) * kStage + wave * 2048;
+    // waves 0 .. 3 bring 32 rows of a each, the others of b: 4 KB a stage
+    const int quarter = wave & 3, half = wave >> 2;
+    const Planes& src = half ? p.b : p.a;
+    const f16* from = src.base + mat * src.stride + ((half ? tj : ti) * 4 + quarter) * src.block + lane * 8;
+    auto load = [&](int slot, bool more) {
+        f16* to = lds + slot * kStage + wave * 2048;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from_a + c * 512),
+        for (int c = 0; c < 4; ++c)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + c * 512),
                                              (__attribute__((address_space(3))) void*)(to + c * 512), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from_b + c * 512),
-                                             (__attribute__((address_space(3))) void*)(to + 8192 + c * 512), 16, 0, 0);
-        }
-        from_a += 2048, from_b += 2048;
+        from += more ? 2048 : 0;
     };
-    const int wi = wave >> 1, wj = wave & 1;
-    f16x8 fa[2][2][2], fb[2][2][2];  // [half of a stage][32 rows][plane]
-    auto read = [&](uint32_t stage, int kk) {
-        const f16* at = lds + (stage & (kRing - 1)) * kStage + kk * 1024 + lane * 8;
+    const int wi = quarter >> 1, wj = quarter & 1;
+    const f16* const mine = lds + half * 1024 + lane * 8;
+    f16x8 fa[2][2][2], fb[2][2][2];  // [stages in turn][32 rows][plane]
+    auto read = [&](int slot) {
+        const f16* at = mine + slot * kStage;
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                fa[kk][q][h] = *reinterpret_cast<const f16x8*>(at + (2 * wi + q) * 2048 + h * 512);
-                fb[kk][q][h] = *reinterpret_cast<const f16x8*>(at + 8192 + (2 * wj + q) * 2048 + h * 512);
+                fa[slot & 1][q][h] = *reinterpret_cast<const f16x8*>(at + (2 * wi + q) * 2048 + h * 512);
+                fb[slot & 1][q][h] = *reinterpret_cast<const f16x8*>(at + 8192 + (2 * wj + q) * 2048 + h * 512);
             }
     };
     f32x16 acc[2][2] = {}, sum[2][2];
-    auto multiply = [&](int kk, bool fresh) {
-#pragma unroll
-        for (int term = 0; term < 3; ++term)  // lo hi, hi lo, hi hi; kSwap: the bits of the other product
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                        fa[kk][i][term == (kSwap ? 1 : 0)], fb[kk][j][term == (kSwap ? 0 : 1)], fresh && term == 0 ? f32x16{} : sum[i][j], 0, 0, 0);
-    };
-    auto meet = [&](bool tail) {
-        if (tail)
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    };
     const uint32_t stages = p.stages;
-    load(0), load(1), load(2);
-    meet(false);
-    load(3);
-    read(0, 0);
-    for (uint32_t s = 0; s < stages; s += 2) {
 #pragma unroll
-        for (int odd = 0; odd < 2; ++odd) {  // a chain of two stages
-            const uint32_t now = s + odd;
-            read(now, 1);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(0, odd == 0);
-            __builtin_amdgcn_sched_barrier(0);
-            if (now + 1 < stages) {
-                meet(now + 3 >= stages);
-                if (now + 4 < stages) load(now + 4);
-                read(now + 1, 0);
+    for (int u = 0; u < kRing; ++u) load(u, u + 1 < kRing || stages > kRing);
+    asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(0);
+    for (uint32_t s = 0; s < stages; s += kRing) {  // a chain
+#pragma unroll
+        for (int u = 0; u < kRing; ++u) {
+            asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            // past the last stage both repeat what is there, and nothing uses it
+            read((u + 1) & (kRing - 1));
+            load(u, s + u + kRing + 1 < stages);
+#pragma unroll
+            for (int term = 0; term < 3; ++term)  // lo hi, hi lo, hi hi; kSwap: the bits of the other product
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                            fa[u & 1][i][term == (kSwap ? 1 : 0)], fb[u & 1][j][term == (kSwap ? 0 : 1)],
+                            u == 0 && term == 0 ? f32x16{} : sum[i][j], 0, 0, 0);
+            // the reads and loads go between the products: issued before them, the
+            // eight waves' reads keep LDS busy for 512 cycles in which nothing is multiplied
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
             }
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(1, false);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // memory read
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -258,42 +263,53 @@ __global__ void __launch_bounds__(256) product_kernel(const ProductArgs p) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) acc[i][j] += sum[i][j];
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last loads have left LDS alone
+    // each wave keeps 32 of its rows and gives the other 32 to its partner
+    __syncthreads();
+    f32x16* const trade = reinterpret_cast<f32x16*>(lds);
 #pragma unroll
-    for (int qi = 0; qi < 2; ++qi)
+    for (int qj = 0; qj < 2; ++qj) trade[(wave * 2 + qj) * 64 + lane] = half ? acc[0][qj] : acc[1][qj];
+    __syncthreads();
+    f32x16 got[2];
 #pragma unroll
-        for (int qj = 0; qj < 2; ++qj) {
-            const uint32_t i0 = ti * kPT + wi * 64 + 32 * qi + 4 * (lane >> 5), j = tj * kPT + wj * 64 + 32 * qj + (lane & 31);
-            if constexpr (kResult) {
-                float w[16];
-                if (p.step) tile_read(p.dst, p.rows, p.cols, mat, i0, j, w);
+    for (int qj = 0; qj < 2; ++qj) {
+        const f32x16 theirs = trade[((wave ^ 4) * 2 + qj) * 64 + lane];
+        got[qj] = half ? theirs + acc[1][qj] : acc[0][qj] + theirs;
+    }
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float o = acc[qi][qj][e] * p.unit;
-                    w[e] = p.step ? p.keep * w[e] - p.rate * o : o;
-                }
-                tile_write(p.dst, p.rows, p.cols, mat, i0, j, w);
-                continue;
+    for (int qj = 0; qj < 2; ++qj) {
+        const uint32_t i0 = ti * kPT + wi * 64 + 32 * half + 4 * (lane >> 5), j = tj * kPT + wj * 64 + 32 * qj + (lane & 31);
+        if constexpr (kResult) {
+            float w[16];
+            if (p.step) tile_read(p.dst, p.rows, p.cols, mat, i0, j, w);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float o = got[qj][e] * p.unit;
+                w[e] = p.step ? p.keep * w[e] - p.rate * o : o;
             }
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const uint32_t i = i0 + 2 * r;  // four rows from here: registers r .. r + 3
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[qi][qj][r + e];
-                if constexpr (KIND == kPolynomial) {
-                    const f16* g = p.gram.at(mat, j, i);
-                    const f16x4 gh = *reinterpret_cast<const f16x4*>(g), gl = *reinterpret_cast<const f16x4*>(g + 512);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        v[e] = p.cc * v[e] + p.cb * ((float)gh[e] + (float)gl[e]) + (i + e == j && j < p.m ? p.ca : 0.0f);
-                }
-                f16x4 hi, lo;
-                split4(v, KIND == kPolynomial ? 1.0f : p.unit, hi, lo);
-                (KIND == kUpdate ? p.out_t : p.out).put(mat, j, i, hi, lo);
-                if (KIND == kUpdate || ti != tj)
-                    p.out.put(mat, i + (lane & 3), j & ~3u, quad_transpose(hi), quad_transpose(lo));
-            }
+            tile_write(p.dst, p.rows, p.cols, mat, i0, j, w);
+            continue;
         }
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const uint32_t i = i0 + 2 * r;  // four rows from here: registers r .. r + 3
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = got[qj][r + e];
+            if constexpr (KIND == kPolynomial) {
+                const f16* g = p.gram.at(mat, j, i);
+                const f16x4 gh = *reinterpret_cast<const f16x4*>(g), gl = *reinterpret_cast<const f16x4*>(g + 512);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[e] = p.cc * v[e] + p.cb * ((float)gh[e] + (float)gl[e]) + (i + e == j && j < p.m ? p.ca : 0.0f);
+            }
+            f16x4 hi, lo;
+            split4(v, KIND == kPolynomial ? 1.0f : p.unit, hi, lo);
+            (KIND == kUpdate ? p.out_t : p.out).put(mat, j, i, hi, lo);
+            if (KIND == kUpdate || ti != tj)
+                p.out.put(mat, i + (lane & 3), j & ~3u, quad_transpose(hi), quad_transpose(lo));
+        }
+    }
 }
 
 }  // namespace dev
