@@ -36,7 +36,16 @@ using dev::kUnitP;
 using dev::kUnitX;
 
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
-uint32_t pad(uint32_t x) { return (x + dev::kPT - 1) / dev::kPT * dev::kPT; }
+uint32_t pad(uint32_t x, uint32_t to) { return (x + to - 1) / to * to; }
+
+// Edge of the product tiles: 128 where the batch's symmetric products, which are most
+// of the launches, then have a tile for every second CU. Under that 64, whose products
+// do half as well per CU but have four times as many tiles: 1000 x 257 237 us on 128,
+// 146 on 64.
+uint32_t tile_edge(uint32_t count, uint32_t m) {
+    const uint64_t t = (m + 127) / 128;
+    return count * t * (t + 1) / 2 >= 128 ? 128 : 64;
+}
 
 // Steps of the next segment of the `left` that remain. On X for small matrices,
 // where a rounding error of A does not average out, and for polynomials that grow
@@ -135,10 +144,11 @@ int check_same(const char* what, const mg_matrices* a, const mg_matrices* b) {
 // The workspace of a batch.
 struct Workspace {
     size_t norms, x, xt[2], gram, product, poly, q[2], total;  // byte offsets
-    uint32_t m, n, mp, np;
+    uint32_t m, n, mp, np, tile;
     Workspace(uint32_t count, uint32_t rows, uint32_t cols) {
         m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
-        mp = pad(m), np = pad(n);
+        tile = tile_edge(count, m);
+        mp = pad(m, tile), np = pad(n, tile);
         // X by rows of np, its transpose by rows of mp
         const size_t wide = dev::planes_block(np) * (mp / 32) * 2 * count, tall = dev::planes_block(mp) * (np / 32) * 2 * count;
         const size_t square = dev::planes_block(mp) * (mp / 32) * 2 * count;
@@ -209,24 +219,9 @@ int newton_schulz_short(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
     return MG_OK;
 }
 
-int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, const dev::SourceArgs& src,
-                  const FinalArgs& fin, void* workspace) {
-    if (is_short(src.rows, src.cols)) {
-        const ShortWorkspace w(count, src.rows, src.cols);
-        char* const base = static_cast<char*>(workspace);
-        dev::ShortArgs a{};
-        a.src = src, a.slabs = w.slabs, a.parts = w.parts;
-        a.xt = reinterpret_cast<dev::f16*>(base + w.xt);
-        a.partial = reinterpret_cast<float*>(base + w.partial);
-        a.q = reinterpret_cast<dev::f16*>(base + w.q);
-        a.state = reinterpret_cast<dev::ShortState*>(base + w.state);
-        a.eps = ns.eps, a.a = ns.a, a.b = ns.b, a.c = ns.c;
-        a.dst = fin.dst, a.step = fin.step, a.keep = fin.keep, a.rate = fin.rate, a.odd_rate = fin.odd_rate;
-        return w.mp == 32   ? newton_schulz_short<32>(st, ns, count, a)
-               : w.mp == 64 ? newton_schulz_short<64>(st, ns, count, a)
-                            : newton_schulz_short<128>(st, ns, count, a);
-    }
-    const Workspace w(count, src.rows, src.cols);
+template <int T>
+int newton_schulz_tiled(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, const dev::SourceArgs& src,
+                        const FinalArgs& fin, const Workspace& w, void* workspace) {
     char* const base = static_cast<char*>(workspace);
     auto planes = [&](size_t at, uint32_t rows, uint32_t k) {
         return dev::Planes{reinterpret_cast<dev::f16*>(base + at), dev::planes_block(k) * (rows / 32), dev::planes_block(k)};
@@ -239,7 +234,7 @@ int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, co
     const dev::Planes Q[2] = {planes(w.q[0], w.mp, w.mp), planes(w.q[1], w.mp, w.mp)};
     const uint32_t tiles = ((src.rows + 63) / 64) * ((src.cols + 63) / 64);
     const uint32_t parts = tiles < (uint32_t)dev::kNormParts ? tiles : dev::kNormParts;
-    const uint32_t mt = w.mp / dev::kPT, nt = w.np / dev::kPT;
+    const uint32_t mt = w.mp / T, nt = w.np / T;
     hipLaunchKernelGGL(dev::source_norm_kernel, dim3(parts, count), dim3(256), 0, st, src, norms);
     MG_HIP(hipGetLastError(), "newton-schulz norm launch");
     const bool tall = src.rows > src.cols;
@@ -255,14 +250,14 @@ int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, co
                          const dev::Planes& out, float unit_out) -> int {
         p.a = a, p.b = b, p.stages = k / dev::kPK, p.tiles_j = mt, p.out = out;
         p.unit = unit_out / (unit_a * unit_b);
-        hipLaunchKernelGGL((dev::product_kernel<dev::kSymmetric>), half, block, 0, st, p);
+        hipLaunchKernelGGL((dev::product_kernel<dev::kSymmetric, T>), half, block, 0, st, p);
         MG_HIP(hipGetLastError(), "newton-schulz product launch");
         return MG_OK;
     };
     auto polynomial = [&](const dev::Planes& out) -> int {
         p.a = p.b = p.gram = gram, p.stages = w.mp / dev::kPK, p.tiles_j = mt, p.out = out;
         p.ca = ns.a * kUnitP, p.cb = ns.b * (kUnitP / kUnitA), p.cc = ns.c * (kUnitP / (kUnitA * kUnitA));
-        hipLaunchKernelGGL((dev::product_kernel<dev::kPolynomial>), half, block, 0, st, p);
+        hipLaunchKernelGGL((dev::product_kernel<dev::kPolynomial, T>), half, block, 0, st, p);
         MG_HIP(hipGetLastError(), "newton-schulz polynomial launch");
         return MG_OK;
     };
@@ -289,7 +284,7 @@ int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, co
         p.a = Q[q], p.b = XT[cur], p.stages = w.mp / dev::kPK, p.tiles_j = nt;
         if (left) {
             p.out = X, p.out_t = XT[cur ^ 1], p.unit = 1.0f / unit_q;
-            hipLaunchKernelGGL((dev::product_kernel<dev::kUpdate>), full, block, 0, st, p);
+            hipLaunchKernelGGL((dev::product_kernel<dev::kUpdate, T>), full, block, 0, st, p);
             MG_HIP(hipGetLastError(), "newton-schulz update launch");
             cur ^= 1;
         } else {
@@ -297,14 +292,36 @@ int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, co
             p.unit = 1.0f / (unit_q * kUnitX);
             if (tall) {
                 p.a = XT[cur], p.b = Q[q], p.tiles_j = mt;
-                hipLaunchKernelGGL((dev::product_kernel<dev::kFinalTall>), full, block, 0, st, p);
+                hipLaunchKernelGGL((dev::product_kernel<dev::kFinalTall, T>), full, block, 0, st, p);
             } else {
-                hipLaunchKernelGGL((dev::product_kernel<dev::kFinal>), full, block, 0, st, p);
+                hipLaunchKernelGGL((dev::product_kernel<dev::kFinal, T>), full, block, 0, st, p);
             }
             MG_HIP(hipGetLastError(), "newton-schulz result launch");
         }
     }
     return MG_OK;
+}
+
+int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, const dev::SourceArgs& src,
+                  const FinalArgs& fin, void* workspace) {
+    if (is_short(src.rows, src.cols)) {
+        const ShortWorkspace w(count, src.rows, src.cols);
+        char* const base = static_cast<char*>(workspace);
+        dev::ShortArgs a{};
+        a.src = src, a.slabs = w.slabs, a.parts = w.parts;
+        a.xt = reinterpret_cast<dev::f16*>(base + w.xt);
+        a.partial = reinterpret_cast<float*>(base + w.partial);
+        a.q = reinterpret_cast<dev::f16*>(base + w.q);
+        a.state = reinterpret_cast<dev::ShortState*>(base + w.state);
+        a.eps = ns.eps, a.a = ns.a, a.b = ns.b, a.c = ns.c;
+        a.dst = fin.dst, a.step = fin.step, a.keep = fin.keep, a.rate = fin.rate, a.odd_rate = fin.odd_rate;
+        return w.mp == 32   ? newton_schulz_short<32>(st, ns, count, a)
+               : w.mp == 64 ? newton_schulz_short<64>(st, ns, count, a)
+                            : newton_schulz_short<128>(st, ns, count, a);
+    }
+    const Workspace w(count, src.rows, src.cols);
+    return w.tile == 128 ? newton_schulz_tiled<128>(st, ns, count, src, fin, w, workspace)
+                         : newton_schulz_tiled<64>(st, ns, count, src, fin, w, workspace);
 }
 
 // The configuration's own checks; *ns receives the iteration.

@@ -60,28 +60,31 @@ __device__ __forceinline__ void with_type(uint32_t type, F&& f) {
         default: return f(f16{});
     }
 }
-// A lane's 16 elements of a 32 x 32 tile as the matrix instructions leave them:
+// A lane's N = 16 elements of a 32 x 32 tile as the matrix instructions leave them, or
+// 8 of 16 rows:
 // element e lies 8 (e / 4) + e % 4 rows under y0, in column x, if the matrix (rows x
 // cols) reaches there.
+template <int N>
 __device__ __forceinline__ void tile_read(const Batch& b, uint32_t rows, uint32_t cols, uint32_t k, uint32_t y0,
-                                          uint32_t x, float (&w)[16]) {
+                                          uint32_t x, float (&w)[N]) {
     with_type(b.type, [&](auto t) {
         const auto* from = static_cast<const decltype(t)*>(b.data) + b.at(k, 0, x < cols ? x : 0);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < N; ++e) {
             const uint32_t y = y0 + 2 * (e & ~3) + (e & 3);
             w[e] = (float)from[(uint64_t)(y < rows ? y : rows - 1) * b.ld];
         }
     });
 }
+template <int N>
 __device__ __forceinline__ void tile_write(const Batch& b, uint32_t rows, uint32_t cols, uint32_t k, uint32_t y0,
-                                           uint32_t x, const float (&w)[16]) {
+                                           uint32_t x, const float (&w)[N]) {
     if (x >= cols) return;
     with_type(b.type, [&](auto t) {
         using T = decltype(t);
         T* const to = static_cast<T*>(b.data) + b.at(k, 0, x);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < N; ++e) {
             const uint32_t y = y0 + 2 * (e & ~3) + (e & 3);
             if (y < rows) to[(uint64_t)y * b.ld] = (T)w[e];
         }

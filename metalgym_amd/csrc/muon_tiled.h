@@ -1,5 +1,6 @@
 // Newton-Schulz steps of matrices whose sides are both over 128: one launch a
-// product of 128 x 128 tiles, half the tiles of symmetric results.
+// product of 128 x 128 tiles, or 64 x 64 where those are too few for the chip; half
+// the tiles of symmetric results.
 //
 // Operands are pairs in the order of the matrix instructions' operands (Frags of
 // muon_short.h): a tile's stage is contiguous runs of 4 KB that go to LDS as they
@@ -11,7 +12,6 @@
 namespace mg {
 namespace dev {
 
-constexpr int kPT = 128;  // edge of a product tile; both sides are padded to it
 constexpr int kPK = 32;   // contraction elements of a stage
 constexpr int kRing = 4;  // stages in LDS
 constexpr int kNormParts = 1024;  // most partial sums of a matrix's squares
@@ -91,8 +91,8 @@ __device__ __forceinline__ float source_scale(const double* partial, uint32_t pa
 
 // A matrix of pairs: every 32 rows' blocks of 16 contraction elements, and 4 KB
 // more. Tiles read the same stage of all their rows at once; without the extra 4 KB
-// those lie a power of two apart, in the same few memory channels (2048 x 2048 x 2048
-// in 60 us instead of SKEWED).
+// those lie a power of two apart, in the same few memory channels (the product of 2048
+// x 8192 with itself: 250 us without, 203 with).
 constexpr uint32_t kSkew = 2048;  // elements
 __host__ __device__ __forceinline__ size_t planes_block(uint32_t k) { return (size_t)k * 64 + kSkew; }
 struct Planes {
@@ -167,18 +167,27 @@ __device__ __forceinline__ uint32_t xcd_run(uint32_t b, uint32_t count) {
     return x * each + (x < more ? x : more) + (b >> 3);
 }
 
-// One 128 x 128 tile of a product a b' of pairs. Eight waves, 64 x 64 each as 2 x 2
+// One T x T tile of a product a b' of pairs. Eight waves, T / 2 x T / 2 each as
 // tiles of v_mfma_f32_32x32x16_f16: four of them take the first half of each stage's
 // 32 contraction elements, four the second, and the two halves' sums meet at the end.
 // So each SIMD has two waves, and one's waits are under the other's products. Stages
-// (32 KB) go from memory straight to a ring of four in LDS. The waves meet once a
-// stage: the next one has then arrived (vmcnt counts in order, 4 loads a wave and
-// stage), this one is in registers and its place free for the fourth one on, and the
-// next one's fragments are read under this one's products.
-template <int KIND>
+// (32 KB at T = 128) go from memory straight to a ring of four in LDS. The waves meet
+// once a stage: the next one has then arrived (vmcnt counts in order), this one is in
+// registers and its place free for the fourth one on, and the next one's fragments
+// are read under this one's products. At T = 128 a stage takes 1150 cycles, of which
+// 768 are matrix instructions.
+template <int T>
+struct Tiling {
+    static constexpr int Q = T / 64;                // 32 x 32 tiles of a wave, along each side
+    static constexpr int kStage = 4 * T * kPK;      // elements: a and b, two planes each
+    static constexpr int kLoads = kStage / 512 / 8;  // of a wave and stage, 1 KB each
+    static constexpr int kChain = T == 128 ? 4 : 2;  // stages; a contraction's are a multiple of it
+};
+template <int KIND, int T>
 __global__ void __launch_bounds__(512) product_kernel(const ProductArgs p) {
+    using G = Tiling<T>;
+    constexpr int Q = G::Q, kStage = G::kStage, L = G::kLoads;
     constexpr bool kResult = KIND >= kFinal, kSwap = KIND == kFinalTall;
-    constexpr int kStage = 4 * kPT * kPK;  // elements: a and b, two planes each
     __shared__ __align__(1024) f16 lds[kRing * kStage];
     const uint32_t mat = blockIdx.y, tile = xcd_run(blockIdx.x, gridDim.x);
     uint32_t ti, tj;
@@ -193,97 +202,114 @@ __global__ void __launch_bounds__(512) product_kernel(const ProductArgs p) {
         ti = tile % tiles_i, tj = tile / tiles_i;
     }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    // waves 0 .. 3 bring 32 rows of a each, the others of b: 4 KB a stage
+    // a stage's 32-row blocks (4 KB), a's first, go to the waves in order: a block each
+    // at T = 128, half of one at 64
     const int quarter = wave & 3, half = wave >> 2;
+    const int block = quarter * L / 4, part = quarter * L % 4;
     const Planes& src = half ? p.b : p.a;
-    const f16* from = src.base + mat * src.stride + ((half ? tj : ti) * 4 + quarter) * src.block + lane * 8;
+    const f16* from = src.base + mat * src.stride + ((half ? tj : ti) * (T / 32) + block) * src.block + part * 512 + lane * 8;
     auto load = [&](int slot, bool more) {
-        f16* to = lds + slot * kStage + wave * 2048;
+        f16* to = lds + slot * kStage + wave * L * 512;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < L; ++c)
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + c * 512),
                                              (__attribute__((address_space(3))) void*)(to + c * 512), 16, 0, 0);
         from += more ? 2048 : 0;
     };
     const int wi = quarter >> 1, wj = quarter & 1;
     const f16* const mine = lds + half * 1024 + lane * 8;
-    f16x8 fa[2][2][2], fb[2][2][2];  // [stages in turn][32 rows][plane]
-    auto read = [&](int slot) {
+    f16x8 fa[2][Q][2], fb[2][Q][2];  // [stages in turn][32 rows][plane]
+    auto read = [&](int set, int slot) {
         const f16* at = mine + slot * kStage;
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
+        for (int q = 0; q < Q; ++q)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                fa[slot & 1][q][h] = *reinterpret_cast<const f16x8*>(at + (2 * wi + q) * 2048 + h * 512);
-                fb[slot & 1][q][h] = *reinterpret_cast<const f16x8*>(at + 8192 + (2 * wj + q) * 2048 + h * 512);
+                fa[set][q][h] = *reinterpret_cast<const f16x8*>(at + (Q * wi + q) * 2048 + h * 512);
+                fb[set][q][h] = *reinterpret_cast<const f16x8*>(at + kStage / 2 + (Q * wj + q) * 2048 + h * 512);
             }
     };
-    f32x16 acc[2][2] = {}, sum[2][2];
+    f32x16 acc[Q][Q] = {}, sum[Q][Q];
     const uint32_t stages = p.stages;
 #pragma unroll
-    for (int u = 0; u < kRing; ++u) load(u, u + 1 < kRing || stages > kRing);
-    asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+    for (uint32_t u = 0; u < (uint32_t)kRing; ++u) load(u, u + 1 < stages);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kRing - 1) * L) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    read(0);
-    for (uint32_t s = 0; s < stages; s += kRing) {  // a chain
+    read(0, 0);
+    for (uint32_t s = 0; s < stages; s += G::kChain) {
 #pragma unroll
-        for (int u = 0; u < kRing; ++u) {
-            asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+        for (int u = 0; u < G::kChain; ++u) {
+            const int slot = G::kChain == kRing ? u : (s + u) & (kRing - 1);
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kRing - 2) * L) : "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
             // past the last stage both repeat what is there, and nothing uses it
-            read((u + 1) & (kRing - 1));
-            load(u, s + u + kRing + 1 < stages);
+            read((u + 1) & 1, (slot + 1) & (kRing - 1));
+            load(slot, s + u + kRing + 1 < stages);
 #pragma unroll
             for (int term = 0; term < 3; ++term)  // lo hi, hi lo, hi hi; kSwap: the bits of the other product
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < Q; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
+                    for (int j = 0; j < Q; ++j)
                         sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
                             fa[u & 1][i][term == (kSwap ? 1 : 0)], fb[u & 1][j][term == (kSwap ? 0 : 1)],
                             u == 0 && term == 0 ? f32x16{} : sum[i][j], 0, 0, 0);
             // the reads and loads go between the products: issued before them, the
             // eight waves' reads keep LDS busy for 512 cycles in which nothing is multiplied
+            if constexpr (T == 128) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
-            }
+                for (int k = 0; k < 8; ++k) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
+                }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // memory read
+                for (int k = 0; k < 4; ++k) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // memory read
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < Q; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) acc[i][j] += sum[i][j];
+            for (int j = 0; j < Q; ++j) acc[i][j] += sum[i][j];
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last loads have left LDS alone
-    // each wave keeps 32 of its rows and gives the other 32 to its partner
+    // The halves' sums. A wave of two by two tiles keeps the rows of one tile and gives
+    // the others to its partner; of one tile, registers 8 half .. 8 half + 7.
     __syncthreads();
-    f32x16* const trade = reinterpret_cast<f32x16*>(lds);
+    constexpr int N = Q == 2 ? 16 : 8;  // registers of a tile that a wave ends up with
+    float* const trade = reinterpret_cast<float*>(lds);
+    float got[2][N];
+    auto keep = [&](int qj, int e, bool other) -> float {
+        if constexpr (Q == 2) return (half != 0) != other ? acc[1][qj][e] : acc[0][qj][e];
+        return (half != 0) != other ? acc[0][0][8 + e] : acc[0][0][e];
+    };
 #pragma unroll
-    for (int qj = 0; qj < 2; ++qj) trade[(wave * 2 + qj) * 64 + lane] = half ? acc[0][qj] : acc[1][qj];
+    for (int qj = 0; qj < Q; ++qj)
+#pragma unroll
+        for (int e = 0; e < N; ++e) trade[((wave * Q + qj) * N + e) * 64 + lane] = keep(qj, e, true);
     __syncthreads();
-    f32x16 got[2];
 #pragma unroll
-    for (int qj = 0; qj < 2; ++qj) {
-        const f32x16 theirs = trade[((wave ^ 4) * 2 + qj) * 64 + lane];
-        got[qj] = half ? theirs + acc[1][qj] : acc[0][qj] + theirs;
-    }
+    for (int qj = 0; qj < Q; ++qj)
 #pragma unroll
-    for (int qj = 0; qj < 2; ++qj) {
-        const uint32_t i0 = ti * kPT + wi * 64 + 32 * half + 4 * (lane >> 5), j = tj * kPT + wj * 64 + 32 * qj + (lane & 31);
+        for (int e = 0; e < N; ++e) {
+            const float theirs = trade[(((wave ^ 4) * Q + qj) * N + e) * 64 + lane], own = keep(qj, e, false);
+            got[qj][e] = half ? theirs + own : own + theirs;
+        }
+#pragma unroll
+    for (int qj = 0; qj < Q; ++qj) {
+        // register e of got lies 8 (e / 4) + e % 4 rows under i0
+        const uint32_t i0 = ti * T + wi * (T / 2) + (Q == 2 ? 32 : 16) * half + 4 * (lane >> 5);
+        const uint32_t j = tj * T + wj * (T / 2) + 32 * qj + (lane & 31);
         if constexpr (kResult) {
-            float w[16];
+            float w[N];
             if (p.step) tile_read(p.dst, p.rows, p.cols, mat, i0, j, w);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
+            for (int e = 0; e < N; ++e) {
                 const float o = got[qj][e] * p.unit;
                 w[e] = p.step ? p.keep * w[e] - p.rate * o : o;
             }
@@ -291,7 +317,7 @@ __global__ void __launch_bounds__(512) product_kernel(const ProductArgs p) {
             continue;
         }
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
+        for (int r = 0; r < N; r += 4) {
             const uint32_t i = i0 + 2 * r;  // four rows from here: registers r .. r + 3
             float v[4];
 #pragma unroll
