@@ -208,7 +208,7 @@ int newton_schulz_short(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
         if (a.steps == 2) most *= step_bounds(ns, &reach);
         a.unit_q = a.steps == 1 ? kUnitP : unit_of(most);
         left -= a.steps;
-        hipLaunchKernelGGL((dev::short_square_kernel<MP>), dim3(count), dim3(64 * Shape::NB * Shape::NB), 0, st, a);
+        hipLaunchKernelGGL((dev::short_square_kernel<MP>), dim3(count), dim3(64 * Shape::SW), 0, st, a);
         MG_HIP(hipGetLastError(), "newton-schulz square launch");
         if (left)
             hipLaunchKernelGGL((dev::short_update_kernel<MP, false>), slabs, block, 0, st, a);

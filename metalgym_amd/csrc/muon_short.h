@@ -3,7 +3,7 @@
 // one workgroup's LDS, and a launch for each product would be all latency.
 //
 // Launches of a batch: `first` once, then for each segment of one or two steps
-// `square` and `update`. X is cut into slabs of 128 columns.
+// `square` and `update`. X is cut into slabs of 64 columns.
 //  first:  X's slabs from the source (with the momentum's update) as pairs, each
 //          workgroup at its own exponent, and the slabs' part of X X'.
 //  square: one workgroup a matrix adds the parts to A (the first time its trace is
@@ -21,8 +21,8 @@
 namespace mg {
 namespace dev {
 
-constexpr int kSlab = 128;      // columns of a slab
-constexpr int kShortParts = 16;  // most workgroups that share a matrix's slabs
+constexpr int kSlab = 64;       // columns of a slab
+constexpr int kShortParts = 8;   // most workgroups that share a matrix's slabs
 constexpr int kMostExp = 120;    // exponent of a slab of zeros, or of next to nothing
 
 // Pairs in the order of the matrix instructions' operands, in LDS and in memory: a
@@ -86,7 +86,7 @@ struct ShortState {
 struct ShortArgs {
     SourceArgs src;
     uint32_t slabs, parts;
-    f16* xt;        // [count][slabs] X transposed: 128 columns of X by MP, Frags<MP>
+    f16* xt;        // [count][slabs] X transposed: a slab's columns of X by MP, Frags<MP>
     float* partial;  // [count][parts][tiles][16][64] X X' on and under the diagonal, in register order
     f16* q;         // [count] MP x MP, Frags<MP>
     ShortState* state;  // [count]
@@ -120,7 +120,10 @@ __device__ __forceinline__ void short_tile(int t, int& bi, int& bj) {
 template <int MP>
 struct ShortShape {
     static constexpr int NB = MP / 32, TILES = NB * (NB + 1) / 2;  // of 32 x 32, on and under the diagonal
-    static constexpr int W = 4 * NB < 8 ? 4 * NB : 8;  // waves over a slab's four column blocks
+    static constexpr int CB = kSlab / 32;               // column blocks of a slab
+    static constexpr int W = CB * NB < 8 ? CB * NB : 8;  // waves over a slab's column and row blocks
+    static constexpr int SJ = 1;         // square: tiles of a wave, side by side
+    static constexpr int SW = NB * NB / SJ;              // and waves
     static constexpr int NT = 64 * W, PER = MP * kSlab / NT;  // elements of a slab a thread
     static constexpr int THREADS = 64 * (W > TILES ? W : TILES);  // first and update: a wave a tile of X X'
     static constexpr int SQ = 2 * MP * MP, SLAB = 2 * MP * kSlab;  // elements of a pair of planes
@@ -149,25 +152,24 @@ __device__ __forceinline__ f32x16 short_product(const f16* x, const f16* y, int 
     return v;
 }
 
-// The slab's part of X X' (rows in LDS as pairs), a wave a tile, into this
-// workgroup's partial sums; added to those of its slabs before unless `first`.
+// Adds the slab's part of X X' (rows in LDS as pairs) to the wave's tile of it.
 template <int MP>
-__device__ __forceinline__ void short_gram(const ShortArgs& a, uint32_t mat, const f16* rows, bool first) {
-    using S = ShortShape<MP>;
-    const int lane = threadIdx.x & 63, t = threadIdx.x >> 6;
-    if (t >= S::TILES) return;
+__device__ __forceinline__ void short_gram(const f16* rows, f32x16& gram) {
+    const int t = threadIdx.x >> 6;
+    if (t >= ShortShape<MP>::TILES) return;
     int bi, bj;
     short_tile(t, bi, bj);
-    f32x16 v = short_product<kSlab>(rows, rows, bi, bj);
-    float* out = a.partial + (((size_t)mat * a.parts + blockIdx.x) * S::TILES + t) * 1024 + lane;
-    if (!first) {
-        f32x16 old;
+    gram += short_product<kSlab>(rows, rows, bi, bj);
+}
+// The workgroup's partial sums, in register order.
+template <int MP>
+__device__ __forceinline__ void short_gram_store(const ShortArgs& a, uint32_t mat, const f32x16& gram) {
+    using S = ShortShape<MP>;
+    const int t = threadIdx.x >> 6;
+    if (t >= S::TILES) return;
+    float* out = a.partial + (((size_t)mat * a.parts + blockIdx.x) * S::TILES + t) * 1024 + (threadIdx.x & 63);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) old[r] = out[r * 64];
-        v += old;
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) out[r * 64] = v[r];
+    for (int r = 0; r < 16; ++r) out[r * 64] = gram[r];
 }
 
 __device__ __forceinline__ float magnitude(float x) {
@@ -270,6 +272,7 @@ __global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_first_kernel(co
     }
     const float unit = ldexpf(1.0f, e);
     if (t == 0) a.state[mat].exp[blockIdx.x] = e;
+    f32x16 gram = {};
 #pragma unroll 1
     for (uint32_t s = blockIdx.x; s < a.slabs; s += a.parts) {
         if (a.slabs > a.parts) {  // else the only slab is still held
@@ -293,63 +296,69 @@ __global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_first_kernel(co
                 }
             }
         __syncthreads();
-        short_gram<MP>(a, mat, rows, s == blockIdx.x);
+        short_gram<MP>(rows, gram);
     }
+    short_gram_store<MP>(a, mat, gram);
 }
 
-// One workgroup a matrix, a wave a tile: A from the partial products (the waves on
-// and under the diagonal), then the segment's steps. Two matrices in LDS are enough
-// for two steps: A and P, then B = P A over A, A' = B P over B, P' over A', and Q =
-// P P'. A wave's four consecutive results lie in one column, and are kept as four of
-// a row, so what is kept is the product's transpose: in this order A' = P A P keeps
-// its symmetry under rounding (with P P A an error of A grows up to threefold).
+// One workgroup a matrix, the tiles spread over its waves: A from the partial products
+// (the tiles on and under the diagonal), then the segment's steps. Two matrices in LDS
+// are enough for two steps: A and P, then B = P A over A, A' = B P over B, P' over A',
+// and Q = P P'. A wave's four consecutive results lie in one column, and are kept as
+// four of a row, so what is kept is the product's transpose: in this order A' = P A P
+// keeps its symmetry under rounding (with P P A an error of A grows up to threefold).
+// At m = 128 a wave holds two tiles side by side: with one each, sixteen waves read
+// 512 KB of LDS a product, 4096 cycles for 3072 of matrix instructions.
 template <int MP>
-__global__ void __launch_bounds__(64 * ShortShape<MP>::NB * ShortShape<MP>::NB) short_square_kernel(const ShortArgs a) {
+__global__ void __launch_bounds__(64 * ShortShape<MP>::SW) short_square_kernel(const ShortArgs a) {
     using S = ShortShape<MP>;
     using F = Frags<MP>;
+    constexpr int SJ = S::SJ;
     __shared__ __align__(16) f16 lds[2][S::SQ];
-    __shared__ float wtrace[S::NB * S::NB];
+    __shared__ float wtrace[S::SW];
     const uint32_t mat = blockIdx.x;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     ShortState& state = a.state[mat];
     int least = kMostExp;
-    // the lower tiles spread over the SIMDs (wave % 4)
-    const int bi = wave / S::NB, bj = (wave - bi) & (S::NB - 1);
-    const bool lower = bi >= bj;
-    const int i0 = 32 * bi + 4 * (lane >> 5), j0 = 32 * bj + (lane & 31);
+    const int bi = wave / (S::NB / SJ), bj = wave % (S::NB / SJ) * SJ;
+    const int i0 = 32 * bi + 4 * (lane >> 5), j0 = 32 * bj + (lane & 31);  // and 32 on for the second tile
     if (a.start)
         for (uint32_t p = 0; p < a.parts; ++p) least = state.exp[p] < least ? state.exp[p] : least;
-    f32x16 v = {};
-    const float* in = a.partial + ((size_t)mat * a.parts * S::TILES + bi * (bi + 1) / 2 + bj) * 1024 + lane;
+    f32x16 v[SJ] = {};
+#pragma unroll
+    for (int u = 0; u < SJ; ++u) {
+        if (bi < bj + u) continue;
+        const float* in = a.partial + ((size_t)mat * a.parts * S::TILES + bi * (bi + 1) / 2 + bj + u) * 1024 + lane;
 #pragma unroll 1
-    for (uint32_t p0 = 0; p0 < (lower ? a.parts : 0); p0 += 4) {  // four parts in flight
-        float x[4][16];
+        for (uint32_t p0 = 0; p0 < a.parts; p0 += 4) {  // four parts in flight
+            float x[4][16];
 #pragma unroll
-        for (uint32_t p = 0; p < 4; ++p) {
-            const float* from = in + (size_t)(p0 + p < a.parts ? p0 + p : p0) * S::TILES * 1024;
+            for (uint32_t p = 0; p < 4; ++p) {
+                const float* from = in + (size_t)(p0 + p < a.parts ? p0 + p : p0) * S::TILES * 1024;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x[p][r] = from[r * 64];
-        }
+                for (int r = 0; r < 16; ++r) x[p][r] = from[r * 64];
+            }
 #pragma unroll
-        for (uint32_t p = 0; p < 4; ++p) {
-            const float f = p0 + p >= a.parts ? 0.0f
-                            : a.start         ? ldexpf(1.0f, 2 * (least - state.exp[p0 + p]))
-                                              : 1.0f;
-            if (f != 0.0f)
+            for (uint32_t p = 0; p < 4; ++p) {
+                if (p0 + p >= a.parts) continue;
+                const float f = a.start ? ldexpf(1.0f, 2 * (least - state.exp[p0 + p])) : 1.0f;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) v[r] += f * x[p][r];
+                for (int r = 0; r < 16; ++r) v[u][r] += f * x[p][r];
+            }
         }
     }
     float to_out = kUnitA / (kUnitX * kUnitX);
     if (a.start) {
         float trace = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) trace += bi == bj && c32_row(r, lane) == (lane & 31) ? v[r] : 0.0f;
+        for (int u = 0; u < SJ; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) trace += bi == bj + u && c32_row(r, lane) == (lane & 31) ? v[u][r] : 0.0f;
         trace = group_sum<64>(trace);
         if (lane == 0) wtrace[wave] = trace;
         __syncthreads();
         trace = 0.0f;
-        for (int w = 0; w < S::NB * S::NB; ++w) trace += wtrace[w];
+        for (int w = 0; w < S::SW; ++w) trace += wtrace[w];
         const float scale = 1.0f / (sqrtf(trace) + a.eps * ldexpf(1.0f, least));
         if (threadIdx.x == 0) state.least = least, state.scale = scale;
         to_out = scale * scale * kUnitA;
@@ -364,34 +373,61 @@ __global__ void __launch_bounds__(64 * ShortShape<MP>::NB * ShortShape<MP>::NB) 
         if (op >= 0) {
             const f16* x = lds[op == 2];
             const f16* y = lds[op == 1 || op == 4];
-            v = short_product<MP>(x, y, bi, bj);
+            // the fragments of a step are read while the one before is multiplied
+            f16x8 fa[2][2], fb[2][SJ][2];
+            auto read = [&](int kk) {
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    fa[kk & 1][p] = F::frag(x, p, bi, kk);
+#pragma unroll
+                    for (int u = 0; u < SJ; ++u) fb[kk & 1][u][p] = F::frag(y, p, bj + u, kk);
+                }
+            };
+            read(0);
+            f32x16 s[SJ];
+#pragma unroll
+            for (int kk = 0; kk < MP / 16; ++kk) {
+                if (kk + 1 < MP / 16) read(kk + 1);
+#pragma unroll
+                for (int u = 0; u < SJ; ++u) {
+                    s[u] = pair_mfma(fa[kk & 1], fb[kk & 1][u], kk & 1 ? s[u] : f32x16{});
+                    if (kk == 1)
+                        v[u] = s[u];
+                    else if (kk & 1)
+                        v[u] += s[u];
+                }
+            }
             to_out = op == 1 || op == 2 ? 1.0f / kUnitP : 1.0f;
             if (op == last) to_out = a.unit_q / (op == 4 ? kUnitP * kUnitP : kUnitP);
             if (op == 0 || op == 3) {  // a I + b A + c (A A), at kUnitP
                 const float cc = a.c * (kUnitP / (kUnitA * kUnitA)), cb = a.b * (kUnitP / kUnitA);
 #pragma unroll
-                for (int r = 0; r < 16; r += 4) {
-                    const int i = i0 + 2 * r;
-                    const f16* from = lds[0] + F::at(0, j0, i);
-                    const f16x4 hi = *reinterpret_cast<const f16x4*>(from);
-                    const f16x4 lo = *reinterpret_cast<const f16x4*>(from + 512);
+                for (int u = 0; u < SJ; ++u)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        v[r + e] = cc * v[r + e] + cb * ((float)hi[e] + (float)lo[e]) +
-                                   (i + e == j0 ? a.a * kUnitP : 0.0f);
-                }
+                    for (int r = 0; r < 16; r += 4) {
+                        const int i = i0 + 2 * r, j = j0 + 32 * u;
+                        const f16* from = lds[0] + F::at(0, j, i);
+                        const f16x4 hi = *reinterpret_cast<const f16x4*>(from);
+                        const f16x4 lo = *reinterpret_cast<const f16x4*>(from + 512);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            v[u][r + e] = cc * v[u][r + e] + cb * ((float)hi[e] + (float)lo[e]) +
+                                          (i + e == j ? a.a * kUnitP : 0.0f);
+                    }
             }
             __syncthreads();  // every wave has read what this goes over
         }
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const float w[4] = {v[r], v[r + 1], v[r + 2], v[r + 3]};
-            const int i = i0 + 2 * r;
-            f16x4 hi, lo;
-            split4(w, to_out, hi, lo);
-            if (op >= 0 || lower) F::put(out, j0, i, hi, lo);
-            if (op < 0 && bi > bj) F::put(out, i + (lane & 3), j0 & ~3, quad_transpose(hi), quad_transpose(lo));
-        }
+        for (int u = 0; u < SJ; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const float w[4] = {v[u][r], v[u][r + 1], v[u][r + 2], v[u][r + 3]};
+                const int i = i0 + 2 * r, j = j0 + 32 * u;
+                f16x4 hi, lo;
+                split4(w, to_out, hi, lo);
+                if (op >= 0 || bi >= bj + u) F::put(out, j, i, hi, lo);
+                if (op < 0 && bi > bj + u) F::put(out, i + (lane & 3), j & ~3, quad_transpose(hi), quad_transpose(lo));
+            }
         __syncthreads();
     }
 }
@@ -409,7 +445,7 @@ __global__ void __launch_bounds__(FINAL ? ShortShape<MP>::NT : ShortShape<MP>::T
     const uint32_t mat = blockIdx.y;
     const ShortArgs a = args.of(mat);
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 31, h = lane >> 5;
-    const int jb = wave & 3;  // the wave's 32 columns of the slab
+    const int jb = wave % S::CB;  // the wave's 32 columns of the slab
     f16x8 x[MP / 16][2];
     auto load_x = [&](uint32_t s) {
         const f16* xt = a.xt + ((size_t)mat * a.slabs + s) * S::SLAB;
@@ -435,6 +471,7 @@ __global__ void __launch_bounds__(FINAL ? ShortShape<MP>::NT : ShortShape<MP>::T
     if (a.start) f = state.scale * ldexpf(1.0f, state.least - state.exp[blockIdx.x]) / a.unit_q;
     if (!FINAL) f *= kUnitX;
     const bool tall = a.src.rows > a.src.cols;
+    f32x16 gram = {};
 #pragma unroll 1
     for (uint32_t s = blockIdx.x; s < a.slabs; s += a.parts) {
         f16* const xt = a.xt + ((size_t)mat * a.slabs + s) * S::SLAB;
@@ -457,7 +494,7 @@ __global__ void __launch_bounds__(FINAL ? ShortShape<MP>::NT : ShortShape<MP>::T
             return acc;
         };
 #pragma unroll 1
-        for (int b = wave / 4; wave < S::W && b < S::NB; b += S::W / 4) {
+        for (int b = wave / S::CB; wave < S::W && b < S::NB; b += S::W / S::CB) {
             if constexpr (FINAL) {
                 // tall: a lane holds row i of X, its registers columns j, which are dst's rows
                 const uint32_t along = s * kSlab + 32 * jb, across = 32 * b;
@@ -489,9 +526,10 @@ __global__ void __launch_bounds__(FINAL ? ShortShape<MP>::NT : ShortShape<MP>::T
         if (s + a.parts < a.slabs) load_x(s + a.parts);
         if constexpr (!FINAL) {
             __syncthreads();
-            short_gram<MP>(a, mat, rows, s == blockIdx.x);
+            short_gram<MP>(rows, gram);
         }
     }
+    if constexpr (!FINAL) short_gram_store<MP>(a, mat, gram);
 }
 
 }  // namespace dev
