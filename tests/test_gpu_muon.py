@@ -124,6 +124,16 @@ def test_in_place(mg, rows, cols):
     np.testing.assert_array_equal(run_orth(mg, g, in_place=True), run_orth(mg, g))
 
 
+@pytest.mark.parametrize("count,rows,cols", [(4, 1000, 1100), (4, 1100, 1000), (2, 1400, 2000), (9, 600, 1100)])
+def test_larger_batches(mg, count, rows, cols):
+    """Batches that take 128 x 128 tiles, with and without segments of two steps."""
+    g = decode(encode(gradients(np.random.RandomState(11), count, rows, cols, "strong"), "bf16"), "bf16")
+    got = run_orth(mg, g, "bf16", "fp32")
+    for k in {0, count - 1}:
+        check_orthogonal(got[k], g[k], "fp32")
+    np.testing.assert_array_equal(got, run_orth(mg, g, "bf16", "fp32"))
+
+
 def test_an_empty_batch_is_nothing(mg):
     mg.orthogonalize(mg.matrices(None, 0, 4, 4), mg.matrices(None, 0, 4, 4))
 
