@@ -164,20 +164,35 @@ struct Workspace {
     }
 };
 
+// Workgroups a matrix (muon_short.h). One fills a CU, so they run in rounds of 256, each
+// as long as a segment's steps, about 8 slabs' worth (17 us to 2.5), and its slabs: the
+// least product of the two, with fewer workgroups among equals. 300 x 128 x 4096 takes
+// 1570 us in 3 rounds with two each, 1851 in 2 rounds with one.
+uint32_t short_parts(uint32_t count, uint32_t slabs) {
+    uint32_t best = 1;
+    uint64_t least = ~0ull;
+    for (uint32_t p = 1; p <= (uint32_t)dev::kShortParts && p <= slabs; ++p) {
+        const uint64_t cost = (((uint64_t)count * p + 255) / 256) * (8 + (slabs + p - 1) / p);
+        if (cost < least) least = cost, best = p;
+    }
+    return best;
+}
+
 // The workspace of a batch whose short side is at most 128 (muon_short.h).
 struct ShortWorkspace {
-    size_t xt, partial, q, state, total;
+    size_t xt, partial[2], state, total;
     uint32_t mp, slabs, parts;
     ShortWorkspace(uint32_t count, uint32_t rows, uint32_t cols) {
         const uint32_t m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
         mp = m <= 32 ? 32 : m <= 64 ? 64 : 128;
         slabs = (n + dev::kSlab - 1) / dev::kSlab;
-        parts = slabs < (uint32_t)dev::kShortParts ? slabs : dev::kShortParts;
+        parts = short_parts(count, slabs);
         const uint32_t tiles = mp / 32 * (mp / 32 + 1) / 2;
         xt = 0;
-        partial = xt + align256((size_t)count * slabs * dev::kSlab * mp * 4);
-        q = partial + align256((size_t)count * parts * tiles * 4096);
-        state = q + align256((size_t)count * mp * mp * 4);
+        const size_t sums = align256((size_t)count * parts * tiles * 4096);
+        partial[0] = xt + align256((size_t)count * slabs * dev::kSlab * mp * 4);
+        partial[1] = partial[0] + sums;
+        state = partial[1] + sums;
         total = state + align256((size_t)count * sizeof(dev::ShortState));
     }
 };
@@ -194,11 +209,13 @@ struct FinalArgs {
 };
 
 template <int MP>
-int newton_schulz_short(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, dev::ShortArgs a) {
+int newton_schulz_short(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, dev::ShortArgs a, float* const (&partial)[2]) {
     const uint32_t m = a.src.rows < a.src.cols ? a.src.rows : a.src.cols;
     using Shape = dev::ShortShape<MP>;
-    const dim3 slabs(a.parts, count), block(Shape::THREADS);
-    hipLaunchKernelGGL((dev::short_first_kernel<MP>), slabs, block, 0, st, a);
+    const dim3 slabs(a.parts, count);
+    int to = 0;
+    a.partial = partial[to];
+    hipLaunchKernelGGL((dev::short_first_kernel<MP>), slabs, dim3(Shape::THREADS), 0, st, a);
     MG_HIP(hipGetLastError(), "newton-schulz first launch");
     double reach = 1.0;
     a.start = 1;
@@ -208,13 +225,12 @@ int newton_schulz_short(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
         if (a.steps == 2) most *= step_bounds(ns, &reach);
         a.unit_q = a.steps == 1 ? kUnitP : unit_of(most);
         left -= a.steps;
-        hipLaunchKernelGGL((dev::short_square_kernel<MP>), dim3(count), dim3(64 * Shape::SW), 0, st, a);
-        MG_HIP(hipGetLastError(), "newton-schulz square launch");
+        a.partial_in = partial[to], a.partial = partial[to ^= 1];
         if (left)
-            hipLaunchKernelGGL((dev::short_update_kernel<MP, false>), slabs, block, 0, st, a);
+            hipLaunchKernelGGL((dev::short_step_kernel<MP, false>), slabs, dim3(Shape::STEP), 0, st, a);
         else
-            hipLaunchKernelGGL((dev::short_update_kernel<MP, true>), slabs, dim3(Shape::NT), 0, st, a);
-        MG_HIP(hipGetLastError(), "newton-schulz update launch");
+            hipLaunchKernelGGL((dev::short_step_kernel<MP, true>), slabs, dim3(Shape::STEP), 0, st, a);
+        MG_HIP(hipGetLastError(), "newton-schulz step launch");
     }
     return MG_OK;
 }
@@ -310,14 +326,13 @@ int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, co
         dev::ShortArgs a{};
         a.src = src, a.slabs = w.slabs, a.parts = w.parts;
         a.xt = reinterpret_cast<dev::f16*>(base + w.xt);
-        a.partial = reinterpret_cast<float*>(base + w.partial);
-        a.q = reinterpret_cast<dev::f16*>(base + w.q);
+        float* const partial[2] = {reinterpret_cast<float*>(base + w.partial[0]), reinterpret_cast<float*>(base + w.partial[1])};
         a.state = reinterpret_cast<dev::ShortState*>(base + w.state);
         a.eps = ns.eps, a.a = ns.a, a.b = ns.b, a.c = ns.c;
         a.dst = fin.dst, a.step = fin.step, a.keep = fin.keep, a.rate = fin.rate, a.odd_rate = fin.odd_rate;
-        return w.mp == 32   ? newton_schulz_short<32>(st, ns, count, a)
-               : w.mp == 64 ? newton_schulz_short<64>(st, ns, count, a)
-                            : newton_schulz_short<128>(st, ns, count, a);
+        return w.mp == 32   ? newton_schulz_short<32>(st, ns, count, a, partial)
+               : w.mp == 64 ? newton_schulz_short<64>(st, ns, count, a, partial)
+                            : newton_schulz_short<128>(st, ns, count, a, partial);
     }
     const Workspace w(count, src.rows, src.cols);
     return w.tile == 128 ? newton_schulz_tiled<128>(st, ns, count, src, fin, w, workspace)

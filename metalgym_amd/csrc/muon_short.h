@@ -2,15 +2,16 @@
 // policy's block matrices are (128 x hidden): their symmetric m x m matrices fit
 // one workgroup's LDS, and a launch for each product would be all latency.
 //
-// Launches of a batch: `first` once, then for each segment of one or two steps
-// `square` and `update`. X is cut into slabs of 64 columns.
-//  first:  X's slabs from the source (with the momentum's update) as pairs, each
-//          workgroup at its own exponent, and the slabs' part of X X'.
-//  square: one workgroup a matrix adds the parts to A (the first time its trace is
-//          the squared norm, so no pass over X is spent on that), and takes the
-//          segment's steps to Q in LDS.
-//  update: X <- Q X slab by slab, and the slabs' part of the new X X', or at the
-//          end the result.
+// Launches of a batch: `first` once, then one `step` for each segment of one or two
+// steps. X is cut into slabs of 64 columns, shared by up to eight workgroups.
+//  first: X's slabs from the source (with the momentum's update) as pairs, each
+//         workgroup at its own exponent, and the slabs' part of X X'.
+//  step:  every workgroup of a matrix adds the parts to A (the first time its trace is
+//         the squared norm, so no pass over X is spent on that) and takes the segment's
+//         steps to Q in LDS, all of them the same; then X <- Q X on its slabs, and
+//         their part of the new X X', or at the end the result. The repeated work is on
+//         CUs that would be idle: with one workgroup a matrix doing it, in launches of
+//         its own, Q went through memory (2 x 512 x 128: 74.6 us, now 67.4; 1000 x 128 x 512: 1262, now 721).
 // Each kernel runs its code once or a few times, so what it costs is latencies: loads
 // are issued in batches, one wave holds one 32 x 32 tile, and code is kept in loops
 // (unrolled four waves' worth of tiles each, the same kernels spent 13 to 25 us
@@ -22,8 +23,8 @@ namespace mg {
 namespace dev {
 
 constexpr int kSlab = 64;       // columns of a slab
-constexpr int kShortParts = 8;   // most workgroups that share a matrix's slabs
-constexpr int kMostExp = 120;    // exponent of a slab of zeros, or of next to nothing
+constexpr int kShortParts = 8;  // most workgroups that share a matrix's slabs
+constexpr int kMostExp = 120;   // exponent of a slab of zeros, or of next to nothing
 
 // Pairs in the order of the matrix instructions' operands, in LDS and in memory: a
 // matrix of K columns (the contraction) is cut into 32 rows x 16 columns, each two
@@ -76,27 +77,25 @@ __device__ __forceinline__ f32x16 pair_mfma(const f16x8 (&a)[2], const f16x8 (&b
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[0], c, 0, 0, 0);
 }
 
-// Exponents and scale of a matrix's X while it is the source's own.
+// Exponents of a matrix's X while it is the source's own.
 struct ShortState {
     int exp[kShortParts];  // of each workgroup's slabs: pairs hold U 2^exp
-    int least;             // the least of them: A's unit before the norm is known
-    float scale;           // 2^-least / (|U| + eps)
 };
 
 struct ShortArgs {
     SourceArgs src;
     uint32_t slabs, parts;
     f16* xt;        // [count][slabs] X transposed: a slab's columns of X by MP, Frags<MP>
-    float* partial;  // [count][parts][tiles][16][64] X X' on and under the diagonal, in register order
-    f16* q;         // [count] MP x MP, Frags<MP>
+    // [count][parts][tiles][16][64] X X' on and under the diagonal, in register order. A
+    // step's workgroups read all of a matrix's and write their own of the next: two buffers.
+    const float* partial_in;
+    float* partial;
     ShortState* state;  // [count]
     float eps;
-    // square
     uint32_t start;  // the first segment
     uint32_t steps;  // 1 or 2
     float a, b, c;
     float unit_q;
-    // update
     Batch dst;
     uint32_t step;
     float keep, rate, odd_rate;  // odd_rate: of the odd matrices of a policy's blocks
@@ -122,10 +121,9 @@ struct ShortShape {
     static constexpr int NB = MP / 32, TILES = NB * (NB + 1) / 2;  // of 32 x 32, on and under the diagonal
     static constexpr int CB = kSlab / 32;               // column blocks of a slab
     static constexpr int W = CB * NB < 8 ? CB * NB : 8;  // waves over a slab's column and row blocks
-    static constexpr int SJ = 1;         // square: tiles of a wave, side by side
-    static constexpr int SW = NB * NB / SJ;              // and waves
     static constexpr int NT = 64 * W, PER = MP * kSlab / NT;  // elements of a slab a thread
-    static constexpr int THREADS = 64 * (W > TILES ? W : TILES);  // first and update: a wave a tile of X X'
+    static constexpr int THREADS = 64 * (W > TILES ? W : TILES);  // first: a wave a tile of X X'
+    static constexpr int STEP = 64 * (W > NB * NB ? W : NB * NB);  // step: a wave a tile of A
     static constexpr int SQ = 2 * MP * MP, SLAB = 2 * MP * kSlab;  // elements of a pair of planes
 };
 
@@ -301,231 +299,178 @@ __global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_first_kernel(co
     short_gram_store<MP>(a, mat, gram);
 }
 
-// One workgroup a matrix, the tiles spread over its waves: A from the partial products
-// (the tiles on and under the diagonal), then the segment's steps. Two matrices in LDS
-// are enough for two steps: A and P, then B = P A over A, A' = B P over B, P' over A',
-// and Q = P P'. A wave's four consecutive results lie in one column, and are kept as
-// four of a row, so what is kept is the product's transpose: in this order A' = P A P
+// Grid (parts, count). The segment's steps, a wave a tile. Two matrices in LDS are
+// enough for two steps: A and P, then B = P A over A, A' = B P over B, P' over A', and
+// Q = P P' over P'. A wave's four consecutive results lie in one column, and are kept
+// as four of a row, so what is kept is the product's transpose: in this order A' = P A P
 // keeps its symmetry under rounding (with P P A an error of A grows up to threefold).
-// At m = 128 a wave holds two tiles side by side: with one each, sixteen waves read
-// 512 KB of LDS a product, 4096 cycles for 3072 of matrix instructions.
-template <int MP>
-__global__ void __launch_bounds__(64 * ShortShape<MP>::SW) short_square_kernel(const ShortArgs a) {
+// A product is 1.7 us of LDS reads at m = 128; two tiles a wave read less, but their
+// code took longer to fetch than that saved.
+//
+// Then X' X = Q X as X' rows: a wave takes 32 columns of X by 32 rows of Q. The first
+// slab is on its way to LDS meanwhile. FINAL writes the result, in the orientation that
+// runs along dst's rows. Otherwise the new pairs replace the old in xt (each
+// workgroup's own slabs) and go to LDS in rows for the Gram product.
+template <int MP, bool FINAL>
+__global__ void __launch_bounds__(ShortShape<MP>::STEP) short_step_kernel(const ShortArgs args) {
     using S = ShortShape<MP>;
     using F = Frags<MP>;
-    constexpr int SJ = S::SJ;
-    __shared__ __align__(16) f16 lds[2][S::SQ];
-    __shared__ float wtrace[S::SW];
-    const uint32_t mat = blockIdx.x;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    ShortState& state = a.state[mat];
+    __shared__ __align__(1024) f16 lds[2][S::SQ > S::SLAB ? S::SQ : S::SLAB];  // at last the slab's rows too
+    __shared__ __align__(1024) f16 slab[S::SLAB];
+    const uint32_t mat = blockIdx.y;
+    const ShortArgs a = args.of(mat);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
+    auto load_slab = [&](uint32_t s) {
+        constexpr int KB = S::SLAB * 2 / 1024, W = S::STEP / 64;
+        const f16* from = a.xt + ((size_t)mat * a.slabs + s) * S::SLAB + lane * 8;
+#pragma unroll
+        for (int k = 0; k < (KB + W - 1) / W; ++k) {
+            const int c = wave + W * k;
+            if (c < KB)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + c * 512),
+                                                 (__attribute__((address_space(3))) void*)(slab + c * 512), 16, 0, 0);
+        }
+    };
+    load_slab(blockIdx.x);
+    const ShortState& state = a.state[mat];
     int least = kMostExp;
-    const int bi = wave / (S::NB / SJ), bj = wave % (S::NB / SJ) * SJ;
-    const int i0 = 32 * bi + 4 * (lane >> 5), j0 = 32 * bj + (lane & 31);  // and 32 on for the second tile
     if (a.start)
         for (uint32_t p = 0; p < a.parts; ++p) least = state.exp[p] < least ? state.exp[p] : least;
-    f32x16 v[SJ] = {};
-#pragma unroll
-    for (int u = 0; u < SJ; ++u) {
-        if (bi < bj + u) continue;
-        const float* in = a.partial + ((size_t)mat * a.parts * S::TILES + bi * (bi + 1) / 2 + bj + u) * 1024 + lane;
+    const int bi = wave / S::NB, bj = wave & (S::NB - 1);
+    const bool on = bi < S::NB, lower = on && bi >= bj;
+    const int i0 = 32 * bi + 4 * h, j0 = 32 * bj + r;
+    f32x16 v = {};
+    const float* in = a.partial_in + ((size_t)mat * a.parts * S::TILES + bi * (bi + 1) / 2 + bj) * 1024 + lane;
 #pragma unroll 1
-        for (uint32_t p0 = 0; p0 < a.parts; p0 += 4) {  // four parts in flight
-            float x[4][16];
+    for (uint32_t p0 = 0; p0 < (lower ? a.parts : 0); p0 += 4) {  // four parts in flight
+        float x[4][16];
 #pragma unroll
-            for (uint32_t p = 0; p < 4; ++p) {
-                const float* from = in + (size_t)(p0 + p < a.parts ? p0 + p : p0) * S::TILES * 1024;
+        for (uint32_t p = 0; p < 4; ++p) {
+            const float* from = in + (size_t)(p0 + p < a.parts ? p0 + p : p0) * S::TILES * 1024;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) x[p][r] = from[r * 64];
-            }
+            for (int e = 0; e < 16; ++e) x[p][e] = from[e * 64];
+        }
 #pragma unroll
-            for (uint32_t p = 0; p < 4; ++p) {
-                if (p0 + p >= a.parts) continue;
-                const float f = a.start ? ldexpf(1.0f, 2 * (least - state.exp[p0 + p])) : 1.0f;
+        for (uint32_t p = 0; p < 4; ++p) {
+            if (p0 + p >= a.parts) continue;
+            const float f = a.start ? ldexpf(1.0f, 2 * (least - state.exp[p0 + p])) : 1.0f;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) v[u][r] += f * x[p][r];
-            }
+            for (int e = 0; e < 16; ++e) v[e] += f * x[p][e];
         }
     }
     float to_out = kUnitA / (kUnitX * kUnitX);
+    float to_x = 1.0f / (a.unit_q * kUnitX);  // takes the exponents out of X Q
     if (a.start) {
+        float* const wtrace = reinterpret_cast<float*>(lds[1]);  // nothing else is there yet
         float trace = 0.0f;
 #pragma unroll
-        for (int u = 0; u < SJ; ++u)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) trace += bi == bj + u && c32_row(r, lane) == (lane & 31) ? v[u][r] : 0.0f;
+        for (int e = 0; e < 16; ++e) trace += on && bi == bj && c32_row(e, lane) == r ? v[e] : 0.0f;
         trace = group_sum<64>(trace);
         if (lane == 0) wtrace[wave] = trace;
         __syncthreads();
         trace = 0.0f;
-        for (int w = 0; w < S::SW; ++w) trace += wtrace[w];
+        for (int w = 0; w < S::STEP / 64; ++w) trace += wtrace[w];
+        __syncthreads();
+        // 2^-least / (|U| + eps)
         const float scale = 1.0f / (sqrtf(trace) + a.eps * ldexpf(1.0f, least));
-        if (threadIdx.x == 0) state.least = least, state.scale = scale;
         to_out = scale * scale * kUnitA;
+        to_x = scale * ldexpf(1.0f, least - state.exp[blockIdx.x]) / a.unit_q;
     }
-    f16* const q = a.q + (size_t)mat * S::SQ;
     // op -1 stores A; then the products of a segment, each of two of the matrices in
-    // LDS, over one of them or to Q
+    // LDS, over one of them; the last leaves Q
     const int last = a.steps == 2 ? 4 : 0;
 #pragma unroll 1
     for (int op = -1; op <= last; ++op) {
-        f16* const out = op == last ? q : lds[op == 0];
+        f16* const out = lds[op == 0];
         if (op >= 0) {
             const f16* x = lds[op == 2];
             const f16* y = lds[op == 1 || op == 4];
-            // the fragments of a step are read while the one before is multiplied
-            f16x8 fa[2][2], fb[2][SJ][2];
-            auto read = [&](int kk) {
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    fa[kk & 1][p] = F::frag(x, p, bi, kk);
-#pragma unroll
-                    for (int u = 0; u < SJ; ++u) fb[kk & 1][u][p] = F::frag(y, p, bj + u, kk);
-                }
-            };
-            read(0);
-            f32x16 s[SJ];
-#pragma unroll
-            for (int kk = 0; kk < MP / 16; ++kk) {
-                if (kk + 1 < MP / 16) read(kk + 1);
-#pragma unroll
-                for (int u = 0; u < SJ; ++u) {
-                    s[u] = pair_mfma(fa[kk & 1], fb[kk & 1][u], kk & 1 ? s[u] : f32x16{});
-                    if (kk == 1)
-                        v[u] = s[u];
-                    else if (kk & 1)
-                        v[u] += s[u];
-                }
-            }
+            if (on) v = short_product<MP>(x, y, bi, bj);
             to_out = op == 1 || op == 2 ? 1.0f / kUnitP : 1.0f;
             if (op == last) to_out = a.unit_q / (op == 4 ? kUnitP * kUnitP : kUnitP);
-            if (op == 0 || op == 3) {  // a I + b A + c (A A), at kUnitP
+            if (on && (op == 0 || op == 3)) {  // a I + b A + c (A A), at kUnitP
                 const float cc = a.c * (kUnitP / (kUnitA * kUnitA)), cb = a.b * (kUnitP / kUnitA);
 #pragma unroll
-                for (int u = 0; u < SJ; ++u)
+                for (int e = 0; e < 16; e += 4) {
+                    const int i = i0 + 2 * e;
+                    const f16* from = lds[0] + F::at(0, j0, i);
+                    const f16x4 hi = *reinterpret_cast<const f16x4*>(from);
+                    const f16x4 lo = *reinterpret_cast<const f16x4*>(from + 512);
 #pragma unroll
-                    for (int r = 0; r < 16; r += 4) {
-                        const int i = i0 + 2 * r, j = j0 + 32 * u;
-                        const f16* from = lds[0] + F::at(0, j, i);
-                        const f16x4 hi = *reinterpret_cast<const f16x4*>(from);
-                        const f16x4 lo = *reinterpret_cast<const f16x4*>(from + 512);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            v[u][r + e] = cc * v[u][r + e] + cb * ((float)hi[e] + (float)lo[e]) +
-                                          (i + e == j ? a.a * kUnitP : 0.0f);
-                    }
+                    for (int k = 0; k < 4; ++k)
+                        v[e + k] = cc * v[e + k] + cb * ((float)hi[k] + (float)lo[k]) +
+                                   (i + k == j0 ? a.a * kUnitP : 0.0f);
+                }
             }
             __syncthreads();  // every wave has read what this goes over
         }
+        if (on)
 #pragma unroll
-        for (int u = 0; u < SJ; ++u)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const float w[4] = {v[u][r], v[u][r + 1], v[u][r + 2], v[u][r + 3]};
-                const int i = i0 + 2 * r, j = j0 + 32 * u;
+            for (int e = 0; e < 16; e += 4) {
+                const float w[4] = {v[e], v[e + 1], v[e + 2], v[e + 3]};
+                const int i = i0 + 2 * e;
                 f16x4 hi, lo;
                 split4(w, to_out, hi, lo);
-                if (op >= 0 || bi >= bj + u) F::put(out, j, i, hi, lo);
-                if (op < 0 && bi > bj + u) F::put(out, i + (lane & 3), j & ~3, quad_transpose(hi), quad_transpose(lo));
+                if (op >= 0 || lower) F::put(out, j0, i, hi, lo);
+                if (op < 0 && bi > bj) F::put(out, i + (lane & 3), j0 & ~3, quad_transpose(hi), quad_transpose(lo));
             }
         __syncthreads();
     }
-}
-
-// Grid (parts, count): X <- Q X. A wave holds 32 columns of X, its fragments straight
-// from xt (two waves share them and split the rows of Q); Q is in LDS. FINAL writes
-// the result, in the orientation that runs along dst's rows. Otherwise the new pairs
-// replace the old in xt (each workgroup's own slabs) and go to LDS in rows for the
-// Gram product.
-template <int MP, bool FINAL>
-__global__ void __launch_bounds__(FINAL ? ShortShape<MP>::NT : ShortShape<MP>::THREADS) short_update_kernel(const ShortArgs args) {
-    using S = ShortShape<MP>;
-    __shared__ __align__(16) f16 q[S::SQ];
-    __shared__ __align__(16) f16 rows[FINAL ? 8 : S::SLAB];
-    const uint32_t mat = blockIdx.y;
-    const ShortArgs a = args.of(mat);
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 31, h = lane >> 5;
-    const int jb = wave % S::CB;  // the wave's 32 columns of the slab
-    f16x8 x[MP / 16][2];
-    auto load_x = [&](uint32_t s) {
-        const f16* xt = a.xt + ((size_t)mat * a.slabs + s) * S::SLAB;
-        if (wave < S::W)
-#pragma unroll
-            for (int kk = 0; kk < MP / 16; ++kk)
-#pragma unroll
-                for (int p = 0; p < 2; ++p) x[kk][p] = Frags<MP>::frag(xt, p, jb, kk);
-    };
-    if (t < S::NT) {
-        constexpr int PER = S::SQ / 8 / S::NT;  // all in flight at once
-        const f16* qin = a.q + (size_t)mat * S::SQ;
-        f16x8 part[PER];
-#pragma unroll
-        for (int k = 0; k < PER; ++k) part[k] = *reinterpret_cast<const f16x8*>(qin + (t + S::NT * k) * 8);
-        load_x(blockIdx.x);
-#pragma unroll
-        for (int k = 0; k < PER; ++k) *reinterpret_cast<f16x8*>(q + (t + S::NT * k) * 8) = part[k];
-    }
-    // takes the exponents out of X Q, and puts X's own in
-    const ShortState& state = a.state[mat];
-    float f = 1.0f / (a.unit_q * kUnitX);
-    if (a.start) f = state.scale * ldexpf(1.0f, state.least - state.exp[blockIdx.x]) / a.unit_q;
-    if (!FINAL) f *= kUnitX;
+    const f16* const q = lds[last == 0];
+    f16* const rows = lds[last != 0];
+    if (!FINAL) to_x *= kUnitX;
     const bool tall = a.src.rows > a.src.cols;
+    const int jb = wave % S::CB, b = wave / S::CB;  // the wave's columns of X and rows of Q
     f32x16 gram = {};
 #pragma unroll 1
     for (uint32_t s = blockIdx.x; s < a.slabs; s += a.parts) {
-        f16* const xt = a.xt + ((size_t)mat * a.slabs + s) * S::SLAB;
-        __syncthreads();  // Q is in place, the slab before has left the rows, and both waves of a column block hold X
-        // x y' of 32 x 32 in chains of 32, or its transpose
-        auto product = [&](int b, bool transpose) {
-            f32x16 acc = {};
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();  // the slab has arrived; the one before has left the rows
+        // tall: a lane holds row i of X, its registers columns j, which are dst's rows
+        const uint32_t along = s * kSlab + 32 * jb, across = 32 * b;
+        const uint32_t y0 = (FINAL && !tall ? across : along) + 4 * h, c = (FINAL && !tall ? along : across) + r;
+        float w[16];
+        f32x16 acc = {};
+        if (b < S::NB) {
+            if (FINAL && a.step) tile_read(a.dst, a.src.rows, a.src.cols, mat, y0, c, w);
+            // x y' of 32 x 32 in chains of 32, or its transpose
 #pragma unroll
             for (int kk = 0; kk < MP / 16; kk += 2) {
-                f32x16 c = {};
+                f32x16 t = {};
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    f16x8 y[2];
+                    f16x8 x[2], y[2];
 #pragma unroll
-                    for (int p = 0; p < 2; ++p) y[p] = Frags<MP>::frag(q, p, b, kk + e);
-                    c = transpose ? pair_mfma<true>(y, x[kk + e], c) : pair_mfma(x[kk + e], y, c);
+                    for (int p = 0; p < 2; ++p) x[p] = F::frag(slab, p, jb, kk + e), y[p] = F::frag(q, p, b, kk + e);
+                    t = FINAL && !tall ? pair_mfma<true>(y, x, t) : pair_mfma(x, y, t);
                 }
-                acc += c;
+                acc += t;
             }
-            return acc;
-        };
-#pragma unroll 1
-        for (int b = wave / S::CB; wave < S::W && b < S::NB; b += S::W / S::CB) {
-            if constexpr (FINAL) {
-                // tall: a lane holds row i of X, its registers columns j, which are dst's rows
-                const uint32_t along = s * kSlab + 32 * jb, across = 32 * b;
-                const uint32_t y0 = (tall ? along : across) + 4 * h, c = (tall ? across : along) + r;
-                float w[16];
-                if (a.step) tile_read(a.dst, a.src.rows, a.src.cols, mat, y0, c, w);
-                f32x16 acc;
-                if (tall)
-                    acc = product(b, false);
-                else
-                    acc = product(b, true);
+        }
+        if constexpr (FINAL) {
+            if (b < S::NB) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) w[e] = a.step ? a.keep * w[e] - a.rate * (acc[e] * f) : acc[e] * f;
+                for (int e = 0; e < 16; ++e) w[e] = a.step ? a.keep * w[e] - a.rate * (acc[e] * to_x) : acc[e] * to_x;
                 tile_write(a.dst, a.src.rows, a.src.cols, mat, y0, c, w);
-            } else {
-                const f32x16 acc = product(b, false);
+            }
+            __syncthreads();
+            if (s + a.parts < a.slabs) load_slab(s + a.parts);
+        } else {
+            if (b < S::NB) {
+                f16* const xt = a.xt + ((size_t)mat * a.slabs + s) * S::SLAB;
                 const int i = 32 * b + r;  // X'(i, j .. j + 3)
 #pragma unroll
                 for (int g = 0; g < 16; g += 4) {
-                    const float w[4] = {acc[g], acc[g + 1], acc[g + 2], acc[g + 3]};
+                    const float u[4] = {acc[g], acc[g + 1], acc[g + 2], acc[g + 3]};
                     const int j = 32 * jb + 2 * g + 4 * h;
                     f16x4 hi, lo;
-                    split4(w, f, hi, lo);
+                    split4(u, to_x, hi, lo);
                     Frags<kSlab>::put(rows, i, j, hi, lo);
-                    Frags<MP>::put(xt, j + (lane & 3), i & ~3, quad_transpose(hi), quad_transpose(lo));
+                    F::put(xt, j + (lane & 3), i & ~3, quad_transpose(hi), quad_transpose(lo));
                 }
             }
-        }
-        if (s + a.parts < a.slabs) load_x(s + a.parts);
-        if constexpr (!FINAL) {
             __syncthreads();
+            if (s + a.parts < a.slabs) load_slab(s + a.parts);
             short_gram<MP>(rows, gram);
         }
     }
