@@ -227,9 +227,9 @@ int newton_schulz_short(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
         left -= a.steps;
         a.partial_in = partial[to], a.partial = partial[to ^= 1];
         if (left)
-            hipLaunchKernelGGL((dev::short_step_kernel<MP, false>), slabs, dim3(Shape::STEP), 0, st, a);
+            hipLaunchKernelGGL((dev::short_step_kernel<MP, false>), slabs, dim3(Shape::THREADS), 0, st, a);
         else
-            hipLaunchKernelGGL((dev::short_step_kernel<MP, true>), slabs, dim3(Shape::STEP), 0, st, a);
+            hipLaunchKernelGGL((dev::short_step_kernel<MP, true>), slabs, dim3(Shape::THREADS), 0, st, a);
         MG_HIP(hipGetLastError(), "newton-schulz step launch");
     }
     return MG_OK;

@@ -122,8 +122,7 @@ struct ShortShape {
     static constexpr int CB = kSlab / 32;               // column blocks of a slab
     static constexpr int W = CB * NB < 8 ? CB * NB : 8;  // waves over a slab's column and row blocks
     static constexpr int NT = 64 * W, PER = MP * kSlab / NT;  // elements of a slab a thread
-    static constexpr int THREADS = 64 * (W > TILES ? W : TILES);  // first: a wave a tile of X X'
-    static constexpr int STEP = 64 * (W > NB * NB ? W : NB * NB);  // step: a wave a tile of A
+    static constexpr int THREADS = 64 * (W > TILES ? W : TILES);  // a wave a tile of a symmetric matrix
     static constexpr int SQ = 2 * MP * MP, SLAB = 2 * MP * kSlab;  // elements of a pair of planes
 };
 
@@ -312,7 +311,7 @@ __global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_first_kernel(co
 // runs along dst's rows. Otherwise the new pairs replace the old in xt (each
 // workgroup's own slabs) and go to LDS in rows for the Gram product.
 template <int MP, bool FINAL>
-__global__ void __launch_bounds__(ShortShape<MP>::STEP) short_step_kernel(const ShortArgs args) {
+__global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_step_kernel(const ShortArgs args) {
     using S = ShortShape<MP>;
     using F = Frags<MP>;
     __shared__ __align__(1024) f16 lds[2][S::SQ > S::SLAB ? S::SQ : S::SLAB];  // at last the slab's rows too
@@ -321,7 +320,7 @@ __global__ void __launch_bounds__(ShortShape<MP>::STEP) short_step_kernel(const 
     const ShortArgs a = args.of(mat);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
     auto load_slab = [&](uint32_t s) {
-        constexpr int KB = S::SLAB * 2 / 1024, W = S::STEP / 64;
+        constexpr int KB = S::SLAB * 2 / 1024, W = S::THREADS / 64;
         const f16* from = a.xt + ((size_t)mat * a.slabs + s) * S::SLAB + lane * 8;
 #pragma unroll
         for (int k = 0; k < (KB + W - 1) / W; ++k) {
@@ -336,13 +335,14 @@ __global__ void __launch_bounds__(ShortShape<MP>::STEP) short_step_kernel(const 
     int least = kMostExp;
     if (a.start)
         for (uint32_t p = 0; p < a.parts; ++p) least = state.exp[p] < least ? state.exp[p] : least;
-    const int bi = wave / S::NB, bj = wave & (S::NB - 1);
-    const bool on = bi < S::NB, lower = on && bi >= bj;
+    const bool on = wave < S::TILES;
+    int bi, bj;
+    short_tile(wave, bi, bj);
     const int i0 = 32 * bi + 4 * h, j0 = 32 * bj + r;
     f32x16 v = {};
-    const float* in = a.partial_in + ((size_t)mat * a.parts * S::TILES + bi * (bi + 1) / 2 + bj) * 1024 + lane;
+    const float* in = a.partial_in + ((size_t)mat * a.parts * S::TILES + wave) * 1024 + lane;
 #pragma unroll 1
-    for (uint32_t p0 = 0; p0 < (lower ? a.parts : 0); p0 += 4) {  // four parts in flight
+    for (uint32_t p0 = 0; p0 < (on ? a.parts : 0); p0 += 4) {  // four parts in flight
         float x[4][16];
 #pragma unroll
         for (uint32_t p = 0; p < 4; ++p) {
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(ShortShape<MP>::STEP) short_step_kernel(const 
         if (lane == 0) wtrace[wave] = trace;
         __syncthreads();
         trace = 0.0f;
-        for (int w = 0; w < S::STEP / 64; ++w) trace += wtrace[w];
+        for (int w = 0; w < S::THREADS / 64; ++w) trace += wtrace[w];
         __syncthreads();
         // 2^-least / (|U| + eps)
         const float scale = 1.0f / (sqrtf(trace) + a.eps * ldexpf(1.0f, least));
@@ -411,8 +411,8 @@ __global__ void __launch_bounds__(ShortShape<MP>::STEP) short_step_kernel(const 
                 const int i = i0 + 2 * e;
                 f16x4 hi, lo;
                 split4(w, to_out, hi, lo);
-                if (op >= 0 || lower) F::put(out, j0, i, hi, lo);
-                if (op < 0 && bi > bj) F::put(out, i + (lane & 3), j0 & ~3, quad_transpose(hi), quad_transpose(lo));
+                F::put(out, j0, i, hi, lo);
+                if (bi > bj) F::put(out, i + (lane & 3), j0 & ~3, quad_transpose(hi), quad_transpose(lo));
             }
         __syncthreads();
     }
