@@ -143,7 +143,7 @@ int check_same(const char* what, const mg_matrices* a, const mg_matrices* b) {
 
 // The workspace of a batch.
 struct Workspace {
-    size_t norms, x, xt[2], gram, product, poly, q[2], total;  // byte offsets
+    size_t norms, rest, x, xt[2], gram, product, poly, q[2], total;  // byte offsets
     uint32_t m, n, mp, np, tile;
     Workspace(uint32_t count, uint32_t rows, uint32_t cols) {
         m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
@@ -159,6 +159,7 @@ struct Workspace {
             return at;
         };
         norms = take((size_t)count * dev::kNormParts * 8);
+        rest = take((size_t)count * 4);
         x = take(wide), xt[0] = take(tall), xt[1] = take(tall);
         gram = take(square), product = take(square), poly = take(square), q[0] = take(square), q[1] = take(square);
     }
@@ -254,19 +255,29 @@ int newton_schulz_tiled(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
     hipLaunchKernelGGL(dev::source_norm_kernel, dim3(parts, count), dim3(256), 0, st, src, norms);
     MG_HIP(hipGetLastError(), "newton-schulz norm launch");
     const bool tall = src.rows > src.cols;
-    hipLaunchKernelGGL(dev::source_split_kernel, dim3((tall ? w.mp : w.np) / 64, (tall ? w.np : w.mp) / 64, count), dim3(256), 0, st, src, norms, parts,
-                       ns.eps, kUnitX, X, XT[0]);
+    // A 16-bit source fits the high halves: two products less for the first A, one for the
+    // first X' (2048 x 8192: 1583 us without, 1457 with).
+    bool exact = src.in.type != MG_TYPE_FP32 && !src.momentum.data && segment_steps(ns, w.m, w.n, ns.steps) < ns.steps;
+    float* const rest = reinterpret_cast<float*>(base + w.rest);
+    const dim3 tiles64((tall ? w.mp : w.np) / 64, (tall ? w.np : w.mp) / 64, count);
+    if (exact)
+        hipLaunchKernelGGL(dev::source_split_kernel<true>, tiles64, dim3(256), 0, st, src, norms, parts, ns.eps, rest, X, XT[0]);
+    else
+        hipLaunchKernelGGL(dev::source_split_kernel<false>, tiles64, dim3(256), 0, st, src, norms, parts, ns.eps, rest, X, XT[0]);
     MG_HIP(hipGetLastError(), "newton-schulz split launch");
 
     const dim3 half(mt * (mt + 1) / 2, count), full(mt * nt, count), block(512);
     dev::ProductArgs p{};
-    p.m = w.m;
+    p.m = w.m, p.rest = rest;
     // out = a b' of symmetric results
     auto symmetric = [&](const dev::Planes& a, const dev::Planes& b, uint32_t k, float unit_a, float unit_b,
                          const dev::Planes& out, float unit_out) -> int {
         p.a = a, p.b = b, p.stages = k / dev::kPK, p.tiles_j = mt, p.out = out;
         p.unit = unit_out / (unit_a * unit_b);
-        hipLaunchKernelGGL((dev::product_kernel<dev::kSymmetric, T>), half, block, 0, st, p);
+        if (a.base == X.base && exact)
+            hipLaunchKernelGGL((dev::product_kernel<dev::kExactGram, T>), half, block, 0, st, p);
+        else
+            hipLaunchKernelGGL((dev::product_kernel<dev::kSymmetric, T>), half, block, 0, st, p);
         MG_HIP(hipGetLastError(), "newton-schulz product launch");
         return MG_OK;
     };
@@ -300,7 +311,11 @@ int newton_schulz_tiled(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
         p.a = Q[q], p.b = XT[cur], p.stages = w.mp / dev::kPK, p.tiles_j = nt;
         if (left) {
             p.out = X, p.out_t = XT[cur ^ 1], p.unit = 1.0f / unit_q;
-            hipLaunchKernelGGL((dev::product_kernel<dev::kUpdate, T>), full, block, 0, st, p);
+            if (exact)
+                hipLaunchKernelGGL((dev::product_kernel<dev::kExactUpdate, T>), full, block, 0, st, p);
+            else
+                hipLaunchKernelGGL((dev::product_kernel<dev::kUpdate, T>), full, block, 0, st, p);
+            exact = false;  // X' is pairs
             MG_HIP(hipGetLastError(), "newton-schulz update launch");
             cur ^= 1;
         } else {

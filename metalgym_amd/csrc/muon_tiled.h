@@ -111,16 +111,26 @@ struct Planes {
     }
 };
 
-// U / (|U| + eps) times `unit` as pairs, X [mp][np] and its transpose XT [np][mp],
+// U / (|U| + eps) times kUnitX as pairs, X [mp][np] and its transpose XT [np][mp],
 // zeros in the padding; one 64 x 64 tile of the source a workgroup. A thread's
 // elements are a run along one of the two; the other takes four threads'.
+// EXACT: a power of two takes the place of the factor, so that a 16-bit source fits the
+// high halves (under 2^-27 of the norm to 2^-38 of it) and the low ones, which nothing
+// reads, are not written. rest[k] is what is left of the factor, in [1, 2).
+template <bool EXACT>
 __global__ void __launch_bounds__(256) source_split_kernel(const SourceArgs a, const double* partial, uint32_t parts,
-                                                           float eps, float unit, Planes X, Planes XT) {
+                                                           float eps, float* rest, Planes X, Planes XT) {
     __shared__ float red;
     const uint32_t k = blockIdx.z, i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
     float u[16];
     tile_load<false>(a, k, i0, j0, u);
-    const float scale = source_scale(partial + (size_t)k * parts, parts, eps, &red) * unit;
+    float scale = source_scale(partial + (size_t)k * parts, parts, eps, &red);
+    if constexpr (EXACT) {
+        const float factor = scale;
+        if (factor == factor) scale = ldexpf(1.0f, ilogbf(factor));
+        if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) rest[k] = factor / scale;
+    }
+    scale *= kUnitX;
     const bool tall = a.rows > a.cols;
     const Planes& by_column = tall ? X : XT;  // rows of it are the source's columns
     const Planes& by_row = tall ? XT : X;
@@ -130,16 +140,23 @@ __global__ void __launch_bounds__(256) source_split_kernel(const SourceArgs a, c
         const float x[4] = {u[e], u[e + 1], u[e + 2], u[e + 3]};
         f16x4 hi, lo;
         split4(x, scale, hi, lo);
-        by_column.put(k, j, i + e, hi, lo);
-        by_row.put(k, i + e + (threadIdx.x & 3), j & ~3u, quad_transpose(hi), quad_transpose(lo));
+        if constexpr (EXACT) {
+            *reinterpret_cast<f16x4*>(by_column.at(k, j, i + e)) = hi;
+            *reinterpret_cast<f16x4*>(by_row.at(k, i + e + (threadIdx.x & 3), j & ~3u)) = quad_transpose(hi);
+        } else {
+            by_column.put(k, j, i + e, hi, lo);
+            by_row.put(k, i + e + (threadIdx.x & 3), j & ~3u, quad_transpose(hi), quad_transpose(lo));
+        }
     }
 }
 
 // What becomes of a product's element v = (a b')(i, j).
 enum {
     kSymmetric = 0,  // out(i, j) = out(j, i) = v
+    kExactGram,      // the same of operands without low halves
     kPolynomial,     // the same with c v + b A(i, j) + a [i = j], v = (A A)(i, j)
     kUpdate,         // X' = v, both X [i][j] and XT [j][i]
+    kExactUpdate,    // the same where b, the old XT, has no low halves
     kFinal,          // the result of a wide matrix: dst(i, j) = v, or keep dst(i, j) - rate v
     kFinalTall,      // and of a tall one, whose product has a and b in each other's place
 };
@@ -148,6 +165,7 @@ struct ProductArgs {
     uint32_t stages;   // K / kPK, a multiple of 4
     uint32_t tiles_j;  // tile columns (symmetric results: tile rows and columns)
     float unit;        // takes the operands' exponents out of the sums and puts the result's in
+    const float* rest;  // kExact..: each matrix's factor of X
     Planes out, out_t;  // X [i][j] and XT [j][i], or a symmetric out
     // kPolynomial
     Planes gram;
@@ -180,14 +198,16 @@ template <int T>
 struct Tiling {
     static constexpr int Q = T / 64;                // 32 x 32 tiles of a wave, along each side
     static constexpr int kStage = 4 * T * kPK;      // elements: a and b, two planes each
-    static constexpr int kLoads = kStage / 512 / 8;  // of a wave and stage, 1 KB each
+    static constexpr int kBlocks = kStage / 512 / 8;  // of a wave and stage, 1 KB each
     static constexpr int kChain = T == 128 ? 4 : 2;  // stages; a contraction's are a multiple of it
 };
 template <int KIND, int T>
 __global__ void __launch_bounds__(512) product_kernel(const ProductArgs p) {
     using G = Tiling<T>;
-    constexpr int Q = G::Q, kStage = G::kStage, L = G::kLoads;
-    constexpr bool kResult = KIND >= kFinal, kSwap = KIND == kFinalTall;
+    // halves that a and b hold; of operands without low ones every second block is left alone
+    constexpr int HA = KIND == kExactGram ? 1 : 2, HB = KIND == kExactGram || KIND == kExactUpdate ? 1 : 2;
+    constexpr int Q = G::Q, kStage = G::kStage, B = G::kBlocks, L = KIND == kExactGram ? B / 2 : B;
+    constexpr bool kResult = KIND >= kFinal, kSwap = KIND == kFinalTall, kX = KIND == kUpdate || KIND == kExactUpdate;
     __shared__ __align__(1024) f16 lds[kRing * kStage];
     const uint32_t mat = blockIdx.y, tile = xcd_run(blockIdx.x, gridDim.x);
     uint32_t ti, tj;
@@ -205,13 +225,13 @@ __global__ void __launch_bounds__(512) product_kernel(const ProductArgs p) {
     // a stage's 32-row blocks (4 KB), a's first, go to the waves in order: a block each
     // at T = 128, half of one at 64
     const int quarter = wave & 3, half = wave >> 2;
-    const int block = quarter * L / 4, part = quarter * L % 4;
+    const int block = quarter * B / 4, part = quarter * B % 4;
     const Planes& src = half ? p.b : p.a;
     const f16* from = src.base + mat * src.stride + ((half ? tj : ti) * (T / 32) + block) * src.block + part * 512 + lane * 8;
     auto load = [&](int slot, bool more) {
-        f16* to = lds + slot * kStage + wave * L * 512;
+        f16* to = lds + slot * kStage + wave * B * 512;
 #pragma unroll
-        for (int c = 0; c < L; ++c)
+        for (int c = 0; c < B; c += B / L)
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + c * 512),
                                              (__attribute__((address_space(3))) void*)(to + c * 512), 16, 0, 0);
         from += more ? 2048 : 0;
@@ -225,8 +245,9 @@ __global__ void __launch_bounds__(512) product_kernel(const ProductArgs p) {
         for (int q = 0; q < Q; ++q)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                fa[set][q][h] = *reinterpret_cast<const f16x8*>(at + (Q * wi + q) * 2048 + h * 512);
-                fb[set][q][h] = *reinterpret_cast<const f16x8*>(at + kStage / 2 + (Q * wj + q) * 2048 + h * 512);
+                if (h < HA) fa[set][q][h] = *reinterpret_cast<const f16x8*>(at + (Q * wi + q) * 2048 + h * 512);
+                if (h < HB)
+                    fb[set][q][h] = *reinterpret_cast<const f16x8*>(at + kStage / 2 + (Q * wj + q) * 2048 + h * 512);
             }
     };
     f32x16 acc[Q][Q] = {}, sum[Q][Q];
@@ -248,24 +269,26 @@ __global__ void __launch_bounds__(512) product_kernel(const ProductArgs p) {
             read((u + 1) & 1, (slot + 1) & (kRing - 1));
             load(slot, s + u + kRing + 1 < stages);
 #pragma unroll
-            for (int term = 0; term < 3; ++term)  // lo hi, hi lo, hi hi; kSwap: the bits of the other product
+            for (int term = 0; term < 3; ++term) {  // lo hi, hi lo, hi hi; kSwap: the bits of the other product
+                if ((term == 0 && HA == 1) || (term == 1 && HB == 1)) continue;
 #pragma unroll
                 for (int i = 0; i < Q; ++i)
 #pragma unroll
                     for (int j = 0; j < Q; ++j)
                         sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
                             fa[u & 1][i][term == (kSwap ? 1 : 0)], fb[u & 1][j][term == (kSwap ? 0 : 1)],
-                            u == 0 && term == 0 ? f32x16{} : sum[i][j], 0, 0, 0);
+                            u == 0 && term == (HA == 1 ? 2 : 0) ? f32x16{} : sum[i][j], 0, 0, 0);
+            }
             // the reads and loads go between the products: issued before them, the
             // eight waves' reads keep LDS busy for 512 cycles in which nothing is multiplied
             if constexpr (T == 128) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
+                for (int k = 0; k < 2 * (HA + HB); ++k) {
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix
                     __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
                 }
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
+                for (int k = 0; k < L; ++k) {
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                     __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // memory read
                 }
@@ -282,6 +305,9 @@ __global__ void __launch_bounds__(512) product_kernel(const ProductArgs p) {
     // the others to its partner; of one tile, registers 8 half .. 8 half + 7.
     __syncthreads();
     constexpr int N = Q == 2 ? 16 : 8;  // registers of a tile that a wave ends up with
+    float unit = p.unit;
+    if constexpr (KIND == kExactGram) unit *= p.rest[mat] * p.rest[mat];
+    if constexpr (KIND == kExactUpdate) unit *= p.rest[mat];
     float* const trade = reinterpret_cast<float*>(lds);
     float got[2][N];
     auto keep = [&](int qj, int e, bool other) -> float {
@@ -310,7 +336,7 @@ __global__ void __launch_bounds__(512) product_kernel(const ProductArgs p) {
             if (p.step) tile_read(p.dst, p.rows, p.cols, mat, i0, j, w);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                const float o = got[qj][e] * p.unit;
+                const float o = got[qj][e] * unit;
                 w[e] = p.step ? p.keep * w[e] - p.rate * o : o;
             }
             tile_write(p.dst, p.rows, p.cols, mat, i0, j, w);
@@ -330,9 +356,9 @@ __global__ void __launch_bounds__(512) product_kernel(const ProductArgs p) {
                     v[e] = p.cc * v[e] + p.cb * ((float)gh[e] + (float)gl[e]) + (i + e == j && j < p.m ? p.ca : 0.0f);
             }
             f16x4 hi, lo;
-            split4(v, KIND == kPolynomial ? 1.0f : p.unit, hi, lo);
-            (KIND == kUpdate ? p.out_t : p.out).put(mat, j, i, hi, lo);
-            if (KIND == kUpdate || ti != tj)
+            split4(v, KIND == kPolynomial ? 1.0f : unit, hi, lo);
+            (kX ? p.out_t : p.out).put(mat, j, i, hi, lo);
+            if (kX || ti != tj)
                 p.out.put(mat, i + (lane & 3), j & ~3u, quad_transpose(hi), quad_transpose(lo));
         }
     }
