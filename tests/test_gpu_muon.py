@@ -134,6 +134,21 @@ def test_larger_batches(mg, count, rows, cols):
     np.testing.assert_array_equal(got, run_orth(mg, g, "bf16", "fp32"))
 
 
+@pytest.mark.parametrize("kind,powers", [("bf16", (110, 60, 0, -12)), ("fp16", (14, 6, 0, -4))])
+@pytest.mark.parametrize("rows,cols", [(200, 333), (500, 150), (90, 200), (170, 180)])
+def test_half_width_sources_of_any_scale(mg, kind, powers, rows, cols):
+    """A batch whose matrices differ by powers of two, from beyond fp32's squares to near
+    eps, with entries over a wide range; in fp32, so that the result's own rounding hides
+    nothing. The formula is taken without the power, which the plain iteration needs."""
+    r = np.random.RandomState(9)
+    g = gradients(r, len(powers), rows, cols, "strong") * np.exp(r.normal(0, 1.5, (1, rows, 1)))
+    g = decode(encode(g * 2.0 ** np.array(powers)[:, None, None], kind), kind)
+    assert np.isfinite(g).all()
+    got = run_orth(mg, g, kind, "fp32")
+    for k, power in enumerate(powers):
+        check_orthogonal(got[k], g[k] / 2.0**power, "fp32", eps=1e-7 / 2.0**power)
+
+
 def test_an_empty_batch_is_nothing(mg):
     mg.orthogonalize(mg.matrices(None, 0, 4, 4), mg.matrices(None, 0, 4, 4))
 
