@@ -14,6 +14,8 @@
 // writes one partial row, and a second launch adds the partial rows in fixed
 // order: chains of at most rows / (groups of the grid) terms, then of 16, with no
 // atomics.
+#include <type_traits>
+
 #include "kernels.h"
 #include "mg/device/common.h"
 #include "operator_types.h"
@@ -74,38 +76,41 @@ __device__ __forceinline__ void norm_sum(float (&v)[N], float (*red)[N][NT / 64]
     }
 }
 
-template <bool EXACT, int V, int E>
+template <int FIT, int V, int E>
 __device__ __forceinline__ void load_vector_param(const float* p, float fill, uint32_t v0, uint32_t stride,
                                                   uint32_t cols, float (&out)[V][E]) {
 #pragma unroll
     for (int k = 0; k < V; ++k)
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
+        for (int e = 0; e < E; e += 4) {
             const uint32_t c = (v0 + k * stride) * E + e;
-            out[k][e] = (EXACT || c < cols) ? (p ? p[c] : fill) : 0.0f;
+            float q[4] = {fill, fill, fill, fill};
+            if (p) load_vec<FIT>(p, c / 4, cols, q);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) out[k][e + u] = q[u];
         }
 }
 
 // E consecutive floats from column c.
-template <bool EXACT, int E>
+template <int FIT, int E>
 __device__ __forceinline__ void store_floats(float* out, uint32_t c, uint32_t cols, const float (&x)[E]) {
 #pragma unroll
     for (int e = 0; e < E; e += 4) {
         const float q[4] = {x[e], x[e + 1], x[e + 2], x[e + 3]};
-        store_vec<EXACT>(out, (c + e) / 4, cols, q);
+        store_vec<FIT>(out, (c + e) / 4, cols, q);
     }
 }
 
-// EXACT: cols = G V E, so no vector is short or missing.
-template <class T, int G, int V, int NT, bool EXACT>
+// FIT: kFull where cols = G V E.
+template <class T, int G, int V, int NT, int FIT>
 __global__ void __launch_bounds__(NT) layernorm_kernel(const NormArgs a) {
     constexpr int E = 16 / sizeof(T), RP = NT / G;  // rows of a workgroup's pass
     __shared__ float red[2][1][NT / 64];
     const uint32_t t = threadIdx.x % G, cols = a.cols;
     const float n = (float)cols;
     float gamma[V][E], beta[V][E];
-    load_vector_param<EXACT>(a.gamma, 1.0f, t, G, cols, gamma);
-    load_vector_param<EXACT>(a.beta, 0.0f, t, G, cols, beta);
+    load_vector_param<FIT>(a.gamma, 1.0f, t, G, cols, gamma);
+    load_vector_param<FIT>(a.beta, 0.0f, t, G, cols, beta);
     for (uint64_t base = (uint64_t)blockIdx.x * RP; base < a.rows; base += (uint64_t)gridDim.x * RP) {
         // groups past the last row repeat it without a store: lane exchanges need every lane
         const uint64_t want = base + threadIdx.x / G;
@@ -114,18 +119,18 @@ __global__ void __launch_bounds__(NT) layernorm_kernel(const NormArgs a) {
         const T* x = static_cast<const T*>(a.x) + r * a.x_ld;
         float v[V][E];
 #pragma unroll
-        for (int k = 0; k < V; ++k) load_vec<EXACT>(x, t + k * G, cols, v[k]);
+        for (int k = 0; k < V; ++k) load_vec<FIT>(x, t + k * G, cols, v[k]);
         if (a.residual) {
             const T* res = static_cast<const T*>(a.residual) + r * a.residual_ld;
             T* sum = static_cast<T*>(a.sum) + r * a.sum_ld;
             float w[V][E];
 #pragma unroll
-            for (int k = 0; k < V; ++k) load_vec<EXACT>(res, t + k * G, cols, w[k]);
+            for (int k = 0; k < V; ++k) load_vec<FIT>(res, t + k * G, cols, w[k]);
 #pragma unroll
             for (int k = 0; k < V; ++k) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) v[k][e] = (float)(T)(v[k][e] + w[k][e]);  // normalised as stored
-                if (live) store_vec<EXACT>(sum, t + k * G, cols, v[k]);
+                if (live) store_vec<FIT>(sum, t + k * G, cols, v[k]);
             }
         }
         float s[1] = {};
@@ -141,7 +146,7 @@ __global__ void __launch_bounds__(NT) layernorm_kernel(const NormArgs a) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 v[k][e] -= mean;
-                if (EXACT || (t + k * G) * E + e < cols) q[0] += v[k][e] * v[k][e];
+                if (FIT == kFull || (t + k * G) * E + e < cols) q[0] += v[k][e] * v[k][e];
             }
         norm_sum<G, NT>(q, red, 1);
         const float rstd = 1.0f / sqrtf(q[0] / n + a.eps);
@@ -152,7 +157,7 @@ __global__ void __launch_bounds__(NT) layernorm_kernel(const NormArgs a) {
             float o[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] = v[k][e] * rstd * gamma[k][e] + beta[k][e];
-            store_vec<EXACT>(y, t + k * G, cols, o);
+            store_vec<FIT>(y, t + k * G, cols, o);
         }
         if (t == 0) {
             if (a.mean) a.mean[r] = mean;
@@ -176,13 +181,13 @@ __global__ void __launch_bounds__(NT) layernorm_wide_kernel(const NormArgs a) {
         float s[1] = {};
         for (uint32_t v = threadIdx.x; v < nv; v += NT) {
             float u[E];
-            load_vec<false>(x, v, cols, u);
+            load_vec<kTail>(x, v, cols, u);
             if (a.residual) {
                 float w[E];
-                load_vec<false>(static_cast<const T*>(a.residual) + r * a.residual_ld, v, cols, w);
+                load_vec<kTail>(static_cast<const T*>(a.residual) + r * a.residual_ld, v, cols, w);
 #pragma unroll
                 for (int e = 0; e < E; ++e) u[e] = (float)(T)(u[e] + w[e]);
-                store_vec<false>(static_cast<T*>(a.sum) + r * a.sum_ld, v, cols, u);
+                store_vec<kTail>(static_cast<T*>(a.sum) + r * a.sum_ld, v, cols, u);
             }
             float p = 0.0f;
 #pragma unroll
@@ -195,7 +200,7 @@ __global__ void __launch_bounds__(NT) layernorm_wide_kernel(const NormArgs a) {
         float q[1] = {};
         for (uint32_t v = threadIdx.x; v < nv; v += NT) {
             float u[E], p = 0.0f;
-            load_vec<false>(x, v, cols, u);
+            load_vec<kTail>(x, v, cols, u);
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 if (v * E + e < cols) p += (u[e] - mean) * (u[e] - mean);
@@ -205,13 +210,13 @@ __global__ void __launch_bounds__(NT) layernorm_wide_kernel(const NormArgs a) {
         const float rstd = 1.0f / sqrtf(q[0] / n + a.eps);
         for (uint32_t v = threadIdx.x; v < nv; v += NT) {
             float u[E];
-            load_vec<false>(x, v, cols, u);
+            load_vec<kTail>(x, v, cols, u);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const uint32_t c = v * E + e;
                 if (c < cols) u[e] = (u[e] - mean) * rstd * (a.gamma ? a.gamma[c] : 1.0f) + (a.beta ? a.beta[c] : 0.0f);
             }
-            store_vec<false>(static_cast<T*>(a.y) + r * a.y_ld, v, cols, u);
+            store_vec<kTail>(static_cast<T*>(a.y) + r * a.y_ld, v, cols, u);
         }
         if (threadIdx.x == 0) {
             if (a.mean) a.mean[r] = mean;
@@ -220,8 +225,12 @@ __global__ void __launch_bounds__(NT) layernorm_wide_kernel(const NormArgs a) {
     }
 }
 
-template <class T, int G, int V, int NT, bool EXACT>
-__global__ void __launch_bounds__(NT) layernorm_backward_kernel(const NormGradArgs a) {
+// At 16 floats a lane and a short vector, gamma is read again for each row, from L1:
+// held, it takes the kernel past 128 registers, with which two workgroups fit a CU
+// (10007 x 1001 binary16: 22.9 us, so 20.0). Without short vectors the second workgroup
+// gains less than the reads cost (100000 x 1024: 117 us, so 121).
+template <class T, int G, int V, int NT, int FIT>
+__global__ void __launch_bounds__(NT, G <= 64 && FIT == kTail ? 4 : 1) layernorm_backward_kernel(const NormGradArgs a) {
     constexpr int E = 16 / sizeof(T), RP = NT / G, W = NT / 64;
     // the workgroup's sums of its waves (groups inside a wave), or norm_sum's sets
     constexpr int LDS = G <= 64 ? W * 2 * G * V * E : 2 * 2 * W;
@@ -230,7 +239,8 @@ __global__ void __launch_bounds__(NT) layernorm_backward_kernel(const NormGradAr
     const uint32_t t = threadIdx.x % G, cols = a.cols;
     const float inv_n = 1.0f / (float)cols;
     float gamma[V][E], sg[V][E] = {}, sb[V][E] = {};
-    load_vector_param<EXACT>(a.gamma, 1.0f, t, G, cols, gamma);
+    constexpr bool HOLD = G > 64 || V * E <= 8 || FIT == kFull;
+    if (HOLD) load_vector_param<FIT>(a.gamma, 1.0f, t, G, cols, gamma);
     int turn = 0;
     for (uint64_t base = (uint64_t)blockIdx.x * RP; base < a.rows; base += (uint64_t)gridDim.x * RP) {
         const uint64_t want = base + threadIdx.x / G;
@@ -240,9 +250,10 @@ __global__ void __launch_bounds__(NT) layernorm_backward_kernel(const NormGradAr
         const T* dyr = static_cast<const T*>(a.dy) + r * a.dy_ld;
         float x[V][E], d[V][E];
 #pragma unroll
-        for (int k = 0; k < V; ++k) load_vec<EXACT>(xr, t + k * G, cols, x[k]);
+        for (int k = 0; k < V; ++k) load_vec<FIT>(xr, t + k * G, cols, x[k]);
 #pragma unroll
-        for (int k = 0; k < V; ++k) load_vec<EXACT>(dyr, t + k * G, cols, d[k]);
+        for (int k = 0; k < V; ++k) load_vec<FIT>(dyr, t + k * G, cols, d[k]);
+        if (!HOLD) load_vector_param<FIT>(a.gamma, 1.0f, t, G, cols, gamma);
         const float mean = a.mean[r], rstd = a.rstd[r];
         float s[2] = {};
 #pragma unroll
@@ -267,10 +278,10 @@ __global__ void __launch_bounds__(NT) layernorm_backward_kernel(const NormGradAr
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             float o[E] = {};
-            if (dsum) load_vec<EXACT>(dsum, t + k * G, cols, o);
+            if (dsum) load_vec<FIT>(dsum, t + k * G, cols, o);
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] += rstd * (d[k][e] - m0 - x[k][e] * m1);
-            store_vec<EXACT>(dx, t + k * G, cols, o);
+            store_vec<FIT>(dx, t + k * G, cols, o);
         }
     }
     float* out_g = a.partial ? a.partial + (size_t)blockIdx.x * 2 * cols : a.dgamma;
@@ -308,8 +319,8 @@ __global__ void __launch_bounds__(NT) layernorm_backward_kernel(const NormGradAr
     } else {
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            if (out_g) store_floats<EXACT>(out_g, (t + k * G) * E, cols, sg[k]);
-            if (out_b) store_floats<EXACT>(out_b, (t + k * G) * E, cols, sb[k]);
+            if (out_g) store_floats<FIT>(out_g, (t + k * G) * E, cols, sg[k]);
+            if (out_b) store_floats<FIT>(out_b, (t + k * G) * E, cols, sb[k]);
         }
     }
 }
@@ -330,8 +341,8 @@ __global__ void __launch_bounds__(NT) layernorm_backward_wide_kernel(const NormG
         float s[2] = {};
         for (uint32_t v = threadIdx.x; v < nv; v += NT) {
             float x[E], d[E], p0 = 0.0f, p1 = 0.0f;
-            load_vec<false>(xr, v, cols, x);
-            load_vec<false>(dyr, v, cols, d);
+            load_vec<kTail>(xr, v, cols, x);
+            load_vec<kTail>(dyr, v, cols, d);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const uint32_t c = v * E + e;
@@ -347,16 +358,16 @@ __global__ void __launch_bounds__(NT) layernorm_backward_wide_kernel(const NormG
         const float m0 = s[0] * inv_n, m1 = s[1] * inv_n;
         for (uint32_t v = threadIdx.x; v < nv; v += NT) {
             float x[E], d[E], o[E] = {};
-            load_vec<false>(xr, v, cols, x);
-            load_vec<false>(dyr, v, cols, d);
-            if (a.dsum) load_vec<false>(static_cast<const T*>(a.dsum) + r * a.dsum_ld, v, cols, o);
+            load_vec<kTail>(xr, v, cols, x);
+            load_vec<kTail>(dyr, v, cols, d);
+            if (a.dsum) load_vec<kTail>(static_cast<const T*>(a.dsum) + r * a.dsum_ld, v, cols, o);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const uint32_t c = v * E + e;
                 const float g = c < cols ? (a.gamma ? a.gamma[c] : 1.0f) * d[e] : 0.0f;
                 o[e] += rstd * (g - m0 - (x[e] - mean) * rstd * m1);
             }
-            store_vec<false>(static_cast<T*>(a.dx) + r * a.dx_ld, v, cols, o);
+            store_vec<kTail>(static_cast<T*>(a.dx) + r * a.dx_ld, v, cols, o);
         }
     }
 }
@@ -372,8 +383,8 @@ __global__ void __launch_bounds__(256) layernorm_columns_kernel(const NormGradAr
     float sg[E] = {}, sb[E] = {};
     for (uint64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
         float x[E], dy[E];
-        load_vec<false>(static_cast<const T*>(a.x) + r * a.x_ld, v, cols, x);
-        load_vec<false>(static_cast<const T*>(a.dy) + r * a.dy_ld, v, cols, dy);
+        load_vec<kTail>(static_cast<const T*>(a.x) + r * a.x_ld, v, cols, x);
+        load_vec<kTail>(static_cast<const T*>(a.dy) + r * a.dy_ld, v, cols, dy);
         const float mean = a.mean[r], rstd = a.rstd[r];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -448,24 +459,32 @@ uint32_t backward_parts(uint32_t rows, uint32_t cols) {
     return need < most ? (uint32_t)need : most;
 }
 
+// f(how rows of cols lie in groups of G lanes and F floats a lane, in vectors of E)
+template <int G, int F, int E, class Fn>
+void with_fit(uint32_t cols, Fn&& f) {
+    if (cols == (uint32_t)(G * F)) return f(std::integral_constant<int, dev::kFull>{});
+    if constexpr (G == 4)
+        if (cols < (uint32_t)E) return f(std::integral_constant<int, dev::kTiny>{});
+    f(std::integral_constant<int, dev::kTail>{});
+}
+
 template <class T, int G, int F>
 void launch_norm(hipStream_t st, const dev::NormArgs& a) {
     constexpr int E = 16 / sizeof(T), V = F / E, NT = G <= 64 ? 256 : G;
     const uint64_t need = ((uint64_t)a.rows + NT / G - 1) / (NT / G), most = kCus * 2048 / NT;
     const dim3 grid((uint32_t)(need < most ? need : most)), block(NT);
-    if (a.cols == (uint32_t)(G * F))
-        hipLaunchKernelGGL((dev::layernorm_kernel<T, G, V, NT, true>), grid, block, 0, st, a);
-    else
-        hipLaunchKernelGGL((dev::layernorm_kernel<T, G, V, NT, false>), grid, block, 0, st, a);
+    with_fit<G, F, E>(a.cols, [&](auto fit) {
+        hipLaunchKernelGGL((dev::layernorm_kernel<T, G, V, NT, decltype(fit)::value>), grid, block, 0, st, a);
+    });
 }
 
 template <class T, int G, int F>
 void launch_norm_backward(hipStream_t st, const dev::NormGradArgs& a, uint32_t parts) {
     constexpr int E = 16 / sizeof(T), V = F / E, NT = G <= 64 ? (int)kBackwardWaveNT : G;
-    if (a.cols == (uint32_t)(G * F))
-        hipLaunchKernelGGL((dev::layernorm_backward_kernel<T, G, V, NT, true>), dim3(parts), dim3(NT), 0, st, a);
-    else
-        hipLaunchKernelGGL((dev::layernorm_backward_kernel<T, G, V, NT, false>), dim3(parts), dim3(NT), 0, st, a);
+    with_fit<G, F, E>(a.cols, [&](auto fit) {
+        hipLaunchKernelGGL((dev::layernorm_backward_kernel<T, G, V, NT, decltype(fit)::value>), dim3(parts), dim3(NT), 0,
+                           st, a);
+    });
 }
 
 // Calls f.template operator()<G, F>() for the shape's constants.

@@ -23,30 +23,52 @@ struct TypeOf<_Float16> {
     static constexpr uint32_t type = MG_TYPE_FP16;
 };
 
-// Vector v (16 bytes, E elements) of a row of cols elements as floats, zeros
-// past the row's end. The row may begin at any element: the hardware takes
-// 16-byte loads and stores at any byte address, so odd widths and offset views
-// run the same instructions as aligned ones.
-template <bool EXACT, class T, int E>
+// How rows of cols elements lie in vectors of 16 bytes (E elements).
+enum Fit {
+    kFull,  // every vector that is asked for is whole
+    kTail,  // the row's last may be short, those past it are empty; cols >= E
+    kTiny,  // cols < E
+};
+
+// Vector v of a row as floats, zeros past the row's end. The row may begin at any
+// element: the hardware takes 16-byte loads and stores at any byte address, so odd
+// widths and offset views run the same instructions as aligned ones. A short vector is
+// read as the row's last 16 bytes and shifted: element by element, in a branch, every
+// vector's load was waited for before the next was issued (LayerNorm of 40000 x 1001
+// binary16: 50 us, so 30).
+template <int FIT, class T, int E>
 __device__ __forceinline__ void load_vec(const T* row, uint32_t v, uint32_t cols, float (&x)[E]) {
     static_assert(E * sizeof(T) == 16, "16-byte vectors");
     const uint32_t c = v * E;
-    if (EXACT || c + E <= cols) {
-        T t[E];
-        __builtin_memcpy(t, row + c, 16);
+    if constexpr (FIT == kTiny) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = (float)t[e];
+        for (int e = 0; e < E; ++e) x[e] = c + e < cols ? (float)row[c + e] : 0.0f;
         return;
     }
+    const uint32_t from = FIT == kTail && c > cols - E ? cols - E : c;
+    uint32_t w[4];
+    __builtin_memcpy(w, row + from, 16);
+    if constexpr (FIT == kTail) {
+        const uint32_t shift = (c - from) * sizeof(T);  // bytes; past 15 nothing is left
+        w[0] = shift & 8 ? w[2] : w[0], w[1] = shift & 8 ? w[3] : w[1];
+        w[0] = shift & 4 ? w[1] : w[0], w[1] = shift & 4 ? w[2] : w[1], w[2] = shift & 4 ? w[3] : w[2];
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = c + e < cols ? (float)row[c + e] : 0.0f;
+            for (int k = 0; k < 3; ++k) w[k] = __builtin_amdgcn_alignbyte(w[k + 1], w[k], shift & 2);
+            w[3] >>= 8 * (shift & 2);
+        }
+    }
+    T t[E];
+    __builtin_memcpy(t, w, 16);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = FIT == kFull || c + e < cols ? (float)t[e] : 0.0f;
 }
 
 // Rounds x to T and writes it; nothing past the row's end.
-template <bool EXACT, class T, int E>
+template <int FIT, class T, int E>
 __device__ __forceinline__ void store_vec(T* row, uint32_t v, uint32_t cols, const float (&x)[E]) {
     const uint32_t c = v * E;
-    if (EXACT || c + E <= cols) {
+    if (FIT == kFull || c + E <= cols) {
         T t[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) t[e] = (T)x[e];
