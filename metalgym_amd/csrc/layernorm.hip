@@ -209,13 +209,12 @@ __global__ void __launch_bounds__(NT) layernorm_wide_kernel(const NormArgs a) {
         norm_sum<NT, NT>(q, red, 1);
         const float rstd = 1.0f / sqrtf(q[0] / n + a.eps);
         for (uint32_t v = threadIdx.x; v < nv; v += NT) {
-            float u[E];
+            float u[E], gamma[1][E], beta[1][E];
             load_vec<kTail>(x, v, cols, u);
+            load_vector_param<kTail>(a.gamma, 1.0f, v, 0, cols, gamma);
+            load_vector_param<kTail>(a.beta, 0.0f, v, 0, cols, beta);
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const uint32_t c = v * E + e;
-                if (c < cols) u[e] = (u[e] - mean) * rstd * (a.gamma ? a.gamma[c] : 1.0f) + (a.beta ? a.beta[c] : 0.0f);
-            }
+            for (int e = 0; e < E; ++e) u[e] = (u[e] - mean) * rstd * gamma[0][e] + beta[0][e];
             store_vec<kTail>(static_cast<T*>(a.y) + r * a.y_ld, v, cols, u);
         }
         if (threadIdx.x == 0) {
@@ -340,13 +339,13 @@ __global__ void __launch_bounds__(NT) layernorm_backward_wide_kernel(const NormG
         const float mean = a.mean[r], rstd = a.rstd[r];
         float s[2] = {};
         for (uint32_t v = threadIdx.x; v < nv; v += NT) {
-            float x[E], d[E], p0 = 0.0f, p1 = 0.0f;
+            float x[E], d[E], gamma[1][E], p0 = 0.0f, p1 = 0.0f;
             load_vec<kTail>(xr, v, cols, x);
             load_vec<kTail>(dyr, v, cols, d);
+            load_vector_param<kTail>(a.gamma, 1.0f, v, 0, cols, gamma);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const uint32_t c = v * E + e;
-                const float g = c < cols ? (a.gamma ? a.gamma[c] : 1.0f) * d[e] : 0.0f;
+                const float g = gamma[0][e] * d[e];  // 0 past the row's end
                 p0 += g;
                 p1 += g * ((x[e] - mean) * rstd);
             }
@@ -357,14 +356,14 @@ __global__ void __launch_bounds__(NT) layernorm_backward_wide_kernel(const NormG
         turn ^= 1;
         const float m0 = s[0] * inv_n, m1 = s[1] * inv_n;
         for (uint32_t v = threadIdx.x; v < nv; v += NT) {
-            float x[E], d[E], o[E] = {};
+            float x[E], d[E], gamma[1][E], o[E] = {};
             load_vec<kTail>(xr, v, cols, x);
             load_vec<kTail>(dyr, v, cols, d);
+            load_vector_param<kTail>(a.gamma, 1.0f, v, 0, cols, gamma);
             if (a.dsum) load_vec<kTail>(static_cast<const T*>(a.dsum) + r * a.dsum_ld, v, cols, o);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const uint32_t c = v * E + e;
-                const float g = c < cols ? (a.gamma ? a.gamma[c] : 1.0f) * d[e] : 0.0f;
+                const float g = gamma[0][e] * d[e];
                 o[e] += rstd * (g - m0 - (x[e] - mean) * rstd * m1);
             }
             store_vec<kTail>(static_cast<T*>(a.dx) + r * a.dx_ld, v, cols, o);
@@ -381,6 +380,7 @@ __global__ void __launch_bounds__(256) layernorm_columns_kernel(const NormGradAr
     const uint32_t v = blockIdx.x * 256 + threadIdx.x, cols = a.cols;
     if (v * E >= cols) return;
     float sg[E] = {}, sb[E] = {};
+#pragma unroll 4
     for (uint64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
         float x[E], dy[E];
         load_vec<kTail>(static_cast<const T*>(a.x) + r * a.x_ld, v, cols, x);
