@@ -11,7 +11,8 @@
 //         steps to Q in LDS, all of them the same; then X <- Q X on its slabs, and
 //         their part of the new X X', or at the end the result. The repeated work is on
 //         CUs that would be idle: with one workgroup a matrix doing it, in launches of
-//         its own, Q went through memory (2 x 512 x 128: 74.6 us, now 67.4; 1000 x 128 x 512: 1262, now 721).
+//         its own, Q went through memory (2 x 512 x 128: 74.6 us, so 67.4; 1000 of 128 x 512:
+//         1262, so 721).
 // Each kernel runs its code once or a few times, so what it costs is latencies: loads
 // are issued in batches, one wave holds one 32 x 32 tile, and code is kept in loops
 // (unrolled four waves' worth of tiles each, the same kernels spent 13 to 25 us
@@ -303,8 +304,11 @@ __global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_first_kernel(co
 // Q = P P' over P'. A wave's four consecutive results lie in one column, and are kept
 // as four of a row, so what is kept is the product's transpose: in this order A' = P A P
 // keeps its symmetry under rounding (with P P A an error of A grows up to threefold).
-// A product is 1.7 us of LDS reads at m = 128; two tiles a wave read less, but their
-// code took longer to fetch than that saved.
+// Only tiles on and under the diagonal are computed (2 x 512 x 128: 67.0 us with all of
+// them, 62.7 so). At m = 128 a product takes 2.3 us: 2300 to 3300 of its 5300 cycles are
+// the products (ten waves: two SIMDs have three), the rest writing the result in both
+// orders and two barriers. Two tiles a wave read less LDS, but their code took longer to
+// fetch than that saved; reading a chain ahead gained nothing.
 //
 // Then X' X = Q X as X' rows: a wave takes 32 columns of X by 32 rows of Q. The first
 // slab is on its way to LDS meanwhile. FINAL writes the result, in the orientation that
