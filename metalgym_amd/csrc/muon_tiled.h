@@ -73,8 +73,15 @@ __global__ void __launch_bounds__(256) source_norm_kernel(const SourceArgs a, do
     if (threadIdx.x == 0) partial[(size_t)k * gridDim.x + blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
 
-// 1 / (|U| + eps) in every thread, NaN where the norm is not finite. red holds 1.
-__device__ __forceinline__ float source_scale(const double* partial, uint32_t parts, float eps, float* red) {
+// kUnitX / (|U| + eps) as 2^exp rest in every thread, rest in [1, 2), or NaN where the
+// norm is not finite. The power is applied as an exponent: as a factor, of matrices near
+// fp32's largest it would be subnormal, with few bits left.
+struct SourceScale {
+    int exp;
+    float rest;
+};
+__device__ __forceinline__ SourceScale source_scale(const double* partial, uint32_t parts, float eps,
+                                                    SourceScale* shared) {
     if (threadIdx.x < 64) {
         double s = 0.0;
 #pragma unroll 4
@@ -82,11 +89,14 @@ __device__ __forceinline__ float source_scale(const double* partial, uint32_t pa
         for (int step = 1; step < 64; step *= 2) s += __shfl_xor(s, step);
         if (threadIdx.x == 0) {
             const double norm = sqrt(s);
-            *red = norm < (double)__builtin_huge_valf() ? (float)(1.0 / (norm + (double)eps)) : __builtin_nanf("");
+            const bool finite = norm < __builtin_huge_val();
+            const double scale = finite ? (double)kUnitX / (norm + (double)eps) : 1.0;
+            shared->exp = ilogb(scale);
+            shared->rest = finite ? (float)ldexp(scale, -ilogb(scale)) : __builtin_nanf("");
         }
     }
     __syncthreads();
-    return *red;
+    return *shared;
 }
 
 // A matrix of pairs: every 32 rows' blocks of 16 contraction elements, and 4 KB
@@ -116,30 +126,28 @@ struct Planes {
 // elements are a run along one of the two; the other takes four threads'.
 // EXACT: a power of two takes the place of the factor, so that a 16-bit source fits the
 // high halves (under 2^-27 of the norm to 2^-38 of it) and the low ones, which nothing
-// reads, are not written. rest[k] is what is left of the factor, in [1, 2).
+// reads, are not written. rest[k] is what is left of the factor.
 template <bool EXACT>
 __global__ void __launch_bounds__(256) source_split_kernel(const SourceArgs a, const double* partial, uint32_t parts,
                                                            float eps, float* rest, Planes X, Planes XT) {
-    __shared__ float red;
+    __shared__ SourceScale shared;
     const uint32_t k = blockIdx.z, i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
     float u[16];
     tile_load<false>(a, k, i0, j0, u);
-    float scale = source_scale(partial + (size_t)k * parts, parts, eps, &red);
-    if constexpr (EXACT) {
-        const float factor = scale;
-        if (factor == factor) scale = ldexpf(1.0f, ilogbf(factor));
-        if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) rest[k] = factor / scale;
-    }
-    scale *= kUnitX;
+    const SourceScale scale = source_scale(partial + (size_t)k * parts, parts, eps, &shared);
+    if (EXACT && threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) rest[k] = scale.rest;
+    const float own = EXACT ? 1.0f : scale.rest;
     const bool tall = a.rows > a.cols;
     const Planes& by_column = tall ? X : XT;  // rows of it are the source's columns
     const Planes& by_row = tall ? XT : X;
     const uint32_t j = j0 + (threadIdx.x & 63), i = i0 + (threadIdx.x >> 6) * 16;
 #pragma unroll
     for (int e = 0; e < 16; e += 4) {
-        const float x[4] = {u[e], u[e + 1], u[e + 2], u[e + 3]};
+        float x[4];
+#pragma unroll
+        for (int f = 0; f < 4; ++f) x[f] = ldexpf(u[e + f], scale.exp);
         f16x4 hi, lo;
-        split4(x, scale, hi, lo);
+        split4(x, own, hi, lo);
         if constexpr (EXACT) {
             *reinterpret_cast<f16x4*>(by_column.at(k, j, i + e)) = hi;
             *reinterpret_cast<f16x4*>(by_row.at(k, i + e + (threadIdx.x & 3), j & ~3u)) = quad_transpose(hi);

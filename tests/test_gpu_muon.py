@@ -168,6 +168,33 @@ def test_steps_and_polynomials(mg, steps, coeffs, rows, cols):
     check_orthogonal(run_orth(mg, g, ns=ns)[0], g[0], "fp32", steps=steps, coeffs=coeffs)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("rows,cols", [(60, 200), (200, 333), (500, 140)])
+def test_special_half_width_matrices(mg, kind, rows, cols):
+    """As below for 16-bit sources, whose norms go from eps to past fp32's range."""
+    r = np.random.RandomState(10)
+    g = gradients(r, 5, rows, cols)
+    g[0] = 0
+    g[1, rows // 2, 3] = np.nan
+    g[2, rows - 1, cols - 1] = -np.inf
+    g[3] = np.sign(g[3]) * (3e38 if kind == "bf16" else 65000.0)
+    g = decode(encode(g, kind), kind)
+    got = run_orth(mg, g, kind, "fp32")
+    assert not got[0].any()
+    assert np.isnan(got[1]).all() and np.isnan(got[2]).all()
+    check_orthogonal(got[3], np.sign(g[3]), "fp32", eps=0.0)
+    check_orthogonal(got[4], g[4], "fp32")
+
+
+@pytest.mark.parametrize("count,rows,cols", [(300, 70, 200), (130, 128, 520), (40, 1300, 96), (260, 200, 20)])
+def test_batches_of_more_matrices_than_fit_at_once(mg, count, rows, cols):
+    """Workgroups that take one, several or all slabs of a matrix."""
+    g = gradients(np.random.RandomState(11), count, rows, cols).astype(np.float32).astype(np.float64)
+    got = run_orth(mg, g)
+    for k in range(count):
+        check_orthogonal(got[k], g[k], "fp32")
+
+
 @pytest.mark.parametrize("rows,cols", [(60, 200), (200, 170)])
 def test_special_matrices(mg, rows, cols):
     """Zeros give zeros, a NaN or an infinity gives NaN throughout, huge and tiny
