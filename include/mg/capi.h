@@ -494,7 +494,8 @@ typedef struct mg_newton_schulz {
 /* `count` row-major matrices of rows x cols elements: element (i, j) of matrix k
  * at data[k stride + i ld + j]. ld 0: cols; stride 0: rows ld. rows and cols are
  * at least 1 and at most 65536, the smaller at most 8192; count may be 0, at most
- * 65535. type is MG_TYPE_*. Matrices of one batch must not overlap. */
+ * 65535; ld is under 2^31 and stride at most 2^44. type is MG_TYPE_*. Matrices of one
+ * batch must not overlap. */
 typedef struct mg_matrices {
     void* data;
     uint64_t ld;
@@ -518,8 +519,8 @@ int mg_orthogonalize(void* stream, const mg_newton_schulz* ns, const mg_matrices
  * U = nesterov ? G + momentum (M - G) : M; W = (1 - lr weight_decay) W - lr scale O,
  * O the Newton-Schulz result of U. scale 0 stands for sqrt(max(1, cols / rows)):
  * rows are a layer's inputs and cols its outputs, as in the policy's matrices.
- * lr, weight_decay and scale are finite and not negative, lr weight_decay at most
- * 1, momentum in [0, 1). */
+ * lr, weight_decay, scale and lr scale are finite and not negative, lr weight_decay
+ * at most 1, momentum in [0, 1). */
 typedef struct mg_muon_config {
     float lr;
     float momentum;

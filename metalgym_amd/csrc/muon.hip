@@ -361,6 +361,7 @@ int check_muon(const char* what, const mg_muon_config* c, mg_newton_schulz* ns) 
     MG_CHECK(fine(c->lr) && fine(c->weight_decay) && fine(c->scale), MG_ERR_INVALID,
              "%s: lr, weight_decay and scale must be finite and not negative", what);
     MG_CHECK(c->lr * c->weight_decay <= 1.0f, MG_ERR_INVALID, "%s: lr * weight_decay must be at most 1", what);
+    MG_CHECK(fine(c->lr * fmaxf(c->scale, 256.0f)), MG_ERR_INVALID, "%s: lr * scale is out of range", what);  // 256: of 1 x 65536
     MG_CHECK(c->momentum >= 0.0f && c->momentum < 1.0f, MG_ERR_INVALID, "%s: momentum must be in [0, 1)", what);
     return check_ns(what, c->ns.steps ? &c->ns : nullptr, ns);
 }

@@ -165,5 +165,11 @@ def test_muon_decay_is_bounded(mg):
     refused(lambda: mg.muon_step(batch(mg), batch(mg), batch(mg), lr=2.0, weight_decay=0.6, **full), "at most 1")
 
 
+@pytest.mark.parametrize("kw", [dict(lr=1e30, scale=1e30), dict(lr=3e38, scale=0.0)])
+def test_muon_rate_is_finite(mg, kw):
+    full = dict(workspace=1 << 20, workspace_bytes=1 << 40)
+    refused(lambda: mg.muon_step(batch(mg), batch(mg), batch(mg), **kw, **full), "lr * scale")
+
+
 def test_set_muon_needs_a_model(mg):
     assert mg.lib().mg_ppo_set_muon(None, None) == -1
