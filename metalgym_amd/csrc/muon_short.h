@@ -11,8 +11,8 @@
 //         steps to Q in LDS, all of them the same; then X <- Q X on its slabs, and
 //         their part of the new X X', or at the end the result. The repeated work is on
 //         CUs that would be idle: with one workgroup a matrix doing it, in launches of
-//         its own, Q went through memory (2 x 512 x 128: 74.6 us, so 67.4; 1000 of 128 x 512:
-//         1262, so 721).
+//         its own, Q went through memory (two of 512 x 128 in three segments: 74.6 us, so 67.4;
+//         1000 of 128 x 512: 1262, so 721).
 // Each kernel runs its code once or a few times, so what it costs is latencies: loads
 // are issued in batches, one wave holds one 32 x 32 tile, and code is kept in loops
 // (unrolled four waves' worth of tiles each, the same kernels spent 13 to 25 us
@@ -69,13 +69,24 @@ __device__ __forceinline__ f16x4 quad_transpose(f16x4 v) {
     return __builtin_bit_cast(f16x4, out);
 }
 
-// c + a b of pairs, a's low halves first; SWAP: b's, which gives the bits of the
-// product with a and b in each other's place.
-template <bool SWAP = false>
-__device__ __forceinline__ f32x16 pair_mfma(const f16x8 (&a)[2], const f16x8 (&b)[2], f32x16 c) {
-    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[!SWAP], b[SWAP], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[SWAP], b[!SWAP], c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[0], c, 0, 0, 0);
+// a b of pairs over 32 contraction elements (two fragments). The products of low halves
+// come first, so that the sum is of full size in the last two instructions only: each
+// rounds it, and cuts off what its small products have under 2^-25 of its largest, 0.1
+// of a last place each (rms error of 72 x 56: 1.71e-6 with the instructions in the order
+// of their elements, 1.58e-6 so). SWAP: with the bits of the product with a and b in each
+// other's place. LOW: with the product of the low halves too, 2^-24 of a square.
+template <bool SWAP, bool LOW>
+__device__ __forceinline__ f32x16 pair_mfma(const f16x8 (&a)[2][2], const f16x8 (&b)[2][2]) {
+    f32x16 c = {};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        if (LOW) c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[e][1], b[e][1], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[e][!SWAP], b[e][SWAP], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[e][SWAP], b[e][!SWAP], c, 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[e][0], b[e][0], c, 0, 0, 0);
+    return c;
 }
 
 // Exponents of a matrix's X while it is the source's own.
@@ -124,28 +135,27 @@ struct ShortShape {
     static constexpr int W = CB * NB < 8 ? CB * NB : 8;  // waves over a slab's column and row blocks
     static constexpr int NT = 64 * W, PER = MP * kSlab / NT;  // elements of a slab a thread
     static constexpr int THREADS = 64 * (W > TILES ? W : TILES);  // a wave a tile of a symmetric matrix
+    // sums of few products: 1 x 5 is off by 7.5e-7 (rms) without, 3.9e-7 with it
+    static constexpr bool LOW = MP == 32;
     static constexpr int SQ = 2 * MP * MP, SLAB = 2 * MP * kSlab;  // elements of a pair of planes
 };
 
 // 32 x 32 of x y' over K contraction elements, rows 32 bi of x and 32 bj of y, in
 // chains of 32.
-template <int K>
+template <int K, bool LOW>
 __device__ __forceinline__ f32x16 short_product(const f16* x, const f16* y, int bi, int bj) {
     f32x16 v = {};
 #pragma unroll 2
     for (int kk = 0; kk < K / 16; kk += 2) {
-        f32x16 s = {};
+        f16x8 a[2][2], b[2][2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            f16x8 a[2], b[2];
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
-                a[p] = Frags<K>::frag(x, p, bi, kk + e);
-                b[p] = Frags<K>::frag(y, p, bj, kk + e);
+                a[e][p] = Frags<K>::frag(x, p, bi, kk + e);
+                b[e][p] = Frags<K>::frag(y, p, bj, kk + e);
             }
-            s = pair_mfma(a, b, s);
-        }
-        v += s;
+        v += pair_mfma<false, LOW>(a, b);
     }
     return v;
 }
@@ -157,7 +167,7 @@ __device__ __forceinline__ void short_gram(const f16* rows, f32x16& gram) {
     if (t >= ShortShape<MP>::TILES) return;
     int bi, bj;
     short_tile(t, bi, bj);
-    gram += short_product<kSlab>(rows, rows, bi, bj);
+    gram += short_product<kSlab, ShortShape<MP>::LOW>(rows, rows, bi, bj);
 }
 // The workgroup's partial sums, in register order.
 template <int MP>
@@ -304,8 +314,7 @@ __global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_first_kernel(co
 // Q = P P' over P'. A wave's four consecutive results lie in one column, and are kept
 // as four of a row, so what is kept is the product's transpose: in this order A' = P A P
 // keeps its symmetry under rounding (with P P A an error of A grows up to threefold).
-// Only tiles on and under the diagonal are computed (2 x 512 x 128: 67.0 us with all of
-// them, 62.7 so). At m = 128 a product takes 2.3 us: 2300 to 3300 of its 5300 cycles are
+// Only tiles on and under the diagonal are computed (67.0 us with all of them, 62.7 so). At m = 128 a product takes 2.3 us: 2300 to 3300 of its 5300 cycles are
 // the products (ten waves: two SIMDs have three), the rest writing the result in both
 // orders and two barriers. Two tiles a wave read less LDS, but their code took longer to
 // fetch than that saved; reading a chain ahead gained nothing.
@@ -389,7 +398,7 @@ __global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_step_kernel(con
         if (op >= 0) {
             const f16* x = lds[op == 2];
             const f16* y = lds[op == 1 || op == 4];
-            if (on) v = short_product<MP>(x, y, bi, bj);
+            if (on) v = short_product<MP, S::LOW>(x, y, bi, bj);
             to_out = op == 1 || op == 2 ? 1.0f / kUnitP : 1.0f;
             if (op == last) to_out = a.unit_q / (op == 4 ? kUnitP * kUnitP : kUnitP);
             if (on && (op == 0 || op == 3)) {  // a I + b A + c (A A), at kUnitP
@@ -440,15 +449,13 @@ __global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_step_kernel(con
             // x y' of 32 x 32 in chains of 32, or its transpose
 #pragma unroll
             for (int kk = 0; kk < MP / 16; kk += 2) {
-                f32x16 t = {};
+                f16x8 x[2][2], y[2][2];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    f16x8 x[2], y[2];
+                for (int e = 0; e < 2; ++e)
 #pragma unroll
-                    for (int p = 0; p < 2; ++p) x[p] = F::frag(slab, p, jb, kk + e), y[p] = F::frag(q, p, b, kk + e);
-                    t = FINAL && !tall ? pair_mfma<true>(y, x, t) : pair_mfma(x, y, t);
-                }
-                acc += t;
+                    for (int p = 0; p < 2; ++p)
+                        x[e][p] = F::frag(slab, p, jb, kk + e), y[e][p] = F::frag(q, p, b, kk + e);
+                acc += FINAL && !tall ? pair_mfma<true, S::LOW>(y, x) : pair_mfma<false, S::LOW>(x, y);
             }
         }
         if constexpr (FINAL) {
