@@ -46,8 +46,10 @@ __device__ __forceinline__ void load_vec(const T* row, uint32_t v, uint32_t cols
         return;
     }
     const uint32_t from = FIT == kTail && c > cols - E ? cols - E : c;
-    uint32_t w[4];
-    __builtin_memcpy(w, row + from, 16);
+    // one load: an array of T filled by memcpy is taken apart into 2- and 4-byte loads
+    // in places (LayerNorm of 32768 x 1024 bf16 with a residual: 47.7 us, so 42.2)
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(2)));
+    u32x4 w = *reinterpret_cast<const u32x4*>(row + from);
     if constexpr (FIT == kTail) {
         const uint32_t shift = (c - from) * sizeof(T);  // bytes; past 15 nothing is left
         w[0] = shift & 8 ? w[2] : w[0], w[1] = shift & 8 ? w[3] : w[1];
@@ -58,8 +60,8 @@ __device__ __forceinline__ void load_vec(const T* row, uint32_t v, uint32_t cols
             w[3] >>= 8 * (shift & 2);
         }
     }
-    T t[E];
-    __builtin_memcpy(t, w, 16);
+    typedef T vec __attribute__((ext_vector_type(E)));
+    const vec t = __builtin_bit_cast(vec, w);
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = FIT == kFull || c + e < cols ? (float)t[e] : 0.0f;
 }
@@ -69,10 +71,11 @@ template <int FIT, class T, int E>
 __device__ __forceinline__ void store_vec(T* row, uint32_t v, uint32_t cols, const float (&x)[E]) {
     const uint32_t c = v * E;
     if (FIT == kFull || c + E <= cols) {
-        T t[E];
+        typedef T vec __attribute__((ext_vector_type(E)));
+        vec t;
 #pragma unroll
         for (int e = 0; e < E; ++e) t[e] = (T)x[e];
-        __builtin_memcpy(row + c, t, 16);
+        __builtin_memcpy(row + c, &t, 16);
         return;
     }
 #pragma unroll
