@@ -39,13 +39,19 @@ using dev::kUnitX;
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 uint32_t pad(uint32_t x, uint32_t to) { return (x + to - 1) / to * to; }
 
-// Edge of the product tiles: 128 where the batch's symmetric products, which are most
-// of the launches, then have a tile for every second CU. Under that 64, whose products
-// do half as well per CU but have four times as many tiles: 1000 x 257 237 us on 128,
-// 146 on 64.
-uint32_t tile_edge(uint32_t count, uint32_t m) {
-    const uint64_t t = (m + 127) / 128;
-    return count * t * (t + 1) / 2 >= 128 ? 128 : 64;
+// Edges of the product tiles, of symmetric results and of products with X: 64 where a
+// CU would have at most one tile, or two of X's, else 128, of which a CU does twice as
+// much. X's are 64 too where 128 would pad m by over a sixteenth, as the squares are
+// padded with it. 1280 x 8192 takes 693 us with 64 throughout, 817 with 128 and 584 so;
+// 900 x 2000 244 with 64 and 397 with 128; 1666 x 1570, just past the first bound, 460 and
+// 473; 9 of 487 x 585, further past it, 276 and 255.
+struct TileEdges {
+    uint32_t square, x;
+};
+TileEdges tile_edges(uint32_t count, uint32_t m, uint32_t n) {
+    const uint64_t tm = (m + 63) / 64, tn = (n + 63) / 64;
+    if (count * tm * (tm + 1) / 2 > 256) return {128, 128};
+    return {64, count * tm * tn > 512 && (pad(m, 128) - pad(m, 64)) * 16 <= m ? 128u : 64u};
 }
 
 // Steps of the next segment of the `left` that remain. One (on X) for small matrices,
@@ -152,11 +158,12 @@ int check_same(const char* what, const mg_matrices* a, const mg_matrices* b) {
 // The workspace of a batch.
 struct Workspace {
     size_t norms, rest, x, xt[2], gram, product, poly, q[2], total;  // byte offsets
-    uint32_t m, n, mp, np, tile;
+    uint32_t m, n, mp, np;
+    TileEdges tile;
     Workspace(uint32_t count, uint32_t rows, uint32_t cols) {
         m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
-        tile = tile_edge(count, m);
-        mp = pad(m, tile), np = pad(n, tile);
+        tile = tile_edges(count, m, n);
+        mp = pad(m, tile.x), np = pad(n, tile.x);  // the larger of the two
         // X by rows of np, its transpose by rows of mp
         const size_t wide = dev::planes_block(np) * (mp / 32) * 2 * count, tall = dev::planes_block(mp) * (np / 32) * 2 * count;
         const size_t square = dev::planes_block(mp) * (mp / 32) * 2 * count;
@@ -244,7 +251,17 @@ int newton_schulz_short(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
     return MG_OK;
 }
 
-template <int T>
+template <int KIND>
+int launch_product(hipStream_t st, const dev::ProductArgs& p, uint32_t tile, uint32_t tiles, uint32_t count,
+                   const char* what) {
+    if (tile == 128)
+        hipLaunchKernelGGL((dev::product_kernel<KIND, 128>), dim3(tiles, count), dim3(512), 0, st, p);
+    else
+        hipLaunchKernelGGL((dev::product_kernel<KIND, 64>), dim3(tiles, count), dim3(512), 0, st, p);
+    MG_HIP(hipGetLastError(), what);
+    return MG_OK;
+}
+
 int newton_schulz_tiled(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, const dev::SourceArgs& src,
                         const FinalArgs& fin, const Workspace& w, void* workspace) {
     char* const base = static_cast<char*>(workspace);
@@ -259,7 +276,8 @@ int newton_schulz_tiled(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
     const dev::Planes Q[2] = {planes(w.q[0], w.mp, w.mp), planes(w.q[1], w.mp, w.mp)};
     const uint32_t tiles = ((src.rows + 63) / 64) * ((src.cols + 63) / 64);
     const uint32_t parts = tiles < (uint32_t)dev::kNormParts ? tiles : dev::kNormParts;
-    const uint32_t mt = w.mp / T, nt = w.np / T;
+    const uint32_t ts = w.tile.square, tx = w.tile.x, sq = w.mp / ts, mt = w.mp / tx, nt = w.np / tx;
+    const uint32_t half = sq * (sq + 1) / 2, full = mt * nt;
     hipLaunchKernelGGL(dev::source_norm_kernel, dim3(parts, count), dim3(256), 0, st, src, norms);
     MG_HIP(hipGetLastError(), "newton-schulz norm launch");
     const bool tall = src.rows > src.cols;
@@ -275,27 +293,21 @@ int newton_schulz_tiled(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
         hipLaunchKernelGGL(dev::source_split_kernel<false>, tiles64, dim3(256), 0, st, src, norms, parts, ns.eps, rest, X, XT[0]);
     MG_HIP(hipGetLastError(), "newton-schulz split launch");
 
-    const dim3 half(mt * (mt + 1) / 2, count), full(mt * nt, count), block(512);
     dev::ProductArgs p{};
     p.m = w.m, p.rest = rest;
     // out = a b' of symmetric results
     auto symmetric = [&](const dev::Planes& a, const dev::Planes& b, uint32_t k, float unit_a, float unit_b,
                          const dev::Planes& out, float unit_out) -> int {
-        p.a = a, p.b = b, p.stages = k / dev::kPK, p.tiles_j = mt, p.out = out;
+        p.a = a, p.b = b, p.stages = k / dev::kPK, p.tiles_j = sq, p.out = out;
         p.unit = unit_out / (unit_a * unit_b);
         if (a.base == X.base && exact)
-            hipLaunchKernelGGL((dev::product_kernel<dev::kExactGram, T>), half, block, 0, st, p);
-        else
-            hipLaunchKernelGGL((dev::product_kernel<dev::kSymmetric, T>), half, block, 0, st, p);
-        MG_HIP(hipGetLastError(), "newton-schulz product launch");
-        return MG_OK;
+            return launch_product<dev::kExactGram>(st, p, ts, half, count, "newton-schulz product launch");
+        return launch_product<dev::kSymmetric>(st, p, ts, half, count, "newton-schulz product launch");
     };
     auto polynomial = [&](const dev::Planes& out) -> int {
-        p.a = p.b = p.gram = gram, p.stages = w.mp / dev::kPK, p.tiles_j = mt, p.out = out;
+        p.a = p.b = p.gram = gram, p.stages = w.mp / dev::kPK, p.tiles_j = sq, p.out = out;
         p.ca = ns.a * kUnitP, p.cb = ns.b * (kUnitP / kUnitA), p.cc = ns.c * (kUnitP / (kUnitA * kUnitA));
-        hipLaunchKernelGGL((dev::product_kernel<dev::kPolynomial, T>), half, block, 0, st, p);
-        MG_HIP(hipGetLastError(), "newton-schulz polynomial launch");
-        return MG_OK;
+        return launch_product<dev::kPolynomial>(st, p, ts, half, count, "newton-schulz polynomial launch");
     };
     int rc, cur = 0;
     double reach = 1.0;
@@ -320,23 +332,18 @@ int newton_schulz_tiled(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
         p.a = Q[q], p.b = XT[cur], p.stages = w.mp / dev::kPK, p.tiles_j = nt;
         if (left) {
             p.out = X, p.out_t = XT[cur ^ 1], p.unit = 1.0f / unit_q;
-            if (exact)
-                hipLaunchKernelGGL((dev::product_kernel<dev::kExactUpdate, T>), full, block, 0, st, p);
-            else
-                hipLaunchKernelGGL((dev::product_kernel<dev::kUpdate, T>), full, block, 0, st, p);
+            rc = exact ? launch_product<dev::kExactUpdate>(st, p, tx, full, count, "newton-schulz update launch")
+                       : launch_product<dev::kUpdate>(st, p, tx, full, count, "newton-schulz update launch");
+            if (rc) return rc;
             exact = false;  // X' is pairs
-            MG_HIP(hipGetLastError(), "newton-schulz update launch");
             cur ^= 1;
         } else {
             p.dst = fin.dst, p.step = fin.step, p.keep = fin.keep, p.rate = fin.rate, p.rows = src.rows, p.cols = src.cols;
             p.unit = 1.0f / (unit_q * kUnitX);
-            if (tall) {
-                p.a = XT[cur], p.b = Q[q], p.tiles_j = mt;
-                hipLaunchKernelGGL((dev::product_kernel<dev::kFinalTall, T>), full, block, 0, st, p);
-            } else {
-                hipLaunchKernelGGL((dev::product_kernel<dev::kFinal, T>), full, block, 0, st, p);
-            }
-            MG_HIP(hipGetLastError(), "newton-schulz result launch");
+            if (tall) p.a = XT[cur], p.b = Q[q], p.tiles_j = mt;
+            rc = tall ? launch_product<dev::kFinalTall>(st, p, tx, full, count, "newton-schulz result launch")
+                      : launch_product<dev::kFinal>(st, p, tx, full, count, "newton-schulz result launch");
+            if (rc) return rc;
         }
     }
     return MG_OK;
@@ -359,8 +366,7 @@ int newton_schulz(hipStream_t st, const mg_newton_schulz& ns, uint32_t count, co
                             : newton_schulz_short<128>(st, ns, count, a, partial);
     }
     const Workspace w(count, src.rows, src.cols);
-    return w.tile == 128 ? newton_schulz_tiled<128>(st, ns, count, src, fin, w, workspace)
-                         : newton_schulz_tiled<64>(st, ns, count, src, fin, w, workspace);
+    return newton_schulz_tiled(st, ns, count, src, fin, w, workspace);
 }
 
 // The configuration's own checks; *ns receives the iteration.

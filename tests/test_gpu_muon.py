@@ -195,6 +195,16 @@ def test_batches_of_more_matrices_than_fit_at_once(mg, count, rows, cols):
         check_orthogonal(got[k], g[k], "fp32")
 
 
+@pytest.mark.parametrize("kind", ["fp32", "fp16"])
+@pytest.mark.parametrize("count,rows,cols", [(1, 250, 8230), (1, 8230, 250), (3, 250, 2800), (1, 500, 4100)])
+def test_long_matrices(mg, kind, count, rows, cols):
+    """Squares in smaller tiles than the products with X."""
+    g = decode(encode(gradients(np.random.RandomState(12), count, rows, cols), kind), kind)
+    got = run_orth(mg, g, kind)
+    for k in range(count):
+        check_orthogonal(got[k], g[k], kind)
+
+
 @pytest.mark.parametrize("rows,cols", [(60, 200), (200, 170)])
 def test_special_matrices(mg, rows, cols):
     """Zeros give zeros, a NaN or an infinity gives NaN throughout, huge and tiny
