@@ -276,6 +276,16 @@ def test_muon_step(mg, kind, grad, rows, cols, nesterov):
     check_muon(run_muon(mg, w, m, g, kind, grad, **kw), w, m, g, kind, **kw)
 
 
+@pytest.mark.parametrize("count,rows,cols", [(2, 128, 1500), (1, 2100, 60), (300, 40, 200), (1, 250, 8230), (2, 1100, 1300)])
+def test_muon_step_of_several_slabs_and_tiles(mg, count, rows, cols):
+    """Sources that are read twice, the momentum's update between."""
+    r = np.random.RandomState(13)
+    q = lambda x, t: decode(encode(x, t), t)  # noqa: E731
+    w, m = q(r.normal(0, rows**-0.5, (count, rows, cols)), "fp32"), q(gradients(r, count, rows, cols), "fp32")
+    g = q(gradients(r, count, rows, cols, "strong"), "bf16")
+    check_muon(run_muon(mg, w, m, g, "fp32", "bf16"), w, m, g, "fp32")
+
+
 def test_muon_scale_strides_and_no_rate(mg):
     r = np.random.RandomState(9)
     w, m, g = (gradients(r, 3, 50, 70).astype(np.float32).astype(np.float64) for _ in range(3))
