@@ -8,21 +8,6 @@
 namespace mg {
 namespace dev {
 
-template <class T>
-struct TypeOf;
-template <>
-struct TypeOf<float> {
-    static constexpr uint32_t type = MG_TYPE_FP32;
-};
-template <>
-struct TypeOf<__bf16> {
-    static constexpr uint32_t type = MG_TYPE_BF16;
-};
-template <>
-struct TypeOf<_Float16> {
-    static constexpr uint32_t type = MG_TYPE_FP16;
-};
-
 // How rows of cols elements lie in vectors of 16 bytes (E elements).
 enum Fit {
     kFull,  // every vector that is asked for is whole
