@@ -261,8 +261,11 @@ __global__ void __launch_bounds__(NT, G <= 64 && FIT == kTail ? 4 : 1) layernorm
         for (int k = 0; k < V; ++k)
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                // a repeated row may be read while its dx is written over it: it adds nothing
-                const float xn = live ? (x[k][e] - mean) * rstd : 0.0f, dy = live ? d[k][e] : 0.0f;
+                // a repeated row may be read while its dx is written over it: it adds nothing.
+                // Nor does what lies past the row's end: -mean rstd may be infinite where no
+                // element's xn is, and infinity times its d = 0 is NaN.
+                const bool in = live && (FIT == kFull || (t + k * G) * E + e < cols);
+                const float xn = in ? (x[k][e] - mean) * rstd : 0.0f, dy = live ? d[k][e] : 0.0f;
                 sg[k][e] += dy * xn;
                 sb[k][e] += dy;
                 x[k][e] = xn;
@@ -347,9 +350,9 @@ __global__ void __launch_bounds__(NT) layernorm_backward_wide_kernel(const NormG
             load_vector_param<kTail>(a.gamma, 1.0f, v, 0, cols, gamma);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float g = gamma[0][e] * d[e];  // 0 past the row's end
+                const float g = gamma[0][e] * d[e];  // 0 past the row's end, where -mean rstd may be infinite
                 p0 += g;
-                p1 += g * ((x[e] - mean) * rstd);
+                p1 += g * (v * E + e < cols ? (x[e] - mean) * rstd : 0.0f);
             }
             s[0] += p0;
             s[1] += p1;
