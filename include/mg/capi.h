@@ -380,7 +380,9 @@ int mg_ppo_params_updated(mg_ppo* model);
 enum { MG_CAPTURE_LN_OUT = 0, MG_CAPTURE_HIDDEN = 1, MG_CAPTURE_DH = 2, MG_CAPTURE_DV = 3 };
 int mg_ppo_train_capture(mg_ppo* model, uint32_t which, const void** ptr, uint32_t* rows, uint32_t* cols,
                          uint32_t* layers);
-/* Adam state: first and second moments, same layout as the parameters. */
+/* Adam state: first and second moments, same layout as the parameters. step counts
+ * all updates; after mg_ppo_set_muon the block matrices' bias correction counts from
+ * their last change of optimiser. */
 int mg_ppo_adam_state(mg_ppo* model, float** m, float** v, uint32_t* step);
 /* model/ppo.h:460-469 (Gaussian head only). */
 int mg_ppo_set_log_std(mg_ppo* model, float value);
@@ -540,7 +542,8 @@ int mg_muon_step(void* stream, const mg_muon_config* config, const mg_matrices* 
  * here). The gradient is clipped by the global norm first, as for Adam; the vector
  * parameters and the head stay on Adam at the model's lr. The momentum lies in the
  * block matrices' part of mg_ppo_adam_state's m. A change of optimiser sets that
- * part of m and v to 0. Blocking. */
+ * part of m and v to 0, and Adam's bias correction of the block matrices starts anew
+ * with them. Blocking. */
 int mg_ppo_set_muon(mg_ppo* model, const mg_muon_config* config);
 
 /* ---------------------------------------------------------------------------

@@ -44,6 +44,7 @@ struct TrainStep {
     uint32_t rows;       // B
     uint32_t mb_index;   // index into the per-minibatch stats output
     float beta1_pow, beta2_pow;
+    float blocks_beta1_pow, blocks_beta2_pow;  // of the block matrices, whose moments may be younger
     const mg_muon_config* muon;  // the block matrices' optimiser, NULL: Adam as for the rest
     void* muon_ws;               // muon_blocks_bytes
 };

@@ -22,6 +22,7 @@ struct mg_ppo {
     float* m = nullptr;
     float* v = nullptr;
     uint32_t step = 0;
+    uint32_t blocks_since = 0;  // the step at which the block matrices' moments were last 0
     uint64_t shuffle_state = 0;
     std::vector<uint32_t> order;       // persistent block order (slotOrder, model/ppo.h:347-348)
     std::vector<uint32_t> last_order;  // block sequence of the last train call
@@ -180,7 +181,7 @@ int enqueue_minibatch(mg_ppo* p, uint32_t block, uint32_t mb_index, const TrainW
     const uint32_t t = block / perSlot, r0 = (block % perSlot) * p->B;
     p->step += 1;
     // model/ppo.h:874-880: float step counter, float powers
-    const float stepF = (float)p->step;
+    const float stepF = (float)p->step, blocksF = (float)(p->step - p->blocks_since);
     TrainStep ts;
     ts.row0 = t * p->n + r0;
     ts.block = block;
@@ -188,6 +189,8 @@ int enqueue_minibatch(mg_ppo* p, uint32_t block, uint32_t mb_index, const TrainW
     ts.mb_index = mb_index;
     ts.beta1_pow = powf(0.9f, stepF);
     ts.beta2_pow = powf(0.999f, stepF);
+    ts.blocks_beta1_pow = powf(0.9f, blocksF);
+    ts.blocks_beta2_pow = powf(0.999f, blocksF);
     ts.muon = p->muon_on ? &p->muon : nullptr;
     ts.muon_ws = p->muon_ws;
     return launch_train_step(p->gym->stream, p->pv, p->hp, p->cfg.lr, ws, ts, p->obs_slots, p->action_slots,
@@ -443,12 +446,14 @@ int mg_ppo_set_muon(mg_ppo* p, const mg_muon_config* config) {
     }
     const bool on = config != nullptr;
     if (on != p->muon_on) {
-        // one optimiser's moments mean nothing to the other
+        // one optimiser's moments mean nothing to the other; the bias correction of
+        // those that begin here counts from here
         const size_t bytes = (size_t)(p->pv.off_head - p->pv.float_group) * sizeof(float);
         MG_HIP(hipMemsetAsync(p->m + p->pv.float_group, 0, bytes, p->gym->stream), "set_muon clear");
         MG_HIP(hipMemsetAsync(p->v + p->pv.float_group, 0, bytes, p->gym->stream), "set_muon clear");
         MG_HIP(hipStreamSynchronize(p->gym->stream), "set_muon synchronize");
         p->muon_on = on;
+        p->blocks_since = p->step;
     }
     return MG_OK;
 }

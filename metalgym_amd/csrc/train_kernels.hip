@@ -1443,6 +1443,7 @@ struct AdamArgs {
     float* mb_stats;
     uint32_t count, float_group, off_head, hidden, mat_tiles;
     float lr, beta1_pow, beta2_pow, max_grad_norm;
+    float blocks_beta1_pow, blocks_beta2_pow;  // of the block matrices
 };
 
 // One parameter's Adam inputs, loaded before the global norm is known so the
@@ -1454,16 +1455,18 @@ __device__ __forceinline__ AdamIn adam_load(const AdamArgs& a, uint32_t i) {
     return AdamIn{a.grad[i], a.mom[i], a.var[i], a.param[i]};
 }
 
-// model/optimizer.metal:36-60 for element i with the clip scale applied.
-__device__ __forceinline__ float adam_elem(const AdamArgs& a, uint32_t i, const AdamIn& in, float scale) {
+// model/optimizer.metal:36-60 for element i with the clip scale applied; the beta
+// powers count the updates of its moments since they were 0.
+__device__ __forceinline__ float adam_elem(const AdamArgs& a, uint32_t i, const AdamIn& in, float scale,
+                                           float beta1_pow, float beta2_pow) {
     const float beta1 = 0.9f, beta2 = 0.999f, eps = 1e-8f;
     const float g = in.g * scale;
     const float m = beta1 * in.m + (1.0f - beta1) * g;
     const float v = beta2 * in.v + (1.0f - beta2) * g * g;
     a.mom[i] = m;
     a.var[i] = v;
-    const float mHat = m / (1.0f - a.beta1_pow);
-    const float vHat = v / (1.0f - a.beta2_pow);
+    const float mHat = m / (1.0f - beta1_pow);
+    const float vHat = v / (1.0f - beta2_pow);
     const float p = in.p - a.lr * mHat / (sqrtf(vHat) + eps);
     a.param[i] = p;
     return p;
@@ -1516,7 +1519,7 @@ __global__ void __launch_bounds__(256) adam_kernel(const AdamArgs a) {
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
             const int r = (256 / kTT) * e + t / kTT;
-            const float p = MUON ? in[e].p : adam_elem(a, idx[e], in[e], scale);
+            const float p = MUON ? in[e].p : adam_elem(a, idx[e], in[e], scale, a.blocks_beta1_pow, a.blocks_beta2_pow);
             lds[r * kTileLd + c] = p;
             if (FP32) most = fmaxf(most, finite_magnitude(p));
         }
@@ -1539,7 +1542,7 @@ __global__ void __launch_bounds__(256) adam_kernel(const AdamArgs a) {
     AdamIn in{};
     if (i < a.count) in = adam_load(a, i);
     const float scale = adam_clip_scale(a);
-    if (i < a.count) adam_elem(a, i, in, scale);
+    if (i < a.count) adam_elem(a, i, in, scale, a.beta1_pow, a.beta2_pow);
 }
 
 }  // namespace dev
@@ -1844,6 +1847,8 @@ int launch_train_step(hipStream_t st, const mg_policy_view& pv, const mg_ppo_hpa
         aa.lr = lr;
         aa.beta1_pow = step.beta1_pow;
         aa.beta2_pow = step.beta2_pow;
+        aa.blocks_beta1_pow = step.blocks_beta1_pow;
+        aa.blocks_beta2_pow = step.blocks_beta2_pow;
         aa.max_grad_norm = hp.max_grad_norm;
         const uint32_t lin = pv.float_group + (pv.count - pv.off_head);
         const dim3 grid(aa.mat_tiles + (lin + 255) / 256);
