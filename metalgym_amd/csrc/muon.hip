@@ -57,12 +57,13 @@ TileEdges tile_edges(uint32_t count, uint32_t m, uint32_t n) {
 // Steps of the next segment of the `left` that remain. One (on X) for small matrices,
 // where a rounding error of A does not average out, and for polynomials that grow
 // small singular values, and their errors, faster than the default's. Else two at the
-// end, and before it too where the result's own rounding, or an optimiser's rate, hides
-// the difference (hidden). Over 117 random shapes with a short side of 36 to 1000 and
-// fp32 results, the error is at most 1.7 times that of the plain fp32 iteration with two
-// steps throughout, 1.2 with two at the end (the most where the short side is under 65),
-// and 1.0 with single steps; two matrices of 512 x 128 take 63.0, 65.8 and 68.6 us,
-// 2048 x 8192 1438, 1667 and 1887.
+// end, and before it too where the rounding of a 16-bit result or weight hides the
+// difference (hidden); an fp32 weight may be 0 and its rate 1, which hide nothing. Over
+// 117 random shapes with a short side of 36 to 1000 and fp32 results, the error is at most
+// 1.7 times that of the plain fp32 iteration with two steps throughout, 1.2 with two at
+// the end (the most where the short side is under 65; 1.3 at 512 x 2048 with few strong
+// directions), and 1.0 with single steps; two matrices of 512 x 128 take 63.0, 65.8 and
+// 68.6 us, 2048 x 8192 1438, 1667 and 1887.
 uint32_t segment_steps(const mg_newton_schulz& ns, uint32_t m, uint32_t left, bool hidden) {
     if (m < (hidden ? 32 : 65) || fabsf(ns.a) > 4.0f) return 1;
     return left == 2 || (hidden && !(left & 1)) ? 2 : 1;
@@ -236,7 +237,7 @@ int newton_schulz_short(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
     double reach = 1.0;
     a.start = 1;
     for (uint32_t left = ns.steps; left; a.start = 0) {
-        a.steps = segment_steps(ns, m, left, a.step || a.dst.type != MG_TYPE_FP32);
+        a.steps = segment_steps(ns, m, left, a.dst.type != MG_TYPE_FP32);
         double most = step_bounds(ns, &reach);
         if (a.steps == 2) most *= step_bounds(ns, &reach);
         a.unit_q = a.steps == 1 ? kUnitP : unit_of(most);
@@ -281,7 +282,7 @@ int newton_schulz_tiled(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
     hipLaunchKernelGGL(dev::source_norm_kernel, dim3(parts, count), dim3(256), 0, st, src, norms);
     MG_HIP(hipGetLastError(), "newton-schulz norm launch");
     const bool tall = src.rows > src.cols;
-    const bool hidden = fin.step || fin.dst.type != MG_TYPE_FP32;
+    const bool hidden = fin.dst.type != MG_TYPE_FP32;
     // A 16-bit source fits the high halves: two products less for the first A, one for the
     // first X' (2048 x 8192: 1583 us without, 1457 with).
     bool exact = src.in.type != MG_TYPE_FP32 && !src.momentum.data && segment_steps(ns, w.m, w.n, ns.steps, hidden) < ns.steps;

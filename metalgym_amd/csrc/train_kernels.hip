@@ -22,7 +22,7 @@
 //  4. adam: every workgroup adds the partial norms in the same fixed order
 //     (so no cross-workgroup synchronisation is needed), applies the clip
 //     scale and Adam (model/optimizer.metal:23-60). With mg_ppo_set_muon the
-//     block matrices take the Muon update first (muon.hip, four launches for the
+//     block matrices take the Muon update first (muon.hip, five launches for the
 //     default iteration), and this launch only writes their copies.
 //
 // Every reduction has a fixed order, so a rerun gives the same bits (the
