@@ -497,7 +497,8 @@ typedef struct mg_newton_schulz {
  * at data[k stride + i ld + j]. ld 0: cols; stride 0: rows ld. rows and cols are
  * at least 1 and at most 65536, the smaller at most 8192; count may be 0, at most
  * 65535; ld is under 2^31 and stride at most 2^44. type is MG_TYPE_*. Matrices of one
- * batch must not overlap. */
+ * batch must not overlap: they lie one after another, or side by side as column panels
+ * of one array (stride at least cols, and all of them within a row's ld). */
 typedef struct mg_matrices {
     void* data;
     uint64_t ld;

@@ -143,8 +143,15 @@ int check_batch(const char* what, const char* name, const mg_matrices* in, dev::
     MG_CHECK(ld >= in->cols && ld < (1ull << 31), MG_ERR_INVALID, "%s: %s: ld %llu must be in [cols, 2^31)", what, name,
              (unsigned long long)ld);
     const uint64_t stride = in->stride ? in->stride : in->rows * ld;
-    MG_CHECK(in->count <= 1 || (stride >= (in->rows - 1) * ld + in->cols && stride <= (1ull << 44)), MG_ERR_INVALID,
-             "%s: %s: stride %llu: the matrices overlap", what, name, (unsigned long long)stride);
+    if (in->count > 1) {
+        MG_CHECK(stride <= (1ull << 44), MG_ERR_INVALID, "%s: %s: stride %llu is out of range", what, name,
+                 (unsigned long long)stride);
+        // one after another, or side by side: column panels of rows of ld
+        const bool after = stride >= (in->rows - 1) * ld + in->cols;
+        const bool beside = stride >= in->cols && (in->count - 1) * stride + in->cols <= ld;
+        MG_CHECK(after || beside, MG_ERR_INVALID, "%s: %s: stride %llu: the matrices overlap", what, name,
+                 (unsigned long long)stride);
+    }
     *out = dev::Batch{in->data, (size_t)stride, (uint32_t)ld, in->type};
     return MG_OK;
 }
