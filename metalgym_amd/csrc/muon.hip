@@ -165,7 +165,7 @@ int check_same(const char* what, const mg_matrices* a, const mg_matrices* b) {
 
 // The workspace of a batch.
 struct Workspace {
-    size_t norms, rest, x, xt[2], gram, product, poly, q[2], total;  // byte offsets
+    size_t norms, scales, x, xt[2], gram, product, poly, q[2], total;  // byte offsets
     uint32_t m, n, mp, np;
     TileEdges tile;
     Workspace(uint32_t count, uint32_t rows, uint32_t cols) {
@@ -182,7 +182,7 @@ struct Workspace {
             return at;
         };
         norms = take((size_t)count * dev::kNormParts * 8);
-        rest = take((size_t)count * 4);
+        scales = take((size_t)count * sizeof(dev::MatrixScale));
         x = take(wide), xt[0] = take(tall), xt[1] = take(tall);
         gram = take(square), product = take(square), poly = take(square), q[0] = take(square), q[1] = take(square);
     }
@@ -241,13 +241,16 @@ int newton_schulz_short(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
     a.partial = partial[to];
     hipLaunchKernelGGL((dev::short_first_kernel<MP>), slabs, dim3(Shape::THREADS), 0, st, a);
     MG_HIP(hipGetLastError(), "newton-schulz first launch");
-    double reach = 1.0;
+    double reach = 1.0, growth = 1.0;
     a.start = 1;
     for (uint32_t left = ns.steps; left; a.start = 0) {
         a.steps = segment_steps(ns, m, left, a.dst.type != MG_TYPE_FP32);
         double most = step_bounds(ns, &reach);
         if (a.steps == 2) most *= step_bounds(ns, &reach);
         a.unit_q = a.steps == 1 ? kUnitP : unit_of(most);
+        a.growth_in = (float)(growth < 1e30 ? growth : 1e30);
+        growth *= most;
+        a.growth = (float)(growth < 1e30 ? growth : 1e30);
         left -= a.steps;
         a.partial_in = partial[to], a.partial = partial[to ^= 1];
         if (left)
@@ -293,21 +296,24 @@ int newton_schulz_tiled(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
     // A 16-bit source fits the high halves: two products less for the first A, one for the
     // first X' (2048 x 8192: 1583 us without, 1457 with).
     bool exact = src.in.type != MG_TYPE_FP32 && !src.momentum.data && segment_steps(ns, w.m, w.n, ns.steps, hidden) < ns.steps;
-    float* const rest = reinterpret_cast<float*>(base + w.rest);
+    dev::MatrixScale* const scales = reinterpret_cast<dev::MatrixScale*>(base + w.scales);
     const dim3 tiles64((tall ? w.mp : w.np) / 64, (tall ? w.np : w.mp) / 64, count);
     if (exact)
-        hipLaunchKernelGGL(dev::source_split_kernel<true>, tiles64, dim3(256), 0, st, src, norms, parts, ns.eps, rest, X, XT[0]);
+        hipLaunchKernelGGL(dev::source_split_kernel<true>, tiles64, dim3(256), 0, st, src, norms, parts, ns.eps, scales, X, XT[0]);
     else
-        hipLaunchKernelGGL(dev::source_split_kernel<false>, tiles64, dim3(256), 0, st, src, norms, parts, ns.eps, rest, X, XT[0]);
+        hipLaunchKernelGGL(dev::source_split_kernel<false>, tiles64, dim3(256), 0, st, src, norms, parts, ns.eps, scales, X, XT[0]);
     MG_HIP(hipGetLastError(), "newton-schulz split launch");
 
     dev::ProductArgs p{};
-    p.m = w.m, p.rest = rest;
+    p.m = w.m, p.scales = scales;
+    double growth = 1.0;  // of X's singular values, by the segments so far, at most
+    auto as_float = [](double x) { return (float)(x < 1e30 ? x : 1e30); };
     // out = a b' of symmetric results
     auto symmetric = [&](const dev::Planes& a, const dev::Planes& b, uint32_t k, float unit_a, float unit_b,
                          const dev::Planes& out, float unit_out) -> int {
         p.a = a, p.b = b, p.stages = k / dev::kPK, p.tiles_j = sq, p.out = out;
         p.unit = unit_out / (unit_a * unit_b);
+        p.growth = a.base == X.base ? as_float(growth) : 0.0f;
         if (a.base == X.base && exact)
             return launch_product<dev::kExactGram>(st, p, ts, half, count, "newton-schulz product launch");
         return launch_product<dev::kSymmetric>(st, p, ts, half, count, "newton-schulz product launch");
@@ -338,6 +344,7 @@ int newton_schulz_tiled(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
         }
         left -= steps;
         p.a = Q[q], p.b = XT[cur], p.stages = w.mp / dev::kPK, p.tiles_j = nt;
+        p.growth = as_float(growth), growth *= most_q, p.growth_out = as_float(growth);
         if (left) {
             p.out = X, p.out_t = XT[cur ^ 1], p.unit = 1.0f / unit_q;
             rc = exact ? launch_product<dev::kExactUpdate>(st, p, tx, full, count, "newton-schulz update launch")

@@ -20,6 +20,17 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 // 64, so that 2^13 and 2^9 keep them under 2^15, half of binary16's range.
 constexpr float kUnitX = 8192.0f, kUnitA = 8192.0f, kUnitP = 512.0f;
 
+// X's pairs hold 2^extra_exp more where its singular values are known to be small, so
+// that a matrix whose norm is far under eps keeps its bits: most = share x growth, share =
+// |U| / (|U| + eps), which X starts at, and growth what its steps so far may have made of
+// that. Where most is not under a half nothing changes. At a fixed exponent, the result was
+// off by 1e-4 of itself at a share of 1e-5, and nothing was left of it at 1e-13.
+__device__ __forceinline__ int extra_exp(float most) {
+    if (!(most > 0.0f && most < 0.5f)) return 0;
+    const int e = -1 - ilogbf(most);
+    return e < 100 ? e : 100;
+}
+
 // x = hi + lo to 22 bits. x is made one value first: where it is a product or a
 // multiply-add, the compiler otherwise rounds that to binary16 in one step for hi
 // (v_fma_mixlo_f16) and to fp32 for lo, and where the two roundings fall on

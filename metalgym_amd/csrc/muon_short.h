@@ -89,9 +89,9 @@ __device__ __forceinline__ f32x16 pair_mfma(const f16x8 (&a)[2][2], const f16x8 
     return c;
 }
 
-// Exponents of a matrix's X while it is the source's own.
 struct ShortState {
-    int exp[kShortParts];  // of each workgroup's slabs: pairs hold U 2^exp
+    int exp[kShortParts];  // of each workgroup's slabs while X is the source's own: pairs hold U 2^exp
+    float share;           // |U| / (|U| + eps), from the first segment on
 };
 
 struct ShortArgs {
@@ -105,6 +105,7 @@ struct ShortArgs {
     ShortState* state;  // [count]
     float eps;
     uint32_t start;  // the first segment
+    float growth_in, growth;  // extra_exp's, of this segment's X and of the next one's
     uint32_t steps;  // 1 or 2
     float a, b, c;
     float unit_q;
@@ -344,7 +345,8 @@ __global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_step_kernel(con
         }
     };
     load_slab(blockIdx.x);
-    const ShortState& state = a.state[mat];
+    ShortState& state = a.state[mat];
+    float share = a.start ? 0.0f : state.share;  // on its way under the sums
     int least = kMostExp;
     if (a.start)
         for (uint32_t p = 0; p < a.parts; ++p) least = state.exp[p] < least ? state.exp[p] : least;
@@ -388,6 +390,12 @@ __global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_step_kernel(con
         const float scale = 1.0f / (sqrtf(trace) + a.eps * ldexpf(1.0f, least));
         to_out = scale * scale * kUnitA;
         to_x = scale * ldexpf(1.0f, least - state.exp[blockIdx.x]) / a.unit_q;
+        share = sqrtf(trace) * scale;
+        if (!FINAL && blockIdx.x == 0 && threadIdx.x == 0) state.share = share;
+    } else {
+        const int extra = extra_exp(share * a.growth_in);
+        to_out = ldexpf(to_out, -2 * extra);
+        to_x = ldexpf(to_x, -extra);
     }
     // op -1 stores A; then the products of a segment, each of two of the matrices in
     // LDS, over one of them; the last leaves Q
@@ -431,7 +439,7 @@ __global__ void __launch_bounds__(ShortShape<MP>::THREADS) short_step_kernel(con
     }
     const f16* const q = lds[last == 0];
     f16* const rows = lds[last != 0];
-    if (!FINAL) to_x *= kUnitX;
+    if (!FINAL) to_x = ldexpf(to_x * kUnitX, extra_exp(share * a.growth));
     const bool tall = a.src.rows > a.src.cols;
     const int jb = wave % S::CB, b = wave / S::CB;  // the wave's columns of X and rows of Q
     f32x16 gram = {};

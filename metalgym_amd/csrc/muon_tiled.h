@@ -73,12 +73,16 @@ __global__ void __launch_bounds__(256) source_norm_kernel(const SourceArgs a, do
     if (threadIdx.x == 0) partial[(size_t)k * gridDim.x + blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
 
-// kUnitX / (|U| + eps) as 2^exp rest in every thread, rest in [1, 2), or NaN where the
-// norm is not finite. The power is applied as an exponent: as a factor, of matrices near
-// fp32's largest it would be subnormal, with few bits left.
+// kUnitX 2^extra_exp / (|U| + eps) as 2^exp rest in every thread, rest in [1, 2), or NaN
+// where the norm is not finite. The power is applied as an exponent: as a factor, of
+// matrices near fp32's largest it would be subnormal, with few bits left.
 struct SourceScale {
     int exp;
     float rest;
+    float share;  // |U| / (|U| + eps)
+};
+struct MatrixScale {  // what the products need of it
+    float rest, share;
 };
 __device__ __forceinline__ SourceScale source_scale(const double* partial, uint32_t parts, float eps,
                                                     SourceScale* shared) {
@@ -91,7 +95,8 @@ __device__ __forceinline__ SourceScale source_scale(const double* partial, uint3
             const double norm = sqrt(s);
             const bool finite = norm < __builtin_huge_val();
             const double scale = finite ? (double)kUnitX / (norm + (double)eps) : 1.0;
-            shared->exp = ilogb(scale);
+            shared->share = finite ? (float)(norm / (norm + (double)eps)) : 1.0f;
+            shared->exp = ilogb(scale) + extra_exp(shared->share);
             shared->rest = finite ? (float)ldexp(scale, -ilogb(scale)) : __builtin_nanf("");
         }
     }
@@ -121,21 +126,21 @@ struct Planes {
     }
 };
 
-// U / (|U| + eps) times kUnitX as pairs, X [mp][np] and its transpose XT [np][mp],
+// U / (|U| + eps) times kUnitX 2^extra_exp as pairs, X [mp][np] and its transpose XT [np][mp],
 // zeros in the padding; one 64 x 64 tile of the source a workgroup. A thread's
 // elements are a run along one of the two; the other takes four threads'.
 // EXACT: a power of two takes the place of the factor, so that a 16-bit source fits the
 // high halves (under 2^-27 of the norm to 2^-38 of it) and the low ones, which nothing
-// reads, are not written. rest[k] is what is left of the factor.
+// reads, are not written; what is left of the factor goes to scales[k].
 template <bool EXACT>
 __global__ void __launch_bounds__(256) source_split_kernel(const SourceArgs a, const double* partial, uint32_t parts,
-                                                           float eps, float* rest, Planes X, Planes XT) {
+                                                           float eps, MatrixScale* scales, Planes X, Planes XT) {
     __shared__ SourceScale shared;
     const uint32_t k = blockIdx.z, i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
     float u[16];
     tile_load<false>(a, k, i0, j0, u);
     const SourceScale scale = source_scale(partial + (size_t)k * parts, parts, eps, &shared);
-    if (EXACT && threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) rest[k] = scale.rest;
+    if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) scales[k] = MatrixScale{scale.rest, scale.share};
     const float own = EXACT ? 1.0f : scale.rest;
     const bool tall = a.rows > a.cols;
     const Planes& by_column = tall ? X : XT;  // rows of it are the source's columns
@@ -173,7 +178,8 @@ struct ProductArgs {
     uint32_t stages;   // K / kPK, a multiple of 4
     uint32_t tiles_j;  // tile columns (symmetric results: tile rows and columns)
     float unit;        // takes the operands' exponents out of the sums and puts the result's in
-    const float* rest;  // kExact..: each matrix's factor of X
+    const MatrixScale* scales;
+    float growth, growth_out;  // extra_exp's, of X in the product, or 0 without X, and of the X that comes out
     Planes out, out_t;  // X [i][j] and XT [j][i], or a symmetric out
     // kPolynomial
     Planes gram;
@@ -233,6 +239,8 @@ __global__ void __launch_bounds__(512) product_kernel(const ProductArgs p) {
         const uint32_t tiles_i = gridDim.x / p.tiles_j;
         ti = tile % tiles_i, tj = tile / tiles_i;
     }
+    // on its way under the products
+    const MatrixScale own = KIND == kPolynomial ? MatrixScale{} : p.scales[mat];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     // a stage's 32-row blocks (4 KB), a's first, go to the waves in order: a block each
     // at T = 128, half of one at 64
@@ -318,8 +326,14 @@ __global__ void __launch_bounds__(512) product_kernel(const ProductArgs p) {
     __syncthreads();
     constexpr int N = Q == 2 ? 16 : 8;  // registers of a tile that a wave ends up with
     float unit = p.unit;
-    if constexpr (KIND == kExactGram) unit *= p.rest[mat] * p.rest[mat];
-    if constexpr (KIND == kExactUpdate) unit *= p.rest[mat];
+    if constexpr (KIND != kPolynomial) {
+        if (p.growth > 0.0f) {
+            const int extra = extra_exp(own.share * p.growth);
+            if constexpr (KIND == kExactGram) unit *= own.rest * own.rest;
+            if constexpr (KIND == kExactUpdate) unit *= own.rest;
+            unit = ldexpf(unit, kX ? extra_exp(own.share * p.growth_out) - extra : kResult ? -extra : -2 * extra);
+        }
+    }
     float* const trade = reinterpret_cast<float*>(lds);
     float got[2][N];
     auto keep = [&](int qj, int e, bool other) -> float {
