@@ -165,7 +165,7 @@ int check_same(const char* what, const mg_matrices* a, const mg_matrices* b) {
 
 // The workspace of a batch.
 struct Workspace {
-    size_t norms, scales, x, xt[2], gram, product, poly, q[2], total;  // byte offsets
+    size_t norms, scales, x, xt[2], gram, product, poly[2], both, total;  // byte offsets
     uint32_t m, n, mp, np;
     TileEdges tile;
     Workspace(uint32_t count, uint32_t rows, uint32_t cols) {
@@ -184,7 +184,7 @@ struct Workspace {
         norms = take((size_t)count * dev::kNormParts * 8);
         scales = take((size_t)count * sizeof(dev::MatrixScale));
         x = take(wide), xt[0] = take(tall), xt[1] = take(tall);
-        gram = take(square), product = take(square), poly = take(square), q[0] = take(square), q[1] = take(square);
+        gram = take(square), product = take(square), poly[0] = take(square), poly[1] = take(square), both = take(square);
     }
 };
 
@@ -248,9 +248,9 @@ int newton_schulz_short(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
         double most = step_bounds(ns, &reach);
         if (a.steps == 2) most *= step_bounds(ns, &reach);
         a.unit_q = a.steps == 1 ? kUnitP : unit_of(most);
-        a.growth_in = (float)(growth < 1e30 ? growth : 1e30);
+        a.growth_in = (float)growth;
         growth *= most;
-        a.growth = (float)(growth < 1e30 ? growth : 1e30);
+        a.growth = (float)growth;
         left -= a.steps;
         a.partial_in = partial[to], a.partial = partial[to ^= 1];
         if (left)
@@ -283,8 +283,8 @@ int newton_schulz_tiled(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
     const dev::Planes X = planes(w.x, w.mp, w.np);
     const dev::Planes XT[2] = {planes(w.xt[0], w.np, w.mp), planes(w.xt[1], w.np, w.mp)};
     const dev::Planes gram = planes(w.gram, w.mp, w.mp), prod = planes(w.product, w.mp, w.mp),
-                      poly = planes(w.poly, w.mp, w.mp);
-    const dev::Planes Q[2] = {planes(w.q[0], w.mp, w.mp), planes(w.q[1], w.mp, w.mp)};
+                      P = planes(w.poly[0], w.mp, w.mp), next = planes(w.poly[1], w.mp, w.mp),
+                      both = planes(w.both, w.mp, w.mp);
     const uint32_t tiles = ((src.rows + 63) / 64) * ((src.cols + 63) / 64);
     const uint32_t parts = tiles < (uint32_t)dev::kNormParts ? tiles : dev::kNormParts;
     const uint32_t ts = w.tile.square, tx = w.tile.x, sq = w.mp / ts, mt = w.mp / tx, nt = w.np / tx;
@@ -306,14 +306,13 @@ int newton_schulz_tiled(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
 
     dev::ProductArgs p{};
     p.m = w.m, p.scales = scales;
-    double growth = 1.0;  // of X's singular values, by the segments so far, at most
-    auto as_float = [](double x) { return (float)(x < 1e30 ? x : 1e30); };
+    double growth = 1.0;  // extra_exp's
     // out = a b' of symmetric results
     auto symmetric = [&](const dev::Planes& a, const dev::Planes& b, uint32_t k, float unit_a, float unit_b,
                          const dev::Planes& out, float unit_out) -> int {
         p.a = a, p.b = b, p.stages = k / dev::kPK, p.tiles_j = sq, p.out = out;
         p.unit = unit_out / (unit_a * unit_b);
-        p.growth = a.base == X.base ? as_float(growth) : 0.0f;
+        p.growth = a.base == X.base ? (float)growth : 0.0f;
         if (a.base == X.base && exact)
             return launch_product<dev::kExactGram>(st, p, ts, half, count, "newton-schulz product launch");
         return launch_product<dev::kSymmetric>(st, p, ts, half, count, "newton-schulz product launch");
@@ -328,23 +327,21 @@ int newton_schulz_tiled(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
     for (uint32_t left = ns.steps; left;) {
         const uint32_t steps = segment_steps(ns, w.m, w.n, left, hidden);
         if ((rc = symmetric(X, X, w.np, kUnitX, kUnitX, gram, kUnitA))) return rc;
-        int q = 0;
         float unit_q = kUnitP;
         double most_q = step_bounds(ns, &reach);
-        if ((rc = polynomial(Q[0]))) return rc;
-        for (uint32_t k = 1; k < steps; ++k) {
-            const dev::Planes& last = k == 1 ? Q[0] : poly;
-            if ((rc = symmetric(last, gram, w.mp, kUnitP, kUnitA, prod, kUnitA)) ||
-                (rc = symmetric(last, prod, w.mp, kUnitP, kUnitA, gram, kUnitA)) || (rc = polynomial(poly)))
+        if ((rc = polynomial(P))) return rc;
+        if (steps == 2) {
+            if ((rc = symmetric(P, gram, w.mp, kUnitP, kUnitA, prod, kUnitA)) ||
+                (rc = symmetric(P, prod, w.mp, kUnitP, kUnitA, gram, kUnitA)) || (rc = polynomial(next)))
                 return rc;
             most_q *= step_bounds(ns, &reach);
-            const float unit = unit_of(most_q);
-            if ((rc = symmetric(poly, Q[q], w.mp, kUnitP, unit_q, Q[q ^ 1], unit))) return rc;
-            unit_q = unit, q ^= 1;
+            unit_q = unit_of(most_q);
+            if ((rc = symmetric(next, P, w.mp, kUnitP, kUnitP, both, unit_q))) return rc;
         }
+        const dev::Planes& Q = steps == 2 ? both : P;
         left -= steps;
-        p.a = Q[q], p.b = XT[cur], p.stages = w.mp / dev::kPK, p.tiles_j = nt;
-        p.growth = as_float(growth), growth *= most_q, p.growth_out = as_float(growth);
+        p.a = Q, p.b = XT[cur], p.stages = w.mp / dev::kPK, p.tiles_j = nt;
+        p.growth = (float)growth, growth *= most_q, p.growth_out = (float)growth;
         if (left) {
             p.out = X, p.out_t = XT[cur ^ 1], p.unit = 1.0f / unit_q;
             rc = exact ? launch_product<dev::kExactUpdate>(st, p, tx, full, count, "newton-schulz update launch")
@@ -355,7 +352,7 @@ int newton_schulz_tiled(hipStream_t st, const mg_newton_schulz& ns, uint32_t cou
         } else {
             p.dst = fin.dst, p.step = fin.step, p.keep = fin.keep, p.rate = fin.rate, p.rows = src.rows, p.cols = src.cols;
             p.unit = 1.0f / (unit_q * kUnitX);
-            if (tall) p.a = XT[cur], p.b = Q[q], p.tiles_j = mt;
+            if (tall) p.a = XT[cur], p.b = Q, p.tiles_j = mt;
             rc = tall ? launch_product<dev::kFinalTall>(st, p, tx, full, count, "newton-schulz result launch")
                       : launch_product<dev::kFinal>(st, p, tx, full, count, "newton-schulz result launch");
             if (rc) return rc;

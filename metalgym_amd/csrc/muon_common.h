@@ -23,7 +23,9 @@ constexpr float kUnitX = 8192.0f, kUnitA = 8192.0f, kUnitP = 512.0f;
 // X's pairs hold 2^extra_exp more where its singular values are known to be small, so
 // that a matrix whose norm is far under eps keeps its bits: most = share x growth, share =
 // |U| / (|U| + eps), which X starts at, and growth what its steps so far may have made of
-// that. Where most is not under a half nothing changes. At a fixed exponent, the result was
+// that, the product of their largest |a + b s^2 + c s^4| (an odd polynomial of degree 5
+// that takes [-r, r] to [-r', r'] has p(s) / s at most 5 r' / r, so it is at most 2 5^32,
+// well inside fp32). Where most is not under a half nothing changes. At a fixed exponent, the result was
 // off by 1e-4 of itself at a share of 1e-5, and nothing was left of it at 1e-13.
 __device__ __forceinline__ int extra_exp(float most) {
     if (!(most > 0.0f && most < 0.5f)) return 0;
@@ -31,15 +33,9 @@ __device__ __forceinline__ int extra_exp(float most) {
     return e < 100 ? e : 100;
 }
 
-// x = hi + lo to 22 bits. x is made one value first: where it is a product or a
-// multiply-add, the compiler otherwise rounds that to binary16 in one step for hi
-// (v_fma_mixlo_f16) and to fp32 for lo, and where the two roundings fall on
-// different sides of a tie, hi and lo are off by a step of hi.
-__device__ __forceinline__ void split(float x, f16& hi, f16& lo) {
-    asm("" : "+v"(x));
-    hi = (f16)x;
-    lo = (f16)(x - (float)hi);
-}
+// x f = hi + lo to 22 bits. The product is made one value first: the compiler otherwise
+// rounds it to binary16 in one step for hi (v_fma_mixlo_f16) and to fp32 for lo, and where
+// the two roundings fall on different sides of a tie, hi and lo are off by a step of hi.
 __device__ __forceinline__ void split4(const float (&x)[4], float f, f16x4& hi, f16x4& lo) {
     f32x4 v;
 #pragma unroll

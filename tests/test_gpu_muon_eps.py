@@ -41,6 +41,21 @@ def test_large_eps(mg, rows, cols, steps, coeffs, eps):
         check_orthogonal(got[k], g[k], "fp32", steps=steps, coeffs=coeffs, eps=eps)
 
 
+@pytest.mark.parametrize("rows,cols", [(60, 200), (200, 170)])
+def test_the_largest_growth(mg, rows, cols):
+    """0.998 of Chebyshev's polynomial (itself takes 1 + 2^-52 out of [-2, 2] in 13 steps)
+    makes up to 4.99^32 = 2e22 of a singular value: from 2^-80 and less it stays a power,
+    and then is bounded by the polynomial alone."""
+    coeffs = (4.99, -19.96, 15.968)
+    ns = mg.NewtonSchulz(32, *coeffs, 1e-7)
+    g = gradients(np.random.RandomState(23), 3, rows, cols)
+    g /= np.linalg.norm(g, axis=(1, 2), keepdims=True)
+    g = decode(encode(g * 2.0 ** np.array([-80.0, -126.0, -138.0])[:, None, None], "fp32"), "fp32")
+    got = run_orth(mg, g, ns=ns)
+    assert np.isfinite(got).all()
+    assert all(np.linalg.svd(x, compute_uv=False).max() < 1.1 for x in got)
+
+
 @pytest.mark.parametrize("rows,cols", [(128, 512), (200, 170)])
 def test_a_step_by_a_vanishing_gradient(mg, rows, cols):
     from test_gpu_muon import iterate
