@@ -418,7 +418,9 @@ enum { MG_TYPE_FP32 = 0, MG_TYPE_BF16 = 1, MG_TYPE_FP16 = 2 };
  * to the arrays' type; rstd = 1 / sqrt(var + eps), var the mean of (s - mean)^2.
  * Row r of an array begins r * its ld elements after the array (ld 0: cols).
  * x, residual, sum and y are of `type` (MG_TYPE_*), the rest fp32; statistics
- * and products are fp32, y is rounded once. y may be x, residual or sum, and sum
+ * and products are fp32, y is rounded once; a row whose sum or sum of squared
+ * deviations passes fp32's range (deviations past 1.8e19 / sqrt(cols)) is not
+ * normalised: y is beta or NaN. y may be x, residual or sum, and sum
  * may be x or residual, where both have one ld. rows may be 0; cols is at least
  * 1 and at most 2^24, eps finite and not negative. */
 typedef struct mg_layernorm_args {
@@ -482,9 +484,11 @@ int mg_layernorm_backward(void* stream, const mg_layernorm_backward_args* args);
  * steps is in [1, 32], eps positive and finite; the polynomial must keep [0, 1]
  * inside [-2, 2] over the steps and a + b s^2 + c s^4 inside [-64, 64] there. The
  * products go through the matrix units as pairs of binary16 halves (22 bits,
- * three products, fp32 sums), for every type: a small singular value's error grows
- * by a with each step, so one 16-bit product would lose the small directions of
- * a matrix with a few strong ones. */
+ * three products, fp32 sums; one or two where a 16-bit source needs no second half),
+ * for every type: a small singular value's error grows by a with each step, so one
+ * 16-bit product would lose the small directions of a matrix with a few strong ones.
+ * By measurement an fp32 result is off by at most 1.3 times what the plain iteration in
+ * fp32 is, or with a side under 16 by 1.4e-6 of its norm; a 16-bit one by its rounding. */
 typedef struct mg_newton_schulz {
     uint32_t steps;
     float a;
@@ -544,12 +548,14 @@ int mg_muon_step(void* stream, const mg_muon_config* config, const mg_matrices* 
  * parameters and the head stay on Adam at the model's lr. The momentum lies in the
  * block matrices' part of mg_ppo_adam_state's m. A change of optimiser sets that
  * part of m and v to 0, and Adam's bias correction of the block matrices starts anew
- * with them. Blocking. */
+ * with them. Muon's launches take about 66 us of a minibatch. Blocking. */
 int mg_ppo_set_muon(mg_ppo* model, const mg_muon_config* config);
 
 /* ---------------------------------------------------------------------------
  * Kernel timing for measurement: when enabled, the library records HIP events
- * around each launch on the stream it uses and accumulates durations.
+ * around each launch of the kernels below on the stream it uses and accumulates
+ * durations. The block matrices' Muon update counts as MG_K_ADAM; the training
+ * operators' own calls are not recorded.
  * ------------------------------------------------------------------------- */
 enum {
     MG_K_ROLLOUT = 0,

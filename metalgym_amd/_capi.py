@@ -98,7 +98,7 @@ class LayernormBackwardArgs(C.Structure):
 
 
 class NewtonSchulz(C.Structure):
-    """mg_newton_schulz; steps 0 stands for the default iteration."""
+    """mg_newton_schulz. In a MuonConfig, steps 0 stands for the default iteration."""
     _fields_ = [("steps", u32)] + [(n, f32) for n in ("a", "b", "c", "eps")]
 
 

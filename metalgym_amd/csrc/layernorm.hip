@@ -6,16 +6,18 @@
 // come from one pass over memory. Rows of up to 1024 columns take a group inside
 // a wave (its sums are lane exchanges, no barrier), up to 16384 a workgroup; a
 // group walks over rows with gamma (and beta, or the gradient's sums) in its
-// registers. Wider rows are read again from L2 for each pass. The kernels are
+// registers; the backward of 8193 to 16384 columns, and of 513 to 1023 in fp32, has more
+// values a lane than registers and keeps some in scratch (28 to 172 bytes a lane, 12 at
+// 513 to 1023). Wider rows are read again from L2 for each pass. The kernels are
 // bound by HBM: 131072 x 128 fp32 with a residual 42 us (6.4 TB/s, where a copy of
-// 1 GiB reaches 5.0), 4095 x 8192 bf16 45, the backward of 262144 x 128 99 us (5.4).
-// Small calls are launches: 64 x 128 2.4 us, the backward of 4096 x 128 4.7 + 3.3.
+// 1 GiB reaches 5.0), 4095 x 8192 bf16 44, the backward of 262144 x 128 100 us (5.4).
+// Small calls are launches: 64 x 128 2.4 us, the backward of 4096 x 128 4.6 + 3.3.
 //
 // The backward's dgamma and dbeta are sums over all rows. Each lane adds its
 // rows' terms for the columns it holds; a workgroup adds its groups' sums and
 // writes one partial row, and a second launch adds the partial rows in fixed
-// order: chains of at most rows / (groups of the grid) terms, then of 16, with no
-// atomics.
+// order: chains of rows / (groups of the grid) terms, 32 slices of up to 32 partial
+// rows, then the slices, with no atomics.
 #include <type_traits>
 
 #include "kernels.h"
@@ -454,8 +456,8 @@ NormShape norm_shape(uint32_t cols) {
 // Workgroups of the backward pass, each of which writes a partial row: two a CU
 // where a workgroup holds many rows; one a CU (of up to 1024 threads) for wide
 // rows, whose partial rows are traffic. Workgroups of 256 threads (1025 to 2048 columns)
-// are two waves a SIMD at four a CU, where each then has eight rows: 22369 x 1500 fp32
-// 120 us with two a CU, 87 with four; 4000 x 1500 bf16 17.9 and 18.9.
+// are two waves a SIMD at two a CU; they go four a CU where each then has eight rows:
+// 22369 x 1500 fp32 120 us with two a CU, 87 with four; 4000 x 1500 bf16 17.9 and 18.9.
 uint32_t backward_parts(uint32_t rows, uint32_t cols) {
     if (!rows) return 0;
     if (cols > kNormCols) return rows < kWideParts ? rows : kWideParts;
