@@ -552,6 +552,181 @@ int mg_muon_step(void* stream, const mg_muon_config* config, const mg_matrices* 
 int mg_ppo_set_muon(mg_ppo* model, const mg_muon_config* config);
 
 /* ---------------------------------------------------------------------------
+ * Operators of a policy with memory: a short causal convolution and a selective
+ * state space scan over the rows of a rollout, forward, backward and, with steps
+ * = 1, a step at a time. No reference counterpart. As above: device pointers,
+ * asynchronous, no allocation, fixed-order sums, workspaces (256-byte aligned) and
+ * overlaps. Rows: step t of sequence n is row t step_rows + n seq_rows of
+ * every array of rows (both 0: step_rows = seqs, seq_rows = 1, the slots'
+ * [steps][seqs]; steps one after another: step_rows = 1, seq_rows = steps), row r
+ * of an array begins r * its ld elements after it (ld 0: packed). Rows must not
+ * overlap. reset holds a byte a row (NULL: none): not 0 where an episode begins with
+ * that step, which then sees nothing of what was before (a gym's done flags, as they are
+ * before the step). lengths holds the steps of each sequence (NULL: steps, which is
+ * also the most); rows behind a sequence's end are neither read nor written. A
+ * sequence that holds NaN or infinity does not reach others, nor episodes that
+ * begin after it. steps or seqs may be 0; channels is at most 65536.
+ * ------------------------------------------------------------------------- */
+
+/* pre[t] = bias + sum over k of weight[k] x[t - (taps - 1) + k], y = pre, or with
+ * silu pre / (1 + exp(-pre)). Steps before the call are initial's, the oldest first, or
+ * 0. final becomes the last taps - 1 inputs, 0 where they are of an earlier episode; it
+ * may be initial. taps is 2, 3 or 4. Sums are fp32, y is rounded once. */
+typedef struct mg_causal_conv_args {
+    const void* x;
+    const float* weight; /* [channels][taps] */
+    const float* bias;   /* [channels], NULL: 0 */
+    void* y;
+    const uint8_t* reset;
+    const uint32_t* lengths;
+    const void* initial; /* [seqs][taps - 1][channels] of type, nullable */
+    void* final;         /* the same, nullable */
+    uint64_t x_ld;
+    uint64_t y_ld;
+    uint64_t step_rows;
+    uint64_t seq_rows;
+    uint32_t steps;
+    uint32_t seqs;
+    uint32_t channels;
+    uint32_t taps;
+    uint32_t type;
+    uint32_t silu;
+} mg_causal_conv_args;
+int mg_causal_conv(void* stream, const mg_causal_conv_args* args);
+
+/* Backward of mg_causal_conv for the gradients dy of y and dfinal of final. dweight and
+ * dbias are sums over all rows. The workspace may be NULL where both are. */
+typedef struct mg_causal_conv_backward_args {
+    const void* x;
+    const float* weight;
+    const float* bias;
+    const void* dy;
+    const uint8_t* reset;
+    const uint32_t* lengths;
+    const void* initial;
+    const void* dfinal; /* nullable: 0 */
+    void* dx;
+    float* dweight; /* nullable */
+    float* dbias;   /* nullable */
+    void* dinitial; /* nullable */
+    uint64_t x_ld;
+    uint64_t dy_ld;
+    uint64_t dx_ld;
+    uint64_t step_rows;
+    uint64_t seq_rows;
+    uint32_t steps;
+    uint32_t seqs;
+    uint32_t channels;
+    uint32_t taps;
+    uint32_t type;
+    uint32_t silu;
+    void* workspace;
+    uint64_t workspace_bytes;
+} mg_causal_conv_backward_args;
+int mg_causal_conv_backward_workspace(uint32_t steps, uint32_t seqs, uint32_t channels, uint32_t taps,
+                                      uint64_t* bytes);
+int mg_causal_conv_backward(void* stream, const mg_causal_conv_backward_args* args);
+
+/* For each channel and its states s: delta = softplus(dt + dt_bias), h[s] = exp(delta
+ * a[s]) h[s] + delta x b[s], y = sum over s of c[s] h[s], + d x, and with z times
+ * z / (1 + exp(-z)). b and c are a row's [groups][states]: channel i takes those of group
+ * i / (channels / groups). a must not be positive; a decay
+ * under 2^-126 counts as 0. h begins as initial, or 0, and ends as
+ * final, which may be initial. checkpoints takes the state before every MG_SCAN_CHUNK
+ * steps (those of steps that a sequence has), which the backward pass starts from. states
+ * is at most 256, groups divides channels. h and the sums are fp32 and y is
+ * rounded once. Few sequences of many steps are split over the steps, which takes the
+ * workspace; it may be NULL where its size is 0. */
+enum { MG_SCAN_CHUNK = 64 };
+typedef struct mg_selective_scan_args {
+    const void* x;  /* rows of channels */
+    const void* dt; /* rows of channels */
+    const float* a; /* [channels][states] */
+    const void* b;  /* rows of groups x states */
+    const void* c;  /* rows of groups x states */
+    const float* d;       /* [channels], NULL: 0 */
+    const float* dt_bias; /* [channels], NULL: 0 */
+    const void* z;        /* rows of channels, nullable */
+    void* y;              /* rows of channels */
+    const uint8_t* reset;
+    const uint32_t* lengths;
+    const float* initial; /* [seqs][channels][states], nullable */
+    float* final;         /* the same, nullable */
+    float* checkpoints;   /* [(steps + MG_SCAN_CHUNK - 1) / MG_SCAN_CHUNK][seqs][channels][states], nullable */
+    uint64_t x_ld;
+    uint64_t dt_ld;
+    uint64_t b_ld;
+    uint64_t c_ld;
+    uint64_t z_ld;
+    uint64_t y_ld;
+    uint64_t step_rows;
+    uint64_t seq_rows;
+    uint32_t steps;
+    uint32_t seqs;
+    uint32_t channels;
+    uint32_t states;
+    uint32_t groups;
+    uint32_t type;
+    void* workspace;
+    uint64_t workspace_bytes;
+} mg_selective_scan_args;
+int mg_selective_scan_workspace(uint32_t steps, uint32_t seqs, uint32_t channels, uint32_t states, uint64_t* bytes);
+int mg_selective_scan(void* stream, const mg_selective_scan_args* args);
+
+/* Backward of mg_selective_scan for the gradients dy of y and dfinal of final.
+ * checkpoints are the forward's, and may be NULL where steps is at most MG_SCAN_CHUNK.
+ * da, dd and ddt_bias are sums over all rows, db and dc over a group's channels. */
+typedef struct mg_selective_scan_backward_args {
+    const void* x;
+    const void* dt;
+    const float* a;
+    const void* b;
+    const void* c;
+    const float* d;
+    const float* dt_bias;
+    const void* z;
+    const void* dy;
+    const uint8_t* reset;
+    const uint32_t* lengths;
+    const float* initial;
+    const float* checkpoints;
+    const float* dfinal; /* nullable: 0 */
+    void* dx;
+    void* ddt;
+    void* db;
+    void* dc;
+    void* dz;        /* NULL without z */
+    float* da;       /* nullable */
+    float* dd;       /* nullable */
+    float* ddt_bias; /* nullable */
+    float* dinitial; /* nullable */
+    uint64_t x_ld;
+    uint64_t dt_ld;
+    uint64_t b_ld;
+    uint64_t c_ld;
+    uint64_t z_ld;
+    uint64_t dy_ld;
+    uint64_t dx_ld;
+    uint64_t ddt_ld;
+    uint64_t db_ld;
+    uint64_t dc_ld;
+    uint64_t dz_ld;
+    uint64_t step_rows;
+    uint64_t seq_rows;
+    uint32_t steps;
+    uint32_t seqs;
+    uint32_t channels;
+    uint32_t states;
+    uint32_t groups;
+    uint32_t type;
+    void* workspace;
+    uint64_t workspace_bytes;
+} mg_selective_scan_backward_args;
+int mg_selective_scan_backward_workspace(uint32_t steps, uint32_t seqs, uint32_t channels, uint32_t states,
+                                         uint32_t groups, uint64_t* bytes);
+int mg_selective_scan_backward(void* stream, const mg_selective_scan_backward_args* args);
+
+/* ---------------------------------------------------------------------------
  * Kernel timing for measurement: when enabled, the library records HIP events
  * around each launch of the kernels below on the stream it uses and accumulates
  * durations. The block matrices' Muon update counts as MG_K_ADAM; the training

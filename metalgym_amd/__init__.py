@@ -23,7 +23,11 @@ from ._capi import (  # noqa: F401
     PPOModel,
     PolicyView,
     DeviceBuffer,
+    SCAN_CHUNK,
     build,
+    causal_conv,
+    causal_conv_backward,
+    causal_conv_backward_workspace,
     d2h,
     env_desc,
     env_names,
@@ -36,6 +40,10 @@ from ._capi import (  # noqa: F401
     muon_step,
     orthogonalize,
     orthogonalize_workspace,
+    selective_scan,
+    selective_scan_backward,
+    selective_scan_backward_workspace,
+    selective_scan_workspace,
     timing_enable,
     timing_get,
     timing_reset,

@@ -113,6 +113,42 @@ class MuonConfig(C.Structure):
                                                                                   ("ns", NewtonSchulz)]
 
 
+class CausalConvArgs(C.Structure):
+    """mg_causal_conv_args"""
+    _fields_ = [(n, P) for n in ("x", "weight", "bias", "y", "reset", "lengths", "initial", "final")] + [
+        (n, u64) for n in ("x_ld", "y_ld", "step_rows", "seq_rows")] + [
+        (n, u32) for n in ("steps", "seqs", "channels", "taps", "type", "silu")]
+
+
+class CausalConvBackwardArgs(C.Structure):
+    """mg_causal_conv_backward_args"""
+    _fields_ = [(n, P) for n in ("x", "weight", "bias", "dy", "reset", "lengths", "initial", "dfinal", "dx", "dweight",
+                                 "dbias", "dinitial")] + [
+        (n, u64) for n in ("x_ld", "dy_ld", "dx_ld", "step_rows", "seq_rows")] + [
+        (n, u32) for n in ("steps", "seqs", "channels", "taps", "type", "silu")] + [("workspace", P),
+                                                                                    ("workspace_bytes", u64)]
+
+
+class SelectiveScanArgs(C.Structure):
+    """mg_selective_scan_args"""
+    _fields_ = [(n, P) for n in ("x", "dt", "a", "b", "c", "d", "dt_bias", "z", "y", "reset", "lengths", "initial",
+                                 "final", "checkpoints")] + [
+        (n, u64) for n in ("x_ld", "dt_ld", "b_ld", "c_ld", "z_ld", "y_ld", "step_rows", "seq_rows")] + [
+        (n, u32) for n in ("steps", "seqs", "channels", "states", "groups", "type")] + [("workspace", P),
+                                                                                        ("workspace_bytes", u64)]
+
+
+class SelectiveScanBackwardArgs(C.Structure):
+    """mg_selective_scan_backward_args"""
+    _fields_ = [(n, P) for n in ("x", "dt", "a", "b", "c", "d", "dt_bias", "z", "dy", "reset", "lengths", "initial",
+                                 "checkpoints", "dfinal", "dx", "ddt", "db", "dc", "dz", "da", "dd", "ddt_bias",
+                                 "dinitial")] + [
+        (n, u64) for n in ("x_ld", "dt_ld", "b_ld", "c_ld", "z_ld", "dy_ld", "dx_ld", "ddt_ld", "db_ld", "dc_ld",
+                           "dz_ld", "step_rows", "seq_rows")] + [
+        (n, u32) for n in ("steps", "seqs", "channels", "states", "groups", "type")] + [("workspace", P),
+                                                                                        ("workspace_bytes", u64)]
+
+
 class KernelTimes(C.Structure):
     _fields_ = [("total_ms", C.c_double * len(K_NAMES)), ("launches", C.c_uint64 * len(K_NAMES))]
 
@@ -194,6 +230,13 @@ def lib():
         "mg_orthogonalize_workspace": (I, [P, u32, u32, u32, P]),
         "mg_orthogonalize": (I, [P, P, P, P, P, u64]),
         "mg_muon_step": (I, [P, P, P, P, P, P, u64]),
+        "mg_causal_conv": (I, [P, P]),
+        "mg_causal_conv_backward_workspace": (I, [u32, u32, u32, u32, P]),
+        "mg_causal_conv_backward": (I, [P, P]),
+        "mg_selective_scan_workspace": (I, [u32, u32, u32, u32, P]),
+        "mg_selective_scan": (I, [P, P]),
+        "mg_selective_scan_backward_workspace": (I, [u32, u32, u32, u32, u32, P]),
+        "mg_selective_scan_backward": (I, [P, P]),
         "mg_timing_enable": (I, [I]),
         "mg_timing_get": (I, [P]),
         "mg_timing_reset": (I, []),
@@ -287,6 +330,80 @@ def muon_step(params: Matrices, momentum_buffer: Matrices, grad: Matrices, *, lr
     cfg = MuonConfig(lr, momentum, weight_decay, scale, int(nesterov), ns or NewtonSchulz())
     check(lib().mg_muon_step(stream, C.byref(cfg), C.byref(params), C.byref(momentum_buffer), C.byref(grad), workspace,
                              workspace_bytes))
+
+
+SCAN_CHUNK = 64  # MG_SCAN_CHUNK
+
+
+def causal_conv(x: int, weight: int, y: int, steps: int, seqs: int, channels: int, taps: int, dtype: str = "fp32", *,
+                bias: int = None, silu: bool = False, reset: int = None, lengths: int = None, initial: int = None,
+                final: int = None, x_ld: int = 0, y_ld: int = 0, step_rows: int = 0, seq_rows: int = 0,
+                stream: int = None) -> None:
+    """mg_causal_conv on device addresses; asynchronous on the HIP stream `stream`."""
+    a = CausalConvArgs(x, weight, bias, y, reset, lengths, initial, final, x_ld, y_ld, step_rows, seq_rows, steps,
+                       seqs, channels, taps, TYPES[dtype], int(silu))
+    check(lib().mg_causal_conv(stream, C.byref(a)))
+
+
+def causal_conv_backward_workspace(steps: int, seqs: int, channels: int, taps: int) -> int:
+    n = u64()
+    check(lib().mg_causal_conv_backward_workspace(steps, seqs, channels, taps, C.byref(n)))
+    return n.value
+
+
+def causal_conv_backward(x: int, weight: int, dy: int, dx: int, steps: int, seqs: int, channels: int, taps: int,
+                         dtype: str = "fp32", *, bias: int = None, silu: bool = False, reset: int = None,
+                         lengths: int = None, initial: int = None, dfinal: int = None, dweight: int = None,
+                         dbias: int = None, dinitial: int = None, x_ld: int = 0, dy_ld: int = 0, dx_ld: int = 0,
+                         step_rows: int = 0, seq_rows: int = 0, workspace: int = None, workspace_bytes: int = 0,
+                         stream: int = None) -> None:
+    """mg_causal_conv_backward on device addresses; asynchronous."""
+    a = CausalConvBackwardArgs(x, weight, bias, dy, reset, lengths, initial, dfinal, dx, dweight, dbias, dinitial,
+                               x_ld, dy_ld, dx_ld, step_rows, seq_rows, steps, seqs, channels, taps, TYPES[dtype],
+                               int(silu), workspace, workspace_bytes)
+    check(lib().mg_causal_conv_backward(stream, C.byref(a)))
+
+
+def selective_scan_workspace(steps: int, seqs: int, channels: int, states: int) -> int:
+    n = u64()
+    check(lib().mg_selective_scan_workspace(steps, seqs, channels, states, C.byref(n)))
+    return n.value
+
+
+def selective_scan(x: int, dt: int, y: int, steps: int, seqs: int, channels: int, states: int, dtype: str = "fp32", *,
+                   a: int, b: int, c: int, groups: int = 1, d: int = None, dt_bias: int = None, z: int = None,
+                   reset: int = None, lengths: int = None, initial: int = None, final: int = None,
+                   checkpoints: int = None, x_ld: int = 0, dt_ld: int = 0, b_ld: int = 0, c_ld: int = 0, z_ld: int = 0,
+                   y_ld: int = 0, step_rows: int = 0, seq_rows: int = 0, workspace: int = None,
+                   workspace_bytes: int = 0, stream: int = None) -> None:
+    """mg_selective_scan on device addresses; asynchronous."""
+    p = SelectiveScanArgs(x, dt, a, b, c, d, dt_bias, z, y, reset, lengths, initial, final, checkpoints, x_ld, dt_ld,
+                          b_ld, c_ld, z_ld, y_ld, step_rows, seq_rows, steps, seqs, channels, states, groups,
+                          TYPES[dtype], workspace, workspace_bytes)
+    check(lib().mg_selective_scan(stream, C.byref(p)))
+
+
+def selective_scan_backward_workspace(steps: int, seqs: int, channels: int, states: int, groups: int = 1) -> int:
+    n = u64()
+    check(lib().mg_selective_scan_backward_workspace(steps, seqs, channels, states, groups, C.byref(n)))
+    return n.value
+
+
+def selective_scan_backward(x: int, dt: int, dy: int, steps: int, seqs: int, channels: int, states: int,
+                            dtype: str = "fp32", *, a: int, b: int, c: int, dx: int, ddt: int, db: int, dc: int,
+                            groups: int = 1, d: int = None, dt_bias: int = None, z: int = None, dz: int = None,
+                            reset: int = None, lengths: int = None, initial: int = None, checkpoints: int = None,
+                            dfinal: int = None, da: int = None, dd: int = None, ddt_bias: int = None,
+                            dinitial: int = None, x_ld: int = 0, dt_ld: int = 0, b_ld: int = 0, c_ld: int = 0,
+                            z_ld: int = 0, dy_ld: int = 0, dx_ld: int = 0, ddt_ld: int = 0, db_ld: int = 0,
+                            dc_ld: int = 0, dz_ld: int = 0, step_rows: int = 0, seq_rows: int = 0,
+                            workspace: int = None, workspace_bytes: int = 0, stream: int = None) -> None:
+    """mg_selective_scan_backward on device addresses; asynchronous."""
+    p = SelectiveScanBackwardArgs(x, dt, a, b, c, d, dt_bias, z, dy, reset, lengths, initial, checkpoints, dfinal, dx,
+                                  ddt, db, dc, dz, da, dd, ddt_bias, dinitial, x_ld, dt_ld, b_ld, c_ld, z_ld, dy_ld,
+                                  dx_ld, ddt_ld, db_ld, dc_ld, dz_ld, step_rows, seq_rows, steps, seqs, channels,
+                                  states, groups, TYPES[dtype], workspace, workspace_bytes)
+    check(lib().mg_selective_scan_backward(stream, C.byref(p)))
 
 
 class DeviceBuffer:
