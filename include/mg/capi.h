@@ -727,6 +727,70 @@ int mg_selective_scan_backward_workspace(uint32_t steps, uint32_t seqs, uint32_t
 int mg_selective_scan_backward(void* stream, const mg_selective_scan_backward_args* args);
 
 /* ---------------------------------------------------------------------------
+ * A head over many actions (or tokens): softmax(x w') with w [classes][width], without
+ * its [rows][classes] logits. No reference counterpart (its head of act_dim + 1 columns
+ * lies inside the fused kernels). As the operators above.
+ * ------------------------------------------------------------------------- */
+
+/* Per row, with s = x w': lse = log sum exp s, loss = lse - s[target] (minus the
+ * log-probability of the taken action), entropy = lse - sum softmax(s) s. A target outside
+ * [0, classes) leaves its row out: loss 0, and no gradients; lse and entropy are
+ * written all the same. Row r of x begins r x_ld elements after it, class c of w c w_ld (ld 0: width).
+ * rows (which may be 0) and classes are at most 2^20, width at most 65536. Products of
+ * 16-bit types are exact, those of fp32 go through the matrix units as pairs of
+ * binary16 halves at a power of two for each array: 22 bits, fewer for elements under 2^-17 of
+ * the array's largest. Sums are fp32. */
+typedef struct mg_cross_entropy_args {
+    const void* x;          /* [rows][width] */
+    const void* w;          /* [classes][width] */
+    const int32_t* targets; /* [rows] */
+    float* loss;            /* [rows], nullable, as are the next two */
+    float* lse;
+    float* entropy;
+    uint64_t x_ld;
+    uint64_t w_ld;
+    uint32_t rows;
+    uint32_t classes;
+    uint32_t width;
+    uint32_t type;
+    void* workspace;
+    uint64_t workspace_bytes;
+} mg_cross_entropy_args;
+int mg_cross_entropy_workspace(uint32_t rows, uint32_t classes, uint32_t width, uint32_t type, uint64_t* bytes);
+int mg_cross_entropy(void* stream, const mg_cross_entropy_args* args);
+
+/* Backward of mg_cross_entropy for the gradients dloss of loss and dentropy of
+ * entropy: with p = exp(s - lse), g = dloss (p - [target]) - dentropy p (log p + entropy),
+ * dx = g w, dw = g' x. lse, and where there is a dentropy entropy, are the forward's. The
+ * logits are computed again, a piece of the classes at a time. g is rounded to type for
+ * the two products (binary16 at a power of two, fp32 as pairs); their sums are fp32, rounded once.
+ * A row that is left out adds nothing, whatever it holds. Without rows dw is 0. */
+typedef struct mg_cross_entropy_backward_args {
+    const void* x;
+    const void* w;
+    const int32_t* targets;
+    const float* lse;
+    const float* dloss;    /* [rows] */
+    const float* entropy;  /* [rows], with dentropy */
+    const float* dentropy; /* [rows], nullable: 0 */
+    void* dx;              /* [rows][width], nullable */
+    void* dw;              /* [classes][width], nullable */
+    uint64_t x_ld;
+    uint64_t w_ld;
+    uint64_t dx_ld;
+    uint64_t dw_ld;
+    uint32_t rows;
+    uint32_t classes;
+    uint32_t width;
+    uint32_t type;
+    void* workspace;
+    uint64_t workspace_bytes;
+} mg_cross_entropy_backward_args;
+int mg_cross_entropy_backward_workspace(uint32_t rows, uint32_t classes, uint32_t width, uint32_t type,
+                                        uint64_t* bytes);
+int mg_cross_entropy_backward(void* stream, const mg_cross_entropy_backward_args* args);
+
+/* ---------------------------------------------------------------------------
  * Kernel timing for measurement: when enabled, the library records HIP events
  * around each launch of the kernels below on the stream it uses and accumulates
  * durations. The block matrices' Muon update counts as MG_K_ADAM; the training

@@ -149,6 +149,20 @@ class SelectiveScanBackwardArgs(C.Structure):
                                                                                         ("workspace_bytes", u64)]
 
 
+class CrossEntropyArgs(C.Structure):
+    """mg_cross_entropy_args"""
+    _fields_ = [(n, P) for n in ("x", "w", "targets", "loss", "lse", "entropy")] + [
+        (n, u64) for n in ("x_ld", "w_ld")] + [(n, u32) for n in ("rows", "classes", "width", "type")] + [
+        ("workspace", P), ("workspace_bytes", u64)]
+
+
+class CrossEntropyBackwardArgs(C.Structure):
+    """mg_cross_entropy_backward_args"""
+    _fields_ = [(n, P) for n in ("x", "w", "targets", "lse", "dloss", "entropy", "dentropy", "dx", "dw")] + [
+        (n, u64) for n in ("x_ld", "w_ld", "dx_ld", "dw_ld")] + [
+        (n, u32) for n in ("rows", "classes", "width", "type")] + [("workspace", P), ("workspace_bytes", u64)]
+
+
 class KernelTimes(C.Structure):
     _fields_ = [("total_ms", C.c_double * len(K_NAMES)), ("launches", C.c_uint64 * len(K_NAMES))]
 
@@ -237,6 +251,10 @@ def lib():
         "mg_selective_scan": (I, [P, P]),
         "mg_selective_scan_backward_workspace": (I, [u32, u32, u32, u32, u32, P]),
         "mg_selective_scan_backward": (I, [P, P]),
+        "mg_cross_entropy_workspace": (I, [u32, u32, u32, u32, P]),
+        "mg_cross_entropy": (I, [P, P]),
+        "mg_cross_entropy_backward_workspace": (I, [u32, u32, u32, u32, P]),
+        "mg_cross_entropy_backward": (I, [P, P]),
         "mg_timing_enable": (I, [I]),
         "mg_timing_get": (I, [P]),
         "mg_timing_reset": (I, []),
@@ -404,6 +422,37 @@ def selective_scan_backward(x: int, dt: int, dy: int, steps: int, seqs: int, cha
                                   dx_ld, ddt_ld, db_ld, dc_ld, dz_ld, step_rows, seq_rows, steps, seqs, channels,
                                   states, groups, TYPES[dtype], workspace, workspace_bytes)
     check(lib().mg_selective_scan_backward(stream, C.byref(p)))
+
+
+def cross_entropy_workspace(rows: int, classes: int, width: int, dtype: str = "fp32") -> int:
+    n = u64()
+    check(lib().mg_cross_entropy_workspace(rows, classes, width, TYPES[dtype], C.byref(n)))
+    return n.value
+
+
+def cross_entropy(x: int, w: int, targets: int, rows: int, classes: int, width: int, dtype: str = "fp32", *,
+                  loss: int = None, lse: int = None, entropy: int = None, x_ld: int = 0, w_ld: int = 0,
+                  workspace: int = None, workspace_bytes: int = 0, stream: int = None) -> None:
+    """mg_cross_entropy on device addresses; asynchronous."""
+    a = CrossEntropyArgs(x, w, targets, loss, lse, entropy, x_ld, w_ld, rows, classes, width, TYPES[dtype], workspace,
+                         workspace_bytes)
+    check(lib().mg_cross_entropy(stream, C.byref(a)))
+
+
+def cross_entropy_backward_workspace(rows: int, classes: int, width: int, dtype: str = "fp32") -> int:
+    n = u64()
+    check(lib().mg_cross_entropy_backward_workspace(rows, classes, width, TYPES[dtype], C.byref(n)))
+    return n.value
+
+
+def cross_entropy_backward(x: int, w: int, targets: int, rows: int, classes: int, width: int, dtype: str = "fp32", *,
+                           lse: int, dloss: int, entropy: int = None, dentropy: int = None, dx: int = None,
+                           dw: int = None, x_ld: int = 0, w_ld: int = 0, dx_ld: int = 0, dw_ld: int = 0,
+                           workspace: int = None, workspace_bytes: int = 0, stream: int = None) -> None:
+    """mg_cross_entropy_backward on device addresses; asynchronous."""
+    a = CrossEntropyBackwardArgs(x, w, targets, lse, dloss, entropy, dentropy, dx, dw, x_ld, w_ld, dx_ld, dw_ld, rows,
+                                 classes, width, TYPES[dtype], workspace, workspace_bytes)
+    check(lib().mg_cross_entropy_backward(stream, C.byref(a)))
 
 
 class DeviceBuffer:

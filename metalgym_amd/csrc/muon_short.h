@@ -50,25 +50,6 @@ struct Frags {
     }
 };
 
-// Lane q of each four lanes holds four values of column 4 a + q; gives it value q
-// of the four columns 4 a .. 4 a + 3. Byte permutes with a lane's own selectors:
-// selects become branches here.
-__device__ __forceinline__ f16x4 quad_transpose(f16x4 v) {
-    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-    const uint32_t q = threadIdx.x & 3;
-    const uint32_t halves = q & 1 ? 0x03020706u : 0x05040100u;  // (partner's high, own high) or (own low, partner's low)
-    const uint32_t first = q & 2 ? 0x07060504u : 0x03020100u;   // the permute's first operand, or its second
-    const u32x2 w = __builtin_bit_cast(u32x2, v);  // values (0, 1), (2, 3)
-    // lanes q and q ^ 1 trade halves: even lanes get value 0 of both columns, then 2
-    const uint32_t n0 = __builtin_amdgcn_mov_dpp(w[0], 0xB1, 0xF, 0xF, true);
-    const uint32_t n1 = __builtin_amdgcn_mov_dpp(w[1], 0xB1, 0xF, 0xF, true);
-    const uint32_t p0 = __builtin_amdgcn_perm(n0, w[0], halves), p1 = __builtin_amdgcn_perm(n1, w[1], halves);
-    // lanes q and q ^ 2 trade words: the lower two lanes keep values 0 and 1
-    const uint32_t got = __builtin_amdgcn_mov_dpp(__builtin_amdgcn_perm(p0, p1, first), 0x4E, 0xF, 0xF, true);
-    const u32x2 out = {__builtin_amdgcn_perm(got, p0, first), __builtin_amdgcn_perm(p1, got, first)};
-    return __builtin_bit_cast(f16x4, out);
-}
-
 // a b of pairs over 32 contraction elements (two fragments). The products of low halves
 // come first, so that the sum is of full size in the last two instructions only: each
 // rounds it, and cuts off what its small products have under 2^-25 of its largest, 0.1

@@ -192,13 +192,6 @@ struct ProductArgs {
     float keep, rate;
 };
 
-// Workgroups go to the 8 XCDs in turn, each of which has its own L2: gives every XCD
-// one run of tiles.
-__device__ __forceinline__ uint32_t xcd_run(uint32_t b, uint32_t count) {
-    const uint32_t x = b & 7, each = count >> 3, more = count & 7;
-    return x * each + (x < more ? x : more) + (b >> 3);
-}
-
 // One T x T tile of a product a b' of pairs. Eight waves, T / 2 x T / 2 each as
 // tiles of v_mfma_f32_32x32x16_f16: four of them take the first half of each stage's
 // 32 contraction elements, four the second, and the two halves' sums meet at the end.
