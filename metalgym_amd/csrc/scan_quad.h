@@ -1,0 +1,676 @@
+// The selective scan of 9 to 16 states: four lanes a channel.
+//
+// A quad of lanes holds C channels, four states of each a lane. What a step needs of a
+// channel (delta, delta x, dy) is worked out by one lane of the quad, which does so for every
+// 4 / C th step of one channel, and the others take it by a DPP move; sums over states come
+// back to that lane by two more. B and C lie in LDS as fp32 for a workgroup's four waves, which
+// otherwise run on their own.
+#pragma once
+#include "scan_common.h"
+
+namespace mg {
+namespace dev {
+
+constexpr int kQuadStates = 16;
+constexpr int kWindow = 32;  // steps of B and C in LDS
+
+// Lane n's value in every lane of each quad; n is a constant once loops are unrolled.
+__device__ __forceinline__ float quad_take(int n, float v) {
+    return n == 0 ? dpp_lane<0x00>(v) : n == 1 ? dpp_lane<0x55>(v) : n == 2 ? dpp_lane<0xAA>(v) : dpp_lane<0xFF>(v);
+}
+// Lane n of a quad gets the quad's sum of v[n].
+__device__ __forceinline__ float quad_sums(const float (&v)[4]) {
+    const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
+    const float a = (odd ? v[1] : v[0]) + dpp_lane<0xB1>(odd ? v[0] : v[1]);
+    const float b = (odd ? v[3] : v[2]) + dpp_lane<0xB1>(odd ? v[2] : v[3]);
+    return (high ? b : a) + dpp_lane<0x4E>(high ? a : b);
+}
+
+// A workgroup's channels, a lane's four states of C of them, and the one it works for.
+template <int C>
+struct QuadLane {
+    static constexpr int P = 4 / C;       // steps that a quad's lanes take at once
+    static constexpr int R = kSteps / P;  // times that they do in a round of kSteps
+    static constexpr int CH = 64 * C;     // channels of a workgroup
+    uint32_t group, first, own;  // the quad's first channel, and this lane's
+    bool in;                     // whether that is one
+    int state, held[C];          // the first of the lane's states, and how many it has of each channel
+    f32x4 a2[C];                 // A log2(e)
+
+    __device__ __forceinline__ QuadLane(const ScanArgs& p, uint32_t block) {
+        group = block / p.apiece;
+        const uint32_t limit = (group + 1) * p.per;
+        first = group * p.per + (block - group * p.apiece) * CH + (threadIdx.x >> 2) * C;
+        own = first + threadIdx.x % C;
+        in = own < limit;
+        own = in ? own : limit - 1;
+        state = 4 * (threadIdx.x & 3);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            held[c] = first + c < limit ? (int)p.states - state : 0;
+            a2[c] = load_states(p.a + (size_t)(first + c) * p.states + state, held[c]) * kLog2e;
+        }
+    }
+    __device__ __forceinline__ size_t at(const ScanArgs& p, uint32_t n, int c) const {
+        return ((size_t)n * p.channels + first + c) * p.states + state;
+    }
+    __device__ __forceinline__ void load(const ScanArgs& p, const float* from, uint32_t n, f32x4 (&h)[C]) const {
+#pragma unroll
+        for (int c = 0; c < C; ++c) h[c] = load_states(from + at(p, n, c), held[c]);
+    }
+    __device__ __forceinline__ void store(const ScanArgs& p, float* to, uint32_t n, const f32x4 (&h)[C]) const {
+#pragma unroll
+        for (int c = 0; c < C; ++c) store_states(to + at(p, n, c), held[c], h[c]);
+    }
+    // which of a round's steps the lane's element j is of
+    static __device__ __forceinline__ uint32_t step(int j) { return j * P + (threadIdx.x & 3) / C; }
+    // and which lane of the quad, at which j, has step k of channel c
+    static __device__ __forceinline__ int lane(int k, int c) { return k % P * C + c; }
+};
+
+// A kernel's arguments, read anew: a round's addresses are worked out from them in scalar
+// registers, which held through a kernel would be twice what there are, and be spilled to vector
+// registers' lanes (the gradient's round then moves a hundred of them).
+typedef const __attribute__((address_space(4))) ScanArgs* ArgsAgain;
+__device__ __forceinline__ ArgsAgain args_again() {
+    ArgsAgain p = (ArgsAgain)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+}
+
+// A lane's elements of a row array of one sequence, by buffer loads: the round's address, a
+// step's distance and the lane's own bytes (the host has made sure that eight steps fit 31
+// bits). As pointers each array took two registers a lane, and the backward pass kept its own
+// in scratch. What is past the end or of no channel lies nowhere: it reads 0, and is not written.
+template <class T, int C>
+struct QuadRows {
+    static constexpr uint32_t kNone = 0x80000000u;
+    const char* base;
+    uint32_t by;    // bytes from step to step
+    uint32_t mine;  // the lane's first step and its channel
+    __device__ __forceinline__ QuadRows(const ArgsAgain p, const QuadLane<C>& at, const void* array, uint64_t ld,
+                                        uint32_t n)
+        : base(static_cast<const char*>(array) + n * p->at.seq_rows * ld * sizeof(T)),
+          by((uint32_t)(p->at.step_rows * ld * sizeof(T))),
+          mine(at.in ? QuadLane<C>::step(0) * by + at.own * (uint32_t)sizeof(T) : kNone) {}
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t at(uint32_t t) const {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + (uint64_t)t * by), (short)0, 0x7fffffff,
+                                                 0x00020000);
+    }
+    __device__ __forceinline__ int place(uint32_t t, uint32_t end, int j) const {
+        return (int)(t + QuadLane<C>::step(j) < end ? mine : kNone);
+    }
+    // the lane's elements of the round at t, as they lie: a conversion here would wait for each
+    __device__ __forceinline__ void load(uint32_t t, uint32_t end, T (&v)[QuadLane<C>::R]) const {
+        const __amdgpu_buffer_rsrc_t r = at(t);
+#pragma unroll
+        for (int j = 0; j < QuadLane<C>::R; ++j) {
+            const int s = j * QuadLane<C>::P * (int)by;
+            if constexpr (sizeof(T) == 2)
+                v[j] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(r, place(t, end, j), s, 0));
+            else
+                v[j] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, place(t, end, j), s, 0));
+        }
+    }
+    __device__ __forceinline__ void store(uint32_t t, uint32_t end, const float (&v)[QuadLane<C>::R]) const {
+        const __amdgpu_buffer_rsrc_t r = at(t);
+#pragma unroll
+        for (int j = 0; j < QuadLane<C>::R; ++j) {
+            const int s = j * QuadLane<C>::P * (int)by;
+            if constexpr (sizeof(T) == 2)
+                __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (T)v[j]), r, place(t, end, j),
+                                                      s, 0);
+            else
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, (T)v[j]), r, place(t, end, j), s, 0);
+        }
+    }
+};
+
+// B and C of a window's steps, [kSteps ...][16] each; a thread's share on its way.
+template <int STEPS, class T>
+struct QuadShared {
+    static constexpr int N = STEPS * kQuadStates / 256;
+    T b[N], c[N];
+    uint8_t reset;
+    __device__ __forceinline__ void load(uint32_t group, uint32_t n, uint32_t t, uint32_t end) {
+        const ArgsAgain p = args_again();
+        const uint32_t states = p->states;
+        const uint64_t row0 = n * p->at.seq_rows, by = p->at.step_rows;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t e = threadIdx.x + i * 256, s = t + e / kQuadStates, k = e % kQuadStates;
+            b[i] = c[i] = (T)0.0f;
+            if (s >= end || k >= states) continue;
+            const uint64_t row = row0 + s * by;
+            b[i] = static_cast<const T*>(p->b)[row * p->b_ld + (size_t)group * states + k];
+            c[i] = static_cast<const T*>(p->c)[row * p->c_ld + (size_t)group * states + k];
+        }
+        const uint32_t lane = threadIdx.x & 63;
+        const uint8_t* const resets = p->at.reset;
+        reset = 0;
+        if (resets && lane < STEPS && t + lane < end) reset = resets[row0 + (t + lane) * by];
+    }
+    __device__ __forceinline__ void put(float* tb, float* tc) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) tb[threadIdx.x + i * 256] = (float)b[i], tc[threadIdx.x + i * 256] = (float)c[i];
+    }
+    __device__ __forceinline__ uint64_t resets() const { return __ballot(reset != 0); }
+};
+
+// The rates of a lane's elements; steps past the end have delta 0, which leaves a state as
+// it is, and so have lanes without a channel.
+template <int C, class T>
+__device__ __forceinline__ void quad_rates(const QuadLane<C>& at, uint32_t t, uint32_t end, float bias,
+                                           const T (&dt)[QuadLane<C>::R], const T (&x)[QuadLane<C>::R],
+                                           float (&delta)[QuadLane<C>::R], float (&u)[QuadLane<C>::R]) {
+#pragma unroll
+    for (int j = 0; j < QuadLane<C>::R; ++j) {
+        const bool live = at.in && t + QuadLane<C>::step(j) < end;
+        delta[j] = live ? softplus((float)dt[j] + bias) : 0.0f;
+        u[j] = live ? delta[j] * (float)x[j] : 0.0f;
+    }
+}
+
+// As scan_kernel.
+template <class T, int C, bool FULL, bool Z>
+__global__ void __launch_bounds__(256, 4) scan_quad_kernel(const ScanArgs p, uint64_t items) {
+    using Lane = QuadLane<C>;
+    constexpr int R = Lane::R;
+    __shared__ __align__(16) float sb[2][kWindow * kQuadStates], sc[2][kWindow * kQuadStates];
+    for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const ScanItem it(p, item);
+        const Lane at(p, it.block);
+        const uint32_t n = it.n, length = p.at.length(n), begin = it.split * p.split_steps;
+        uint32_t end = begin + p.split_steps;
+        end = end < length ? end : length;
+        f32x4 h[C] = {};
+        if constexpr (FULL) {
+            if (p.initial) at.load(p, p.splits > 1 ? p.saved : p.initial, n, h);
+            const size_t cells = (size_t)p.at.seqs * p.channels;
+#pragma unroll 2
+            for (uint32_t k = 0; k < it.split; ++k) {
+                f32x4 behind[C];
+                at.load(p, p.ends + k * cells * p.states, n, behind);
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const float sum = at.held[c] > 0 ? p.decays[k * cells + (size_t)n * p.channels + at.first + c] : 0.0f;
+                    const f32x4 decay = decay_of(at.a2[c], sum);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        h[c][i] = sum < 0.0f ? behind[c][i] : __builtin_fmaf(decay[i], h[c][i], behind[c][i]);
+                }
+            }
+        } else if (it.split == 0 && p.initial) {
+            f32x4 first[C];
+            at.load(p, p.initial, n, first);
+            at.store(p, p.saved, n, first);
+        }
+        const float bias = p.dt_bias ? p.dt_bias[at.own] : 0.0f, skip = FULL && p.d ? p.d[at.own] : 0.0f;
+        float sum[C] = {};
+        bool begun = false;
+        T x[R], dt[R], z[R];
+        auto fetch = [&](uint32_t t) {
+            const ArgsAgain q = args_again();
+            QuadRows<T, C>(q, at, q->x, q->x_ld, n).load(t, end, x);
+            QuadRows<T, C>(q, at, q->dt, q->dt_ld, n).load(t, end, dt);
+            if constexpr (FULL && Z) QuadRows<T, C>(q, at, q->z, q->z_ld, n).load(t, end, z);
+        };
+        QuadShared<kWindow, T> shared;
+        if (begin < end) {
+            shared.load(at.group, n, begin, end);
+            fetch(begin);
+        }
+        __syncthreads();  // the item before is done with LDS
+        if (begin < end) shared.put(sb[0], sc[0]);
+        __syncthreads();
+        int turn = 0;
+        for (uint32_t w = begin; w < end; w += kWindow, turn ^= 1) {
+            uint32_t resets = (uint32_t)shared.resets();
+            if (!FULL) begun |= resets != 0;
+            const bool more = w + kWindow < end;
+            if (more) shared.load(at.group, n, w + kWindow, end);
+            const uint32_t until = more ? w + kWindow : end;
+            const float* b_at = sb[turn] + at.state;
+            const float* c_at = sc[turn] + at.state;
+            for (uint32_t t = w; t < until; t += kSteps, resets >>= kSteps) {
+                float delta[R], u[R];
+                T was[R], gate[R];
+                quad_rates<C>(at, t, end, bias, dt, x, delta, u);
+#pragma unroll
+                for (int j = 0; j < R; ++j) was[j] = x[j], gate[j] = FULL && Z ? z[j] : (T)0.0f;
+                if (t + kSteps < end) fetch(t + kSteps);
+                if (FULL && p.checkpoints && t % kChunk == 0)
+                    at.store(p, p.checkpoints + (size_t)(t / kChunk) * p.at.seqs * p.channels * p.states, n, h);
+                float out[R];
+                {
+                    float part[4];
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k) {
+                        if (resets >> k & 1) clear_states(h);
+                        const f32x4 b = *reinterpret_cast<const f32x4*>(b_at + k * kQuadStates);
+                        f32x4 cc;
+                        if constexpr (FULL) cc = *reinterpret_cast<const f32x4*>(c_at + k * kQuadStates);
+#pragma unroll
+                        for (int c = 0; c < C; ++c) {
+                            const int from = Lane::lane(k, c), j = k / Lane::P;
+                            const float d = quad_take(from, delta[j]), uu = quad_take(from, u[j]);
+                            const f32x4 decay = decay_of(at.a2[c], d);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) h[c][i] = __builtin_fmaf(decay[i], h[c][i], uu * b[i]);
+                            if constexpr (FULL) {
+                                float y = h[c][0] * cc[0];
+#pragma unroll
+                                for (int i = 1; i < 4; ++i) y = __builtin_fmaf(h[c][i], cc[i], y);
+                                part[from] = y;
+                            } else {
+                                sum[c] += d;
+                            }
+                        }
+                        if constexpr (FULL)
+                            if (k % Lane::P == Lane::P - 1) out[k / Lane::P] = quad_sums(part);
+                    }
+                }
+                if constexpr (FULL) {
+#pragma unroll
+                    for (int j = 0; j < R; ++j) {
+                        float y = __builtin_fmaf(skip, (float)was[j], out[j]);
+                        if (Z) y *= silu((float)gate[j]);
+                        out[j] = y;
+                    }
+                    const ArgsAgain q = args_again();
+                    QuadRows<T, C>(q, at, q->y, q->y_ld, n).store(t, end, out);
+                }
+                b_at += kSteps * kQuadStates, c_at += kSteps * kQuadStates;
+            }
+            if (more) shared.put(sb[turn ^ 1], sc[turn ^ 1]);
+            __syncthreads();
+        }
+        if constexpr (FULL) {
+            if (p.final && it.split == p.splits - 1) at.store(p, p.final, n, h);
+        } else {
+            const size_t row = ((size_t)it.split * p.at.seqs + n) * p.channels;
+            at.store(p, p.ends + (size_t)it.split * p.at.seqs * p.channels * p.states, n, h);
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (at.held[c] > 0 && at.state == 0) p.decays[row + at.first + c] = begun ? -1.0f : sum[c];
+        }
+    }
+}
+
+// As scan_ends_backward_kernel.
+template <class T, int C>
+__global__ void __launch_bounds__(256) scan_quad_ends_backward_kernel(const ScanArgs p, uint64_t items) {
+    using Lane = QuadLane<C>;
+    constexpr int R = Lane::R;
+    __shared__ __align__(16) float sb[kChunk * kQuadStates], sc[kChunk * kQuadStates];
+    for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const ScanItem it(p, item);
+        const Lane at(p, it.block);
+        const uint32_t n = it.n, length = p.at.length(n), split = it.split + 1, begin = split * p.split_steps;
+        uint32_t end = begin + p.split_steps;
+        end = end < length ? end : length;
+        const float bias = p.dt_bias ? p.dt_bias[at.own] : 0.0f;
+        f32x4 g[C] = {};
+        float sum[C] = {};
+        bool begun = false;
+        for (uint32_t chunks = begin < end ? (end - begin + kChunk - 1) / kChunk : 0; chunks--;) {
+            const uint32_t from = begin + chunks * kChunk, to = end - from < (uint32_t)kChunk ? end : from + kChunk;
+            QuadShared<kChunk, T> shared;
+            shared.load(at.group, n, from, to);
+            __syncthreads();
+            shared.put(sb, sc);
+            __syncthreads();
+            const uint64_t resets = shared.resets();
+            begun |= resets != 0;
+            for (int r = (int)((to - from + kSteps - 1) / kSteps); r--;) {
+                const uint32_t t = from + r * kSteps;
+                T dt[R], z[R], dy[R];
+                float delta[R], none[R], into[R];
+                const ArgsAgain q = args_again();
+                QuadRows<T, C>(q, at, q->dt, q->dt_ld, n).load(t, to, dt);
+                QuadRows<T, C>(q, at, q->dy, q->dy_ld, n).load(t, to, dy);
+                if (q->z) QuadRows<T, C>(q, at, q->z, q->z_ld, n).load(t, to, z);
+                quad_rates<C>(at, t, to, bias, dt, dt, delta, none);
+#pragma unroll
+                for (int j = 0; j < R; ++j) into[j] = p.z ? (float)dy[j] * silu((float)z[j]) : (float)dy[j];
+                const uint32_t bits = (uint32_t)(resets >> (r * kSteps)) & ((1u << kSteps) - 1);
+#pragma unroll
+                for (int k = kSteps - 1; k >= 0; --k) {
+                    const f32x4 cc = *reinterpret_cast<const f32x4*>(sc + (r * kSteps + k) * kQuadStates + at.state);
+#pragma unroll
+                    for (int c = 0; c < C; ++c) {
+                        const int lane = Lane::lane(k, c), j = k / Lane::P;
+                        const float d = quad_take(lane, delta[j]), dyk = quad_take(lane, into[j]);
+                        const f32x4 decay = decay_of(at.a2[c], d);
+                        sum[c] += d;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) g[c][i] = __builtin_fmaf(cc[i], dyk, g[c][i]) * decay[i];
+                    }
+                    if (bits >> k & 1) {
+#pragma unroll
+                        for (int c = 0; c < C; ++c) g[c] = f32x4{};
+                    }
+                }
+            }
+        }
+        const size_t row = ((size_t)split * p.at.seqs + n) * p.channels;
+        at.store(p, p.ends + (size_t)split * p.at.seqs * p.channels * p.states, n, g);
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            if (at.held[c] > 0 && at.state == 0) p.decays[row + at.first + c] = begun ? -1.0f : sum[c];
+    }
+}
+
+// As scan_backward_kernel, 32 steps at a time: their states every kSteps steps wait in LDS,
+// each lane's own. The second half of a chunk walks over the first to its own first state.
+// The decays are worked out twice: to keep them beside the states would take the registers of
+// a wave a SIMD.
+template <class T, int C, bool Z>
+__global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanArgs p, uint32_t parts) {
+    using Lane = QuadLane<C>;
+    constexpr int R = Lane::R, kRounds = kWindow / kSteps;
+    __shared__ __align__(16) float sb[kWindow * kQuadStates], sc[kWindow * kQuadStates];
+    __shared__ f32x4 starts[kRounds - 1][C][256];
+    __shared__ float rates[kRounds - 1][R][256];           // delta of the rounds that are walked over
+    __shared__ float sums[2][kSteps][4][2 * kQuadStates];  // each wave's for dB and dC
+    const uint32_t block = blockIdx.x % p.blocks, part = blockIdx.x / p.blocks;
+    const int wave = threadIdx.x >> 6;
+    const Lane at(p, block);
+    const float skip = p.d ? p.d[at.own] : 0.0f, bias = p.dt_bias ? p.dt_bias[at.own] : 0.0f;
+    f32x4 da[C] = {};
+    float dd = 0.0f, dbias = 0.0f;
+    int turn = 0;
+    const uint64_t items = (uint64_t)p.at.seqs * p.splits;
+    for (uint64_t item = part; item < items; item += parts) {
+        const uint32_t split = (uint32_t)(item / p.at.seqs), n = (uint32_t)(item - (uint64_t)split * p.at.seqs);
+        const uint32_t length = p.at.length(n), begin = split * p.split_steps;
+        uint32_t end = begin + p.split_steps;
+        end = end < length ? end : length;
+        f32x4 g[C] = {};
+        if (p.dfinal) at.load(p, p.dfinal, n, g);
+        const size_t cells = (size_t)p.at.seqs * p.channels;
+#pragma unroll 4
+        for (uint32_t k = p.splits - 1; k > split; --k) {
+            f32x4 behind[C];
+            at.load(p, p.ends + k * cells * p.states, n, behind);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const float sum = at.held[c] > 0 ? p.decays[k * cells + (size_t)n * p.channels + at.first + c] : 0.0f;
+                const f32x4 decay = decay_of(at.a2[c], sum);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    g[c][i] = sum < 0.0f ? behind[c][i] : __builtin_fmaf(decay[i], g[c][i], behind[c][i]);
+            }
+        }
+        for (uint32_t window = begin < end ? (end - begin + kWindow - 1) / kWindow : 0; window--;) {
+            const uint32_t from = begin + window * kWindow, to = end - from < (uint32_t)kWindow ? end : from + kWindow;
+            const uint32_t chunk = from / kChunk * kChunk;
+            const int rounds = (int)((to - from + kSteps - 1) / kSteps);
+            f32x4 h[C] = {};
+            if (chunk && p.kept)
+                at.load(p, p.kept + chunk / kChunk * cells * p.states, n, h);
+            else if (!chunk && p.initial)
+                at.load(p, p.initial, n, h);
+            T x[R], dt[R], dy[R], z[R];
+            auto fetch = [&](uint32_t t, uint32_t last, bool all) {
+                const ArgsAgain q = args_again();
+                QuadRows<T, C>(q, at, q->x, q->x_ld, n).load(t, last, x);
+                QuadRows<T, C>(q, at, q->dt, q->dt_ld, n).load(t, last, dt);
+                if (!all) return;
+                QuadRows<T, C>(q, at, q->dy, q->dy_ld, n).load(t, last, dy);
+                if constexpr (Z) QuadRows<T, C>(q, at, q->z, q->z_ld, n).load(t, last, z);
+            };
+            uint32_t resets = 0;
+            for (uint32_t w = chunk; w <= from; w += kWindow) {
+                const uint32_t last = w == from ? to : w + kWindow;
+                const int walk = w == from ? rounds - 1 : kRounds;
+                QuadShared<kWindow, T> shared;
+                shared.load(at.group, n, w, last);
+                fetch(w, last, walk == 0);
+                __syncthreads();  // every wave is done with B and C
+                shared.put(sb, sc);
+                __syncthreads();
+                resets = (uint32_t)shared.resets();
+                for (int r = 0; r < walk; ++r) {
+                    const uint32_t t = w + r * kSteps;
+                    float delta[R], u[R];
+                    quad_rates<C>(at, t, last, bias, dt, x, delta, u);
+                    if (t + kSteps < last) fetch(t + kSteps, last, w == from && r + 1 == walk);
+                    if (w == from) {
+#pragma unroll
+                        for (int c = 0; c < C; ++c) starts[r][c][threadIdx.x] = h[c];
+#pragma unroll
+                        for (int j = 0; j < R; ++j) rates[r][j][threadIdx.x] = delta[j];
+                    }
+                    const uint32_t bits = resets >> (r * kSteps);
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k) {
+                        if (bits >> k & 1) clear_states(h);
+                        const f32x4 b = *reinterpret_cast<const f32x4*>(sb + (r * kSteps + k) * kQuadStates + at.state);
+#pragma unroll
+                        for (int c = 0; c < C; ++c) {
+                            const int lane = Lane::lane(k, c), j = k / Lane::P;
+                            const f32x4 decay = decay_of(at.a2[c], quad_take(lane, delta[j]));
+                            const float uu = quad_take(lane, u[j]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) h[c][i] = __builtin_fmaf(decay[i], h[c][i], uu * b[i]);
+                        }
+                    }
+                }
+            }
+            for (int r = rounds; r--; turn ^= 1) {
+                const uint32_t t = from + r * kSteps;
+                float delta[R], u[R], into[R];  // dy before the gate
+                if (r + 1 < rounds) {
+#pragma unroll
+                    for (int j = 0; j < R; ++j) delta[j] = rates[r][j][threadIdx.x], u[j] = delta[j] * (float)x[j];
+                } else {
+                    quad_rates<C>(at, t, to, bias, dt, x, delta, u);
+                }
+#pragma unroll
+                for (int j = 0; j < R; ++j) {
+                    into[j] = Z ? (float)dy[j] * silu((float)z[j]) : (float)dy[j];
+                    // a lane without a channel, or past the end, adds nothing
+                    into[j] = at.in && t + Lane::step(j) < to ? into[j] : 0.0f;
+                }
+                if (r + 1 < rounds) {
+#pragma unroll
+                    for (int c = 0; c < C; ++c) h[c] = starts[r][c][threadIdx.x];
+                }
+                const uint32_t bits = resets >> (r * kSteps);
+                float gb[R], ga[R], y[R];
+                f32x4 first[C], states[kSteps][C];
+#pragma unroll
+                for (int c = 0; c < C; ++c) first[c] = h[c];
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    if (bits >> k & 1) clear_states(h);
+                    const f32x4 b = *reinterpret_cast<const f32x4*>(sb + (r * kSteps + k) * kQuadStates + at.state);
+#pragma unroll
+                    for (int c = 0; c < C; ++c) {
+                        const int lane = Lane::lane(k, c), j = k / Lane::P;
+                        const f32x4 decay = decay_of(at.a2[c], quad_take(lane, delta[j]));
+                        const float uu = quad_take(lane, u[j]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) h[c][i] = __builtin_fmaf(decay[i], h[c][i], uu * b[i]);
+                        states[k][c] = h[c];
+                    }
+                }
+                // or the compiler keeps what it knows of the decays, B and the moved values
+#pragma unroll
+                for (int j = 0; j < R; ++j) asm volatile("" : "+v"(delta[j]), "+v"(u[j])::"memory");
+                float part_b[4], part_a[4], part_y[4];
+#pragma unroll
+                for (int k = kSteps - 1; k >= 0; --k) {
+                    const f32x4 b = *reinterpret_cast<const f32x4*>(sb + (r * kSteps + k) * kQuadStates + at.state);
+                    const f32x4 cc = *reinterpret_cast<const f32x4*>(sc + (r * kSteps + k) * kQuadStates + at.state);
+                    float v[8] = {};
+#pragma unroll
+                    for (int c = 0; c < C; ++c) {
+                        const int lane = Lane::lane(k, c), j = k / Lane::P;
+                        const float dyk = quad_take(lane, into[j]), uu = quad_take(lane, u[j]);
+                        float sum_b = 0.0f, sum_y = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            g[c][i] = __builtin_fmaf(cc[i], dyk, g[c][i]);
+                            v[i] = __builtin_fmaf(g[c][i], uu, v[i]);
+                            v[4 + i] = __builtin_fmaf(states[k][c][i], dyk, v[4 + i]);
+                            if (Z) sum_y = __builtin_fmaf(cc[i], states[k][c][i], sum_y);
+                            sum_b = __builtin_fmaf(g[c][i], b[i], sum_b);
+                        }
+                        part_b[lane] = sum_b, part_y[lane] = sum_y;
+                    }
+                    // where an episode begins nothing goes further back
+                    if (bits >> k & 1) {
+                        clear_states(g);
+#pragma unroll
+                        for (int c = 0; c < C; ++c) part_a[Lane::lane(k, c)] = 0.0f;
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < C; ++c) {
+                            const int lane = Lane::lane(k, c), j = k / Lane::P;
+                            const float d = quad_take(lane, delta[j]);
+                            const f32x4 decay = decay_of(at.a2[c], d);
+                            const f32x4 before = k ? states[k ? k - 1 : 0][c] : first[c];
+                            float sum_a = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                g[c][i] *= decay[i];
+                                const float via = g[c][i] * before[i];
+                                sum_a = __builtin_fmaf(via, at.a2[c][i], sum_a);
+                                da[c][i] = __builtin_fmaf(via, d, da[c][i]);
+                            }
+                            part_a[lane] = sum_a;
+                        }
+                    }
+                    sum_channels<4>(v, sums[turn][k][wave]);
+                    if (k % Lane::P == 0) {
+                        const int j = k / Lane::P;
+                        gb[j] = quad_sums(part_b), ga[j] = quad_sums(part_a);
+                        if (Z) y[j] = quad_sums(part_y);
+                    }
+                }
+                T x0[R], dt0[R], dy0[R], z0[R];
+#pragma unroll
+                for (int j = 0; j < R; ++j) x0[j] = x[j], dt0[j] = dt[j], dy0[j] = dy[j], z0[j] = Z ? z[j] : (T)0.0f;
+                if (r) fetch(t - kSteps, to, true);
+#pragma unroll
+                for (int j = 0; j < R; ++j) {
+                    if (Z) y[j] = (float)dy0[j] * __builtin_fmaf(skip, (float)x0[j], y[j]) * silu_slope((float)z0[j]);
+                    float slope, rest;
+                    sigmoid_of((float)dt0[j] + bias, slope, rest);
+                    ga[j] = __builtin_fmaf((float)x0[j], gb[j], ga[j] * 0.693147181f) * slope;
+                    gb[j] = __builtin_fmaf(into[j], skip, delta[j] * gb[j]);
+                    if (at.in && t + Lane::step(j) < to) {
+                        dd = __builtin_fmaf(into[j], (float)x0[j], dd);
+                        dbias += ga[j];
+                    }
+                }
+                {
+                    const ArgsAgain q = args_again();
+                    QuadRows<T, C>(q, at, q->dx, q->dx_ld, n).store(t, to, gb);
+                    QuadRows<T, C>(q, at, q->ddt, q->ddt_ld, n).store(t, to, ga);
+                    if (Z && q->dz) QuadRows<T, C>(q, at, q->dz, q->dz_ld, n).store(t, to, y);
+                }
+                __syncthreads();
+                const int k = threadIdx.x >> 5, w = threadIdx.x & 31, i = w & 15;
+                if (t + k < to && i < (int)p.states) {
+                    const float sum = (sums[turn][k][0][w] + sums[turn][k][1][w]) +
+                                      (sums[turn][k][2][w] + sums[turn][k][3][w]);
+                    const uint32_t which = w >> 4;
+                    const ArgsAgain q = args_again();
+                    if (q->apiece == 1) {
+                        const uint64_t row = (t + k) * q->at.step_rows + n * q->at.seq_rows;
+                        const uint64_t place = row * (which ? q->dc_ld : q->db_ld) + (size_t)at.group * q->states + i;
+                        static_cast<T*>(which ? q->dc : q->db)[place] = (T)sum;
+                    } else {
+                        const size_t row = ((size_t)(block % q->apiece) * q->at.steps + t + k) * q->at.seqs + n;
+                        q->shared[((row * q->groups + at.group) * 2 + which) * q->states + i] = sum;
+                    }
+                }
+            }
+        }
+        if (p.dinitial && split == 0) at.store(p, p.dinitial, n, g);
+    }
+    if (!p.sums) return;
+    float* const out = p.sums + (size_t)part * p.channels * (p.states + 2);
+    at.store(p, out, 0, da);
+    // a channel's lanes of the quad
+    if constexpr (C == 1) dd += dpp_lane<0xB1>(dd), dbias += dpp_lane<0xB1>(dbias);
+    dd += dpp_lane<0x4E>(dd), dbias += dpp_lane<0x4E>(dbias);
+    if (at.in && (threadIdx.x & 3) < C) {
+        out[(size_t)p.channels * p.states + at.own] = dd;
+        out[(size_t)p.channels * (p.states + 1) + at.own] = dbias;
+    }
+}
+
+// One step of every sequence, four sequences at a time: no LDS, every load at once, the
+// states to memory and back. A quad's lanes each work for one of the four.
+template <class T, bool Z>
+__global__ void __launch_bounds__(256) scan_quad_step_kernel(const ScanArgs p, uint64_t items) {
+    using Lane = QuadLane<1>;
+    typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const uint32_t n0 = (uint32_t)(item / p.blocks) * 4;
+        const Lane at(p, (uint32_t)(item % p.blocks));
+        const uint32_t last = p.at.seqs - 1;
+        const float skip = p.d ? p.d[at.own] : 0.0f, bias = p.dt_bias ? p.dt_bias[at.own] : 0.0f;
+        f32x4 h[4], b[4], c[4];
+        bool fresh[4], live[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t n = n0 + q < last ? n0 + q : last;
+            const uint64_t row = p.at.row(0, n);
+            h[q] = p.initial ? load_states(p.initial + at.at(p, n, 0), at.held[0]) : f32x4{};
+            live[q] = p.at.length(n) != 0;
+            fresh[q] = live[q] && p.at.reset && p.at.reset[row];
+            b[q] = c[q] = f32x4{};
+            if (!live[q]) continue;
+            const T* const bs = static_cast<const T*>(p.b) + row * p.b_ld + (size_t)at.group * p.states + at.state;
+            const T* const cs = static_cast<const T*>(p.c) + row * p.c_ld + (size_t)at.group * p.states + at.state;
+            if (p.states == kQuadStates) {
+                const four vb = *reinterpret_cast<const four*>(bs), vc = *reinterpret_cast<const four*>(cs);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) b[q][i] = (float)vb[i], c[q][i] = (float)vc[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (at.state + i < (int)p.states) b[q][i] = (float)bs[i], c[q][i] = (float)cs[i];
+            }
+        }
+        const uint32_t mine = n0 + (threadIdx.x & 3), n = mine < last ? mine : last;
+        const bool works = mine <= last && p.at.length(n) != 0;
+        float x = 0.0f, dt = 0.0f, z = 0.0f;
+        const uint64_t row = p.at.row(0, n);
+        if (works) {
+            x = (float)static_cast<const T*>(p.x)[row * p.x_ld + at.own];
+            dt = (float)static_cast<const T*>(p.dt)[row * p.dt_ld + at.own];
+            if (Z) z = (float)static_cast<const T*>(p.z)[row * p.z_ld + at.own];
+        }
+        const float delta = works ? softplus(dt + bias) : 0.0f, u = works ? delta * x : 0.0f;
+        float part[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (fresh[q]) h[q] = f32x4{};
+            const f32x4 decay = decay_of(at.a2[0], quad_take(q, delta));
+            const float uu = quad_take(q, u);
+            part[q] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float moved = __builtin_fmaf(decay[i], h[q][i], uu * b[q][i]);
+                h[q][i] = live[q] ? moved : h[q][i];
+                part[q] = __builtin_fmaf(h[q][i], c[q][i], part[q]);
+            }
+            if (p.final && n0 + q <= last) store_states(p.final + at.at(p, n0 + q, 0), at.held[0], h[q]);
+        }
+        float y = quad_sums(part);
+        if (works && at.in) {
+            y = __builtin_fmaf(skip, x, y);
+            if (Z) y *= silu(z);
+            static_cast<T*>(p.y)[row * p.y_ld + at.own] = (T)y;
+        }
+    }
+}
+
+}  // namespace dev
+}  // namespace mg

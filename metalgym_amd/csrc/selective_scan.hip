@@ -18,75 +18,11 @@
 // LDS, and takes the 8 steps back to front with their states and decays in registers.
 #include <type_traits>
 
-#include "mg/device/common.h"
-#include "sequence.h"
+#include "scan_common.h"
+#include "scan_quad.h"
 
 namespace mg {
 namespace dev {
-
-constexpr int kSteps = 8;   // of a round between barriers
-constexpr int kChunk = 64;  // steps between the kept states
-constexpr int kSubs = kChunk / kSteps;
-constexpr float kLog2e = 1.44269504f;
-
-struct ScanArgs {
-    Rollout at;
-    const void* x;
-    const void* dt;
-    const void* b;
-    const void* c;
-    const void* z;
-    void* y;
-    const float* a;
-    const float* d;
-    const float* dt_bias;
-    const float* initial;
-    float* final;
-    float* checkpoints;
-    // the backward pass's
-    const void* dy;
-    const float* kept;
-    const float* dfinal;
-    void* dx;
-    void* ddt;
-    void* db;
-    void* dc;
-    void* dz;
-    float* dinitial;
-    float* sums;     // [parts][channels (states + 2)]: dA, dD, ddt_bias
-    float* shared;   // [blocks of a group][steps seqs][groups][2][states]: parts of dB and dC
-    // of each split but the last (the first, backwards), from a state of zero
-    float* ends;     // [splits][seqs][channels][states]
-    float* decays;   // [splits][seqs][channels]: the sum of delta, or -1 where an episode begins
-    float* saved;    // the initial state, as the final one may take its place
-    uint64_t x_ld, dt_ld, b_ld, c_ld, z_ld, y_ld, dy_ld, dx_ld, ddt_ld, db_ld, dc_ld, dz_ld;
-    uint32_t channels, states, groups;
-    uint32_t per;     // channels of a group
-    uint32_t apiece;  // blocks of a group
-    uint32_t blocks;  // of all channels
-    uint32_t splits, split_steps;
-};
-
-// Four consecutive states of a channel; past `count` 0, or not written.
-__device__ __forceinline__ f32x4 load_states(const float* p, int count) {
-    typedef float near __attribute__((ext_vector_type(4), aligned(4)));
-    if (count >= 4) return *reinterpret_cast<const near*>(p);
-    f32x4 v = {};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (i < count) v[i] = p[i];
-    return v;
-}
-__device__ __forceinline__ void store_states(float* p, int count, f32x4 v) {
-    typedef float near __attribute__((ext_vector_type(4), aligned(4)));
-    if (count >= 4) {
-        *reinterpret_cast<near*>(p) = v;
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (i < count) p[i] = v[i];
-}
 
 // A workgroup's channels of one group, and a lane's four states among them.
 template <int L>
@@ -112,13 +48,6 @@ struct ScanLane {
     }
 };
 
-__device__ __forceinline__ f32x4 decay_of(f32x4 a2, float delta) {
-    f32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_exp2f(a2[i] * delta);
-    return r;
-}
-
 // What a round of steps needs, in LDS.
 template <int L>
 struct ScanRound {
@@ -129,14 +58,15 @@ struct ScanRound {
     uint32_t resets;  // a bit a step
 };
 
-// A thread's elements of a round: the same channel of every few steps.
-template <int L>
+// A thread's elements of a round: the same channel of every few steps. They stay as they
+// lie until they are used: a conversion waits for its load.
+template <class T, int L>
 struct ScanFetch {
     using Lane = ScanLane<L>;
     static constexpr int N = (kSteps * Lane::CH + 255) / 256;
     static constexpr int NB = (kSteps * Lane::SP + 255) / 256;
-    float x[N], dt[N], z[N], dy[N], b[NB], c[NB];
-    uint32_t reset;
+    T x[N], dt[N], z[N], dy[N], b[NB], c[NB];
+    uint8_t reset;
 
     static __device__ __forceinline__ int step(int i) { return (threadIdx.x + i * 256) / Lane::CH; }
     static __device__ __forceinline__ int slot(int i) { return threadIdx.x + i * 256; }
@@ -148,29 +78,30 @@ struct ScanFetch {
         return slot(i) < kSteps * Lane::CH && t + step(i) < end && channel(at) < at.limit;
     }
 
-    template <class T, bool DY>
+    template <bool DY>
     __device__ __forceinline__ void load(const ScanArgs& p, const Lane& at, uint32_t n, uint32_t t, uint32_t end) {
         const uint32_t ch = channel(at);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            x[i] = dt[i] = z[i] = dy[i] = 0.0f;
+            x[i] = dt[i] = z[i] = dy[i] = (T)0.0f;
             if (!in(at, i, t, end)) continue;
             const uint64_t row = p.at.row(t + step(i), n);
-            x[i] = (float)static_cast<const T*>(p.x)[row * p.x_ld + ch];
-            dt[i] = (float)static_cast<const T*>(p.dt)[row * p.dt_ld + ch];
-            if (p.z) z[i] = (float)static_cast<const T*>(p.z)[row * p.z_ld + ch];
-            if (DY) dy[i] = (float)static_cast<const T*>(p.dy)[row * p.dy_ld + ch];
+            x[i] = static_cast<const T*>(p.x)[row * p.x_ld + ch];
+            dt[i] = static_cast<const T*>(p.dt)[row * p.dt_ld + ch];
+            if (p.z) z[i] = static_cast<const T*>(p.z)[row * p.z_ld + ch];
+            if (DY) dy[i] = static_cast<const T*>(p.dy)[row * p.dy_ld + ch];
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             const int e = threadIdx.x + i * 256, k = e / Lane::SP, s = e % Lane::SP;
-            b[i] = c[i] = 0.0f;
+            b[i] = c[i] = (T)0.0f;
             if (e >= kSteps * Lane::SP || t + k >= end || s >= (int)p.states) continue;
             const uint64_t row = p.at.row(t + k, n);
-            b[i] = (float)static_cast<const T*>(p.b)[row * p.b_ld + (size_t)at.group * p.states + s];
-            c[i] = (float)static_cast<const T*>(p.c)[row * p.c_ld + (size_t)at.group * p.states + s];
+            b[i] = static_cast<const T*>(p.b)[row * p.b_ld + (size_t)at.group * p.states + s];
+            c[i] = static_cast<const T*>(p.c)[row * p.c_ld + (size_t)at.group * p.states + s];
         }
-        reset = p.at.reset && threadIdx.x < kSteps && t + threadIdx.x < end && p.at.reset[p.at.row(t + threadIdx.x, n)];
+        reset = 0;
+        if (p.at.reset && threadIdx.x < kSteps && t + threadIdx.x < end) reset = p.at.reset[p.at.row(t + threadIdx.x, n)];
     }
     // Steps past the end have delta 0: they leave the state as it is.
     __device__ __forceinline__ void put(const ScanArgs& p, const Lane& at, uint32_t t, uint32_t end,
@@ -180,15 +111,15 @@ struct ScanFetch {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (slot(i) >= kSteps * Lane::CH) continue;
-            const float delta = in(at, i, t, end) ? softplus(dt[i] + bias) : 0.0f;
+            const float delta = in(at, i, t, end) ? softplus((float)dt[i] + bias) : 0.0f;
             to.delta[slot(i)] = delta;
-            to.u[slot(i)] = delta * x[i];
+            to.u[slot(i)] = delta * (float)x[i];
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             const int e = threadIdx.x + i * 256;
             if (e >= kSteps * Lane::SP) continue;
-            to.b[e] = b[i], to.c[e] = c[i];
+            to.b[e] = (float)b[i], to.c[e] = (float)c[i];
         }
         if (threadIdx.x < 64) {
             const uint32_t bits = (uint32_t)__ballot(reset != 0);
@@ -205,7 +136,7 @@ __device__ __forceinline__ f32x4 join_before(const ScanArgs& p, const ScanLane<L
     if (p.initial && at.count > 0) h = load_states(first + at.at(p, n), at.count);
     if (at.count <= 0) return h;
     const size_t step = (size_t)p.at.seqs * p.channels;
-#pragma unroll 4
+#pragma unroll 8
     for (uint32_t k = 0; k < split; ++k) {
         const f32x4 end = load_states(p.ends + k * step * p.states + at.at(p, n), at.count);
         const float sum = p.decays[k * step + (size_t)n * p.channels + at.channel];
@@ -216,23 +147,12 @@ __device__ __forceinline__ f32x4 join_before(const ScanArgs& p, const ScanLane<L
     return h;
 }
 
-// The items of a launch: (split, sequence, block of channels), the last fastest.
-struct ScanItem {
-    uint32_t block, n, split;
-    __device__ __forceinline__ ScanItem(const ScanArgs& p, uint64_t item) {
-        const uint64_t rest = item / p.blocks;
-        block = (uint32_t)(item - rest * p.blocks);
-        split = (uint32_t)(rest / p.at.seqs);
-        n = (uint32_t)(rest - (uint64_t)split * p.at.seqs);
-    }
-};
-
 // FULL: y, the final state and the kept ones. Else each split but the last from a state of
 // zero to its end.
 template <class T, int L, bool FULL>
 __global__ void __launch_bounds__(256) scan_kernel(const ScanArgs p, uint64_t items) {
     using Lane = ScanLane<L>;
-    using Fetch = ScanFetch<L>;
+    using Fetch = ScanFetch<T, L>;
     __shared__ ScanRound<L> rounds[2];
     __shared__ float out[2][kSteps * Lane::CH];
     const int mine = threadIdx.x / L, sub = threadIdx.x % L;
@@ -252,7 +172,7 @@ __global__ void __launch_bounds__(256) scan_kernel(const ScanArgs p, uint64_t it
         const uint32_t ch = Fetch::channel(at);
         const float skip = FULL && p.d && ch < at.limit ? p.d[ch] : 0.0f;
         Fetch now;
-        now.template load<T, false>(p, at, n, begin, end);
+        now.template load<false>(p, at, n, begin, end);
         __syncthreads();  // the item before is done with LDS
         now.put(p, at, begin, end, rounds[0]);
         __syncthreads();
@@ -260,7 +180,7 @@ __global__ void __launch_bounds__(256) scan_kernel(const ScanArgs p, uint64_t it
         for (uint32_t t = begin; t < end; t += kSteps, turn ^= 1) {
             Fetch next;
             const bool more = t + kSteps < end;
-            if (more) next.template load<T, false>(p, at, n, t + kSteps, end);
+            if (more) next.template load<false>(p, at, n, t + kSteps, end);
             if (FULL && p.checkpoints && t % kChunk == 0 && at.count > 0)
                 store_states(p.checkpoints + (size_t)(t / kChunk) * p.at.seqs * p.channels * p.states + at.at(p, n),
                              at.count, h);
@@ -269,7 +189,7 @@ __global__ void __launch_bounds__(256) scan_kernel(const ScanArgs p, uint64_t it
             if (!FULL) begun |= resets != 0;
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
-                if (resets >> k & 1) h = f32x4{};
+                if (resets >> k & 1) clear_states(h);
                 const float delta = r.delta[k * Lane::CH + mine], u = r.u[k * Lane::CH + mine];
                 const f32x4 b = *reinterpret_cast<const f32x4*>(&r.b[k * Lane::SP + 4 * sub]);
                 const f32x4 decay = decay_of(at.a2, delta);
@@ -292,8 +212,8 @@ __global__ void __launch_bounds__(256) scan_kernel(const ScanArgs p, uint64_t it
 #pragma unroll
                 for (int i = 0; i < Fetch::N; ++i) {
                     if (!Fetch::in(at, i, t, end)) continue;
-                    float y = __builtin_fmaf(skip, now.x[i], out[turn][Fetch::slot(i)]);
-                    if (p.z) y *= silu(now.z[i]);
+                    float y = __builtin_fmaf(skip, (float)now.x[i], out[turn][Fetch::slot(i)]);
+                    if (p.z) y *= silu((float)now.z[i]);
                     static_cast<T*>(p.y)[p.at.row(t + Fetch::step(i), n) * p.y_ld + ch] = (T)y;
                 }
             }
@@ -337,8 +257,8 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const ScanArgs p, uint64
             for (int i = 0; i < 4; ++i)
                 if (i < at.count) {
                     const size_t s = (size_t)at.group * p.states + at.state + i;
-                    b[i] = (float)static_cast<const T*>(p.b)[row * p.b_ld + s];
-                    c[i] = (float)static_cast<const T*>(p.c)[row * p.c_ld + s];
+                    b[i] = static_cast<const T*>(p.b)[row * p.b_ld + s];
+                    c[i] = static_cast<const T*>(p.c)[row * p.c_ld + s];
                 }
             if (p.at.reset && p.at.reset[row]) h = f32x4{};
             const float delta = softplus(dt), u = delta * x;
@@ -363,7 +283,7 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const ScanArgs p, uint64
 template <class T, int L>
 __global__ void __launch_bounds__(256) scan_ends_backward_kernel(const ScanArgs p, uint64_t items) {
     using Lane = ScanLane<L>;
-    using Fetch = ScanFetch<L>;
+    using Fetch = ScanFetch<T, L>;
     __shared__ ScanRound<L> r;
     const int mine = threadIdx.x / L, sub = threadIdx.x % L;
     for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
@@ -378,12 +298,12 @@ __global__ void __launch_bounds__(256) scan_ends_backward_kernel(const ScanArgs 
         for (uint32_t left = begin < end ? (end - begin + kSteps - 1) / kSteps : 0; left--;) {
             const uint32_t t = begin + left * kSteps;
             Fetch f;
-            f.template load<T, true>(p, at, n, t, end);
+            f.template load<true>(p, at, n, t, end);
             __syncthreads();
             f.put(p, at, t, end, r);
 #pragma unroll
             for (int i = 0; i < Fetch::N; ++i)  // u's place takes the gradient before the gate
-                if (Fetch::slot(i) < kSteps * Lane::CH) r.u[Fetch::slot(i)] = p.z ? f.dy[i] * silu(f.z[i]) : f.dy[i];
+                if (Fetch::slot(i) < kSteps * Lane::CH) r.u[Fetch::slot(i)] = p.z ? (float)f.dy[i] * silu((float)f.z[i]) : (float)f.dy[i];
             __syncthreads();
             const uint32_t resets = __builtin_amdgcn_readfirstlane(r.resets);
             begun |= resets != 0;
@@ -395,59 +315,13 @@ __global__ void __launch_bounds__(256) scan_ends_backward_kernel(const ScanArgs 
                 sum += delta;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) g[i] = __builtin_fmaf(c[i], dy, g[i]) * decay[i];
-                if (resets >> k & 1) g = f32x4{};
+                if (resets >> k & 1) clear_states(g);
             }
         }
         if (at.count <= 0) continue;
         const size_t row = ((size_t)(it.split + 1) * p.at.seqs + n) * p.channels + at.channel;
         store_states(p.ends + row * p.states + at.state, at.count, g);
         if (sub == 0) p.decays[row] = begun ? -1.0f : sum;
-    }
-}
-
-// Register i of a and b, of which lanes l and l ^ X hold one part each: the lower lanes'
-// sum of a, the upper lanes' of b.
-template <int X>
-__device__ __forceinline__ float swap_add(float a, float b) {
-    if constexpr (X == 16)
-        asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-    else
-        asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-    return a + b;
-}
-
-// Sums of eight values (four states of dB, then of dC) over a wave's channels: each pair
-// of values shares a register from the swaps on. Writes them to LDS, [2][SP].
-template <int L>
-__device__ __forceinline__ void sum_channels(const float (&v)[8], float* to) {
-    constexpr int SP = 4 * L;
-    const int lane = threadIdx.x & 63, s = 4 * (lane % L);
-    if constexpr (L == 64) {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) to[(q >> 2) * SP + s + (q & 3)] = v[q];
-        return;
-    }
-    float w[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) w[q] = swap_add<32>(v[2 * q], v[2 * q + 1]);
-    const int upper = lane >> 5;
-    if constexpr (L == 32) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) to[(q >> 1) * SP + s + 2 * (q & 1) + upper] = w[q];
-        return;
-    }
-    float r[2];
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        r[q] = swap_add<16>(w[2 * q], w[2 * q + 1]);
-        if constexpr (L <= 8) r[q] += dpp_lane<0x128>(r[q]);  // row_ror 8, 4, 2, 1
-        if constexpr (L <= 4) r[q] += dpp_lane<0x124>(r[q]);
-        if constexpr (L <= 2) r[q] += dpp_lane<0x122>(r[q]);
-        if constexpr (L <= 1) r[q] += dpp_lane<0x121>(r[q]);
-    }
-    if ((lane & 15) < L) {
-        const int i = s + 2 * (lane >> 4 & 1) + upper;
-        to[i] = r[0], to[SP + i] = r[1];
     }
 }
 
@@ -467,7 +341,7 @@ struct BackwardShared {
 template <class T, int L>
 __global__ void __launch_bounds__(256) scan_backward_kernel(const ScanArgs p, uint32_t parts) {
     using Lane = ScanLane<L>;
-    using Fetch = ScanFetch<L>;
+    using Fetch = ScanFetch<T, L>;
     __shared__ BackwardShared<L> s;
     const int mine = threadIdx.x / L, sub = threadIdx.x % L, wave = threadIdx.x >> 6;
     const uint32_t block = blockIdx.x % p.blocks, part = blockIdx.x / p.blocks;
@@ -487,6 +361,7 @@ __global__ void __launch_bounds__(256) scan_backward_kernel(const ScanArgs p, ui
         if (at.count > 0) {
             if (p.dfinal) g = load_states(p.dfinal + at.at(p, n), at.count);
             const size_t step = (size_t)p.at.seqs * p.channels;
+#pragma unroll 8
             for (uint32_t k = p.splits - 1; k > split; --k) {
                 const f32x4 behind = load_states(p.ends + k * step * p.states + at.at(p, n), at.count);
                 const float sum = p.decays[k * step + (size_t)n * p.channels + at.channel];
@@ -512,14 +387,14 @@ __global__ void __launch_bounds__(256) scan_backward_kernel(const ScanArgs p, ui
             for (int j = 0; j + 1 < subs; ++j) {
                 s.starts[j][threadIdx.x] = h;
                 Fetch f;
-                f.template load<T, false>(p, at, n, from + j * kSteps, to);
+                f.template load<false>(p, at, n, from + j * kSteps, to);
                 __syncthreads();
                 f.put(p, at, from + j * kSteps, to, s.r);
                 __syncthreads();
                 const uint32_t resets = __builtin_amdgcn_readfirstlane(s.r.resets);
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
-                    if (resets >> k & 1) h = f32x4{};
+                    if (resets >> k & 1) clear_states(h);
                     const float delta = s.r.delta[k * Lane::CH + mine], u = s.r.u[k * Lane::CH + mine];
                     const f32x4 b = *reinterpret_cast<const f32x4*>(&s.r.b[k * Lane::SP + 4 * sub]);
                     const f32x4 decay = decay_of(at.a2, delta);
@@ -531,13 +406,13 @@ __global__ void __launch_bounds__(256) scan_backward_kernel(const ScanArgs p, ui
             for (int j = subs; j--;) {
                 const uint32_t t = from + j * kSteps;
                 Fetch f;
-                f.template load<T, true>(p, at, n, t, to);
+                f.template load<true>(p, at, n, t, to);
                 __syncthreads();
                 f.put(p, at, t, to, s.r);
 #pragma unroll
                 for (int i = 0; i < Fetch::N; ++i)
                     if (Fetch::slot(i) < kSteps * Lane::CH)
-                        s.dy[Fetch::slot(i)] = p.z ? f.dy[i] * silu(f.z[i]) : f.dy[i];
+                        s.dy[Fetch::slot(i)] = p.z ? (float)f.dy[i] * silu((float)f.z[i]) : (float)f.dy[i];
                 __syncthreads();
                 const uint32_t resets = __builtin_amdgcn_readfirstlane(s.r.resets);
                 f32x4 before[kSteps], decay[kSteps];
@@ -547,7 +422,7 @@ __global__ void __launch_bounds__(256) scan_backward_kernel(const ScanArgs p, ui
                     const float delta = s.r.delta[k * Lane::CH + mine], u = s.r.u[k * Lane::CH + mine];
                     const f32x4 b = *reinterpret_cast<const f32x4*>(&s.r.b[k * Lane::SP + 4 * sub]);
                     decay[k] = decay_of(at.a2, delta);
-                    if (resets >> k & 1) h = f32x4{};
+                    if (resets >> k & 1) clear_states(h);
                     before[k] = h;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) h[i] = __builtin_fmaf(decay[k][i], h[i], u * b[i]);
@@ -573,7 +448,7 @@ __global__ void __launch_bounds__(256) scan_backward_kernel(const ScanArgs p, ui
                         h[i] = before[k][i];
                     }
                     // the state before an episode's first step is not h but 0
-                    if (resets >> k & 1) g = f32x4{};
+                    if (resets >> k & 1) clear_states(g);
                     sum_channels<L>(v, s.bc[k][wave]);
                     float three[3] = {gb, ga, y};
                     group_sum_n<L>(three);
@@ -599,17 +474,17 @@ __global__ void __launch_bounds__(256) scan_backward_kernel(const ScanArgs p, ui
                     if (!Fetch::in(at, i, t, to)) continue;
                     const int e = Fetch::slot(i);
                     const uint64_t row = p.at.row(t + Fetch::step(i), n);
-                    const float raw = f.dt[i] + bias, delta = s.r.delta[e], dy = s.dy[e];
+                    const float x = (float)f.x[i], raw = (float)f.dt[i] + bias, delta = s.r.delta[e], dy = s.dy[e];
                     if (p.z && p.dz) {
-                        const float y = __builtin_fmaf(skip, f.x[i], s.y[e]);
-                        static_cast<T*>(p.dz)[row * p.dz_ld + ch] = (T)(f.dy[i] * y * silu_slope(f.z[i]));
+                        const float y = __builtin_fmaf(skip, x, s.y[e]);
+                        static_cast<T*>(p.dz)[row * p.dz_ld + ch] = (T)((float)f.dy[i] * y * silu_slope((float)f.z[i]));
                     }
                     static_cast<T*>(p.dx)[row * p.dx_ld + ch] = (T)__builtin_fmaf(dy, skip, delta * s.gb[e]);
                     float slope, rest;
                     sigmoid_of(raw, slope, rest);
-                    const float ddt = __builtin_fmaf(f.x[i], s.gb[e], s.ga[e] * 0.693147181f) * slope;
+                    const float ddt = __builtin_fmaf(x, s.gb[e], s.ga[e] * 0.693147181f) * slope;
                     static_cast<T*>(p.ddt)[row * p.ddt_ld + ch] = (T)ddt;
-                    dd = __builtin_fmaf(dy, f.x[i], dd);
+                    dd = __builtin_fmaf(dy, x, dd);
                     dbias += ddt;
                 }
                 for (int e = threadIdx.x; e < kSteps * 2 * Lane::SP; e += 256) {
@@ -679,10 +554,14 @@ uint32_t lanes_of(uint32_t states) {
 
 struct ScanShape {
     uint32_t lanes, per, apiece, blocks, splits, split_steps;
+    uint32_t wide;  // channels of a quad, 0 where it is not quads that scan
 };
 // The steps are split where the channels and sequences alone give fewer than two workgroups
-// a CU: each split's steps are walked over twice, which pays once the chip is half idle.
-ScanShape scan_shape(uint32_t steps, uint32_t seqs, uint32_t channels, uint32_t states, uint32_t groups) {
+// a CU: each split's steps are walked over twice, which pays once the chip is half idle. Quads take
+// 9 to 16 states (32 steps of 4096 x 256 with 16, bf16: 265 us without them, so 176; the gradient
+// 1170 and 720), two channels each where that leaves four workgroups a CU (the same with one: 195
+// and 760), but not rows whose steps lie too far apart for 31 bits.
+ScanShape scan_shape(uint32_t steps, uint32_t seqs, uint32_t channels, uint32_t states, uint32_t groups, bool far) {
     ScanShape s;
     s.lanes = lanes_of(states);
     s.per = channels / groups;
@@ -693,12 +572,20 @@ ScanShape scan_shape(uint32_t steps, uint32_t seqs, uint32_t channels, uint32_t 
     const uint32_t units = (steps + dev::kChunk - 1) / dev::kChunk;
     uint64_t splits = 1;
     if (have && have < 2 * kCus) splits = (4 * kCus + have - 1) / have;
-    if (splits > units / 2) splits = units / 2;
+    if (splits > units) splits = units;
     if (splits < 1) splits = 1;
     const uint32_t each = units ? (uint32_t)((units + splits - 1) / splits) : 1;
     s.splits = units ? (units + each - 1) / each : 1;
     s.split_steps = each * dev::kChunk;
+    s.wide = s.lanes == 4 && !far;
+    const uint32_t pairs = (s.per + 127) / 128;
+    if (s.wide && (uint64_t)pairs * groups * seqs * s.splits >= 4 * kCus)
+        s.wide = 2, s.apiece = pairs, s.blocks = pairs * groups;
     return s;
+}
+// Whether eight steps of an array of rows pass 31 bits.
+bool lies_far(uint64_t step_rows, uint64_t ld, uint32_t type) {
+    return step_rows * ld > (1ull << 27) / type_bytes(type);
 }
 
 uint64_t padded(uint64_t bytes) { return (bytes + 255) & ~(uint64_t)255; }
@@ -717,6 +604,10 @@ char* place_splits(char* at, const ScanShape& s, dev::ScanArgs& a) {
     return at;
 }
 
+// Each block's part of dB and dC, where a group has several.
+uint64_t shared_bytes(const ScanShape& s, uint64_t steps, uint64_t seqs, uint64_t groups, uint64_t states) {
+    return s.apiece > 1 ? padded(s.apiece * steps * seqs * groups * 2 * states * 4) : 0;
+}
 uint32_t backward_parts(const ScanShape& s, uint32_t seqs) {
     const uint64_t items = (uint64_t)seqs * s.splits, want = (8 * kCus + s.blocks - 1) / s.blocks;
     return (uint32_t)(items < want ? items : want);
@@ -736,41 +627,81 @@ void with_lanes(uint32_t lanes, Fn&& f) {
 }
 dim3 grid_of(uint64_t items) { return dim3((uint32_t)(items < kMostGroups ? items : kMostGroups)); }
 
+template <int C, bool FULL, class T>
+void launch_quad(hipStream_t st, const dev::ScanArgs& a, uint64_t items) {
+    if (FULL && a.z)
+        hipLaunchKernelGGL((dev::scan_quad_kernel<T, C, FULL, FULL>), grid_of(items), dim3(256), 0, st, a, items);
+    else
+        hipLaunchKernelGGL((dev::scan_quad_kernel<T, C, FULL, false>), grid_of(items), dim3(256), 0, st, a, items);
+}
+
 template <class T>
-int scan(hipStream_t st, const dev::ScanArgs& a, const ScanShape& s) {
-    const uint64_t each = (uint64_t)s.blocks * a.at.seqs;
+int scan(hipStream_t st, const dev::ScanArgs& given, const ScanShape& s) {
+    dev::ScanArgs a = given;
     if (a.at.steps <= 1 && !a.checkpoints) {
-        with_lanes(s.lanes, [&](auto l) {
-            hipLaunchKernelGGL((dev::scan_step_kernel<T, decltype(l)::value>), grid_of(each), dim3(256), 0, st, a, each);
-        });
+        if (s.wide) {
+            a.apiece = (s.per + 63) / 64, a.blocks = a.apiece * a.groups;
+            const uint64_t items = (uint64_t)a.blocks * ((a.at.seqs + 3) / 4);
+            if (a.z)
+                hipLaunchKernelGGL((dev::scan_quad_step_kernel<T, true>), grid_of(items), dim3(256), 0, st, a, items);
+            else
+                hipLaunchKernelGGL((dev::scan_quad_step_kernel<T, false>), grid_of(items), dim3(256), 0, st, a, items);
+        } else {
+            const uint64_t items = (uint64_t)s.blocks * a.at.seqs;
+            with_lanes(s.lanes, [&](auto l) {
+                hipLaunchKernelGGL((dev::scan_step_kernel<T, decltype(l)::value>), grid_of(items), dim3(256), 0, st, a,
+                                   items);
+            });
+        }
         MG_HIP(hipGetLastError(), "selective scan step launch");
         return MG_OK;
     }
-    with_lanes(s.lanes, [&](auto l) {
-        constexpr int L = decltype(l)::value;
-        if (s.splits > 1) {
-            const uint64_t ends = each * (s.splits - 1);
-            hipLaunchKernelGGL((dev::scan_kernel<T, L, false>), grid_of(ends), dim3(256), 0, st, a, ends);
-        }
-        const uint64_t all = each * s.splits;
-        hipLaunchKernelGGL((dev::scan_kernel<T, L, true>), grid_of(all), dim3(256), 0, st, a, all);
-    });
+    const uint64_t each = (uint64_t)s.blocks * a.at.seqs, ends = each * (s.splits - 1), all = each * s.splits;
+    if (s.wide == 2) {
+        if (ends) launch_quad<2, false, T>(st, a, ends);
+        launch_quad<2, true, T>(st, a, all);
+    } else if (s.wide) {
+        if (ends) launch_quad<1, false, T>(st, a, ends);
+        launch_quad<1, true, T>(st, a, all);
+    } else {
+        with_lanes(s.lanes, [&](auto l) {
+            constexpr int L = decltype(l)::value;
+            if (ends) hipLaunchKernelGGL((dev::scan_kernel<T, L, false>), grid_of(ends), dim3(256), 0, st, a, ends);
+            hipLaunchKernelGGL((dev::scan_kernel<T, L, true>), grid_of(all), dim3(256), 0, st, a, all);
+        });
+    }
     MG_HIP(hipGetLastError(), "selective scan launch");
     return MG_OK;
+}
+
+template <int C, class T>
+void launch_quad_backward(hipStream_t st, const dev::ScanArgs& a, uint64_t ends, uint32_t parts) {
+    if (ends)
+        hipLaunchKernelGGL((dev::scan_quad_ends_backward_kernel<T, C>), grid_of(ends), dim3(256), 0, st, a, ends);
+    const dim3 grid(a.blocks * parts);
+    if (a.z)
+        hipLaunchKernelGGL((dev::scan_quad_backward_kernel<T, C, true>), grid, dim3(256), 0, st, a, parts);
+    else
+        hipLaunchKernelGGL((dev::scan_quad_backward_kernel<T, C, false>), grid, dim3(256), 0, st, a, parts);
 }
 
 template <class T>
 int scan_backward(hipStream_t st, const dev::ScanArgs& a, const ScanShape& s, float* da, float* dd, float* dbias) {
     const uint32_t parts = backward_parts(s, a.at.seqs);
     if (parts) {
-        with_lanes(s.lanes, [&](auto l) {
-            constexpr int L = decltype(l)::value;
-            if (s.splits > 1) {
-                const uint64_t ends = (uint64_t)s.blocks * a.at.seqs * (s.splits - 1);
-                hipLaunchKernelGGL((dev::scan_ends_backward_kernel<T, L>), grid_of(ends), dim3(256), 0, st, a, ends);
-            }
-            hipLaunchKernelGGL((dev::scan_backward_kernel<T, L>), dim3(s.blocks * parts), dim3(256), 0, st, a, parts);
-        });
+        const uint64_t ends = (uint64_t)s.blocks * a.at.seqs * (s.splits - 1);
+        if (s.wide == 2)
+            launch_quad_backward<2, T>(st, a, ends, parts);
+        else if (s.wide)
+            launch_quad_backward<1, T>(st, a, ends, parts);
+        else
+            with_lanes(s.lanes, [&](auto l) {
+                constexpr int L = decltype(l)::value;
+                if (ends)
+                    hipLaunchKernelGGL((dev::scan_ends_backward_kernel<T, L>), grid_of(ends), dim3(256), 0, st, a, ends);
+                hipLaunchKernelGGL((dev::scan_backward_kernel<T, L>), dim3(s.blocks * parts), dim3(256), 0, st, a,
+                                   parts);
+            });
         MG_HIP(hipGetLastError(), "selective scan backward launch");
         if (s.apiece > 1 && a.at.steps) {
             const uint64_t cells = (uint64_t)a.at.steps * a.at.seqs * a.groups * 2 * a.states;
@@ -812,6 +743,11 @@ int check_inputs(const char* what, Args& p, bool any) {
     return MG_OK;
 }
 template <class Args>
+bool inputs_far(const Args& p) {
+    return lies_far(p.step_rows, p.x_ld, p.type) || lies_far(p.step_rows, p.dt_ld, p.type) ||
+           lies_far(p.step_rows, p.z_ld, p.type);
+}
+template <class Args>
 dev::ScanArgs inputs_of(const Args& p, const ScanShape& s) {
     dev::ScanArgs a{};
     a.at = {p.reset, p.lengths, p.step_rows, p.seq_rows, p.steps, p.seqs};
@@ -839,7 +775,7 @@ int mg_selective_scan_workspace(uint32_t steps, uint32_t seqs, uint32_t channels
         (rc = check_states(what, channels, states, 1)))
         return rc;
     // more groups make more blocks, and those at most as many splits
-    *bytes = split_bytes(scan_shape(steps, seqs, channels, states, 1), seqs, channels, states);
+    *bytes = split_bytes(scan_shape(steps, seqs, channels, states, 1, false), seqs, channels, states);
     return MG_OK;
 }
 
@@ -858,7 +794,8 @@ int mg_selective_scan(void* stream, const mg_selective_scan_args* args) {
         (rc = check_vector(what, "checkpoints", p.checkpoints, MG_TYPE_FP32, false)))
         return rc;
     if (!p.seqs || (!p.steps && !p.final)) return MG_OK;
-    const ScanShape s = scan_shape(p.steps, p.seqs, p.channels, p.states, p.groups);
+    const ScanShape s = scan_shape(p.steps, p.seqs, p.channels, p.states, p.groups,
+                                   inputs_far(p) || lies_far(p.step_rows, p.y_ld, p.type));
     if ((rc = check_workspace(what, p.workspace, p.workspace_bytes, split_bytes(s, p.seqs, p.channels, p.states))))
         return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
@@ -881,10 +818,13 @@ int mg_selective_scan_backward_workspace(uint32_t steps, uint32_t seqs, uint32_t
     if ((rc = check_rollout(what, steps, seqs, channels, MG_TYPE_FP32, &a, &b, nullptr)) ||
         (rc = check_states(what, channels, states, groups)))
         return rc;
-    const ScanShape s = scan_shape(steps, seqs, channels, states, groups);
-    const uint64_t shared = s.apiece > 1 ? (uint64_t)s.apiece * steps * seqs * groups * 2 * states * 4 : 0;
-    *bytes = split_bytes(s, seqs, channels, states) + padded(shared) +
-             padded((uint64_t)backward_parts(s, seqs) * channels * (states + 2) * 4);
+    *bytes = 0;
+    for (bool far : {false, true}) {
+        const ScanShape s = scan_shape(steps, seqs, channels, states, groups, far);
+        const uint64_t need = split_bytes(s, seqs, channels, states) + shared_bytes(s, steps, seqs, groups, states) +
+                              padded((uint64_t)backward_parts(s, seqs) * channels * (states + 2) * 4);
+        *bytes = need > *bytes ? need : *bytes;
+    }
     return MG_OK;
 }
 
@@ -915,7 +855,11 @@ int mg_selective_scan_backward(void* stream, const mg_selective_scan_backward_ar
     MG_CHECK(p.z || !p.dz, MG_ERR_INVALID, "selective scan backward: dz without z");
     const bool sums = p.da || p.dd || p.ddt_bias;
     if (!sums && (!p.seqs || (!p.steps && !p.dinitial))) return MG_OK;
-    const ScanShape s = scan_shape(p.steps, p.seqs, p.channels, p.states, p.groups);
+    const ScanShape s = scan_shape(p.steps, p.seqs, p.channels, p.states, p.groups,
+                                   inputs_far(p) || lies_far(p.step_rows, p.dy_ld, p.type) ||
+                                       lies_far(p.step_rows, p.dx_ld, p.type) ||
+                                       lies_far(p.step_rows, p.ddt_ld, p.type) ||
+                                       lies_far(p.step_rows, p.dz_ld, p.type));
     uint64_t need = 0;
     mg_selective_scan_backward_workspace(p.steps, p.seqs, p.channels, p.states, p.groups, &need);
     if ((rc = check_workspace(what, p.workspace, p.workspace_bytes, need))) return rc;
@@ -928,7 +872,7 @@ int mg_selective_scan_backward(void* stream, const mg_selective_scan_backward_ar
     a.dy_ld = p.dy_ld, a.dx_ld = p.dx_ld, a.ddt_ld = p.ddt_ld, a.db_ld = p.db_ld, a.dc_ld = p.dc_ld, a.dz_ld = p.dz_ld;
     char* at = place_splits(static_cast<char*>(p.workspace), s, a);
     a.shared = reinterpret_cast<float*>(at);
-    if (s.apiece > 1) at += padded((uint64_t)s.apiece * p.steps * p.seqs * p.groups * 2 * p.states * 4);
+    at += shared_bytes(s, p.steps, p.seqs, p.groups, p.states);
     a.sums = sums ? reinterpret_cast<float*>(at) : nullptr;
     return p.type == MG_TYPE_FP32   ? scan_backward<float>(st, a, s, p.da, p.dd, p.ddt_bias)
            : p.type == MG_TYPE_BF16 ? scan_backward<__bf16>(st, a, s, p.da, p.dd, p.ddt_bias)

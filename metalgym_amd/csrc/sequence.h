@@ -28,12 +28,10 @@ __device__ __forceinline__ void sigmoid_of(float v, float& s, float& rest) {
     const float r = __builtin_amdgcn_rcpf(1.0f + t), tr = t * r;
     s = v >= 0.0f ? r : tr;
     rest = v >= 0.0f ? tr : r;
-    if (v != v) s = rest = v;
 }
+// v / (1 + e^-v): 0 where the exponential leaves fp32's range.
 __device__ __forceinline__ float silu(float v) {
-    float s, rest;
-    sigmoid_of(v, s, rest);
-    return v * s;
+    return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * v));
 }
 __device__ __forceinline__ float silu_slope(float v) {
     float s, rest;
@@ -41,25 +39,17 @@ __device__ __forceinline__ float silu_slope(float v) {
     return s * (1.0f + v * rest);
 }
 
-// log(1 + e^v) = max(v, 0) + log1p(t), t = e^-|v|. A small t is the whole of the result for
-// negative v, so e^-|v| takes its argument's rounding along, and log1p is 2 atanh(t / (2 + t))
-// by its series (its argument is at most 1/3: eight terms leave 2^-28).
+// log(1 + e^v) = max(v, 0) + log(1 + t), t = e^-|v|. A small t is the whole of the result for
+// negative v: e^-|v| takes its argument's rounding along, and the logarithm what 1 + t lost of t.
 __device__ __forceinline__ float softplus(float v) {
     const float u = __builtin_fmaxf(-__builtin_fabsf(v), -200.0f);
     const float hi = u * 1.44269504f;
-    const float lo = __builtin_fmaf(u, 1.44269504f, -hi) + u * 1.92596299e-8f;
+    const float lo = __builtin_fmaf(u, 1.92596299e-8f, __builtin_fmaf(u, 1.44269504f, -hi));
     float t = __builtin_amdgcn_exp2f(hi);
     t = __builtin_fmaf(t, lo * 0.693147181f, t);
-    const float s = t * __builtin_amdgcn_rcpf(2.0f + t), q = s * s;
-    float p = 1.0f / 15;
-    p = __builtin_fmaf(p, q, 1.0f / 13);
-    p = __builtin_fmaf(p, q, 1.0f / 11);
-    p = __builtin_fmaf(p, q, 1.0f / 9);
-    p = __builtin_fmaf(p, q, 1.0f / 7);
-    p = __builtin_fmaf(p, q, 1.0f / 5);
-    p = __builtin_fmaf(p, q, 1.0f / 3);
-    p = __builtin_fmaf(p, q, 1.0f);
-    const float r = __builtin_fmaxf(v, 0.0f) + 2.0f * s * p;
+    const float w = 1.0f + t;
+    const float l = __builtin_fmaf(__builtin_amdgcn_logf(w), 0.693147181f, t - (w - 1.0f));
+    const float r = __builtin_fmaxf(v, 0.0f) + l;
     return v != v ? v : r;
 }
 

@@ -66,7 +66,8 @@ def silu_slope(v):
 
 
 def softplus(v):
-    """Exponential 4, quotient 5, series and its products 6 half steps of the logarithm, then a sum."""
+    """Exponential 4 half steps, its sum with 1 what is made good again but for a share t, the
+    logarithm's instruction 2, its product and sums 4, then a sum."""
     with np.errstate(over="ignore"):
         log = np.log1p(np.exp(-np.abs(v.v)))
         slope = 1 / (1 + np.exp(-v.v))

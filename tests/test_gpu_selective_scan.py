@@ -324,3 +324,48 @@ def test_selective_scan_gradient_against_differences(mg, steps):
         got = got.get(c.live) if isinstance(got, Operand) else got.get()
         # h^2 of the differences (third derivatives of a few), fp32's sums of terms that cancel
         assert abs((got * along).sum() - (ends[0] - ends[1]) / (2 * h)) <= 2e-5 * np.abs(got * along).sum() + 1e-4, name
+
+
+def test_selective_scan_rows_far_apart(mg):
+    """Steps 192 MB apart, every array a column panel of the same rows: past what 31 bits hold in
+    eight steps, and past 32 in all."""
+    c = Case(27, 2, 20, 16, "fp32", seed=14)
+    near_f = c.forward(mg)
+    near_b = c.backward(mg, None)
+    ld, wide = 1 << 24, 64
+    p = {k: v for k, v in c.inputs(mg).items() if not k.endswith("_ld")}
+    p.update(step_rows=3, seq_rows=1, **{k + "_ld": ld for k in ("x", "dt", "b", "c", "z")})
+    whole = mg.DeviceBuffer((27 * 3 * ld) * 4)
+    names = ("x", "dt", "b", "c", "z", "dy", "y", "dx", "ddt", "db", "dc", "dz")
+    at = {k: whole.ptr + 4 * wide * i for i, k in enumerate(names)}
+    row = lambda t, n: 4 * (3 * t + n) * ld  # noqa: E731
+    reset = np.zeros(27 * 3, np.uint8)
+    for t in range(27):
+        for n in range(2):
+            for k in ("x", "dt", "b", "c", "z", "dy"):
+                mg.h2d(at[k] + row(t, n), getattr(c, k)[t, n].astype(np.float32))
+            reset[3 * t + n] = c.reset[t, n]
+    resets = bytes_of(mg, reset)
+    state = (2, 20, 16)
+    final, kept = Held(mg, None, shape=state), Held(mg, None, shape=(1,) + state)
+    p.update(reset=resets.ptr, b=at["b"], c=at["c"], z=at["z"])
+    mg.selective_scan(at["x"], at["dt"], at["y"], *c.dims(), y_ld=ld, final=final.ptr, checkpoints=kept.ptr, **p)
+    sums = dict(da=Held(mg, None, shape=c.a.shape), dd=Held(mg, None, shape=(20,)),
+                ddt_bias=Held(mg, None, shape=(20,)), dinitial=Held(mg, None, shape=state))
+    space = mg.DeviceBuffer(mg.selective_scan_backward_workspace(*c.dims()[:4]) + 256)
+    grads = {k: at[k] for k in ("dx", "ddt", "db", "dc", "dz")}
+    dfinal = Held(mg, c.dfinal)
+    mg.selective_scan_backward(at["x"], at["dt"], at["dy"], *c.dims(), dfinal=dfinal.ptr, workspace=space.ptr,
+                               workspace_bytes=space.nbytes, dy_ld=ld, **{k + "_ld": ld for k in grads}, **grads,
+                               **{k: v.ptr for k, v in sums.items()}, **p)
+    mg._capi.check(mg.lib().mg_synchronize())
+    want = c.reference()
+    assert_within(final.get(), want["final"].v, want["final"].tolerance("fp32"), "final")
+    for k in ("y",) + tuple(grads):
+        w = want[k]
+        got = np.array([[mg.d2h(at[k] + row(t, n), np.float32, (w.v.shape[2],)) for n in range(2)] for t in range(27)])
+        assert_within(got.astype(np.float64), w.v, w.tolerance("fp32"), k)
+    for k, v in sums.items():
+        assert_within(v.get(), want[k].v, want[k].tolerance("fp32"), k)
+    assert_within(near_f["final"].get(), final.get(), 2 * want["final"].tolerance("fp32"), "near and far")
+    assert_within(near_b["da"].get(), sums["da"].get(), 2 * want["da"].tolerance("fp32"), "near and far")
