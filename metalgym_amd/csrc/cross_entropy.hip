@@ -49,13 +49,12 @@ struct HeadScales {
     float x_back, w_back, g_back;
 };
 
-// An operand of `rows` rows of 16-bit elements, `ld` apart: a high plane, and where values
-// are pairs a low one `plane` elements after it.
+// Rows of 16-bit elements, `ld` apart: a high plane, and where values are pairs a low one
+// `plane` elements after it.
 struct HeadOperand {
     const void* base;
     uint64_t plane;
     uint32_t ld;
-    uint32_t rows;
 };
 
 enum { kStats = 0, kLogitGrad = 1, kGrad = 2 };
@@ -63,7 +62,9 @@ enum { kStats = 0, kLogitGrad = 1, kGrad = 2 };
 // One product's tiles: M from a, N from b, contraction K in `splits` ranges of `range`.
 struct HeadProduct {
     HeadOperand a, b;
+    const uint32_t* live;  // a bit for each row of a turned a; the others count as 0. NULL: all
     uint32_t k, range, splits;
+    uint32_t m, n;  // the result's sides
     uint32_t tiles_m, tiles_n;
     // kGrad: out(n, m) = sum, n down the rows of out; or fp32 parts [splits][out rows][parts_ld]
     void* out;
@@ -90,8 +91,8 @@ struct HeadArgs {
     const float* dloss;
     const float* entropy;
     const float* dentropy;
-    void* g;    // [rows_ld][g_ld], planes g_plane apart
-    void* gt;   // [g_ld][rows_ld]
+    void* g;  // [rows][g_ld], planes g_plane apart
+    uint32_t* live;
     uint32_t g_ld;
     uint64_t g_plane;
 };
@@ -104,6 +105,15 @@ constexpr uint32_t kNowhere = 0x80000000u;  // an offset past every operand's en
 // The logarithm and the exponential in base 2, by the hardware's instructions.
 __device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
 constexpr float kLog2 = 1.44269504f, kLn2 = 0.693147181f;
+
+// The two halves of a value; what is not finite lies in the low one alone, so that its products
+// with another's halves are of fp32's sign and infinity.
+template <class H>
+__device__ __forceinline__ void split_half(float v, H& hi, H& lo) {
+    const bool odd = !(__builtin_fabsf(v) < 65504.0f);
+    hi = odd ? (H)0.0f : (H)v;
+    lo = odd ? (H)v : (H)(v - (float)hi);
+}
 
 // max, sum of 2^(s - max), sum of 2^(s - max) (s - max), of logits in base 2. Of
 // nothing: -inf, 0, 0.
@@ -121,91 +131,122 @@ struct RowStats {
     }
 };
 
-// One tile of MI x 64 rows of a by 256 rows of b. Eight waves, two along a and four
-// along b, MI x 2 tiles of 32 x 32 each. A stage is 32 contraction elements of every row, 64
-// bytes, which go from memory straight to LDS: a lane's 16 bytes lie in the order of the
-// lanes, so the places of a row's four are exchanged on the way by the lane's own address
-// (bits 1 and 2 of the row), and the reads of eight rows then meet no bank twice. The ring
-// holds four stages; the waves meet once a stage, when the next has arrived, and read the
-// next one's fragments under this one's products.
-template <class H, int KIND, int MI, bool PAIRS>
-__global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
+// One operand's part in the main loop: SIDE rows of a tile, of which a stage holds 32
+// contraction elements in LDS. Rows go from memory straight there, a wave's 64 lanes in order, 16
+// bytes each; where they come from is each lane's own choice, which keeps reads off one bank.
+//
+// Not TURNED: the contraction runs along a row in memory, and a stage is 64 bytes of every row. The
+// places of a row's four 16 bytes are exchanged by bits 1 and 2 of the row: a read of eight rows'
+// fragments (lane l holds row l % 32 and eight elements of 16, by l / 32) then meets no bank twice.
+//
+// TURNED: it runs from row to row, and a stage is 32 rows of SIDE elements. Reads of four
+// elements by 16 lanes that hold each other's columns (ds_read_b64_tr_b16: of 4 rows x 16 columns
+// a lane gets a column) make the same fragments; the places of 32 bytes are exchanged by the
+// row's last two bits, so that the four rows lie in different banks.
+template <class H, int SIDE, bool TURNED>
+struct HeadSide {
+    typedef typename Halves<H>::x8 x8;
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    static constexpr int L = SIDE / 128;  // loads of a wave and stage
+    static constexpr int kBytes = SIDE * 64;
+    const H* base[2];
+    uint32_t ld, off[L], row[L];
+
+    // `from`: the tile's first row (or column) of `rows`
+    __device__ __forceinline__ HeadSide(const HeadOperand& o, uint32_t from, uint32_t rows, int wave, int lane) {
+        ld = o.ld;
+        base[0] = static_cast<const H*>(o.base) + (TURNED ? from : (uint64_t)from * ld);
+        base[1] = base[0] + o.plane;
+        const uint32_t have = rows > from ? rows - from : 0;
+#pragma unroll
+        for (int c = 0; c < L; ++c) {
+            if constexpr (TURNED) {
+                constexpr uint32_t kLanes = SIDE / 8;  // of a row
+                row[c] = (wave * L + c) * (64 / kLanes) + lane / kLanes;
+                const uint32_t at = lane % kLanes, col = (((at >> 1 ^ (row[c] & 3)) << 1) + (at & 1)) * 8;
+                off[c] = col < have ? (row[c] * ld + col) * 2 : kNowhere;
+            } else {
+                const uint32_t r = (wave * L + c) * 16 + (lane >> 2);
+                row[c] = ((lane & 3) ^ (lane >> 3 & 3)) * 8;  // the first of its elements
+                off[c] = r < have ? (r * ld + row[c]) * 2 : kNowhere;
+            }
+        }
+    }
+    // The stage of contraction elements k ..., up to `to`.
+    __device__ __forceinline__ void load(char* at, int wave, uint32_t k, uint32_t to, bool low, uint32_t live) const {
+        // a row of W or X may lie anywhere, so its stage has an address of its own
+        const H* const p = base[low] + (TURNED ? (uint64_t)k * ld : (uint64_t)k);
+        const __amdgpu_buffer_rsrc_t r =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<H*>(p), (short)0, 0x7fffffff, 0x00020000);
+#pragma unroll
+        for (int c = 0; c < L; ++c) {
+            bool in = k + row[c] < to;
+            if constexpr (TURNED) in = in && (live >> row[c] & 1);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                r, (__attribute__((address_space(3))) void*)(at + (wave * L + c) * 1024), 16,
+                (int)(in ? off[c] : kNowhere), 0, 0, 0);
+        }
+    }
+    // the fragment of rows 32 b ... of the tile and the stage's elements 16 h ...
+    static __device__ __forceinline__ x8 read(const char* at, int b, int h, int lane) {
+        if constexpr (TURNED) {
+            const int k = 16 * h + 8 * (lane >> 5) + (lane >> 2 & 3), chunk = 2 * b + (lane >> 4 & 1);
+            auto four = [&](int more) {
+                const int r = k + more;  // its last two bits are k's
+                const char* const p = at + r * (SIDE * 2) + ((chunk ^ (r & 3)) << 5) + ((lane & 3) << 3);
+                return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+            };
+            const s16x4 lo = four(0), hi = four(4);
+            return __builtin_bit_cast(x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            const int row = lane & 31;
+            return *reinterpret_cast<const x8*>(at + b * 2048 + row * 64 +
+                                                (((2 * h + (lane >> 5)) ^ (row >> 1 & 3)) << 4));
+        }
+    }
+};
+
+// One tile of MI x 64 by 256. Eight waves, two along a and four along b, MI x 2 tiles of 32 x 32
+// each. The ring holds four stages; the waves meet once a stage, when the next has arrived,
+// and read the next one's fragments under this one's products.
+template <class H, int MI, bool PAIRS, bool AT, bool BT>
+__device__ __forceinline__ void head_product(const HeadProduct& p, uint32_t tm, uint32_t tn, uint32_t split, char* lds,
+                                             f32x16 (&acc)[MI][2]) {
     using X = Halves<H>;
     typedef typename X::x8 x8;
-    typedef typename X::x4 x4;
-    constexpr int TM = MI * 64, kStage = (TM + kHeadN) * 64, LA = TM / 128, LB = kHeadN / 128, L = LA + LB;
-    __shared__ __align__(1024) char lds[kHeadRing * kStage];
-    const uint32_t tile_of_all = xcd_run(blockIdx.x, gridDim.x);
-    const uint32_t sel = KIND == kGrad && tile_of_all >= args.tiles ? 1 : 0;
-    const HeadProduct& p = args.p[sel];
-    uint32_t tile = tile_of_all - (sel ? args.tiles : 0);
-    const uint32_t per = p.tiles_m * p.tiles_n, split = tile / per;
-    tile -= split * per;
-    // tiles that share their rows of a lie side by side
-    const uint32_t tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
+    using A = HeadSide<H, MI * 64, AT>;
+    using B = HeadSide<H, kHeadN, BT>;
+    constexpr int kStage = A::kBytes + B::kBytes, L = A::L + B::L;
     const uint32_t from = split * p.range, to = p.k - from < p.range ? p.k : from + p.range;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
-
-    // this wave's loads of a stage: 16 rows each
-    const uint32_t chunk = (lane & 3) ^ (lane >> 3 & 3);  // of the row's four
-    __amdgpu_buffer_rsrc_t res[2][2];                      // [a, b][high, low]
-    uint32_t off[L];
-    {
-        const uint32_t m0 = tm * TM, n0 = tn * kHeadN;
-        auto bind = [&](const HeadOperand& o, uint32_t r0, int which) {
-            const uint32_t left = o.rows > r0 ? o.rows - r0 : 0;
-            const uint32_t most = which ? kHeadN : TM, have = left < most ? left : most;
-            const uint32_t bytes = have ? ((have - 1) * o.ld + p.k) * 2 : 0;
-            H* at = const_cast<H*>(static_cast<const H*>(o.base)) + (uint64_t)r0 * o.ld;
-            res[which][0] = __builtin_amdgcn_make_buffer_rsrc(at, (short)0, (int)bytes, 0x00020000);
-            res[which][1] = __builtin_amdgcn_make_buffer_rsrc(at + o.plane, (short)0, (int)bytes, 0x00020000);
-            const int n = which ? LB : LA;
-#pragma unroll
-            for (int c = 0; c < (which ? LB : LA); ++c) {
-                const uint32_t r = (wave * n + c) * 16 + (lane >> 2);
-                off[(which ? LA : 0) + c] = r < have ? r * o.ld * 2 + chunk * 16 : kNowhere;
-            }
-        };
-        bind(p.a, m0, 0);
-        bind(p.b, n0, 1);
-    }
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1;
+    const A a(p.a, tm * (MI * 64), p.m, wave, lane);
+    const B b(p.b, tn * kHeadN, p.n, wave, lane);
     uint32_t k = from;
     int seg = 0;
     const uint32_t each = (to - from + kHeadK - 1) / kHeadK;
     const uint32_t stages = (each * (PAIRS ? 3 : 1) + 1) & ~1u;  // the last may be empty
+    const uint32_t* const live = AT ? p.live : nullptr;
     auto load = [&](uint32_t slot) {
         char* const at = lds + slot * kStage;
-        const bool in = k + chunk * 8 < to && (!PAIRS || seg < 3);
-#pragma unroll
-        for (int c = 0; c < L; ++c) {
-            const int which = c >= LA;
-            const int n = which ? LB : LA, i = which ? c - LA : c;
-            char* const dst = at + (which ? TM * 64 : 0) + (wave * n + i) * 1024;
-            const uint32_t o = in && off[c] != kNowhere ? off[c] + k * 2 : kNowhere;
-            const bool low = PAIRS && seg == which;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(low ? res[which][1] : res[which][0],
-                                                     (__attribute__((address_space(3))) void*)dst, 16, (int)o, 0, 0, 0);
-        }
+        // pairs: low high, high low, high high; past the last an empty stage
+        const uint32_t end = PAIRS && seg > 2 ? 0 : to;
+        const uint32_t bits = live && k < end ? live[k / kHeadK] : ~0u;
+        a.load(at, wave, k, end, PAIRS && seg == 0, bits);
+        b.load(at + A::kBytes, wave, k, end, PAIRS && seg == 1, ~0u);
         k += kHeadK;
         if (PAIRS && k >= to) k = from, ++seg;
     };
-    // fragments: lane l holds row l % 32 and eight elements of the 16, by l / 32
-    const int row = lane & 31, twist = row >> 1 & 3;
-    const int at0 = row * 64 + (((lane >> 5) ^ twist) << 4), at1 = row * 64 + ((2 + (lane >> 5) ^ twist) << 4);
     x8 fa[2][2][MI], fb[2][2][2];
     auto read = [&](int set, uint32_t slot) {
-        const char* const a = lds + slot * kStage + wm * (MI * 2048);
-        const char* const b = lds + slot * kStage + TM * 64 + wn * 4096;
+        const char* const at = lds + slot * kStage;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int at = h ? at1 : at0;
 #pragma unroll
-            for (int i = 0; i < MI; ++i) fa[set][h][i] = *reinterpret_cast<const x8*>(a + i * 2048 + at);
+            for (int i = 0; i < MI; ++i) fa[set][h][i] = A::read(at, wm * MI + i, h, lane);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) fb[set][h][j] = *reinterpret_cast<const x8*>(b + j * 2048 + at);
+            for (int j = 0; j < 2; ++j) fb[set][h][j] = B::read(at + A::kBytes, wn * 2 + j, h, lane);
         }
     };
-    f32x16 acc[MI][2] = {};
 #pragma unroll
     for (uint32_t u = 0; u < (uint32_t)kHeadRing; ++u) load(u);
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kHeadRing - 1) * L) : "memory");
@@ -228,15 +269,42 @@ __global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
                 for (int i = 0; i < MI; ++i)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) acc[i][j] = X::mfma(fa[u][h][i], fb[u][h][j], acc[i][j]);
+            constexpr int kReads = 2 * (MI * (AT ? 2 : 1) + 2 * (BT ? 2 : 1)), kProducts = 4 * MI;
 #pragma unroll
-            for (int q = 0; q < 2 * (MI + 2); ++q) {
+            for (int q = 0; q < kProducts; ++q) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
+                if ((q + 1) * kReads / kProducts - q * kReads / kProducts == 1)
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
+                else
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last loads have left LDS alone
+}
+
+template <class H, int KIND, int MI, bool PAIRS>
+__global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
+    typedef typename Halves<H>::x4 x4;
+    constexpr int TM = MI * 64;
+    __shared__ __align__(1024) char lds[kHeadRing * (TM + kHeadN) * 64];
+    const uint32_t tile_of_all = xcd_run(blockIdx.x, gridDim.x);
+    const uint32_t sel = KIND == kGrad && tile_of_all >= args.tiles ? 1 : 0;
+    const HeadProduct& p = args.p[sel];
+    uint32_t tile = tile_of_all - (sel ? args.tiles : 0);
+    const uint32_t per = p.tiles_m * p.tiles_n, split = tile / per;
+    tile -= split * per;
+    // tiles that share their rows of a lie side by side
+    const uint32_t tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
+    f32x16 acc[MI][2] = {};
+    if constexpr (KIND != kGrad)
+        head_product<H, MI, PAIRS, false, false>(p, tm, tn, split, lds, acc);
+    else if (p.which)
+        head_product<H, MI, PAIRS, true, true>(p, tm, tn, split, lds, acc);
+    else
+        head_product<H, MI, PAIRS, true, false>(p, tm, tn, split, lds, acc);
 
     // register e of tile (i, j): row of a m(i, e), row of b n(j)
     const uint32_t m0 = tm * TM + wm * (MI * 32) + 4 * (lane >> 5), n0 = tn * kHeadN + wn * 64 + (lane & 31);
@@ -246,24 +314,24 @@ __global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const uint32_t n = n0 + 32 * j;
-            if (n >= p.b.rows) continue;
+            if (n >= p.n) continue;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
                     const uint32_t m = m0 + 32 * i + 2 * e;
-                    if (m >= p.a.rows) continue;
+                    if (m >= p.m) continue;
                     f32x4 v = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
                     if (p.parts) {
                         f32x4* const at = reinterpret_cast<f32x4*>(
-                            p.parts + ((uint64_t)split * p.b.rows + n) * p.parts_ld + m);
+                            p.parts + ((uint64_t)split * p.n + n) * p.parts_ld + m);
                         if (p.add) v += *at;
                         *at = v;
                         continue;
                     }
 #pragma unroll
                     for (int q = 0; q < 4; ++q) v[q] = v[q] * b0 * b1;
-                    const uint32_t count = p.a.rows - m;
+                    const uint32_t count = p.m - m;
                     auto put = [&](auto t) {
                         using T = decltype(t);
                         T* const at = static_cast<T*>(p.out) + n * p.out_ld + m;
@@ -284,38 +352,64 @@ __global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
                 }
         }
     } else {
-        const float to2 = sc.w_back * kLog2;
-        const uint32_t c0 = m0;  // of the piece
-        const bool edge = (tm + 1) * TM > p.a.rows;
-        if constexpr (KIND == kStats) {
-            __syncthreads();  // every wave is done with the ring
-            RowStats* const trade = reinterpret_cast<RowStats*>(lds);
+        // logits in base 2: two factors for pairs, as their product may leave fp32's range
+        const float to2 = PAIRS ? sc.w_back * kLog2 : kLog2;
+        const bool edge = (tm + 1) * TM > p.m;
+        if constexpr (KIND == kStats) __syncthreads();  // every wave is done with the ring
+        RowStats* const trade = reinterpret_cast<RowStats*>(lds);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t n = n0 + 32 * j;
-                const int32_t target = n < args.rows ? args.targets[n] : -1;
-                // two factors: their product may leave fp32's range
-                const float back = PAIRS && n < args.rows ? ldexpf(1.0f, -args.row_exp[n]) : 1.0f;
-                RowStats r{-__builtin_huge_valf(), 0.0f, 0.0f};
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t n = n0 + 32 * j;
+            int32_t target = -1;
+            if (n < args.rows) {
+                target = args.targets[n];
+                if constexpr (PAIRS) {
+                    const float back = ldexpf(1.0f, -args.row_exp[n]);
+#pragma unroll
+                    for (int i = 0; i < MI; ++i) acc[i][j] *= back;
+                }
+            }
+            // the target's place among the lane's classes, which are m0 - args.first + ...
+            const uint32_t hit = (uint32_t)target - args.first - m0;
+            const bool live = target >= 0 && (uint32_t)target < args.classes;
+            const bool meets = __any(live && hit < MI * 32);
+            if constexpr (KIND == kStats) {
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (m0 + 32 * i + 8 * (e >> 2) + (e & 3) >= p.m) acc[i][j][e] = -__builtin_huge_valf();
+                }
+                if (meets) {
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (live && hit == (uint32_t)(32 * i + 8 * (e >> 2) + (e & 3))) args.of[n] = acc[i][j][e] * to2;
+                }
+                float top = -__builtin_huge_valf();
 #pragma unroll
                 for (int i = 0; i < MI; ++i)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const uint32_t c = c0 + 32 * i + 8 * (e >> 2) + (e & 3);
-                        const float s = acc[i][j][e] * back * to2;
-                        acc[i][j][e] = edge && c >= p.a.rows ? -__builtin_huge_valf() : s;
-                        r.top = __builtin_fmaxf(r.top, acc[i][j][e]);
-                        if (target >= 0 && (uint32_t)target == c) args.of[n] = s;
-                    }
-                const float zero = r.top == -__builtin_huge_valf() ? 0.0f : r.top;
+                    for (int e = 0; e < 16; ++e) top = __builtin_fmaxf(top, acc[i][j][e]);
+                RowStats r{top * to2, 0.0f, 0.0f};
+                const float zero = top == -__builtin_huge_valf() ? 0.0f : r.top;
+                if (args.want_entropy) {
 #pragma unroll
-                for (int i = 0; i < MI; ++i)
+                    for (int i = 0; i < MI; ++i)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float d = acc[i][j][e] - zero, w = exp2_of(d);
-                        r.sum += w;
-                        r.weighted = __builtin_fmaf(w, __builtin_fmaxf(d, -1000.0f), r.weighted);
-                    }
+                        for (int e = 0; e < 16; ++e) {
+                            const float d = __builtin_fmaf(acc[i][j][e], to2, -zero), w = exp2_of(d);
+                            r.sum += w;
+                            r.weighted = __builtin_fmaf(w, __builtin_fmaxf(d, -1000.0f), r.weighted);
+                        }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) r.sum += exp2_of(__builtin_fmaf(acc[i][j][e], to2, -zero));
+                }
                 RowStats o;
                 float lo, hi;
                 lane_pair<32>(r.top, lo, hi), r.top = lo, o.top = hi;
@@ -323,7 +417,60 @@ __global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
                 lane_pair<32>(r.weighted, lo, hi), r.weighted = lo, o.weighted = hi;
                 r.join(o);
                 if (lane < 32) trade[wm * kHeadN + wn * 64 + 32 * j + lane] = r;
+            } else {
+                const uint32_t bits = (uint32_t)__ballot(live);  // the upper lanes' rows are the lower ones'
+                if (tm == 0 && wm == 0 && lane == 0) args.live[n / 32] = bits;
+                float lse2 = 0.0f, dl = 0.0f, de = 0.0f, ent = 0.0f;
+                if (live) {
+                    lse2 = args.lse[n] * kLog2, dl = args.dloss[n] * sc.g;
+                    if (args.dentropy) de = args.dentropy[n] * sc.g * kLn2, ent = args.entropy[n] * kLog2;
+                }
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float d = __builtin_fmaf(acc[i][j][e], to2, -lse2), prob = exp2_of(d);
+                        float g = dl * prob;
+                        if (args.dentropy) g = __builtin_fmaf(-de * prob, __builtin_fmaxf(d, -1000.0f) + ent, g);
+                        acc[i][j][e] = live ? g : 0.0f;
+                    }
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (m0 + 32 * i + 8 * (e >> 2) + (e & 3) >= p.m) acc[i][j][e] = 0.0f;
+                }
+                if (meets) {
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (live && hit == (uint32_t)(32 * i + 8 * (e >> 2) + (e & 3))) acc[i][j][e] -= dl;
+                }
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const uint32_t c = m0 + 32 * i + 2 * e;
+                        x4 hi, lo;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const float v = acc[i][j][e + q];
+                            hi[q] = (H)v;
+                            if constexpr (PAIRS) {
+                                H h, l;
+                                split_half<H>(v, h, l);
+                                hi[q] = h, lo[q] = l;
+                            }
+                        }
+                        H* const g = static_cast<H*>(args.g) + (uint64_t)n * args.g_ld + c;
+                        *reinterpret_cast<x4*>(g) = hi;
+                        if constexpr (PAIRS) *reinterpret_cast<x4*>(g + args.g_plane) = lo;
+                    }
             }
+        }
+        if constexpr (KIND == kStats) {
             __syncthreads();
             if (threadIdx.x < kHeadN) {
                 const uint32_t n = tn * kHeadN + threadIdx.x;
@@ -333,55 +480,6 @@ __global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
                     float* const at = args.stats + (uint64_t)tm * 3 * args.rows_ld + n;
                     at[0] = r.top, at[args.rows_ld] = r.sum, at[2 * (uint64_t)args.rows_ld] = r.weighted;
                 }
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t n = n0 + 32 * j;
-                int32_t target = -1;
-                float lse2 = 0.0f, dl = 0.0f, de = 0.0f, ent = 0.0f, back = 1.0f;
-                if (n < args.rows) {
-                    if (PAIRS) back = ldexpf(1.0f, -args.row_exp[n]);
-                    target = args.targets[n];
-                    lse2 = args.lse[n] * kLog2, dl = args.dloss[n] * sc.g;
-                    if (args.dentropy) de = args.dentropy[n] * sc.g, ent = args.entropy[n];
-                }
-                const bool live = target >= 0 && (uint32_t)target < args.classes;
-#pragma unroll
-                for (int i = 0; i < MI; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        const uint32_t c = c0 + 32 * i + 2 * e;
-                        float v[4];
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const float d = __builtin_fmaf(acc[i][j][e + q] * back, to2, -lse2), prob = exp2_of(d);
-                            float g = dl * prob;
-                            if (args.dentropy)
-                                g -= de * prob * __builtin_fmaf(__builtin_fmaxf(d, -1000.0f), kLn2, ent);
-                            if (live && c + q == (uint32_t)target - args.first) g -= dl;
-                            v[q] = live && !(edge && c + q >= p.a.rows) ? g : 0.0f;
-                        }
-                        x4 hi, lo;
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            hi[q] = (H)v[q];
-                            if constexpr (PAIRS) {
-                                // what is not finite lies in the low half alone
-                                const bool odd = !(__builtin_fabsf(v[q]) < 65504.0f);
-                                hi[q] = odd ? (H)0.0f : hi[q];
-                                lo[q] = odd ? (H)v[q] : (H)(v[q] - (float)hi[q]);
-                            }
-                        }
-                        H* const g = static_cast<H*>(args.g) + (uint64_t)n * args.g_ld + c;
-                        *reinterpret_cast<x4*>(g) = hi;
-                        if constexpr (PAIRS) *reinterpret_cast<x4*>(g + args.g_plane) = lo;
-                        // four rows of one class: the quad's lanes trade theirs
-                        H* const gt =
-                            static_cast<H*>(args.gt) + (uint64_t)(c + (lane & 3)) * args.rows_ld + (n & ~3u);
-                        *reinterpret_cast<x4*>(gt) = quad_transpose(hi);
-                        if constexpr (PAIRS) *reinterpret_cast<x4*>(gt + args.g_plane) = quad_transpose(lo);
-                    }
             }
         }
     }
@@ -462,108 +560,76 @@ __global__ void __launch_bounds__(256) head_amax_kernel(const AmaxArgs a0, const
         a.parts[blockIdx.x] = __builtin_fmaxf(__builtin_fmaxf(red[0], red[1]), __builtin_fmaxf(red[2], red[3]));
 }
 
-// Powers of two that bring the largest of each under 2^15, from the three arrays'
-// parts (NULL: 1).
-__global__ void __launch_bounds__(256) head_scales_kernel(const float* x, const float* w, const float* g,
-                                                          HeadScales* out) {
-    __shared__ float red[3][4];
-    const float* const from[3] = {x, w, g};
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
-        const float v = group_max<64>(from[k] ? from[k][threadIdx.x] : 0.0f);
-        if ((threadIdx.x & 63) == 0) red[k][threadIdx.x >> 6] = v;
-    }
-    __syncthreads();
-    if (threadIdx.x) return;
-    float s[3], back[3];
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
-        const float v = __builtin_fmaxf(__builtin_fmaxf(red[k][0], red[k][1]), __builtin_fmaxf(red[k][2], red[k][3]));
-        const int e = lift(v);
-        s[k] = from[k] ? ldexpf(1.0f, e) : 1.0f, back[k] = from[k] ? ldexpf(1.0f, -e) : 1.0f;
-    }
-    *out = HeadScales{s[0], s[1], s[2], back[0], back[1], back[2]};
-}
-
-// 16-bit copies of a [rows][cols] array: as it lies, [rows][ld], or turned, [cols][ld] with
-// rows whose target is none as zeros; zeros up to `fill` in the contraction. fp32 becomes
-// pairs at the scale.
-struct CopyArgs {
+// 16-bit copies of x (job 0) and W (job 1), [rows][ld] with zeros past their columns, of what
+// cannot be read as it lies. fp32 becomes pairs: W at the scale of all of it, x at each row's own
+// for the logits and at that of all rows with a target for the gradient of W.
+struct PrepareArgs {
     const void* from;
     uint64_t from_ld;
     uint32_t rows, cols;
-    uint32_t fill;  // elements of a copy's row that are written
+    void* to;  // nullable
+    void* to_even;  // of x, nullable
     uint32_t ld;
-    void* to;
     uint64_t plane;
-    const HeadScales* scales;
-    const int* row_exp;  // in place of the scale
-    uint32_t which;      // 0: x's scale, 1: W's
-    const int32_t* targets;
-    uint32_t classes;
+    const int* row_exp;  // of x
 };
-template <class H>
-__device__ __forceinline__ void split_half(float v, H& hi, H& lo) {
-    const bool odd = !(__builtin_fabsf(v) < 65504.0f);
-    hi = odd ? (H)0.0f : (H)v;
-    lo = odd ? (H)v : (H)(v - (float)hi);
-}
+struct PrepareScales {
+    const float* parts[3];  // of x, W and the gradients; NULL: 1
+    HeadScales* out;
+};
 template <class T, class H>
-__global__ void __launch_bounds__(256) head_copy_kernel(const CopyArgs a) {
-    constexpr bool kPairs = sizeof(T) == 4;
-    const uint32_t c = (blockIdx.x * 256 + threadIdx.x) * 4;
-    if (c >= a.fill) return;
+__global__ void __launch_bounds__(256) head_prepare_kernel(const PrepareArgs a0, const PrepareArgs a1,
+                                                           const PrepareScales s) {
     typedef typename Halves<H>::x4 x4;
-    for (uint32_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
-        const float scale = !kPairs ? 1.0f : a.row_exp ? ldexpf(1.0f, a.row_exp[r]) : a.scales->w;
-        const T* const from = static_cast<const T*>(a.from) + r * a.from_ld;
-        x4 hi, lo;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const T v = c + q < a.cols ? from[c + q] : (T)0.0f;
-            H h, l;
-            if constexpr (kPairs)
-                split_half<H>((float)v * scale, h, l);
-            else
-                h = (H)v;
-            hi[q] = h;
-            if constexpr (kPairs) lo[q] = l;
-        }
-        H* const to = static_cast<H*>(a.to) + (uint64_t)r * a.ld + c;
-        *reinterpret_cast<x4*>(to) = hi;
-        if constexpr (kPairs) *reinterpret_cast<x4*>(to + a.plane) = lo;
-    }
-}
-template <class T, class H>
-__global__ void __launch_bounds__(256) head_turn_kernel(const CopyArgs a) {
     constexpr bool kPairs = sizeof(T) == 4;
-    __shared__ T tile[64][65];
-    const float scale = kPairs ? (a.which ? a.scales->w : a.scales->x) : 1.0f;
-    const uint32_t c0 = blockIdx.x * 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (uint32_t r0 = blockIdx.y * 64; r0 < a.fill; r0 += gridDim.y * 64) {
-        __syncthreads();
+    __shared__ float red[3][4];
+    const uint32_t job = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const PrepareArgs& a = job ? a1 : a0;
+    // the largest of the parts, and with it each array's scale, in every workgroup
+    float scale[3] = {1.0f, 1.0f, 1.0f}, back[3] = {1.0f, 1.0f, 1.0f};
+    if (s.out) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            const uint32_t r = r0 + wave * 16 + k;
-            bool in = r < a.rows && c0 + lane < a.cols;
-            if (in && a.targets) in = a.targets[r] >= 0 && (uint32_t)a.targets[r] < a.classes;
-            tile[wave * 16 + k][lane] = in ? static_cast<const T*>(a.from)[r * a.from_ld + c0 + lane] : (T)0.0f;
+        for (int k = 0; k < 3; ++k) {
+            const float v = group_max<64>(s.parts[k] ? s.parts[k][threadIdx.x] : 0.0f);
+            if (!lane) red[k][wave] = v;
         }
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            const uint32_t c = c0 + wave * 16 + k;
-            if (c >= a.cols || r0 + lane >= a.fill) continue;
-            const T v = tile[lane][wave * 16 + k];
-            H* const to = static_cast<H*>(a.to) + (uint64_t)c * a.ld + r0 + lane;
-            if constexpr (kPairs) {
-                H h, l;
-                split_half<H>((float)v * scale, h, l);
-                to[0] = h, to[a.plane] = l;
-            } else {
-                to[0] = (H)v;
+        for (int k = 0; k < 3; ++k) {
+            if (!s.parts[k]) continue;
+            const int e = lift(__builtin_fmaxf(__builtin_fmaxf(red[k][0], red[k][1]), __builtin_fmaxf(red[k][2], red[k][3])));
+            scale[k] = ldexpf(1.0f, e), back[k] = ldexpf(1.0f, -e);
+        }
+        if (blockIdx.x == 0 && job == 0 && threadIdx.x == 0)
+            *s.out = HeadScales{scale[0], scale[1], scale[2], back[0], back[1], back[2]};
+    }
+    if (!a.to) return;
+    const uint32_t across = a.ld / 4;
+    const uint64_t all = (uint64_t)across * a.rows;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
+        const uint32_t r = (uint32_t)(i / across), c = (uint32_t)(i - (uint64_t)r * across) * 4;
+        const T* const from = static_cast<const T*>(a.from) + r * a.from_ld + c;
+        T v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = c + q < a.cols ? from[q] : (T)0.0f;
+        const uint64_t at = (uint64_t)r * a.ld + c;
+        auto put = [&](void* to, float by) {
+            x4 hi, lo;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if constexpr (kPairs) {
+                    H h, l;
+                    split_half<H>((float)v[q] * by, h, l);
+                    hi[q] = h, lo[q] = l;
+                } else {
+                    hi[q] = (H)v[q];
+                }
             }
-        }
+            *reinterpret_cast<x4*>(static_cast<H*>(to) + at) = hi;
+            if constexpr (kPairs) *reinterpret_cast<x4*>(static_cast<H*>(to) + a.plane + at) = lo;
+        };
+        put(a.to, !kPairs ? 1.0f : job ? scale[1] : ldexpf(1.0f, a.row_exp[r]));
+        if (kPairs && a.to_even) put(a.to_even, scale[0]);
     }
 }
 
@@ -591,8 +657,10 @@ namespace {
 
 constexpr uint32_t kMostHeadRows = 1u << 20, kMostClasses = 1u << 20, kMostWidth = 1u << 16;
 constexpr uint32_t kHeadM = 256;          // classes of a tile
-constexpr uint32_t kPieceCells = 1u << 25;  // logits of a piece: 512 tiles, two rounds of the chip's CUs
-constexpr uint32_t kRange = 4096;         // contraction elements of a gradient's tile
+constexpr uint32_t kPieceCells = 1u << 25;  // logits of a piece
+constexpr uint32_t kSkew = 128;            // elements past a row: rows a power of two apart meet in few memory channels
+constexpr uint32_t kMostPiece = 1u << 17;   // classes of one
+constexpr uint32_t kMostRange = 4096;       // contraction elements of a gradient's tile
 
 uint32_t up_to(uint64_t n, uint32_t m) { return (uint32_t)((n + m - 1) / m * m); }
 uint64_t padded(uint64_t bytes) { return (bytes + 255) & ~(uint64_t)255; }
@@ -611,9 +679,10 @@ struct Carve {
 
 // What a call keeps in its workspace. 16-bit planes; pairs have two.
 struct HeadSpace {
-    uint32_t width8, rows_ld, piece, pieces, splits_x, splits_w, range_x, range_w, parts_ld;
-    uint64_t planes;
-    uint16_t *x, *w, *xt, *wt, *g, *gt;
+    uint32_t width8, rows_ld, g_ld, piece, pieces, tall, splits_x, splits_w, range_x, range_w, parts_ld;
+    uint64_t planes, g_plane;
+    uint16_t *x, *x_even, *w, *g;
+    uint32_t* live;
     float *stats, *of, *parts_x, *parts_w, *amax;
     int* row_exp;
     dev::HeadScales* scales;
@@ -636,11 +705,20 @@ struct HeadSpace {
         }
         const uint32_t all = up_to(classes, kHeadM);
         piece = rows_ld ? up_to(kPieceCells / rows_ld, kHeadM) : kHeadM;
-        piece = piece < kRange ? kRange : piece > 32 * kRange ? 32 * kRange : piece;
+        piece = piece < kMostRange ? kMostRange : piece > kMostPiece ? kMostPiece : piece;
         pieces = (all + piece - 1) / piece;
         piece = up_to((all + pieces - 1) / pieces, kHeadM);
-        auto cut = [](uint32_t k, uint32_t& splits, uint32_t& range) {
-            splits = (k + kRange / 2) / kRange;
+        g_ld = piece + kSkew;
+        // The gradients' contractions, over a piece's classes and over all rows, are cut so that
+        // their tiles are about as many as CUs, or of kMostRange elements where they are more.
+        tall = width > 128 ? 256 : 128;
+        const uint64_t across = (width + tall - 1) / tall;
+        const uint64_t work = across * (rows_ld / dev::kHeadN) * piece + across * (piece / dev::kHeadN) * rows_ld;
+        const uint32_t each = up_to((work + kCus - 1) / kCus, 64);
+        auto cut = [&](uint32_t k, uint32_t& splits, uint32_t& range) {
+            uint32_t most = each < kMostRange ? each : kMostRange;
+            if (most < 256) most = 256;
+            splits = (k + most / 2) / most;
             if (!splits) splits = 1;
             range = up_to((k + splits - 1) / splits, dev::kHeadK);
             if (k) splits = (k + range - 1) / range;
@@ -648,10 +726,10 @@ struct HeadSpace {
         cut(piece, splits_x, range_x);
         cut(rows_ld, splits_w, range_w);
         parts_ld = up_to(width, 4);
-        xt = c.take<uint16_t>(planes * width * rows_ld);
-        wt = c.take<uint16_t>(planes * width * piece);
-        g = c.take<uint16_t>(planes * rows_ld * piece);
-        gt = c.take<uint16_t>(planes * rows_ld * piece);
+        x_even = c.take<uint16_t>(planes > 1 ? planes * rows * width8 : 0);
+        live = c.take<uint32_t>(rows_ld / 32);
+        g_plane = (uint64_t)rows_ld * g_ld;
+        g = c.take<uint16_t>(planes * g_plane);
         parts_x = c.take<float>(splits_x > 1 || pieces > 1 ? (uint64_t)splits_x * rows * parts_ld : 0);
         parts_w = c.take<float>(splits_w > 1 ? (uint64_t)splits_w * piece * parts_ld : 0);
         bytes = c.used;
@@ -665,18 +743,6 @@ bool fits(const void* p, uint64_t ld, uint32_t cols, uint32_t type) {
 
 dim3 copy_grid(uint32_t cols, uint32_t rows) { return dim3((cols + 1023) / 1024, rows < 65535 ? rows : 65535); }
 
-// x or W as an operand: where it lies, or its copy.
-template <class T, class H>
-dev::HeadOperand operand_of(hipStream_t st, const void* p, uint64_t ld, uint32_t rows, uint32_t cols, uint32_t type,
-                            const HeadSpace& s, uint16_t* copy, uint32_t which, const dev::HeadScales* scales) {
-    if (fits(p, ld, cols, type)) return {p, 0, (uint32_t)ld, rows};
-    const uint64_t plane = (uint64_t)rows * s.width8;
-    const dev::CopyArgs a{p,      ld,   rows,    cols, s.width8, s.width8, copy, plane, scales, which ? nullptr : s.row_exp,
-                          which, nullptr, 0};
-    hipLaunchKernelGGL((dev::head_copy_kernel<T, H>), copy_grid(s.width8, rows), dim3(256), 0, st, a);
-    return {copy, plane, s.width8, rows};
-}
-
 template <class T>
 struct HeadType {
     typedef T H;
@@ -686,25 +752,46 @@ struct HeadType<float> {
     typedef _Float16 H;
 };
 
-// The scales of fp32 operands and, backwards, of 16-bit floats' gradients.
-template <class T>
-const dev::HeadScales* scales_of(hipStream_t st, const void* x, uint64_t x_ld, const void* w, uint64_t w_ld,
-                                 uint32_t rows, uint32_t classes, uint32_t width, const float* dloss,
-                                 const float* dentropy, const int32_t* targets, const HeadSpace& s) {
+// x and W as the products' operands, and their scales.
+struct HeadInputs {
+    dev::HeadOperand x, w;
+    dev::HeadOperand x_even;  // x at one scale
+    const dev::HeadScales* scales;
+};
+template <class T, class P>
+HeadInputs prepare(hipStream_t st, const P& p, const HeadSpace& s, const float* dloss, const float* dentropy,
+                   bool even) {
+    typedef typename HeadType<T>::H H;
     const bool pairs = std::is_same<T, float>::value, g = dloss && !std::is_same<T, __bf16>::value;
-    if (!pairs && !g) return nullptr;
-    float* const parts = s.amax;
-    const dev::AmaxArgs ax{static_cast<const float*>(pairs ? x : nullptr), x_ld, pairs ? rows : 0, width, nullptr, 0,
-                           targets, classes, parts, s.row_exp};
-    const dev::AmaxArgs aw{static_cast<const float*>(pairs ? w : nullptr), w_ld, pairs ? classes : 0, width, nullptr, 0,
-                           nullptr, 0, parts + dev::kAmaxParts, nullptr};
-    // |p (log p + H)| is at most 1/e + H, and H at most log(classes)
-    const dev::AmaxArgs ag{dloss,   0,       g ? rows : 0, 0, dentropy, __builtin_logf((float)classes) + 1.0f, targets,
-                           classes, parts + 2 * dev::kAmaxParts, nullptr};
-    hipLaunchKernelGGL(dev::head_amax_kernel, dim3(dev::kAmaxParts, 3), dim3(256), 0, st, ax, aw, ag);
-    hipLaunchKernelGGL(dev::head_scales_kernel, dim3(1), dim3(256), 0, st, pairs ? parts : nullptr,
-                       pairs ? parts + dev::kAmaxParts : nullptr, g ? parts + 2 * dev::kAmaxParts : nullptr, s.scales);
-    return s.scales;
+    HeadInputs in{};
+    in.x = {p.x, 0, (uint32_t)p.x_ld};
+    in.w = {p.w, 0, (uint32_t)p.w_ld};
+    dev::PrepareArgs ax{p.x, p.x_ld, p.rows, p.width, nullptr, nullptr, s.width8, (uint64_t)p.rows * s.width8, s.row_exp};
+    dev::PrepareArgs aw{p.w, p.w_ld, p.classes, p.width, nullptr, nullptr, s.width8, (uint64_t)p.classes * s.width8,
+                        nullptr};
+    if (!fits(p.x, p.x_ld, p.width, p.type)) ax.to = s.x, in.x = {s.x, ax.plane, s.width8};
+    if (!fits(p.w, p.w_ld, p.width, p.type)) aw.to = s.w, in.w = {s.w, aw.plane, s.width8};
+    in.x_even = in.x;
+    if (pairs && even) ax.to_even = s.x_even, in.x_even.base = s.x_even;
+    dev::PrepareScales scales{{nullptr, nullptr, nullptr}, nullptr};
+    if (pairs || g) {
+        float* const parts = s.amax;
+        const dev::AmaxArgs mx{reinterpret_cast<const float*>(pairs ? p.x : nullptr), p.x_ld, pairs ? p.rows : 0,
+                               p.width, nullptr, 0, p.targets, p.classes, parts, s.row_exp};
+        const dev::AmaxArgs mw{reinterpret_cast<const float*>(pairs ? p.w : nullptr), p.w_ld, pairs ? p.classes : 0,
+                               p.width, nullptr, 0, nullptr, 0, parts + dev::kAmaxParts, nullptr};
+        // |p (log p + H)| is at most 1/e + H, and H at most log(classes)
+        const dev::AmaxArgs mg{dloss, 0, g ? p.rows : 0, 0, dentropy, __builtin_logf((float)p.classes) + 1.0f,
+                               p.targets, p.classes, parts + 2 * dev::kAmaxParts, nullptr};
+        hipLaunchKernelGGL(dev::head_amax_kernel, dim3(dev::kAmaxParts, 3), dim3(256), 0, st, mx, mw, mg);
+        if (pairs) scales.parts[0] = parts, scales.parts[1] = parts + dev::kAmaxParts;
+        if (g) scales.parts[2] = parts + 2 * dev::kAmaxParts;
+        scales.out = s.scales;
+        in.scales = s.scales;
+    }
+    if (ax.to || aw.to || scales.out)
+        hipLaunchKernelGGL((dev::head_prepare_kernel<T, H>), dim3(4 * kCus, 2), dim3(256), 0, st, ax, aw, scales);
+    return in;
 }
 
 template <class T>
@@ -713,15 +800,15 @@ int cross_entropy(hipStream_t st, const mg_cross_entropy_args& p) {
     constexpr bool kPairs = sizeof(T) == 4;
     const HeadSpace s(p.workspace, p.rows, p.classes, p.width, p.type, false);
     dev::HeadArgs a{};
-    a.scales = scales_of<T>(st, p.x, p.x_ld, p.w, p.w_ld, p.rows, p.classes, p.width, nullptr, nullptr, nullptr, s);
+    const HeadInputs in = prepare<T>(st, p, s, nullptr, nullptr, false);
+    a.scales = in.scales;
     dev::HeadProduct& m = a.p[0];
-    m.a = operand_of<T, H>(st, p.w, p.w_ld, p.classes, p.width, p.type, s, s.w, 1, a.scales);
-    m.b = operand_of<T, H>(st, p.x, p.x_ld, p.rows, p.width, p.type, s, s.x, 0, a.scales);
-    m.k = m.range = s.width8, m.splits = 1;
+    m.a = in.w, m.b = in.x;
+    m.k = m.range = s.width8, m.splits = 1, m.m = p.classes, m.n = p.rows;
     m.tiles_m = up_to(p.classes, kHeadM) / kHeadM, m.tiles_n = s.rows_ld / dev::kHeadN;
     a.tiles = m.tiles_m * m.tiles_n;
     a.rows = p.rows, a.classes = p.classes, a.targets = p.targets, a.row_exp = s.row_exp;
-    a.stats = s.stats, a.of = s.of, a.rows_ld = s.rows_ld;
+    a.stats = s.stats, a.of = s.of, a.rows_ld = s.rows_ld, a.want_entropy = p.entropy != nullptr;
     hipLaunchKernelGGL((dev::head_kernel<H, dev::kStats, 4, kPairs>), dim3(a.tiles), dim3(512), 0, st, a);
     MG_HIP(hipGetLastError(), "cross entropy launch");
     const uint32_t blocks = (p.rows + 3) / 4;
@@ -743,43 +830,31 @@ int cross_entropy_backward(hipStream_t st, const mg_cross_entropy_backward_args&
     }
     const HeadSpace s(p.workspace, p.rows, p.classes, p.width, p.type, true);
     dev::HeadArgs a{};
-    a.scales = scales_of<T>(st, p.x, p.x_ld, p.w, p.w_ld, p.rows, p.classes, p.width, p.dloss, p.dentropy, p.targets, s);
-    const dev::HeadOperand w = operand_of<T, H>(st, p.w, p.w_ld, p.classes, p.width, p.type, s, s.w, 1, a.scales);
-    const dev::HeadOperand x = operand_of<T, H>(st, p.x, p.x_ld, p.rows, p.width, p.type, s, s.x, 0, a.scales);
+    const HeadInputs in = prepare<T>(st, p, s, p.dloss, p.dentropy, p.dw != nullptr);
+    a.scales = in.scales;
     a.rows = p.rows, a.classes = p.classes, a.targets = p.targets, a.row_exp = s.row_exp;
     a.lse = p.lse, a.dloss = p.dloss, a.entropy = p.entropy, a.dentropy = p.dentropy;
-    a.rows_ld = s.rows_ld, a.g = s.g, a.gt = s.gt, a.g_ld = s.piece, a.g_plane = (uint64_t)s.rows_ld * s.piece;
-    const uint64_t xt_plane = (uint64_t)p.width * s.rows_ld, wt_plane = (uint64_t)p.width * s.piece;
-    auto turn = [&](const void* from, uint64_t ld, uint32_t rows, uint32_t fill, uint32_t to_ld, uint16_t* to,
-                    uint64_t plane, uint32_t which) {
-        const dev::CopyArgs c{from, ld, rows,     p.width, fill, to_ld, to, plane, a.scales, nullptr,
-                              which, which ? nullptr : p.targets, p.classes};
-        const uint32_t down = (fill + 63) / 64;
-        hipLaunchKernelGGL((dev::head_turn_kernel<T, H>), dim3((p.width + 63) / 64, down < 4096 ? down : 4096),
-                           dim3(256), 0, st, c);
-    };
-    if (p.dw) turn(p.x, p.x_ld, p.rows, s.rows_ld, s.rows_ld, s.xt, xt_plane, 0);
+    a.rows_ld = s.rows_ld, a.g = s.g, a.g_ld = s.g_ld, a.g_plane = s.g_plane, a.live = s.live;
     const bool parts_x = s.splits_x > 1 || s.pieces > 1, parts_w = s.splits_w > 1;
-    const uint32_t tall = p.width > 128 ? 256 : 128, tiles_m = (p.width + tall - 1) / tall;
+    const uint32_t tiles_m = (p.width + s.tall - 1) / s.tall;
     for (uint32_t first = 0; first < p.classes; first += s.piece) {
         const uint32_t here = p.classes - first < s.piece ? p.classes - first : s.piece, fill = up_to(here, kHeadM);
-        const T* const w0 = static_cast<const T*>(p.w) + (uint64_t)first * p.w_ld;
-        if (p.dx) turn(w0, p.w_ld, here, fill, s.piece, s.wt, wt_plane, 1);
         dev::HeadProduct& m = a.p[0];
         m = {};
-        m.a = w, m.b = x;
-        m.a.base = static_cast<const H*>(w.base) + (uint64_t)first * w.ld, m.a.rows = here;
-        m.k = m.range = s.width8, m.splits = 1;
+        m.a = in.w, m.b = in.x;
+        m.a.base = static_cast<const H*>(in.w.base) + (uint64_t)first * in.w.ld;
+        m.k = m.range = s.width8, m.splits = 1, m.m = here, m.n = p.rows;
         m.tiles_m = fill / kHeadM, m.tiles_n = s.rows_ld / dev::kHeadN;
         a.tiles = m.tiles_m * m.tiles_n, a.first = first;
         hipLaunchKernelGGL((dev::head_kernel<H, dev::kLogitGrad, 4, kPairs>), dim3(a.tiles), dim3(512), 0, st, a);
         MG_HIP(hipGetLastError(), "cross entropy logits launch");
+        const dev::HeadOperand m_of_w = m.a;
         uint32_t n = 0, tiles = 0;
         if (p.dx) {
             dev::HeadProduct& q = a.p[n++];
             q = {};
-            q.a = {s.wt, wt_plane, s.piece, p.width}, q.b = {s.g, a.g_plane, s.piece, p.rows};
-            q.k = fill, q.range = s.range_x, q.splits = (fill + s.range_x - 1) / s.range_x;
+            q.a = m_of_w, q.b = {s.g, s.g_plane, s.g_ld}, q.m = p.width, q.n = p.rows;
+            q.k = here, q.range = s.range_x, q.splits = (here + s.range_x - 1) / s.range_x;
             q.tiles_m = tiles_m, q.tiles_n = s.rows_ld / dev::kHeadN;
             q.out = p.dx, q.out_ld = p.dx_ld, q.parts = parts_x ? s.parts_x : nullptr, q.parts_ld = s.parts_ld;
             q.add = first != 0, q.which = 0;
@@ -788,8 +863,8 @@ int cross_entropy_backward(hipStream_t st, const mg_cross_entropy_backward_args&
         if (p.dw) {
             dev::HeadProduct& q = a.p[n++];
             q = {};
-            q.a = {s.xt, xt_plane, s.rows_ld, p.width}, q.b = {s.gt, a.g_plane, s.rows_ld, here};
-            q.k = s.rows_ld, q.range = s.range_w, q.splits = s.splits_w;
+            q.a = in.x_even, q.b = {s.g, s.g_plane, s.g_ld}, q.m = p.width, q.n = here, q.live = s.live;
+            q.k = p.rows, q.range = s.range_w, q.splits = (p.rows + s.range_w - 1) / s.range_w;
             q.tiles_m = tiles_m, q.tiles_n = fill / dev::kHeadN;
             q.out = static_cast<T*>(p.dw) + (uint64_t)first * p.dw_ld, q.out_ld = p.dw_ld;
             q.parts = parts_w ? s.parts_w : nullptr, q.parts_ld = s.parts_ld, q.which = 1;
@@ -797,14 +872,14 @@ int cross_entropy_backward(hipStream_t st, const mg_cross_entropy_backward_args&
             if (n == 1) a.tiles = more;
             tiles += more;
         }
-        if (tall == 128)
+        if (s.tall == 128)
             hipLaunchKernelGGL((dev::head_kernel<H, dev::kGrad, 2, kPairs>), dim3(tiles), dim3(512), 0, st, a);
         else
             hipLaunchKernelGGL((dev::head_kernel<H, dev::kGrad, 4, kPairs>), dim3(tiles), dim3(512), 0, st, a);
         MG_HIP(hipGetLastError(), "cross entropy gradients launch");
         if (p.dw && parts_w)
             hipLaunchKernelGGL(dev::head_sum_kernel<T>, copy_grid(p.width, here), dim3(256), 0, st, s.parts_w,
-                               s.splits_w, here, p.width, s.parts_ld,
+                               a.p[n - 1].splits, here, p.width, s.parts_ld,
                                static_cast<T*>(p.dw) + (uint64_t)first * p.dw_ld, p.dw_ld, a.scales, 1u);
     }
     if (p.dx && parts_x)
