@@ -737,9 +737,9 @@ int mg_selective_scan_backward(void* stream, const mg_selective_scan_backward_ar
  * [0, classes) leaves its row out: loss 0, and no gradients; lse and entropy are
  * written all the same. Row r of x begins r x_ld elements after it, class c of w c w_ld (ld 0: width).
  * rows (which may be 0) and classes are at most 2^20, width at most 65536. Products of
- * 16-bit types are exact, those of fp32 go through the matrix units as pairs of
- * binary16 halves at a power of two for each array: 22 bits, fewer for elements under 2^-17 of
- * the array's largest. Sums are fp32. */
+ * 16-bit types are exact, those of fp32 are too in small calls; in large ones they go
+ * through the matrix units as pairs of binary16 halves at a power of two for each row of x
+ * and for all of w: 22 bits, fewer for elements under 2^-17 of its largest. Sums are fp32. */
 typedef struct mg_cross_entropy_args {
     const void* x;          /* [rows][width] */
     const void* w;          /* [classes][width] */
@@ -762,8 +762,9 @@ int mg_cross_entropy(void* stream, const mg_cross_entropy_args* args);
 /* Backward of mg_cross_entropy for the gradients dloss of loss and dentropy of
  * entropy: with p = exp(s - lse), g = dloss (p - [target]) - dentropy p (log p + entropy),
  * dx = g w, dw = g' x. lse, and where there is a dentropy entropy, are the forward's. The
- * logits are computed again, a piece of the classes at a time. g is rounded to type for
- * the two products (binary16 at a power of two, fp32 as pairs); their sums are fp32, rounded once.
+ * logits are computed again, in large calls a piece of the classes at a time, whose g is
+ * rounded to type for the two products (binary16 at a power of two, fp32 as pairs at one for
+ * each array); in small ones it stays fp32. Their sums are fp32, rounded once.
  * A row that is left out adds nothing, whatever it holds. Without rows dw is 0. */
 typedef struct mg_cross_entropy_backward_args {
     const void* x;

@@ -49,13 +49,13 @@ struct HeadScales {
     float x_back, w_back, g_back;
 };
 
-// Rows of 16-bit elements, `ld` apart: a high plane, and where values are pairs a low one
-// `plane` elements after it.
+// Rows of 16-bit elements, `ld` of them apart. Pairs lie in blocks of 16 high halves and the 16
+// low ones: element c of a row at pair_place(c), its low half 16 further.
 struct HeadOperand {
     const void* base;
-    uint64_t plane;
     uint32_t ld;
 };
+__host__ __device__ __forceinline__ uint32_t pair_place(uint32_t c) { return (c & ~15u) * 2 + (c & 15); }
 
 enum { kStats = 0, kLogitGrad = 1, kGrad = 2 };
 
@@ -91,13 +91,12 @@ struct HeadArgs {
     const float* dloss;
     const float* entropy;
     const float* dentropy;
-    void* g;  // [rows][g_ld], planes g_plane apart
+    void* g;  // the piece's, g_ld between rows
     uint32_t* live;
     uint32_t g_ld;
-    uint64_t g_plane;
 };
 
-constexpr int kHeadK = 32;     // contraction elements of a stage
+constexpr int kHeadK = 32;     // contraction elements of a stage, or 16 pairs
 constexpr int kHeadRing = 4;   // stages in LDS
 constexpr int kHeadN = 256;    // columns of a tile
 constexpr uint32_t kNowhere = 0x80000000u;  // an offset past every operand's end: reads 0
@@ -132,50 +131,52 @@ struct RowStats {
 };
 
 // One operand's part in the main loop: SIDE rows of a tile, of which a stage holds 32
-// contraction elements in LDS. Rows go from memory straight there, a wave's 64 lanes in order, 16
-// bytes each; where they come from is each lane's own choice, which keeps reads off one bank.
+// contraction elements (16 pairs) in LDS. Rows go from memory straight there, a wave's 64 lanes in
+// order, 16 bytes each; where they come from is each lane's own choice, which keeps reads off one
+// bank.
 //
 // Not TURNED: the contraction runs along a row in memory, and a stage is 64 bytes of every row. The
 // places of a row's four 16 bytes are exchanged by bits 1 and 2 of the row: a read of eight rows'
 // fragments (lane l holds row l % 32 and eight elements of 16, by l / 32) then meets no bank twice.
 //
-// TURNED: it runs from row to row, and a stage is 32 rows of SIDE elements. Reads of four
-// elements by 16 lanes that hold each other's columns (ds_read_b64_tr_b16: of 4 rows x 16 columns
-// a lane gets a column) make the same fragments; the places of 32 bytes are exchanged by the
-// row's last two bits, so that the four rows lie in different banks.
-template <class H, int SIDE, bool TURNED>
+// TURNED: it runs from row to row, and a stage is 32 rows of SIDE elements, or 16 of SIDE pairs.
+// Reads of four elements by 16 lanes that hold each other's columns (ds_read_b64_tr_b16: of 4 rows
+// x 16 columns a lane gets a column) make the same fragments; the places of 32 bytes are exchanged
+// by the row's last two bits, so that the four rows lie in different banks.
+template <class H, int SIDE, bool TURNED, bool PAIRS>
 struct HeadSide {
     typedef typename Halves<H>::x8 x8;
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     static constexpr int L = SIDE / 128;  // loads of a wave and stage
-    static constexpr int kBytes = SIDE * 64;
-    const H* base[2];
+    static constexpr int kBytes = SIDE * 64, kWide = PAIRS ? 2 : 1;
+    static constexpr int kRow = SIDE * 2 * kWide;  // bytes of a TURNED row
+    const H* base;
     uint32_t ld, off[L], row[L];
 
     // `from`: the tile's first row (or column) of `rows`
     __device__ __forceinline__ HeadSide(const HeadOperand& o, uint32_t from, uint32_t rows, int wave, int lane) {
         ld = o.ld;
-        base[0] = static_cast<const H*>(o.base) + (TURNED ? from : (uint64_t)from * ld);
-        base[1] = base[0] + o.plane;
+        base = static_cast<const H*>(o.base) + (TURNED ? (uint64_t)from * kWide : (uint64_t)from * ld);
         const uint32_t have = rows > from ? rows - from : 0;
 #pragma unroll
         for (int c = 0; c < L; ++c) {
             if constexpr (TURNED) {
-                constexpr uint32_t kLanes = SIDE / 8;  // of a row
+                constexpr uint32_t kLanes = kRow / 16;  // of a row
                 row[c] = (wave * L + c) * (64 / kLanes) + lane / kLanes;
-                const uint32_t at = lane % kLanes, col = (((at >> 1 ^ (row[c] & 3)) << 1) + (at & 1)) * 8;
-                off[c] = col < have ? (row[c] * ld + col) * 2 : kNowhere;
+                const uint32_t at = lane % kLanes, place = (((at >> 1 ^ (row[c] & 3)) << 1) + (at & 1)) * 8;
+                const uint32_t col = PAIRS ? (place >> 5 << 4) + (place & 15) : place;
+                off[c] = col < have ? (row[c] * ld + place) * 2 : kNowhere;
             } else {
-                const uint32_t r = (wave * L + c) * 16 + (lane >> 2);
-                row[c] = ((lane & 3) ^ (lane >> 3 & 3)) * 8;  // the first of its elements
-                off[c] = r < have ? (r * ld + row[c]) * 2 : kNowhere;
+                const uint32_t r = (wave * L + c) * 16 + (lane >> 2), place = ((lane & 3) ^ (lane >> 3 & 3)) * 8;
+                row[c] = PAIRS ? place & 15 : place;  // the first of its elements
+                off[c] = r < have ? (r * ld + place) * 2 : kNowhere;
             }
         }
     }
     // The stage of contraction elements k ..., up to `to`.
-    __device__ __forceinline__ void load(char* at, int wave, uint32_t k, uint32_t to, bool low, uint32_t live) const {
+    __device__ __forceinline__ void load(char* at, int wave, uint32_t k, uint32_t to, uint32_t live) const {
         // a row of W or X may lie anywhere, so its stage has an address of its own
-        const H* const p = base[low] + (TURNED ? (uint64_t)k * ld : (uint64_t)k);
+        const H* const p = base + (TURNED ? (uint64_t)k * ld : (uint64_t)k * kWide);
         const __amdgpu_buffer_rsrc_t r =
             __builtin_amdgcn_make_buffer_rsrc(const_cast<H*>(p), (short)0, 0x7fffffff, 0x00020000);
 #pragma unroll
@@ -187,13 +188,15 @@ struct HeadSide {
                 (int)(in ? off[c] : kNowhere), 0, 0, 0);
         }
     }
-    // the fragment of rows 32 b ... of the tile and the stage's elements 16 h ...
+    // the fragment of rows 32 b ... of the tile: the stage's elements 16 h ..., or of its pairs
+    // the high (h = 0) or the low halves
     static __device__ __forceinline__ x8 read(const char* at, int b, int h, int lane) {
         if constexpr (TURNED) {
-            const int k = 16 * h + 8 * (lane >> 5) + (lane >> 2 & 3), chunk = 2 * b + (lane >> 4 & 1);
+            const int k = (PAIRS ? 0 : 16 * h) + 8 * (lane >> 5) + (lane >> 2 & 3);
+            const int block = 2 * b + (lane >> 4 & 1), chunk = PAIRS ? 2 * block + h : block;
             auto four = [&](int more) {
                 const int r = k + more;  // its last two bits are k's
-                const char* const p = at + r * (SIDE * 2) + ((chunk ^ (r & 3)) << 5) + ((lane & 3) << 3);
+                const char* const p = at + r * kRow + ((chunk ^ (r & 3)) << 5) + ((lane & 3) << 3);
                 return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
             };
             const s16x4 lo = four(0), hi = four(4);
@@ -208,33 +211,29 @@ struct HeadSide {
 
 // One tile of MI x 64 by 256. Eight waves, two along a and four along b, MI x 2 tiles of 32 x 32
 // each. The ring holds four stages; the waves meet once a stage, when the next has arrived,
-// and read the next one's fragments under this one's products.
+// and read the next one's fragments under this one's products: two of 16 elements, or of pairs
+// low high, high low and high high.
 template <class H, int MI, bool PAIRS, bool AT, bool BT>
 __device__ __forceinline__ void head_product(const HeadProduct& p, uint32_t tm, uint32_t tn, uint32_t split, char* lds,
                                              f32x16 (&acc)[MI][2]) {
     using X = Halves<H>;
     typedef typename X::x8 x8;
-    using A = HeadSide<H, MI * 64, AT>;
-    using B = HeadSide<H, kHeadN, BT>;
-    constexpr int kStage = A::kBytes + B::kBytes, L = A::L + B::L;
+    using A = HeadSide<H, MI * 64, AT, PAIRS>;
+    using B = HeadSide<H, kHeadN, BT, PAIRS>;
+    constexpr int kStage = A::kBytes + B::kBytes, L = A::L + B::L, K = PAIRS ? 16 : kHeadK;
     const uint32_t from = split * p.range, to = p.k - from < p.range ? p.k : from + p.range;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1;
     const A a(p.a, tm * (MI * 64), p.m, wave, lane);
     const B b(p.b, tn * kHeadN, p.n, wave, lane);
     uint32_t k = from;
-    int seg = 0;
-    const uint32_t each = (to - from + kHeadK - 1) / kHeadK;
-    const uint32_t stages = (each * (PAIRS ? 3 : 1) + 1) & ~1u;  // the last may be empty
+    const uint32_t stages = ((to - from + K - 1) / K + 1) & ~1u;  // the last may be empty
     const uint32_t* const live = AT ? p.live : nullptr;
     auto load = [&](uint32_t slot) {
         char* const at = lds + slot * kStage;
-        // pairs: low high, high low, high high; past the last an empty stage
-        const uint32_t end = PAIRS && seg > 2 ? 0 : to;
-        const uint32_t bits = live && k < end ? live[k / kHeadK] : ~0u;
-        a.load(at, wave, k, end, PAIRS && seg == 0, bits);
-        b.load(at + A::kBytes, wave, k, end, PAIRS && seg == 1, ~0u);
-        k += kHeadK;
-        if (PAIRS && k >= to) k = from, ++seg;
+        const uint32_t bits = live && k < to ? live[k / 32] >> (k & 31) : ~0u;
+        a.load(at, wave, k, to, bits);
+        b.load(at + A::kBytes, wave, k, to, ~0u);
+        k += K;
     };
     x8 fa[2][2][MI], fb[2][2][2];
     auto read = [&](int set, uint32_t slot) {
@@ -263,20 +262,22 @@ __device__ __forceinline__ void head_product(const HeadProduct& p, uint32_t tm, 
             asm volatile("" ::: "memory");
             read(u ^ 1, (slot + 1) & (kHeadRing - 1));
             load(slot);
+            constexpr int kTerms = PAIRS ? 3 : 2;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < kTerms; ++h) {
+                const int ha = PAIRS ? h == 0 : h, hb = PAIRS ? h == 1 : h;
 #pragma unroll
                 for (int i = 0; i < MI; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) acc[i][j] = X::mfma(fa[u][h][i], fb[u][h][j], acc[i][j]);
-            constexpr int kReads = 2 * (MI * (AT ? 2 : 1) + 2 * (BT ? 2 : 1)), kProducts = 4 * MI;
+                    for (int j = 0; j < 2; ++j) acc[i][j] = X::mfma(fa[u][ha][i], fb[u][hb][j], acc[i][j]);
+            }
+            constexpr int kReads = 2 * (MI * (AT ? 2 : 1) + 2 * (BT ? 2 : 1)), kProducts = 2 * MI * kTerms;
 #pragma unroll
             for (int q = 0; q < kProducts; ++q) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix
-                if ((q + 1) * kReads / kProducts - q * kReads / kProducts == 1)
-                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
-                else
-                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                const int n = (q + 1) * kReads / kProducts - q * kReads / kProducts;
+                if (n == 1) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
+                if (n == 2) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -464,9 +465,9 @@ __global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
                                 hi[q] = h, lo[q] = l;
                             }
                         }
-                        H* const g = static_cast<H*>(args.g) + (uint64_t)n * args.g_ld + c;
+                        H* const g = static_cast<H*>(args.g) + (uint64_t)n * args.g_ld + (PAIRS ? pair_place(c) : c);
                         *reinterpret_cast<x4*>(g) = hi;
-                        if constexpr (PAIRS) *reinterpret_cast<x4*>(g + args.g_plane) = lo;
+                        if constexpr (PAIRS) *reinterpret_cast<x4*>(g + 16) = lo;
                     }
             }
         }
@@ -529,7 +530,7 @@ struct AmaxArgs {
     float* parts;
     int* row_exp;
 };
-constexpr uint32_t kAmaxParts = 256;
+constexpr uint32_t kAmaxParts = 1024;
 __global__ void __launch_bounds__(256) head_amax_kernel(const AmaxArgs a0, const AmaxArgs a1, const AmaxArgs a2) {
     __shared__ float red[4];
     const AmaxArgs a = blockIdx.y == 0 ? a0 : blockIdx.y == 1 ? a1 : a2;
@@ -560,8 +561,8 @@ __global__ void __launch_bounds__(256) head_amax_kernel(const AmaxArgs a0, const
         a.parts[blockIdx.x] = __builtin_fmaxf(__builtin_fmaxf(red[0], red[1]), __builtin_fmaxf(red[2], red[3]));
 }
 
-// 16-bit copies of x (job 0) and W (job 1), [rows][ld] with zeros past their columns, of what
-// cannot be read as it lies. fp32 becomes pairs: W at the scale of all of it, x at each row's own
+// 16-bit copies of x (job 0) and W (job 1), rows of `wide` elements with zeros past their
+// columns, of what cannot be read as it lies. fp32 becomes pairs: W at the scale of all of it, x at each row's own
 // for the logits and at that of all rows with a target for the gradient of W.
 struct PrepareArgs {
     const void* from;
@@ -569,8 +570,7 @@ struct PrepareArgs {
     uint32_t rows, cols;
     void* to;  // nullable
     void* to_even;  // of x, nullable
-    uint32_t ld;
-    uint64_t plane;
+    uint32_t wide;
     const int* row_exp;  // of x
 };
 struct PrepareScales {
@@ -590,8 +590,10 @@ __global__ void __launch_bounds__(256) head_prepare_kernel(const PrepareArgs a0,
     if (s.out) {
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
-            const float v = group_max<64>(s.parts[k] ? s.parts[k][threadIdx.x] : 0.0f);
-            if (!lane) red[k][wave] = v;
+            f32x4 v = {};
+            if (s.parts[k]) v = *reinterpret_cast<const f32x4*>(s.parts[k] + 4 * threadIdx.x);
+            const float most = group_max<64>(__builtin_fmaxf(__builtin_fmaxf(v[0], v[1]), __builtin_fmaxf(v[2], v[3])));
+            if (!lane) red[k][wave] = most;
         }
         __syncthreads();
 #pragma unroll
@@ -604,7 +606,7 @@ __global__ void __launch_bounds__(256) head_prepare_kernel(const PrepareArgs a0,
             *s.out = HeadScales{scale[0], scale[1], scale[2], back[0], back[1], back[2]};
     }
     if (!a.to) return;
-    const uint32_t across = a.ld / 4;
+    const uint32_t across = a.wide / 4;
     const uint64_t all = (uint64_t)across * a.rows;
     for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
         const uint32_t r = (uint32_t)(i / across), c = (uint32_t)(i - (uint64_t)r * across) * 4;
@@ -612,7 +614,7 @@ __global__ void __launch_bounds__(256) head_prepare_kernel(const PrepareArgs a0,
         T v[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) v[q] = c + q < a.cols ? from[q] : (T)0.0f;
-        const uint64_t at = (uint64_t)r * a.ld + c;
+        const uint64_t at = kPairs ? (uint64_t)r * a.wide * 2 + pair_place(c) : (uint64_t)r * a.wide + c;
         auto put = [&](void* to, float by) {
             x4 hi, lo;
 #pragma unroll
@@ -626,7 +628,7 @@ __global__ void __launch_bounds__(256) head_prepare_kernel(const PrepareArgs a0,
                 }
             }
             *reinterpret_cast<x4*>(static_cast<H*>(to) + at) = hi;
-            if constexpr (kPairs) *reinterpret_cast<x4*>(static_cast<H*>(to) + a.plane + at) = lo;
+            if constexpr (kPairs) *reinterpret_cast<x4*>(static_cast<H*>(to) + at + 16) = lo;
         };
         put(a.to, !kPairs ? 1.0f : job ? scale[1] : ldexpf(1.0f, a.row_exp[r]));
         if (kPairs && a.to_even) put(a.to_even, scale[0]);
@@ -651,16 +653,238 @@ __global__ void __launch_bounds__(256) head_sum_kernel(const float* parts, uint3
     }
 }
 
+// ---- small products ----------------------------------------------------------------------------------
+//
+// Where the tiles above would be few, all of it is latency: of launches that scale and copy, and of a
+// tile's 256 x 256. These take 32 x 32 a workgroup, straight from memory as fp32 whatever the type, on
+// the fp32 matrix instruction, its four waves a quarter of the contraction each.
+
+// Elements k .. k + 3 of a row; those from `end` on are 0, and not read, unless ALL are before it.
+template <bool ALL, class T>
+__device__ __forceinline__ f32x4 four_of(const T* row, uint32_t k, uint32_t end) {
+    f32x4 v = {};
+    if constexpr (ALL) {
+        typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+        const vec w = *reinterpret_cast<const vec*>(row + k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (float)w[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (k + e < end) v[e] = (float)row[k + e];
+    }
+    return v;
+}
+// The same of a column, ld apart.
+template <bool ALL, class T>
+__device__ __forceinline__ f32x4 four_down(const T* column, uint64_t ld, uint32_t k, uint32_t end) {
+    f32x4 v = {};
+    column += k * ld;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (ALL || k + e < end) v[e] = (float)column[e * ld];
+    return v;
+}
+
+// acc += a b over the wave's share of k0 .. k1, a quarter in steps of 8: instruction e of a
+// step takes element 8 j + e from lanes 0 to 31 and 8 j + 4 + e from the others. Four steps' loads go
+// ahead of their products.
+template <class FA, class FB>
+__device__ __forceinline__ f32x16 small_product(uint32_t k0, uint32_t k1, FA&& a, FB&& b) {
+    f32x16 acc = {};
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = threadIdx.x >> 5 & 1;
+    const uint32_t each = (k1 - k0 + 31) / 32 * 8, from = k0 + wave * each, to = from + each < k1 ? from + each : k1;
+    uint32_t k = from;
+    for (; k + 32 <= to; k += 32) {
+        f32x4 va[4], vb[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            va[u] = a(std::true_type{}, k + 8 * u + 4 * half, to);
+            vb[u] = b(std::true_type{}, k + 8 * u + 4 * half, to);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(va[u][e], vb[u][e], acc, 0, 0, 0);
+    }
+    for (; k < to; k += 8) {
+        const f32x4 va = a(std::false_type{}, k + 4 * half, to), vb = b(std::false_type{}, k + 4 * half, to);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(va[e], vb[e], acc, 0, 0, 0);
+    }
+    return acc;
+}
+
+// The waves' sums: thread (wave w, lane l) gets rows 8 w + 4 (l / 32) .. of a, row l % 32 of b.
+__device__ __forceinline__ f32x4 small_sum(const f32x16& acc, float (&lds)[4][16][64]) {
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) lds[wave][e][lane] = acc[e];
+    __syncthreads();
+    f32x4 v;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const uint32_t e = 4 * wave + q;
+        v[q] = (lds[0][e][lane] + lds[1][e][lane]) + (lds[2][e][lane] + lds[3][e][lane]);
+    }
+    return v;
+}
+
+struct SmallArgs {
+    const void* x;
+    const void* w;
+    uint64_t x_ld, w_ld;
+    uint32_t rows, classes, width, tiles_c;  // tiles of 32 classes
+    const int32_t* targets;
+    float* stats;  // [tiles_c][rows][3] as planes of rows_ld
+    float* of;
+    uint32_t rows_ld;
+    const float* lse;
+    const float* dloss;
+    const float* entropy;
+    const float* dentropy;
+    float* g;  // [rows][g_ld]
+    uint32_t g_ld;
+    void* dx;
+    void* dw;
+    uint64_t dx_ld, dw_ld;
+    uint32_t tiles_x;  // workgroups of dX: the rest are dW's
+    // contractions cut into ranges: parts [splits][rows or classes][parts_ld], NULL: not cut
+    uint32_t range;
+    float* parts_x;
+    float* parts_w;
+    uint32_t parts_ld;
+};
+
+template <class T, int KIND>
+__global__ void __launch_bounds__(256) small_logits_kernel(const SmallArgs a) {
+    __shared__ float lds[4][16][64];
+    __shared__ RowStats trade[4][32];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t tn = blockIdx.x / a.tiles_c, tc = blockIdx.x - tn * a.tiles_c;
+    const uint32_t n = tn * 32 + (lane & 31), c = tc * 32 + (lane & 31);
+    const T* const w = static_cast<const T*>(a.w) + (uint64_t)(c < a.classes ? c : a.classes - 1) * a.w_ld;
+    const T* const x = static_cast<const T*>(a.x) + (uint64_t)(n < a.rows ? n : a.rows - 1) * a.x_ld;
+    const f32x16 acc = small_product(
+        0, a.width, [&](auto all, uint32_t k, uint32_t end) { return four_of<decltype(all)::value>(w, k, end); },
+        [&](auto all, uint32_t k, uint32_t end) { return four_of<decltype(all)::value>(x, k, end); });
+    const f32x4 s = small_sum(acc, lds);
+    const uint32_t c0 = tc * 32 + 8 * wave + 4 * (lane >> 5);
+    const int32_t target = n < a.rows ? a.targets[n] : -1;
+    const bool live = target >= 0 && (uint32_t)target < a.classes;
+    const uint32_t hit = (uint32_t)target - c0;
+    if constexpr (KIND == kStats) {
+        RowStats r{-__builtin_huge_valf(), 0.0f, 0.0f};
+        float v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            v[q] = c0 + q < a.classes ? s[q] * kLog2 : -__builtin_huge_valf();
+            r.top = __builtin_fmaxf(r.top, v[q]);
+            if (live && hit == (uint32_t)q) a.of[n] = v[q];
+        }
+        const float zero = r.top == -__builtin_huge_valf() ? 0.0f : r.top;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float d = v[q] - zero, e = exp2_of(d);
+            r.sum += e;
+            r.weighted = __builtin_fmaf(e, __builtin_fmaxf(d, -1000.0f), r.weighted);
+        }
+        RowStats o;
+        float lo, hi;
+        lane_pair<32>(r.top, lo, hi), r.top = lo, o.top = hi;
+        lane_pair<32>(r.sum, lo, hi), r.sum = lo, o.sum = hi;
+        lane_pair<32>(r.weighted, lo, hi), r.weighted = lo, o.weighted = hi;
+        r.join(o);
+        if (lane < 32) trade[wave][lane] = r;
+        __syncthreads();
+        if (threadIdx.x < 32 && n < a.rows) {
+            r = trade[0][lane];
+#pragma unroll
+            for (int k = 1; k < 4; ++k) r.join(trade[k][lane]);
+            float* const at = a.stats + (uint64_t)tc * 3 * a.rows_ld + n;
+            at[0] = r.top, at[a.rows_ld] = r.sum, at[2 * (uint64_t)a.rows_ld] = r.weighted;
+        }
+    } else {
+        if (n >= a.rows) return;
+        f32x4 g = {};
+        if (live) {
+            const float lse2 = a.lse[n] * kLog2, dl = a.dloss[n];
+            const float de = a.dentropy ? a.dentropy[n] * kLn2 : 0.0f, ent = a.dentropy ? a.entropy[n] * kLog2 : 0.0f;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float d = __builtin_fmaf(s[q], kLog2, -lse2), p = exp2_of(d);
+                g[q] = dl * p;
+                if (a.dentropy) g[q] = __builtin_fmaf(-de * p, __builtin_fmaxf(d, -1000.0f) + ent, g[q]);
+                if (hit == (uint32_t)q) g[q] -= dl;
+                if (c0 + q >= a.classes) g[q] = 0.0f;
+            }
+        }
+        *reinterpret_cast<f32x4*>(a.g + (uint64_t)n * a.g_ld + c0) = g;
+    }
+}
+
+// dX = G W and dW = G' X: a's rows are the width's.
+template <class T>
+__global__ void __launch_bounds__(256) small_grad_kernel(const SmallArgs a) {
+    __shared__ float lds[4][16][64];
+    const bool dw = blockIdx.x >= a.tiles_x;
+    const uint32_t tile = blockIdx.x - (dw ? a.tiles_x : 0), tiles_m = (a.width + 31) / 32;
+    const uint32_t tiles_n = ((dw ? a.classes : a.rows) + 31) / 32, split = tile / (tiles_m * tiles_n);
+    const uint32_t of = tile - split * tiles_m * tiles_n, tn = of / tiles_m, tm = of - tn * tiles_m;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t K = dw ? a.rows : a.classes, k0 = split * a.range, k1 = K - k0 < a.range ? K : k0 + a.range;
+    const uint32_t m = tm * 32 + (lane & 31), n = tn * 32 + (lane & 31);
+    const uint32_t mc = m < a.width ? m : a.width - 1;
+    f32x16 acc;
+    if (dw) {
+        const T* const x = static_cast<const T*>(a.x) + mc;
+        const float* const g = a.g + n;  // up to g_ld, a multiple of 32
+        acc = small_product(
+            k0, k1,
+            [&](auto all, uint32_t k, uint32_t end) {
+                f32x4 r = four_down<decltype(all)::value>(x, a.x_ld, k, end);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {  // a row without a target may hold anything
+                    const int32_t target = decltype(all)::value || k + e < end ? a.targets[k + e] : -1;
+                    r[e] = target >= 0 && (uint32_t)target < a.classes ? r[e] : 0.0f;
+                }
+                return r;
+            },
+            [&](auto all, uint32_t k, uint32_t end) { return four_down<decltype(all)::value>(g, a.g_ld, k, end); });
+    } else {
+        const T* const w = static_cast<const T*>(a.w) + mc;
+        const float* const g = a.g + (uint64_t)(n < a.rows ? n : a.rows - 1) * a.g_ld;
+        acc = small_product(
+            k0, k1,
+            [&](auto all, uint32_t k, uint32_t end) { return four_down<decltype(all)::value>(w, a.w_ld, k, end); },
+            [&](auto all, uint32_t k, uint32_t end) { return four_of<decltype(all)::value>(g, k, end); });
+    }
+    const f32x4 v = small_sum(acc, lds);
+    const uint32_t m0 = tm * 32 + 8 * wave + 4 * (lane >> 5);
+    if (n >= (dw ? a.classes : a.rows)) return;
+    float* const parts = dw ? a.parts_w : a.parts_x;
+    if (parts) {  // parts_ld is a multiple of 4
+        if (m0 < a.width)
+            *reinterpret_cast<f32x4*>(parts + ((uint64_t)split * (dw ? a.classes : a.rows) + n) * a.parts_ld + m0) = v;
+        return;
+    }
+    T* const out = static_cast<T*>(dw ? a.dw : a.dx) + n * (dw ? a.dw_ld : a.dx_ld) + m0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        if (m0 + q < a.width) out[q] = (T)v[q];
+}
+
 }  // namespace dev
 
 namespace {
 
 constexpr uint32_t kMostHeadRows = 1u << 20, kMostClasses = 1u << 20, kMostWidth = 1u << 16;
 constexpr uint32_t kHeadM = 256;          // classes of a tile
-constexpr uint32_t kPieceCells = 1u << 25;  // logits of a piece
+constexpr uint32_t kPieceCells = 1u << 25;  // logits of a piece, about
 constexpr uint32_t kSkew = 128;            // elements past a row: rows a power of two apart meet in few memory channels
 constexpr uint32_t kMostPiece = 1u << 17;   // classes of one
 constexpr uint32_t kMostRange = 4096;       // contraction elements of a gradient's tile
+constexpr uint32_t kSmallRange = 512;       // and of a small one's
 
 uint32_t up_to(uint64_t n, uint32_t m) { return (uint32_t)((n + m - 1) / m * m); }
 uint64_t padded(uint64_t bytes) { return (bytes + 255) & ~(uint64_t)255; }
@@ -677,10 +901,27 @@ struct Carve {
     }
 };
 
+// Where the small products take over, by the multiply-adds of one product (both ways measured,
+// us, small first). fp32 saves the launches that scale and split it, and with few rows the passes over
+// W that those make: forward 1024 x 4096 x 128 26 and 31, with a width of 512 71 and 53, 16 x 16384 x 2048
+// 44 and 167; gradients 4096 x 512 x 128 47 and 74, 1024 x 4096 x 128 76 and 71, 256 x 1024 x 2048 68
+// and 164. Of 16-bit types the gradients save launches (1024 x 1024 x 128 33 and 36, 4096 x 512 x 128 46
+// and 43), and where there are few large tiles nothing waits for one tile's long contraction: forward 256
+// x 1024 x 2048 25 and 46, 1024 x 4096 x 128 26 and 18; gradients of the first 61 and 71.
+bool is_small(uint32_t rows, uint32_t classes, uint32_t width, uint32_t type, bool backward) {
+    const uint64_t work = (uint64_t)up_to(rows, 32) * up_to(classes, 32) * up_to(width, 32);
+    const uint64_t tiles = (uint64_t)((rows + 255) / 256) * ((classes + 255) / 256);
+    const bool few = work <= 1u << 29 && tiles <= (backward ? 8 : 16);
+    if (type == MG_TYPE_FP32) return rows <= 32 || work <= 1u << (backward ? 28 : 29) || (backward && few);
+    return backward ? work <= 1u << 27 || few : few && width >= 512;
+}
+
 // What a call keeps in its workspace. 16-bit planes; pairs have two.
 struct HeadSpace {
-    uint32_t width8, rows_ld, g_ld, piece, pieces, tall, splits_x, splits_w, range_x, range_w, parts_ld;
-    uint64_t planes, g_plane;
+    bool small;
+    float* small_g;
+    uint32_t tiles, wide, rows_ld, g_ld, piece, pieces, tall, splits_x, splits_w, range_x, range_w, parts_ld;
+    uint64_t planes;
     uint16_t *x, *x_even, *w, *g;
     uint32_t* live;
     float *stats, *of, *parts_x, *parts_w, *amax;
@@ -690,13 +931,29 @@ struct HeadSpace {
 
     HeadSpace(void* base, uint32_t rows, uint32_t classes, uint32_t width, uint32_t type, bool backward) {
         Carve c{static_cast<char*>(base)};
+        small = is_small(rows, classes, width, type, backward);
+        if (small) {
+            tiles = (classes + 31) / 32, rows_ld = rows, g_ld = tiles * 32;
+            if (backward) {
+                small_g = c.take<float>((uint64_t)rows * g_ld);
+                range_x = range_w = kSmallRange, parts_ld = up_to(width, 4);
+                splits_x = (classes + kSmallRange - 1) / kSmallRange, splits_w = (rows + kSmallRange - 1) / kSmallRange;
+                parts_x = splits_x > 1 ? c.take<float>((uint64_t)splits_x * rows * parts_ld) : nullptr;
+                parts_w = splits_w > 1 ? c.take<float>((uint64_t)splits_w * classes * parts_ld) : nullptr;
+            } else {
+                stats = c.take<float>((uint64_t)tiles * 3 * rows_ld);
+                of = c.take<float>(rows_ld);
+            }
+            bytes = c.used;
+            return;
+        }
         planes = type == MG_TYPE_FP32 ? 2 : 1;
-        width8 = up_to(width, 8), rows_ld = up_to(rows, dev::kHeadN);
+        wide = up_to(width, planes > 1 ? 16 : 8), rows_ld = up_to(rows, dev::kHeadN);
         scales = c.take<dev::HeadScales>(1);
         amax = c.take<float>(3 * dev::kAmaxParts);
         row_exp = c.take<int>(planes > 1 ? rows : 0);
-        x = c.take<uint16_t>(planes * rows * width8);
-        w = c.take<uint16_t>(planes * classes * width8);
+        x = c.take<uint16_t>(planes * rows * wide);
+        w = c.take<uint16_t>(planes * classes * wide);
         if (!backward) {
             stats = c.take<float>((uint64_t)up_to(classes, kHeadM) / kHeadM * 3 * rows_ld);
             of = c.take<float>(rows_ld);
@@ -704,11 +961,11 @@ struct HeadSpace {
             return;
         }
         const uint32_t all = up_to(classes, kHeadM);
-        piece = rows_ld ? up_to(kPieceCells / rows_ld, kHeadM) : kHeadM;
-        piece = piece < kMostRange ? kMostRange : piece > kMostPiece ? kMostPiece : piece;
-        pieces = (all + piece - 1) / piece;
+        pieces = (uint32_t)(((uint64_t)all * rows_ld + kPieceCells / 2) / kPieceCells);
+        if (pieces > all / kMostRange) pieces = all / kMostRange;
+        if (pieces < (all + kMostPiece - 1) / kMostPiece) pieces = (all + kMostPiece - 1) / kMostPiece;
         piece = up_to((all + pieces - 1) / pieces, kHeadM);
-        g_ld = piece + kSkew;
+        g_ld = (uint32_t)planes * piece + kSkew;
         // The gradients' contractions, over a piece's classes and over all rows, are cut so that
         // their tiles are about as many as CUs, or of kMostRange elements where they are more.
         tall = width > 128 ? 256 : 128;
@@ -726,10 +983,9 @@ struct HeadSpace {
         cut(piece, splits_x, range_x);
         cut(rows_ld, splits_w, range_w);
         parts_ld = up_to(width, 4);
-        x_even = c.take<uint16_t>(planes > 1 ? planes * rows * width8 : 0);
+        x_even = c.take<uint16_t>(planes > 1 ? planes * rows * wide : 0);
         live = c.take<uint32_t>(rows_ld / 32);
-        g_plane = (uint64_t)rows_ld * g_ld;
-        g = c.take<uint16_t>(planes * g_plane);
+        g = c.take<uint16_t>((uint64_t)rows_ld * g_ld);
         parts_x = c.take<float>(splits_x > 1 || pieces > 1 ? (uint64_t)splits_x * rows * parts_ld : 0);
         parts_w = c.take<float>(splits_w > 1 ? (uint64_t)splits_w * piece * parts_ld : 0);
         bytes = c.used;
@@ -764,13 +1020,12 @@ HeadInputs prepare(hipStream_t st, const P& p, const HeadSpace& s, const float* 
     typedef typename HeadType<T>::H H;
     const bool pairs = std::is_same<T, float>::value, g = dloss && !std::is_same<T, __bf16>::value;
     HeadInputs in{};
-    in.x = {p.x, 0, (uint32_t)p.x_ld};
-    in.w = {p.w, 0, (uint32_t)p.w_ld};
-    dev::PrepareArgs ax{p.x, p.x_ld, p.rows, p.width, nullptr, nullptr, s.width8, (uint64_t)p.rows * s.width8, s.row_exp};
-    dev::PrepareArgs aw{p.w, p.w_ld, p.classes, p.width, nullptr, nullptr, s.width8, (uint64_t)p.classes * s.width8,
-                        nullptr};
-    if (!fits(p.x, p.x_ld, p.width, p.type)) ax.to = s.x, in.x = {s.x, ax.plane, s.width8};
-    if (!fits(p.w, p.w_ld, p.width, p.type)) aw.to = s.w, in.w = {s.w, aw.plane, s.width8};
+    in.x = {p.x, (uint32_t)p.x_ld};
+    in.w = {p.w, (uint32_t)p.w_ld};
+    dev::PrepareArgs ax{p.x, p.x_ld, p.rows, p.width, nullptr, nullptr, s.wide, s.row_exp};
+    dev::PrepareArgs aw{p.w, p.w_ld, p.classes, p.width, nullptr, nullptr, s.wide, nullptr};
+    if (!fits(p.x, p.x_ld, p.width, p.type)) ax.to = s.x, in.x = {s.x, (uint32_t)s.planes * s.wide};
+    if (!fits(p.w, p.w_ld, p.width, p.type)) aw.to = s.w, in.w = {s.w, (uint32_t)s.planes * s.wide};
     in.x_even = in.x;
     if (pairs && even) ax.to_even = s.x_even, in.x_even.base = s.x_even;
     dev::PrepareScales scales{{nullptr, nullptr, nullptr}, nullptr};
@@ -794,28 +1049,47 @@ HeadInputs prepare(hipStream_t st, const P& p, const HeadSpace& s, const float* 
     return in;
 }
 
+template <class P>
+dev::SmallArgs small_args(const P& p, const HeadSpace& s) {
+    dev::SmallArgs a{};
+    a.x = p.x, a.w = p.w, a.x_ld = p.x_ld, a.w_ld = p.w_ld, a.rows = p.rows, a.classes = p.classes, a.width = p.width;
+    a.tiles_c = s.tiles, a.targets = p.targets, a.rows_ld = s.rows_ld, a.g_ld = s.g_ld;
+    return a;
+}
+int join_tiles(hipStream_t st, const mg_cross_entropy_args& p, const HeadSpace& s, uint32_t tiles) {
+    const uint32_t blocks = (p.rows + 3) / 4;
+    hipLaunchKernelGGL(dev::head_join_kernel, dim3(blocks < 16384 ? blocks : 16384), dim3(256), 0, st, s.stats, s.of,
+                       p.targets, p.rows, s.rows_ld, tiles, p.classes, p.loss, p.lse, p.entropy);
+    MG_HIP(hipGetLastError(), "cross entropy join launch");
+    return MG_OK;
+}
+
 template <class T>
 int cross_entropy(hipStream_t st, const mg_cross_entropy_args& p) {
     typedef typename HeadType<T>::H H;
     constexpr bool kPairs = sizeof(T) == 4;
     const HeadSpace s(p.workspace, p.rows, p.classes, p.width, p.type, false);
+    if (s.small) {
+        dev::SmallArgs a = small_args(p, s);
+        a.stats = s.stats, a.of = s.of;
+        hipLaunchKernelGGL((dev::small_logits_kernel<T, dev::kStats>), dim3((p.rows + 31) / 32 * s.tiles), dim3(256), 0,
+                           st, a);
+        MG_HIP(hipGetLastError(), "cross entropy launch");
+        return join_tiles(st, p, s, s.tiles);
+    }
     dev::HeadArgs a{};
     const HeadInputs in = prepare<T>(st, p, s, nullptr, nullptr, false);
     a.scales = in.scales;
     dev::HeadProduct& m = a.p[0];
     m.a = in.w, m.b = in.x;
-    m.k = m.range = s.width8, m.splits = 1, m.m = p.classes, m.n = p.rows;
+    m.k = m.range = s.wide, m.splits = 1, m.m = p.classes, m.n = p.rows;
     m.tiles_m = up_to(p.classes, kHeadM) / kHeadM, m.tiles_n = s.rows_ld / dev::kHeadN;
     a.tiles = m.tiles_m * m.tiles_n;
     a.rows = p.rows, a.classes = p.classes, a.targets = p.targets, a.row_exp = s.row_exp;
     a.stats = s.stats, a.of = s.of, a.rows_ld = s.rows_ld, a.want_entropy = p.entropy != nullptr;
     hipLaunchKernelGGL((dev::head_kernel<H, dev::kStats, 4, kPairs>), dim3(a.tiles), dim3(512), 0, st, a);
     MG_HIP(hipGetLastError(), "cross entropy launch");
-    const uint32_t blocks = (p.rows + 3) / 4;
-    hipLaunchKernelGGL(dev::head_join_kernel, dim3(blocks < 16384 ? blocks : 16384), dim3(256), 0, st, s.stats, s.of,
-                       p.targets, p.rows, s.rows_ld, m.tiles_m, p.classes, p.loss, p.lse, p.entropy);
-    MG_HIP(hipGetLastError(), "cross entropy join launch");
-    return MG_OK;
+    return join_tiles(st, p, s, m.tiles_m);
 }
 
 template <class T>
@@ -829,12 +1103,33 @@ int cross_entropy_backward(hipStream_t st, const mg_cross_entropy_backward_args&
         return MG_OK;
     }
     const HeadSpace s(p.workspace, p.rows, p.classes, p.width, p.type, true);
+    if (s.small) {
+        dev::SmallArgs a = small_args(p, s);
+        a.lse = p.lse, a.dloss = p.dloss, a.entropy = p.entropy, a.dentropy = p.dentropy, a.g = s.small_g;
+        a.dx = p.dx, a.dw = p.dw, a.dx_ld = p.dx_ld, a.dw_ld = p.dw_ld;
+        const uint32_t tiles_n = (p.rows + 31) / 32, tiles_m = (p.width + 31) / 32;
+        a.tiles_x = p.dx ? tiles_n * tiles_m * s.splits_x : 0;
+        a.range = kSmallRange, a.parts_ld = s.parts_ld;
+        a.parts_x = p.dx && s.splits_x > 1 ? s.parts_x : nullptr, a.parts_w = p.dw && s.splits_w > 1 ? s.parts_w : nullptr;
+        hipLaunchKernelGGL((dev::small_logits_kernel<T, dev::kLogitGrad>), dim3(tiles_n * s.tiles), dim3(256), 0, st, a);
+        MG_HIP(hipGetLastError(), "cross entropy logits launch");
+        hipLaunchKernelGGL(dev::small_grad_kernel<T>, dim3(a.tiles_x + (p.dw ? s.tiles * tiles_m * s.splits_w : 0)),
+                           dim3(256), 0, st, a);
+        if (a.parts_x)
+            hipLaunchKernelGGL(dev::head_sum_kernel<T>, copy_grid(p.width, p.rows), dim3(256), 0, st, a.parts_x,
+                               s.splits_x, p.rows, p.width, s.parts_ld, static_cast<T*>(p.dx), p.dx_ld, nullptr, 0u);
+        if (a.parts_w)
+            hipLaunchKernelGGL(dev::head_sum_kernel<T>, copy_grid(p.width, p.classes), dim3(256), 0, st, a.parts_w,
+                               s.splits_w, p.classes, p.width, s.parts_ld, static_cast<T*>(p.dw), p.dw_ld, nullptr, 1u);
+        MG_HIP(hipGetLastError(), "cross entropy gradients launch");
+        return MG_OK;
+    }
     dev::HeadArgs a{};
     const HeadInputs in = prepare<T>(st, p, s, p.dloss, p.dentropy, p.dw != nullptr);
     a.scales = in.scales;
     a.rows = p.rows, a.classes = p.classes, a.targets = p.targets, a.row_exp = s.row_exp;
     a.lse = p.lse, a.dloss = p.dloss, a.entropy = p.entropy, a.dentropy = p.dentropy;
-    a.rows_ld = s.rows_ld, a.g = s.g, a.g_ld = s.g_ld, a.g_plane = s.g_plane, a.live = s.live;
+    a.rows_ld = s.rows_ld, a.g = s.g, a.g_ld = s.g_ld, a.live = s.live;
     const bool parts_x = s.splits_x > 1 || s.pieces > 1, parts_w = s.splits_w > 1;
     const uint32_t tiles_m = (p.width + s.tall - 1) / s.tall;
     for (uint32_t first = 0; first < p.classes; first += s.piece) {
@@ -843,7 +1138,7 @@ int cross_entropy_backward(hipStream_t st, const mg_cross_entropy_backward_args&
         m = {};
         m.a = in.w, m.b = in.x;
         m.a.base = static_cast<const H*>(in.w.base) + (uint64_t)first * in.w.ld;
-        m.k = m.range = s.width8, m.splits = 1, m.m = here, m.n = p.rows;
+        m.k = m.range = s.wide, m.splits = 1, m.m = here, m.n = p.rows;
         m.tiles_m = fill / kHeadM, m.tiles_n = s.rows_ld / dev::kHeadN;
         a.tiles = m.tiles_m * m.tiles_n, a.first = first;
         hipLaunchKernelGGL((dev::head_kernel<H, dev::kLogitGrad, 4, kPairs>), dim3(a.tiles), dim3(512), 0, st, a);
@@ -853,7 +1148,7 @@ int cross_entropy_backward(hipStream_t st, const mg_cross_entropy_backward_args&
         if (p.dx) {
             dev::HeadProduct& q = a.p[n++];
             q = {};
-            q.a = m_of_w, q.b = {s.g, s.g_plane, s.g_ld}, q.m = p.width, q.n = p.rows;
+            q.a = m_of_w, q.b = {s.g, s.g_ld}, q.m = p.width, q.n = p.rows;
             q.k = here, q.range = s.range_x, q.splits = (here + s.range_x - 1) / s.range_x;
             q.tiles_m = tiles_m, q.tiles_n = s.rows_ld / dev::kHeadN;
             q.out = p.dx, q.out_ld = p.dx_ld, q.parts = parts_x ? s.parts_x : nullptr, q.parts_ld = s.parts_ld;
@@ -863,7 +1158,7 @@ int cross_entropy_backward(hipStream_t st, const mg_cross_entropy_backward_args&
         if (p.dw) {
             dev::HeadProduct& q = a.p[n++];
             q = {};
-            q.a = in.x_even, q.b = {s.g, s.g_plane, s.g_ld}, q.m = p.width, q.n = here, q.live = s.live;
+            q.a = in.x_even, q.b = {s.g, s.g_ld}, q.m = p.width, q.n = here, q.live = s.live;
             q.k = p.rows, q.range = s.range_w, q.splits = (p.rows + s.range_w - 1) / s.range_w;
             q.tiles_m = tiles_m, q.tiles_n = fill / dev::kHeadN;
             q.out = static_cast<T*>(p.dw) + (uint64_t)first * p.dw_ld, q.out_ld = p.dw_ld;

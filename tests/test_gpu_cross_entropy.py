@@ -171,6 +171,14 @@ def test_cross_entropy_long_contractions(mg, kind):
     Case(40, 20011, 520, kind, seed=3).check(mg)
 
 
+@pytest.mark.parametrize("kind", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows,classes,width", [(32, 4100, 1030), (33, 4100, 1030), (700, 1100, 1100), (513, 9000, 129),
+                                                (1030, 300, 72), (2, 70000, 16), (260, 270, 4104)])
+def test_cross_entropy_either_way(mg, kind, rows, classes, width):
+    """Sizes around those where small products take over, each with tiles that stick out."""
+    Case(rows, classes, width, kind, seed=12).check(mg)
+
+
 @pytest.mark.parametrize("kind", ["fp32", "fp16"])
 def test_cross_entropy_sharp_rows(mg, kind):
     """Logits of a spread of 40: most probabilities are under fp32's range."""
@@ -178,14 +186,15 @@ def test_cross_entropy_sharp_rows(mg, kind):
 
 
 @pytest.mark.parametrize("kind", ["fp32", "bf16", "fp16"])
-def test_cross_entropy_rows_left_out(mg, kind):
+@pytest.mark.parametrize("classes,width", [(300, 48), (30011, 200)])
+def test_cross_entropy_rows_left_out(mg, kind, classes, width):
     """Rows without a target hold NaN, infinity and large numbers, and reach nothing."""
-    c = Case(80, 300, 48, kind, seed=5)
-    c.targets[10:14] = [-1, 300, -5, 2**31 - 1]
+    c = Case(80, classes, width, kind, seed=5)
+    c.targets[10:14] = [-1, classes, -5, 2**31 - 1]
     want = c.reference()
     lse, entropy = rounded(want["lse"], "fp32"), rounded(want["entropy"], "fp32")
     grads = c.gradients(lse, entropy)
-    c.x[10], c.x[11, 3], c.x[12] = np.nan, np.inf, rounded(np.full(48, 3e4), kind)
+    c.x[10], c.x[11, 3], c.x[12] = np.nan, np.inf, rounded(np.full(width, 3e4), kind)
     c.dloss[10], c.dloss[12], c.dentropy[13] = np.nan, 1e30, np.inf
     lse[10], entropy[11] = np.nan, np.inf
     c.upload(mg)
@@ -202,9 +211,10 @@ def test_cross_entropy_rows_left_out(mg, kind):
 
 
 @pytest.mark.parametrize("kind", ["fp32", "bf16"])
-def test_cross_entropy_not_finite(mg, kind):
+@pytest.mark.parametrize("classes,width", [(300, 32), (30000, 520)])
+def test_cross_entropy_not_finite(mg, kind, classes, width):
     """A row's NaN is its own, forward; minus infinity as a logit is a class that is never taken."""
-    c = Case(70, 300, 32, kind, seed=6, out=0)
+    c = Case(70, classes, width, kind, seed=6, out=0)
     want = c.reference()
     clean = want["loss"].copy()
     c.x[7, 5] = np.nan
@@ -213,11 +223,11 @@ def test_cross_entropy_not_finite(mg, kind):
     others = np.arange(70) != 7
     assert np.isnan(got["lse"][7]) and np.isnan(got["loss"][7]) and np.isnan(got["entropy"][7])
     assert_within(got["loss"][others], clean[others], 2 * c.err["loss"][others], "loss")
-    c = Case(70, 300, 32, kind, seed=6, out=0)
+    c = Case(70, classes, width, kind, seed=6, out=0)
     c.x = np.abs(c.x) + rounded(np.full(c.x.shape, 0.0078125), kind)
     c.x = rounded(c.x, kind)
     c.targets[c.targets == 9] = 8
-    without = Case(70, 299, 32, kind, seed=6, out=0)
+    without = Case(70, classes - 1, width, kind, seed=6, out=0)
     without.x, without.w = c.x, np.delete(c.w, 9, 0)
     without.targets = np.where(c.targets > 9, c.targets - 1, c.targets).astype(np.int32)
     want = without.reference()
@@ -230,17 +240,19 @@ def test_cross_entropy_not_finite(mg, kind):
 
 @pytest.mark.parametrize("kind", ["fp32", "fp16"])
 @pytest.mark.parametrize("size", [1e-30, 1e30])
-def test_cross_entropy_gradients_of_any_size(mg, kind, size):
-    c = Case(50, 260, 40, kind, seed=7)
+@pytest.mark.parametrize("rows,classes,width", [(50, 260, 40), (300, 5000, 264)])
+def test_cross_entropy_gradients_of_any_size(mg, kind, size, rows, classes, width):
+    c = Case(rows, classes, width, kind, seed=7)
     c.dloss, c.dentropy = rounded(c.dloss * size, "fp32"), rounded(c.dentropy * size, "fp32")
     if kind == "fp16":  # a result's own range
         c.dloss, c.dentropy = rounded(c.dloss / size * 1e-3, "fp32"), rounded(c.dentropy / size * 1e-3, "fp32")
     c.check(mg)
 
 
-def test_cross_entropy_rows_of_different_sizes(mg):
+@pytest.mark.parametrize("classes,width", [(200, 40), (40000, 264)])
+def test_cross_entropy_rows_of_different_sizes(mg, classes, width):
     """fp32 rows of x over twenty powers of ten: each keeps its own accuracy."""
-    c = Case(64, 200, 40, "fp32", seed=8)
+    c = Case(64, classes, width, "fp32", seed=8)
     c.x = rounded(c.x * 10.0 ** np.linspace(-20, 0.5, 64)[:, None], "fp32")
     want = c.reference()
     c.upload(mg)
@@ -250,13 +262,14 @@ def test_cross_entropy_rows_of_different_sizes(mg):
 
 
 @pytest.mark.parametrize("dx,dw", [(True, False), (False, True)])
-def test_cross_entropy_one_gradient(mg, dx, dw):
-    c = Case(60, 500, 72, "bf16", seed=9)
+@pytest.mark.parametrize("rows,classes,width", [(60, 500, 72), (600, 5000, 136)])
+def test_cross_entropy_one_gradient(mg, dx, dw, rows, classes, width):
+    c = Case(rows, classes, width, "bf16", seed=9)
     want = c.reference()
     c.upload(mg)
     lse, entropy = rounded(want["lse"], "fp32"), rounded(want["entropy"], "fp32")
     both = c.backward(mg, lse, entropy)
-    out = Rows(mg, None, "bf16", shape=(60 if dx else 500, 72))
+    out = Rows(mg, None, "bf16", shape=(rows if dx else classes, width))
     space = mg.DeviceBuffer(mg.cross_entropy_backward_workspace(*c.dims()) + 256)
     mg.cross_entropy_backward(*c.at, *c.dims(), lse=c.dev["lse"].ptr, dloss=c.dev["dloss"].ptr,
                               dentropy=c.dev["dentropy"].ptr, entropy=c.dev["entropy"].ptr, workspace=space.ptr,
