@@ -37,9 +37,35 @@ __device__ __forceinline__ void clear(float (&v)[E]) {
     for (int e = 0; e < E; ++e) v[e] = 0.0f;
 }
 
-// The weights and the bias of a thread's channels.
+// The weights and the bias of a thread's channels. Those of a whole vector lie one after the
+// other: read one by one they cost a step of 4096 x 512 bf16 9 of its 19 us.
 template <int W, int E>
 __device__ __forceinline__ void load_taps(const ConvArgs& a, uint32_t v, float (&w)[W][E], float (&bias)[E]) {
+    typedef float four __attribute__((ext_vector_type(4), aligned(4)));
+    if (v * E + E <= a.channels) {
+        const float* const from = a.weight + (size_t)v * E * W;
+        float all[E * W];
+#pragma unroll
+        for (int i = 0; i < E * W; i += 4) {
+            const four r = *reinterpret_cast<const four*>(from + i);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) all[i + q] = r[q];
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            bias[e] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < W; ++k) w[k][e] = all[e * W + k];
+        }
+        if (!a.bias) return;
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+            const four r = *reinterpret_cast<const four*>(a.bias + (size_t)v * E + e);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) bias[e + q] = r[q];
+        }
+        return;
+    }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const uint32_t c = v * E + e;
@@ -92,7 +118,8 @@ struct ConvWalk {
     }
 };
 
-template <class T, int W, int FIT>
+// U: steps whose inputs are read ahead.
+template <class T, int W, int FIT, int U>
 __global__ void __launch_bounds__(256) conv_kernel(const ConvArgs a) {
     constexpr int E = 16 / sizeof(T);
     const uint32_t v = blockIdx.x * a.lanes + (threadIdx.x & (a.lanes - 1));
@@ -109,17 +136,17 @@ __global__ void __launch_bounds__(256) conv_kernel(const ConvArgs a) {
         if (t0 < end) {
             float win[W - 1][E];
             walk.window(t0, win);
-            for (uint32_t t = t0; t < end; t += 4) {
-                float x[4][E];
-                bool fresh[4];
+            for (uint32_t t = t0; t < end; t += U) {
+                float x[U][E];
+                bool fresh[U];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
+                for (int u = 0; u < U; ++u) {
                     const uint32_t s = t + u < end ? t + u : end - 1;
                     walk.row(a.x, a.x_ld, s, x[u]);
                     fresh[u] = walk.reset(s);
                 }
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
+                for (int u = 0; u < U; ++u) {
                     if (t + u >= end) break;
                     if (fresh[u]) {
 #pragma unroll
@@ -321,8 +348,11 @@ int conv(hipStream_t st, const dev::ConvArgs& a, uint32_t taps, const ConvShape&
     const dim3 grid(s.columns, (uint32_t)(s.groups < 65535 ? s.groups : 65535));
     with_fit<T>(a.channels, [&](auto fit) {
         with_taps(taps, [&](auto w) {
-            hipLaunchKernelGGL((dev::conv_kernel<T, decltype(w)::value, decltype(fit)::value>), grid, dim3(256), 0, st,
-                               a);
+            constexpr int W = decltype(w)::value, F = decltype(fit)::value;
+            if (a.at.steps <= 1)
+                hipLaunchKernelGGL((dev::conv_kernel<T, W, F, 1>), grid, dim3(256), 0, st, a);
+            else
+                hipLaunchKernelGGL((dev::conv_kernel<T, W, F, 4>), grid, dim3(256), 0, st, a);
         });
     });
     MG_HIP(hipGetLastError(), "causal conv launch");
