@@ -123,9 +123,8 @@ __device__ __forceinline__ void swap_add(const float (&v)[2 * N], float (&w)[N])
 
 // Sums of eight values (four states of dB, then of dC) over a wave's channels: each pair
 // of values shares a register from the swaps on. Writes them to LDS, [2][SP].
-template <int L>
+template <int L, int SP = 4 * L>
 __device__ __forceinline__ void sum_channels(const float (&v)[8], float* to) {
-    constexpr int SP = 4 * L;
     const int lane = threadIdx.x & 63, s = 4 * (lane % L);
     if constexpr (L == 64) {
 #pragma unroll

@@ -1,6 +1,6 @@
-// The selective scan of 9 to 16 states: four lanes a channel.
+// The selective scan of 9 to 16 states, and of 17 to 64: four lanes a channel.
 //
-// A quad of lanes holds C channels, four states of each a lane. What a step needs of a
+// A quad of lanes holds C channels, NS times four states of each a lane. What a step needs of a
 // channel (delta, delta x, dy) is worked out by one lane of the quad, which does so for every
 // 4 / C th step of one channel, and the others take it by a DPP move; sums over states come
 // back to that lane by two more. B and C lie in LDS as fp32 for a workgroup's four waves, which
@@ -11,7 +11,6 @@
 namespace mg {
 namespace dev {
 
-constexpr int kQuadStates = 16;
 constexpr int kWindow = 32;  // steps of B and C in LDS
 
 // Lane n's value in every lane of each quad; n is a constant once loops are unrolled.
@@ -26,16 +25,28 @@ __device__ __forceinline__ float quad_sums(const float (&v)[4]) {
     return (high ? b : a) + dpp_lane<0x4E>(high ? a : b);
 }
 
-// A workgroup's channels, a lane's four states of C of them, and the one it works for.
+// How a quad's lanes share out C channels' elements.
 template <int C>
-struct QuadLane {
+struct QuadMap {
     static constexpr int P = 4 / C;       // steps that a quad's lanes take at once
     static constexpr int R = kSteps / P;  // times that they do in a round of kSteps
-    static constexpr int CH = 64 * C;     // channels of a workgroup
+    // which of a round's steps the lane's element j is of
+    static __device__ __forceinline__ uint32_t step(int j) { return j * P + (threadIdx.x & 3) / C; }
+    // and which lane of the quad, at which j, has step k of channel c
+    static __device__ __forceinline__ int lane(int k, int c) { return k % P * C + c; }
+};
+
+// A workgroup's channels, a lane's states of C of them, and the one it works for. Vector c NS + q
+// of a lane holds states 16 q + 4 lane ... of channel c.
+template <int C, int NS>
+struct QuadLane : QuadMap<C> {
+    static constexpr int CH = 64 * C;  // channels of a workgroup
+    static constexpr int U = C * NS;   // vectors of a lane
+    static constexpr int SP = 16 * NS;  // states, with padding
     uint32_t group, first, own;  // the quad's first channel, and this lane's
     bool in;                     // whether that is one
-    int state, held[C];          // the first of the lane's states, and how many it has of each channel
-    f32x4 a2[C];                 // A log2(e)
+    int state, held[U];          // the first of the lane's states, and how many each vector has
+    f32x4 a2[U];                 // A log2(e)
 
     __device__ __forceinline__ QuadLane(const ScanArgs& p, uint32_t block) {
         group = block / p.apiece;
@@ -46,26 +57,22 @@ struct QuadLane {
         own = in ? own : limit - 1;
         state = 4 * (threadIdx.x & 3);
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            held[c] = first + c < limit ? (int)p.states - state : 0;
-            a2[c] = load_states(p.a + (size_t)(first + c) * p.states + state, held[c]) * kLog2e;
+        for (int u = 0; u < U; ++u) {
+            held[u] = first + u / NS < limit ? (int)p.states - state - 16 * (u % NS) : 0;
+            a2[u] = load_states(p.a + (size_t)(first + u / NS) * p.states + state + 16 * (u % NS), held[u]) * kLog2e;
         }
     }
-    __device__ __forceinline__ size_t at(const ScanArgs& p, uint32_t n, int c) const {
-        return ((size_t)n * p.channels + first + c) * p.states + state;
+    __device__ __forceinline__ size_t at(const ScanArgs& p, uint32_t n, int u) const {
+        return ((size_t)n * p.channels + first + u / NS) * p.states + state + 16 * (u % NS);
     }
-    __device__ __forceinline__ void load(const ScanArgs& p, const float* from, uint32_t n, f32x4 (&h)[C]) const {
+    __device__ __forceinline__ void load(const ScanArgs& p, const float* from, uint32_t n, f32x4 (&h)[U]) const {
 #pragma unroll
-        for (int c = 0; c < C; ++c) h[c] = load_states(from + at(p, n, c), held[c]);
+        for (int u = 0; u < U; ++u) h[u] = load_states(from + at(p, n, u), held[u]);
     }
-    __device__ __forceinline__ void store(const ScanArgs& p, float* to, uint32_t n, const f32x4 (&h)[C]) const {
+    __device__ __forceinline__ void store(const ScanArgs& p, float* to, uint32_t n, const f32x4 (&h)[U]) const {
 #pragma unroll
-        for (int c = 0; c < C; ++c) store_states(to + at(p, n, c), held[c], h[c]);
+        for (int u = 0; u < U; ++u) store_states(to + at(p, n, u), held[u], h[u]);
     }
-    // which of a round's steps the lane's element j is of
-    static __device__ __forceinline__ uint32_t step(int j) { return j * P + (threadIdx.x & 3) / C; }
-    // and which lane of the quad, at which j, has step k of channel c
-    static __device__ __forceinline__ int lane(int k, int c) { return k % P * C + c; }
 };
 
 // A kernel's arguments, read anew: a round's addresses are worked out from them in scalar
@@ -88,35 +95,36 @@ struct QuadRows {
     const char* base;
     uint32_t by;    // bytes from step to step
     uint32_t mine;  // the lane's first step and its channel
-    __device__ __forceinline__ QuadRows(const ArgsAgain p, const QuadLane<C>& at, const void* array, uint64_t ld,
+    template <int NS>
+    __device__ __forceinline__ QuadRows(const ArgsAgain p, const QuadLane<C, NS>& at, const void* array, uint64_t ld,
                                         uint32_t n)
         : base(static_cast<const char*>(array) + n * p->at.seq_rows * ld * sizeof(T)),
           by((uint32_t)(p->at.step_rows * ld * sizeof(T))),
-          mine(at.in ? QuadLane<C>::step(0) * by + at.own * (uint32_t)sizeof(T) : kNone) {}
+          mine(at.in ? QuadMap<C>::step(0) * by + at.own * (uint32_t)sizeof(T) : kNone) {}
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t at(uint32_t t) const {
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + (uint64_t)t * by), (short)0, 0x7fffffff,
                                                  0x00020000);
     }
     __device__ __forceinline__ int place(uint32_t t, uint32_t end, int j) const {
-        return (int)(t + QuadLane<C>::step(j) < end ? mine : kNone);
+        return (int)(t + QuadMap<C>::step(j) < end ? mine : kNone);
     }
     // the lane's elements of the round at t, as they lie: a conversion here would wait for each
-    __device__ __forceinline__ void load(uint32_t t, uint32_t end, T (&v)[QuadLane<C>::R]) const {
+    __device__ __forceinline__ void load(uint32_t t, uint32_t end, T (&v)[QuadMap<C>::R]) const {
         const __amdgpu_buffer_rsrc_t r = at(t);
 #pragma unroll
-        for (int j = 0; j < QuadLane<C>::R; ++j) {
-            const int s = j * QuadLane<C>::P * (int)by;
+        for (int j = 0; j < QuadMap<C>::R; ++j) {
+            const int s = j * QuadMap<C>::P * (int)by;
             if constexpr (sizeof(T) == 2)
                 v[j] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(r, place(t, end, j), s, 0));
             else
                 v[j] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, place(t, end, j), s, 0));
         }
     }
-    __device__ __forceinline__ void store(uint32_t t, uint32_t end, const float (&v)[QuadLane<C>::R]) const {
+    __device__ __forceinline__ void store(uint32_t t, uint32_t end, const float (&v)[QuadMap<C>::R]) const {
         const __amdgpu_buffer_rsrc_t r = at(t);
 #pragma unroll
-        for (int j = 0; j < QuadLane<C>::R; ++j) {
-            const int s = j * QuadLane<C>::P * (int)by;
+        for (int j = 0; j < QuadMap<C>::R; ++j) {
+            const int s = j * QuadMap<C>::P * (int)by;
             if constexpr (sizeof(T) == 2)
                 __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (T)v[j]), r, place(t, end, j),
                                                       s, 0);
@@ -126,10 +134,10 @@ struct QuadRows {
     }
 };
 
-// B and C of a window's steps, [kSteps ...][16] each; a thread's share on its way.
-template <int STEPS, class T>
+// B and C of a window's steps, [steps][SP] each; a thread's share on its way.
+template <int STEPS, class T, int SP>
 struct QuadShared {
-    static constexpr int N = STEPS * kQuadStates / 256;
+    static constexpr int N = STEPS * SP / 256;
     T b[N], c[N];
     uint8_t reset;
     __device__ __forceinline__ void load(uint32_t group, uint32_t n, uint32_t t, uint32_t end) {
@@ -138,7 +146,7 @@ struct QuadShared {
         const uint64_t row0 = n * p->at.seq_rows, by = p->at.step_rows;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const uint32_t e = threadIdx.x + i * 256, s = t + e / kQuadStates, k = e % kQuadStates;
+            const uint32_t e = threadIdx.x + i * 256, s = t + e / SP, k = e % SP;
             b[i] = c[i] = (T)0.0f;
             if (s >= end || k >= states) continue;
             const uint64_t row = row0 + s * by;
@@ -157,51 +165,62 @@ struct QuadShared {
     __device__ __forceinline__ uint64_t resets() const { return __ballot(reset != 0); }
 };
 
+template <int NS>
+__device__ __forceinline__ void quad_row(const float* row, f32x4 (&v)[NS]) {
+#pragma unroll
+    for (int q = 0; q < NS; ++q) v[q] = *reinterpret_cast<const f32x4*>(row + 16 * q);
+}
+
+// The state (or, backwards, the gradient) that the splits up to one leave, each a decay and an end.
+template <int C, int NS>
+__device__ __forceinline__ void quad_join(const ScanArgs& p, const QuadLane<C, NS>& at, uint32_t n, uint32_t split,
+                                          f32x4 (&h)[C * NS]) {
+    const size_t cells = (size_t)p.at.seqs * p.channels;
+    f32x4 behind[C * NS];
+    at.load(p, p.ends + split * cells * p.states, n, behind);
+#pragma unroll
+    for (int u = 0; u < C * NS; ++u) {
+        const float sum = at.held[u] > 0 ? p.decays[split * cells + (size_t)n * p.channels + at.first + u / NS] : 0.0f;
+        const f32x4 decay = decay_of(at.a2[u], sum);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[u][i] = sum < 0.0f ? behind[u][i] : __builtin_fmaf(decay[i], h[u][i], behind[u][i]);
+    }
+}
+
 // The rates of a lane's elements; steps past the end have delta 0, which leaves a state as
 // it is, and so have lanes without a channel.
 template <int C, class T>
-__device__ __forceinline__ void quad_rates(const QuadLane<C>& at, uint32_t t, uint32_t end, float bias,
-                                           const T (&dt)[QuadLane<C>::R], const T (&x)[QuadLane<C>::R],
-                                           float (&delta)[QuadLane<C>::R], float (&u)[QuadLane<C>::R]) {
+__device__ __forceinline__ void quad_rates(bool in, uint32_t t, uint32_t end, float bias,
+                                           const T (&dt)[QuadMap<C>::R], const T (&x)[QuadMap<C>::R],
+                                           float (&delta)[QuadMap<C>::R], float (&u)[QuadMap<C>::R]) {
 #pragma unroll
-    for (int j = 0; j < QuadLane<C>::R; ++j) {
-        const bool live = at.in && t + QuadLane<C>::step(j) < end;
+    for (int j = 0; j < QuadMap<C>::R; ++j) {
+        const bool live = in && t + QuadMap<C>::step(j) < end;
         delta[j] = live ? softplus((float)dt[j] + bias) : 0.0f;
         u[j] = live ? delta[j] * (float)x[j] : 0.0f;
     }
 }
 
 // As scan_kernel.
-template <class T, int C, bool FULL, bool Z>
-__global__ void __launch_bounds__(256, 4) scan_quad_kernel(const ScanArgs p, uint64_t items) {
-    using Lane = QuadLane<C>;
+template <class T, int C, int NS, bool FULL, bool Z>
+__global__ void __launch_bounds__(256, NS > 2 ? 2 : 4) scan_quad_kernel(const ScanArgs p, uint64_t items) {
+    using Lane = QuadLane<C, NS>;
     constexpr int R = Lane::R;
-    __shared__ __align__(16) float sb[2][kWindow * kQuadStates], sc[2][kWindow * kQuadStates];
+    constexpr int SP = Lane::SP;
+    __shared__ __align__(16) float sb[2][kWindow * SP], sc[2][kWindow * SP];
     for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const ScanItem it(p, item);
         const Lane at(p, it.block);
         const uint32_t n = it.n, length = p.at.length(n), begin = it.split * p.split_steps;
         uint32_t end = begin + p.split_steps;
         end = end < length ? end : length;
-        f32x4 h[C] = {};
+        f32x4 h[Lane::U] = {};
         if constexpr (FULL) {
             if (p.initial) at.load(p, p.splits > 1 ? p.saved : p.initial, n, h);
-            const size_t cells = (size_t)p.at.seqs * p.channels;
 #pragma unroll 2
-            for (uint32_t k = 0; k < it.split; ++k) {
-                f32x4 behind[C];
-                at.load(p, p.ends + k * cells * p.states, n, behind);
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const float sum = at.held[c] > 0 ? p.decays[k * cells + (size_t)n * p.channels + at.first + c] : 0.0f;
-                    const f32x4 decay = decay_of(at.a2[c], sum);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        h[c][i] = sum < 0.0f ? behind[c][i] : __builtin_fmaf(decay[i], h[c][i], behind[c][i]);
-                }
-            }
+            for (uint32_t k = 0; k < it.split; ++k) quad_join(p, at, n, k, h);
         } else if (it.split == 0 && p.initial) {
-            f32x4 first[C];
+            f32x4 first[Lane::U];
             at.load(p, p.initial, n, first);
             at.store(p, p.saved, n, first);
         }
@@ -215,7 +234,7 @@ __global__ void __launch_bounds__(256, 4) scan_quad_kernel(const ScanArgs p, uin
             QuadRows<T, C>(q, at, q->dt, q->dt_ld, n).load(t, end, dt);
             if constexpr (FULL && Z) QuadRows<T, C>(q, at, q->z, q->z_ld, n).load(t, end, z);
         };
-        QuadShared<kWindow, T> shared;
+        QuadShared<kWindow, T, SP> shared;
         if (begin < end) {
             shared.load(at.group, n, begin, end);
             fetch(begin);
@@ -235,7 +254,7 @@ __global__ void __launch_bounds__(256, 4) scan_quad_kernel(const ScanArgs p, uin
             for (uint32_t t = w; t < until; t += kSteps, resets >>= kSteps) {
                 float delta[R], u[R];
                 T was[R], gate[R];
-                quad_rates<C>(at, t, end, bias, dt, x, delta, u);
+                quad_rates<C>(at.in, t, end, bias, dt, x, delta, u);
 #pragma unroll
                 for (int j = 0; j < R; ++j) was[j] = x[j], gate[j] = FULL && Z ? z[j] : (T)0.0f;
                 if (t + kSteps < end) fetch(t + kSteps);
@@ -247,24 +266,28 @@ __global__ void __launch_bounds__(256, 4) scan_quad_kernel(const ScanArgs p, uin
 #pragma unroll
                     for (int k = 0; k < kSteps; ++k) {
                         if (resets >> k & 1) clear_states(h);
-                        const f32x4 b = *reinterpret_cast<const f32x4*>(b_at + k * kQuadStates);
-                        f32x4 cc;
-                        if constexpr (FULL) cc = *reinterpret_cast<const f32x4*>(c_at + k * kQuadStates);
+                        f32x4 b[NS], cc[NS];
+                        quad_row(b_at + k * SP, b);
+                        if constexpr (FULL) quad_row(c_at + k * SP, cc);
 #pragma unroll
                         for (int c = 0; c < C; ++c) {
                             const int from = Lane::lane(k, c), j = k / Lane::P;
                             const float d = quad_take(from, delta[j]), uu = quad_take(from, u[j]);
-                            const f32x4 decay = decay_of(at.a2[c], d);
+                            float y = 0.0f;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) h[c][i] = __builtin_fmaf(decay[i], h[c][i], uu * b[i]);
-                            if constexpr (FULL) {
-                                float y = h[c][0] * cc[0];
+                            for (int q = 0; q < NS; ++q) {
+                                f32x4& s = h[c * NS + q];
+                                const f32x4 decay = decay_of(at.a2[c * NS + q], d);
 #pragma unroll
-                                for (int i = 1; i < 4; ++i) y = __builtin_fmaf(h[c][i], cc[i], y);
-                                part[from] = y;
-                            } else {
-                                sum[c] += d;
+                                for (int i = 0; i < 4; ++i) {
+                                    s[i] = __builtin_fmaf(decay[i], s[i], uu * b[q][i]);
+                                    if constexpr (FULL) y = q + i ? __builtin_fmaf(s[i], cc[q][i], y) : s[i] * cc[q][i];
+                                }
                             }
+                            if constexpr (FULL)
+                                part[from] = y;
+                            else
+                                sum[c] += d;
                         }
                         if constexpr (FULL)
                             if (k % Lane::P == Lane::P - 1) out[k / Lane::P] = quad_sums(part);
@@ -280,7 +303,7 @@ __global__ void __launch_bounds__(256, 4) scan_quad_kernel(const ScanArgs p, uin
                     const ArgsAgain q = args_again();
                     QuadRows<T, C>(q, at, q->y, q->y_ld, n).store(t, end, out);
                 }
-                b_at += kSteps * kQuadStates, c_at += kSteps * kQuadStates;
+                b_at += kSteps * SP, c_at += kSteps * SP;
             }
             if (more) shared.put(sb[turn ^ 1], sc[turn ^ 1]);
             __syncthreads();
@@ -292,17 +315,18 @@ __global__ void __launch_bounds__(256, 4) scan_quad_kernel(const ScanArgs p, uin
             at.store(p, p.ends + (size_t)it.split * p.at.seqs * p.channels * p.states, n, h);
 #pragma unroll
             for (int c = 0; c < C; ++c)
-                if (at.held[c] > 0 && at.state == 0) p.decays[row + at.first + c] = begun ? -1.0f : sum[c];
+                if (at.held[c * NS] > 0 && at.state == 0) p.decays[row + at.first + c] = begun ? -1.0f : sum[c];
         }
     }
 }
 
 // As scan_ends_backward_kernel.
-template <class T, int C>
+template <class T, int C, int NS>
 __global__ void __launch_bounds__(256) scan_quad_ends_backward_kernel(const ScanArgs p, uint64_t items) {
-    using Lane = QuadLane<C>;
+    using Lane = QuadLane<C, NS>;
     constexpr int R = Lane::R;
-    __shared__ __align__(16) float sb[kChunk * kQuadStates], sc[kChunk * kQuadStates];
+    constexpr int SP = Lane::SP;
+    __shared__ __align__(16) float sb[kWindow * SP], sc[kWindow * SP];
     for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const ScanItem it(p, item);
         const Lane at(p, it.block);
@@ -310,17 +334,17 @@ __global__ void __launch_bounds__(256) scan_quad_ends_backward_kernel(const Scan
         uint32_t end = begin + p.split_steps;
         end = end < length ? end : length;
         const float bias = p.dt_bias ? p.dt_bias[at.own] : 0.0f;
-        f32x4 g[C] = {};
+        f32x4 g[Lane::U] = {};
         float sum[C] = {};
         bool begun = false;
-        for (uint32_t chunks = begin < end ? (end - begin + kChunk - 1) / kChunk : 0; chunks--;) {
-            const uint32_t from = begin + chunks * kChunk, to = end - from < (uint32_t)kChunk ? end : from + kChunk;
-            QuadShared<kChunk, T> shared;
+        for (uint32_t window = begin < end ? (end - begin + kWindow - 1) / kWindow : 0; window--;) {
+            const uint32_t from = begin + window * kWindow, to = end - from < (uint32_t)kWindow ? end : from + kWindow;
+            QuadShared<kWindow, T, SP> shared;
             shared.load(at.group, n, from, to);
             __syncthreads();
             shared.put(sb, sc);
             __syncthreads();
-            const uint64_t resets = shared.resets();
+            const uint32_t resets = (uint32_t)shared.resets();
             begun |= resets != 0;
             for (int r = (int)((to - from + kSteps - 1) / kSteps); r--;) {
                 const uint32_t t = from + r * kSteps;
@@ -330,26 +354,28 @@ __global__ void __launch_bounds__(256) scan_quad_ends_backward_kernel(const Scan
                 QuadRows<T, C>(q, at, q->dt, q->dt_ld, n).load(t, to, dt);
                 QuadRows<T, C>(q, at, q->dy, q->dy_ld, n).load(t, to, dy);
                 if (q->z) QuadRows<T, C>(q, at, q->z, q->z_ld, n).load(t, to, z);
-                quad_rates<C>(at, t, to, bias, dt, dt, delta, none);
+                quad_rates<C>(at.in, t, to, bias, dt, dt, delta, none);
 #pragma unroll
                 for (int j = 0; j < R; ++j) into[j] = p.z ? (float)dy[j] * silu((float)z[j]) : (float)dy[j];
-                const uint32_t bits = (uint32_t)(resets >> (r * kSteps)) & ((1u << kSteps) - 1);
+                const uint32_t bits = resets >> (r * kSteps);
 #pragma unroll
                 for (int k = kSteps - 1; k >= 0; --k) {
-                    const f32x4 cc = *reinterpret_cast<const f32x4*>(sc + (r * kSteps + k) * kQuadStates + at.state);
+                    f32x4 cc[NS];
+                    quad_row(sc + (r * kSteps + k) * SP + at.state, cc);
 #pragma unroll
                     for (int c = 0; c < C; ++c) {
                         const int lane = Lane::lane(k, c), j = k / Lane::P;
                         const float d = quad_take(lane, delta[j]), dyk = quad_take(lane, into[j]);
-                        const f32x4 decay = decay_of(at.a2[c], d);
                         sum[c] += d;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) g[c][i] = __builtin_fmaf(cc[i], dyk, g[c][i]) * decay[i];
-                    }
-                    if (bits >> k & 1) {
+                        for (int q = 0; q < NS; ++q) {
+                            const f32x4 decay = decay_of(at.a2[c * NS + q], d);
+                            f32x4& s = g[c * NS + q];
 #pragma unroll
-                        for (int c = 0; c < C; ++c) g[c] = f32x4{};
+                            for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(cc[q][i], dyk, s[i]) * decay[i];
+                        }
                     }
+                    if (bits >> k & 1) clear_states(g);
                 }
             }
         }
@@ -357,7 +383,28 @@ __global__ void __launch_bounds__(256) scan_quad_ends_backward_kernel(const Scan
         at.store(p, p.ends + (size_t)split * p.at.seqs * p.channels * p.states, n, g);
 #pragma unroll
         for (int c = 0; c < C; ++c)
-            if (at.held[c] > 0 && at.state == 0) p.decays[row + at.first + c] = begun ? -1.0f : sum[c];
+            if (at.held[c * NS] > 0 && at.state == 0) p.decays[row + at.first + c] = begun ? -1.0f : sum[c];
+    }
+}
+
+// Step k of a round: the states on, from delta and delta x in the lanes that have them.
+template <int C, int NS>
+__device__ __forceinline__ void quad_step(const QuadLane<C, NS>& at, const float* b_row, int k,
+                                          const float (&delta)[QuadMap<C>::R], const float (&u)[QuadMap<C>::R],
+                                          f32x4 (&h)[C * NS]) {
+    f32x4 b[NS];
+    quad_row(b_row + at.state, b);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int lane = QuadMap<C>::lane(k, c), j = k / QuadMap<C>::P;
+        const float d = quad_take(lane, delta[j]), uu = quad_take(lane, u[j]);
+#pragma unroll
+        for (int q = 0; q < NS; ++q) {
+            const f32x4 decay = decay_of(at.a2[c * NS + q], d);
+            f32x4& s = h[c * NS + q];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(decay[i], s[i], uu * b[q][i]);
+        }
     }
 }
 
@@ -365,19 +412,19 @@ __global__ void __launch_bounds__(256) scan_quad_ends_backward_kernel(const Scan
 // each lane's own. The second half of a chunk walks over the first to its own first state.
 // The decays are worked out twice: to keep them beside the states would take the registers of
 // a wave a SIMD.
-template <class T, int C, bool Z>
+template <class T, int C, int NS, bool Z>
 __global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanArgs p, uint32_t parts) {
-    using Lane = QuadLane<C>;
-    constexpr int R = Lane::R, kRounds = kWindow / kSteps;
-    __shared__ __align__(16) float sb[kWindow * kQuadStates], sc[kWindow * kQuadStates];
-    __shared__ f32x4 starts[kRounds - 1][C][256];
+    using Lane = QuadLane<C, NS>;
+    constexpr int R = Lane::R, U = Lane::U, SP = Lane::SP, kRounds = kWindow / kSteps;
+    __shared__ __align__(16) float sb[kWindow * SP], sc[kWindow * SP];
+    __shared__ f32x4 starts[kRounds - 1][U][256];
     __shared__ float rates[kRounds - 1][R][256];           // delta of the rounds that are walked over
-    __shared__ float sums[2][kSteps][4][2 * kQuadStates];  // each wave's for dB and dC
+    __shared__ float sums[2][kSteps][4][2 * SP];  // each wave's for dB and dC
     const uint32_t block = blockIdx.x % p.blocks, part = blockIdx.x / p.blocks;
     const int wave = threadIdx.x >> 6;
     const Lane at(p, block);
     const float skip = p.d ? p.d[at.own] : 0.0f, bias = p.dt_bias ? p.dt_bias[at.own] : 0.0f;
-    f32x4 da[C] = {};
+    f32x4 da[U] = {};
     float dd = 0.0f, dbias = 0.0f;
     int turn = 0;
     const uint64_t items = (uint64_t)p.at.seqs * p.splits;
@@ -386,27 +433,16 @@ __global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanAr
         const uint32_t length = p.at.length(n), begin = split * p.split_steps;
         uint32_t end = begin + p.split_steps;
         end = end < length ? end : length;
-        f32x4 g[C] = {};
+        f32x4 g[U] = {};
         if (p.dfinal) at.load(p, p.dfinal, n, g);
         const size_t cells = (size_t)p.at.seqs * p.channels;
-#pragma unroll 4
-        for (uint32_t k = p.splits - 1; k > split; --k) {
-            f32x4 behind[C];
-            at.load(p, p.ends + k * cells * p.states, n, behind);
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const float sum = at.held[c] > 0 ? p.decays[k * cells + (size_t)n * p.channels + at.first + c] : 0.0f;
-                const f32x4 decay = decay_of(at.a2[c], sum);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    g[c][i] = sum < 0.0f ? behind[c][i] : __builtin_fmaf(decay[i], g[c][i], behind[c][i]);
-            }
-        }
+#pragma unroll 2
+        for (uint32_t k = p.splits - 1; k > split; --k) quad_join(p, at, n, k, g);
         for (uint32_t window = begin < end ? (end - begin + kWindow - 1) / kWindow : 0; window--;) {
             const uint32_t from = begin + window * kWindow, to = end - from < (uint32_t)kWindow ? end : from + kWindow;
             const uint32_t chunk = from / kChunk * kChunk;
             const int rounds = (int)((to - from + kSteps - 1) / kSteps);
-            f32x4 h[C] = {};
+            f32x4 h[U] = {};
             if (chunk && p.kept)
                 at.load(p, p.kept + chunk / kChunk * cells * p.states, n, h);
             else if (!chunk && p.initial)
@@ -424,7 +460,7 @@ __global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanAr
             for (uint32_t w = chunk; w <= from; w += kWindow) {
                 const uint32_t last = w == from ? to : w + kWindow;
                 const int walk = w == from ? rounds - 1 : kRounds;
-                QuadShared<kWindow, T> shared;
+                QuadShared<kWindow, T, SP> shared;
                 shared.load(at.group, n, w, last);
                 fetch(w, last, walk == 0);
                 __syncthreads();  // every wave is done with B and C
@@ -434,11 +470,11 @@ __global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanAr
                 for (int r = 0; r < walk; ++r) {
                     const uint32_t t = w + r * kSteps;
                     float delta[R], u[R];
-                    quad_rates<C>(at, t, last, bias, dt, x, delta, u);
+                    quad_rates<C>(at.in, t, last, bias, dt, x, delta, u);
                     if (t + kSteps < last) fetch(t + kSteps, last, w == from && r + 1 == walk);
                     if (w == from) {
 #pragma unroll
-                        for (int c = 0; c < C; ++c) starts[r][c][threadIdx.x] = h[c];
+                        for (int u = 0; u < U; ++u) starts[r][u][threadIdx.x] = h[u];
 #pragma unroll
                         for (int j = 0; j < R; ++j) rates[r][j][threadIdx.x] = delta[j];
                     }
@@ -446,15 +482,7 @@ __global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanAr
 #pragma unroll
                     for (int k = 0; k < kSteps; ++k) {
                         if (bits >> k & 1) clear_states(h);
-                        const f32x4 b = *reinterpret_cast<const f32x4*>(sb + (r * kSteps + k) * kQuadStates + at.state);
-#pragma unroll
-                        for (int c = 0; c < C; ++c) {
-                            const int lane = Lane::lane(k, c), j = k / Lane::P;
-                            const f32x4 decay = decay_of(at.a2[c], quad_take(lane, delta[j]));
-                            const float uu = quad_take(lane, u[j]);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) h[c][i] = __builtin_fmaf(decay[i], h[c][i], uu * b[i]);
-                        }
+                        quad_step(at, sb + (r * kSteps + k) * SP, k, delta, u, h);
                     }
                 }
             }
@@ -465,7 +493,7 @@ __global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanAr
 #pragma unroll
                     for (int j = 0; j < R; ++j) delta[j] = rates[r][j][threadIdx.x], u[j] = delta[j] * (float)x[j];
                 } else {
-                    quad_rates<C>(at, t, to, bias, dt, x, delta, u);
+                    quad_rates<C>(at.in, t, to, bias, dt, x, delta, u);
                 }
 #pragma unroll
                 for (int j = 0; j < R; ++j) {
@@ -475,26 +503,19 @@ __global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanAr
                 }
                 if (r + 1 < rounds) {
 #pragma unroll
-                    for (int c = 0; c < C; ++c) h[c] = starts[r][c][threadIdx.x];
+                    for (int u = 0; u < U; ++u) h[u] = starts[r][u][threadIdx.x];
                 }
                 const uint32_t bits = resets >> (r * kSteps);
                 float gb[R], ga[R], y[R];
-                f32x4 first[C], states[kSteps][C];
+                f32x4 first[U], states[kSteps][U];
 #pragma unroll
-                for (int c = 0; c < C; ++c) first[c] = h[c];
+                for (int w = 0; w < U; ++w) first[w] = h[w];
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
                     if (bits >> k & 1) clear_states(h);
-                    const f32x4 b = *reinterpret_cast<const f32x4*>(sb + (r * kSteps + k) * kQuadStates + at.state);
+                    quad_step(at, sb + (r * kSteps + k) * SP, k, delta, u, h);
 #pragma unroll
-                    for (int c = 0; c < C; ++c) {
-                        const int lane = Lane::lane(k, c), j = k / Lane::P;
-                        const f32x4 decay = decay_of(at.a2[c], quad_take(lane, delta[j]));
-                        const float uu = quad_take(lane, u[j]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) h[c][i] = __builtin_fmaf(decay[i], h[c][i], uu * b[i]);
-                        states[k][c] = h[c];
-                    }
+                    for (int w = 0; w < U; ++w) states[k][w] = h[w];
                 }
                 // or the compiler keeps what it knows of the decays, B and the moved values
 #pragma unroll
@@ -502,21 +523,26 @@ __global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanAr
                 float part_b[4], part_a[4], part_y[4];
 #pragma unroll
                 for (int k = kSteps - 1; k >= 0; --k) {
-                    const f32x4 b = *reinterpret_cast<const f32x4*>(sb + (r * kSteps + k) * kQuadStates + at.state);
-                    const f32x4 cc = *reinterpret_cast<const f32x4*>(sc + (r * kSteps + k) * kQuadStates + at.state);
-                    float v[8] = {};
+                    f32x4 b[NS], cc[NS];
+                    quad_row(sb + (r * kSteps + k) * SP + at.state, b);
+                    quad_row(sc + (r * kSteps + k) * SP + at.state, cc);
+                    float v[NS][8] = {};
 #pragma unroll
                     for (int c = 0; c < C; ++c) {
                         const int lane = Lane::lane(k, c), j = k / Lane::P;
                         const float dyk = quad_take(lane, into[j]), uu = quad_take(lane, u[j]);
                         float sum_b = 0.0f, sum_y = 0.0f;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            g[c][i] = __builtin_fmaf(cc[i], dyk, g[c][i]);
-                            v[i] = __builtin_fmaf(g[c][i], uu, v[i]);
-                            v[4 + i] = __builtin_fmaf(states[k][c][i], dyk, v[4 + i]);
-                            if (Z) sum_y = __builtin_fmaf(cc[i], states[k][c][i], sum_y);
-                            sum_b = __builtin_fmaf(g[c][i], b[i], sum_b);
+                        for (int q = 0; q < NS; ++q) {
+                            const int w = c * NS + q;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                g[w][i] = __builtin_fmaf(cc[q][i], dyk, g[w][i]);
+                                v[q][i] = __builtin_fmaf(g[w][i], uu, v[q][i]);
+                                v[q][4 + i] = __builtin_fmaf(states[k][w][i], dyk, v[q][4 + i]);
+                                if (Z) sum_y = __builtin_fmaf(cc[q][i], states[k][w][i], sum_y);
+                                sum_b = __builtin_fmaf(g[w][i], b[q][i], sum_b);
+                            }
                         }
                         part_b[lane] = sum_b, part_y[lane] = sum_y;
                     }
@@ -530,20 +556,25 @@ __global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanAr
                         for (int c = 0; c < C; ++c) {
                             const int lane = Lane::lane(k, c), j = k / Lane::P;
                             const float d = quad_take(lane, delta[j]);
-                            const f32x4 decay = decay_of(at.a2[c], d);
-                            const f32x4 before = k ? states[k ? k - 1 : 0][c] : first[c];
                             float sum_a = 0.0f;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                g[c][i] *= decay[i];
-                                const float via = g[c][i] * before[i];
-                                sum_a = __builtin_fmaf(via, at.a2[c][i], sum_a);
-                                da[c][i] = __builtin_fmaf(via, d, da[c][i]);
+                            for (int q = 0; q < NS; ++q) {
+                                const int w = c * NS + q;
+                                const f32x4 decay = decay_of(at.a2[w], d);
+                                const f32x4 before = k ? states[k ? k - 1 : 0][w] : first[w];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    g[w][i] *= decay[i];
+                                    const float via = g[w][i] * before[i];
+                                    sum_a = __builtin_fmaf(via, at.a2[w][i], sum_a);
+                                    da[w][i] = __builtin_fmaf(via, d, da[w][i]);
+                                }
                             }
                             part_a[lane] = sum_a;
                         }
                     }
-                    sum_channels<4>(v, sums[turn][k][wave]);
+#pragma unroll
+                    for (int q = 0; q < NS; ++q) sum_channels<4, SP>(v[q], sums[turn][k][wave] + 16 * q);
                     if (k % Lane::P == 0) {
                         const int j = k / Lane::P;
                         gb[j] = quad_sums(part_b), ga[j] = quad_sums(part_a);
@@ -573,11 +604,13 @@ __global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanAr
                     if (Z && q->dz) QuadRows<T, C>(q, at, q->dz, q->dz_ld, n).store(t, to, y);
                 }
                 __syncthreads();
-                const int k = threadIdx.x >> 5, w = threadIdx.x & 31, i = w & 15;
-                if (t + k < to && i < (int)p.states) {
+#pragma unroll
+                for (int e = threadIdx.x; e < kSteps * 2 * SP; e += 256) {
+                    const int k = e / (2 * SP), w = e % (2 * SP), i = w % SP;
+                    if (t + k >= to || i >= (int)p.states) continue;
                     const float sum = (sums[turn][k][0][w] + sums[turn][k][1][w]) +
                                       (sums[turn][k][2][w] + sums[turn][k][3][w]);
-                    const uint32_t which = w >> 4;
+                    const uint32_t which = w / SP;
                     const ArgsAgain q = args_again();
                     if (q->apiece == 1) {
                         const uint64_t row = (t + k) * q->at.step_rows + n * q->at.seq_rows;
@@ -606,36 +639,40 @@ __global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanAr
 
 // One step of every sequence, four sequences at a time: no LDS, every load at once, the
 // states to memory and back. A quad's lanes each work for one of the four.
-template <class T, bool Z>
+template <class T, int NS, bool Z>
 __global__ void __launch_bounds__(256) scan_quad_step_kernel(const ScanArgs p, uint64_t items) {
-    using Lane = QuadLane<1>;
+    using Lane = QuadLane<1, NS>;
     typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
     for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const uint32_t n0 = (uint32_t)(item / p.blocks) * 4;
         const Lane at(p, (uint32_t)(item % p.blocks));
         const uint32_t last = p.at.seqs - 1;
         const float skip = p.d ? p.d[at.own] : 0.0f, bias = p.dt_bias ? p.dt_bias[at.own] : 0.0f;
-        f32x4 h[4], b[4], c[4];
+        f32x4 h[4][NS], b[4][NS], c[4][NS];
         bool fresh[4], live[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const uint32_t n = n0 + q < last ? n0 + q : last;
+        for (int s = 0; s < 4; ++s) {
+            const uint32_t n = n0 + s < last ? n0 + s : last;
             const uint64_t row = p.at.row(0, n);
-            h[q] = p.initial ? load_states(p.initial + at.at(p, n, 0), at.held[0]) : f32x4{};
-            live[q] = p.at.length(n) != 0;
-            fresh[q] = live[q] && p.at.reset && p.at.reset[row];
-            b[q] = c[q] = f32x4{};
-            if (!live[q]) continue;
-            const T* const bs = static_cast<const T*>(p.b) + row * p.b_ld + (size_t)at.group * p.states + at.state;
-            const T* const cs = static_cast<const T*>(p.c) + row * p.c_ld + (size_t)at.group * p.states + at.state;
-            if (p.states == kQuadStates) {
-                const four vb = *reinterpret_cast<const four*>(bs), vc = *reinterpret_cast<const four*>(cs);
+            live[s] = p.at.length(n) != 0;
+            fresh[s] = live[s] && p.at.reset && p.at.reset[row];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) b[q][i] = (float)vb[i], c[q][i] = (float)vc[i];
-            } else {
+            for (int q = 0; q < NS; ++q) {
+                h[s][q] = p.initial ? load_states(p.initial + at.at(p, n, q), at.held[q]) : f32x4{};
+                b[s][q] = c[s][q] = f32x4{};
+                if (!live[s]) continue;
+                const size_t from = (size_t)at.group * p.states + at.state + 16 * q;
+                const T* const bs = static_cast<const T*>(p.b) + row * p.b_ld + from;
+                const T* const cs = static_cast<const T*>(p.c) + row * p.c_ld + from;
+                if (p.states == Lane::SP) {
+                    const four vb = *reinterpret_cast<const four*>(bs), vc = *reinterpret_cast<const four*>(cs);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (at.state + i < (int)p.states) b[q][i] = (float)bs[i], c[q][i] = (float)cs[i];
+                    for (int i = 0; i < 4; ++i) b[s][q][i] = (float)vb[i], c[s][q][i] = (float)vc[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (at.state + 16 * q + i < (int)p.states) b[s][q][i] = (float)bs[i], c[s][q][i] = (float)cs[i];
+                }
             }
         }
         const uint32_t mine = n0 + (threadIdx.x & 3), n = mine < last ? mine : last;
@@ -650,18 +687,22 @@ __global__ void __launch_bounds__(256) scan_quad_step_kernel(const ScanArgs p, u
         const float delta = works ? softplus(dt + bias) : 0.0f, u = works ? delta * x : 0.0f;
         float part[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            if (fresh[q]) h[q] = f32x4{};
-            const f32x4 decay = decay_of(at.a2[0], quad_take(q, delta));
-            const float uu = quad_take(q, u);
-            part[q] = 0.0f;
+        for (int s = 0; s < 4; ++s) {
+            const float d = quad_take(s, delta), uu = quad_take(s, u);
+            part[s] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float moved = __builtin_fmaf(decay[i], h[q][i], uu * b[q][i]);
-                h[q][i] = live[q] ? moved : h[q][i];
-                part[q] = __builtin_fmaf(h[q][i], c[q][i], part[q]);
+            for (int q = 0; q < NS; ++q) {
+                f32x4& v = h[s][q];
+                if (fresh[s]) v = f32x4{};
+                const f32x4 decay = decay_of(at.a2[q], d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float moved = __builtin_fmaf(decay[i], v[i], uu * b[s][q][i]);
+                    v[i] = live[s] ? moved : v[i];
+                    part[s] = __builtin_fmaf(v[i], c[s][q][i], part[s]);
+                }
+                if (p.final && n0 + s <= last) store_states(p.final + at.at(p, n0 + s, q), at.held[q], v);
             }
-            if (p.final && n0 + q <= last) store_states(p.final + at.at(p, n0 + q, 0), at.held[0], h[q]);
         }
         float y = quad_sums(part);
         if (works && at.in) {

@@ -558,14 +558,17 @@ struct ScanShape {
 };
 // The steps are split where the channels and sequences alone give fewer than two workgroups
 // a CU: each split's steps are walked over twice, which pays once the chip is half idle. Quads take
-// 9 to 16 states (32 steps of 4096 x 256 with 16, bf16: 265 us without them, so 176; the gradient
-// 1170 and 720), two channels each where that leaves four workgroups a CU (the same with one: 195
-// and 760), but not rows whose steps lie too far apart for 31 bits.
-ScanShape scan_shape(uint32_t steps, uint32_t seqs, uint32_t channels, uint32_t states, uint32_t groups, bool far) {
+// 9 to 64 states (32 steps of 4096 x 256 with 16, bf16: 265 us without them, so 176; the gradient
+// 1170 and 720), but not rows whose steps lie too far apart for 31 bits, nor the gradient of more than
+// 32 (a lane's registers). Two channels each where 16 states leave four workgroups a CU (the same
+// with one: 195 and 760).
+ScanShape scan_shape(uint32_t steps, uint32_t seqs, uint32_t channels, uint32_t states, uint32_t groups, bool far,
+                     bool backward) {
     ScanShape s;
     s.lanes = lanes_of(states);
+    s.wide = !far && s.lanes >= 4 && s.lanes <= (backward ? 8 : 16);
     s.per = channels / groups;
-    const uint32_t ch = 256 / s.lanes;
+    const uint32_t ch = s.wide ? 64 : 256 / s.lanes;
     s.apiece = (s.per + ch - 1) / ch;
     s.blocks = s.apiece * groups;
     const uint64_t have = (uint64_t)s.blocks * seqs;
@@ -577,9 +580,8 @@ ScanShape scan_shape(uint32_t steps, uint32_t seqs, uint32_t channels, uint32_t 
     const uint32_t each = units ? (uint32_t)((units + splits - 1) / splits) : 1;
     s.splits = units ? (units + each - 1) / each : 1;
     s.split_steps = each * dev::kChunk;
-    s.wide = s.lanes == 4 && !far;
     const uint32_t pairs = (s.per + 127) / 128;
-    if (s.wide && (uint64_t)pairs * groups * seqs * s.splits >= 4 * kCus)
+    if (s.wide && s.lanes == 4 && (uint64_t)pairs * groups * seqs * s.splits >= 4 * kCus)
         s.wide = 2, s.apiece = pairs, s.blocks = pairs * groups;
     return s;
 }
@@ -627,12 +629,18 @@ void with_lanes(uint32_t lanes, Fn&& f) {
 }
 dim3 grid_of(uint64_t items) { return dim3((uint32_t)(items < kMostGroups ? items : kMostGroups)); }
 
-template <int C, bool FULL, class T>
-void launch_quad(hipStream_t st, const dev::ScanArgs& a, uint64_t items) {
-    if (FULL && a.z)
-        hipLaunchKernelGGL((dev::scan_quad_kernel<T, C, FULL, FULL>), grid_of(items), dim3(256), 0, st, a, items);
-    else
-        hipLaunchKernelGGL((dev::scan_quad_kernel<T, C, FULL, false>), grid_of(items), dim3(256), 0, st, a, items);
+// f(channels of a quad, vectors of a lane for each) for a shape whose quads scan.
+template <class Fn>
+void with_quads(const ScanShape& s, Fn&& f) {
+    if (s.wide == 2) return f(std::integral_constant<int, 2>{}, std::integral_constant<int, 1>{});
+    if (s.lanes == 4) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+    if (s.lanes == 8) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});
+    f(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
+}
+template <class Fn>
+void with_gate(const void* z, Fn&& f) {
+    if (z) return f(std::true_type{});
+    f(std::false_type{});
 }
 
 template <class T>
@@ -642,10 +650,12 @@ int scan(hipStream_t st, const dev::ScanArgs& given, const ScanShape& s) {
         if (s.wide) {
             a.apiece = (s.per + 63) / 64, a.blocks = a.apiece * a.groups;
             const uint64_t items = (uint64_t)a.blocks * ((a.at.seqs + 3) / 4);
-            if (a.z)
-                hipLaunchKernelGGL((dev::scan_quad_step_kernel<T, true>), grid_of(items), dim3(256), 0, st, a, items);
-            else
-                hipLaunchKernelGGL((dev::scan_quad_step_kernel<T, false>), grid_of(items), dim3(256), 0, st, a, items);
+            with_quads(s, [&](auto, auto ns) {
+                with_gate(a.z, [&](auto z) {
+                    hipLaunchKernelGGL((dev::scan_quad_step_kernel<T, decltype(ns)::value, decltype(z)::value>),
+                                       grid_of(items), dim3(256), 0, st, a, items);
+                });
+            });
         } else {
             const uint64_t items = (uint64_t)s.blocks * a.at.seqs;
             with_lanes(s.lanes, [&](auto l) {
@@ -657,12 +667,17 @@ int scan(hipStream_t st, const dev::ScanArgs& given, const ScanShape& s) {
         return MG_OK;
     }
     const uint64_t each = (uint64_t)s.blocks * a.at.seqs, ends = each * (s.splits - 1), all = each * s.splits;
-    if (s.wide == 2) {
-        if (ends) launch_quad<2, false, T>(st, a, ends);
-        launch_quad<2, true, T>(st, a, all);
-    } else if (s.wide) {
-        if (ends) launch_quad<1, false, T>(st, a, ends);
-        launch_quad<1, true, T>(st, a, all);
+    if (s.wide) {
+        with_quads(s, [&](auto c, auto ns) {
+            constexpr int C = decltype(c)::value, NS = decltype(ns)::value;
+            if (ends)
+                hipLaunchKernelGGL((dev::scan_quad_kernel<T, C, NS, false, false>), grid_of(ends), dim3(256), 0, st, a,
+                                   ends);
+            with_gate(a.z, [&](auto z) {
+                hipLaunchKernelGGL((dev::scan_quad_kernel<T, C, NS, true, decltype(z)::value>), grid_of(all), dim3(256),
+                                   0, st, a, all);
+            });
+        });
     } else {
         with_lanes(s.lanes, [&](auto l) {
             constexpr int L = decltype(l)::value;
@@ -674,26 +689,22 @@ int scan(hipStream_t st, const dev::ScanArgs& given, const ScanShape& s) {
     return MG_OK;
 }
 
-template <int C, class T>
-void launch_quad_backward(hipStream_t st, const dev::ScanArgs& a, uint64_t ends, uint32_t parts) {
-    if (ends)
-        hipLaunchKernelGGL((dev::scan_quad_ends_backward_kernel<T, C>), grid_of(ends), dim3(256), 0, st, a, ends);
-    const dim3 grid(a.blocks * parts);
-    if (a.z)
-        hipLaunchKernelGGL((dev::scan_quad_backward_kernel<T, C, true>), grid, dim3(256), 0, st, a, parts);
-    else
-        hipLaunchKernelGGL((dev::scan_quad_backward_kernel<T, C, false>), grid, dim3(256), 0, st, a, parts);
-}
-
 template <class T>
 int scan_backward(hipStream_t st, const dev::ScanArgs& a, const ScanShape& s, float* da, float* dd, float* dbias) {
     const uint32_t parts = backward_parts(s, a.at.seqs);
     if (parts) {
         const uint64_t ends = (uint64_t)s.blocks * a.at.seqs * (s.splits - 1);
-        if (s.wide == 2)
-            launch_quad_backward<2, T>(st, a, ends, parts);
-        else if (s.wide)
-            launch_quad_backward<1, T>(st, a, ends, parts);
+        if (s.wide)
+            with_quads(s, [&](auto c, auto ns) {
+                constexpr int C = decltype(c)::value, NS = decltype(ns)::value <= 2 ? decltype(ns)::value : 2;
+                if (ends)
+                    hipLaunchKernelGGL((dev::scan_quad_ends_backward_kernel<T, C, NS>), grid_of(ends), dim3(256), 0, st,
+                                       a, ends);
+                with_gate(a.z, [&](auto z) {
+                    hipLaunchKernelGGL((dev::scan_quad_backward_kernel<T, C, NS, decltype(z)::value>),
+                                       dim3(s.blocks * parts), dim3(256), 0, st, a, parts);
+                });
+            });
         else
             with_lanes(s.lanes, [&](auto l) {
                 constexpr int L = decltype(l)::value;
@@ -775,7 +786,11 @@ int mg_selective_scan_workspace(uint32_t steps, uint32_t seqs, uint32_t channels
         (rc = check_states(what, channels, states, 1)))
         return rc;
     // more groups make more blocks, and those at most as many splits
-    *bytes = split_bytes(scan_shape(steps, seqs, channels, states, 1, false), seqs, channels, states);
+    *bytes = 0;
+    for (bool far : {false, true}) {
+        const uint64_t need = split_bytes(scan_shape(steps, seqs, channels, states, 1, far, false), seqs, channels, states);
+        *bytes = need > *bytes ? need : *bytes;
+    }
     return MG_OK;
 }
 
@@ -795,7 +810,7 @@ int mg_selective_scan(void* stream, const mg_selective_scan_args* args) {
         return rc;
     if (!p.seqs || (!p.steps && !p.final)) return MG_OK;
     const ScanShape s = scan_shape(p.steps, p.seqs, p.channels, p.states, p.groups,
-                                   inputs_far(p) || lies_far(p.step_rows, p.y_ld, p.type));
+                                   inputs_far(p) || lies_far(p.step_rows, p.y_ld, p.type), false);
     if ((rc = check_workspace(what, p.workspace, p.workspace_bytes, split_bytes(s, p.seqs, p.channels, p.states))))
         return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
@@ -820,7 +835,7 @@ int mg_selective_scan_backward_workspace(uint32_t steps, uint32_t seqs, uint32_t
         return rc;
     *bytes = 0;
     for (bool far : {false, true}) {
-        const ScanShape s = scan_shape(steps, seqs, channels, states, groups, far);
+        const ScanShape s = scan_shape(steps, seqs, channels, states, groups, far, true);
         const uint64_t need = split_bytes(s, seqs, channels, states) + shared_bytes(s, steps, seqs, groups, states) +
                               padded((uint64_t)backward_parts(s, seqs) * channels * (states + 2) * 4);
         *bytes = need > *bytes ? need : *bytes;
@@ -859,7 +874,8 @@ int mg_selective_scan_backward(void* stream, const mg_selective_scan_backward_ar
                                    inputs_far(p) || lies_far(p.step_rows, p.dy_ld, p.type) ||
                                        lies_far(p.step_rows, p.dx_ld, p.type) ||
                                        lies_far(p.step_rows, p.ddt_ld, p.type) ||
-                                       lies_far(p.step_rows, p.dz_ld, p.type));
+                                       lies_far(p.step_rows, p.dz_ld, p.type),
+                                   true);
     uint64_t need = 0;
     mg_selective_scan_backward_workspace(p.steps, p.seqs, p.channels, p.states, p.groups, &need);
     if ((rc = check_workspace(what, p.workspace, p.workspace_bytes, need))) return rc;
