@@ -136,13 +136,14 @@ struct RowStats {
 // bank.
 //
 // Not TURNED: the contraction runs along a row in memory, and a stage is 64 bytes of every row. The
-// places of a row's four 16 bytes are exchanged by bits 1 and 2 of the row: a read of eight rows'
-// fragments (lane l holds row l % 32 and eight elements of 16, by l / 32) then meets no bank twice.
+// places of a row's four 16 bytes are exchanged by bits 2 and 3 of the row: 16 rows' parts of a
+// fragment (lane l holds row l % 32 and eight elements of 16, by l / 32), which are read at once, then
+// lie in 64 different banks.
 //
 // TURNED: it runs from row to row, and a stage is 32 rows of SIDE elements, or 16 of SIDE pairs.
 // Reads of four elements by 16 lanes that hold each other's columns (ds_read_b64_tr_b16: of 4 rows
 // x 16 columns a lane gets a column) make the same fragments; the places of 32 bytes are exchanged
-// by the row's last two bits, so that the four rows lie in different banks.
+// by the row's last two bits, so that four rows and two blocks of columns lie in different banks.
 template <class H, int SIDE, bool TURNED, bool PAIRS>
 struct HeadSide {
     typedef typename Halves<H>::x8 x8;
@@ -152,6 +153,12 @@ struct HeadSide {
     static constexpr int kRow = SIDE * 2 * kWide;  // bytes of a TURNED row
     const H* base;
     uint32_t ld, off[L], row[L];
+
+    // what exchanges a TURNED row's places: blocks of columns are their last bit, or of pairs
+    // the one before it
+    static __device__ __forceinline__ int spread(int row) {
+        return PAIRS ? (row & 1) | (row & 2) << 1 : (row & 3) << 1;
+    }
 
     // `from`: the tile's first row (or column) of `rows`
     __device__ __forceinline__ HeadSide(const HeadOperand& o, uint32_t from, uint32_t rows, int wave, int lane) {
@@ -163,11 +170,11 @@ struct HeadSide {
             if constexpr (TURNED) {
                 constexpr uint32_t kLanes = kRow / 16;  // of a row
                 row[c] = (wave * L + c) * (64 / kLanes) + lane / kLanes;
-                const uint32_t at = lane % kLanes, place = (((at >> 1 ^ (row[c] & 3)) << 1) + (at & 1)) * 8;
+                const uint32_t at = lane % kLanes, place = (((at >> 1 ^ spread(row[c])) << 1) + (at & 1)) * 8;
                 const uint32_t col = PAIRS ? (place >> 5 << 4) + (place & 15) : place;
                 off[c] = col < have ? (row[c] * ld + place) * 2 : kNowhere;
             } else {
-                const uint32_t r = (wave * L + c) * 16 + (lane >> 2), place = ((lane & 3) ^ (lane >> 3 & 3)) * 8;
+                const uint32_t r = (wave * L + c) * 16 + (lane >> 2), place = ((lane & 3) ^ (lane >> 4 & 3)) * 8;
                 row[c] = PAIRS ? place & 15 : place;  // the first of its elements
                 off[c] = r < have ? (r * ld + place) * 2 : kNowhere;
             }
@@ -196,7 +203,7 @@ struct HeadSide {
             const int block = 2 * b + (lane >> 4 & 1), chunk = PAIRS ? 2 * block + h : block;
             auto four = [&](int more) {
                 const int r = k + more;  // its last two bits are k's
-                const char* const p = at + r * kRow + ((chunk ^ (r & 3)) << 5) + ((lane & 3) << 3);
+                const char* const p = at + r * kRow + ((chunk ^ spread(r)) << 5) + ((lane & 3) << 3);
                 return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
             };
             const s16x4 lo = four(0), hi = four(4);
@@ -204,7 +211,7 @@ struct HeadSide {
         } else {
             const int row = lane & 31;
             return *reinterpret_cast<const x8*>(at + b * 2048 + row * 64 +
-                                                (((2 * h + (lane >> 5)) ^ (row >> 1 & 3)) << 4));
+                                                (((2 * h + (lane >> 5)) ^ (row >> 2 & 3)) << 4));
         }
     }
 };
