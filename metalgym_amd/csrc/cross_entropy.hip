@@ -144,7 +144,11 @@ struct RowStats {
 // Reads of four elements by 16 lanes that hold each other's columns (ds_read_b64_tr_b16: of 4 rows
 // x 16 columns a lane gets a column) make the same fragments; the places of 32 bytes are exchanged
 // by the row's last two bits, so that four rows and two blocks of columns lie in different banks.
-template <class H, int SIDE, bool TURNED, bool PAIRS>
+//
+// A matrix instruction's result leaves a lane with four of each eight rows of its first operand. So
+// that they are 16 in a row, to be stored 32 bytes and more at a time, OUTER fragments' lane 8 q + 4 h + r
+// holds row 16 h + 4 q + r.
+template <class H, int SIDE, bool TURNED, bool PAIRS, bool OUTER>
 struct HeadSide {
     typedef typename Halves<H>::x8 x8;
     typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -158,6 +162,11 @@ struct HeadSide {
     // the one before it
     static __device__ __forceinline__ int spread(int row) {
         return PAIRS ? (row & 1) | (row & 2) << 1 : (row & 3) << 1;
+    }
+
+    // and a row's places that is not TURNED: of 16 rows that are read at once four have each value
+    static __device__ __forceinline__ int shift(int row) {
+        return OUTER ? (row >> 2 & 1) | (row >> 4 & 1) << 1 : row >> 2 & 3;
     }
 
     // `from`: the tile's first row (or column) of `rows`
@@ -174,7 +183,7 @@ struct HeadSide {
                 const uint32_t col = PAIRS ? (place >> 5 << 4) + (place & 15) : place;
                 off[c] = col < have ? (row[c] * ld + place) * 2 : kNowhere;
             } else {
-                const uint32_t r = (wave * L + c) * 16 + (lane >> 2), place = ((lane & 3) ^ (lane >> 4 & 3)) * 8;
+                const uint32_t r = (wave * L + c) * 16 + (lane >> 2), place = ((lane & 3) ^ shift(r)) * 8;
                 row[c] = PAIRS ? place & 15 : place;  // the first of its elements
                 off[c] = r < have ? (r * ld + place) * 2 : kNowhere;
             }
@@ -200,18 +209,19 @@ struct HeadSide {
     static __device__ __forceinline__ x8 read(const char* at, int b, int h, int lane) {
         if constexpr (TURNED) {
             const int k = (PAIRS ? 0 : 16 * h) + 8 * (lane >> 5) + (lane >> 2 & 3);
-            const int block = 2 * b + (lane >> 4 & 1), chunk = PAIRS ? 2 * block + h : block;
+            // four columns of the 32 that a lane reads for the others
+            const int lot = (lane >> 2 & 4) | (lane & 3), quad = OUTER ? (lot & 1) * 4 + (lot >> 1) : lot;
+            const int block = 2 * b + (quad >> 2), chunk = PAIRS ? 2 * block + h : block;
             auto four = [&](int more) {
                 const int r = k + more;  // its last two bits are k's
-                const char* const p = at + r * kRow + ((chunk ^ spread(r)) << 5) + ((lane & 3) << 3);
+                const char* const p = at + r * kRow + ((chunk ^ spread(r)) << 5) + ((quad & 3) << 3);
                 return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
             };
             const s16x4 lo = four(0), hi = four(4);
             return __builtin_bit_cast(x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
-            const int row = lane & 31;
-            return *reinterpret_cast<const x8*>(at + b * 2048 + row * 64 +
-                                                (((2 * h + (lane >> 5)) ^ (row >> 2 & 3)) << 4));
+            const int m = lane & 31, row = OUTER ? (m & 4) * 4 | (m >> 1 & 12) | (m & 3) : m;
+            return *reinterpret_cast<const x8*>(at + b * 2048 + row * 64 + (((2 * h + (lane >> 5)) ^ shift(row)) << 4));
         }
     }
 };
@@ -225,8 +235,8 @@ __device__ __forceinline__ void head_product(const HeadProduct& p, uint32_t tm, 
                                              f32x16 (&acc)[MI][2]) {
     using X = Halves<H>;
     typedef typename X::x8 x8;
-    using A = HeadSide<H, MI * 64, AT, PAIRS>;
-    using B = HeadSide<H, kHeadN, BT, PAIRS>;
+    using A = HeadSide<H, MI * 64, AT, PAIRS, true>;
+    using B = HeadSide<H, kHeadN, BT, PAIRS, false>;
     constexpr int kStage = A::kBytes + B::kBytes, L = A::L + B::L, K = PAIRS ? 16 : kHeadK;
     const uint32_t from = split * p.range, to = p.k - from < p.range ? p.k : from + p.range;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1;
@@ -294,7 +304,7 @@ __device__ __forceinline__ void head_product(const HeadProduct& p, uint32_t tm, 
 
 template <class H, int KIND, int MI, bool PAIRS>
 __global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
-    typedef typename Halves<H>::x4 x4;
+    typedef typename Halves<H>::x8 x8;
     constexpr int TM = MI * 64;
     __shared__ __align__(1024) char lds[kHeadRing * (TM + kHeadN) * 64];
     const uint32_t tile_of_all = xcd_run(blockIdx.x, gridDim.x);
@@ -314,8 +324,8 @@ __global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
     else
         head_product<H, MI, PAIRS, true, false>(p, tm, tn, split, lds, acc);
 
-    // register e of tile (i, j): row of a m(i, e), row of b n(j)
-    const uint32_t m0 = tm * TM + wm * (MI * 32) + 4 * (lane >> 5), n0 = tn * kHeadN + wn * 64 + (lane & 31);
+    // register e of tile (i, j): row m0 + 32 i + e of a, row n0 + 32 j of b
+    const uint32_t m0 = tm * TM + wm * (MI * 32) + 16 * (lane >> 5), n0 = tn * kHeadN + wn * 64 + (lane & 31);
     const HeadScales sc = args.scales ? *args.scales : HeadScales{1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
     if constexpr (KIND == kGrad) {
         const float b0 = sc.g_back, b1 = p.which ? sc.x_back : sc.w_back;
@@ -324,40 +334,47 @@ __global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
             const uint32_t n = n0 + 32 * j;
             if (n >= p.n) continue;
 #pragma unroll
-            for (int i = 0; i < MI; ++i)
+            for (int i = 0; i < MI; ++i) {
+                const uint32_t m = m0 + 32 * i;
+                if (m >= p.m) continue;
+                f32x16& v = acc[i][j];
+                const uint32_t count = p.m - m;
+                if (p.parts) {  // parts_ld is a multiple of 4
+                    f32x4* const at = reinterpret_cast<f32x4*>(p.parts + ((uint64_t)split * p.n + n) * p.parts_ld + m);
 #pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    const uint32_t m = m0 + 32 * i + 2 * e;
-                    if (m >= p.m) continue;
-                    f32x4 v = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
-                    if (p.parts) {
-                        f32x4* const at = reinterpret_cast<f32x4*>(
-                            p.parts + ((uint64_t)split * p.n + n) * p.parts_ld + m);
-                        if (p.add) v += *at;
-                        *at = v;
-                        continue;
+                    for (int e = 0; e < 16; e += 4) {
+                        if ((uint32_t)e >= count) continue;
+                        f32x4 four = {v[e], v[e + 1], v[e + 2], v[e + 3]};
+                        if (p.add) four += at[e / 4];
+                        at[e / 4] = four;
                     }
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) v[q] = v[q] * b0 * b1;
-                    const uint32_t count = p.m - m;
-                    auto put = [&](auto t) {
-                        using T = decltype(t);
-                        T* const at = static_cast<T*>(p.out) + n * p.out_ld + m;
-                        if (count >= 4) {
-                            typedef T vec __attribute__((ext_vector_type(4)));
-                            const vec w = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-                            __builtin_memcpy(at, &w, sizeof(w));
-                        } else {
-#pragma unroll
-                            for (int q = 0; q < 3; ++q)
-                                if (q < (int)count) at[q] = (T)v[q];
-                        }
-                    };
-                    if constexpr (PAIRS)
-                        put(0.0f);
-                    else
-                        put(H{});
+                    continue;
                 }
+                v = v * b0 * b1;
+                auto put = [&](auto t) {
+                    using T = decltype(t);
+                    typedef T vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+                    constexpr int E = 16 / sizeof(T);
+                    T* const at = static_cast<T*>(p.out) + n * p.out_ld + m;
+                    if (count >= 16) {
+#pragma unroll
+                        for (int e = 0; e < 16; e += E) {
+                            vec w;
+#pragma unroll
+                            for (int q = 0; q < E; ++q) w[q] = (T)v[e + q];
+                            *reinterpret_cast<vec*>(at + e) = w;
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 15; ++e)
+                            if (e < (int)count) at[e] = (T)v[e];
+                    }
+                };
+                if constexpr (PAIRS)
+                    put(0.0f);
+                else
+                    put(H{});
+            }
         }
     } else {
         // logits in base 2: two factors for pairs, as their product may leave fp32's range
@@ -387,14 +404,14 @@ __global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
                     for (int i = 0; i < MI; ++i)
 #pragma unroll
                         for (int e = 0; e < 16; ++e)
-                            if (m0 + 32 * i + 8 * (e >> 2) + (e & 3) >= p.m) acc[i][j][e] = -__builtin_huge_valf();
+                            if (m0 + 32 * i + e >= p.m) acc[i][j][e] = -__builtin_huge_valf();
                 }
                 if (meets) {
 #pragma unroll
                     for (int i = 0; i < MI; ++i)
 #pragma unroll
                         for (int e = 0; e < 16; ++e)
-                            if (live && hit == (uint32_t)(32 * i + 8 * (e >> 2) + (e & 3))) args.of[n] = acc[i][j][e] * to2;
+                            if (live && hit == (uint32_t)(32 * i + e)) args.of[n] = acc[i][j][e] * to2;
                 }
                 float top = -__builtin_huge_valf();
 #pragma unroll
@@ -447,35 +464,36 @@ __global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
                     for (int i = 0; i < MI; ++i)
 #pragma unroll
                         for (int e = 0; e < 16; ++e)
-                            if (m0 + 32 * i + 8 * (e >> 2) + (e & 3) >= p.m) acc[i][j][e] = 0.0f;
+                            if (m0 + 32 * i + e >= p.m) acc[i][j][e] = 0.0f;
                 }
                 if (meets) {
 #pragma unroll
                     for (int i = 0; i < MI; ++i)
 #pragma unroll
                         for (int e = 0; e < 16; ++e)
-                            if (live && hit == (uint32_t)(32 * i + 8 * (e >> 2) + (e & 3))) acc[i][j][e] -= dl;
+                            if (live && hit == (uint32_t)(32 * i + e)) acc[i][j][e] -= dl;
                 }
 #pragma unroll
-                for (int i = 0; i < MI; ++i)
+                for (int i = 0; i < MI; ++i) {
+                    const uint32_t c = m0 + 32 * i;  // a multiple of 16: pairs' halves lie side by side
+                    H* const g = static_cast<H*>(args.g) + (uint64_t)n * args.g_ld + (PAIRS ? pair_place(c) : c);
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        const uint32_t c = m0 + 32 * i + 2 * e;
-                        x4 hi, lo;
+                    for (int e = 0; e < 16; e += 8) {
+                        x8 hi, lo;
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const float v = acc[i][j][e + q];
-                            hi[q] = (H)v;
+                        for (int q = 0; q < 8; ++q) {
                             if constexpr (PAIRS) {
                                 H h, l;
-                                split_half<H>(v, h, l);
+                                split_half<H>(acc[i][j][e + q], h, l);
                                 hi[q] = h, lo[q] = l;
+                            } else {
+                                hi[q] = (H)acc[i][j][e + q];
                             }
                         }
-                        H* const g = static_cast<H*>(args.g) + (uint64_t)n * args.g_ld + (PAIRS ? pair_place(c) : c);
-                        *reinterpret_cast<x4*>(g) = hi;
-                        if constexpr (PAIRS) *reinterpret_cast<x4*>(g + 16) = lo;
+                        *reinterpret_cast<x8*>(g + e) = hi;
+                        if constexpr (PAIRS) *reinterpret_cast<x8*>(g + 16 + e) = lo;
                     }
+                }
             }
         }
         if constexpr (KIND == kStats) {
