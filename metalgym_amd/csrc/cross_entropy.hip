@@ -62,7 +62,7 @@ enum { kStats = 0, kLogitGrad = 1, kGrad = 2 };
 // One product's tiles: M from a, N from b, contraction K in `splits` ranges of `range`.
 struct HeadProduct {
     HeadOperand a, b;
-    const uint32_t* live;  // a bit for each row of a turned a; the others count as 0. NULL: all
+    const uint32_t* live;  // dW: a bit for each row of a; the others count as 0
     uint32_t k, range, splits;
     uint32_t m, n;  // the result's sides
     uint32_t tiles_m, tiles_n;
@@ -193,15 +193,23 @@ struct HeadSide {
     __device__ __forceinline__ void load(char* at, int wave, uint32_t k, uint32_t to, uint32_t live) const {
         // a row of W or X may lie anywhere, so its stage has an address of its own
         const H* const p = base + (TURNED ? (uint64_t)k * ld : (uint64_t)k * kWide);
-        const __amdgpu_buffer_rsrc_t r =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<H*>(p), (short)0, 0x7fffffff, 0x00020000);
+        const uint64_t address = reinterpret_cast<uint64_t>(p);
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        const u32x4 r = {(uint32_t)address, (uint32_t)(address >> 32) & 0xffffu, 0x7fffffffu, 0x00020000u};
 #pragma unroll
         for (int c = 0; c < L; ++c) {
             bool in = k + row[c] < to;
             if constexpr (TURNED) in = in && (live >> row[c] & 1);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                r, (__attribute__((address_space(3))) void*)(at + (wave * L + c) * 1024), 16,
-                (int)(in ? off[c] : kNowhere), 0, 0, 0);
+            // Not the builtin: the compiler cannot tell the ring's stages apart, and would wait for all
+            // loads before each stage's first read. Nothing here comes back in a register; the
+            // loop's own waits are for LDS.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: it is in nobody else's use here
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
+                             (__attribute__((address_space(3))) char*)(at + (wave * L + c) * 1024)),
+                         "v"(in ? off[c] : kNowhere), "s"(r)
+                         : "memory", "m0");
+#pragma clang diagnostic pop
         }
     }
     // the fragment of rows 32 b ... of the tile: the stage's elements 16 h ..., or of its pairs
@@ -244,13 +252,21 @@ __device__ __forceinline__ void head_product(const HeadProduct& p, uint32_t tm, 
     const B b(p.b, tn * kHeadN, p.n, wave, lane);
     uint32_t k = from;
     const uint32_t stages = ((to - from + K - 1) / K + 1) & ~1u;  // the last may be empty
-    const uint32_t* const live = AT ? p.live : nullptr;
+    // read a stage ahead, and without a branch, which would part the loop
+    auto* const rows_live = (const __attribute__((address_space(4))) uint32_t*)p.live;
+    auto live_of = [&](uint32_t at) {
+        if constexpr (AT && BT)
+            return rows_live[(at < to ? at : to - 1) / 32];
+        else
+            return ~0u;
+    };
+    uint32_t bits = live_of(k);
     auto load = [&](uint32_t slot) {
         char* const at = lds + slot * kStage;
-        const uint32_t bits = live && k < to ? live[k / 32] >> (k & 31) : ~0u;
-        a.load(at, wave, k, to, bits);
+        a.load(at, wave, k, to, bits >> (k & 31));
         b.load(at + A::kBytes, wave, k, to, ~0u);
         k += K;
+        bits = live_of(k);
     };
     x8 fa[2][2][MI], fb[2][2][2];
     auto read = [&](int set, uint32_t slot) {
@@ -277,8 +293,8 @@ __device__ __forceinline__ void head_product(const HeadProduct& p, uint32_t tm, 
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kHeadRing - 2) * L) : "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            read(u ^ 1, (slot + 1) & (kHeadRing - 1));
             load(slot);
+            read(u ^ 1, (slot + 1) & (kHeadRing - 1));
             constexpr int kTerms = PAIRS ? 3 : 2;
 #pragma unroll
             for (int h = 0; h < kTerms; ++h) {
@@ -289,12 +305,15 @@ __device__ __forceinline__ void head_product(const HeadProduct& p, uint32_t tm, 
                     for (int j = 0; j < 2; ++j) acc[i][j] = X::mfma(fa[u][ha][i], fb[u][hb][j], acc[i][j]);
             }
             constexpr int kReads = 2 * (MI * (AT ? 2 : 1) + 2 * (BT ? 2 : 1)), kProducts = 2 * MI * kTerms;
+            // the last reads have a quarter of the products' time to arrive
+            constexpr int kCover = kProducts * 3 / 4;
 #pragma unroll
             for (int q = 0; q < kProducts; ++q) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix
-                const int n = (q + 1) * kReads / kProducts - q * kReads / kProducts;
+                const int n = q < kCover ? (q + 1) * kReads / kCover - q * kReads / kCover : 0;
                 if (n == 1) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
                 if (n == 2) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                if (n == 3) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -313,8 +332,11 @@ __global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
     uint32_t tile = tile_of_all - (sel ? args.tiles : 0);
     const uint32_t per = p.tiles_m * p.tiles_n, split = tile / per;
     tile -= split * per;
-    // tiles that share their rows of a lie side by side
-    const uint32_t tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
+    // down four tiles of m, then on by one of n: an XCD's 32 tiles at a time are 4 x 8 and share their
+    // operands in its L2
+    const uint32_t first = tile / (4 * p.tiles_n) * 4, deep = p.tiles_m - first < 4 ? p.tiles_m - first : 4;
+    tile -= first * p.tiles_n;
+    const uint32_t tn = tile / deep, tm = first + tile - tn * deep;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
     f32x16 acc[MI][2] = {};
     if constexpr (KIND != kGrad)
