@@ -932,6 +932,7 @@ constexpr uint32_t kSkew = 128;            // elements past a row: rows a power 
 constexpr uint32_t kMostPiece = 1u << 17;   // classes of one
 constexpr uint32_t kMostRange = 4096;       // contraction elements of a gradient's tile
 constexpr uint32_t kSmallRange = 512;       // and of a small one's
+constexpr uint32_t kMostTiles = 1u << 22;   // of a launch, whose threads have to stay under 2^32
 
 uint32_t up_to(uint64_t n, uint32_t m) { return (uint32_t)((n + m - 1) / m * m); }
 uint64_t padded(uint64_t bytes) { return (bytes + 255) & ~(uint64_t)255; }
@@ -959,7 +960,11 @@ bool is_small(uint32_t rows, uint32_t classes, uint32_t width, uint32_t type, bo
     const uint64_t work = (uint64_t)up_to(rows, 32) * up_to(classes, 32) * up_to(width, 32);
     const uint64_t tiles = (uint64_t)((rows + 255) / 256) * ((classes + 255) / 256);
     const bool few = work <= 1u << 29 && tiles <= (backward ? 8 : 16);
-    if (type == MG_TYPE_FP32) return rows <= 32 || work <= 1u << (backward ? 28 : 29) || (backward && few);
+    if (type == MG_TYPE_FP32) {
+        // a launch has a tile of 32 x 32 for all of W, at 256 threads
+        if (rows <= 32) return (uint64_t)classes * width <= 1ull << 33;
+        return work <= 1u << (backward ? 28 : 29) || (backward && few);
+    }
     return backward ? work <= 1u << 27 || few : few && width >= 512;
 }
 
@@ -1129,14 +1134,19 @@ int cross_entropy(hipStream_t st, const mg_cross_entropy_args& p) {
     a.scales = in.scales;
     dev::HeadProduct& m = a.p[0];
     m.a = in.w, m.b = in.x;
-    m.k = m.range = s.wide, m.splits = 1, m.m = p.classes, m.n = p.rows;
-    m.tiles_m = up_to(p.classes, kHeadM) / kHeadM, m.tiles_n = s.rows_ld / dev::kHeadN;
-    a.tiles = m.tiles_m * m.tiles_n;
+    m.k = m.range = s.wide, m.splits = 1, m.n = p.rows, m.tiles_n = s.rows_ld / dev::kHeadN;
     a.rows = p.rows, a.classes = p.classes, a.targets = p.targets, a.row_exp = s.row_exp;
-    a.stats = s.stats, a.of = s.of, a.rows_ld = s.rows_ld, a.want_entropy = p.entropy != nullptr;
-    hipLaunchKernelGGL((dev::head_kernel<H, dev::kStats, 4, kPairs>), dim3(a.tiles), dim3(512), 0, st, a);
+    a.of = s.of, a.rows_ld = s.rows_ld, a.want_entropy = p.entropy != nullptr;
+    const uint32_t tiles = up_to(p.classes, kHeadM) / kHeadM, most = kMostTiles / m.tiles_n;
+    for (uint32_t first = 0; first < tiles; first += most) {
+        m.tiles_m = tiles - first < most ? tiles - first : most;
+        a.tiles = m.tiles_m * m.tiles_n, a.first = first * kHeadM, m.m = p.classes - a.first;
+        m.a.base = static_cast<const H*>(in.w.base) + (uint64_t)a.first * in.w.ld;
+        a.stats = s.stats + (uint64_t)first * 3 * s.rows_ld;
+        hipLaunchKernelGGL((dev::head_kernel<H, dev::kStats, 4, kPairs>), dim3(a.tiles), dim3(512), 0, st, a);
+    }
     MG_HIP(hipGetLastError(), "cross entropy launch");
-    return join_tiles(st, p, s, m.tiles_m);
+    return join_tiles(st, p, s, tiles);
 }
 
 template <class T>

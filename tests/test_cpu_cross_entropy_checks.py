@@ -88,3 +88,10 @@ def test_workspaces(mg):
             assert back <= 4 * once + (1 << 30)
     with pytest.raises(CapiError):
         mg.cross_entropy_workspace(1, 0, 8)
+
+
+def test_wide_heads_of_few_rows(mg):
+    """Past 2^33 elements of W small tiles are too many for a launch: pairs of halves take their place."""
+    classes, width = 1 << 18, 1 << 15
+    assert mg.cross_entropy_workspace(8, classes, width, "fp32") < 1 << 30
+    assert mg.cross_entropy_workspace(8, classes + 1, width, "fp32") > 4 * classes * width

@@ -95,3 +95,61 @@ def test_classes_past_32_bits(mg, kind, rows, classes, width):
     for c in (2, classes // 2, classes - 2):
         ref = (dloss * (np.exp(-want) - (targets == c))) @ x
         assert np.linalg.norm(row(c) - ref) <= near * (np.linalg.norm(ref) + 1e-5), c
+
+
+def test_more_tiles_than_a_launch_takes(mg):
+    """2^20 rows of 262444 classes: 2^22 tiles of logits and more, whose threads pass 32 bits."""
+    rows, classes, width, kind = 1 << 20, (1 << 18) + 300, 16, "bf16"
+    r = np.random.RandomState(2)
+    x = rounded(r.standard_normal((rows, width)).astype(np.float32), kind)
+    w = rounded(r.standard_normal((classes, width)).astype(np.float32) * 0.5, kind)
+    targets = r.randint(0, classes, rows).astype(np.int32)
+    targets[:8] = classes - 1 - np.arange(8)
+    targets[8] = -1
+    dloss = rounded(r.standard_normal(rows).astype(np.float32), "fp32")
+    up = mg.DeviceBuffer.from_array
+    dx_, dw_, dt, dl = up(encode(x, kind)), up(encode(w, kind)), up(targets), up(dloss.astype(np.float32))
+    loss, lse, entropy = (mg.DeviceBuffer(4 * rows) for _ in range(3))
+    dx, dw = mg.DeviceBuffer(2 * rows * width), mg.DeviceBuffer(2 * classes * width)
+    space = mg.DeviceBuffer(max(mg.cross_entropy_workspace(rows, classes, width, kind),
+                                mg.cross_entropy_backward_workspace(rows, classes, width, kind)) + 256)
+    use = dict(workspace=space.ptr, workspace_bytes=space.nbytes)
+    mg.cross_entropy(dx_.ptr, dw_.ptr, dt.ptr, rows, classes, width, kind, loss=loss.ptr, lse=lse.ptr,
+                     entropy=entropy.ptr, **use)
+    mg.cross_entropy_backward(dx_.ptr, dw_.ptr, dt.ptr, rows, classes, width, kind, lse=lse.ptr, dloss=dl.ptr, dx=dx.ptr,
+                              dw=dw.ptr, **use)
+    sync(mg)
+    got = [mg.d2h(b.ptr, np.float32, (rows,)).astype(np.float64) for b in (loss, lse, entropy)]
+    some = np.concatenate([np.arange(12), [rows // 2, rows - 2, rows - 1]])
+    s = x[some] @ w.T
+    want_lse = np.log(np.exp(s).sum(1))
+    p = np.exp(s - want_lse[:, None])
+    live = targets[some] >= 0
+    want_loss = np.where(live, want_lse - s[np.arange(len(some)), np.maximum(targets[some], 0)], 0)
+    want_entropy = want_lse - (p * s).sum(1)
+    # logits: 32 products in turn, at the size of the largest row's; a lane's sums have 128 terms and
+    # meet in 20 joins; each exponential, logarithm and difference from the maximum adds a few steps of |s|
+    size = (np.abs(x[some])[:, None, :] * np.abs(w[None, :, :])).sum(2).max(1)
+    tol = 2.0**-24 * (2 * 40 * size + 256 + 16 * np.abs(want_lse))
+    assert (np.abs(got[1][some] - want_lse) <= tol).all()
+    assert (np.abs(got[0][some] - want_loss) <= 2 * tol).all()
+    # the entropy is a mean of (lse - s), off by twice as much and by its weights' relative error of `tol`
+    assert (np.abs(got[2][some] - want_entropy) <= 2 * tol * (2 + np.abs(want_entropy))).all()
+    # gradients: each g rounded to bfloat16, and the result; 2^-11 stands for the fp32 sums (4096
+    # terms at a time) and for the probabilities' own errors
+    share = 2.0**-8 + 2.0**-11
+    g = p * dloss[some][:, None]
+    g[np.arange(len(some))[live], targets[some][live]] -= dloss[some][live]
+    g[~live] = 0
+    want = g @ w
+    have = decode(mg.d2h(dx.ptr, np.uint16, (rows, width)), kind)[some]
+    assert (np.abs(have - want) <= share * (np.abs(g) @ np.abs(w)) + 2.0**-8 * np.abs(want)).all()
+    ends = np.array([0, 255, (1 << 18) - 1, 1 << 18, classes - 1])
+    p = np.exp(x @ w[ends].T - got[1][:, None])
+    g = p * dloss[:, None]
+    for k, c in enumerate(ends):
+        g[targets == c, k] -= dloss[targets == c]
+    g[targets < 0] = 0
+    want = g.T @ x
+    have = decode(mg.d2h(dw.ptr, np.uint16, (classes, width)), kind)[ends]
+    assert (np.abs(have - want) <= share * (np.abs(g).T @ np.abs(x)) + 2.0**-8 * np.abs(want)).all()
