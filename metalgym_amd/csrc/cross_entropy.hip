@@ -97,7 +97,12 @@ struct HeadArgs {
 };
 
 constexpr int kHeadK = 32;     // contraction elements of a stage, or 16 pairs
-constexpr int kHeadRing = 4;   // stages in LDS
+// Stages in LDS. Tiles of MI = 4, and all of the gradients', have a CU to themselves; logits' of MI = 2
+// share one by twos.
+template <int KIND, int MI>
+constexpr bool kByTwos = KIND != kGrad && MI == 2;
+template <int KIND, int MI>
+constexpr int kHeadRing = kByTwos<KIND, MI> ? 3 : 4;
 constexpr int kHeadN = 256;    // columns of a tile
 constexpr uint32_t kNowhere = 0x80000000u;  // an offset past every operand's end: reads 0
 
@@ -235,10 +240,11 @@ struct HeadSide {
 };
 
 // One tile of MI x 64 by 256. Eight waves, two along a and four along b, MI x 2 tiles of 32 x 32
-// each. The ring holds four stages; the waves meet once a stage, when the next has arrived,
-// and read the next one's fragments under this one's products: two of 16 elements, or of pairs
-// low high, high low and high high.
-template <class H, int MI, bool PAIRS, bool AT, bool BT>
+// each. The waves meet once a stage, when the next has arrived. With a ring of four stages they read
+// the next one's fragments under this one's products: two of 16 elements, or of pairs low high,
+// high low and high high. With three there is another workgroup on the CU, and a lane holds one
+// stage's fragments.
+template <class H, int RING, int MI, bool PAIRS, bool AT, bool BT>
 __device__ __forceinline__ void head_product(const HeadProduct& p, uint32_t tm, uint32_t tn, uint32_t split, char* lds,
                                              f32x16 (&acc)[MI][2]) {
     using X = Halves<H>;
@@ -251,7 +257,8 @@ __device__ __forceinline__ void head_product(const HeadProduct& p, uint32_t tm, 
     const A a(p.a, tm * (MI * 64), p.m, wave, lane);
     const B b(p.b, tn * kHeadN, p.n, wave, lane);
     uint32_t k = from;
-    const uint32_t stages = ((to - from + K - 1) / K + 1) & ~1u;  // the last may be empty
+    constexpr int kSets = RING == 3 ? 1 : 2, kTerms = PAIRS ? 3 : 2;  // of fragments
+    const uint32_t stages = ((to - from + K - 1) / K + kSets - 1) & ~(kSets - 1u);  // the last may be empty
     // read a stage ahead, and without a branch, which would part the loop
     auto* const rows_live = (const __attribute__((address_space(4))) uint32_t*)p.live;
     auto live_of = [&](uint32_t at) {
@@ -268,7 +275,7 @@ __device__ __forceinline__ void head_product(const HeadProduct& p, uint32_t tm, 
         k += K;
         bits = live_of(k);
     };
-    x8 fa[2][2][MI], fb[2][2][2];
+    x8 fa[kSets][2][MI], fb[kSets][2][2];
     auto read = [&](int set, uint32_t slot) {
         const char* const at = lds + slot * kStage;
 #pragma unroll
@@ -279,53 +286,72 @@ __device__ __forceinline__ void head_product(const HeadProduct& p, uint32_t tm, 
             for (int j = 0; j < 2; ++j) fb[set][h][j] = B::read(at + A::kBytes, wn * 2 + j, h, lane);
         }
     };
+    auto multiply = [&](int set) {
 #pragma unroll
-    for (uint32_t u = 0; u < (uint32_t)kHeadRing; ++u) load(u);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kHeadRing - 1) * L) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    read(0, 0);
-    for (uint32_t s = 0; s < stages; s += 2) {
+        for (int h = 0; h < kTerms; ++h) {
+            const int ha = PAIRS ? h == 0 : h, hb = PAIRS ? h == 1 : h;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const uint32_t slot = (s + u) & (kHeadRing - 1);
-            // the next stage is there, this one is in registers
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kHeadRing - 2) * L) : "memory");
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[i][j] = X::mfma(fa[set][ha][i], fb[set][hb][j], acc[i][j]);
+        }
+    };
+    if constexpr (kSets == 1) {
+        // the CU's other workgroup has the matrix units meanwhile
+#pragma unroll
+        for (uint32_t u = 0; u + 1 < (uint32_t)RING; ++u) load(u);
+        for (uint32_t s = 0, slot = 0, free = RING - 1; s < stages; ++s) {
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((RING - 2) * L) : "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            load(slot);
-            read(u ^ 1, (slot + 1) & (kHeadRing - 1));
-            constexpr int kTerms = PAIRS ? 3 : 2;
+            load(free);
+            read(0, slot);
+            multiply(0);
+            free = slot;
+            slot = slot + 1 == RING ? 0 : slot + 1;
+        }
+    } else {
 #pragma unroll
-            for (int h = 0; h < kTerms; ++h) {
-                const int ha = PAIRS ? h == 0 : h, hb = PAIRS ? h == 1 : h;
+        for (uint32_t u = 0; u < (uint32_t)RING; ++u) load(u);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RING - 1) * L) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        read(0, 0);
+        for (uint32_t s = 0; s < stages; s += 2) {
 #pragma unroll
-                for (int i = 0; i < MI; ++i)
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t slot = (s + u) & (RING - 1);
+                // the next stage is there, this one is in registers
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((RING - 2) * L) : "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                load(slot);
+                read(u ^ 1, (slot + 1) & (RING - 1));
+                multiply(u);
+                constexpr int kReads = 2 * (MI * (AT ? 2 : 1) + 2 * (BT ? 2 : 1)), kProducts = 2 * MI * kTerms;
+                // the last reads have a quarter of the products' time to arrive
+                constexpr int kCover = kProducts * 3 / 4;
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) acc[i][j] = X::mfma(fa[u][ha][i], fb[u][hb][j], acc[i][j]);
+                for (int q = 0; q < kProducts; ++q) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix
+                    const int n = q < kCover ? (q + 1) * kReads / kCover - q * kReads / kCover : 0;
+                    if (n == 1) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
+                    if (n == 2) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                    if (n == 3) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            constexpr int kReads = 2 * (MI * (AT ? 2 : 1) + 2 * (BT ? 2 : 1)), kProducts = 2 * MI * kTerms;
-            // the last reads have a quarter of the products' time to arrive
-            constexpr int kCover = kProducts * 3 / 4;
-#pragma unroll
-            for (int q = 0; q < kProducts; ++q) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix
-                const int n = q < kCover ? (q + 1) * kReads / kCover - q * kReads / kCover : 0;
-                if (n == 1) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
-                if (n == 2) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-                if (n == 3) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
-            }
-            __builtin_amdgcn_sched_barrier(0);
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last loads have left LDS alone
 }
 
 template <class H, int KIND, int MI, bool PAIRS>
-__global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
+__global__ void __launch_bounds__(512, (kByTwos<KIND, MI> ? 4 : 2)) head_kernel(const HeadArgs args) {
     typedef typename Halves<H>::x8 x8;
     constexpr int TM = MI * 64;
-    __shared__ __align__(1024) char lds[kHeadRing * (TM + kHeadN) * 64];
+    constexpr int kRing = kHeadRing<KIND, MI>;
+    __shared__ __align__(1024) char lds[kRing * (TM + kHeadN) * 64];
     const uint32_t tile_of_all = xcd_run(blockIdx.x, gridDim.x);
     const uint32_t sel = KIND == kGrad && tile_of_all >= args.tiles ? 1 : 0;
     const HeadProduct& p = args.p[sel];
@@ -340,11 +366,11 @@ __global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
     f32x16 acc[MI][2] = {};
     if constexpr (KIND != kGrad)
-        head_product<H, MI, PAIRS, false, false>(p, tm, tn, split, lds, acc);
+        head_product<H, kRing, MI, PAIRS, false, false>(p, tm, tn, split, lds, acc);
     else if (p.which)
-        head_product<H, MI, PAIRS, true, true>(p, tm, tn, split, lds, acc);
+        head_product<H, kRing, MI, PAIRS, true, true>(p, tm, tn, split, lds, acc);
     else
-        head_product<H, MI, PAIRS, true, false>(p, tm, tn, split, lds, acc);
+        head_product<H, kRing, MI, PAIRS, true, false>(p, tm, tn, split, lds, acc);
 
     // register e of tile (i, j): row m0 + 32 i + e of a, row n0 + 32 j of b
     const uint32_t m0 = tm * TM + wm * (MI * 32) + 16 * (lane >> 5), n0 = tn * kHeadN + wn * 64 + (lane & 31);
@@ -495,10 +521,15 @@ __global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
                         for (int e = 0; e < 16; ++e)
                             if (live && hit == (uint32_t)(32 * i + e)) acc[i][j][e] -= dl;
                 }
+                // by way of LDS, from where a wave stores whole rows of the tile: places of 16 bytes are
+                // exchanged by the row, whose own lie in the same banks
+                constexpr uint32_t kChunks = TM * (PAIRS ? 4 : 2) / 16;  // of a row
+                const uint32_t r = wn * 32 + (lane & 31);
+                x8* const row = reinterpret_cast<x8*>(lds) + r * kChunks;
+                __syncthreads();  // every wave is done with the ring, or the rows before
 #pragma unroll
                 for (int i = 0; i < MI; ++i) {
-                    const uint32_t c = m0 + 32 * i;  // a multiple of 16: pairs' halves lie side by side
-                    H* const g = static_cast<H*>(args.g) + (uint64_t)n * args.g_ld + (PAIRS ? pair_place(c) : c);
+                    const uint32_t c = wm * (MI * 32) + 32 * i + 16 * (lane >> 5);  // of the tile: 16 pairs, or elements
 #pragma unroll
                     for (int e = 0; e < 16; e += 8) {
                         x8 hi, lo;
@@ -512,9 +543,18 @@ __global__ void __launch_bounds__(512) head_kernel(const HeadArgs args) {
                                 hi[q] = (H)acc[i][j][e + q];
                             }
                         }
-                        *reinterpret_cast<x8*>(g + e) = hi;
-                        if constexpr (PAIRS) *reinterpret_cast<x8*>(g + 16 + e) = lo;
+                        const uint32_t chunk = (PAIRS ? c / 4 : c / 8) + e / 8;
+                        row[chunk ^ (r & 15)] = hi;
+                        if constexpr (PAIRS) row[(chunk + 2) ^ (r & 15)] = lo;
                     }
+                }
+                __syncthreads();
+                H* const g = static_cast<H*>(args.g) + (uint64_t)(tn * kHeadN + 32 * j) * args.g_ld + tm * TM * (PAIRS ? 2 : 1);
+#pragma unroll
+                for (uint32_t u = 0; u < kChunks / 4; ++u) {
+                    const uint32_t at = u * 512 + threadIdx.x, r = at / kChunks, chunk = at % kChunks;
+                    const x8 v = reinterpret_cast<const x8*>(lds)[r * kChunks + (chunk ^ (r & 15))];
+                    *reinterpret_cast<x8*>(g + (uint64_t)((r >> 5) * 64 + (r & 31)) * args.g_ld + chunk * 8) = v;
                 }
             }
         }
@@ -926,7 +966,7 @@ __global__ void __launch_bounds__(256) small_grad_kernel(const SmallArgs a) {
 namespace {
 
 constexpr uint32_t kMostHeadRows = 1u << 20, kMostClasses = 1u << 20, kMostWidth = 1u << 16;
-constexpr uint32_t kHeadM = 256;          // classes of a tile
+constexpr uint32_t kHeadM = 256;          // classes that a piece is filled up to
 constexpr uint32_t kPieceCells = 1u << 25;  // logits of a piece, about
 constexpr uint32_t kSkew = 128;            // elements past a row: rows a power of two apart meet in few memory channels
 constexpr uint32_t kMostPiece = 1u << 17;   // classes of one
@@ -972,7 +1012,7 @@ bool is_small(uint32_t rows, uint32_t classes, uint32_t width, uint32_t type, bo
 struct HeadSpace {
     bool small;
     float* small_g;
-    uint32_t tiles, wide, rows_ld, g_ld, piece, pieces, tall, splits_x, splits_w, range_x, range_w, parts_ld;
+    uint32_t tiles, wide, rows_ld, high, g_ld, piece, pieces, tall, splits_x, splits_w, range_x, range_w, parts_ld;
     uint64_t planes;
     uint16_t *x, *x_even, *w, *g;
     uint32_t* live;
@@ -1001,13 +1041,19 @@ struct HeadSpace {
         }
         planes = type == MG_TYPE_FP32 ? 2 : 1;
         wide = up_to(width, planes > 1 ? 16 : 8), rows_ld = up_to(rows, dev::kHeadN);
+        // Classes of a tile of logits. One of 128 by 256 leaves half a CU to another, whose products run
+        // under its epilogue; one of 256 by 256 reads less for each product. us, the first of the two first, 4096
+        // rows, bf16: forward of 49152 classes, width 256 162 and 170, 512 249 and 244, 1024 479 and 440, 4096
+        // 1612 and 1384; gradients of 10007 classes, 128 84 and 97, 512 221 and 233, 1024 312 and 321, of 65536
+        // 1024 1733 and 1701. Pairs as fp32 the same way: forward of 10007, 128 66 and 74, 512 149 and 158.
+        high = width <= (backward ? 512 : 256) ? 128 : 256;
         scales = c.take<dev::HeadScales>(1);
         amax = c.take<float>(3 * dev::kAmaxParts);
         row_exp = c.take<int>(planes > 1 ? rows : 0);
         x = c.take<uint16_t>(planes * rows * wide);
         w = c.take<uint16_t>(planes * classes * wide);
         if (!backward) {
-            stats = c.take<float>((uint64_t)up_to(classes, kHeadM) / kHeadM * 3 * rows_ld);
+            stats = c.take<float>((uint64_t)up_to(classes, high) / high * 3 * rows_ld);
             of = c.take<float>(rows_ld);
             bytes = c.used;
             return;
@@ -1116,6 +1162,14 @@ int join_tiles(hipStream_t st, const mg_cross_entropy_args& p, const HeadSpace& 
     return MG_OK;
 }
 
+template <class H, int KIND, bool PAIRS>
+void launch_logits(hipStream_t st, const dev::HeadArgs& a, const HeadSpace& s) {
+    if (s.high == 128)
+        hipLaunchKernelGGL((dev::head_kernel<H, KIND, 2, PAIRS>), dim3(a.tiles), dim3(512), 0, st, a);
+    else
+        hipLaunchKernelGGL((dev::head_kernel<H, KIND, 4, PAIRS>), dim3(a.tiles), dim3(512), 0, st, a);
+}
+
 template <class T>
 int cross_entropy(hipStream_t st, const mg_cross_entropy_args& p) {
     typedef typename HeadType<T>::H H;
@@ -1137,13 +1191,13 @@ int cross_entropy(hipStream_t st, const mg_cross_entropy_args& p) {
     m.k = m.range = s.wide, m.splits = 1, m.n = p.rows, m.tiles_n = s.rows_ld / dev::kHeadN;
     a.rows = p.rows, a.classes = p.classes, a.targets = p.targets, a.row_exp = s.row_exp;
     a.of = s.of, a.rows_ld = s.rows_ld, a.want_entropy = p.entropy != nullptr;
-    const uint32_t tiles = up_to(p.classes, kHeadM) / kHeadM, most = kMostTiles / m.tiles_n;
+    const uint32_t tiles = up_to(p.classes, s.high) / s.high, most = kMostTiles / m.tiles_n;
     for (uint32_t first = 0; first < tiles; first += most) {
         m.tiles_m = tiles - first < most ? tiles - first : most;
-        a.tiles = m.tiles_m * m.tiles_n, a.first = first * kHeadM, m.m = p.classes - a.first;
+        a.tiles = m.tiles_m * m.tiles_n, a.first = first * s.high, m.m = p.classes - a.first;
         m.a.base = static_cast<const H*>(in.w.base) + (uint64_t)a.first * in.w.ld;
         a.stats = s.stats + (uint64_t)first * 3 * s.rows_ld;
-        hipLaunchKernelGGL((dev::head_kernel<H, dev::kStats, 4, kPairs>), dim3(a.tiles), dim3(512), 0, st, a);
+        launch_logits<H, dev::kStats, kPairs>(st, a, s);
     }
     MG_HIP(hipGetLastError(), "cross entropy launch");
     return join_tiles(st, p, s, tiles);
@@ -1196,9 +1250,9 @@ int cross_entropy_backward(hipStream_t st, const mg_cross_entropy_backward_args&
         m.a = in.w, m.b = in.x;
         m.a.base = static_cast<const H*>(in.w.base) + (uint64_t)first * in.w.ld;
         m.k = m.range = s.wide, m.splits = 1, m.m = here, m.n = p.rows;
-        m.tiles_m = fill / kHeadM, m.tiles_n = s.rows_ld / dev::kHeadN;
+        m.tiles_m = fill / s.high, m.tiles_n = s.rows_ld / dev::kHeadN;
         a.tiles = m.tiles_m * m.tiles_n, a.first = first;
-        hipLaunchKernelGGL((dev::head_kernel<H, dev::kLogitGrad, 4, kPairs>), dim3(a.tiles), dim3(512), 0, st, a);
+        launch_logits<H, dev::kLogitGrad, kPairs>(st, a, s);
         MG_HIP(hipGetLastError(), "cross entropy logits launch");
         const dev::HeadOperand m_of_w = m.a;
         uint32_t n = 0, tiles = 0;
