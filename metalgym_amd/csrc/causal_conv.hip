@@ -313,16 +313,18 @@ struct ConvShape {
     uint32_t vectors, lanes, columns, tile, tiles;
     uint64_t groups;  // of thread rows over (sequence, tile)
 };
-ConvShape conv_shape(uint32_t steps, uint32_t seqs, uint32_t channels, uint32_t type) {
+ConvShape conv_shape(uint32_t steps, uint32_t seqs, uint32_t channels, uint32_t type, bool backward) {
     ConvShape s;
     const uint32_t e = 16 / type_bytes(type);
     s.vectors = (channels + e - 1) / e;
     for (s.lanes = 1; s.lanes < 256 && s.lanes < s.vectors;) s.lanes *= 2;
     s.columns = (s.vectors + s.lanes - 1) / s.lanes;
     s.tile = 32;
-    // a tile of 8 steps reads 3 inputs more than it needs, one of 32 as many; the shorter
-    // gives four times the threads where those of 32 steps would leave the chip idle
-    if ((uint64_t)seqs * s.vectors * ((steps + 31) / 32) < kCus * 1024) s.tile = 8;
+    // A tile of 8 steps reads 3 inputs more than it needs (and, backwards, their gradients), one of 32
+    // as many; the shorter gives four times the threads where those of 32 steps would leave the chip
+    // idle. us, 8 first: forward bf16 1000 x 64 x 256 20 and 29, 32 x 4096 x 256 35 and 34; backward 32 x
+    // 512 x 256 34 and 53, 1000 x 64 x 256 74 and 65, 32 x 4096 x 256 102 and 73.
+    if ((uint64_t)seqs * s.vectors * ((steps + 31) / 32) < kCus * (backward ? 256 : 512)) s.tile = 8;
     s.tiles = steps ? (steps + s.tile - 1) / s.tile : 1;
     const uint64_t items = (uint64_t)seqs * s.tiles, rows = 256 / s.lanes;
     s.groups = (items + rows - 1) / rows;
@@ -413,7 +415,7 @@ int mg_causal_conv(void* stream, const mg_causal_conv_args* args) {
     hipStream_t st = static_cast<hipStream_t>(stream);
     StreamDevice on;
     if ((rc = on.enter(st, "causal conv: stream device"))) return rc;
-    const ConvShape s = conv_shape(p.steps, p.seqs, p.channels, p.type);
+    const ConvShape s = conv_shape(p.steps, p.seqs, p.channels, p.type, false);
     dev::ConvArgs a{};
     a.at = {p.reset, p.lengths, p.step_rows, p.seq_rows, p.steps, p.seqs};
     a.x = p.x, a.weight = p.weight, a.bias = p.bias, a.y = p.y, a.initial = p.initial, a.final = p.final;
@@ -434,8 +436,8 @@ int mg_causal_conv_backward_workspace(uint32_t steps, uint32_t seqs, uint32_t ch
         (rc = check_taps(what, taps)))
         return rc;
     // the partial rows of whichever type has more
-    const uint32_t wide = conv_parts(conv_shape(steps, seqs, channels, MG_TYPE_FP32));
-    const uint32_t narrow = conv_parts(conv_shape(steps, seqs, channels, MG_TYPE_BF16));
+    const uint32_t wide = conv_parts(conv_shape(steps, seqs, channels, MG_TYPE_FP32, true));
+    const uint32_t narrow = conv_parts(conv_shape(steps, seqs, channels, MG_TYPE_BF16, true));
     *bytes = (uint64_t)(wide > narrow ? wide : narrow) * channels * (taps + 1) * 4;
     return MG_OK;
 }
@@ -460,7 +462,7 @@ int mg_causal_conv_backward(void* stream, const mg_causal_conv_backward_args* ar
         (rc = check_vector(what, "dweight", p.dweight, MG_TYPE_FP32, false)) ||
         (rc = check_vector(what, "dbias", p.dbias, MG_TYPE_FP32, false)))
         return rc;
-    const ConvShape s = conv_shape(p.steps, p.seqs, p.channels, p.type);
+    const ConvShape s = conv_shape(p.steps, p.seqs, p.channels, p.type, true);
     const bool sums = p.dweight || p.dbias;
     if (sums) {
         uint64_t need = 0;

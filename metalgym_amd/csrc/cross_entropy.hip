@@ -352,10 +352,11 @@ __global__ void __launch_bounds__(512, (kByTwos<KIND, MI> ? 4 : 2)) head_kernel(
     constexpr int TM = MI * 64;
     constexpr int kRing = kHeadRing<KIND, MI>;
     __shared__ __align__(1024) char lds[kRing * (TM + kHeadN) * 64];
-    const uint32_t tile_of_all = xcd_run(blockIdx.x, gridDim.x);
-    const uint32_t sel = KIND == kGrad && tile_of_all >= args.tiles ? 1 : 0;
+    // Each XCD has its share of both products, whose tiles take different times: 512 x 50000 x 512 bf16
+    // gradients 136 us, and 220 with the first XCDs' all of one product.
+    const uint32_t sel = blockIdx.x >= args.tiles ? 1 : 0;
     const HeadProduct& p = args.p[sel];
-    uint32_t tile = tile_of_all - (sel ? args.tiles : 0);
+    uint32_t tile = sel ? xcd_run(blockIdx.x - args.tiles, gridDim.x - args.tiles) : xcd_run(blockIdx.x, args.tiles);
     const uint32_t per = p.tiles_m * p.tiles_n, split = tile / per;
     tile -= split * per;
     // down four tiles of m, then on by one of n: an XCD's 32 tiles at a time are 4 x 8 and share their
@@ -967,10 +968,17 @@ namespace {
 
 constexpr uint32_t kMostHeadRows = 1u << 20, kMostClasses = 1u << 20, kMostWidth = 1u << 16;
 constexpr uint32_t kHeadM = 256;          // classes that a piece is filled up to
-constexpr uint32_t kPieceCells = 1u << 25;  // logits of a piece, about
-constexpr uint32_t kSkew = 128;            // elements past a row: rows a power of two apart meet in few memory channels
+// Logits of a piece, about: 256 MB of 16-bit gradients, as much as the last cache. us with 2^25, 2^26 and
+// 2^27: gradients of 4096 x 65536 x 128 bf16 569, 530 and 442, x 1024 1710, 1605 and 1617; 4096 x 32768 x
+// 512 fp32 1298, 1172 and 1152.
+constexpr uint32_t kPieceCells = 1u << 27;
+// Elements past a row: rows a power of two apart meet in few memory channels. 16384 x 32768 x 256 bf16 1178
+// us with them and 1263 without.
+constexpr uint32_t kSkew = 128;
 constexpr uint32_t kMostPiece = 1u << 17;   // classes of one
-constexpr uint32_t kMostRange = 4096;       // contraction elements of a gradient's tile
+// Contraction elements of a gradient's tile: more keep fewer partial sums, 8192 x 8192 x 1024 bf16 397 us with
+// 8192 and 458 with 4096; 16384 changes nothing.
+constexpr uint32_t kMostRange = 8192;
 constexpr uint32_t kSmallRange = 512;       // and of a small one's
 constexpr uint32_t kMostTiles = 1u << 22;   // of a launch, whose threads have to stay under 2^32
 
@@ -1066,6 +1074,8 @@ struct HeadSpace {
         g_ld = (uint32_t)planes * piece + kSkew;
         // The gradients' contractions, over a piece's classes and over all rows, are cut so that
         // their tiles are about as many as CUs, or of kMostRange elements where they are more.
+        // Of their tiles' two heights the lower for narrow heads, where the other is half empty (4096 x 10007 x
+        // 128 fp32 180 us, else 219); with a width of 256 it would read twice as much of G (123 us, else 142).
         tall = width > 128 ? 256 : 128;
         const uint64_t across = (width + tall - 1) / tall;
         const uint64_t work = across * (rows_ld / dev::kHeadN) * piece + across * (piece / dev::kHeadN) * rows_ld;
