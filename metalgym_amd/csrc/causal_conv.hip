@@ -121,7 +121,7 @@ struct ConvWalk {
 };
 
 // U: steps whose inputs are read ahead: four for a tile, while a single step would only repeat its
-// own reads (4096 x 512 bf16 15 us then).
+// own reads (4096 x 512 bf16 13.5 us for 12.7, 65536 x 512 182 for 173).
 template <class T, int W, int FIT, int U>
 __global__ void __launch_bounds__(256) conv_kernel(const ConvArgs a) {
     constexpr int E = 16 / sizeof(T);

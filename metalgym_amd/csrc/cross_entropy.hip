@@ -992,7 +992,6 @@ constexpr uint32_t kPieceCells = 1u << 27;
 // Elements past a row: rows a power of two apart meet in few memory channels. 16384 x 32768 x 256 bf16 1178
 // us with them and 1263 without.
 constexpr uint32_t kSkew = 128;
-constexpr uint32_t kMostPiece = 1u << 17;   // classes of one
 // Contraction elements of a gradient's tile: more keep fewer partial sums, 8192 x 8192 x 1024 bf16 397 us with
 // 8192 and 458 with 4096; 16384 changes nothing.
 constexpr uint32_t kMostRange = 8192;
@@ -1086,7 +1085,7 @@ struct HeadSpace {
         const uint32_t all = up_to(classes, kHeadM);
         pieces = (uint32_t)(((uint64_t)all * rows_ld + kPieceCells / 2) / kPieceCells);
         if (pieces > all / kMostRange) pieces = all / kMostRange;
-        if (pieces < (all + kMostPiece - 1) / kMostPiece) pieces = (all + kMostPiece - 1) / kMostPiece;
+        if (!pieces) pieces = 1;
         piece = up_to((all + pieces - 1) / pieces, kHeadM);
         g_ld = (uint32_t)planes * piece + kSkew;
         // The gradients' contractions, over a piece's classes and over all rows, are cut so that
