@@ -59,8 +59,13 @@ struct QuadLane : QuadMap<C> {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             held[u] = first + u / NS < limit ? (int)p.states - state - 16 * (u % NS) : 0;
-            a2[u] = load_states(p.a + (size_t)(first + u / NS) * p.states + state + 16 * (u % NS), held[u]) * kLog2e;
+            a2[u] = load_states(p.a + (size_t)(first + u / NS) * p.states + state + 16 * (u % NS), held[u]);
         }
+    }
+    // a2 as it is meant: apart from its loads, which the others need not wait for
+    __device__ __forceinline__ void ready() {
+#pragma unroll
+        for (int u = 0; u < U; ++u) a2[u] = a2[u] * kLog2e;
     }
     __device__ __forceinline__ size_t at(const ScanArgs& p, uint32_t n, int u) const {
         return ((size_t)n * p.channels + first + u / NS) * p.states + state + 16 * (u % NS);
@@ -83,6 +88,33 @@ __device__ __forceinline__ ArgsAgain args_again() {
     ArgsAgain p = (ArgsAgain)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(p));
     return p;
+}
+
+// An element on its way, in a register of its own: two that share one wait for their loads there, and
+// a round's then come when they are asked for instead of under the round before (32 x 4096 x 256 with 16
+// states, bf16: XXX us).
+template <class T>
+struct Raw {
+    uint32_t bits;
+    __device__ __forceinline__ operator float() const {
+        if constexpr (sizeof(T) == 2)
+            return (float)__builtin_bit_cast(T, (uint16_t)bits);
+        else
+            return __builtin_bit_cast(T, bits);
+    }
+};
+template <class T>
+__device__ __forceinline__ Raw<T> raw_at(const T* p) {
+    if constexpr (sizeof(T) == 2)
+        return Raw<T>{__builtin_bit_cast(uint16_t, *p)};
+    else
+        return Raw<T>{__builtin_bit_cast(uint32_t, *p)};
+}
+// Keeps the conversions of a round's elements behind this point.
+template <class T, int R>
+__device__ __forceinline__ void arrive(Raw<T> (&v)[R]) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) asm volatile("" : "+v"(v[j].bits));
 }
 
 // A lane's elements of a row array of one sequence, by buffer loads: the round's address, a
@@ -109,15 +141,15 @@ struct QuadRows {
         return (int)(t + QuadMap<C>::step(j) < end ? mine : kNone);
     }
     // the lane's elements of the round at t, as they lie: a conversion here would wait for each
-    __device__ __forceinline__ void load(uint32_t t, uint32_t end, T (&v)[QuadMap<C>::R]) const {
+    __device__ __forceinline__ void load(uint32_t t, uint32_t end, Raw<T> (&v)[QuadMap<C>::R]) const {
         const __amdgpu_buffer_rsrc_t r = at(t);
 #pragma unroll
         for (int j = 0; j < QuadMap<C>::R; ++j) {
             const int s = j * QuadMap<C>::P * (int)by;
             if constexpr (sizeof(T) == 2)
-                v[j] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(r, place(t, end, j), s, 0));
+                v[j].bits = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, place(t, end, j), s, 0);
             else
-                v[j] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, place(t, end, j), s, 0));
+                v[j].bits = __builtin_amdgcn_raw_buffer_load_b32(r, place(t, end, j), s, 0);
         }
     }
     __device__ __forceinline__ void store(uint32_t t, uint32_t end, const float (&v)[QuadMap<C>::R]) const {
@@ -138,7 +170,7 @@ struct QuadRows {
 template <int STEPS, class T, int SP>
 struct QuadShared {
     static constexpr int N = STEPS * SP / 256;
-    T b[N], c[N];
+    Raw<T> b[N], c[N];
     uint8_t reset;
     __device__ __forceinline__ void load(uint32_t group, uint32_t n, uint32_t t, uint32_t end) {
         const ArgsAgain p = args_again();
@@ -147,11 +179,11 @@ struct QuadShared {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const uint32_t e = threadIdx.x + i * 256, s = t + e / SP, k = e % SP;
-            b[i] = c[i] = (T)0.0f;
+            b[i] = c[i] = Raw<T>{0};
             if (s >= end || k >= states) continue;
             const uint64_t row = row0 + s * by;
-            b[i] = static_cast<const T*>(p->b)[row * p->b_ld + (size_t)group * states + k];
-            c[i] = static_cast<const T*>(p->c)[row * p->c_ld + (size_t)group * states + k];
+            b[i] = raw_at(static_cast<const T*>(p->b) + row * p->b_ld + (size_t)group * states + k);
+            c[i] = raw_at(static_cast<const T*>(p->c) + row * p->c_ld + (size_t)group * states + k);
         }
         const uint32_t lane = threadIdx.x & 63;
         const uint8_t* const resets = p->at.reset;
@@ -191,7 +223,7 @@ __device__ __forceinline__ void quad_join(const ScanArgs& p, const QuadLane<C, N
 // it is, and so have lanes without a channel.
 template <int C, class T>
 __device__ __forceinline__ void quad_rates(bool in, uint32_t t, uint32_t end, float bias,
-                                           const T (&dt)[QuadMap<C>::R], const T (&x)[QuadMap<C>::R],
+                                           const Raw<T> (&dt)[QuadMap<C>::R], const Raw<T> (&x)[QuadMap<C>::R],
                                            float (&delta)[QuadMap<C>::R], float (&u)[QuadMap<C>::R]) {
 #pragma unroll
     for (int j = 0; j < QuadMap<C>::R; ++j) {
@@ -214,15 +246,13 @@ __global__ void __launch_bounds__(256, NS > 2 ? 2 : 4) scan_quad_kernel(const Sc
     __shared__ __align__(16) float sb[2][kWindow * SP], sc[2][kWindow * SP];
     for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const ScanItem it(p, item);
-        const Lane at(p, it.block);
+        Lane at(p, it.block);
         const uint32_t n = it.n, length = p.at.length(n), begin = it.split * p.split_steps;
         uint32_t end = begin + p.split_steps;
         end = end < length ? end : length;
         f32x4 h[Lane::U] = {};
         if constexpr (FULL) {
             if (p.initial) at.load(p, p.splits > 1 ? p.saved : p.initial, n, h);
-#pragma unroll 2
-            for (uint32_t k = 0; k < it.split; ++k) quad_join(p, at, n, k, h);
         } else if (it.split == 0 && p.initial) {
             f32x4 first[Lane::U];
             at.load(p, p.initial, n, first);
@@ -231,7 +261,7 @@ __global__ void __launch_bounds__(256, NS > 2 ? 2 : 4) scan_quad_kernel(const Sc
         const float bias = p.dt_bias ? p.dt_bias[at.own] : 0.0f, skip = FULL && p.d ? p.d[at.own] : 0.0f;
         float sum[C] = {};
         bool begun = false;
-        T x[R], dt[R], z[R];
+        Raw<T> x[R], dt[R], z[R];
         auto fetch = [&](uint32_t t) {
             const ArgsAgain q = args_again();
             QuadRows<T, C>(q, at, q->x, q->x_ld, n).load(t, end, x);
@@ -242,6 +272,11 @@ __global__ void __launch_bounds__(256, NS > 2 ? 2 : 4) scan_quad_kernel(const Sc
         if (begin < end) {
             shared.load(at.group, n, begin, end);
             fetch(begin);
+        }
+        at.ready();
+        if constexpr (FULL) {
+#pragma unroll 2
+            for (uint32_t k = 0; k < it.split; ++k) quad_join(p, at, n, k, h);
         }
         __syncthreads();  // the item before is done with LDS
         if (begin < end) shared.put(sb[0], sc[0]);
@@ -257,10 +292,11 @@ __global__ void __launch_bounds__(256, NS > 2 ? 2 : 4) scan_quad_kernel(const Sc
             const float* c_at = sc[turn] + at.state;
             for (uint32_t t = w; t < until; t += kSteps, resets >>= kSteps) {
                 float delta[R], u[R];
-                T was[R], gate[R];
+                Raw<T> was[R], gate[R];
+                arrive(x), arrive(dt);
                 quad_rates<C>(at.in, t, end, bias, dt, x, delta, u);
 #pragma unroll
-                for (int j = 0; j < R; ++j) was[j] = x[j], gate[j] = FULL && Z ? z[j] : (T)0.0f;
+                for (int j = 0; j < R; ++j) was[j] = x[j], gate[j] = FULL && Z ? z[j] : Raw<T>{0};
                 if (t + kSteps < end) fetch(t + kSteps);
                 if (FULL && p.checkpoints && t % kChunk == 0)
                     at.store(p, p.checkpoints + (size_t)(t / kChunk) * p.at.seqs * p.channels * p.states, n, h);
@@ -333,7 +369,8 @@ __global__ void __launch_bounds__(256) scan_quad_ends_backward_kernel(const Scan
     __shared__ __align__(16) float sb[kWindow * SP], sc[kWindow * SP];
     for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const ScanItem it(p, item);
-        const Lane at(p, it.block);
+        Lane at(p, it.block);
+        at.ready();
         const uint32_t n = it.n, length = p.at.length(n), split = it.split + 1, begin = split * p.split_steps;
         uint32_t end = begin + p.split_steps;
         end = end < length ? end : length;
@@ -352,7 +389,7 @@ __global__ void __launch_bounds__(256) scan_quad_ends_backward_kernel(const Scan
             begun |= resets != 0;
             for (int r = (int)((to - from + kSteps - 1) / kSteps); r--;) {
                 const uint32_t t = from + r * kSteps;
-                T dt[R], z[R], dy[R];
+                Raw<T> dt[R], z[R], dy[R];
                 float delta[R], none[R], into[R];
                 const ArgsAgain q = args_again();
                 QuadRows<T, C>(q, at, q->dt, q->dt_ld, n).load(t, to, dt);
@@ -428,7 +465,8 @@ __global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanAr
     __shared__ float sums[2][kSteps][4][2 * SP];  // each wave's for dB and dC
     const uint32_t block = blockIdx.x % p.blocks, part = blockIdx.x / p.blocks;
     const int wave = threadIdx.x >> 6;
-    const Lane at(p, block);
+    Lane at(p, block);
+    at.ready();
     const float skip = p.d ? p.d[at.own] : 0.0f, bias = p.dt_bias ? p.dt_bias[at.own] : 0.0f;
     f32x4 da[U] = {};
     float dd = 0.0f, dbias = 0.0f;
@@ -453,7 +491,7 @@ __global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanAr
                 at.load(p, p.kept + chunk / kChunk * cells * p.states, n, h);
             else if (!chunk && p.initial)
                 at.load(p, p.initial, n, h);
-            T x[R], dt[R], dy[R], z[R];
+            Raw<T> x[R], dt[R], dy[R], z[R];
             auto fetch = [&](uint32_t t, uint32_t last, bool all) {
                 const ArgsAgain q = args_again();
                 QuadRows<T, C>(q, at, q->x, q->x_ld, n).load(t, last, x);
@@ -476,6 +514,7 @@ __global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanAr
                 for (int r = 0; r < walk; ++r) {
                     const uint32_t t = w + r * kSteps;
                     float delta[R], u[R];
+                    arrive(x), arrive(dt);
                     quad_rates<C>(at.in, t, last, bias, dt, x, delta, u);
                     if (t + kSteps < last) fetch(t + kSteps, last, w == from && r + 1 == walk);
                     if (w == from) {
@@ -495,6 +534,8 @@ __global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanAr
             for (int r = rounds; r--; turn ^= 1) {
                 const uint32_t t = from + r * kSteps;
                 float delta[R], u[R], into[R];  // dy before the gate
+                arrive(x), arrive(dt), arrive(dy);
+                if constexpr (Z) arrive(z);
                 if (r + 1 < rounds) {
 #pragma unroll
                     for (int j = 0; j < R; ++j) delta[j] = rates[r][j][threadIdx.x], u[j] = delta[j] * (float)x[j];
@@ -587,9 +628,9 @@ __global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanAr
                         if (Z) y[j] = quad_sums(part_y);
                     }
                 }
-                T x0[R], dt0[R], dy0[R], z0[R];
+                Raw<T> x0[R], dt0[R], dy0[R], z0[R];
 #pragma unroll
-                for (int j = 0; j < R; ++j) x0[j] = x[j], dt0[j] = dt[j], dy0[j] = dy[j], z0[j] = Z ? z[j] : (T)0.0f;
+                for (int j = 0; j < R; ++j) x0[j] = x[j], dt0[j] = dt[j], dy0[j] = dy[j], z0[j] = Z ? z[j] : Raw<T>{0};
                 if (r) fetch(t - kSteps, to, true);
 #pragma unroll
                 for (int j = 0; j < R; ++j) {
@@ -652,7 +693,8 @@ __global__ void __launch_bounds__(256) scan_quad_step_kernel(const ScanArgs p, u
     typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
     for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const uint32_t n0 = (uint32_t)(item / p.blocks) * 4;
-        const Lane at(p, (uint32_t)(item % p.blocks));
+        Lane at(p, (uint32_t)(item % p.blocks));
+        at.ready();
         const uint32_t last = p.at.seqs - 1;
         const float skip = p.d ? p.d[at.own] : 0.0f, bias = p.dt_bias ? p.dt_bias[at.own] : 0.0f;
         f32x4 h[4][NS], b[4][NS], c[4][NS];

@@ -17,7 +17,7 @@ struct Rollout {
     __device__ __forceinline__ uint64_t row(uint32_t t, uint32_t n) const { return t * step_rows + n * seq_rows; }
     __device__ __forceinline__ uint32_t length(uint32_t n) const {
         if (!lengths) return steps;
-        const uint32_t l = lengths[n];
+        const uint32_t l = ((const __attribute__((address_space(4))) uint32_t*)lengths)[n];  // nobody writes it meanwhile
         return l < steps ? l : steps;
     }
 };
