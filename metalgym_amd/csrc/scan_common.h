@@ -50,6 +50,33 @@ struct ScanArgs {
     uint32_t splits, split_steps;
 };
 
+// An element on its way, in a register of its own. Two of 16 bits that share one wait for their loads as
+// they are put together, and a round's then do not come under the round before: 32 steps of 4096 x 256
+// with 16 states, bf16, took 167 us for 161, the gradients 725 for 611.
+template <class T>
+struct Raw {
+    uint32_t bits;
+    __device__ __forceinline__ operator float() const {
+        if constexpr (sizeof(T) == 2)
+            return (float)__builtin_bit_cast(T, (uint16_t)bits);
+        else
+            return __builtin_bit_cast(T, bits);
+    }
+};
+template <class T>
+__device__ __forceinline__ Raw<T> raw_at(const T* p) {
+    if constexpr (sizeof(T) == 2)
+        return Raw<T>{__builtin_bit_cast(uint16_t, *p)};
+    else
+        return Raw<T>{__builtin_bit_cast(uint32_t, *p)};
+}
+// Keeps the conversions of a round's elements behind this point.
+template <class T, int R>
+__device__ __forceinline__ void arrive(Raw<T> (&v)[R]) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) asm volatile("" : "+v"(v[j].bits));
+}
+
 // Four consecutive states of a channel; past `count` 0, or not written.
 __device__ __forceinline__ f32x4 load_states(const float* p, int count) {
     typedef float near __attribute__((ext_vector_type(4), aligned(4)));

@@ -90,33 +90,6 @@ __device__ __forceinline__ ArgsAgain args_again() {
     return p;
 }
 
-// An element on its way, in a register of its own: two that share one wait for their loads there, and
-// a round's then come when they are asked for instead of under the round before (32 x 4096 x 256 with 16
-// states, bf16: XXX us).
-template <class T>
-struct Raw {
-    uint32_t bits;
-    __device__ __forceinline__ operator float() const {
-        if constexpr (sizeof(T) == 2)
-            return (float)__builtin_bit_cast(T, (uint16_t)bits);
-        else
-            return __builtin_bit_cast(T, bits);
-    }
-};
-template <class T>
-__device__ __forceinline__ Raw<T> raw_at(const T* p) {
-    if constexpr (sizeof(T) == 2)
-        return Raw<T>{__builtin_bit_cast(uint16_t, *p)};
-    else
-        return Raw<T>{__builtin_bit_cast(uint32_t, *p)};
-}
-// Keeps the conversions of a round's elements behind this point.
-template <class T, int R>
-__device__ __forceinline__ void arrive(Raw<T> (&v)[R]) {
-#pragma unroll
-    for (int j = 0; j < R; ++j) asm volatile("" : "+v"(v[j].bits));
-}
-
 // A lane's elements of a row array of one sequence, by buffer loads: the round's address, a
 // step's distance and the lane's own bytes (the host has made sure that eight steps fit 31
 // bits). As pointers each array took two registers a lane, and the backward pass kept its own
@@ -234,7 +207,7 @@ __device__ __forceinline__ void quad_rates(bool in, uint32_t t, uint32_t end, fl
 }
 
 // As scan_kernel. A state's step is a product, an exponential at half rate and three multiply-adds,
-// six issues of a wave: 32 steps of 4096 x 256 with 16 states, bf16 take 176 us, of which those issues
+// six issues of a wave: 32 steps of 4096 x 256 with 16 states, bf16 take 163 us, of which those issues
 // are 89 and the 479 MB would be 94, only partly under each other. Four waves a SIMD (two where a lane
 // has 16 states: three spill 54 registers, 32 x 4096 x 128 of 64 states, fp16 384 us for 291): five spill,
 // 201 us.
@@ -452,9 +425,10 @@ __device__ __forceinline__ void quad_step(const QuadLane<C, NS>& at, const float
 // As scan_backward_kernel, 32 steps at a time: their states every kSteps steps wait in LDS,
 // each lane's own. The second half of a chunk walks over the first to its own first state.
 // The decays are worked out twice: to keep them beside the states would take the registers of
-// a wave a SIMD. 32 steps of 4096 x 256 with 16 states, bf16: 723 us, where 688 MB are 135; the vector
-// units issue in 71 of 100 cycles, about 21 times a state's step (three walks over its decay, ten
-// products of the gradient itself), from two waves a SIMD, as many as 235 registers leave.
+// a wave a SIMD. 32 steps of 4096 x 256 with 16 states, bf16: 611 us, where 688 MB are 135; the vector
+// units issue most of the time, about 21 times a state's step (three walks over its decay, ten
+// products of the gradient itself) and for the sums over channels, from two waves a SIMD, as many as
+// 241 registers leave. Elements asked for half a round sooner changed nothing.
 template <class T, int C, int NS, bool Z>
 __global__ void __launch_bounds__(256, 2) scan_quad_backward_kernel(const ScanArgs p, uint32_t parts) {
     using Lane = QuadLane<C, NS>;

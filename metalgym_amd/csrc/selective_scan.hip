@@ -9,7 +9,7 @@
 // once, and the eight steps then run from LDS and registers.
 //
 // What it costs is a v_exp (half the rate) and four products for each state and step: 16001 steps of
-// 512 channels with 64 states take 298 us, 100 of them for the splits' ends (see below), where the
+// 512 channels with 64 states take 283 us, 95 of them for the splits' ends (see below), where the
 // bytes would take 10. Where there are few sequences the steps are split over workgroups: a first
 // launch takes each split from a state of zero to its end, a second joins the splits before
 // its own (a split's decay is exp(A sum of delta)) and walks over its steps again.
@@ -60,15 +60,24 @@ struct ScanRound {
 };
 
 // A thread's elements of a round: the same channel of every few steps. They stay as they
-// lie until they are used: a conversion waits for its load.
-template <class T, int L>
+// lie until they are used: a conversion waits for its load. RAW: in registers of their own, for the
+// gradients of 16-bit types (32 x 4096 x 256 with 4 states, bf16 959 us without, so 824); the forward
+// pass has more waves from fewer registers (the same shape 136 us, and 151 with them).
+template <class T, int L, bool RAW>
 struct ScanFetch {
+    using E = std::conditional_t<RAW, Raw<T>, T>;
     using Lane = ScanLane<L>;
     static constexpr int N = (kSteps * Lane::CH + 255) / 256;
     static constexpr int NB = (kSteps * Lane::SP + 255) / 256;
-    T x[N], dt[N], z[N], dy[N], b[NB], c[NB];
+    E x[N], dt[N], z[N], dy[N], b[NB], c[NB];
     uint8_t reset;
 
+    static __device__ __forceinline__ E take(const T* p) {
+        if constexpr (RAW)
+            return raw_at(p);
+        else
+            return *p;
+    }
     static __device__ __forceinline__ int step(int i) { return (threadIdx.x + i * 256) / Lane::CH; }
     static __device__ __forceinline__ int slot(int i) { return threadIdx.x + i * 256; }
     static __device__ __forceinline__ uint32_t channel(const Lane& at) {
@@ -84,29 +93,30 @@ struct ScanFetch {
         const uint32_t ch = channel(at);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            x[i] = dt[i] = z[i] = dy[i] = (T)0.0f;
+            x[i] = dt[i] = z[i] = dy[i] = E{};
             if (!in(at, i, t, end)) continue;
             const uint64_t row = p.at.row(t + step(i), n);
-            x[i] = static_cast<const T*>(p.x)[row * p.x_ld + ch];
-            dt[i] = static_cast<const T*>(p.dt)[row * p.dt_ld + ch];
-            if (p.z) z[i] = static_cast<const T*>(p.z)[row * p.z_ld + ch];
-            if (DY) dy[i] = static_cast<const T*>(p.dy)[row * p.dy_ld + ch];
+            x[i] = take(static_cast<const T*>(p.x) + row * p.x_ld + ch);
+            dt[i] = take(static_cast<const T*>(p.dt) + row * p.dt_ld + ch);
+            if (p.z) z[i] = take(static_cast<const T*>(p.z) + row * p.z_ld + ch);
+            if (DY) dy[i] = take(static_cast<const T*>(p.dy) + row * p.dy_ld + ch);
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             const int e = threadIdx.x + i * 256, k = e / Lane::SP, s = e % Lane::SP;
-            b[i] = c[i] = (T)0.0f;
+            b[i] = c[i] = E{};
             if (e >= kSteps * Lane::SP || t + k >= end || s >= (int)p.states) continue;
             const uint64_t row = p.at.row(t + k, n);
-            b[i] = static_cast<const T*>(p.b)[row * p.b_ld + (size_t)at.group * p.states + s];
-            c[i] = static_cast<const T*>(p.c)[row * p.c_ld + (size_t)at.group * p.states + s];
+            b[i] = take(static_cast<const T*>(p.b) + row * p.b_ld + (size_t)at.group * p.states + s);
+            c[i] = take(static_cast<const T*>(p.c) + row * p.c_ld + (size_t)at.group * p.states + s);
         }
         reset = 0;
         if (p.at.reset && threadIdx.x < kSteps && t + threadIdx.x < end) reset = p.at.reset[p.at.row(t + threadIdx.x, n)];
     }
     // Steps past the end have delta 0: they leave the state as it is.
     __device__ __forceinline__ void put(const ScanArgs& p, const Lane& at, uint32_t t, uint32_t end,
-                                        ScanRound<L>& to) const {
+                                        ScanRound<L>& to) {
+        if constexpr (RAW) arrive(x), arrive(dt), arrive(b), arrive(c);
         const uint32_t ch = channel(at);
         const float bias = p.dt_bias && ch < at.limit ? p.dt_bias[ch] : 0.0f;
 #pragma unroll
@@ -153,7 +163,7 @@ __device__ __forceinline__ f32x4 join_before(const ScanArgs& p, const ScanLane<L
 template <class T, int L, bool FULL>
 __global__ void __launch_bounds__(256) scan_kernel(const ScanArgs p, uint64_t items) {
     using Lane = ScanLane<L>;
-    using Fetch = ScanFetch<T, L>;
+    using Fetch = ScanFetch<T, L, false>;
     __shared__ ScanRound<L> rounds[2];
     __shared__ float out[2][kSteps * Lane::CH];
     const int mine = threadIdx.x / L, sub = threadIdx.x % L;
@@ -284,7 +294,7 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const ScanArgs p, uint64
 template <class T, int L>
 __global__ void __launch_bounds__(256) scan_ends_backward_kernel(const ScanArgs p, uint64_t items) {
     using Lane = ScanLane<L>;
-    using Fetch = ScanFetch<T, L>;
+    using Fetch = ScanFetch<T, L, false>;
     __shared__ ScanRound<L> r;
     const int mine = threadIdx.x / L, sub = threadIdx.x % L;
     for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
@@ -342,7 +352,7 @@ struct BackwardShared {
 template <class T, int L>
 __global__ void __launch_bounds__(256) scan_backward_kernel(const ScanArgs p, uint32_t parts) {
     using Lane = ScanLane<L>;
-    using Fetch = ScanFetch<T, L>;
+    using Fetch = ScanFetch<T, L, sizeof(T) == 2>;
     __shared__ BackwardShared<L> s;
     const int mine = threadIdx.x / L, sub = threadIdx.x % L, wave = threadIdx.x >> 6;
     const uint32_t block = blockIdx.x % p.blocks, part = blockIdx.x / p.blocks;
@@ -562,8 +572,8 @@ struct ScanShape {
 // of 256 channels with 16 states, bf16, split and not, us: 16 sequences 55 and 215, 64 160 and 214, 100
 // 239 and 256, 128, which are 512 workgroups, 294 and 280; backwards 150 and 731, 529 and 792, 913
 // and 964, 1074 and 965). Quads take
-// 9 to 64 states (32 steps of 4096 x 256 with 16, bf16: 265 us without them, so 176; the gradient
-// 1170 and 720), but not rows whose steps lie too far apart for 31 bits, nor the gradient of more than
+// 9 to 64 states (32 steps of 4096 x 256 with 16, bf16: 265 us without them, so 163; the gradient
+// 1170 and 611), but not rows whose steps lie too far apart for 31 bits, nor the gradient of more than
 // 32 (a lane's registers). Two channels each where 16 states leave four workgroups a CU (the same
 // with one: 195 and 760).
 ScanShape scan_shape(uint32_t steps, uint32_t seqs, uint32_t channels, uint32_t states, uint32_t groups, bool far,
