@@ -13,11 +13,11 @@
 // halves at a power of two (22 bits), and their product three: low high + high low + high high, one
 // after the other.
 //
-// Matrix instructions bound it. bf16, 4095 x 50001 x 1024: forward 412 us, 1020 TFLOP/s;
+// Matrix instructions bound it. bf16, 4095 x 50001 x 1024: forward 412 to 432 us on different cards, 970 to 1020 TFLOP/s;
 // 4096 x 49152 x 4096 1190, and 8192 cubed as a library product 1387. Its gradients of 4096 x 65536 x
-// 1024 take 1620 us, 1010 TFLOP/s: an epilogue of about 10 us follows 30 us of products for each tile
+// 1024 take 1617 to 1652 us, 1000 to 1020 TFLOP/s: an epilogue of about 10 us follows 30 us of products for each tile
 // of logits, and in the loop the products alone, without loads or LDS reads, take four fifths of the
-// time. fp32 gradients of 4096 x 10007 x 128 take 155 us, 70 for logits and G, whose products are 8
+// time. fp32 gradients of 4096 x 10007 x 128 take 153 to 165 us, 70 for logits and G, whose products are 8
 // stages a tile, and 80 for the two products.
 #include <type_traits>
 

@@ -9,7 +9,7 @@
 // once, and the eight steps then run from LDS and registers.
 //
 // What it costs is a v_exp (half the rate) and four products for each state and step: 16001 steps of
-// 512 channels with 64 states take 283 us, 95 of them for the splits' ends (see below), where the
+// 512 channels with 64 states take 285 us, 95 of them for the splits' ends (see below), where the
 // bytes would take 10. Where there are few sequences the steps are split over workgroups: a first
 // launch takes each split from a state of zero to its end, a second joins the splits before
 // its own (a split's decay is exp(A sum of delta)) and walks over its steps again.
@@ -572,10 +572,10 @@ struct ScanShape {
 // of 256 channels with 16 states, bf16, split and not, us: 16 sequences 55 and 215, 64 160 and 214, 100
 // 239 and 256, 128, which are 512 workgroups, 294 and 280; backwards 150 and 731, 529 and 792, 913
 // and 964, 1074 and 965). Quads take
-// 9 to 64 states (32 steps of 4096 x 256 with 16, bf16: 265 us without them, so 163; the gradient
-// 1170 and 611), but not rows whose steps lie too far apart for 31 bits, nor the gradient of more than
+// 9 to 64 states (32 steps of 4096 x 256 with 16, bf16: 251 us without them, so 165; the gradient
+// 983 and 611), but not rows whose steps lie too far apart for 31 bits, nor the gradient of more than
 // 32 (a lane's registers). Two channels each where 16 states leave four workgroups a CU (the same
-// with one: 195 and 760).
+// with one: 198 and 791).
 ScanShape scan_shape(uint32_t steps, uint32_t seqs, uint32_t channels, uint32_t states, uint32_t groups, bool far,
                      bool backward) {
     ScanShape s;
