@@ -555,6 +555,7 @@ __global__ void __launch_bounds__(256) scan_shared_kernel(const ScanArgs p) {
 namespace {
 
 constexpr uint32_t kMostStates = 256;
+static_assert(dev::kChunk == MG_SCAN_CHUNK, "the states that callers keep room for");
 constexpr uint64_t kMostGroups = 1u << 20;  // workgroups of a launch
 
 uint32_t lanes_of(uint32_t states) {
