@@ -1045,6 +1045,7 @@ struct HeadSpace {
     dev::HeadScales* scales;
     uint64_t bytes;
 
+    static uint32_t ranges(uint32_t k, uint32_t range) { return range ? (k + range - 1) / range : 0; }
     HeadSpace(void* base, uint32_t rows, uint32_t classes, uint32_t width, uint32_t type, bool backward) {
         Carve c{static_cast<char*>(base)};
         small = is_small(rows, classes, width, type, backward);
@@ -1102,10 +1103,12 @@ struct HeadSpace {
             splits = (k + most / 2) / most;
             if (!splits) splits = 1;
             range = up_to((k + splits - 1) / splits, dev::kHeadK);
-            if (k) splits = (k + range - 1) / range;
         };
         cut(piece, splits_x, range_x);
         cut(rows_ld, splits_w, range_w);
+        // What is launched, kept and summed are the ranges of what there is: the last of a filled-up piece may
+        // hold nothing else. The first piece is the longest.
+        splits_x = ranges(classes < piece ? classes : piece, range_x), splits_w = ranges(rows, range_w);
         parts_ld = up_to(width, 4);
         x_even = c.take<uint16_t>(planes > 1 ? planes * rows * wide : 0);
         live = c.take<uint32_t>(rows_ld / 32);
@@ -1289,7 +1292,7 @@ int cross_entropy_backward(hipStream_t st, const mg_cross_entropy_backward_args&
             dev::HeadProduct& q = a.p[n++];
             q = {};
             q.a = m_of_w, q.b = {s.g, s.g_ld}, q.m = p.width, q.n = p.rows;
-            q.k = here, q.range = s.range_x, q.splits = (here + s.range_x - 1) / s.range_x;
+            q.k = here, q.range = s.range_x, q.splits = s.ranges(here, s.range_x);
             q.tiles_m = tiles_m, q.tiles_n = s.rows_ld / dev::kHeadN;
             q.out = p.dx, q.out_ld = p.dx_ld, q.parts = parts_x ? s.parts_x : nullptr, q.parts_ld = s.parts_ld;
             q.add = first != 0, q.which = 0;
@@ -1299,7 +1302,7 @@ int cross_entropy_backward(hipStream_t st, const mg_cross_entropy_backward_args&
             dev::HeadProduct& q = a.p[n++];
             q = {};
             q.a = in.x_even, q.b = {s.g, s.g_ld}, q.m = p.width, q.n = here, q.live = s.live;
-            q.k = p.rows, q.range = s.range_w, q.splits = (p.rows + s.range_w - 1) / s.range_w;
+            q.k = p.rows, q.range = s.range_w, q.splits = s.splits_w;
             q.tiles_m = tiles_m, q.tiles_n = fill / dev::kHeadN;
             q.out = static_cast<T*>(p.dw) + (uint64_t)first * p.dw_ld, q.out_ld = p.dw_ld;
             q.parts = parts_w ? s.parts_w : nullptr, q.parts_ld = s.parts_ld, q.which = 1;
@@ -1314,7 +1317,7 @@ int cross_entropy_backward(hipStream_t st, const mg_cross_entropy_backward_args&
         MG_HIP(hipGetLastError(), "cross entropy gradients launch");
         if (p.dw && parts_w)
             hipLaunchKernelGGL(dev::head_sum_kernel<T>, copy_grid(p.width, here), dim3(256), 0, st, s.parts_w,
-                               a.p[n - 1].splits, here, p.width, s.parts_ld,
+                               s.splits_w, here, p.width, s.parts_ld,
                                static_cast<T*>(p.dw) + (uint64_t)first * p.dw_ld, p.dw_ld, a.scales, 1u);
     }
     if (p.dx && parts_x)

@@ -25,4 +25,18 @@ def mg():
     import metalgym_amd
 
     metalgym_amd.lib()
+    fill_new_memory(metalgym_amd)
     return metalgym_amd
+
+
+def fill_new_memory(mg):
+    """Device memory that a test asks for holds 0xFF bytes, NaN in every float type: fresh memory is often zeros,
+    which hide what is read before it is written (a workspace needs no clearing)."""
+    make = mg.DeviceBuffer.__init__
+
+    def filled(self, nbytes):
+        make(self, nbytes)
+        mg._capi.check(mg.lib().mg_memset(self.ptr, 0xFF, self.nbytes))
+        mg._capi.check(mg.lib().mg_synchronize())
+
+    mg.DeviceBuffer.__init__ = filled
