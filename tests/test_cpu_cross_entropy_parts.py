@@ -72,3 +72,11 @@ def test_many_shapes(launches):
         check(shape, words)
         parts += any(w.startswith("dx=") for w in words)
     assert parts > len(shapes) // 4
+
+
+def test_pieces(launches):
+    """How many pieces tests/test_gpu_cross_entropy_pieces.py takes, so that it keeps testing several."""
+    shapes = [(t, *s) for t in (FP32, BF16) for s in ((9000, 24001, 24), (8200, 40500, 24), (16384, 139310, 16))]
+    counts = [[int(w[3:]) for w in words if w.startswith("dx+")] for words in launches(shapes)]
+    assert [len(c) for c in counts] == [2, 3, 17] * 2
+    assert all(c[-1] < c[0] for c in counts[2::3])
