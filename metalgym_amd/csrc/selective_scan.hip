@@ -575,8 +575,10 @@ struct ScanShape {
 // and 964, 1074 and 965). Quads take
 // 9 to 64 states (32 steps of 4096 x 256 with 16, bf16: 251 us without them, so 165; the gradient
 // 983 and 611), but not rows whose steps lie too far apart for 31 bits, nor the gradient of more than
-// 32 (a lane's registers). Two channels each where 16 states leave four workgroups a CU (the same
-// with one: 198 and 791).
+// 32 (a lane's registers). Two channels each where 16 states leave four workgroups a CU without a split (the
+// same with one: 198 and 791), but not where that leaves more lanes without a channel, backwards a third more: us
+// of 32 x 4096 bf16 with one and two, 64 channels 46 and 76, 256 in four groups 164 and 260, 160 in one 108 and
+// 135; backwards 193 and 279, 768 and 1109, 598 and 573.
 ScanShape scan_shape(uint32_t steps, uint32_t seqs, uint32_t channels, uint32_t states, uint32_t groups, bool far,
                      bool backward) {
     ScanShape s;
@@ -596,7 +598,8 @@ ScanShape scan_shape(uint32_t steps, uint32_t seqs, uint32_t channels, uint32_t 
     s.splits = units ? (units + each - 1) / each : 1;
     s.split_steps = each * dev::kChunk;
     const uint32_t pairs = (s.per + 127) / 128;
-    if (s.wide && s.lanes == 4 && (uint64_t)pairs * groups * seqs * s.splits >= 4 * kCus)
+    const bool filled = 6 * pairs <= (backward ? 4 : 3) * s.apiece;
+    if (s.wide && s.lanes == 4 && filled && s.splits == 1 && (uint64_t)pairs * groups * seqs >= 4 * kCus)
         s.wide = 2, s.apiece = pairs, s.blocks = pairs * groups;
     return s;
 }
@@ -685,9 +688,10 @@ int scan(hipStream_t st, const dev::ScanArgs& given, const ScanShape& s) {
     if (s.wide) {
         with_quads(s, [&](auto c, auto ns) {
             constexpr int C = decltype(c)::value, NS = decltype(ns)::value;
-            if (ends)
-                hipLaunchKernelGGL((dev::scan_quad_kernel<T, C, NS, false, false>), grid_of(ends), dim3(256), 0, st, a,
-                                   ends);
+            if constexpr (C == 1)  // pairs of channels have no splits
+                if (ends)
+                    hipLaunchKernelGGL((dev::scan_quad_kernel<T, C, NS, false, false>), grid_of(ends), dim3(256), 0, st,
+                                       a, ends);
             with_gate(a.z, [&](auto z) {
                 hipLaunchKernelGGL((dev::scan_quad_kernel<T, C, NS, true, decltype(z)::value>), grid_of(all), dim3(256),
                                    0, st, a, all);
@@ -712,9 +716,10 @@ int scan_backward(hipStream_t st, const dev::ScanArgs& a, const ScanShape& s, fl
         if (s.wide)
             with_quads(s, [&](auto c, auto ns) {
                 constexpr int C = decltype(c)::value, NS = decltype(ns)::value <= 2 ? decltype(ns)::value : 2;
-                if (ends)
-                    hipLaunchKernelGGL((dev::scan_quad_ends_backward_kernel<T, C, NS>), grid_of(ends), dim3(256), 0, st,
-                                       a, ends);
+                if constexpr (C == 1)
+                    if (ends)
+                        hipLaunchKernelGGL((dev::scan_quad_ends_backward_kernel<T, C, NS>), grid_of(ends), dim3(256), 0,
+                                           st, a, ends);
                 with_gate(a.z, [&](auto z) {
                     hipLaunchKernelGGL((dev::scan_quad_backward_kernel<T, C, NS, decltype(z)::value>),
                                        dim3(s.blocks * parts), dim3(256), 0, st, a, parts);
