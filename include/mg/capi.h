@@ -630,9 +630,9 @@ int mg_causal_conv_backward(void* stream, const mg_causal_conv_backward_args* ar
 /* For each channel and its states s: delta = softplus(dt + dt_bias), h[s] = exp(delta
  * a[s]) h[s] + delta x b[s], y = sum over s of c[s] h[s], + d x, and with z times
  * z / (1 + exp(-z)). b and c are a row's [groups][states]: channel i takes those of group
- * i / (channels / groups). a must not be positive; a decay
- * under 2^-126 counts as 0. h begins as initial, or 0, and ends as
- * final, which may be initial. checkpoints takes the state before every MG_SCAN_CHUNK
+ * i / (channels / groups). a must not be positive (-infinity: a state that keeps nothing);
+ * a decay under 2^-126 counts as 0. h begins as initial, or 0, and ends as final, which may
+ * be initial. checkpoints takes the state before every MG_SCAN_CHUNK
  * steps (those of steps that a sequence has), which the backward pass starts from. states
  * is at most 256, groups divides channels. h and the sums are fp32 and y is
  * rounded once. Few sequences of many steps are split over the steps, which takes the

@@ -98,6 +98,17 @@ __device__ __forceinline__ void store_states(float* p, int count, f32x4 v) {
         if (i < count) p[i] = v[i];
 }
 
+// A in base 2. A rate of -infinity is fp32's lowest value: a step of delta 0 (past the end, or a split that is empty)
+// then leaves the state as it is, and not NaN.
+__device__ __forceinline__ f32x4 base2_of(f32x4 a) {
+    f32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r[i] = a[i] * kLog2e;
+        r[i] = r[i] < -3.402823466e38f ? -3.402823466e38f : r[i];
+    }
+    return r;
+}
 __device__ __forceinline__ f32x4 decay_of(f32x4 a2, float delta) {
     f32x4 r;
 #pragma unroll

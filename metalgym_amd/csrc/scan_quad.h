@@ -65,7 +65,7 @@ struct QuadLane : QuadMap<C> {
     // a2 as it is meant: apart from its loads, which the others need not wait for
     __device__ __forceinline__ void ready() {
 #pragma unroll
-        for (int u = 0; u < U; ++u) a2[u] = a2[u] * kLog2e;
+        for (int u = 0; u < U; ++u) a2[u] = base2_of(a2[u]);
     }
     __device__ __forceinline__ size_t at(const ScanArgs& p, uint32_t n, int u) const {
         return ((size_t)n * p.channels + first + u / NS) * p.states + state + 16 * (u % NS);

@@ -42,7 +42,7 @@ struct ScanLane {
         channel = first + threadIdx.x / L;
         state = 4 * (threadIdx.x % L);
         count = channel < limit ? (int)p.states - state : 0;
-        a2 = load_states(p.a + (size_t)channel * p.states + state, count) * kLog2e;
+        a2 = base2_of(load_states(p.a + (size_t)channel * p.states + state, count));
     }
     __device__ __forceinline__ size_t at(const ScanArgs& p, uint32_t n) const {
         return ((size_t)n * p.channels + channel) * p.states + state;
