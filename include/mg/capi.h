@@ -739,7 +739,9 @@ int mg_selective_scan_backward(void* stream, const mg_selective_scan_backward_ar
  * rows (which may be 0) and classes are at most 2^20, width at most 65536. Products of
  * 16-bit types are exact, those of fp32 are too in small calls; in large ones they go
  * through the matrix units as pairs of binary16 halves at a power of two for each row of x
- * and for all of w: 22 bits, fewer for elements under 2^-17 of its largest. Sums are fp32. */
+ * and for all of w: 22 bits, fewer for elements under 2^-17 of its largest (and nothing of the others beside
+ * fp32's lowest value). Sums are fp32. Logits past 2.3e38 in size count as infinite: a class of minus
+ * infinity is never taken, a row with one of plus infinity is NaN. */
 typedef struct mg_cross_entropy_args {
     const void* x;          /* [rows][width] */
     const void* w;          /* [classes][width] */

@@ -476,7 +476,8 @@ __global__ void __launch_bounds__(512, (kByTwos<KIND, MI> ? 4 : 2)) head_kernel(
 #pragma unroll
                     for (int e = 0; e < 16; ++e) top = __builtin_fmaxf(top, acc[i][j][e]);
                 RowStats r{top * to2, 0.0f, 0.0f};
-                const float zero = top == -__builtin_huge_valf() ? 0.0f : r.top;
+                // also where the lowest finite logits leave fp32's range in base 2
+                const float zero = r.top == -__builtin_huge_valf() ? 0.0f : r.top;
                 if (args.want_entropy) {
 #pragma unroll
                     for (int i = 0; i < MI; ++i)
