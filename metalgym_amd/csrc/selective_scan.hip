@@ -756,6 +756,16 @@ int check_states(const char* what, uint32_t channels, uint32_t states, uint32_t 
     return MG_OK;
 }
 
+// The parts of dB and dC are one for each row of `steps` x `seqs`, of which lengths may leave most out: what no memory
+// holds must not wrap around to what some does.
+int check_shared(const char* what, const ScanShape& s, uint64_t steps, uint64_t seqs, uint64_t states) {
+    const uint64_t row = (uint64_t)s.blocks * 2 * states * 4;
+    MG_CHECK(s.apiece <= 1 || steps * seqs <= (1ull << 48) / row, MG_ERR_INVALID,
+             "%s: the workspace of %llu steps of %llu seqs would pass 2^48 bytes", what, (unsigned long long)steps,
+             (unsigned long long)seqs);
+    return MG_OK;
+}
+
 // What both directions take alike.
 template <class Args>
 int check_inputs(const char* what, Args& p, bool any) {
@@ -856,6 +866,7 @@ int mg_selective_scan_backward_workspace(uint32_t steps, uint32_t seqs, uint32_t
     *bytes = 0;
     for (bool far : {false, true}) {
         const ScanShape s = scan_shape(steps, seqs, channels, states, groups, far, true);
+        if ((rc = check_shared(what, s, steps, seqs, states))) return rc;
         const uint64_t need = split_bytes(s, seqs, channels, states) + shared_bytes(s, steps, seqs, groups, states) +
                               padded((uint64_t)backward_parts(s, seqs) * channels * (states + 2) * 4);
         *bytes = need > *bytes ? need : *bytes;
@@ -897,8 +908,9 @@ int mg_selective_scan_backward(void* stream, const mg_selective_scan_backward_ar
                                        lies_far(p.step_rows, p.dz_ld, p.type),
                                    true);
     uint64_t need = 0;
-    mg_selective_scan_backward_workspace(p.steps, p.seqs, p.channels, p.states, p.groups, &need);
-    if ((rc = check_workspace(what, p.workspace, p.workspace_bytes, need))) return rc;
+    if ((rc = mg_selective_scan_backward_workspace(p.steps, p.seqs, p.channels, p.states, p.groups, &need)) ||
+        (rc = check_workspace(what, p.workspace, p.workspace_bytes, need)))
+        return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     StreamDevice on;
     if ((rc = on.enter(st, "selective scan backward: stream device"))) return rc;
