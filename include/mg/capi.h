@@ -675,7 +675,11 @@ int mg_selective_scan(void* stream, const mg_selective_scan_args* args);
 
 /* Backward of mg_selective_scan for the gradients dy of y and dfinal of final.
  * checkpoints are the forward's, and may be NULL where steps is at most MG_SCAN_CHUNK.
- * da, dd and ddt_bias are sums over all rows, db and dc over a group's channels. */
+ * da, dd and ddt_bias are sums over all rows, db and dc over a group's channels. The workspace
+ * holds fp32 parts of db and dc where a group has several workgroups: 8 bytes for each row, group, state
+ * and workgroup, of 256 channels to 4 states, 128 to 8, 64 or 128 to 32, 16 to 64, 8 to 128 and 4 to 256. 32 x
+ * 4096 rows of 2048 channels take 0.5 GB with 16 states, 8.6 with 64 and 137 with 256; sequences
+ * in several calls take less. Sizes past 2^48 bytes are refused. */
 typedef struct mg_selective_scan_backward_args {
     const void* x;
     const void* dt;
@@ -727,9 +731,9 @@ int mg_selective_scan_backward_workspace(uint32_t steps, uint32_t seqs, uint32_t
 int mg_selective_scan_backward(void* stream, const mg_selective_scan_backward_args* args);
 
 /* ---------------------------------------------------------------------------
- * A head over many actions (or tokens): softmax(x w') with w [classes][width], without
- * its [rows][classes] logits. No reference counterpart (its head of act_dim + 1 columns
- * lies inside the fused kernels). As the operators above.
+ * A head over many actions (or tokens): softmax(x w') with w [classes][width]. No logits
+ * are kept forwards, and a piece of the classes at a time backwards. No reference counterpart (its
+ * head of act_dim + 1 columns lies inside the fused kernels). As the operators above.
  * ------------------------------------------------------------------------- */
 
 /* Per row, with s = x w': lse = log sum exp s, loss = lse - s[target] (minus the
@@ -767,7 +771,10 @@ int mg_cross_entropy(void* stream, const mg_cross_entropy_args* args);
  * logits are computed again, in large calls a piece of the classes at a time, whose g is
  * rounded to type for the two products (binary16 at a power of two, fp32 as pairs at one for
  * each array); in small ones it stays fp32. Their sums are fp32, rounded once.
- * A row that is left out adds nothing, whatever it holds. Without rows dw is 0. */
+ * A row that is left out adds nothing, whatever it holds. Without rows dw is 0.
+ * The workspace holds g of a piece for all rows: about 2^27 logits, but of 8192 classes at least, so that
+ * with up to 16128 classes it is g of every logit (2 bytes each, 4 of fp32: 131072 x 10007 of fp32 takes
+ * 5.8 GB). More rows than there is memory for go in several calls, whose dw are added up. */
 typedef struct mg_cross_entropy_backward_args {
     const void* x;
     const void* w;

@@ -1,12 +1,15 @@
-// Softmax cross entropy over many classes without its logits, and its gradients
-// (mg_cross_entropy, mg_cross_entropy_backward).
+// Softmax cross entropy over many classes without its logits, and its gradients, which keep a piece of
+// them at a time (mg_cross_entropy, mg_cross_entropy_backward).
 //
 // Forward: one product W X' whose tiles end in each row's maximum, sum of exponentials and
 // sum weighted by the logits, and a launch that joins the tiles' statistics. Backward: the
 // logits again, a piece of the classes at a time; each piece's gradient with respect to the
 // logits, G = dloss (p - [target]) - dentropy p (log p + H), is stored in 16 bits (fp32's as
 // pairs) and enters two products, dX += G W and dW = G' X, in one launch. Their contractions run from
-// row to row of an operand: LDS hands those out transposed.
+// row to row of an operand: LDS hands those out transposed. G is rounded because the matrix instructions take 16
+// bits: a second half of it would double both products, which are three fifths of the time. That is the gradients'
+// largest error: 4096 x 65536 x 1024 bf16 is 2.4e-3 off its 64-bit value, where rounding the results alone
+// leaves 1.7e-3.
 //
 // All three are one kernel (head_kernel): tiles of a b', 16-bit operands, fp32 sums. 16-bit arrays of a
 // fitting shape are read where they lie, others are copied. fp32 operands become two binary16
