@@ -1388,7 +1388,7 @@ int mg_cross_entropy_backward_workspace(uint32_t rows, uint32_t classes, uint32_
     MG_CHECK(bytes, MG_ERR_INVALID, "%s: null argument", what);
     int rc = check_head(what, rows, classes, width, type);
     if (rc) return rc;
-    *bytes = HeadSpace(nullptr, rows, classes, width, type, true).bytes;
+    *bytes = rows ? HeadSpace(nullptr, rows, classes, width, type, true).bytes : 0;
     return MG_OK;
 }
 

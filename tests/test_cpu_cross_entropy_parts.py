@@ -80,3 +80,10 @@ def test_pieces(launches):
     counts = [[int(w[3:]) for w in words if w.startswith("dx+")] for words in launches(shapes)]
     assert [len(c) for c in counts] == [2, 3, 17] * 2
     assert all(c[-1] < c[0] for c in counts[2::3])
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("classes,width", [(10, 8), (1 << 18, 1 << 15), ((1 << 18) + 1, 1 << 15), (1 << 20, 1 << 16)])
+def test_no_rows_take_no_workspace(mg, dtype, classes, width):
+    """Zeros in dW are all that there is to write."""
+    assert mg.cross_entropy_backward_workspace(0, classes, width, dtype) == 0
