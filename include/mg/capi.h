@@ -770,7 +770,8 @@ int mg_cross_entropy(void* stream, const mg_cross_entropy_args* args);
  * dx = g w, dw = g' x. lse, and where there is a dentropy entropy, are the forward's. The
  * logits are computed again, in large calls a piece of the classes at a time, whose g is
  * rounded to type for the two products (binary16 at a power of two, fp32 as pairs at one for
- * each array); in small ones it stays fp32. Their sums are fp32, rounded once.
+ * each array; of up to 128 rows of 16 bits with what the rounding leaves as a second half); in small ones
+ * it stays fp32. Their sums are fp32, rounded once.
  * A row that is left out adds nothing, whatever it holds. Without rows dw is 0.
  * The workspace holds g of a piece for all rows: about 2^27 logits, but of 8192 classes at least, so that
  * with up to 16128 classes it is g of every logit (2 bytes each, 4 of fp32: 131072 x 10007 of fp32 takes

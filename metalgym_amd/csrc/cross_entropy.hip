@@ -9,7 +9,7 @@
 // row to row of an operand: LDS hands those out transposed. G is rounded because the matrix instructions take 16
 // bits: a second half of it would double both products, which are three fifths of the time. That is the gradients'
 // largest error: 4096 x 65536 x 1024 bf16 is 2.4e-3 off its 64-bit value, where rounding the results alone
-// leaves 1.7e-3.
+// leaves 1.7e-3. Up to 128 rows have room for that half in their own tile.
 //
 // All three are one kernel (head_kernel): tiles of a b', 16-bit operands, fp32 sums. 16-bit arrays of a
 // fitting shape are read where they lie, others are copied. fp32 operands become two binary16
@@ -65,6 +65,8 @@ struct HeadScales {
 struct HeadOperand {
     const void* base;
     uint32_t ld;
+    uint32_t again = ~0u;  // rows from here on are the first ones once more
+    __device__ __forceinline__ uint32_t row(uint32_t r) const { return r >= again ? r - again : r; }
 };
 __host__ __device__ __forceinline__ uint32_t pair_place(uint32_t c) { return (c & ~15u) * 2 + (c & 15); }
 
@@ -82,6 +84,7 @@ struct HeadProduct {
     float* parts;
     uint64_t out_ld;
     uint32_t parts_ld;
+    uint32_t low;      // dX, not 0: of G's rows those from here on are the first ones' low halves, with parts of their own
     uint32_t add;      // parts += sum
     uint32_t which;    // 0: dX, 1: dW (whose scale takes the product back)
 };
@@ -172,7 +175,7 @@ struct HeadSide {
     static constexpr int kBytes = SIDE * 64, kWide = PAIRS ? 2 : 1;
     static constexpr int kRow = SIDE * 2 * kWide;  // bytes of a TURNED row
     const H* base;
-    uint32_t ld, off[L], row[L];
+    uint32_t ld, again, off[L], row[L];
 
     // what exchanges a TURNED row's places: blocks of columns are their last bit, or of pairs
     // the one before it
@@ -187,7 +190,7 @@ struct HeadSide {
 
     // `from`: the tile's first row (or column) of `rows`
     __device__ __forceinline__ HeadSide(const HeadOperand& o, uint32_t from, uint32_t rows, int wave, int lane) {
-        ld = o.ld;
+        ld = o.ld, again = o.again;
         base = static_cast<const H*>(o.base) + (TURNED ? (uint64_t)from * kWide : (uint64_t)from * ld);
         const uint32_t have = rows > from ? rows - from : 0;
 #pragma unroll
@@ -200,15 +203,17 @@ struct HeadSide {
                 off[c] = col < have ? (row[c] * ld + place) * 2 : kNowhere;
             } else {
                 const uint32_t r = (wave * L + c) * 16 + (lane >> 2), place = ((lane & 3) ^ shift(r)) * 8;
+                const uint32_t at = o.row(r);
                 row[c] = PAIRS ? place & 15 : place;  // the first of its elements
-                off[c] = r < have ? (r * ld + place) * 2 : kNowhere;
+                off[c] = at < have ? (at * ld + place) * 2 : kNowhere;
             }
         }
     }
     // The stage of contraction elements k ..., up to `to`.
     __device__ __forceinline__ void load(char* at, int wave, uint32_t k, uint32_t to, uint32_t live) const {
         // a row of W or X may lie anywhere, so its stage has an address of its own
-        const H* const p = base + (TURNED ? (uint64_t)k * ld : (uint64_t)k * kWide);
+        const uint32_t first = !PAIRS && TURNED && k >= again ? k - again : k;
+        const H* const p = base + (TURNED ? (uint64_t)first * ld : (uint64_t)k * kWide);
         const uint64_t address = reinterpret_cast<uint64_t>(p);
         typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
         const u32x4 r = {(uint32_t)address, (uint32_t)(address >> 32) & 0xffffu, 0x7fffffffu, 0x00020000u};
@@ -391,8 +396,12 @@ __global__ void __launch_bounds__(512, (kByTwos<KIND, MI> ? 4 : 2)) head_kernel(
         const float b0 = sc.g_back, b1 = p.which ? sc.x_back : sc.w_back;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const uint32_t n = n0 + 32 * j;
-            if (n >= p.n) continue;
+            uint32_t n = n0 + 32 * j, part = split, rows = p.n;
+            if (p.low) {
+                part = 2 * split + (n >= p.low), rows = args.rows;
+                if (n >= p.low) n -= p.low;
+            }
+            if (n >= rows) continue;
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
                 const uint32_t m = m0 + 32 * i;
@@ -400,7 +409,7 @@ __global__ void __launch_bounds__(512, (kByTwos<KIND, MI> ? 4 : 2)) head_kernel(
                 f32x16& v = acc[i][j];
                 const uint32_t count = p.m - m;
                 if (p.parts) {  // parts_ld is a multiple of 4
-                    f32x4* const at = reinterpret_cast<f32x4*>(p.parts + ((uint64_t)split * p.n + n) * p.parts_ld + m);
+                    f32x4* const at = reinterpret_cast<f32x4*>(p.parts + ((uint64_t)part * rows + n) * p.parts_ld + m);
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) {
                         if ((uint32_t)e >= count) continue;
@@ -444,7 +453,7 @@ __global__ void __launch_bounds__(512, (kByTwos<KIND, MI> ? 4 : 2)) head_kernel(
         RowStats* const trade = reinterpret_cast<RowStats*>(lds);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const uint32_t n = n0 + 32 * j;
+            const uint32_t place = n0 + 32 * j, n = p.b.row(place);  // of G, and of x
             int32_t target = -1;
             if (n < args.rows) {
                 target = args.targets[n];
@@ -505,7 +514,7 @@ __global__ void __launch_bounds__(512, (kByTwos<KIND, MI> ? 4 : 2)) head_kernel(
                 if (lane < 32) trade[wm * kHeadN + wn * 64 + 32 * j + lane] = r;
             } else {
                 const uint32_t bits = (uint32_t)__ballot(live);  // the upper lanes' rows are the lower ones'
-                if (tm == 0 && wm == 0 && lane == 0) args.live[n / 32] = bits;
+                if (tm == 0 && wm == 0 && lane == 0) args.live[place / 32] = bits;
                 float lse2 = 0.0f, dl = 0.0f, de = 0.0f, ent = 0.0f;
                 if (live) {
                     lse2 = args.lse[n] * kLog2, dl = args.dloss[n] * sc.g;
@@ -533,6 +542,15 @@ __global__ void __launch_bounds__(512, (kByTwos<KIND, MI> ? 4 : 2)) head_kernel(
 #pragma unroll
                         for (int e = 0; e < 16; ++e)
                             if (live && hit == (uint32_t)(32 * i + e)) acc[i][j][e] -= dl;
+                }
+                if (!PAIRS && place >= p.b.again) {  // what the same row's rounding leaves, of 32 rows at once
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float rest = acc[i][j][e] - (float)(H)acc[i][j][e];
+                            acc[i][j][e] = __builtin_fabsf(rest) < __builtin_huge_valf() ? rest : 0.0f;
+                        }
                 }
                 // by way of LDS, from where a wave stores whole rows of the tile: places of 16 bytes are
                 // exchanged by the row, whose own lie in the same banks
@@ -753,6 +771,7 @@ __global__ void __launch_bounds__(256) head_sum_kernel(const float* parts, uint3
     if (c >= cols) return;
     for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
         f32x4 v = {};
+#pragma unroll 8  // loads at once: gradients of 4 x 100000 x 128 bf16 103 us with one at a time, 58 with these
         for (uint32_t k = 0; k < count; ++k)
             v += *reinterpret_cast<const f32x4*>(parts + ((uint64_t)k * rows + r) * ld + c);
 #pragma unroll
@@ -1041,6 +1060,7 @@ struct HeadSpace {
     bool small;
     float* small_g;
     uint32_t tiles, wide, rows_ld, high, g_ld, piece, pieces, tall, splits_x, splits_w, range_x, range_w, parts_ld;
+    uint32_t low;  // the row of G where the low halves begin, 0: there are none
     uint64_t planes;
     uint16_t *x, *x_even, *w, *g;
     uint32_t* live;
@@ -1110,14 +1130,19 @@ struct HeadSpace {
         };
         cut(piece, splits_x, range_x);
         cut(rows_ld, splits_w, range_w);
+        // G's rounding to 16 bits is as large as the results' own: the gradients' error is 1.4 times that of rounding
+        // them alone, and with few rows, whose targets' elements are most of G, up to 1.9 times. Where they are at
+        // most half of a tile's rows the others take what the rounding leaves (1.0 times). us without and with, bf16,
+        // 30000 x 2048: 32 rows 120 and 121, 64 122 and 133, 128 133 and 161; more rows would take the products twice.
+        low = planes == 1 && 2 * up_to(rows, 32) <= dev::kHeadN ? up_to(rows, 32) : 0;
         // What is launched, kept and summed are the ranges of what there is: the last of a filled-up piece may
         // hold nothing else. The first piece is the longest.
-        splits_x = ranges(classes < piece ? classes : piece, range_x), splits_w = ranges(rows, range_w);
+        splits_x = ranges(classes < piece ? classes : piece, range_x), splits_w = ranges(low ? 2 * low : rows, range_w);
         parts_ld = up_to(width, 4);
         x_even = c.take<uint16_t>(planes > 1 ? planes * rows * wide : 0);
         live = c.take<uint32_t>(rows_ld / 32);
         g = c.take<uint16_t>((uint64_t)rows_ld * g_ld);
-        parts_x = c.take<float>(splits_x > 1 || pieces > 1 ? (uint64_t)splits_x * rows * parts_ld : 0);
+        parts_x = c.take<float>(splits_x > 1 || pieces > 1 || low ? (uint64_t)splits_x * (low ? 2 : 1) * rows * parts_ld : 0);
         parts_w = c.take<float>(splits_w > 1 ? (uint64_t)splits_w * piece * parts_ld : 0);
         bytes = c.used;
     }
@@ -1277,7 +1302,7 @@ int cross_entropy_backward(hipStream_t st, const mg_cross_entropy_backward_args&
     a.rows = p.rows, a.classes = p.classes, a.targets = p.targets, a.row_exp = s.row_exp;
     a.lse = p.lse, a.dloss = p.dloss, a.entropy = p.entropy, a.dentropy = p.dentropy;
     a.rows_ld = s.rows_ld, a.g = s.g, a.g_ld = s.g_ld, a.live = s.live;
-    const bool parts_x = s.splits_x > 1 || s.pieces > 1, parts_w = s.splits_w > 1;
+    const bool parts_x = s.splits_x > 1 || s.pieces > 1 || s.low, parts_w = s.splits_w > 1;
     const uint32_t tiles_m = (p.width + s.tall - 1) / s.tall;
     for (uint32_t first = 0; first < p.classes; first += s.piece) {
         const uint32_t here = p.classes - first < s.piece ? p.classes - first : s.piece, fill = up_to(here, kHeadM);
@@ -1287,6 +1312,7 @@ int cross_entropy_backward(hipStream_t st, const mg_cross_entropy_backward_args&
         m.a.base = static_cast<const H*>(in.w.base) + (uint64_t)first * in.w.ld;
         m.k = m.range = s.wide, m.splits = 1, m.m = here, m.n = p.rows;
         m.tiles_m = fill / s.high, m.tiles_n = s.rows_ld / dev::kHeadN;
+        if (s.low) m.b.again = s.low;
         a.tiles = m.tiles_m * m.tiles_n, a.first = first;
         launch_logits<H, dev::kLogitGrad, kPairs>(st, a, s);
         MG_HIP(hipGetLastError(), "cross entropy logits launch");
@@ -1295,7 +1321,7 @@ int cross_entropy_backward(hipStream_t st, const mg_cross_entropy_backward_args&
         if (p.dx) {
             dev::HeadProduct& q = a.p[n++];
             q = {};
-            q.a = m_of_w, q.b = {s.g, s.g_ld}, q.m = p.width, q.n = p.rows;
+            q.a = m_of_w, q.b = {s.g, s.g_ld}, q.m = p.width, q.n = s.low ? 2 * s.low : p.rows, q.low = s.low;
             q.k = here, q.range = s.range_x, q.splits = s.ranges(here, s.range_x);
             q.tiles_m = tiles_m, q.tiles_n = s.rows_ld / dev::kHeadN;
             q.out = p.dx, q.out_ld = p.dx_ld, q.parts = parts_x ? s.parts_x : nullptr, q.parts_ld = s.parts_ld;
@@ -1306,7 +1332,8 @@ int cross_entropy_backward(hipStream_t st, const mg_cross_entropy_backward_args&
             dev::HeadProduct& q = a.p[n++];
             q = {};
             q.a = in.x_even, q.b = {s.g, s.g_ld}, q.m = p.width, q.n = here, q.live = s.live;
-            q.k = p.rows, q.range = s.range_w, q.splits = s.splits_w;
+            q.k = s.low ? 2 * s.low : p.rows, q.range = s.range_w, q.splits = s.splits_w;
+            if (s.low) q.a.again = s.low;
             q.tiles_m = tiles_m, q.tiles_n = fill / dev::kHeadN;
             q.out = static_cast<T*>(p.dw) + (uint64_t)first * p.dw_ld, q.out_ld = p.dw_ld;
             q.parts = parts_w ? s.parts_w : nullptr, q.parts_ld = s.parts_ld, q.which = 1;
@@ -1326,7 +1353,8 @@ int cross_entropy_backward(hipStream_t st, const mg_cross_entropy_backward_args&
     }
     if (p.dx && parts_x)
         hipLaunchKernelGGL(dev::head_sum_kernel<T>, copy_grid(p.width, p.rows), dim3(256), 0, st, s.parts_x,
-                           s.splits_x, p.rows, p.width, s.parts_ld, static_cast<T*>(p.dx), p.dx_ld, a.scales, 0u);
+                           s.splits_x * (s.low ? 2 : 1), p.rows, p.width, s.parts_ld, static_cast<T*>(p.dx), p.dx_ld,
+                           a.scales, 0u);
     MG_HIP(hipGetLastError(), "cross entropy sums launch");
     return MG_OK;
 }

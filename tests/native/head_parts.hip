@@ -70,7 +70,8 @@ void launch(const mg::dev::HeadArgs& a) {
     for (const auto& p : a.p) {
         if (!p.out || p.b.base != a.g) continue;
         if (&p == &a.p[1] && a.p[0].which) continue;  // one product alone
-        part(p.which, p.splits, p.parts, (uint64_t)p.splits * p.n * p.parts_ld);
+        const uint32_t sums = p.low ? 2 * p.splits : p.splits;
+        part(p.which, sums, p.parts, (uint64_t)sums * (p.low ? a.rows : p.n) * p.parts_ld);
     }
     touched(a.g, 2ull * a.rows_ld * a.g_ld);
 }

@@ -18,8 +18,9 @@ def statistics(c):
     return (rounded(most + 1.125 + r.normal(0, 0.1, c.rows), "fp32"), rounded(most - 1.125 + r.normal(0, 0.1, c.rows), "fp32"))
 
 
-def some_gradients(c, lse, entropy, rows, classes):
-    """dX of some rows and dW of some classes, with the bounds of Case.gradients."""
+def some_gradients(c, lse, entropy, rows, classes, held=None):
+    """dX of some rows and dW of some classes, with the bounds of Case.gradients; `held`: half a step of what the
+    logits' gradient is kept in, where that is less than the type's."""
     pairs = c.kind == "fp32"
     live = c.live
     most = np.abs(c.dloss[live])
@@ -46,7 +47,7 @@ def some_gradients(c, lse, entropy, rows, classes):
                 off + 4 * U32 * np.abs(entropy[R])[:, None])
         g = g - np.where(c.targets[R][:, None] == C[None], c.dloss[R][:, None], 0)
         eg = eg + U32 * np.abs(g)
-        eg = eg + np.abs(g) * (2.0**-22 if pairs else HALF[c.kind])
+        eg = eg + np.abs(g) * (held or (2.0**-22 if pairs else HALF[c.kind]))
         if c.kind != "bf16":
             eg = eg + most.max() * 2.0**-38
         g[~live[R]], eg[~live[R]] = 0, 0
@@ -69,11 +70,11 @@ def some_gradients(c, lse, entropy, rows, classes):
     return dx, product(g.T, eg.T, np.where(live[:, None], c.x, 0.0))
 
 
-def check_some(c, mg, rows, classes):
+def check_some(c, mg, rows, classes, held=None):
     lse, entropy = statistics(c)
     c.upload(mg)
     got = c.backward(mg, lse, entropy)
-    dx, dw = some_gradients(c, lse, entropy, rows, classes)
+    dx, dw = some_gradients(c, lse, entropy, rows, classes, held)
     assert_within(got["dx"][rows], *dx, "dx")
     assert_within(got["dw"][classes], *dw, "dw")
     assert np.isfinite(got["dx"]).all() and np.isfinite(got["dw"]).all()
