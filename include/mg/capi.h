@@ -745,7 +745,9 @@ int mg_selective_scan_backward(void* stream, const mg_selective_scan_backward_ar
  * through the matrix units as pairs of binary16 halves at a power of two for each row of x
  * and for all of w: 22 bits, fewer for elements under 2^-17 of its largest (and nothing of the others beside
  * fp32's lowest value). Sums are fp32. Logits past 2.3e38 in size count as infinite: a class of minus
- * infinity is never taken, a row with one of plus infinity is NaN. */
+ * infinity is never taken, a row with one of plus infinity is NaN. The workspace holds 12 bytes for each row and
+ * tile of 32 classes in small calls, of 128 in large ones up to a width of 256 and of 256 past it, and in large
+ * calls room for copies of x and w, which fp32 and rows that are not made of aligned 16-byte vectors take. */
 typedef struct mg_cross_entropy_args {
     const void* x;          /* [rows][width] */
     const void* w;          /* [classes][width] */
